@@ -648,7 +648,8 @@ int mhlo_cuda_peer_barrier(void* const* flag_devs, int32_t n_ranks, int32_t rank
 /*
  * Every wait inside the tensor-core kernels (mbarrier phases fed by TMA and tcgen05.commit) is bounded; a kernel
  * whose wait expires records a non-zero word and drains instead of spinning. This call synchronises the device,
- * reads and clears that word: *out_code = 0 when no kernel gave up since the last call.
+ * reads and clears that word: *out_code = 0 when no kernel gave up since the last call. It also reports (200 and above) what
+ * the key/value cache kernels found wrong with their page tables, lengths and starts.
  */
 int mhlo_cuda_device_error(int32_t* out_code);
 
@@ -689,6 +690,128 @@ int mhlo_cuda_attention(int32_t dtype, const void* q_dev, const int64_t q_stride
                         const void* mask_dev, void* o_dev, const int64_t o_strides[3], int64_t batch,
                         int64_t heads, int64_t seq_q, int64_t seq_k, int64_t head_dim, float scale,
                         int32_t causal, mhlo_cuda_stream_t stream);
+
+/* ---- keys and values of earlier tokens: a paged cache in 8 bits, attention over it ------------------ */
+
+/*
+ * A cache of keys and values in pages of page_tokens tokens. The codes are int8, one scale per page and head stands for the
+ * whole block of page_tokens x head_dim codes: value = scale * code. All pointers are device memory, 16-byte aligned.
+ *   k_codes, v_codes    [pages, heads, page_tokens, head_dim]
+ *   k_scales, v_scales  [pages, heads]
+ *   page_tokens         16, 32, 64 or 128
+ *   head_dim            a multiple of 16 up to 256 (attention: 64, 96, 128 or 256)
+ * No counterpart in the reference, whose attention takes dense keys and values of the whole sequence
+ * (Sources/MetalHLOCore/Metal/Kernels/FlashAttentionKernel.swift:469-670).
+ */
+typedef struct {
+    int8_t* k_codes;
+    int8_t* v_codes;
+    float* k_scales;
+    float* v_scales;
+    int64_t pages, heads, page_tokens, head_dim;
+} mhlo_cuda_kv_cache;
+
+/*
+ * The sequences of one call, in device memory:
+ *   page_table    [seqs, pages_per_seq], rows table_stride entries apart: page i of a sequence holds its tokens
+ *                 i * page_tokens ... ; entries behind a sequence's last page are not read
+ *   lengths       [seqs] tokens of each sequence, those of this call included; 0: an unused entry, whose rows are passed over
+ *   token_starts  [seqs + 1] ascending: rows token_starts[b] .. token_starts[b + 1] - 1 of the call's tensors are the newest
+ *                 tokens of sequence b, in order. NULL: one row per sequence (tokens = seqs)
+ *   tokens        rows of the call's tensors; rows behind token_starts[seqs] are left alone
+ * What the host cannot see is checked by the kernels: a page outside the cache (nothing is written to it, its tokens are not
+ * seen), a length beyond the table or below the sequence's rows (the sequence is passed over) and starts that are out of order
+ * (the same) are never followed, and mhlo_cuda_device_error reports them as 200 + one of MHLO_CUDA_KV_ERROR_*.
+ */
+typedef struct {
+    const int32_t* page_table;
+    const int32_t* lengths;
+    const int32_t* token_starts;
+    int64_t seqs, pages_per_seq, table_stride, tokens;
+} mhlo_cuda_kv_batch;
+
+enum {
+    MHLO_CUDA_KV_ERROR_PAGE = 1,     /* a page table entry outside [0, pages) */
+    MHLO_CUDA_KV_ERROR_LENGTH = 2,   /* a length below 0, beyond the table, or below the sequence's rows in the call */
+    MHLO_CUDA_KV_ERROR_STARTS = 3,   /* token_starts not ascending inside [0, tokens] */
+    MHLO_CUDA_KV_ERROR_POSITION = 4  /* a position behind the rotation table (its last row is taken) */
+};
+
+/*
+ * Puts the keys and values of the call's tokens into the cache. k, v: [tokens, heads, head_dim] of `dtype` (F16, BF16 or F32),
+ * *_strides = {token, head} in elements, head_dim contiguous. Token at position p (0 = first of its sequence) goes to slot
+ * p mod page_tokens of page page_table[seq, p / page_tokens].
+ *
+ * rope: [rope_positions, rotary_dim] floats, the cosines of a position and then its sines, rotary_dim / 2 each; rotary_dim a
+ * multiple of 16 up to head_dim. Keys are rotated by their position before they are stored: pair i of the first rotary_dim
+ * elements (i and i + rotary_dim / 2; interleaved: 2 i and 2 i + 1) becomes (a cos - b sin, b cos + a sin), products and sums
+ * rounded to fp32 one by one. rope NULL: no rotation. q (may be NULL): [tokens, q_heads, head_dim], rotated by the same
+ * positions into q_out (may be q itself with the same strides).
+ *
+ * The scale of a block is max |x| * (1 / 127) over the tokens that it holds (in fp32, 1 / 127 as well). When a call adds tokens to a block that has some and the
+ * scale grows, the earlier codes are rewritten, c -> round(c * (old / new)); codes of new tokens are round(x * (1 / scale)), to
+ * nearest even. Rewriting adds at most half a step of the new scale to the error of an earlier value. A call that fills slot 0
+ * starts the block afresh, whatever the page held. Values below 127 * 2^-126 become 0; a block that is given a NaN or an
+ * infinity gets the scale NaN, so that it reads as NaN. Slots behind the last token keep their codes. One page must not be written
+ * for two sequences in one call.
+ */
+int mhlo_cuda_kv_cache_append(int32_t dtype, const mhlo_cuda_kv_cache* cache, const mhlo_cuda_kv_batch* batch, const void* k_dev,
+                              const int64_t k_strides[2], const void* v_dev, const int64_t v_strides[2], const void* q_dev,
+                              const int64_t q_strides[2], void* q_out_dev, const int64_t q_out_strides[2], int64_t q_heads,
+                              const float* rope_dev, int64_t rope_positions, int64_t rotary_dim, int32_t interleaved,
+                              mhlo_cuda_stream_t stream);
+
+/*
+ * The first max_tokens keys and values of every sequence as dense tensors of `dtype`: k_out, v_out [seqs, max_tokens, heads,
+ * head_dim], *_strides = {sequence, token, head}; either may be NULL. Tokens behind a sequence's length are zero. batch->tokens
+ * and token_starts are not used.
+ */
+int mhlo_cuda_kv_cache_read(int32_t dtype, const mhlo_cuda_kv_cache* cache, const mhlo_cuda_kv_batch* batch, int64_t max_tokens,
+                            void* k_out_dev, void* v_out_dev, const int64_t out_strides[3], mhlo_cuda_stream_t stream);
+
+/*
+ * Attention of the call's tokens over the cache, which already holds them: the token at position p of its sequence sees
+ * positions 0 .. p. q, o: [tokens, q_heads, head_dim] of `dtype` (F16, BF16 or F32), *_strides = {token, head}, head_dim 64, 96,
+ * 128 or 256 contiguous; q_heads a multiple of the cache's heads: query head i reads head i / (q_heads / heads).
+ * o = softmax(scale * q . k) v with fp32 statistics; lse (NULL, or [tokens, q_heads] floats) receives the logarithm of the sum of
+ * exponentials. A token that sees nothing (its sequence is unused or was passed over) gets zeros and lse -infinity; where the
+ * starts are out of order, rows may be left alone. o may be q itself.
+ * scratch: cached_attention_scratch_bytes() bytes of device memory, 16-byte aligned, that nothing else uses until the call's
+ * work is done; its contents do not matter.
+ */
+int64_t mhlo_cuda_cached_attention_scratch_bytes(const mhlo_cuda_kv_cache* cache, const mhlo_cuda_kv_batch* batch, int64_t q_heads);
+int mhlo_cuda_cached_attention(int32_t dtype, const void* q_dev, const int64_t q_strides[2], const mhlo_cuda_kv_cache* cache,
+                               const mhlo_cuda_kv_batch* batch, int64_t q_heads, float scale, void* o_dev, const int64_t o_strides[2],
+                               float* lse_dev, void* scratch_dev, int64_t scratch_bytes, mhlo_cuda_stream_t stream);
+
+/* ---- log probabilities ------------------------------------------------------------------------------ */
+
+#define MHLO_CUDA_TOP_LOGPROBS_MAX 32
+
+/*
+ * Log probabilities of given tokens under z = scale * x, x [rows, vocab] of `dtype` (F16, BF16 or F32) with rows row_stride
+ * elements apart, scale > 0 (1 / temperature): lse = log sum exp z, logprobs = z[target] - lse, entropy = lse - sum p z, and the
+ * top_k (0 .. 32) largest entries with their log probabilities in descending order, equal logits in ascending order of their
+ * ids, NaN first. targets: [rows] of target_dtype (I32 or I64); a negative target names no token: log probability 0. A target
+ * beyond the vocabulary gives NaN, and so does a row that has a NaN, a +infinity or nothing but -infinities. Statistics and
+ * results are fp32. targets and logprobs may be NULL together, and so may entropy, lse and (top_k = 0) the alternatives.
+ */
+int mhlo_cuda_token_logprobs(int32_t dtype, const void* x_dev, int64_t row_stride, int64_t rows, int64_t vocab, float scale,
+                             const void* targets_dev, int32_t target_dtype, float* logprobs_dev, float* entropy_dev, float* lse_dev,
+                             int32_t top_k, float* top_logprobs_dev, int32_t* top_ids_dev, mhlo_cuda_stream_t stream);
+
+/*
+ * Gradient of the above: with g = d/d logprobs, e = d/d entropy and t_k = d/d top_logprobs (each [rows] or [rows, top_k] floats,
+ * NULL = 0), ids as they were given and returned, and lse and entropy as computed (entropy may be NULL when e is),
+ *   dx[i] = scale * ( g [i = target] + sum_k t_k [i = id_k] - p_i (g + sum_k t_k) - e p_i (log p_i + entropy) ).
+ * Negative ids have no part in it, ids beyond the vocabulary make their row NaN. dx: like x, rows dx_row_stride elements apart; it
+ * may be x itself (with the same stride).
+ */
+int mhlo_cuda_token_logprobs_grad(int32_t dtype, const void* x_dev, int64_t row_stride, int64_t rows, int64_t vocab, float scale,
+                                  const void* targets_dev, int32_t target_dtype, const float* lse_dev, const float* entropy_dev,
+                                  const float* grad_logprobs_dev, const float* grad_entropy_dev, int32_t top_k,
+                                  const int32_t* top_ids_dev, const float* grad_top_dev, void* dx_dev, int64_t dx_row_stride,
+                                  mhlo_cuda_stream_t stream);
 
 /*
  * stablehlo.rng: `count` values of `dtype` between the scalars *a_dev and *b_dev. distribution 0 = UNIFORM (floats in

@@ -96,6 +96,8 @@ bool gemm_fp32_supported(const GemmProblem& p);
 int gemm_fp32_launch(const GemmProblem& p, cudaStream_t stream);
 int gemm_device_error();       // synchronises; returns and clears the GEMM kernel's error word (-1: CUDA error)
 int attention_device_error();  // same for the attention kernel
+int kv_cache_device_error();          // same for the kernels that write and read the key/value cache: MHLO_CUDA_KV_ERROR_*
+int cached_attention_device_error();  // same for the attention over it
 // Stream-ordered copies of the error words into pinned host memory, and host stores into them (clearing, or the test hook).
 bool gemm_error_fetch_async(int* pinned_dst, cudaStream_t stream);
 bool attention_error_fetch_async(int* pinned_dst, cudaStream_t stream);

@@ -7,6 +7,8 @@ There is no fallback: if the shared library has not been built, importing this m
 """
 from __future__ import annotations
 
+import collections
+import contextlib
 import ctypes as C
 import os
 
@@ -75,6 +77,16 @@ class ScatterDims(C.Structure):
                 ("inserted_window_dims", C.c_int32 * 8), ("input_batching_dims", C.c_int32 * 8),
                 ("scatter_indices_batching_dims", C.c_int32 * 8), ("scatter_dims_to_operand_dims", C.c_int32 * 8),
                 ("index_vector_dim", C.c_int32)]
+
+
+class KvCacheArgs(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p), ("pages", C.c_int64),
+                ("heads", C.c_int64), ("page_tokens", C.c_int64), ("head_dim", C.c_int64)]
+
+
+class KvBatchArgs(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("lengths", C.c_void_p), ("token_starts", C.c_void_p), ("seqs", C.c_int64),
+                ("pages_per_seq", C.c_int64), ("table_stride", C.c_int64), ("tokens", C.c_int64)]
 
 
 if not os.path.exists(LIB_PATH):
@@ -185,6 +197,14 @@ _PROTOTYPES = {
                                       C.POINTER(_i64), _i64, _i64, _i64, _i64, _i64, _f32, _i32, _vp]),
     "mhlo_cuda_attention_tuned": (C.c_int, [_i32, _vp, C.POINTER(_i64), _vp, C.POINTER(_i64), _vp, C.POINTER(_i64), _vp, _vp,
                                             C.POINTER(_i64), _i64, _i64, _i64, _i64, _i64, _f32, _i32, _vp, _vp]),
+    "mhlo_cuda_kv_cache_append": (C.c_int, [_i32, C.POINTER(KvCacheArgs), C.POINTER(KvBatchArgs), _vp, C.POINTER(_i64), _vp, C.POINTER(_i64), _vp,
+                                            C.POINTER(_i64), _vp, C.POINTER(_i64), _i64, _vp, _i64, _i64, _i32, _vp]),
+    "mhlo_cuda_kv_cache_read": (C.c_int, [_i32, C.POINTER(KvCacheArgs), C.POINTER(KvBatchArgs), _i64, _vp, _vp, C.POINTER(_i64), _vp]),
+    "mhlo_cuda_cached_attention_scratch_bytes": (_i64, [C.POINTER(KvCacheArgs), C.POINTER(KvBatchArgs), _i64]),
+    "mhlo_cuda_cached_attention": (C.c_int, [_i32, _vp, C.POINTER(_i64), C.POINTER(KvCacheArgs), C.POINTER(KvBatchArgs), _i64, _f32, _vp,
+                                             C.POINTER(_i64), _vp, _vp, _i64, _vp]),
+    "mhlo_cuda_token_logprobs": (C.c_int, [_i32, _vp, _i64, _i64, _i64, _f32, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
+    "mhlo_cuda_token_logprobs_grad": (C.c_int, [_i32, _vp, _i64, _i64, _i64, _f32, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp]),
 }
 for _name, (_res, _args) in _PROTOTYPES.items():
     _fn = getattr(lib, _name)  # AttributeError here = the library does not export a declared symbol
@@ -444,4 +464,199 @@ def softmax(x, axis: int = -1, out=None, tuning=None, stream=None):
     inner = math.prod(x.shape[axis + 1:])
     check(lib.mhlo_cuda_softmax(torch_dtype_code(x.dtype), _ptr(x), _ptr(out), outer, x.shape[axis], inner,
                                 _tuning(tuning), _stream(stream)))
+    return out
+
+
+# ---- a paged cache of keys and values in 8 bits, and the attention over it ------------------------------------------------
+
+
+@contextlib.contextmanager
+def _on_stream(device, stream):
+    """The stream a call runs on: ``stream`` (a raw handle) or the current one of ``device``. That device is current inside, and
+    what is allocated there belongs to that stream."""
+    import torch
+
+    with torch.cuda.device(device):
+        if stream is None:
+            yield torch.cuda.current_stream().cuda_stream
+        elif int(stream) == torch.cuda.current_stream().cuda_stream:
+            yield int(stream)
+        else:
+            with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
+                yield int(stream)
+
+
+def _same_device(first, *others):
+    assert first.is_cuda
+    for t in others:
+        assert t is None or t.device == first.device, f"{t.device} and {first.device} in one call"
+
+
+class KvCache:
+    """The tensors of a ``mhlo_cuda_kv_cache``: int8 codes ``k``, ``v`` [pages, heads, page_tokens, head_dim] and float32 scales
+    ``k_scale``, ``v_scale`` [pages, heads]. Its owner hands pages to sequences (``page_table``) as they grow."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        import torch
+
+        _same_device(k, v, k_scale, v_scale)
+        assert k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype == torch.int8 and k.is_contiguous() and v.is_contiguous()
+        assert k_scale.shape == v_scale.shape == k.shape[:2] and k_scale.dtype == v_scale.dtype == torch.float32
+        assert k_scale.is_contiguous() and v_scale.is_contiguous()
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._args = KvCacheArgs(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.shape)
+
+    @classmethod
+    def empty(cls, pages: int, heads: int, head_dim: int, page_tokens: int = 64, device="cuda") -> "KvCache":
+        import torch
+
+        codes = [torch.zeros(pages, heads, page_tokens, head_dim, dtype=torch.int8, device=device) for _ in range(2)]
+        scales = [torch.zeros(pages, heads, dtype=torch.float32, device=device) for _ in range(2)]
+        return cls(*codes, *scales)
+
+
+def _kv_batch(page_table, lengths, token_starts, tokens) -> KvBatchArgs:
+    import torch
+
+    assert page_table.dim() == 2 and lengths.dim() == 1 and page_table.shape[0] == lengths.shape[0]
+    assert page_table.dtype == lengths.dtype == torch.int32 and lengths.is_contiguous()
+    assert page_table.shape[0] <= 1 or page_table.shape[1] == 0 or page_table.stride(0) >= page_table.shape[1]
+    assert page_table.shape[1] <= 1 or page_table.stride(1) == 1
+    if token_starts is not None:
+        assert token_starts.dtype == torch.int32 and token_starts.is_contiguous() and token_starts.shape == (lengths.shape[0] + 1,)
+    stride = max(page_table.stride(0), page_table.shape[1])
+    return KvBatchArgs(page_table.data_ptr(), lengths.data_ptr(), _ptr(token_starts), page_table.shape[0], page_table.shape[1], stride, tokens)
+
+
+def _rows(x, heads=None):
+    """[tokens, heads, head_dim] with a contiguous last dimension: its {token, head} strides."""
+    assert x.dim() == 3 and (x.stride(2) == 1 or x.shape[2] <= 1) and (heads is None or x.shape[1] == heads), tuple(x.shape)
+    return _i64s(x.stride()[:2])
+
+
+def rope_table(positions: int, rotary_dim: int, base: float = 10000.0, device="cuda"):
+    """Rotation table of :func:`kv_cache_append`: float32 [positions, rotary_dim], cosines then sines of position * base^(-2i / rotary_dim),
+    computed in 64 bits (at far positions a 32-bit angle has no correct digit behind the point)."""
+    import torch
+
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+    return torch.cat([angle.cos(), angle.sin()], dim=1).float().to(device)
+
+
+def kv_cache_append(cache: KvCache, k, v, page_table, lengths, token_starts=None, rope=None, interleaved: bool = False, q=None, q_out=None, stream=None):
+    """Puts the newest tokens' k, v [tokens, heads, head_dim] into the cache, keys rotated by ``rope`` (see :func:`rope_table`), and
+    returns q [tokens, q_heads, head_dim] rotated beside them (None without q; rows of no sequence are not written). ``lengths``
+    counts the new tokens already. See ``mhlo_cuda_kv_cache_append``."""
+    import torch
+
+    _same_device(cache.k, k, v, page_table, lengths, token_starts, rope, q, q_out)
+    heads, dim = cache.k.shape[1], cache.k.shape[3]
+    assert k.dtype == v.dtype and k.shape == v.shape and k.shape[2] == dim
+    assert q is None or (q.dtype == k.dtype and q.shape[0] == k.shape[0] and q.shape[2] == dim)
+    assert rope is None or (rope.dim() == 2 and rope.dtype == torch.float32 and rope.is_contiguous())
+    batch = _kv_batch(page_table, lengths, token_starts, k.shape[0])
+    with _on_stream(k.device, stream) as s:
+        if q is not None and q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        assert q_out is None or (q is not None and q_out.shape == q.shape and q_out.dtype == q.dtype)
+        check(lib.mhlo_cuda_kv_cache_append(torch_dtype_code(k.dtype), C.byref(cache._args), C.byref(batch), _ptr(k), _rows(k, heads), _ptr(v),
+                                            _rows(v, heads), _ptr(q), None if q is None else _rows(q), _ptr(q_out),
+                                            None if q is None else _rows(q_out), 0 if q is None else q.shape[1], _ptr(rope),
+                                            0 if rope is None else rope.shape[0], 0 if rope is None else rope.shape[1], 1 if interleaved else 0, s))
+    return q_out
+
+
+def kv_cache_read(cache: KvCache, page_table, lengths, max_tokens: int, dtype=None, k_out=None, v_out=None, stream=None):
+    """(k, v), each [seqs, max_tokens, heads, head_dim] of ``dtype`` (float32): the values in the cache, zero behind a sequence's
+    length. See ``mhlo_cuda_kv_cache_read``."""
+    import torch
+
+    _same_device(cache.k, page_table, lengths, k_out, v_out)
+    batch = _kv_batch(page_table, lengths, None, lengths.shape[0])
+    shape = (lengths.shape[0], max_tokens, cache.k.shape[1], cache.k.shape[3])
+    with _on_stream(cache.k.device, stream) as s:
+        dtype = k_out.dtype if k_out is not None else dtype or torch.float32
+        k_out = torch.empty(shape, dtype=dtype, device=cache.k.device) if k_out is None else k_out
+        v_out = torch.empty_strided(shape, k_out.stride(), dtype=dtype, device=cache.k.device) if v_out is None else v_out
+        assert k_out.shape == v_out.shape == shape and k_out.dtype == v_out.dtype and k_out.stride() == v_out.stride() and k_out.stride(3) == 1
+        check(lib.mhlo_cuda_kv_cache_read(torch_dtype_code(dtype), C.byref(cache._args), C.byref(batch), max_tokens, _ptr(k_out), _ptr(v_out),
+                                          _i64s(k_out.stride()[:3]), s))
+    return k_out, v_out
+
+
+def cached_attention(q, cache: KvCache, page_table, lengths, scale: float, token_starts=None, out=None, lse=None, stream=None):
+    """Attention of the newest tokens' q [tokens, q_heads, head_dim] over the cache, which holds them (and ``lengths`` counts them).
+    ``lse`` (float32 [tokens, q_heads]) receives the logarithms of the sums of exponentials. See ``mhlo_cuda_cached_attention``."""
+    import torch
+
+    _same_device(q, cache.k, page_table, lengths, token_starts, out, lse)
+    assert q.dim() == 3 and q.shape[2] == cache.k.shape[3]
+    batch = _kv_batch(page_table, lengths, token_starts, q.shape[0])
+    with _on_stream(q.device, stream) as s:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+        assert out.shape == q.shape and out.dtype == q.dtype
+        assert lse is None or (lse.shape == q.shape[:2] and lse.dtype == torch.float32 and lse.is_contiguous())
+        need = lib.mhlo_cuda_cached_attention_scratch_bytes(C.byref(cache._args), C.byref(batch), q.shape[1])
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+        check(lib.mhlo_cuda_cached_attention(torch_dtype_code(q.dtype), _ptr(q), _rows(q), C.byref(cache._args), C.byref(batch), q.shape[1], scale,
+                                             _ptr(out), _rows(out), _ptr(lse), _ptr(scratch), max(need, 0), s))
+    return out
+
+
+# ---- log probabilities ------------------------------------------------------------------------------------------------
+
+TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprobs entropy lse top_logprobs top_ids")
+
+
+def _logit_rows(x):
+    """[..., vocab] as rows of one stride: (rows, stride)."""
+    assert x.dim() >= 1 and (x.stride(-1) == 1 or x.shape[-1] == 1)
+    if x.dim() == 1:
+        return 1, x.shape[0]
+    for d in range(x.dim() - 2):
+        assert x.shape[d] == 1 or x.stride(d) == x.stride(d + 1) * x.shape[d + 1], "the rows of the logits need one stride"
+    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+    return rows, max(x.stride(-2), x.shape[-1]) if rows > 1 else x.shape[-1]
+
+
+def token_logprobs(logits, targets=None, top_k: int = 0, scale: float = 1.0, entropy: bool = True, stream=None) -> TokenLogprobs:
+    """Log probabilities of ``targets`` [...] (int32 or int64; negative: none) under softmax(scale * logits [..., vocab]), the entropy,
+    the logarithm of the sum of exponentials and the ``top_k`` likeliest ids with their log probabilities. See ``mhlo_cuda_token_logprobs``."""
+    import torch
+
+    _same_device(logits, targets)
+    rows, pitch = _logit_rows(logits)
+    lead = logits.shape[:-1]
+    assert targets is None or (targets.shape == lead and targets.is_contiguous())
+    with _on_stream(logits.device, stream) as s:
+        new = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=logits.device)
+        r = TokenLogprobs(None if targets is None else new(*lead), new(*lead) if entropy else None, new(*lead),
+                          new(*lead, top_k) if top_k else None, new(*lead, top_k, dtype=torch.int32) if top_k else None)
+        check(lib.mhlo_cuda_token_logprobs(torch_dtype_code(logits.dtype), _ptr(logits), pitch, rows, logits.shape[-1], scale, _ptr(targets),
+                                           I64 if targets is None else torch_dtype_code(targets.dtype), _ptr(r.logprobs), _ptr(r.entropy), _ptr(r.lse),
+                                           top_k, _ptr(r.top_logprobs), _ptr(r.top_ids), s))
+    return r
+
+
+def token_logprobs_grad(logits, targets, lse, entropy=None, grad_logprobs=None, grad_entropy=None, top_ids=None, grad_top=None, scale: float = 1.0,
+                        out=None, stream=None):
+    """Gradient of :func:`token_logprobs` with respect to the logits, from the gradients of its results; ``out`` may be ``logits``. See
+    ``mhlo_cuda_token_logprobs_grad``."""
+    import torch
+
+    _same_device(logits, targets, lse, entropy, grad_logprobs, grad_entropy, top_ids, grad_top, out)
+    rows, pitch = _logit_rows(logits)
+    lead = logits.shape[:-1]
+    assert targets is None or (targets.shape == lead and targets.is_contiguous())
+    for t in (lse, entropy, grad_logprobs, grad_entropy):
+        assert t is None or (t.shape == lead and t.dtype == torch.float32 and t.is_contiguous())
+    assert grad_top is None or (top_ids is not None and grad_top.shape == top_ids.shape and top_ids.shape[:-1] == lead and grad_top.dtype == torch.float32
+                                and top_ids.dtype == torch.int32 and grad_top.is_contiguous() and top_ids.is_contiguous())
+    with _on_stream(logits.device, stream) as s:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else out
+        assert out.shape == logits.shape and out.dtype == logits.dtype
+        check(lib.mhlo_cuda_token_logprobs_grad(torch_dtype_code(logits.dtype), _ptr(logits), pitch, rows, logits.shape[-1], scale, _ptr(targets),
+                                                I64 if targets is None else torch_dtype_code(targets.dtype), _ptr(lse), _ptr(entropy), _ptr(grad_logprobs),
+                                                _ptr(grad_entropy), 0 if grad_top is None else grad_top.shape[-1], _ptr(top_ids), _ptr(grad_top),
+                                                _ptr(out), _logit_rows(out)[1], s))
     return out
