@@ -697,7 +697,7 @@ int mhlo_cuda_attention(int32_t dtype, const void* q_dev, const int64_t q_stride
  * A cache of keys and values in pages of page_tokens tokens. The codes are int8, one scale per page and head stands for the
  * whole block of page_tokens x head_dim codes: value = scale * code. All pointers are device memory, 16-byte aligned.
  *   k_codes, v_codes    [pages, heads, page_tokens, head_dim]
- *   k_scales, v_scales  [pages, heads]
+ *   k_scales, v_scales  [pages, heads], not negative
  *   page_tokens         16, 32, 64 or 128
  *   head_dim            a multiple of 16 up to 256 (attention: 64, 96, 128 or 256)
  * No counterpart in the reference, whose attention takes dense keys and values of the whole sequence

@@ -1,13 +1,38 @@
 // Attention of new tokens over the paged 8-bit key/value cache: o = softmax(scale q k^T) v with k = ks c, v = vs c.
 //
-// One CTA per (row, query head): its warps take keys in turn, a lane holds head_dim / 32 elements of q and o, and every warp keeps
-// a running maximum, sum and output that are joined at the end.
+// The work is cut into segments: (sequence, 16 rows, cache head). The rows of a segment are (token, query head) pairs that read the
+// same cache head: row r of a sequence is token r / group, query head head * group + r % group. A segment's keys are walked in tiles
+// of 32; CTAs share all tiles of the call evenly (Plan), so a CTA's piece may begin or end inside a segment. Whole segments are
+// written at once, pieces go to scratch as (maximum, sum, output) and a second kernel joins them in the order of the CTAs.
+//
+// Inside a CTA every warp takes tiles by itself and keeps a running maximum, sum and output of its 16 rows; the warps are joined
+// through shared memory at the end of a segment. Nothing but the segment's end synchronises the warps.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_cache.cuh"
 
 namespace mhlo {
 namespace {
+
+constexpr int kTileKeys = 32;
+constexpr int kRows = 16;
+constexpr int kLeastTiles = 12;  // a CTA's share where there is little to do: a tile per warp
+constexpr int kGrid = kNumSMs;   // one CTA per SM: the rings of its warps take the shared memory
+
+template <int D>
+struct Layout {
+    static constexpr int kWarps = D == 256 ? 6 : 12;
+    static constexpr int kThreads = 32 * kWarps;
+    static constexpr int kStages = D == 64 ? 4 : 2;
+    static constexpr int kTileBytes = kTileKeys * D;  // of keys, and of values
+    static constexpr int kRing = kWarps * kStages * 2 * kTileBytes;
+    // A row of codes is stored as parts of 128, 64 or 32 bytes, each [32 keys][W].
+    static constexpr int kParts = D == 256 ? 2 : D == 96 ? 2 : 1;
+    __host__ __device__ static constexpr int width(int part) { return D == 96 ? (part == 0 ? 64 : 32) : D == 64 ? 64 : 128; }
+    __host__ __device__ static constexpr int first(int part) { return part == 0 ? 0 : D == 96 ? 64 : 128; }
+    static constexpr int kSteps = D / 16;
+};
 
 template <typename T>
 struct CachedParams {
@@ -18,54 +43,626 @@ struct CachedParams {
     int64_t qs[2], os[2];
     int32_t q_heads, group;
     float scale;
+    int32_t whole;      // no segment has more than kLeastTiles tiles: none is cut
+    int32_t o_vec;      // four results at a time
+    int32_t* pieces;    // [kGrid][8]: the cut segment that a CTA's share ends with (Piece), count 0 if none
+    float* partial;     // [kGrid][2][kRows (D + 2)]
 };
 
-constexpr int kRowThreads = 128, kRowWarps = kRowThreads / 32;
+struct Piece {  // what joining a cut segment needs
+    int32_t count, first_row, rows, seq_first, head, pad[3];
+};
+
+// ---- how the work is shared ------------------------------------------------------------------------------------------------
+
+struct Share {  // of one sequence
+    KvSequence s;
+    int32_t row_tiles, tiles;  // of 16 rows; of 32 keys (1 where there are none: somebody has to write the zeros)
+};
 
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) cached_rows_kernel(const __grid_constant__ CachedParams<T> p) {
+__device__ __forceinline__ Share share_of(const CachedParams<T>& p, int32_t b) {
+    Share w;
+    w.s = kv_sequence(p.kv, b);
+    w.row_tiles = static_cast<int32_t>((static_cast<int64_t>(w.s.count) * p.group + kRows - 1) / kRows);
+    w.tiles = max(1, (w.s.length + kTileKeys - 1) / kTileKeys);
+    return w;
+}
+
+__device__ __forceinline__ int32_t padded(int32_t tiles) { return (tiles + kLeastTiles - 1) / kLeastTiles * kLeastTiles; }
+
+__device__ __forceinline__ int64_t warp_sum(int64_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// ---- the kernel's parts ----------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void mma_f16(float* d, const uint4& a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// Codes as fp16, exactly: 0x64xx is 1024 + xx, so a code with its sign bit turned round behind 0x64 is 1152 + code.
+constexpr uint32_t kSignBits = 0x80808080u, kMagic = 0x64646464u;
+__device__ __forceinline__ uint32_t unbias(uint32_t x) {
+    const uint32_t bias = 0x64806480u;  // 1152, 1152
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void cp_async16(uint32_t smem, const void* src) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(smem), "l"(src) : "memory");
+}
+
+// Where 16-byte chunk `chunk` of row `row` of a part lies. Keys are read 16 bytes a lane, four lanes a row; values by eight groups of
+// lanes, each W / 8 bytes of rows 2 c + e (c = 0 .. 3). The exclusive ors make both free of bank conflicts for 128-byte and 64-byte
+// parts; 32-byte parts lie in order.
+template <int W, bool VALUES>
+__device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
+    if (W == 128) return row * 128 + ((chunk ^ (VALUES ? row & 6 : (row & 1) << 2)) << 4);
+    if (W == 64) {
+        const int slot = (row & 1) * 4 + chunk;
+        return (row >> 1) * 128 + ((VALUES ? slot ^ (row & 6) : slot) << 4);
+    }
+    return row * 32 + (chunk << 4);
+}
+
+// Starts the copies of one tile's keys and values: halves of 16 keys, each contiguous in a page. base[h] = first code of half h, -1: not there.
+template <int D>
+__device__ __forceinline__ void load_tile(const KvArgs& a, uint32_t keys, int64_t base0, int64_t base1) {
+    using L = Layout<D>;
+    const int lane = threadIdx.x & 31;
+    constexpr int kChunks = D / 16;  // of a row
+#pragma unroll
+    for (int i = 0; i < kTileKeys * kChunks / 32; ++i) {
+        const int index = i * 32 + lane, row = index / kChunks, chunk = index % kChunks;
+        const int64_t base = row < 16 ? base0 : base1;
+        const int64_t at = base + (row & 15) * D + chunk * 16;
+        const int part = L::kParts == 1 ? 0 : chunk * 16 >= L::first(1);
+        const int c = part == 0 ? chunk : chunk - L::first(1) / 16;
+        uint32_t ko, vo;
+        if (part == 0) {
+            ko = chunk_at<L::width(0), false>(row, c);
+            vo = chunk_at<L::width(0), true>(row, c);
+        } else {
+            ko = kTileKeys * L::width(0) + chunk_at<L::width(1), false>(row, c);
+            vo = kTileKeys * L::width(0) + chunk_at<L::width(1), true>(row, c);
+        }
+        if (base >= 0) {
+            cp_async16(keys + ko, a.k_codes + at);
+            cp_async16(keys + L::kTileBytes + vo, a.v_codes + at);
+        }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+// Fragment order of a row's elements. A step of 16 products uses, from lane c of four, four neighbouring elements: in a 64-byte
+// stretch those at 16 c + 4 s (s = 0 .. 3), in a 32-byte part those at 8 c + 4 s (s = 0, 1). Any order will do as long as q and k agree.
+template <int D>
+__device__ __forceinline__ int step_element(int step, int c) {
+    if (D == 96 && step >= 4) return 64 + 8 * c + 4 * (step - 4);
+    return 64 * (step >> 2) + 16 * c + 4 * (step & 3);
+}
+
+constexpr float kWeightUnit = 16384.f;  // fp16 weights are held times 2^14: the largest is 2^14, the smallest step 2^-24
+
+template <typename T, int D>
+__global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kernel(const __grid_constant__ CachedParams<T> p) {
+    using L = Layout<D>;
+    constexpr bool kTwoParts = sizeof(T) == 4;  // fp32: q and the weights as sums of two fp16 numbers
+    constexpr int W = L::kWarps;
+    extern __shared__ __align__(128) uint8_t smem[];
+    uint4* const q_frag = reinterpret_cast<uint4*>(smem + L::kRing);  // [1 or 2 parts][steps][32]
+    __shared__ float row_factor[kRows];                               // scale log2(e) 2^exponent of the row's q
+    __shared__ float sm[W][kRows], sl[W][kRows], sf[W][kRows], sv[W], top_m[kRows], top_l[kRows];
+    __shared__ int32_t used[W];
+    __shared__ float4 meta[W][L::kStages];  // scales of a tile's halves: keys 0, 1 (-infinity: not there), values 0, 1
+    __shared__ int64_t totals[2], found[2];
+    __shared__ int64_t scan[32];
+
     const KvArgs& a = p.kv;
-    const int32_t h = static_cast<int32_t>(blockIdx.x % p.q_heads), row = static_cast<int32_t>(blockIdx.x / p.q_heads);
-    int32_t b = row;
-    if (a.starts != nullptr) b = kv_search(a.seqs, row, [&](int32_t i) { return static_cast<int64_t>(a.starts[i]); });
-    const KvSequence s = kv_sequence(a, b);
-    if (row < s.first || row >= s.first + s.count) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, dim = a.head_dim, each = dim / 32, head = h / p.group;
-    const int32_t keys = s.length == 0 ? 0 : s.position(row) + 1;
-    float q[8], o[8], m = -INFINITY, l = 0.f;
-    for (int i = 0; i < each; ++i) {
-        q[i] = VecTraits<T>::to_float(p.q[row * p.qs[0] + h * p.qs[1] + lane + 32 * i]);
-        o[i] = 0.f;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
+
+    // -- the share of this CTA
+    {
+        int64_t all = 0, all_padded = 0;
+        for (int32_t b = tid; b < a.seqs; b += L::kThreads) {
+            const Share w = share_of(p, b);
+            const int64_t segments = static_cast<int64_t>(w.row_tiles) * a.heads;
+            all += segments * w.tiles;
+            all_padded += segments * padded(w.tiles);
+        }
+        all = warp_sum(all);
+        all_padded = warp_sum(all_padded);
+        if (lane == 0) scan[warp] = all, scan[16 + warp] = all_padded;
+        __syncthreads();
+        if (tid == 0) {
+            int64_t x = 0, y = 0;
+            for (int w = 0; w < W; ++w) x += scan[w], y += scan[16 + w];
+            totals[0] = x;
+            totals[1] = y;
+            found[0] = -1;
+        }
+        __syncthreads();
     }
-    for (int32_t j = warp; j < keys; j += kRowWarps) {
-        const int32_t page = kv_page(a, b, j >> a.page_shift);
-        if (page < 0) continue;
-        const int64_t block = static_cast<int64_t>(page) * a.heads + head, at = ((block << a.page_shift) + (j & ((1 << a.page_shift) - 1))) * dim + lane;
-        float z = 0.f;
-        for (int i = 0; i < each; ++i) z += q[i] * static_cast<float>(a.k_codes[at + 32 * i]);
-        z = warp_reduce<SumOp>(z) * a.k_scales[block] * p.scale;
-        const float top = fmaxf(m, z), keep = m == top ? 1.f : expf(m - top), w = z == top ? 1.f : expf(z - top);
-        m = top;
-        l = l * keep + w;
-        for (int i = 0; i < each; ++i) o[i] = o[i] * keep + w * a.v_scales[block] * static_cast<float>(a.v_codes[at + 32 * i]);
+    const bool pad = p.whole || totals[1] <= static_cast<int64_t>(kGrid) * kLeastTiles;
+    const int64_t total = totals[pad ? 1 : 0];
+    const int64_t per = pad ? (totals[1] / kLeastTiles + kGrid - 1) / kGrid * kLeastTiles : (total + kGrid - 1) / kGrid;
+    int64_t at = blockIdx.x * per;
+    const int64_t end = min(total, at + per);
+    if (tid == 0) p.pieces[blockIdx.x * 8] = 0;
+    grid_dependency_release();
+    if (at >= end) return;
+    // the sequence that holds tile `at`, and where in it
+    {
+        int64_t before = 0;
+        for (int32_t base = 0; base < a.seqs; base += L::kThreads) {
+            int64_t mine = 0;
+            if (base + tid < a.seqs) {
+                const Share w = share_of(p, base + tid);
+                mine = static_cast<int64_t>(w.row_tiles) * a.heads * (pad ? padded(w.tiles) : w.tiles);
+            }
+            int64_t sum = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t other = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += other;
+            }
+            if (lane == 31) scan[warp] = sum;
+            __syncthreads();
+            int64_t chunk = 0, lower = 0;
+            for (int w = 0; w < W; ++w) {
+                lower += w < warp ? scan[w] : 0;
+                chunk += scan[w];
+            }
+            const int64_t first = before + lower + sum - mine;
+            if (mine > 0 && at >= first && at < first + mine) {
+                found[0] = base + tid;
+                found[1] = at - first;
+            }
+            before += chunk;
+            __syncthreads();
+            if (before > at) break;
+        }
     }
-    __shared__ float sm[kRowWarps], sl[kRowWarps], so[kRowWarps][256];
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
-    for (int i = 0; i < each; ++i) so[warp][lane + 32 * i] = o[i];
-    __syncthreads();
-    float top = -INFINITY, total = 0.f;
-    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm[w]);
-    for (int w = 0; w < kRowWarps; ++w) total += sl[w] * (sm[w] == top ? 1.f : expf(sm[w] - top));
-    for (int d = threadIdx.x; d < dim; d += kRowThreads) {
+    int32_t b = static_cast<int32_t>(found[0]);
+    if (b < 0) return;  // cannot be: lengths that change under the kernel
+    Share w = share_of(p, b);
+    int64_t inside = found[1];
+
+    while (at < end) {
+        const int32_t tiles = pad ? padded(w.tiles) : w.tiles;
+        const int64_t segments = static_cast<int64_t>(w.row_tiles) * a.heads;
+        if (inside >= segments * tiles) {  // on to the next sequence that has work
+            if (++b >= a.seqs) return;
+            w = share_of(p, b);
+            inside = 0;
+            continue;
+        }
+        const int32_t segment = static_cast<int32_t>(inside / tiles), t0 = static_cast<int32_t>(inside % tiles);
+        const int32_t head = segment % a.heads, row_tile = segment / a.heads;
+        const int32_t t1 = static_cast<int32_t>(min(static_cast<int64_t>(tiles), t0 + (end - at)));
+        const int32_t all_rows = w.s.count * p.group, row0 = row_tile * kRows, rows = min(kRows, all_rows - row0);
+        // keys that row r sees
+        auto seen_by = [&](int r) { return w.s.length == 0 ? 0 : w.s.length - w.s.count + (row0 + r) / p.group + 1; };
+        const int32_t limit = seen_by(rows - 1), least = seen_by(0);
+        const int32_t last = min(t1, (limit + kTileKeys - 1) / kTileKeys);  // tiles t0 .. last - 1 have keys to read
+
+        // -- q as fragments in shared memory, rows brought to the same size by powers of two
+        const float to_log2 = p.scale * 1.4426950408889634f;
+        for (int r = warp; r < kRows; r += W) {
+            const int32_t row = row0 + r;
+            float most = 0.f;
+            if (!std::is_same<T, __half>::value) {
+                if (r < rows) {
+                    const T* q = p.q + (w.s.first + row / p.group) * p.qs[0] + (head * p.group + row % p.group) * p.qs[1];
+                    for (int d = lane; d < D; d += 32) most = fmaxf(most, fabsf(VecTraits<T>::to_float(q[d])));
+                }
+                most = warp_reduce<MaxOp>(most);
+            }
+            int shift = 0;
+            if (most > 0.f && most < INFINITY) shift = max(-120, ilogbf(most) - 13);
+            if (lane == 0) {
+                row_factor[r] = scalbnf(to_log2, shift);
+                sf[0][r] = scalbnf(1.f, -shift);
+            }
+        }
+        __syncthreads();
+        for (int i = tid; i < L::kSteps * 32; i += L::kThreads) {
+            const int step = i >> 5, l = i & 31;
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {  // rows g and g + 8
+                const int r = (l >> 2) + 8 * half;
+                float x[4] = {0.f, 0.f, 0.f, 0.f};
+                if (r < rows) {
+                    const int32_t row = row0 + r;
+                    const T* q = p.q + (w.s.first + row / p.group) * p.qs[0] + (head * p.group + row % p.group) * p.qs[1] + step_element<D>(step, l & 3);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = VecTraits<T>::to_float(q[e]) * sf[0][r];
+                }
+                hi[half] = pack_half2(x[0], x[1]);
+                hi[2 + half] = pack_half2(x[2], x[3]);
+                if (kTwoParts) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] -= __half2float(__float2half_rn(x[e]));
+                    lo[half] = pack_half2(x[0], x[1]);
+                    lo[2 + half] = pack_half2(x[2], x[3]);
+                }
+            }
+            q_frag[i] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            if (kTwoParts) q_frag[L::kSteps * 32 + i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        __syncthreads();
+
+        // -- this warp's tiles: t0 + warp, t0 + warp + W, ...
+        float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, v_most = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+        const float factor[2] = {row_factor[g], row_factor[g + 8]};
+        const int32_t mine = last > t0 + warp ? (last - t0 - warp + W - 1) / W : 0;
+        const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * L::kStages * 2 * L::kTileBytes;
+        // Pages and scales of 16 tiles at a time, a half tile per lane.
+        int64_t base = -1;
+        float ks = 0.f, vs = 0.f;
+        auto issue = [&](int32_t i) {
+            if (i < mine) {
+                if ((i & 15) == 0) {
+                    const int32_t tile = t0 + warp + (i + (lane >> 1)) * W, key = tile * kTileKeys + (lane & 1) * 16;
+                    base = -1;
+                    if (tile < last && key < limit) {
+                        const int32_t page = kv_page(a, b, key >> a.page_shift);
+                        if (page >= 0) {
+                            const int64_t block = static_cast<int64_t>(page) * a.heads + head;
+                            base = ((block << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * D;
+                            ks = a.k_scales[block];
+                            vs = a.v_scales[block];
+                        }
+                    }
+                }
+                const int from = (i & 15) * 2, stage = i % L::kStages;
+                const int64_t base0 = __shfl_sync(0xffffffffu, base, from), base1 = __shfl_sync(0xffffffffu, base, from + 1);
+                load_tile<D>(a, ring + stage * 2 * L::kTileBytes, base0, base1);
+                const float k1 = __shfl_down_sync(0xffffffffu, ks, 1), v1 = __shfl_down_sync(0xffffffffu, vs, 1);
+                if (lane == from) meta[warp][stage] = make_float4(base0 < 0 ? -INFINITY : ks, base1 < 0 ? -INFINITY : k1, vs, v1);
+            } else {
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
+        };
+        for (int i = 0; i < L::kStages - 1; ++i) issue(i);
+        for (int32_t i = 0; i < mine; ++i) {
+            issue(i + L::kStages - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(L::kStages - 1) : "memory");
+            __syncwarp();
+            const int stage = i % L::kStages;
+            const uint8_t* const keys = smem + warp * L::kStages * 2 * L::kTileBytes + stage * 2 * L::kTileBytes;
+            const uint8_t* const values = keys + L::kTileBytes;
+            const float4 scales = meta[warp][stage];
+            const bool half_there[2] = {scales.x != -INFINITY, scales.y != -INFINITY};
+
+            // S = q c^T: four groups of eight keys
+            float s[4][4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+            for (int part = 0; part < L::kParts; ++part) {
+                const int width = L::width(part), step0 = L::first(part) / 16;
+                const uint8_t* const base_part = keys + kTileKeys * L::first(part);
+#pragma unroll
+                for (int chunk = 0; chunk < (width + 63) / 64; ++chunk) {
+                    uint32_t codes[4][4];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const int row = n * 8 + g;
+                        if (width == 32) {
+                            const uint2 x = *reinterpret_cast<const uint2*>(base_part + row * 32 + c * 8);
+                            codes[n][0] = x.x ^ kSignBits;
+                            codes[n][1] = x.y ^ kSignBits;
+                        } else {
+                            const uint32_t where = width == 128 ? chunk_at<128, false>(row, chunk * 4 + c) : chunk_at<64, false>(row, c);
+                            const uint4 x = *reinterpret_cast<const uint4*>(base_part + where);
+                            codes[n][0] = x.x ^ kSignBits;
+                            codes[n][1] = x.y ^ kSignBits;
+                            codes[n][2] = x.z ^ kSignBits;
+                            codes[n][3] = x.w ^ kSignBits;
+                        }
+                    }
+#pragma unroll
+                    for (int i4 = 0; i4 < (width == 32 ? 2 : 4); ++i4) {
+                        const int step = step0 + chunk * 4 + i4;
+                        const uint4 qa = q_frag[step * 32 + lane];
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const uint32_t b0 = unbias(__byte_perm(codes[n][i4], kMagic, 0x4140)), b1 = unbias(__byte_perm(codes[n][i4], kMagic, 0x4342));
+                            mma_f16(s[n], qa, b0, b1);
+                            if (kTwoParts) mma_f16(s[n], q_frag[L::kSteps * 32 + step * 32 + lane], b0, b1);
+                        }
+                    }
+                }
+            }
+            // scores in units of log2(e), masked
+            const int32_t key0 = (t0 + warp + i * W) * kTileKeys;
+            const float k_scale[2] = {scales.x, scales.y};
+            float top[2] = {m[0], m[1]};
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[n][e] *= factor[e >> 1] * k_scale[n >> 1];
+            const bool edge = key0 + kTileKeys > least || !half_there[0] || !half_there[1];
+            if (edge) {
+                const int32_t seen[2] = {seen_by(g), seen_by(g + 8)};
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!half_there[n >> 1] || key0 + n * 8 + 2 * c + (e & 1) >= seen[e >> 1]) s[n][e] = -INFINITY;
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+            }
+            // the largest value scale so far is the unit of the output
+            const float v_scale[2] = {half_there[0] ? scales.z : 0.f, half_there[1] ? scales.w : 0.f};
+            const float v_top = fmaxf(v_most, fmaxf(v_scale[0], v_scale[1]));
+            if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1] || v_top > v_most)) {
+                const float unit = v_top > v_most ? v_most / v_top : 1.f;
+                float keep[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    keep[r] = top[r] > m[r] ? ex2(m[r] - top[r]) : 1.f;
+                    l[r] *= keep[r];
+                    keep[r] *= unit;
+                    m[r] = top[r];
+                }
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][e] *= keep[e >> 1];
+                v_most = v_top;
+            }
+            const float shift[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+            const float ratio[2] = {v_scale[0] == 0.f ? 0.f : kWeightUnit * (v_scale[0] / v_most), v_scale[1] == 0.f ? 0.f : kWeightUnit * (v_scale[1] / v_most)};
+            // weights: fragments of P, keys 2 c, 2 c + 1 and 8 + 2 c, 9 + 2 c of each half
+            uint4 pa[2], pb[2];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float x[2][4];
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float z = s[half * 2 + n][e], weight = ex2(z - shift[e >> 1]);
+                        l[e >> 1] += weight;
+                        x[n][e] = weight * ratio[half];
+                        if (edge && z == -INFINITY) x[n][e] = 0.f;  // whatever the scale of a block that the row does not see
+                    }
+                pa[half] = make_uint4(pack_half2(x[0][0], x[0][1]), pack_half2(x[0][2], x[0][3]), pack_half2(x[1][0], x[1][1]), pack_half2(x[1][2], x[1][3]));
+                if (kTwoParts) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[n][e] -= __half2float(__float2half_rn(x[n][e]));
+                    pb[half] = make_uint4(pack_half2(x[0][0], x[0][1]), pack_half2(x[0][2], x[0][3]), pack_half2(x[1][0], x[1][1]), pack_half2(x[1][2], x[1][3]));
+                }
+            }
+            // O += P c: group g of lanes holds W / 8 neighbouring elements of a part, one per product
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int part = 0; part < L::kParts; ++part) {
+                    const int width = L::width(part), words = width / 32, j0 = L::first(part) / 8;
+                    const uint8_t* const base_part = values + kTileKeys * L::first(part);
+                    uint32_t rows4[4][4];  // rows 2 c, 2 c + 1, 8 + 2 c, 9 + 2 c
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int row = half * 16 + (r >> 1) * 8 + 2 * c + (r & 1);
+                        if (width == 128) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(base_part + chunk_at<128, true>(row, g));
+                            rows4[r][0] = x.x ^ kSignBits;
+                            rows4[r][1] = x.y ^ kSignBits;
+                            rows4[r][2] = x.z ^ kSignBits;
+                            rows4[r][3] = x.w ^ kSignBits;
+                        } else if (width == 64) {
+                            const uint2 x = *reinterpret_cast<const uint2*>(base_part + chunk_at<64, true>(row, g >> 1) + (g & 1) * 8);
+                            rows4[r][0] = x.x ^ kSignBits;
+                            rows4[r][1] = x.y ^ kSignBits;
+                        } else {
+                            rows4[r][0] = *reinterpret_cast<const uint32_t*>(base_part + row * 32 + g * 4) ^ kSignBits;
+                        }
+                    }
+#pragma unroll
+                    for (int word = 0; word < words; ++word) {
+#pragma unroll
+                        for (int pair = 0; pair < 2; ++pair) {  // bytes 2 pair, 2 pair + 1
+                            const uint32_t even = __byte_perm(rows4[0][word], rows4[1][word], pair ? 0x7362 : 0x5140);
+                            const uint32_t odd = __byte_perm(rows4[2][word], rows4[3][word], pair ? 0x7362 : 0x5140);
+#pragma unroll
+                            for (int byte = 0; byte < 2; ++byte) {
+                                const uint32_t order = byte ? 0x4342 : 0x4140;
+                                const uint32_t b0 = unbias(__byte_perm(even, kMagic, order)), b1 = unbias(__byte_perm(odd, kMagic, order));
+                                float* const acc = o[j0 + word * 4 + pair * 2 + byte];
+                                mma_f16(acc, pa[half], b0, b1);
+                                if (kTwoParts) mma_f16(acc, pb[half], b0, b1);
+                            }
+                        }
+                    }
+                }
+            __syncwarp();
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();  // every warp is done with the rings: they hold the warps' outputs now
+
+        // -- join the warps. A lane holds W / 4 neighbouring elements (from W / 4 * c) of rows g and g + 8 of each part.
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        }
+        if (c == 0) {
+            sm[warp][g] = m[0];
+            sm[warp][g + 8] = m[1];
+            sl[warp][g] = l[0];
+            sl[warp][g + 8] = l[1];
+        }
+        if (lane == 0) {
+            sv[warp] = v_most;
+            used[warp] = mine > 0;
+        }
+        float4* const joined = reinterpret_cast<float4*>(smem);  // [warp][row][D / 4], chunks turned against bank conflicts
+        auto joined_at = [](int w_, int row, int d4) { return (w_ * kRows + row) * (D / 4) + (d4 ^ ((d4 >> 3) & 7) ^ ((row & 1) << 2)); };
+        if (mine > 0) {
+#pragma unroll
+            for (int part = 0; part < L::kParts; ++part) {
+                const int width = L::width(part), j0 = L::first(part) / 8, each = width / 8;
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int col = 0; col < 2; ++col)
+#pragma unroll
+                        for (int k = 0; k < each; k += 4) {
+                            const int d = L::first(part) + (2 * c + col) * each + k, e = half * 2 + col;
+                            joined[joined_at(warp, g + 8 * half, d >> 2)] = make_float4(o[j0 + k][e], o[j0 + k + 1][e], o[j0 + k + 2][e], o[j0 + k + 3][e]);
+                        }
+            }
+        }
+        __syncthreads();
+        if (tid < kRows) {
+            float most = -INFINITY, sum = 0.f;
+            for (int i = 0; i < W; ++i) most = fmaxf(most, sm[i][tid]);
+            const float shift = most == -INFINITY ? 0.f : most;
+            for (int i = 0; i < W; ++i) {
+                const float f = ex2(sm[i][tid] - shift);
+                sum += sl[i][tid] * f;
+                sf[i][tid] = f * sv[i] * (1.f / kWeightUnit);
+            }
+            top_m[tid] = most;
+            top_l[tid] = sum;
+        }
+        __syncthreads();
+        const bool cut = t0 != 0 || t1 != tiles;
+        float* const out = p.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (t0 == 0 ? 1 : 0)) * (kRows * (D + 2));
+        for (int i = tid; i < kRows * (D / 4); i += L::kThreads) {
+            const int r = i / (D / 4), d4 = i % (D / 4);
+            if (r >= rows) break;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < W; ++k) {
+                if (!used[k]) continue;
+                const float4 x = joined[joined_at(k, r, d4)];
+                const float f = sf[k][r];
+                sum.x += x.x * f;
+                sum.y += x.y * f;
+                sum.z += x.z * f;
+                sum.w += x.w * f;
+            }
+            if (cut) {
+                reinterpret_cast<float4*>(out + 2 * kRows)[i] = sum;
+                continue;
+            }
+            const float total_l = top_l[r], inv = total_l == 0.f ? 0.f : 1.f / total_l;
+            const int32_t row = row0 + r;
+            T* const y = p.o + (w.s.first + row / p.group) * p.os[0] + (head * p.group + row % p.group) * p.os[1] + d4 * 4;
+            const float4 x = total_l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+            if constexpr (sizeof(T) == 4) {
+                if (p.o_vec) *reinterpret_cast<float4*>(y) = x;
+                else y[0] = x.x, y[1] = x.y, y[2] = x.z, y[3] = x.w;
+            } else {
+                const float xs[8] = {x.x, x.y, x.z, x.w, 0.f, 0.f, 0.f, 0.f};
+                const uint4 packed = VecTraits<T>::pack(xs);
+                if (p.o_vec) *reinterpret_cast<uint2*>(y) = make_uint2(packed.x, packed.y);
+                else
+                    for (int e = 0; e < 4; ++e) y[e] = VecTraits<T>::from_float(xs[e]);
+            }
+        }
+        if (tid < rows) {
+            if (cut) {
+                out[tid] = top_m[tid];
+                out[kRows + tid] = top_l[tid];
+            } else if (p.lse != nullptr) {
+                const int32_t row = row0 + tid;
+                p.lse[static_cast<int64_t>(w.s.first + row / p.group) * p.q_heads + head * p.group + row % p.group] =
+                    top_l[tid] == 0.f ? -INFINITY : (top_m[tid] + log2f(top_l[tid])) * 0.6931471805599453f;
+            }
+        }
+        if (cut && t0 == 0 && tid == 0) {
+            const int64_t last_cta = (at + tiles - 1) / per;
+            int32_t* const piece = p.pieces + blockIdx.x * 8;
+            piece[1] = row0;
+            piece[2] = rows;
+            piece[3] = w.s.first;
+            piece[4] = head;
+            piece[0] = static_cast<int32_t>(last_cta - blockIdx.x) + 1;
+        }
+        __syncthreads();
+        at += t1 - t0;
+        inside += t1 - t0;
+    }
+}
+
+// Joins the pieces of the segment that CTA blockIdx.x began and others went on with: sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
+template <typename T, int D>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ CachedParams<T> p) {
+    grid_dependency_wait();
+    const int32_t* const piece = p.pieces + blockIdx.x * 8;
+    const int32_t count = piece[0];
+    if (count == 0) return;
+    const int32_t row0 = piece[1], rows = piece[2], seq_first = piece[3], head = piece[4];
+    auto part = [&](int32_t i) { return p.partial + ((static_cast<int64_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0)) * (kRows * (D + 2)); };
+    const int r = blockIdx.y;
+    if (r >= rows) return;
+    float most = -INFINITY;
+    for (int32_t i = 0; i < count; ++i) most = fmaxf(most, part(i)[r]);
+    const float shift = most == -INFINITY ? 0.f : most;
+    const int32_t row = row0 + r;
+    const int64_t token = seq_first + row / p.group, q_head = head * p.group + row % p.group;
+    float total = 0.f;
+    for (int32_t i = 0; i < count; ++i) total += part(i)[kRows + r] * ex2(part(i)[r] - shift);
+    for (int d = threadIdx.x; d < D; d += 128) {
         float sum = 0.f;
-        for (int w = 0; w < kRowWarps; ++w) sum += so[w][d] * (sm[w] == top ? 1.f : expf(sm[w] - top));
-        p.o[row * p.os[0] + h * p.os[1] + d] = VecTraits<T>::from_float(total == 0.f ? 0.f : sum / total);
+        for (int32_t i = 0; i < count; ++i) sum += part(i)[2 * kRows + r * D + d] * ex2(part(i)[r] - shift);
+        p.o[token * p.os[0] + q_head * p.os[1] + d] = VecTraits<T>::from_float(total == 0.f ? 0.f : sum / total);
     }
-    if (p.lse != nullptr && threadIdx.x == 0) p.lse[static_cast<int64_t>(row) * p.q_heads + h] = total == 0.f ? -INFINITY : top + logf(total);
+    if (p.lse != nullptr && threadIdx.x == 0) p.lse[token * p.q_heads + q_head] = total == 0.f ? -INFINITY : (most + log2f(total)) * 0.6931471805599453f;
+}
+
+template <int D>
+constexpr int64_t scratch_bytes() { return kGrid * (8 * 4 + 2 * kRows * (D + 2) * 4); }
+
+template <typename T, int D>
+int launch_rows(CachedParams<T> p, void* scratch, cudaStream_t stream) {
+    using L = Layout<D>;
+    p.pieces = static_cast<int32_t*>(scratch);
+    p.partial = reinterpret_cast<float*>(p.pieces + kGrid * 8);
+    constexpr int smem = L::kRing + L::kSteps * 32 * 16 * (sizeof(T) == 4 ? 2 : 1);
+    auto kernel = cached_attention_kernel<T, D>;
+    static std::atomic<bool> smem_set[64];
+    if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, smem_set)) return st;
+    kernel<<<kGrid, L::kThreads, smem, stream>>>(p);
+    MHLO_CUDA_CHECK_LAUNCH("cached_attention");
+    if (p.whole) return MHLO_CUDA_OK;
+    const cudaError_t e = launch_dependent(join_kernel<T, D>, dim3(kGrid, kRows), dim3(128), 0, stream, 1, true, p);
+    if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of cached_attention failed: %s", cudaGetErrorString(e));
+    MHLO_CUDA_CHECK_LAUNCH("cached_attention (joining)");
+    return MHLO_CUDA_OK;
 }
 
 template <typename T>
-int launch(const KvArgs& kv, const void* q, const int64_t* qs, int64_t q_heads, float scale, void* o, const int64_t* os, float* lse, cudaStream_t stream) {
+int launch(const KvArgs& kv, const void* q, const int64_t* qs, int64_t q_heads, float scale, void* o, const int64_t* os, float* lse, void* scratch, cudaStream_t stream) {
     CachedParams<T> p;
     p.kv = kv;
     p.q = static_cast<const T*>(q);
@@ -75,10 +672,15 @@ int launch(const KvArgs& kv, const void* q, const int64_t* qs, int64_t q_heads, 
     p.q_heads = static_cast<int32_t>(q_heads);
     p.group = static_cast<int32_t>(q_heads / kv.heads);
     p.scale = scale;
-    if (kv.tokens * q_heads > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "cached_attention: too many rows");
-    cached_rows_kernel<T><<<static_cast<unsigned>(kv.tokens * q_heads), kRowThreads, 0, stream>>>(p);
-    MHLO_CUDA_CHECK_LAUNCH("cached_attention");
-    return MHLO_CUDA_OK;
+    p.whole = (static_cast<int64_t>(kv.pages_per_seq) << kv.page_shift) <= kLeastTiles * kTileKeys;
+    const int64_t four = 4 * static_cast<int64_t>(sizeof(T));
+    p.o_vec = reinterpret_cast<uintptr_t>(o) % four == 0 && os[0] % 4 == 0 && os[1] % 4 == 0;
+    switch (kv.head_dim) {
+        case 64: return launch_rows<T, 64>(p, scratch, stream);
+        case 96: return launch_rows<T, 96>(p, scratch, stream);
+        case 128: return launch_rows<T, 128>(p, scratch, stream);
+        default: return launch_rows<T, 256>(p, scratch, stream);
+    }
 }
 
 }  // namespace
@@ -93,7 +695,13 @@ extern "C" {
 
 int64_t mhlo_cuda_cached_attention_scratch_bytes(const mhlo_cuda_kv_cache* cache, const mhlo_cuda_kv_batch* batch, int64_t q_heads) {
     if (!cache || !batch || q_heads < 1) return 0;
-    return 0;
+    switch (cache->head_dim) {
+        case 64: return scratch_bytes<64>();
+        case 96: return scratch_bytes<96>();
+        case 128: return scratch_bytes<128>();
+        case 256: return scratch_bytes<256>();
+        default: return 0;
+    }
 }
 
 int mhlo_cuda_cached_attention(int32_t dtype, const void* q_dev, const int64_t q_strides[2], const mhlo_cuda_kv_cache* cache, const mhlo_cuda_kv_batch* batch,
@@ -120,9 +728,9 @@ int mhlo_cuda_cached_attention(int32_t dtype, const void* q_dev, const int64_t q
     if (need > 0 && (!scratch_dev || scratch_bytes < need || !aligned16(scratch_dev)))
         return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: needs %lld bytes of 16-byte aligned scratch", what, static_cast<long long>(need));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == MHLO_DT_F32) return launch<float>(kv, q_dev, q_strides, q_heads, scale, o_dev, o_strides, lse_dev, st);
-    if (dtype == MHLO_DT_F16) return launch<__half>(kv, q_dev, q_strides, q_heads, scale, o_dev, o_strides, lse_dev, st);
-    return launch<__nv_bfloat16>(kv, q_dev, q_strides, q_heads, scale, o_dev, o_strides, lse_dev, st);
+    if (dtype == MHLO_DT_F32) return launch<float>(kv, q_dev, q_strides, q_heads, scale, o_dev, o_strides, lse_dev, scratch_dev, st);
+    if (dtype == MHLO_DT_F16) return launch<__half>(kv, q_dev, q_strides, q_heads, scale, o_dev, o_strides, lse_dev, scratch_dev, st);
+    return launch<__nv_bfloat16>(kv, q_dev, q_strides, q_heads, scale, o_dev, o_strides, lse_dev, scratch_dev, st);
 }
 
 }  // extern "C"

@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 
@@ -116,6 +117,18 @@ constexpr size_t kScratchKept = size_t{256} << 20;
 int scratch_alloc(void** out, size_t bytes, cudaStream_t stream);
 int scratch_free(void* p, cudaStream_t stream);
 void scratch_trim();  // current device
+
+// Lets `kernel` have `bytes` of dynamic shared memory. The attribute belongs to the (kernel, device) pair: `done` holds the kernel's
+// flags, one per device ordinal.
+inline int allow_dynamic_smem(const void* kernel, int bytes, std::atomic<bool> (&done)[64]) {
+    int dev = 0;
+    MHLO_CUDA_TRY(cudaGetDevice(&dev), MHLO_CUDA_EXECUTION_FAILED);
+    const bool known = dev >= 0 && dev < 64;
+    if (known && done[dev].load(std::memory_order_acquire)) return MHLO_CUDA_OK;
+    MHLO_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), MHLO_CUDA_EXECUTION_FAILED);
+    if (known) done[dev].store(true, std::memory_order_release);
+    return MHLO_CUDA_OK;
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
