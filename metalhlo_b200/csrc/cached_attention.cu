@@ -89,13 +89,21 @@ __device__ __forceinline__ void mma_f16(float* d, const uint4& a, uint32_t b0, u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-// Codes as fp16, exactly: 0x64xx is 1024 + xx, so a code with its sign bit turned round behind 0x64 is 1152 + code.
-constexpr uint32_t kSignBits = 0x80808080u, kMagic = 0x64646464u;
-__device__ __forceinline__ uint32_t unbias(uint32_t x) {
-    const uint32_t bias = 0x64806480u;  // 1152, 1152
+// Codes as fp16. A code with its sign bit turned round is code + 128 in 0 .. 255: as the low byte of an fp16 number with nothing else
+// that is the subnormal (code + 128) 2^-24, which the tensor cores take as it is. The 128 comes off again from the sums: those of q
+// are known beforehand, those of the weights are one more column of the product. With 16-bit inputs that saves the subtraction of
+// every code (a quarter of all instructions); in fp32 the sums would lose too much, so there a code is put behind 0x64 (1024 + x) and
+// 1152 is taken off, which is exact.
+constexpr uint32_t kSignBits = 0x80808080u;
+template <bool EXACT>
+__device__ __forceinline__ uint32_t two_codes(uint32_t codes, uint32_t order) {
+    if (!EXACT) return __byte_perm(codes, 0, order);
+    const uint32_t x = __byte_perm(codes, 0x64646464u, order), bias = 0x64806480u;  // 1152, 1152
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&bias));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
+constexpr float kCodeUnit = 16777216.f;    // 2^24: what the sums of 16-bit inputs are short of
+constexpr uint32_t kBiasPair = 0x00800080u;  // 128 2^-24, twice
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -164,6 +172,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
     extern __shared__ __align__(128) uint8_t smem[];
     uint4* const q_frag = reinterpret_cast<uint4*>(smem + L::kRing);  // [1 or 2 parts][steps][32]
     __shared__ float row_factor[kRows];                               // scale log2(e) 2^exponent of the row's q
+    __shared__ float row_bias[kRows];                                 // -128 2^-24 times the sum of the row's q as fp16
     __shared__ float sm[W][kRows], sl[W][kRows], sf[W][kRows], sv[W], top_m[kRows], top_l[kRows];
     __shared__ int32_t used[W];
     __shared__ float4 meta[W][L::kStages];  // scales of a tile's halves: keys 0, 1 (-infinity: not there), values 0, 1
@@ -262,19 +271,29 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
         const float to_log2 = p.scale * 1.4426950408889634f;
         for (int r = warp; r < kRows; r += W) {
             const int32_t row = row0 + r;
-            float most = 0.f;
-            if (!std::is_same<T, __half>::value) {
-                if (r < rows) {
-                    const T* q = p.q + (w.s.first + row / p.group) * p.qs[0] + (head * p.group + row % p.group) * p.qs[1];
-                    for (int d = lane; d < D; d += 32) most = fmaxf(most, fabsf(VecTraits<T>::to_float(q[d])));
-                }
-                most = warp_reduce<MaxOp>(most);
+            float most = 0.f, x[D / 32];
+            const T* q = p.q + (w.s.first + row / p.group) * p.qs[0] + (head * p.group + row % p.group) * p.qs[1];
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                x[i] = r < rows ? VecTraits<T>::to_float(q[lane + 32 * i]) : 0.f;
+                most = fmaxf(most, fabsf(x[i]));
             }
             int shift = 0;
-            if (most > 0.f && most < INFINITY) shift = max(-120, ilogbf(most) - 13);
+            if (!std::is_same<T, __half>::value) {
+                most = warp_reduce<MaxOp>(most);
+                if (most > 0.f && most < INFINITY) shift = max(-120, ilogbf(most) - 13);
+            }
+            const float unit = scalbnf(1.f, -shift);
+            float sum = 0.f;
+            if (!kTwoParts) {
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) sum += __half2float(__float2half_rn(x[i] * unit));
+                sum = warp_reduce<SumOp>(sum);
+            }
             if (lane == 0) {
-                row_factor[r] = scalbnf(to_log2, shift);
-                sf[0][r] = scalbnf(1.f, -shift);
+                row_factor[r] = scalbnf(to_log2, shift) * (kTwoParts ? 1.f : kCodeUnit);
+                row_bias[r] = sum * (-128.f / kCodeUnit);
+                sf[0][r] = unit;
             }
         }
         __syncthreads();
@@ -306,10 +325,10 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
         __syncthreads();
 
         // -- this warp's tiles: t0 + warp, t0 + warp + W, ...
-        float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, v_most = 0.f;
+        float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, v_most = 0.f, o_bias[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-        const float factor[2] = {row_factor[g], row_factor[g + 8]};
+        const float factor[2] = {row_factor[g], row_factor[g + 8]}, bias[2] = {row_bias[g], row_bias[g + 8]};
         const int32_t mine = last > t0 + warp ? (last - t0 - warp + W - 1) / W : 0;
         const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * L::kStages * 2 * L::kTileBytes;
         // Pages and scales of 16 tiles at a time, a half tile per lane.
@@ -353,7 +372,10 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
             // S = q c^T: four groups of eight keys
             float s[4][4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+            for (int n = 0; n < 4; ++n) {
+                s[n][0] = s[n][1] = kTwoParts ? 0.f : bias[0];
+                s[n][2] = s[n][3] = kTwoParts ? 0.f : bias[1];
+            }
 #pragma unroll
             for (int part = 0; part < L::kParts; ++part) {
                 const int width = L::width(part), step0 = L::first(part) / 16;
@@ -383,41 +405,44 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
                         const uint4 qa = q_frag[step * 32 + lane];
 #pragma unroll
                         for (int n = 0; n < 4; ++n) {
-                            const uint32_t b0 = unbias(__byte_perm(codes[n][i4], kMagic, 0x4140)), b1 = unbias(__byte_perm(codes[n][i4], kMagic, 0x4342));
+                            const uint32_t b0 = two_codes<kTwoParts>(codes[n][i4], 0x4140), b1 = two_codes<kTwoParts>(codes[n][i4], 0x4342);
                             mma_f16(s[n], qa, b0, b1);
                             if (kTwoParts) mma_f16(s[n], q_frag[L::kSteps * 32 + step * 32 + lane], b0, b1);
                         }
                     }
                 }
             }
-            // scores in units of log2(e), masked
+            // Scores in units of log2(e) are s f. Tiles that every row sees whole keep them so; others are brought to f = 1 and masked.
             const int32_t key0 = (t0 + warp + i * W) * kTileKeys;
-            const float k_scale[2] = {scales.x, scales.y};
-            float top[2] = {m[0], m[1]};
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[n][e] *= factor[e >> 1] * k_scale[n >> 1];
+            const float v_scale[2] = {half_there[0] ? scales.z : 0.f, half_there[1] ? scales.w : 0.f};
+            float f[2][2] = {{factor[0] * scales.x, factor[1] * scales.x}, {factor[0] * scales.y, factor[1] * scales.y}};  // [half][row]
             const bool edge = key0 + kTileKeys > least || !half_there[0] || !half_there[1];
             if (edge) {
                 const int32_t seen[2] = {seen_by(g), seen_by(g + 8)};
 #pragma unroll
                 for (int n = 0; n < 4; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (!half_there[n >> 1] || key0 + n * 8 + 2 * c + (e & 1) >= seen[e >> 1]) s[n][e] = -INFINITY;
+                    for (int e = 0; e < 4; ++e) {
+                        const bool hidden = !half_there[n >> 1] || key0 + n * 8 + 2 * c + (e & 1) >= seen[e >> 1];
+                        s[n][e] = hidden ? -INFINITY : s[n][e] * f[n >> 1][e >> 1];
+                    }
+                f[0][0] = f[0][1] = f[1][0] = f[1][1] = 1.f;
             }
+            float top[2] = {m[0], m[1]};
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+                for (int r = 0; r < 2; ++r) {
+                    const float* const x = &s[half * 2][2 * r];
+                    const float* const y = &s[half * 2 + 1][2 * r];
+                    top[r] = fmaxf(top[r], fmaxf(fmaxf(x[0], x[1]), fmaxf(y[0], y[1])) * f[half][r]);
+                }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
                 top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
             }
             // the largest value scale so far is the unit of the output
-            const float v_scale[2] = {half_there[0] ? scales.z : 0.f, half_there[1] ? scales.w : 0.f};
             const float v_top = fmaxf(v_most, fmaxf(v_scale[0], v_scale[1]));
             if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1] || v_top > v_most)) {
                 const float unit = v_top > v_most ? v_most / v_top : 1.f;
@@ -433,24 +458,45 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
                 for (int j = 0; j < D / 8; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[j][e] *= keep[e >> 1];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o_bias[e] *= keep[e >> 1];
                 v_most = v_top;
             }
             const float shift[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
             const float ratio[2] = {v_scale[0] == 0.f ? 0.f : kWeightUnit * (v_scale[0] / v_most), v_scale[1] == 0.f ? 0.f : kWeightUnit * (v_scale[1] / v_most)};
-            // weights: fragments of P, keys 2 c, 2 c + 1 and 8 + 2 c, 9 + 2 c of each half
+            // Weights as fragments of P (keys 2 c, 2 c + 1 and 8 + 2 c, 9 + 2 c of each half), times the ratio of the value scales. Where
+            // that is an ordinary number it goes into the exponent, and the sum takes it out again once per half.
+            const bool plain = !kTwoParts && !edge && ratio[0] > 1e-18f && ratio[1] > 1e-18f;
             uint4 pa[2], pb[2];
+            if (plain) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                float x[2][4];
+                for (int half = 0; half < 2; ++half) {
+                    const float in_exponent = __log2f(ratio[half]), out_again = __fdividef(1.f, ratio[half]);
+                    float sum[2] = {0.f, 0.f};
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float& x = s[half * 2 + n][e];
+                            x = ex2(fmaf(x, f[half][e >> 1], in_exponent - shift[e >> 1]));
+                            sum[e >> 1] += x;
+                        }
+                    l[0] = fmaf(sum[0], out_again, l[0]);
+                    l[1] = fmaf(sum[1], out_again, l[1]);
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float z = s[half * 2 + n][e], weight = ex2(z - shift[e >> 1]);
+                        const float z = s[n][e], weight = ex2(fmaf(z, f[n >> 1][e >> 1], -shift[e >> 1]));
                         l[e >> 1] += weight;
-                        x[n][e] = weight * ratio[half];
-                        if (edge && z == -INFINITY) x[n][e] = 0.f;  // whatever the scale of a block that the row does not see
+                        s[n][e] = edge && z == -INFINITY ? 0.f : weight * ratio[n >> 1];  // 0 whatever the scale of a block that the row does not see
                     }
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float(*x)[4] = &s[half * 2];
                 pa[half] = make_uint4(pack_half2(x[0][0], x[0][1]), pack_half2(x[0][2], x[0][3]), pack_half2(x[1][0], x[1][1]), pack_half2(x[1][2], x[1][3]));
                 if (kTwoParts) {
 #pragma unroll
@@ -458,6 +504,8 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
 #pragma unroll
                         for (int e = 0; e < 4; ++e) x[n][e] -= __half2float(__float2half_rn(x[n][e]));
                     pb[half] = make_uint4(pack_half2(x[0][0], x[0][1]), pack_half2(x[0][2], x[0][3]), pack_half2(x[1][0], x[1][1]), pack_half2(x[1][2], x[1][3]));
+                } else {
+                    mma_f16(o_bias, pa[half], kBiasPair, kBiasPair);
                 }
             }
             // O += P c: group g of lanes holds W / 8 neighbouring elements of a part, one per product
@@ -494,7 +542,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
 #pragma unroll
                             for (int byte = 0; byte < 2; ++byte) {
                                 const uint32_t order = byte ? 0x4342 : 0x4140;
-                                const uint32_t b0 = unbias(__byte_perm(even, kMagic, order)), b1 = unbias(__byte_perm(odd, kMagic, order));
+                                const uint32_t b0 = two_codes<kTwoParts>(even, order), b1 = two_codes<kTwoParts>(odd, order);
                                 float* const acc = o[j0 + word * 4 + pair * 2 + byte];
                                 mma_f16(acc, pa[half], b0, b1);
                                 if (kTwoParts) mma_f16(acc, pb[half], b0, b1);
@@ -536,7 +584,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
 #pragma unroll
                         for (int k = 0; k < each; k += 4) {
                             const int d = L::first(part) + (2 * c + col) * each + k, e = half * 2 + col;
-                            joined[joined_at(warp, g + 8 * half, d >> 2)] = make_float4(o[j0 + k][e], o[j0 + k + 1][e], o[j0 + k + 2][e], o[j0 + k + 3][e]);
+                            joined[joined_at(warp, g + 8 * half, d >> 2)] = make_float4(o[j0 + k][e] - o_bias[e], o[j0 + k + 1][e] - o_bias[e], o[j0 + k + 2][e] - o_bias[e], o[j0 + k + 3][e] - o_bias[e]);
                         }
             }
         }
@@ -548,7 +596,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
             for (int i = 0; i < W; ++i) {
                 const float f = ex2(sm[i][tid] - shift);
                 sum += sl[i][tid] * f;
-                sf[i][tid] = f * sv[i] * (1.f / kWeightUnit);
+                sf[i][tid] = f * sv[i] * ((kTwoParts ? 1.f : kCodeUnit) / kWeightUnit);
             }
             top_m[tid] = most;
             top_l[tid] = sum;

@@ -82,9 +82,9 @@ class Cache:
         return x.transpose(0, 2, 1, 3).reshape(pages * self.page, *x.shape[1:2], x.shape[3])[:length], np.repeat(good, self.page)[:length]
 
 
-def attention(cache, q, table, lengths, starts, scale, out):
+def attention(cache, q, table, lengths, starts, scale, out, bias=0):
     """q fp64 [tokens, q_heads, dim]. Returns (o, lse, magnitude = sum p |v|, largest sum of |q k| a row meets, keys seen times the
-    largest value a code of theirs can stand for); rows of no sequence keep ``out``."""
+    largest value a code of theirs can stand for); rows of no sequence keep ``out``. ``bias``: what the sums carry with every code."""
     o, lse = out.copy(), np.full(q.shape[:2], np.nan)
     magnitude, products, reach = np.zeros(q.shape), np.zeros(q.shape[:2]), np.zeros(q.shape[:2])
     group = q.shape[1] // cache.codes[0].shape[1]
@@ -109,7 +109,7 @@ def attention(cache, q, table, lengths, starts, scale, out):
                 o[first + i, h] = w @ vv / w.sum()
                 lse[first + i, h] = m + np.log(w.sum())
                 magnitude[first + i, h] = w @ np.abs(vv) / w.sum()
-                products[first + i, h] = (np.abs(kk) @ np.abs(row)).max()
                 on = table[b, np.flatnonzero(seen) // cache.page]
+                products[first + i, h] = ((np.abs(kk) + bias * cache.scales[0][on, h // group][:, None]) @ np.abs(row)).max()
                 reach[first + i, h] = seen.sum() * 127 * cache.scales[1][on, h // group].max()
     return o, lse, magnitude, products, reach

@@ -9,6 +9,10 @@ weight. That error is twice a score's absolute error (numerator and denominator)
 are held in fp16 (16-bit types), 2^-20 for exponential, sums and the two-part weights of fp32. A score is a sum of head_dim products in
 steps of 16, each step off by 2^-22 of the sum of magnitudes at most (the tensor cores cut their sums off). Weights far below the
 largest one vanish: in fp16 times 2^14 the last step is 2^-24, so each key may lose 2^-39 of the largest weight times the largest value.
+
+With 16-bit inputs the sums carry 128 with every code (code + 128 is what is multiplied) and lose it at the end. So a score's sum of
+magnitudes is that of |q| (|k| + 128 scale); and in an output each step of 16 keys is off by 2^-23 of a sum of up to 128 times the
+weights (which add up to 1) times the largest scale: n / 16 steps make n * 128 * 2^-27 scale, that is 2^-27 of (n * 127 * scale), whatever |v|.
 """
 import math
 
@@ -206,11 +210,13 @@ def test_read(dtype, page, dim):
 
 def check_attention(cache, want, q, table, lengths, starts, scale, got, lse, before):
     dtype = q.dtype
-    o, want_lse, magnitude, products, reach = ref.attention(want, q.double().cpu().numpy(), table, lengths, starts, scale, before)
+    o, want_lse, magnitude, products, reach = ref.attention(want, q.double().cpu().numpy(), table, lengths, starts, scale, before,
+                                                              bias=0 if dtype == torch.float32 else 128)
     dim = q.shape[2]
     score = (dim / 16) * 2.0 ** -22 * scale * products
     weight = 2 * score + (2.0 ** -20 if dtype == torch.float32 else 2.0 ** -11 + 2.0 ** -20)
-    bound = HALF_STEP[dtype] * np.abs(o) + weight[:, :, None] * magnitude + 2.0 ** -39 * reach[:, :, None] + HALF_SUBNORMAL[dtype]
+    lost = 2.0 ** -39 if dtype == torch.float32 else 2.0 ** -39 + 2.0 ** -27 * (128 / 127)
+    bound = HALF_STEP[dtype] * np.abs(o) + weight[:, :, None] * magnitude + lost * reach[:, :, None] + HALF_SUBNORMAL[dtype]
     got = got.double().cpu().numpy()
     assert np.isfinite(got).all()
     worst = np.max((np.abs(got - o) - bound) / (magnitude + 1e-30))
