@@ -1,12 +1,16 @@
 // Attention of new tokens over the paged 8-bit key/value cache: o = softmax(scale q k^T) v with k = ks c, v = vs c.
 //
-// The work is cut into segments: (sequence, 16 rows, cache head). The rows of a segment are (token, query head) pairs that read the
+// The work is cut into segments: (sequence, 8 or 16 rows, cache head). The rows of a segment are (token, query head) pairs that read the
 // same cache head: row r of a sequence is token r / group, query head head * group + r % group. A segment's keys are walked in tiles
 // of 32; CTAs share all tiles of the call evenly (Plan), so a CTA's piece may begin or end inside a segment. Whole segments are
 // written at once, pieces go to scratch as (maximum, sum, output) and a second kernel joins them in the order of the CTAs.
 //
-// Inside a CTA every warp takes tiles by itself and keeps a running maximum, sum and output of its 16 rows; the warps are joined
+// Inside a CTA every warp takes tiles by itself and keeps a running maximum, sum and output of the rows; the warps are joined
 // through shared memory at the end of a segment. Nothing but the segment's end synchronises the warps.
+//
+// The products are transposed, S^T = C q^T and O^T = C^T P^T (16 x 8 x 16 steps): keys and elements of values take the long side of
+// the instruction, rows the short one. A decoding step has as many rows as query heads share a cache head, mostly 4 to 8, and would
+// fill 16 to a half or less: half the products, exponentials and output registers.
 #include <algorithm>
 #include <type_traits>
 
@@ -16,7 +20,6 @@ namespace mhlo {
 namespace {
 
 constexpr int kTileKeys = 32;
-constexpr int kRows = 16;
 constexpr int kLeastTiles = 12;  // a CTA's share where there is little to do: a tile per warp
 constexpr int kGrid = kNumSMs;   // one CTA per SM: the rings of its warps take the shared memory
 
@@ -46,7 +49,7 @@ struct CachedParams {
     int32_t whole;      // no segment has more than kLeastTiles tiles: none is cut
     int32_t o_vec;      // four results at a time
     int32_t* pieces;    // [kGrid][8]: the cut segment that a CTA's share ends with (Piece), count 0 if none
-    float* partial;     // [kGrid][2][kRows (D + 2)]
+    float* partial;     // [kGrid][2][rows (D + 2)]
 };
 
 struct Piece {  // what joining a cut segment needs
@@ -57,10 +60,10 @@ struct Piece {  // what joining a cut segment needs
 
 struct Share {  // of one sequence
     KvSequence s;
-    int32_t row_tiles, tiles;  // of 16 rows; of 32 keys (1 where there are none: somebody has to write the zeros)
+    int32_t row_tiles, tiles;  // of 8 or 16 rows; of 32 keys (1 where there are none: somebody has to write the zeros)
 };
 
-template <typename T>
+template <int kRows, typename T>
 __device__ __forceinline__ Share share_of(const CachedParams<T>& p, int32_t b) {
     Share w;
     w.s = kv_sequence(p.kv, b);
@@ -79,15 +82,25 @@ __device__ __forceinline__ int64_t warp_sum(int64_t v) {
 
 // ---- the kernel's parts ----------------------------------------------------------------------------------------------------
 
+__device__ __forceinline__ float fmax3(float a, float b, float c) {  // one instruction on sm_100
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void mma_f16(float* d, const uint4& a, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+}
+__device__ __forceinline__ uint32_t turned(uint32_t x) {  // the transpose of an 8 x 8 matrix of 16-bit elements, two a lane
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 // Codes as fp16. A code with its sign bit turned round is code + 128 in 0 .. 255: as the low byte of an fp16 number with nothing else
 // that is the subnormal (code + 128) 2^-24, which the tensor cores take as it is. The 128 comes off again from the sums: those of q
@@ -125,17 +138,16 @@ __device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
     return row * 32 + (chunk << 4);
 }
 
-// Starts the copies of one tile's keys and values: halves of 16 keys, each contiguous in a page. base[h] = first code of half h, -1: not there.
+// Starts the copies of 16 keys and values (half a tile, contiguous in a page): `from` their offset in the codes. The lane's part of
+// every address is the same for each pass of the loop but for the exclusive or, so it costs no more than that.
 template <int D>
-__device__ __forceinline__ void load_tile(const KvArgs& a, uint32_t keys, int64_t base0, int64_t base1) {
+__device__ __forceinline__ void load_half(const int8_t* k, const int8_t* v, uint32_t keys, int half) {
     using L = Layout<D>;
     const int lane = threadIdx.x & 31;
     constexpr int kChunks = D / 16;  // of a row
 #pragma unroll
-    for (int i = 0; i < kTileKeys * kChunks / 32; ++i) {
-        const int index = i * 32 + lane, row = index / kChunks, chunk = index % kChunks;
-        const int64_t base = row < 16 ? base0 : base1;
-        const int64_t at = base + (row & 15) * D + chunk * 16;
+    for (int i = 0; i < 16 * kChunks / 32; ++i) {
+        const int index = i * 32 + lane, row = half * 16 + index / kChunks, chunk = index % kChunks;
         const int part = L::kParts == 1 ? 0 : chunk * 16 >= L::first(1);
         const int c = part == 0 ? chunk : chunk - L::first(1) / 16;
         uint32_t ko, vo;
@@ -146,12 +158,9 @@ __device__ __forceinline__ void load_tile(const KvArgs& a, uint32_t keys, int64_
             ko = kTileKeys * L::width(0) + chunk_at<L::width(1), false>(row, c);
             vo = kTileKeys * L::width(0) + chunk_at<L::width(1), true>(row, c);
         }
-        if (base >= 0) {
-            cp_async16(keys + ko, a.k_codes + at);
-            cp_async16(keys + L::kTileBytes + vo, a.v_codes + at);
-        }
+        cp_async16(keys + ko, k + i * 512);
+        cp_async16(keys + L::kTileBytes + vo, v + i * 512);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
 // Fragment order of a row's elements. A step of 16 products uses, from lane c of four, four neighbouring elements: in a 64-byte
@@ -162,15 +171,24 @@ __device__ __forceinline__ int step_element(int step, int c) {
     return 64 * (step >> 2) + 16 * c + 4 * (step & 3);
 }
 
-constexpr float kWeightUnit = 16384.f;  // fp16 weights are held times 2^14: the largest is 2^14, the smallest step 2^-24
+// fp16 weights are held times a power of two, so that those far below the largest keep some bits above the smallest step, 2^-24. In
+// fp32 the largest weight is 2^14; with 16-bit inputs 2^6, and scores may exceed the maximum that was seen last by 2^8 before
+// everything is scaled anew: with exact maxima some row of 16 found a new one in almost every tile, 10 % of all instructions.
+template <typename T>
+constexpr float kWeightUnitOf = sizeof(T) == 4 ? 16384.f : 64.f;
+template <typename T>
+constexpr float kHeadroomOf = sizeof(T) == 4 ? 0.f : 8.f;
 
-template <typename T, int D>
+// NT: groups of 8 rows.
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kernel(const __grid_constant__ CachedParams<T> p) {
     using L = Layout<D>;
+    constexpr int kRows = 8 * NT;
     constexpr bool kTwoParts = sizeof(T) == 4;  // fp32: q and the weights as sums of two fp16 numbers
+    constexpr float kWeightUnit = kWeightUnitOf<T>, kHeadroom = kHeadroomOf<T>;
     constexpr int W = L::kWarps;
     extern __shared__ __align__(128) uint8_t smem[];
-    uint4* const q_frag = reinterpret_cast<uint4*>(smem + L::kRing);  // [1 or 2 parts][steps][32]
+    uint2* const q_frag = reinterpret_cast<uint2*>(smem + L::kRing);  // [1 or 2 parts][steps][NT][32]
     __shared__ float row_factor[kRows];                               // scale log2(e) 2^exponent of the row's q
     __shared__ float row_bias[kRows];                                 // -128 2^-24 times the sum of the row's q as fp16
     __shared__ float sm[W][kRows], sl[W][kRows], sf[W][kRows], sv[W], top_m[kRows], top_l[kRows];
@@ -186,7 +204,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
     {
         int64_t all = 0, all_padded = 0;
         for (int32_t b = tid; b < a.seqs; b += L::kThreads) {
-            const Share w = share_of(p, b);
+            const Share w = share_of<kRows>(p, b);
             const int64_t segments = static_cast<int64_t>(w.row_tiles) * a.heads;
             all += segments * w.tiles;
             all_padded += segments * padded(w.tiles);
@@ -218,7 +236,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
         for (int32_t base = 0; base < a.seqs; base += L::kThreads) {
             int64_t mine = 0;
             if (base + tid < a.seqs) {
-                const Share w = share_of(p, base + tid);
+                const Share w = share_of<kRows>(p, base + tid);
                 mine = static_cast<int64_t>(w.row_tiles) * a.heads * (pad ? padded(w.tiles) : w.tiles);
             }
             int64_t sum = mine;
@@ -246,7 +264,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
     }
     int32_t b = static_cast<int32_t>(found[0]);
     if (b < 0) return;  // cannot be: lengths that change under the kernel
-    Share w = share_of(p, b);
+    Share w = share_of<kRows>(p, b);
     int64_t inside = found[1];
 
     while (at < end) {
@@ -254,7 +272,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
         const int64_t segments = static_cast<int64_t>(w.row_tiles) * a.heads;
         if (inside >= segments * tiles) {  // on to the next sequence that has work
             if (++b >= a.seqs) return;
-            w = share_of(p, b);
+            w = share_of<kRows>(p, b);
             inside = 0;
             continue;
         }
@@ -297,41 +315,51 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
             }
         }
         __syncthreads();
-        for (int i = tid; i < L::kSteps * 32; i += L::kThreads) {
-            const int step = i >> 5, l = i & 31;
-            uint32_t hi[4], lo[4];
+        for (int i = tid; i < L::kSteps * NT * 32; i += L::kThreads) {
+            const int l = i & 31, j = (i >> 5) % NT, step = (i >> 5) / NT, r = 8 * j + (l >> 2);
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            if (r < rows) {
+                const int32_t row = row0 + r;
+                const T* q = p.q + (w.s.first + row / p.group) * p.qs[0] + (head * p.group + row % p.group) * p.qs[1] + step_element<D>(step, l & 3);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {  // rows g and g + 8
-                const int r = (l >> 2) + 8 * half;
-                float x[4] = {0.f, 0.f, 0.f, 0.f};
-                if (r < rows) {
-                    const int32_t row = row0 + r;
-                    const T* q = p.q + (w.s.first + row / p.group) * p.qs[0] + (head * p.group + row % p.group) * p.qs[1] + step_element<D>(step, l & 3);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = VecTraits<T>::to_float(q[e]) * sf[0][r];
-                }
-                hi[half] = pack_half2(x[0], x[1]);
-                hi[2 + half] = pack_half2(x[2], x[3]);
-                if (kTwoParts) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] -= __half2float(__float2half_rn(x[e]));
-                    lo[half] = pack_half2(x[0], x[1]);
-                    lo[2 + half] = pack_half2(x[2], x[3]);
-                }
+                for (int e = 0; e < 4; ++e) x[e] = VecTraits<T>::to_float(q[e]) * sf[0][r];
             }
-            q_frag[i] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            if (kTwoParts) q_frag[L::kSteps * 32 + i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            q_frag[i] = make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
+            if (kTwoParts) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] -= __half2float(__float2half_rn(x[e]));
+                q_frag[L::kSteps * NT * 32 + i] = make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
+            }
         }
         __syncthreads();
 
         // -- this warp's tiles: t0 + warp, t0 + warp + W, ...
-        float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, v_most = 0.f, o_bias[4] = {0.f, 0.f, 0.f, 0.f};
+        // Lane (g, c) has rows 8 j + 2 c + i of keys g and g + 8 of a half, and of elements W / 8 g .. of each part of the values.
+        float o[D / 16][NT][4], m[NT][2], l[NT][2], v_most = 0.f, o_bias[NT][4], factor[NT][2], bias[NT][2];
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-        const float factor[2] = {row_factor[g], row_factor[g + 8]}, bias[2] = {row_bias[g], row_bias[g + 8]};
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t) o[t][j][e] = 0.f;
+                o_bias[j][e] = 0.f;
+                if (e < 2) {
+                    m[j][e] = -INFINITY;
+                    l[j][e] = 0.f;
+                    factor[j][e] = row_factor[8 * j + 2 * c + e];
+                    bias[j][e] = row_bias[8 * j + 2 * c + e];
+                }
+            }
+        constexpr bool kKeepQ = NT == 1 && !kTwoParts && D <= 128;  // in registers
+        uint2 q_kept[kKeepQ ? L::kSteps : 1];
+        if (kKeepQ) {
+#pragma unroll
+            for (int i = 0; i < L::kSteps; ++i) q_kept[i] = q_frag[i * 32 + lane];
+        }
         const int32_t mine = last > t0 + warp ? (last - t0 - warp + W - 1) / W : 0;
         const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * L::kStages * 2 * L::kTileBytes;
         // Pages and scales of 16 tiles at a time, a half tile per lane.
+        const int8_t *const k_lane = a.k_codes + lane * 16, *const v_lane = a.v_codes + lane * 16;
         int64_t base = -1;
         float ks = 0.f, vs = 0.f;
         auto issue = [&](int32_t i) {
@@ -351,7 +379,9 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
                 }
                 const int from = (i & 15) * 2, stage = i % L::kStages;
                 const int64_t base0 = __shfl_sync(0xffffffffu, base, from), base1 = __shfl_sync(0xffffffffu, base, from + 1);
-                load_tile<D>(a, ring + stage * 2 * L::kTileBytes, base0, base1);
+                if (base0 >= 0) load_half<D>(k_lane + base0, v_lane + base0, ring + stage * 2 * L::kTileBytes, 0);
+                if (base1 >= 0) load_half<D>(k_lane + base1, v_lane + base1, ring + stage * 2 * L::kTileBytes, 1);
+                asm volatile("cp.async.commit_group;" ::: "memory");
                 const float k1 = __shfl_down_sync(0xffffffffu, ks, 1), v1 = __shfl_down_sync(0xffffffffu, vs, 1);
                 if (lane == from) meta[warp][stage] = make_float4(base0 < 0 ? -INFINITY : ks, base1 < 0 ? -INFINITY : k1, vs, v1);
             } else {
@@ -369,13 +399,14 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
             const float4 scales = meta[warp][stage];
             const bool half_there[2] = {scales.x != -INFINITY, scales.y != -INFINITY};
 
-            // S = q c^T: four groups of eight keys
-            float s[4][4];
+            // S^T = C q^T, 16 keys a step
+            float s[2][NT][4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                s[n][0] = s[n][1] = kTwoParts ? 0.f : bias[0];
-                s[n][2] = s[n][3] = kTwoParts ? 0.f : bias[1];
-            }
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[half][j][e] = kTwoParts ? 0.f : bias[j][e & 1];
 #pragma unroll
             for (int part = 0; part < L::kParts; ++part) {
                 const int width = L::width(part), step0 = L::first(part) / 16;
@@ -402,12 +433,16 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
 #pragma unroll
                     for (int i4 = 0; i4 < (width == 32 ? 2 : 4); ++i4) {
                         const int step = step0 + chunk * 4 + i4;
-                        const uint4 qa = q_frag[step * 32 + lane];
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            const uint32_t b0 = two_codes<kTwoParts>(codes[n][i4], 0x4140), b1 = two_codes<kTwoParts>(codes[n][i4], 0x4342);
-                            mma_f16(s[n], qa, b0, b1);
-                            if (kTwoParts) mma_f16(s[n], q_frag[L::kSteps * 32 + step * 32 + lane], b0, b1);
+                        for (int half = 0; half < 2; ++half) {
+                            const uint32_t a0 = two_codes<kTwoParts>(codes[2 * half][i4], 0x4140), a1 = two_codes<kTwoParts>(codes[2 * half + 1][i4], 0x4140);
+                            const uint32_t a2 = two_codes<kTwoParts>(codes[2 * half][i4], 0x4342), a3 = two_codes<kTwoParts>(codes[2 * half + 1][i4], 0x4342);
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) {
+                                const uint2 qb = kKeepQ ? q_kept[kKeepQ ? step : 0] : q_frag[(step * NT + j) * 32 + lane];
+                                mma_f16(s[half][j], a0, a1, a2, a3, qb);
+                                if (kTwoParts) mma_f16(s[half][j], a0, a1, a2, a3, q_frag[((L::kSteps + step) * NT + j) * 32 + lane]);
+                            }
                         }
                     }
                 }
@@ -415,105 +450,121 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
             // Scores in units of log2(e) are s f. Tiles that every row sees whole keep them so; others are brought to f = 1 and masked.
             const int32_t key0 = (t0 + warp + i * W) * kTileKeys;
             const float v_scale[2] = {half_there[0] ? scales.z : 0.f, half_there[1] ? scales.w : 0.f};
-            float f[2][2] = {{factor[0] * scales.x, factor[1] * scales.x}, {factor[0] * scales.y, factor[1] * scales.y}};  // [half][row]
             const bool edge = key0 + kTileKeys > least || !half_there[0] || !half_there[1];
-            if (edge) {
-                const int32_t seen[2] = {seen_by(g), seen_by(g + 8)};
+            float f[2][NT][2];
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    f[0][j][r] = factor[j][r] * scales.x;
+                    f[1][j][r] = factor[j][r] * scales.y;
+                }
+            if (edge) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const int32_t seen[2] = {seen_by(8 * j + 2 * c), seen_by(8 * j + 2 * c + 1)};
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool hidden = !half_there[half] || key0 + half * 16 + (e >> 1) * 8 + g >= seen[e & 1];
+                            s[half][j][e] = hidden ? -INFINITY : s[half][j][e] * f[half][j][e & 1];
+                        }
+                        f[half][j][0] = f[half][j][1] = 1.f;
+                    }
+                }
+            }
+            // The maxima that exponents are taken against, and the largest value scale so far, the unit of the output, move only when a
+            // score leaves the headroom of the weights: every lane looks at its own scores, and lanes talk only when they have to.
+            float top[NT][2];
+            const float v_top = fmax3(v_most, v_scale[0], v_scale[1]);
+            bool move = v_top > v_most;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    top[j][r] = fmaxf(fmaxf(s[0][j][r], s[0][j][2 + r]) * f[0][j][r], fmaxf(s[1][j][r], s[1][j][2 + r]) * f[1][j][r]);
+                    move = move || top[j][r] > m[j][r] + kHeadroom;
+                }
+            if (__any_sync(0xffffffffu, move)) {
+                const float unit = v_top > v_most ? v_most / v_top : 1.f;
+                v_most = v_top;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    float keep[2];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                        for (int x = 4; x < 32; x <<= 1) top[j][r] = fmaxf(top[j][r], __shfl_xor_sync(0xffffffffu, top[j][r], x));
+                        keep[r] = top[j][r] > m[j][r] ? ex2(m[j][r] - top[j][r]) : 1.f;
+                        l[j][r] *= keep[r];
+                        keep[r] *= unit;
+                        m[j][r] = fmaxf(m[j][r], top[j][r]);
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const bool hidden = !half_there[n >> 1] || key0 + n * 8 + 2 * c + (e & 1) >= seen[e >> 1];
-                        s[n][e] = hidden ? -INFINITY : s[n][e] * f[n >> 1][e >> 1];
+#pragma unroll
+                        for (int t = 0; t < D / 16; ++t) o[t][j][e] *= keep[e & 1];
+                        o_bias[j][e] *= keep[e & 1];
                     }
-                f[0][0] = f[0][1] = f[1][0] = f[1][1] = 1.f;
-            }
-            float top[2] = {m[0], m[1]};
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float* const x = &s[half * 2][2 * r];
-                    const float* const y = &s[half * 2 + 1][2 * r];
-                    top[r] = fmaxf(top[r], fmaxf(fmaxf(x[0], x[1]), fmaxf(y[0], y[1])) * f[half][r]);
                 }
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
             }
-            // the largest value scale so far is the unit of the output
-            const float v_top = fmaxf(v_most, fmaxf(v_scale[0], v_scale[1]));
-            if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1] || v_top > v_most)) {
-                const float unit = v_top > v_most ? v_most / v_top : 1.f;
-                float keep[2];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    keep[r] = top[r] > m[r] ? ex2(m[r] - top[r]) : 1.f;
-                    l[r] *= keep[r];
-                    keep[r] *= unit;
-                    m[r] = top[r];
-                }
-#pragma unroll
-                for (int j = 0; j < D / 8; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[j][e] *= keep[e >> 1];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o_bias[e] *= keep[e >> 1];
-                v_most = v_top;
-            }
-            const float shift[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
             const float ratio[2] = {v_scale[0] == 0.f ? 0.f : kWeightUnit * (v_scale[0] / v_most), v_scale[1] == 0.f ? 0.f : kWeightUnit * (v_scale[1] / v_most)};
-            // Weights as fragments of P (keys 2 c, 2 c + 1 and 8 + 2 c, 9 + 2 c of each half), times the ratio of the value scales. Where
-            // that is an ordinary number it goes into the exponent, and the sum takes it out again once per half.
+            // Weights times the ratio of the value scales. Where that is an ordinary number it goes into the exponent, and the sum takes it
+            // out again once per half.
             const bool plain = !kTwoParts && !edge && ratio[0] > 1e-18f && ratio[1] > 1e-18f;
-            uint4 pa[2], pb[2];
             if (plain) {
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const float in_exponent = __log2f(ratio[half]), out_again = __fdividef(1.f, ratio[half]);
-                    float sum[2] = {0.f, 0.f};
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int j = 0; j < NT; ++j) {
+                        float sum[2] = {0.f, 0.f};
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            float& x = s[half * 2 + n][e];
-                            x = ex2(fmaf(x, f[half][e >> 1], in_exponent - shift[e >> 1]));
-                            sum[e >> 1] += x;
+                            float& x = s[half][j][e];
+                            x = ex2(fmaf(x, f[half][j][e & 1], in_exponent - m[j][e & 1]));
+                            sum[e & 1] += x;
                         }
-                    l[0] = fmaf(sum[0], out_again, l[0]);
-                    l[1] = fmaf(sum[1], out_again, l[1]);
+                        l[j][0] = fmaf(sum[0], out_again, l[j][0]);
+                        l[j][1] = fmaf(sum[1], out_again, l[j][1]);
+                    }
                 }
             } else {
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float z = s[n][e], weight = ex2(fmaf(z, f[n >> 1][e >> 1], -shift[e >> 1]));
-                        l[e >> 1] += weight;
-                        s[n][e] = edge && z == -INFINITY ? 0.f : weight * ratio[n >> 1];  // 0 whatever the scale of a block that the row does not see
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float z = s[half][j][e], top_so_far = m[j][e & 1];
+                            const float weight = ex2(fmaf(z, f[half][j][e & 1], top_so_far == -INFINITY ? 0.f : -top_so_far));
+                            l[j][e & 1] += weight;
+                            s[half][j][e] = edge && z == -INFINITY ? 0.f : weight * ratio[half];  // 0 whatever the scale of a block that the row does not see
+                        }
+            }
+            // P^T as fragments: keys 2 c, 2 c + 1 and 8 + 2 c, 9 + 2 c of row g
+            uint2 pa[2][NT], pb[2][NT];
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    float* const x = s[half][j];
+                    pa[half][j] = make_uint2(turned(pack_half2(x[0], x[1])), turned(pack_half2(x[2], x[3])));
+                    if (kTwoParts) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] -= __half2float(__float2half_rn(x[e]));
+                        pb[half][j] = make_uint2(turned(pack_half2(x[0], x[1])), turned(pack_half2(x[2], x[3])));
+                    } else {
+                        mma_f16(o_bias[j], kBiasPair, kBiasPair, kBiasPair, kBiasPair, pa[half][j]);
                     }
-            }
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                float(*x)[4] = &s[half * 2];
-                pa[half] = make_uint4(pack_half2(x[0][0], x[0][1]), pack_half2(x[0][2], x[0][3]), pack_half2(x[1][0], x[1][1]), pack_half2(x[1][2], x[1][3]));
-                if (kTwoParts) {
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[n][e] -= __half2float(__float2half_rn(x[n][e]));
-                    pb[half] = make_uint4(pack_half2(x[0][0], x[0][1]), pack_half2(x[0][2], x[0][3]), pack_half2(x[1][0], x[1][1]), pack_half2(x[1][2], x[1][3]));
-                } else {
-                    mma_f16(o_bias, pa[half], kBiasPair, kBiasPair);
                 }
-            }
-            // O += P c: group g of lanes holds W / 8 neighbouring elements of a part, one per product
+            // O^T += C^T P^T: group g of lanes holds W / 8 neighbouring elements of a part, two per product
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
                 for (int part = 0; part < L::kParts; ++part) {
-                    const int width = L::width(part), words = width / 32, j0 = L::first(part) / 8;
+                    const int width = L::width(part), words = width / 32, tile0 = L::first(part) / 16;
                     const uint8_t* const base_part = values + kTileKeys * L::first(part);
                     uint32_t rows4[4][4];  // rows 2 c, 2 c + 1, 8 + 2 c, 9 + 2 c
 #pragma unroll
@@ -534,57 +585,61 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
                         }
                     }
 #pragma unroll
-                    for (int word = 0; word < words; ++word) {
+                    for (int word = 0; word < words; ++word)
 #pragma unroll
                         for (int pair = 0; pair < 2; ++pair) {  // bytes 2 pair, 2 pair + 1
                             const uint32_t even = __byte_perm(rows4[0][word], rows4[1][word], pair ? 0x7362 : 0x5140);
                             const uint32_t odd = __byte_perm(rows4[2][word], rows4[3][word], pair ? 0x7362 : 0x5140);
+                            const uint32_t a0 = two_codes<kTwoParts>(even, 0x4140), a1 = two_codes<kTwoParts>(even, 0x4342);
+                            const uint32_t a2 = two_codes<kTwoParts>(odd, 0x4140), a3 = two_codes<kTwoParts>(odd, 0x4342);
 #pragma unroll
-                            for (int byte = 0; byte < 2; ++byte) {
-                                const uint32_t order = byte ? 0x4342 : 0x4140;
-                                const uint32_t b0 = two_codes<kTwoParts>(even, order), b1 = two_codes<kTwoParts>(odd, order);
-                                float* const acc = o[j0 + word * 4 + pair * 2 + byte];
-                                mma_f16(acc, pa[half], b0, b1);
-                                if (kTwoParts) mma_f16(acc, pb[half], b0, b1);
+                            for (int j = 0; j < NT; ++j) {
+                                float* const acc = o[tile0 + word * 2 + pair][j];
+                                mma_f16(acc, a0, a1, a2, a3, pa[half][j]);
+                                if (kTwoParts) mma_f16(acc, a0, a1, a2, a3, pb[half][j]);
                             }
                         }
-                    }
                 }
             __syncwarp();
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncthreads();  // every warp is done with the rings: they hold the warps' outputs now
 
-        // -- join the warps. A lane holds W / 4 neighbouring elements (from W / 4 * c) of rows g and g + 8 of each part.
+        // -- join the warps
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        }
-        if (c == 0) {
-            sm[warp][g] = m[0];
-            sm[warp][g + 8] = m[1];
-            sl[warp][g] = l[0];
-            sl[warp][g + 8] = l[1];
-        }
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[j][r] += __shfl_xor_sync(0xffffffffu, l[j][r], x);
+                if (g == 0) {
+                    sm[warp][8 * j + 2 * c + r] = m[j][r];
+                    sl[warp][8 * j + 2 * c + r] = l[j][r];
+                }
+            }
         if (lane == 0) {
             sv[warp] = v_most;
             used[warp] = mine > 0;
         }
         float4* const joined = reinterpret_cast<float4*>(smem);  // [warp][row][D / 4], chunks turned against bank conflicts
-        auto joined_at = [](int w_, int row, int d4) { return (w_ * kRows + row) * (D / 4) + (d4 ^ ((d4 >> 3) & 7) ^ ((row & 1) << 2)); };
+        auto joined_at = [](int w_, int row, int d4) {
+            const int pair = (row >> 1) & 3;
+            return (w_ * kRows + row) * (D / 4) + (d4 ^ (D == 64 ? (pair & 1) | (pair >> 1) << 2 : pair));
+        };
         if (mine > 0) {
 #pragma unroll
             for (int part = 0; part < L::kParts; ++part) {
-                const int width = L::width(part), j0 = L::first(part) / 8, each = width / 8;
+                const int each = L::width(part) / 8, tile0 = L::first(part) / 16;  // elements L::first + each g ..
 #pragma unroll
-                for (int half = 0; half < 2; ++half)
+                for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int col = 0; col < 2; ++col)
+                    for (int r = 0; r < 2; ++r)
 #pragma unroll
                         for (int k = 0; k < each; k += 4) {
-                            const int d = L::first(part) + (2 * c + col) * each + k, e = half * 2 + col;
-                            joined[joined_at(warp, g + 8 * half, d >> 2)] = make_float4(o[j0 + k][e] - o_bias[e], o[j0 + k + 1][e] - o_bias[e], o[j0 + k + 2][e] - o_bias[e], o[j0 + k + 3][e] - o_bias[e]);
+                            const float off = o_bias[j][r];
+                            const float(*x)[NT][4] = &o[tile0 + k / 2];
+                            joined[joined_at(warp, 8 * j + 2 * c + r, (L::first(part) + g * each + k) >> 2)] =
+                                make_float4(x[0][j][r] - off, x[0][j][2 + r] - off, x[1][j][r] - off, x[1][j][2 + r] - off);
                         }
             }
         }
@@ -663,7 +718,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
 }
 
 // Joins the pieces of the segment that CTA blockIdx.x began and others went on with: sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
-template <typename T, int D>
+template <typename T, int D, int kRows>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ CachedParams<T> p) {
     grid_dependency_wait();
     const int32_t* const piece = p.pieces + blockIdx.x * 8;
@@ -689,24 +744,31 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Cache
 }
 
 template <int D>
-constexpr int64_t scratch_bytes() { return kGrid * (8 * 4 + 2 * kRows * (D + 2) * 4); }
+constexpr int64_t scratch_bytes() { return kGrid * (8 * 4 + 2 * 16 * (D + 2) * 4); }
 
-template <typename T, int D>
+template <typename T, int D, int NT>
 int launch_rows(CachedParams<T> p, void* scratch, cudaStream_t stream) {
     using L = Layout<D>;
     p.pieces = static_cast<int32_t*>(scratch);
     p.partial = reinterpret_cast<float*>(p.pieces + kGrid * 8);
-    constexpr int smem = L::kRing + L::kSteps * 32 * 16 * (sizeof(T) == 4 ? 2 : 1);
-    auto kernel = cached_attention_kernel<T, D>;
+    constexpr int smem = L::kRing + L::kSteps * NT * 32 * 8 * (sizeof(T) == 4 ? 2 : 1);
+    auto kernel = cached_attention_kernel<T, D, NT>;
     static std::atomic<bool> smem_set[64];
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, smem_set)) return st;
     kernel<<<kGrid, L::kThreads, smem, stream>>>(p);
     MHLO_CUDA_CHECK_LAUNCH("cached_attention");
     if (p.whole) return MHLO_CUDA_OK;
-    const cudaError_t e = launch_dependent(join_kernel<T, D>, dim3(kGrid, kRows), dim3(128), 0, stream, 1, true, p);
+    const cudaError_t e = launch_dependent(join_kernel<T, D, 8 * NT>, dim3(kGrid, 8 * NT), dim3(128), 0, stream, 1, true, p);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of cached_attention failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("cached_attention (joining)");
     return MHLO_CUDA_OK;
+}
+
+template <typename T, int D>
+int launch_dim(const CachedParams<T>& p, void* scratch, cudaStream_t stream) {
+    // groups of 8 rows as long as the sequences have no more on average
+    if (static_cast<int64_t>(p.kv.tokens) * p.group <= 8 * static_cast<int64_t>(p.kv.seqs)) return launch_rows<T, D, 1>(p, scratch, stream);
+    return launch_rows<T, D, 2>(p, scratch, stream);
 }
 
 template <typename T>
@@ -724,10 +786,10 @@ int launch(const KvArgs& kv, const void* q, const int64_t* qs, int64_t q_heads, 
     const int64_t four = 4 * static_cast<int64_t>(sizeof(T));
     p.o_vec = reinterpret_cast<uintptr_t>(o) % four == 0 && os[0] % 4 == 0 && os[1] % 4 == 0;
     switch (kv.head_dim) {
-        case 64: return launch_rows<T, 64>(p, scratch, stream);
-        case 96: return launch_rows<T, 96>(p, scratch, stream);
-        case 128: return launch_rows<T, 128>(p, scratch, stream);
-        default: return launch_rows<T, 256>(p, scratch, stream);
+        case 64: return launch_dim<T, 64>(p, scratch, stream);
+        case 96: return launch_dim<T, 96>(p, scratch, stream);
+        case 128: return launch_dim<T, 128>(p, scratch, stream);
+        default: return launch_dim<T, 256>(p, scratch, stream);
     }
 }
 

@@ -8,7 +8,8 @@ Attention: with u = half a step of the result's type, an output is off by u |o| 
 weight. That error is twice a score's absolute error (numerator and denominator) plus the weight's own rounding: 2^-11 where weights
 are held in fp16 (16-bit types), 2^-20 for exponential, sums and the two-part weights of fp32. A score is a sum of head_dim products in
 steps of 16, each step off by 2^-22 of the sum of magnitudes at most (the tensor cores cut their sums off). Weights far below the
-largest one vanish: in fp16 times 2^14 the last step is 2^-24, so each key may lose 2^-39 of the largest weight times the largest value.
+largest one vanish: in fp16 times 2^14 (fp32 inputs) or 2^6 (others) the last step is 2^-24, so each key may lose 2^-39 or 2^-31 of the
+largest weight times the largest value.
 
 With 16-bit inputs the sums carry 128 with every code (code + 128 is what is multiplied) and lose it at the end. So a score's sum of
 magnitudes is that of |q| (|k| + 128 scale); and in an output each step of 16 keys is off by 2^-23 of a sum of up to 128 times the
@@ -215,7 +216,7 @@ def check_attention(cache, want, q, table, lengths, starts, scale, got, lse, bef
     dim = q.shape[2]
     score = (dim / 16) * 2.0 ** -22 * scale * products
     weight = 2 * score + (2.0 ** -20 if dtype == torch.float32 else 2.0 ** -11 + 2.0 ** -20)
-    lost = 2.0 ** -39 if dtype == torch.float32 else 2.0 ** -39 + 2.0 ** -27 * (128 / 127)
+    lost = 2.0 ** -39 if dtype == torch.float32 else 2.0 ** -31 + 2.0 ** -27 * (128 / 127)
     bound = HALF_STEP[dtype] * np.abs(o) + weight[:, :, None] * magnitude + lost * reach[:, :, None] + HALF_SUBNORMAL[dtype]
     got = got.double().cpu().numpy()
     assert np.isfinite(got).all()
