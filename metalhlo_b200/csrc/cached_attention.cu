@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
     const int64_t per = pad ? (totals[1] / kLeastTiles + kGrid - 1) / kGrid * kLeastTiles : (total + kGrid - 1) / kGrid;
     int64_t at = blockIdx.x * per;
     const int64_t end = min(total, at + per);
-    if (tid == 0) p.pieces[blockIdx.x * 8] = 0;
+    if (tid == 0 && !p.whole) p.pieces[blockIdx.x * 8] = 0;
     grid_dependency_release();
     if (at >= end) return;
     // the sequence that holds tile `at`, and where in it
@@ -782,7 +782,7 @@ int launch(const KvArgs& kv, const void* q, const int64_t* qs, int64_t q_heads, 
     p.q_heads = static_cast<int32_t>(q_heads);
     p.group = static_cast<int32_t>(q_heads / kv.heads);
     p.scale = scale;
-    p.whole = (static_cast<int64_t>(kv.pages_per_seq) << kv.page_shift) <= kLeastTiles * kTileKeys;
+    p.whole = scratch == nullptr;
     const int64_t four = 4 * static_cast<int64_t>(sizeof(T));
     p.o_vec = reinterpret_cast<uintptr_t>(o) % four == 0 && os[0] % 4 == 0 && os[1] % 4 == 0;
     switch (kv.head_dim) {
@@ -805,6 +805,7 @@ extern "C" {
 
 int64_t mhlo_cuda_cached_attention_scratch_bytes(const mhlo_cuda_kv_cache* cache, const mhlo_cuda_kv_batch* batch, int64_t q_heads) {
     if (!cache || !batch || q_heads < 1) return 0;
+    if (batch->pages_per_seq * cache->page_tokens <= kLeastTiles * kTileKeys) return 0;  // no segment is worth cutting
     switch (cache->head_dim) {
         case 64: return scratch_bytes<64>();
         case 96: return scratch_bytes<96>();
@@ -838,9 +839,9 @@ int mhlo_cuda_cached_attention(int32_t dtype, const void* q_dev, const int64_t q
     if (need > 0 && (!scratch_dev || scratch_bytes < need || !aligned16(scratch_dev)))
         return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: needs %lld bytes of 16-byte aligned scratch", what, static_cast<long long>(need));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (dtype == MHLO_DT_F32) return launch<float>(kv, q_dev, q_strides, q_heads, scale, o_dev, o_strides, lse_dev, scratch_dev, st);
-    if (dtype == MHLO_DT_F16) return launch<__half>(kv, q_dev, q_strides, q_heads, scale, o_dev, o_strides, lse_dev, scratch_dev, st);
-    return launch<__nv_bfloat16>(kv, q_dev, q_strides, q_heads, scale, o_dev, o_strides, lse_dev, scratch_dev, st);
+    if (dtype == MHLO_DT_F32) return launch<float>(kv, q_dev, q_strides, q_heads, scale, o_dev, o_strides, lse_dev, need > 0 ? scratch_dev : nullptr, st);
+    if (dtype == MHLO_DT_F16) return launch<__half>(kv, q_dev, q_strides, q_heads, scale, o_dev, o_strides, lse_dev, need > 0 ? scratch_dev : nullptr, st);
+    return launch<__nv_bfloat16>(kv, q_dev, q_strides, q_heads, scale, o_dev, o_strides, lse_dev, need > 0 ? scratch_dev : nullptr, st);
 }
 
 }  // extern "C"

@@ -15,36 +15,80 @@
 namespace mhlo {
 namespace {
 
+// Both kernels work in units of 16 elements of a row. A unit of a rotated row holds whole pairs: 8 neighbouring elements of the first
+// half and their partners, or 16 neighbours where pairs are interleaved.
 template <typename T>
 struct AppendParams {
     KvArgs kv;
-    const T* k;
-    const T* v;
+    const T* x[2];       // keys, values
+    int64_t xs[2][2];    // their {token, head} strides
     const T* q;
     T* q_out;
-    int64_t ks[2], vs[2], qs[2], os[2];
+    int64_t qs[2], os[2];
     const float* rope;
     int64_t rope_positions;
     int32_t rotary_dim, interleaved, q_heads;
-    int64_t blocks;  // CTAs that append; the CTAs behind them rotate queries
+    int32_t vec[4];      // k, v, q, q_out: rows on the 16-byte grid
+    FastDiv units;       // units of a row
+    int64_t blocks;      // CTAs that append, a block of keys or values each; the CTAs behind them rotate queries
 };
 
-// One element of a rotated row. x: the row.
 template <typename T>
-__device__ __forceinline__ float rotated(const T* x, int d, const float* rope, int rotary_dim, int interleaved) {
-    const float own = VecTraits<T>::to_float(x[d]);
-    if (rope == nullptr || d >= rotary_dim) return own;
-    const int half = rotary_dim >> 1;
-    const int i = interleaved ? d >> 1 : d < half ? d : d - half;
-    const bool second = interleaved ? d & 1 : d >= half;
-    const float other = VecTraits<T>::to_float(x[interleaved ? d ^ 1 : second ? d - half : d + half]);
-    const float c = rope[i], s = rope[half + i];
-    return second ? __fadd_rn(__fmul_rn(own, c), __fmul_rn(other, s)) : __fsub_rn(__fmul_rn(own, c), __fmul_rn(other, s));
+__device__ __forceinline__ void load8(const T* x, bool vec, float* f) {
+    if (vec) {
+        constexpr int E = VecTraits<T>::kElems;
+#pragma unroll
+        for (int i = 0; i < 8; i += E) VecTraits<T>::unpack(__ldcs(reinterpret_cast<const uint4*>(x + i)), f + i);  // not the read-only path: q may be rotated in place
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = VecTraits<T>::to_float(x[i]);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* y, bool vec, const float* f) {
+    if (vec) {
+        constexpr int E = VecTraits<T>::kElems;
+#pragma unroll
+        for (int i = 0; i < 8; i += E) *reinterpret_cast<uint4*>(y + i) = VecTraits<T>::pack(f + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = VecTraits<T>::from_float(f[i]);
+    }
 }
 
+// Where a unit's two groups of eight elements lie.
+struct Unit {
+    int32_t low, high;
+    bool rotated;
+};
+__device__ __forceinline__ Unit unit_at(int32_t unit, int32_t rotary_dim, int32_t interleaved) {
+    Unit u{unit * 16, unit * 16 + 8, unit * 16 < rotary_dim};
+    if (u.rotated && !interleaved) {
+        u.low = unit * 8;
+        u.high = (rotary_dim >> 1) + unit * 8;
+    }
+    return u;
+}
+
+// The cosines and sines of a unit's eight pairs.
+__device__ __forceinline__ void load_turn(const float* row, int32_t unit, int32_t rotary_dim, float* cs, float* sn) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+        *reinterpret_cast<float4*>(cs + i) = __ldg(reinterpret_cast<const float4*>(row + unit * 8 + i));
+        *reinterpret_cast<float4*>(sn + i) = __ldg(reinterpret_cast<const float4*>(row + (rotary_dim >> 1) + unit * 8 + i));
+    }
+}
+__device__ __forceinline__ void turn(float* f, const float* cs, const float* sn, int32_t interleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int lo = interleaved ? 2 * i : i, hi = interleaved ? 2 * i + 1 : i + 8;
+        const float a = f[lo], b = f[hi];
+        f[lo] = __fsub_rn(__fmul_rn(a, cs[i]), __fmul_rn(b, sn[i]));
+        f[hi] = __fadd_rn(__fmul_rn(b, cs[i]), __fmul_rn(a, sn[i]));
+    }
+}
 template <typename T>
 __device__ __forceinline__ const float* rope_row(const AppendParams<T>& p, int32_t position) {
-    if (p.rope == nullptr) return nullptr;
     if (position >= p.rope_positions) {
         kv_report(MHLO_CUDA_KV_ERROR_POSITION);
         position = static_cast<int32_t>(p.rope_positions - 1);
@@ -52,40 +96,50 @@ __device__ __forceinline__ const float* rope_row(const AppendParams<T>& p, int32
     return p.rope + static_cast<int64_t>(position) * p.rotary_dim;
 }
 
-constexpr int kAppendThreads = 128;
+constexpr int kKeep = 4;  // units a thread keeps in registers between the maximum and the codes
 
 template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendParams<T> p) {
+__device__ __forceinline__ void rotate_row(const AppendParams<T>& p, int32_t row) {
     const KvArgs& a = p.kv;
-    const int page_tokens = 1 << a.page_shift, dim = a.head_dim;
-    if (blockIdx.x >= p.blocks) {  // a row of queries
-        const int32_t row = static_cast<int32_t>(blockIdx.x - p.blocks);
-        int32_t b = row;
-        if (a.starts != nullptr) b = kv_search(a.seqs, row, [&](int32_t i) { return static_cast<int64_t>(a.starts[i]); });
-        const KvSequence s = kv_sequence(a, b);
-        if (s.length == 0 || row < s.first || row >= s.first + s.count) return;
-        const float* rope = rope_row(p, s.position(row));
-        for (int i = threadIdx.x; i < p.q_heads * (dim / 16); i += kAppendThreads) {
-            const int h = i / (dim / 16), unit = i % (dim / 16), half = p.rotary_dim >> 1;
-            const T* x = p.q + row * p.qs[0] + h * p.qs[1];
-            T* y = p.q_out + row * p.os[0] + h * p.os[1];
-            float out[16];
-            int at[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {  // both elements of each pair in one thread: y may be x
-                at[e] = unit * 16 + e;
-                if (!p.interleaved && unit * 16 < p.rotary_dim) at[e] = unit * 8 + (e & 7) + (e < 8 ? 0 : half);
-                out[e] = rotated(x, at[e], rope, p.rotary_dim, p.interleaved);
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) y[at[e]] = VecTraits<T>::from_float(out[e]);
+    int32_t b = row;
+    if (a.starts != nullptr) b = kv_search(a.seqs, row, [&](int32_t i) { return static_cast<int64_t>(a.starts[i]); });
+    const KvSequence s = kv_sequence(a, b);
+    if (s.length == 0 || row < s.first || row >= s.first + s.count) return;
+    const float* const rope = rope_row(p, s.position(row));
+    const int32_t threads = blockDim.x, all = p.q_heads * static_cast<int32_t>(p.units.d);
+    float cs[8], sn[8];
+    int32_t have = -1;  // the unit whose cosines and sines are loaded: the same every time where the units of a row divide the threads
+    for (int32_t i = threadIdx.x; i < all; i += threads) {
+        const int32_t head = static_cast<int32_t>(p.units.div(i)), unit = i - head * static_cast<int32_t>(p.units.d);
+        const Unit u = unit_at(unit, p.rotary_dim, p.interleaved);
+        const T* const x = p.q + row * p.qs[0] + head * p.qs[1];
+        float f[16];
+        load8(x + u.low, p.vec[2], f);
+        load8(x + u.high, p.vec[2], f + 8);
+        if (u.rotated) {
+            if (have != unit) load_turn(rope, unit, p.rotary_dim, cs, sn);
+            have = unit;
+            if (p.interleaved) turn(f, cs, sn, 1);
+            else turn(f, cs, sn, 0);
         }
-        return;
+        T* const y = p.q_out + row * p.os[0] + head * p.os[1];
+        store8(y + u.low, p.vec[3], f);
+        store8(y + u.high, p.vec[3], f + 8);
     }
-    // block `slot` of the sequences' touched blocks. A sequence has n / P + 2 slots at least, as many as n tokens can touch:
+}
+
+__device__ __forceinline__ uint32_t code_of(float x, float step) {
+    return static_cast<uint32_t>(min(127, max(-127, __float2int_rn(__fmul_rn(x, step))))) & 255u;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ AppendParams<T> p) {
+    const KvArgs& a = p.kv;
+    if (blockIdx.x >= p.blocks) return rotate_row(p, static_cast<int32_t>(blockIdx.x - p.blocks));
+    // Block `slot` of the sequences' touched blocks. A sequence has n / P + 2 slots at least, as many as n tokens can touch:
     // slot of its first block = floor(first row / P) + 2 b.
-    const int32_t head = static_cast<int32_t>(blockIdx.x % a.heads);
-    const int64_t slot = blockIdx.x / a.heads;
+    const int32_t which = static_cast<int32_t>(blockIdx.x & 1), head = static_cast<int32_t>((blockIdx.x >> 1) % a.heads);
+    const int64_t slot = (blockIdx.x >> 1) / a.heads;
     int32_t b, nth = 0;
     if (a.starts == nullptr) {
         b = static_cast<int32_t>(slot);
@@ -96,55 +150,111 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_con
     }
     const KvSequence s = kv_sequence(a, b);
     if (s.length == 0 || s.count == 0 || nth < 0) return;
-    const int32_t page_index = ((s.length - s.count) >> a.page_shift) + nth;
+    const int32_t page_index = ((s.length - s.count) >> a.page_shift) + nth, page_tokens = 1 << a.page_shift, dim = a.head_dim;
     const int32_t from = max(s.length - s.count, page_index << a.page_shift), to = min(s.length, (page_index + 1) << a.page_shift);
     if (from >= to) return;
     const int32_t page = kv_page(a, b, page_index);
     if (page < 0) return;
-    const int32_t slot0 = from & (page_tokens - 1), n = to - from, row0 = from - (s.length - s.count) + s.first;
-    const int64_t block = static_cast<int64_t>(page) * a.heads + head;
-    __shared__ uint32_t largest[2][kAppendThreads / 32];
-    for (int which = 0; which < 2; ++which) {
-        const T* x = which == 0 ? p.k + row0 * p.ks[0] + head * p.ks[1] : p.v + row0 * p.vs[0] + head * p.vs[1];
-        const int64_t pitch = which == 0 ? p.ks[0] : p.vs[0];
-        int8_t* codes = (which == 0 ? a.k_codes : a.v_codes) + block * page_tokens * dim;
-        float* scales = (which == 0 ? a.k_scales : a.v_scales) + block;
-        uint32_t m = 0;  // magnitudes as bits: ordered like the numbers, infinity and NaN above all
-        auto value = [&](int i) {
-            const int t = i / dim, d = i % dim;
-            if (which == 1) return VecTraits<T>::to_float(x[t * pitch + d]);
-            return rotated(x + t * pitch, d, rope_row(p, from + t), p.rotary_dim, p.interleaved);
-        };
-        for (int i = threadIdx.x; i < n * dim; i += kAppendThreads) m = max(m, __float_as_uint(value(i)) & 0x7fffffffu);
-        m = __reduce_max_sync(0xffffffffu, m);
-        if ((threadIdx.x & 31) == 0) largest[which][threadIdx.x >> 5] = m;
-        const float before = slot0 == 0 ? 0.f : *scales;
-        __syncthreads();
-        for (int w = 0; w < kAppendThreads / 32; ++w) m = max(m, largest[which][w]);
-        float scale = __fmul_rn(__uint_as_float(m), 1.f / 127.f);
-        if (scale < 1.17549435e-38f) scale = 0.f;
-        scale = before > scale || before != before ? before : scale;
-        if (m >= 0x7f800000u) scale = __uint_as_float(0x7fffffffu);
-        if (threadIdx.x == 0) *scales = scale;
-        if (scale > before) {
-            const float ratio = __fdiv_rn(before, scale);
-            for (int i = threadIdx.x; i < slot0 * dim; i += kAppendThreads) codes[i] = static_cast<int8_t>(__float2int_rn(__fmul_rn(static_cast<float>(codes[i]), ratio)));
+    const int32_t slot0 = from & (page_tokens - 1), row0 = from - (s.length - s.count) + s.first;
+    const int32_t threads = blockDim.x, all = (to - from) * static_cast<int32_t>(p.units.d);
+    const int64_t block = static_cast<int64_t>(page) * a.heads + head, pitch = p.xs[which][0];
+    const T* const x = p.x[which] + row0 * pitch + head * p.xs[which][1];
+    int8_t* const codes = (which == 0 ? a.k_codes : a.v_codes) + block * page_tokens * dim;
+    float* const scales = (which == 0 ? a.k_scales : a.v_scales) + block;
+    const int32_t rotary = which == 0 ? p.rotary_dim : 0;
+    const float before = slot0 == 0 ? 0.f : *scales;
+
+    auto load_unit = [&](int32_t i, float* f) {
+        const int32_t t = static_cast<int32_t>(p.units.div(i)), unit = i - t * static_cast<int32_t>(p.units.d);
+        const Unit u = unit_at(unit, rotary, p.interleaved);
+        load8(x + t * pitch + u.low, p.vec[which], f);
+        load8(x + t * pitch + u.high, p.vec[which], f + 8);
+        if (u.rotated) {
+            float cs[8], sn[8];
+            load_turn(rope_row(p, from + t), unit, rotary, cs, sn);
+            if (p.interleaved) turn(f, cs, sn, 1);
+            else turn(f, cs, sn, 0);
         }
-        const float step = scale > 0.f ? __fdiv_rn(1.f, scale) : 0.f;  // NaN scales: codes 0
-        for (int i = threadIdx.x; i < n * dim; i += kAppendThreads) {
-            const int c = step > 0.f ? __float2int_rn(__fmul_rn(value(i), step)) : 0;
-            codes[slot0 * dim + i] = static_cast<int8_t>(min(127, max(-127, c)));
+    };
+    uint32_t m = 0;  // magnitudes as bits: ordered like the numbers, infinity and NaN above all
+    auto largest_of = [&](const float* f) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m = max(m, __float_as_uint(f[e]) & 0x7fffffffu);
+    };
+    float kept[kKeep][16];
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) {
+        const int32_t i = threadIdx.x + k * threads;
+        if (i < all) {
+            load_unit(i, kept[k]);
+            largest_of(kept[k]);
         }
+    }
+    for (int32_t i = threadIdx.x + kKeep * threads; i < all; i += threads) {  // blocks of more than 512 threads' units
+        float f[16];
+        load_unit(i, f);
+        largest_of(f);
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    __shared__ uint32_t largest[16];
+    if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = m;
+    __syncthreads();
+    for (int w = 0; w < threads >> 5; ++w) m = max(m, largest[w]);
+    float scale = __fmul_rn(__uint_as_float(m), 1.f / 127.f);
+    if (scale < 1.17549435e-38f) scale = 0.f;
+    scale = before > scale || before != before ? before : scale;
+    if (m >= 0x7f800000u) scale = __uint_as_float(0x7fffffffu);
+    if (threadIdx.x == 0) *scales = scale;
+    if (scale > before) {  // earlier tokens of the block
+        const float ratio = __fdiv_rn(before, scale);
+        for (int32_t i = threadIdx.x * 16; i < slot0 * dim; i += threads * 16) {
+            uint4 v = *reinterpret_cast<const uint4*>(codes + i);
+            uint32_t* const w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t out = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    out |= (static_cast<uint32_t>(__float2int_rn(__fmul_rn(static_cast<float>(static_cast<int8_t>(w[k] >> (8 * e))), ratio))) & 255u) << (8 * e);
+                w[k] = out;
+            }
+            *reinterpret_cast<uint4*>(codes + i) = v;
+        }
+    }
+    const float step = scale > 0.f ? __fdiv_rn(1.f, scale) : 0.f;  // NaN scales: codes 0
+    auto store_unit = [&](int32_t i, const float* f) {
+        const int32_t t = static_cast<int32_t>(p.units.div(i)), unit = i - t * static_cast<int32_t>(p.units.d);
+        const Unit u = unit_at(unit, rotary, p.interleaved);
+        int8_t* const y = codes + (slot0 + t) * dim;
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (step > 0.f) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[e >> 2] |= code_of(f[e], step) << (8 * (e & 3));
+        }
+        *reinterpret_cast<uint2*>(y + u.low) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(y + u.high) = make_uint2(w[2], w[3]);
+    };
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) {
+        const int32_t i = threadIdx.x + k * threads;
+        if (i < all) store_unit(i, kept[k]);
+    }
+    for (int32_t i = threadIdx.x + kKeep * threads; i < all; i += threads) {
+        float f[16];
+        load_unit(i, f);
+        store_unit(i, f);
     }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(128) read_kernel(const __grid_constant__ KvArgs a, T* k_out, T* v_out, int64_t s_seq, int64_t s_token, int64_t s_head,
-                                                   int64_t max_tokens, int64_t pieces) {
-    const int page_tokens = 1 << a.page_shift, dim = a.head_dim;
-    const int32_t head = static_cast<int32_t>(blockIdx.x % a.heads);
-    const int64_t unit = blockIdx.x / a.heads;
-    const int32_t b = static_cast<int32_t>(unit / pieces), i0 = static_cast<int32_t>(unit % pieces);
+                                                   int64_t max_tokens, int64_t pieces, FastDiv units, int32_t vec) {
+    const int32_t page_tokens = 1 << a.page_shift, dim = a.head_dim;
+    const int32_t which = static_cast<int32_t>(blockIdx.x & 1), head = static_cast<int32_t>((blockIdx.x >> 1) % a.heads);
+    T* out = which == 0 ? k_out : v_out;
+    if (out == nullptr) return;
+    const int64_t piece = (blockIdx.x >> 1) / a.heads;
+    const int32_t b = static_cast<int32_t>(piece / pieces), i0 = static_cast<int32_t>(piece % pieces);
     int32_t length = a.lengths[b];
     if (length < 0 || length > static_cast<int64_t>(a.pages_per_seq) << a.page_shift) {
         kv_report(MHLO_CUDA_KV_ERROR_LENGTH);
@@ -153,19 +263,35 @@ __global__ void __launch_bounds__(128) read_kernel(const __grid_constant__ KvArg
     const int64_t first = static_cast<int64_t>(i0) << a.page_shift;
     const int32_t page = first < length ? kv_page(a, b, i0) : -1;
     const int64_t block = static_cast<int64_t>(page) * a.heads + head;
-    for (int which = 0; which < 2; ++which) {
-        T* out = which == 0 ? k_out : v_out;
-        if (out == nullptr) continue;
-        out += b * s_seq + head * s_head;
-        const float scale = page < 0 ? 0.f : (which == 0 ? a.k_scales : a.v_scales)[block];
-        const int8_t* codes = (which == 0 ? a.k_codes : a.v_codes) + block * page_tokens * dim;
-        for (int i = threadIdx.x; i < page_tokens * dim; i += 128) {
-            const int64_t token = first + i / dim;
-            if (token >= max_tokens) break;
-            const float x = page >= 0 && token < length ? __fmul_rn(static_cast<float>(codes[i]), scale) : 0.f;
-            out[token * s_token + i % dim] = VecTraits<T>::from_float(x);
+    const float scale = page < 0 ? 0.f : (which == 0 ? a.k_scales : a.v_scales)[block];
+    const int8_t* const codes = (which == 0 ? a.k_codes : a.v_codes) + block * page_tokens * dim;
+    const int32_t tokens = static_cast<int32_t>(min(static_cast<int64_t>(page_tokens), max_tokens - first));
+    const int32_t there = page < 0 ? 0 : static_cast<int32_t>(min(static_cast<int64_t>(tokens), length - first));
+    out += b * s_seq + head * s_head + first * s_token;
+#pragma unroll 4
+    for (int32_t i = threadIdx.x; i < tokens * static_cast<int32_t>(units.d); i += 128) {
+        const int32_t t = static_cast<int32_t>(units.div(i)), unit = i - t * static_cast<int32_t>(units.d);
+        float f[16];
+        if (t < there) {
+            const uint4 v = ld_stream16(codes + i * 16);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 16; ++e) f[e] = __fmul_rn(static_cast<float>(static_cast<int8_t>(w[e >> 2] >> (8 * (e & 3)))), scale);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) f[e] = 0.f;
         }
+        T* const y = out + t * s_token + unit * 16;
+        store8(y, vec, f);
+        store8(y + 8, vec, f + 8);
     }
+}
+
+// Rows of a tensor on the 16-byte grid.
+template <typename T>
+int32_t on_grid(const void* x, int64_t s0, int64_t s1) {
+    constexpr int64_t E = VecTraits<T>::kElems;
+    return aligned16(x) && s0 % E == 0 && s1 % E == 0;
 }
 
 template <typename T>
@@ -173,35 +299,44 @@ int append(const KvArgs& kv, const void* k, const int64_t* ks, const void* v, co
            const int64_t* os, int64_t q_heads, const float* rope, int64_t rope_positions, int64_t rotary_dim, int32_t interleaved, cudaStream_t stream) {
     AppendParams<T> p;
     p.kv = kv;
-    p.k = static_cast<const T*>(k);
-    p.v = static_cast<const T*>(v);
+    p.x[0] = static_cast<const T*>(k);
+    p.x[1] = static_cast<const T*>(v);
     p.q = static_cast<const T*>(q);
     p.q_out = static_cast<T*>(q_out);
     for (int i = 0; i < 2; ++i) {
-        p.ks[i] = ks[i];
-        p.vs[i] = vs[i];
+        p.xs[0][i] = ks[i];
+        p.xs[1][i] = vs[i];
         p.qs[i] = q ? qs[i] : 0;
         p.os[i] = q ? os[i] : 0;
     }
+    p.vec[0] = on_grid<T>(k, ks[0], ks[1]);
+    p.vec[1] = on_grid<T>(v, vs[0], vs[1]);
+    p.vec[2] = q && on_grid<T>(q, qs[0], qs[1]);
+    p.vec[3] = q && on_grid<T>(q_out, os[0], os[1]);
     p.rope = rope;
     p.rope_positions = rope_positions;
     p.rotary_dim = static_cast<int32_t>(rope ? rotary_dim : 0);
-    p.interleaved = interleaved;
+    p.interleaved = interleaved != 0;
     p.q_heads = static_cast<int32_t>(q_heads);
-    p.blocks = (kv.starts ? (static_cast<int64_t>(kv.tokens) >> kv.page_shift) + 2 * static_cast<int64_t>(kv.seqs) : kv.seqs) * kv.heads;
+    p.units = FastDiv(static_cast<uint32_t>(kv.head_dim / 16));
+    p.blocks = 2 * kv.heads * (kv.starts ? (static_cast<int64_t>(kv.tokens) >> kv.page_shift) + 2 * static_cast<int64_t>(kv.seqs) : kv.seqs);
     const int64_t grid = p.blocks + (q ? kv.tokens : 0);
     if (grid > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "kv_cache_append: too many blocks");
-    append_kernel<T><<<static_cast<unsigned>(grid), kAppendThreads, 0, stream>>>(p);
+    // a whole block in the registers of a CTA, kKeep units a thread; single tokens need a warp or two
+    const int units = (kv.starts ? 1 << kv.page_shift : 4) * (kv.head_dim / 16);
+    const int threads = std::min(512, std::max(64, (units / kKeep + 31) / 32 * 32));
+    append_kernel<T><<<static_cast<unsigned>(grid), threads, 0, stream>>>(p);
     MHLO_CUDA_CHECK_LAUNCH("kv_cache_append");
     return MHLO_CUDA_OK;
 }
 
 template <typename T>
 int read(const KvArgs& kv, int64_t max_tokens, void* k_out, void* v_out, const int64_t* strides, cudaStream_t stream) {
-    const int64_t pieces = (max_tokens + (int64_t{1} << kv.page_shift) - 1) >> kv.page_shift, grid = pieces * kv.heads * kv.seqs;
+    const int64_t pieces = (max_tokens + (int64_t{1} << kv.page_shift) - 1) >> kv.page_shift, grid = 2 * pieces * kv.heads * kv.seqs;
     if (grid > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "kv_cache_read: too many blocks");
+    const int32_t vec = on_grid<T>(k_out, strides[0], strides[1]) && on_grid<T>(v_out, strides[2], 0);
     read_kernel<T><<<static_cast<unsigned>(grid), 128, 0, stream>>>(kv, static_cast<T*>(k_out), static_cast<T*>(v_out), strides[0], strides[1], strides[2],
-                                                                    max_tokens, pieces);
+                                                                    max_tokens, pieces, FastDiv(static_cast<uint32_t>(kv.head_dim / 16)), vec);
     MHLO_CUDA_CHECK_LAUNCH("kv_cache_read");
     return MHLO_CUDA_OK;
 }

@@ -8,8 +8,8 @@ There is no fallback: if the shared library has not been built, importing this m
 from __future__ import annotations
 
 import collections
-import contextlib
 import ctypes as C
+import functools
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -226,6 +226,7 @@ def check(status: int) -> None:
         raise MhloCudaError(status, last_error())
 
 
+@functools.lru_cache(maxsize=None)
 def torch_dtype_code(dtype) -> int:
     import torch
 
@@ -470,20 +471,21 @@ def softmax(x, axis: int = -1, out=None, tuning=None, stream=None):
 # ---- a paged cache of keys and values in 8 bits, and the attention over it ------------------------------------------------
 
 
-@contextlib.contextmanager
-def _on_stream(device, stream):
-    """The stream a call runs on: ``stream`` (a raw handle) or the current one of ``device``. That device is current inside, and
-    what is allocated there belongs to that stream."""
+def _run_on(device, stream, call):
+    """call(stream handle) with ``device`` current and ``stream`` (a raw handle, or None: the current one of that device) as the stream
+    that owns what is allocated inside. A decoding step makes several of these calls a layer: the ordinary case, everything on the
+    current device and stream, enters no context."""
     import torch
 
+    index = device.index
+    if torch.cuda.current_device() == index:
+        current = torch._C._cuda_getCurrentRawStream(index)
+        if stream is None or stream == current:
+            return call(current)
+        with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
+            return call(int(stream))
     with torch.cuda.device(device):
-        if stream is None:
-            yield torch.cuda.current_stream().cuda_stream
-        elif int(stream) == torch.cuda.current_stream().cuda_stream:
-            yield int(stream)
-        else:
-            with torch.cuda.stream(torch.cuda.ExternalStream(int(stream), device=device)):
-                yield int(stream)
+        return _run_on(device, stream, call)
 
 
 def _same_device(first, *others):
@@ -505,6 +507,8 @@ class KvCache:
         assert k_scale.is_contiguous() and v_scale.is_contiguous()
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self._args = KvCacheArgs(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.shape)
+        self.pointer = C.byref(self._args)
+        self.head_shape = (k.shape[1], k.shape[3])
 
     @classmethod
     def empty(cls, pages: int, heads: int, head_dim: int, page_tokens: int = 64, device="cuda") -> "KvCache":
@@ -518,20 +522,24 @@ class KvCache:
 def _kv_batch(page_table, lengths, token_starts, tokens) -> KvBatchArgs:
     import torch
 
-    assert page_table.dim() == 2 and lengths.dim() == 1 and page_table.shape[0] == lengths.shape[0]
-    assert page_table.dtype == lengths.dtype == torch.int32 and lengths.is_contiguous()
-    assert page_table.shape[0] <= 1 or page_table.shape[1] == 0 or page_table.stride(0) >= page_table.shape[1]
-    assert page_table.shape[1] <= 1 or page_table.stride(1) == 1
+    (seqs, pages), (pitch, step) = page_table.shape, page_table.stride()
+    assert lengths.shape == (seqs,) and page_table.dtype == lengths.dtype == torch.int32 and lengths.is_contiguous()
+    assert (seqs <= 1 or pages == 0 or pitch >= pages) and (pages <= 1 or step == 1)
     if token_starts is not None:
-        assert token_starts.dtype == torch.int32 and token_starts.is_contiguous() and token_starts.shape == (lengths.shape[0] + 1,)
-    stride = max(page_table.stride(0), page_table.shape[1])
-    return KvBatchArgs(page_table.data_ptr(), lengths.data_ptr(), _ptr(token_starts), page_table.shape[0], page_table.shape[1], stride, tokens)
+        assert token_starts.dtype == torch.int32 and token_starts.is_contiguous() and token_starts.shape == (seqs + 1,)
+    return KvBatchArgs(page_table.data_ptr(), lengths.data_ptr(), _ptr(token_starts), seqs, pages, max(pitch, pages), tokens)
 
 
-def _rows(x, heads=None):
+@functools.lru_cache(maxsize=1024)
+def _strides(*values):
+    return _i64s(values)
+
+
+def _rows(x):
     """[tokens, heads, head_dim] with a contiguous last dimension: its {token, head} strides."""
-    assert x.dim() == 3 and (x.stride(2) == 1 or x.shape[2] <= 1) and (heads is None or x.shape[1] == heads), tuple(x.shape)
-    return _i64s(x.stride()[:2])
+    token, head, step = x.stride()
+    assert step == 1 or x.shape[2] <= 1, (tuple(x.shape), x.stride())
+    return _strides(token, head)
 
 
 def rope_table(positions: int, rotary_dim: int, base: float = 10000.0, device="cuda"):
@@ -550,20 +558,29 @@ def kv_cache_append(cache: KvCache, k, v, page_table, lengths, token_starts=None
     import torch
 
     _same_device(cache.k, k, v, page_table, lengths, token_starts, rope, q, q_out)
-    heads, dim = cache.k.shape[1], cache.k.shape[3]
-    assert k.dtype == v.dtype and k.shape == v.shape and k.shape[2] == dim
-    assert q is None or (q.dtype == k.dtype and q.shape[0] == k.shape[0] and q.shape[2] == dim)
-    assert rope is None or (rope.dim() == 2 and rope.dtype == torch.float32 and rope.is_contiguous())
-    batch = _kv_batch(page_table, lengths, token_starts, k.shape[0])
-    with _on_stream(k.device, stream) as s:
-        if q is not None and q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        assert q_out is None or (q is not None and q_out.shape == q.shape and q_out.dtype == q.dtype)
-        check(lib.mhlo_cuda_kv_cache_append(torch_dtype_code(k.dtype), C.byref(cache._args), C.byref(batch), _ptr(k), _rows(k, heads), _ptr(v),
-                                            _rows(v, heads), _ptr(q), None if q is None else _rows(q), _ptr(q_out),
-                                            None if q is None else _rows(q_out), 0 if q is None else q.shape[1], _ptr(rope),
-                                            0 if rope is None else rope.shape[0], 0 if rope is None else rope.shape[1], 1 if interleaved else 0, s))
-    return q_out
+    shape, dtype = k.shape, k.dtype
+    tokens, heads, dim = shape
+    assert (heads, dim) == cache.head_shape and v.dtype == dtype and v.shape == shape
+    positions, rotary = 0, 0
+    if rope is not None:
+        positions, rotary = rope.shape
+        assert rope.dtype == torch.float32 and rope.is_contiguous()
+    batch = _kv_batch(page_table, lengths, token_starts, tokens)
+    q_heads, q_strides = 0, None
+    if q is not None:
+        q_tokens, q_heads, q_dim = q.shape
+        assert q.dtype == dtype and q_tokens == tokens and q_dim == dim
+        q_strides = _rows(q)
+    assert q_out is None or (q is not None and q_out.shape == q.shape and q_out.dtype == dtype)
+
+    def call(s):
+        out = torch.empty(q.shape, dtype=dtype, device=q.device) if q is not None and q_out is None else q_out
+        check(lib.mhlo_cuda_kv_cache_append(torch_dtype_code(dtype), cache.pointer, C.byref(batch), k.data_ptr(), _rows(k), v.data_ptr(), _rows(v),
+                                            _ptr(q), q_strides, _ptr(out), None if q is None else _rows(out), q_heads, _ptr(rope), positions, rotary,
+                                            1 if interleaved else 0, s))
+        return out
+
+    return _run_on(k.device, stream, call)
 
 
 def kv_cache_read(cache: KvCache, page_table, lengths, max_tokens: int, dtype=None, k_out=None, v_out=None, stream=None):
@@ -572,16 +589,21 @@ def kv_cache_read(cache: KvCache, page_table, lengths, max_tokens: int, dtype=No
     import torch
 
     _same_device(cache.k, page_table, lengths, k_out, v_out)
-    batch = _kv_batch(page_table, lengths, None, lengths.shape[0])
-    shape = (lengths.shape[0], max_tokens, cache.k.shape[1], cache.k.shape[3])
-    with _on_stream(cache.k.device, stream) as s:
-        dtype = k_out.dtype if k_out is not None else dtype or torch.float32
-        k_out = torch.empty(shape, dtype=dtype, device=cache.k.device) if k_out is None else k_out
-        v_out = torch.empty_strided(shape, k_out.stride(), dtype=dtype, device=cache.k.device) if v_out is None else v_out
-        assert k_out.shape == v_out.shape == shape and k_out.dtype == v_out.dtype and k_out.stride() == v_out.stride() and k_out.stride(3) == 1
-        check(lib.mhlo_cuda_kv_cache_read(torch_dtype_code(dtype), C.byref(cache._args), C.byref(batch), max_tokens, _ptr(k_out), _ptr(v_out),
-                                          _i64s(k_out.stride()[:3]), s))
-    return k_out, v_out
+    seqs = lengths.shape[0]
+    batch = _kv_batch(page_table, lengths, None, seqs)
+    shape = (seqs, max_tokens, *cache.head_shape)
+    dtype = k_out.dtype if k_out is not None else dtype or torch.float32
+
+    def call(s):
+        k = torch.empty(shape, dtype=dtype, device=lengths.device) if k_out is None else k_out
+        v = torch.empty_like(k) if v_out is None else v_out
+        seq, token, head, step = k.stride()
+        assert k.shape == v.shape == shape and v.dtype == dtype and v.stride() == k.stride() and step == 1
+        check(lib.mhlo_cuda_kv_cache_read(torch_dtype_code(dtype), cache.pointer, C.byref(batch), max_tokens, k.data_ptr(), v.data_ptr(),
+                                          _strides(seq, token, head), s))
+        return k, v
+
+    return _run_on(lengths.device, stream, call)
 
 
 def cached_attention(q, cache: KvCache, page_table, lengths, scale: float, token_starts=None, out=None, lse=None, stream=None):
@@ -590,17 +612,22 @@ def cached_attention(q, cache: KvCache, page_table, lengths, scale: float, token
     import torch
 
     _same_device(q, cache.k, page_table, lengths, token_starts, out, lse)
-    assert q.dim() == 3 and q.shape[2] == cache.k.shape[3]
-    batch = _kv_batch(page_table, lengths, token_starts, q.shape[0])
-    with _on_stream(q.device, stream) as s:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
-        assert out.shape == q.shape and out.dtype == q.dtype
-        assert lse is None or (lse.shape == q.shape[:2] and lse.dtype == torch.float32 and lse.is_contiguous())
-        need = lib.mhlo_cuda_cached_attention_scratch_bytes(C.byref(cache._args), C.byref(batch), q.shape[1])
+    shape, dtype = q.shape, q.dtype
+    tokens, q_heads, dim = shape
+    assert dim == cache.head_shape[1]
+    assert out is None or (out.shape == shape and out.dtype == dtype)
+    assert lse is None or (lse.shape == shape[:2] and lse.dtype == torch.float32 and lse.is_contiguous())
+    batch = _kv_batch(page_table, lengths, token_starts, tokens)
+
+    def call(s):
+        o = torch.empty(shape, dtype=dtype, device=q.device) if out is None else out
+        need = lib.mhlo_cuda_cached_attention_scratch_bytes(cache.pointer, C.byref(batch), q_heads)
         scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
-        check(lib.mhlo_cuda_cached_attention(torch_dtype_code(q.dtype), _ptr(q), _rows(q), C.byref(cache._args), C.byref(batch), q.shape[1], scale,
-                                             _ptr(out), _rows(out), _ptr(lse), _ptr(scratch), max(need, 0), s))
-    return out
+        check(lib.mhlo_cuda_cached_attention(torch_dtype_code(dtype), q.data_ptr(), _rows(q), cache.pointer, C.byref(batch), q_heads, scale, o.data_ptr(),
+                                             _rows(o), _ptr(lse), _ptr(scratch), need, s))
+        return o
+
+    return _run_on(q.device, stream, call)
 
 
 # ---- log probabilities ------------------------------------------------------------------------------------------------
@@ -628,14 +655,22 @@ def token_logprobs(logits, targets=None, top_k: int = 0, scale: float = 1.0, ent
     rows, pitch = _logit_rows(logits)
     lead = logits.shape[:-1]
     assert targets is None or (targets.shape == lead and targets.is_contiguous())
-    with _on_stream(logits.device, stream) as s:
-        new = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=logits.device)
-        r = TokenLogprobs(None if targets is None else new(*lead), new(*lead) if entropy else None, new(*lead),
-                          new(*lead, top_k) if top_k else None, new(*lead, top_k, dtype=torch.int32) if top_k else None)
-        check(lib.mhlo_cuda_token_logprobs(torch_dtype_code(logits.dtype), _ptr(logits), pitch, rows, logits.shape[-1], scale, _ptr(targets),
-                                           I64 if targets is None else torch_dtype_code(targets.dtype), _ptr(r.logprobs), _ptr(r.entropy), _ptr(r.lse),
-                                           top_k, _ptr(r.top_logprobs), _ptr(r.top_ids), s))
-    return r
+    assert top_k >= 0
+
+    def call(s):
+        # one allocation for the numbers of a row, one for its alternatives
+        logprobs, ent, lse = torch.empty((3, *lead), dtype=torch.float32, device=logits.device).unbind(0)
+        top = ids = None
+        if top_k:
+            top = torch.empty((*lead, top_k), dtype=torch.float32, device=logits.device)
+            ids = torch.empty((*lead, top_k), dtype=torch.int32, device=logits.device)
+        r = TokenLogprobs(None if targets is None else logprobs, ent if entropy else None, lse, top, ids)
+        check(lib.mhlo_cuda_token_logprobs(torch_dtype_code(logits.dtype), logits.data_ptr(), pitch, rows, logits.shape[-1], scale, _ptr(targets),
+                                           I64 if targets is None else torch_dtype_code(targets.dtype), _ptr(r.logprobs), _ptr(r.entropy), lse.data_ptr(),
+                                           top_k, _ptr(top), _ptr(ids), s))
+        return r
+
+    return _run_on(logits.device, stream, call)
 
 
 def token_logprobs_grad(logits, targets, lse, entropy=None, grad_logprobs=None, grad_entropy=None, top_ids=None, grad_top=None, scale: float = 1.0,
@@ -652,11 +687,14 @@ def token_logprobs_grad(logits, targets, lse, entropy=None, grad_logprobs=None, 
         assert t is None or (t.shape == lead and t.dtype == torch.float32 and t.is_contiguous())
     assert grad_top is None or (top_ids is not None and grad_top.shape == top_ids.shape and top_ids.shape[:-1] == lead and grad_top.dtype == torch.float32
                                 and top_ids.dtype == torch.int32 and grad_top.is_contiguous() and top_ids.is_contiguous())
-    with _on_stream(logits.device, stream) as s:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else out
-        assert out.shape == logits.shape and out.dtype == logits.dtype
-        check(lib.mhlo_cuda_token_logprobs_grad(torch_dtype_code(logits.dtype), _ptr(logits), pitch, rows, logits.shape[-1], scale, _ptr(targets),
-                                                I64 if targets is None else torch_dtype_code(targets.dtype), _ptr(lse), _ptr(entropy), _ptr(grad_logprobs),
+    assert out is None or (out.shape == logits.shape and out.dtype == logits.dtype)
+
+    def call(s):
+        dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else out
+        check(lib.mhlo_cuda_token_logprobs_grad(torch_dtype_code(logits.dtype), logits.data_ptr(), pitch, rows, logits.shape[-1], scale, _ptr(targets),
+                                                I64 if targets is None else torch_dtype_code(targets.dtype), lse.data_ptr(), _ptr(entropy), _ptr(grad_logprobs),
                                                 _ptr(grad_entropy), 0 if grad_top is None else grad_top.shape[-1], _ptr(top_ids), _ptr(grad_top),
-                                                _ptr(out), _logit_rows(out)[1], s))
-    return out
+                                                dx.data_ptr(), _logit_rows(dx)[1], s))
+        return dx
+
+    return _run_on(logits.device, stream, call)

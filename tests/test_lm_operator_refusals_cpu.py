@@ -75,9 +75,10 @@ def test_attention():
         assert attention(scale=scale) == UNSUPPORTED
     assert attention(q=None) == INVALID and attention(o=None) == INVALID
     assert attention(os=cuda._i64s([256, 64])) == INVALID
-    need = cuda.lib.mhlo_cuda_cached_attention_scratch_bytes(C.byref(cache()), C.byref(batch()), 4)
-    if need:
-        assert attention(size=need - 1) == INVALID and attention(scratch=None) == INVALID and attention(scratch=P + 8) == INVALID
+    long = batch(pages_per_seq=400, table_stride=400)
+    need = cuda.lib.mhlo_cuda_cached_attention_scratch_bytes(C.byref(cache()), C.byref(long), 4)
+    assert need > 0 and cuda.lib.mhlo_cuda_cached_attention_scratch_bytes(None, None, 4) == 0
+    assert attention(b=long, size=need - 1) == INVALID and attention(b=long, scratch=None) == INVALID and attention(b=long, scratch=P + 8) == INVALID
     assert attention(b=batch(tokens=0), scratch=None, size=0) == OK
 
 
