@@ -1,15 +1,37 @@
 // Log probabilities of given tokens, entropy, the largest alternatives, and their gradient with respect to the logits.
 //
-// With z = scale x and m = max z: S = sum exp(z - m), T = sum exp(z - m) (z - m), lse = m + log S, entropy = log S - T / S. A logit
-// of -infinity has probability 0 and no part in T.
+// With z = scale x and m = max x: d_i = (x_i - m) scale log2(e), S = sum 2^d, T = sum 2^d d, so lse = scale m + log S and entropy =
+// log S - log(2) T / S. A logit of -infinity has probability 0 and no part in T. Differences to the maximum are taken before the
+// scale: rows at the lowest value of their type neither overflow nor lose their digits.
+//
+// One pass. A thread has 4 vectors of 16 bytes in flight and keeps a running maximum with its S and T; when a batch of its vectors
+// holds a larger logit, S and T move to it (T' = f (T + S delta), S' = f S with f = 2^delta). Everything is joined at the end of the
+// row. Per element that is about five instructions and one exponential (16 a clock and SM), against 11 16-bit elements a clock and
+// SM that the memory delivers.
+//
+// Alternatives come out of the same pass. Keys are 64 bits, the logit's order above the complement of its place, so no two are equal
+// and ties go to the lowest id. After the first batch the k-th largest of 64 groups' maxima bounds the k-th largest key from below;
+// from then on only elements above the bound, some dozens of a row, are put on a list. When a batch would overflow the list (rising
+// logits), the list is cut to its k largest and the bound raised by that batch's own maxima, at last by those of single threads: then
+// at most k threads have anything to add.
+#include <cooperative_groups.h>
+
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace mhlo {
 namespace {
 
-constexpr int kThreads = 512;
+typedef unsigned long long Key;
+
+constexpr int kBatch = 4;     // vectors of a thread in flight
+constexpr int kGroups = 64;   // whose maxima give the first bound: twice the most alternatives
+constexpr int kList = 2048;   // keys
+constexpr float kLowest = -150.f;  // 2^-150 is 0 in fp32: what exponents are kept above, so that 0 * -infinity never comes up
 
 template <typename T>
 struct LogprobParams {
@@ -30,58 +52,269 @@ __device__ __forceinline__ int64_t target_of(const void* targets, int32_t wide, 
     return wide ? static_cast<const int64_t*>(targets)[row] : static_cast<const int32_t*>(targets)[row];
 }
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
 // Logits in the order of the alternatives: NaN above all, -0 = +0.
 __device__ __forceinline__ uint32_t order_of(float x) {
     if (x != x) return 0xffffffffu;
     const uint32_t u = __float_as_uint(x + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ Key key_of(float x, uint32_t place) { return static_cast<Key>(order_of(x)) << 32 | (0xffffffffu - place); }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const __grid_constant__ LogprobParams<T> p) {
-    __shared__ float scratch[3][32];
-    __shared__ unsigned long long best[kThreads / 32];
-    const int64_t row = blockIdx.x;
-    const T* x = p.x + row * p.row_stride;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float m = -INFINITY;
-    for (int64_t i = threadIdx.x; i < p.vocab; i += kThreads) m = fmaxf(m, VecTraits<T>::to_float(x[i]) * p.scale);
-    m = cta_reduce<MaxOp>(m, scratch[0]);
-    float s = 0.f, t = 0.f;
-    for (int64_t i = threadIdx.x; i < p.vocab; i += kThreads) {
-        const float d = VecTraits<T>::to_float(x[i]) * p.scale - m, e = expf(d);
-        s += e;
-        t += e * fmaxf(d, -200.f);
+__device__ __forceinline__ uint4 all_lowest();  // a vector of -infinities
+template <>
+__device__ __forceinline__ uint4 all_lowest<float>() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+template <>
+__device__ __forceinline__ uint4 all_lowest<__half>() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+template <>
+__device__ __forceinline__ uint4 all_lowest<__nv_bfloat16>() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+
+// The largest element of a vector, NaN if there is one.
+template <typename T>
+__device__ __forceinline__ float largest_of(const uint4& v) {
+    if constexpr (sizeof(T) == 4) {
+        return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+    } else if constexpr (std::is_same<T, __half>::value) {
+        const __half2* h = reinterpret_cast<const __half2*>(&v);
+        const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        return max_nan(__low2float(m), __high2float(m));
+    } else {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        return max_nan(__low2float(m), __high2float(m));
     }
-    s = cta_reduce<SumOp>(s, scratch[1]);
-    t = cta_reduce<SumOp>(t, scratch[2]);
-    const float lse = m + logf(s);
-    if (threadIdx.x == 0) {
-        if (p.lse) p.lse[row] = lse;
-        if (p.entropy) p.entropy[row] = logf(s) - t / s;
+}
+
+// A row as up to E - 1 elements in front of the first 16-byte boundary, vectors, and up to E - 1 elements behind the last one.
+template <typename T>
+struct Row {
+    const T* x;
+    int64_t vectors;
+    int32_t head, tail;
+    __device__ __forceinline__ Row(const T* row, int64_t n) : x(row) {
+        constexpr int E = VecTraits<T>::kElems;
+        const int64_t off = static_cast<int64_t>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int64_t>(sizeof(T));
+        head = static_cast<int32_t>(off < n ? off : n);
+        vectors = (n - head) / E;
+        tail = static_cast<int32_t>(n - head - vectors * E);
+    }
+    __device__ __forceinline__ int32_t singles() const { return head + tail; }
+    __device__ __forceinline__ int64_t place_of_single(int32_t i) const { return i < head ? i : vectors * VecTraits<T>::kElems + i; }
+    __device__ __forceinline__ int64_t place(int64_t vector) const { return head + vector * VecTraits<T>::kElems; }
+};
+
+// The kept keys' ranks among `n` in shared memory: those below k go to list[rank]. All threads call it.
+template <int THREADS>
+__device__ __forceinline__ void take_largest(const Key* keys, int n, int k, Key* list) {
+    for (int i = threadIdx.x; i < n; i += THREADS) {
+        const Key mine = keys[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += keys[j] > mine;
+        if (rank < k) list[rank] = mine;
+    }
+}
+
+// CTAs of a cluster share a row (clusters of 1 to 8, along x): the first one joins them.
+template <typename T, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const __grid_constant__ LogprobParams<T> p) {
+    constexpr int E = VecTraits<T>::kElems, kWarps = THREADS / 32;
+    __shared__ float scratch[3][32];
+    __shared__ float joined[4];  // maximum, S, T of this CTA
+    __shared__ Key list[TOP ? kList : 1], group[TOP ? THREADS : 1], best[TOP ? MHLO_CUDA_TOP_LOGPROBS_MAX : 1], bound_shared;
+    __shared__ int listed;
+    grid_dependency_wait();
+    cg::cluster_group cluster = cg::this_cluster();
+    const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
+    const int64_t row = blockIdx.x / parts;
+    const Row<T> r(p.x + row * p.row_stride, p.vocab);
+    const int64_t v0 = r.vectors * part / parts, v1 = r.vectors * (part + 1) / parts;
+    const uint4* const vectors = reinterpret_cast<const uint4*>(r.x + r.head);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float c = p.scale * 1.4426950408889634f;
+
+    float m = -INFINITY, s = 0.f, t = 0.f;
+    Key bound = 0;
+    int kept = 0;  // keys on the list before this batch
+    if (TOP && tid == 0) listed = 0;
+    bool first = true;
+    for (int64_t base = v0; first || base < v1; base += THREADS * kBatch) {
+        uint4 raw[kBatch];
+        float single = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int64_t v = base + tid + i * THREADS;
+            raw[i] = v < v1 ? ld_stream16(vectors + v) : all_lowest<T>();
+        }
+        const bool has_single = first && part == 0 && tid < r.singles();
+        if (has_single) single = VecTraits<T>::to_float(r.x[r.place_of_single(tid)]);
+        float most = single;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) most = max_nan(most, largest_of<T>(raw[i]));
+        if (most > m) {
+            const float delta = fmaxf((m - most) * c, kLowest), f = ex2(delta);
+            t = f * fmaf(s, delta, t);
+            s *= f;
+            m = most;
+        }
+        const float from = m == -INFINITY ? 0.f : m;
+        const float2 minus = make_float2(-from, -from), by = make_float2(c, c);
+        float2 s2 = make_float2(0.f, 0.f), t2 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            float2 f[E / 2];
+            VecTraits<T>::unpack2(raw[i], f);
+#pragma unroll
+            for (int e = 0; e < E / 2; ++e) {
+                float2 d = __fmul2_rn(__fadd2_rn(f[e], minus), by);
+                d.x = max_nan(d.x, kLowest);
+                d.y = max_nan(d.y, kLowest);
+                const float2 w = make_float2(ex2(d.x), ex2(d.y));
+                s2 = __fadd2_rn(s2, w);
+                t2 = __ffma2_rn(w, d, t2);
+            }
+        }
+        if (has_single) {
+            const float d = max_nan((single - from) * c, kLowest), w = ex2(d);
+            s2.x += w;
+            t2.x = fmaf(w, d, t2.x);
+        }
+        s += s2.x + s2.y;
+        t += t2.x + t2.y;
+
+        if constexpr (TOP) {
+            auto each_key = [&](auto&& use) {  // this thread's keys of the batch
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const int64_t v = base + tid + i * THREADS;
+                    if (v >= v1) continue;
+                    float f[E];
+                    VecTraits<T>::unpack(raw[i], f);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) use(key_of(f[e], static_cast<uint32_t>(r.place(v) + e)));
+                }
+                if (has_single) use(key_of(single, static_cast<uint32_t>(r.place_of_single(tid))));
+            };
+            // The bound from the maxima of `groups` groups of neighbouring threads: the k-th largest of them.
+            auto raise_bound = [&](int groups) {
+                Key mine = 0;
+                each_key([&](Key key) { mine = max(mine, key); });
+                const int width = THREADS / groups;
+                for (int o = 1; o < width; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+                if (tid % width == 0) group[tid / width] = mine;
+                if (tid == 0) bound_shared = 0;
+                __syncthreads();
+                for (int i = tid; i < groups; i += THREADS) {
+                    const Key own = group[i];
+                    int rank = 0;
+                    for (int j = 0; j < groups; ++j) rank += group[j] > own || (group[j] == own && j < i);  // empty groups are equal
+                    if (rank == p.top_k - 1) bound_shared = own;
+                }
+                __syncthreads();
+                bound = max(bound, bound_shared);
+            };
+            auto add = [&]() {
+                if (order_of(most) < static_cast<uint32_t>(bound >> 32)) return;
+                each_key([&](Key key) {
+                    if (key < bound) return;
+                    const int at = atomicAdd(&listed, 1);
+                    if (at < kList) list[at] = key;
+                });
+            };
+            if (first) raise_bound(kGroups);
+            add();
+            __syncthreads();
+            for (int groups = kGroups; listed > kList; groups = THREADS) {  // too many: at most twice
+                __syncthreads();
+                if (kept > p.top_k) {  // earlier batches' keys, cut to the k largest
+                    take_largest<THREADS>(list, kept, p.top_k, best);
+                    __syncthreads();
+                    if (tid < p.top_k) list[tid] = best[tid];
+                    kept = p.top_k;
+                }
+                if (tid == 0) listed = kept;
+                raise_bound(groups);
+                add();
+                __syncthreads();
+            }
+            kept = listed;
+            __syncthreads();  // everybody has read it
+        }
+        first = false;
+    }
+
+    const float top = cta_reduce<MaxOp>(m, scratch[0]), from = top == -INFINITY ? 0.f : top;
+    const float delta = fmaxf((m - from) * c, kLowest), f = ex2(delta);
+    const float all_t = cta_reduce<SumOp>(f * fmaf(s, delta, t), scratch[1]);
+    const float all_s = cta_reduce<SumOp>(f * s, scratch[2]);
+    if (tid == 0) {
+        joined[0] = top;
+        joined[1] = all_s;
+        joined[2] = all_t;
+    }
+    if constexpr (TOP) {
+        if (tid < MHLO_CUDA_TOP_LOGPROBS_MAX) best[tid] = 0;
+        __syncthreads();
+        take_largest<THREADS>(list, kept, p.top_k, best);
+    }
+    if (parts > 1) {
+        cluster.sync();
+        if (part == 0) {
+            if (TOP) {  // the parts' alternatives
+                for (int i = tid; i < parts * p.top_k; i += THREADS) list[i] = cluster.map_shared_rank(best, i / p.top_k)[i % p.top_k];
+            }
+            if (tid == 0) {
+                float most = joined[0];
+                for (int i = 1; i < parts; ++i) most = fmaxf(most, cluster.map_shared_rank(joined, i)[0]);
+                float sum = 0.f, weighted = 0.f;
+                for (int i = 0; i < parts; ++i) {
+                    const float* other = cluster.map_shared_rank(joined, i);
+                    const float move = fmaxf((other[0] - (most == -INFINITY ? 0.f : most)) * c, kLowest), g = ex2(move);
+                    weighted += g * fmaf(other[1], move, other[2]);
+                    sum += g * other[1];
+                }
+                scratch[0][0] = most;
+                scratch[0][1] = sum;
+                scratch[0][2] = weighted;
+            }
+        }
+        cluster.sync();  // no CTA leaves while its shared memory is read
+        if (part != 0) return;
+        if (tid == 0) {
+            joined[0] = scratch[0][0];
+            joined[1] = scratch[0][1];
+            joined[2] = scratch[0][2];
+        }
+        if constexpr (TOP) {
+            if (tid < MHLO_CUDA_TOP_LOGPROBS_MAX) best[tid] = 0;
+            __syncthreads();
+            take_largest<THREADS>(list, parts * p.top_k, p.top_k, best);
+        }
+    }
+    __syncthreads();
+    const float most = joined[0], sum = most == -INFINITY ? NAN : joined[1], log_s = logf(sum);
+    if (tid == 0) {
+        if (p.lse) p.lse[row] = most * p.scale + log_s;
+        if (p.entropy) p.entropy[row] = log_s - 0.6931471805599453f * (joined[2] / sum);
         if (p.targets) {
             const int64_t id = target_of(p.targets, p.wide_targets, row);
-            p.logprobs[row] = id < 0 ? 0.f : id >= p.vocab ? NAN : VecTraits<T>::to_float(x[id]) * p.scale - lse;
+            p.logprobs[row] = id < 0 ? 0.f : id >= p.vocab ? NAN : (VecTraits<T>::to_float(r.x[id]) - most) * p.scale - log_s;
         }
     }
-    unsigned long long below = ~0ull;  // the last alternative taken
-    for (int k = 0; k < p.top_k; ++k) {
-        unsigned long long mine = 0;
-        for (int64_t i = threadIdx.x; i < p.vocab; i += kThreads) {
-            const unsigned long long key = static_cast<unsigned long long>(order_of(VecTraits<T>::to_float(x[i]))) << 32 | (0xffffffffu - static_cast<uint32_t>(i));
-            if (key < below && key > mine) mine = key;
-        }
-        for (int o = 16; o > 0; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-        __syncthreads();
-        if (lane == 0) best[warp] = mine;
-        __syncthreads();
-        for (int w = 0; w < kThreads / 32; ++w) mine = max(mine, best[w]);
-        below = mine;
-        if (threadIdx.x == 0) {
-            const uint32_t id = 0xffffffffu - static_cast<uint32_t>(mine);
-            p.top_ids[row * p.top_k + k] = static_cast<int32_t>(id);
-            p.top_logprobs[row * p.top_k + k] = VecTraits<T>::to_float(x[id]) * p.scale - lse;
-        }
+    if (TOP && tid < p.top_k) {
+        const uint32_t id = 0xffffffffu - static_cast<uint32_t>(best[tid]);
+        p.top_ids[row * p.top_k + tid] = static_cast<int32_t>(id);
+        p.top_logprobs[row * p.top_k + tid] = id < p.vocab ? (VecTraits<T>::to_float(r.x[id]) - most) * p.scale - log_s : NAN;
     }
 }
 
@@ -103,34 +336,86 @@ struct GradParams {
     int64_t dx_row_stride;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_grad_kernel(const __grid_constant__ GradParams<T> p) {
+// dx = scale (picked - p (all + e (log p + entropy))): one pass, 16 bytes in and out a step. The target is picked as its vector comes
+// by; alternatives are few, and their elements are computed once more by a thread each behind the row (their logits are read before
+// anything is written: dx may be x).
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) logprobs_grad_kernel(const __grid_constant__ GradParams<T> p) {
+    constexpr int E = VecTraits<T>::kElems;
     __shared__ float weight[MHLO_CUDA_TOP_LOGPROBS_MAX];
     __shared__ int32_t ids[MHLO_CUDA_TOP_LOGPROBS_MAX];
     const int64_t row = blockIdx.x;
-    const T* x = p.x + row * p.row_stride;
-    T* dx = p.dx + row * p.dx_row_stride;
+    const Row<T> r(p.x + row * p.row_stride, p.vocab);
+    T* const dx = p.dx + row * p.dx_row_stride;
+    const int tid = threadIdx.x;
     int64_t target = -1;
     float g = 0.f;
-    if (p.g && p.targets) {
+    if (p.g) {
         target = target_of(p.targets, p.wide_targets, row);
         g = target < 0 ? 0.f : target >= p.vocab ? NAN : p.g[row];
     }
-    if (threadIdx.x < p.top_k) {
-        const int32_t id = p.top_ids[row * p.top_k + threadIdx.x];
-        ids[threadIdx.x] = id;
-        weight[threadIdx.x] = id < 0 ? 0.f : id >= p.vocab ? NAN : p.t[row * p.top_k + threadIdx.x];
+    float all = g, own = 0.f;
+    int32_t own_id = -1;
+    if (p.top_k > 0) {
+        if (tid < p.top_k) {
+            own_id = p.top_ids[row * p.top_k + tid];
+            ids[tid] = own_id;
+            weight[tid] = own_id < 0 ? 0.f : own_id >= p.vocab ? NAN : p.t[row * p.top_k + tid];
+            if (own_id >= 0 && own_id < p.vocab) own = VecTraits<T>::to_float(r.x[own_id]);
+            else own_id = -1;
+        }
+        __syncthreads();
+        for (int k = 0; k < p.top_k; ++k) all += weight[k];
     }
-    __syncthreads();
-    float all = g;
-    for (int k = 0; k < p.top_k; ++k) all += weight[k];
     const float lse = p.lse[row], e = p.e ? p.e[row] : 0.f, h = p.e ? p.entropy[row] : 0.f;
-    for (int64_t i = threadIdx.x; i < p.vocab; i += kThreads) {
-        const float logp = VecTraits<T>::to_float(x[i]) * p.scale - lse, pr = expf(logp);
-        float d = -pr * (all + e * (fmaxf(logp, -200.f) + h));
-        if (i == target) d += g;
-        for (int k = 0; k < p.top_k; ++k) d += ids[k] == i ? weight[k] : 0.f;
-        dx[i] = VecTraits<T>::from_float(d * p.scale);
+    const float constant = fmaf(e, h, all), minus_scale = -p.scale;
+    auto unpicked = [&](float x) {  // scale (-p (all + e (log p + h)))
+        const float logp = fmaf(x, p.scale, -lse), low = max_nan(logp, -200.f);
+        return ex2(logp * 1.4426950408889634f) * fmaf(e, low, constant) * minus_scale;
+    };
+    const float picked = g * p.scale;
+    const bool together = ((reinterpret_cast<uintptr_t>(r.x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;  // both rows' vectors on the grid
+    const uint4* const vectors = reinterpret_cast<const uint4*>(r.x + r.head);
+    for (int64_t base = 0; base < r.vectors; base += THREADS * kBatch) {
+        uint4 raw[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int64_t v = base + tid + i * THREADS;
+            if (v < r.vectors) raw[i] = __ldcs(vectors + v);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int64_t v = base + tid + i * THREADS;
+            if (v >= r.vectors) break;
+            float f[E];
+            VecTraits<T>::unpack(raw[i], f);
+            const int64_t at = target - r.place(v);
+#pragma unroll
+            for (int k = 0; k < E; ++k) f[k] = unpicked(f[k]);
+            if (at >= 0 && at < E) {
+#pragma unroll
+                for (int k = 0; k < E; ++k) f[k] += at == k ? picked : 0.f;
+            }
+            T* const y = dx + r.place(v);
+            if (together) {
+                st_stream16(y, VecTraits<T>::pack(f));
+            } else {
+#pragma unroll
+                for (int k = 0; k < E; ++k) y[k] = VecTraits<T>::from_float(f[k]);
+            }
+        }
+    }
+    if (tid < r.singles()) {
+        const int64_t i = r.place_of_single(tid);
+        dx[i] = VecTraits<T>::from_float(unpicked(VecTraits<T>::to_float(r.x[i])) + (i == target ? picked : 0.f));
+    }
+    if (p.top_k > 0) {
+        __syncthreads();
+        if (own_id >= 0) {
+            float sum = own_id == target ? g : 0.f;
+            for (int k = 0; k < p.top_k; ++k) sum += ids[k] == own_id ? weight[k] : 0.f;
+            dx[own_id] = VecTraits<T>::from_float(fmaf(sum, p.scale, unpicked(own)));
+        }
     }
 }
 
@@ -146,19 +431,27 @@ int check_rows(const char* what, int32_t dtype, const void* x, int64_t row_strid
     return MHLO_CUDA_OK;
 }
 
-template <typename T>
-int launch(const void* x, LogprobParams<T> p, int64_t rows, cudaStream_t stream) {
-    p.x = static_cast<const T*>(x);
-    logprobs_kernel<T><<<static_cast<unsigned>(rows), kThreads, 0, stream>>>(p);
+// Short rows take CTAs of 128 threads: a row of 100 logits keeps 13 to 25 of them busy.
+inline bool short_rows(int64_t vocab, int64_t size) { return vocab * size <= 16 * 512; }
+
+template <typename T, bool TOP>
+int launch(const LogprobParams<T>& p, int64_t rows, cudaStream_t stream) {
+    // Few long rows are shared by clusters of CTAs, as long as a thread gets two vectors of its own.
+    int parts = 1;
+    while (parts < 8 && rows * parts * 2 <= kNumSMs && p.vocab * static_cast<int64_t>(sizeof(T)) >= int64_t{16} * 512 * 2 * parts * 2) parts *= 2;
+    if (rows * parts > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "token_logprobs: too many rows");
+    const dim3 grid(static_cast<unsigned>(rows * parts));
+    const cudaError_t e = short_rows(p.vocab, sizeof(T)) ? launch_dependent(logprobs_kernel<T, TOP, 128>, grid, dim3(128), 0, stream, 1, rows < kNumSMs, p)
+                                                         : launch_dependent(logprobs_kernel<T, TOP, 512>, grid, dim3(512), 0, stream, parts, rows * parts < kNumSMs, p);
+    if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of token_logprobs failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("token_logprobs");
     return MHLO_CUDA_OK;
 }
 
 template <typename T>
-int launch_grad(const void* x, void* dx, GradParams<T> p, int64_t rows, cudaStream_t stream) {
-    p.x = static_cast<const T*>(x);
-    p.dx = static_cast<T*>(dx);
-    logprobs_grad_kernel<T><<<static_cast<unsigned>(rows), kThreads, 0, stream>>>(p);
+int launch_grad(const GradParams<T>& p, int64_t rows, cudaStream_t stream) {
+    if (short_rows(p.vocab, sizeof(T))) logprobs_grad_kernel<T, 128><<<static_cast<unsigned>(rows), 128, 0, stream>>>(p);
+    else logprobs_grad_kernel<T, 512><<<static_cast<unsigned>(rows), 512, 0, stream>>>(p);
     MHLO_CUDA_CHECK_LAUNCH("token_logprobs_grad");
     return MHLO_CUDA_OK;
 }
@@ -180,8 +473,9 @@ int mhlo_cuda_token_logprobs(int32_t dtype, const void* x_dev, int64_t row_strid
     if (top_k > 0 && (!top_logprobs_dev || !top_ids_dev)) return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: null result for the alternatives", what);
     auto run = [&](auto zero) {
         using T = decltype(zero);
-        LogprobParams<T> p{nullptr, row_stride, vocab, scale, targets_dev, target_dtype == MHLO_DT_I64, logprobs_dev, entropy_dev, lse_dev, top_k, top_logprobs_dev, top_ids_dev};
-        return launch<T>(x_dev, p, rows, static_cast<cudaStream_t>(stream));
+        LogprobParams<T> p{static_cast<const T*>(x_dev), row_stride, vocab, scale, targets_dev, target_dtype == MHLO_DT_I64, logprobs_dev, entropy_dev, lse_dev, top_k, top_logprobs_dev, top_ids_dev};
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        return top_k > 0 ? launch<T, true>(p, rows, st) : launch<T, false>(p, rows, st);
     };
     if (dtype == MHLO_DT_F32) return run(float{});
     if (dtype == MHLO_DT_F16) return run(__half{});
@@ -203,9 +497,9 @@ int mhlo_cuda_token_logprobs_grad(int32_t dtype, const void* x_dev, int64_t row_
         return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: rows of the result %lld apart", what, static_cast<long long>(dx_row_stride));
     auto run = [&](auto zero) {
         using T = decltype(zero);
-        GradParams<T> p{nullptr, row_stride, vocab, scale, targets_dev, target_dtype == MHLO_DT_I64, lse_dev, entropy_dev, grad_logprobs_dev, grad_entropy_dev,
-                        grad_top_dev ? top_k : 0, top_ids_dev, grad_top_dev, nullptr, dx_row_stride};
-        return launch_grad<T>(x_dev, dx_dev, p, rows, static_cast<cudaStream_t>(stream));
+        GradParams<T> p{static_cast<const T*>(x_dev), row_stride, vocab, scale, targets_dev, target_dtype == MHLO_DT_I64, lse_dev, entropy_dev, grad_logprobs_dev, grad_entropy_dev,
+                        grad_top_dev ? top_k : 0, top_ids_dev, grad_top_dev, static_cast<T*>(dx_dev), dx_row_stride};
+        return launch_grad<T>(p, rows, static_cast<cudaStream_t>(stream));
     };
     if (dtype == MHLO_DT_F32) return run(float{});
     if (dtype == MHLO_DT_F16) return run(__half{});
