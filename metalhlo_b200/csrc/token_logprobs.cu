@@ -46,6 +46,7 @@ struct LogprobParams {
     int32_t top_k;
     float* top_logprobs;
     int32_t* top_ids;
+    int32_t log2_parts;  // CTAs that share a row
 };
 
 __device__ __forceinline__ int64_t target_of(const void* targets, int32_t wide, int64_t row) {
@@ -96,22 +97,54 @@ __device__ __forceinline__ float largest_of(const uint4& v) {
     }
 }
 
+// Raises elements to `span` below the maximum m or a step of the type further down. NaN stays. Where the type has no number that far
+// below m (m next to its lowest number, or its steps at m not fine enough for fp32 to tell), below() is less than span.
+template <typename T>
+struct Floor {
+    T low;
+    float m;
+    __device__ __forceinline__ Floor(float m_, float span) : m(m_) {
+        if constexpr (sizeof(T) == 4) low = fmaxf(m - span, -3.4028235e38f);
+        else if constexpr (std::is_same<T, __half>::value) low = __float2half_rd(fmaxf(m - span, -65504.f));
+        else low = __float2bfloat16_rd(fmaxf(m - span, -3.3895314e38f));
+    }
+    __device__ __forceinline__ float below() const { return m - VecTraits<T>::to_float(low); }
+    __device__ __forceinline__ uint4 raise(const uint4& v) const {
+        if constexpr (sizeof(T) == 4) {
+            return make_uint4(__float_as_uint(max_nan(__uint_as_float(v.x), low)), __float_as_uint(max_nan(__uint_as_float(v.y), low)),
+                              __float_as_uint(max_nan(__uint_as_float(v.z), low)), __float_as_uint(max_nan(__uint_as_float(v.w), low)));
+        } else {
+            uint4 out = v;
+            if constexpr (std::is_same<T, __half>::value) {
+                __half2* h = reinterpret_cast<__half2*>(&out);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], __half2half2(low));
+            } else {
+                __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&out);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = __hmax2_nan(h[i], __bfloat162bfloat162(low));
+            }
+            return out;
+        }
+    }
+};
+
 // A row as up to E - 1 elements in front of the first 16-byte boundary, vectors, and up to E - 1 elements behind the last one.
 template <typename T>
 struct Row {
     const T* x;
-    int64_t vectors;
+    uint32_t vectors;  // rows have fewer than 2^31 elements
     int32_t head, tail;
     __device__ __forceinline__ Row(const T* row, int64_t n) : x(row) {
         constexpr int E = VecTraits<T>::kElems;
         const int64_t off = static_cast<int64_t>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / static_cast<int64_t>(sizeof(T));
         head = static_cast<int32_t>(off < n ? off : n);
-        vectors = (n - head) / E;
-        tail = static_cast<int32_t>(n - head - vectors * E);
+        vectors = static_cast<uint32_t>(n - head) / E;
+        tail = static_cast<int32_t>(static_cast<uint32_t>(n - head) % E);
     }
     __device__ __forceinline__ int32_t singles() const { return head + tail; }
-    __device__ __forceinline__ int64_t place_of_single(int32_t i) const { return i < head ? i : vectors * VecTraits<T>::kElems + i; }
-    __device__ __forceinline__ int64_t place(int64_t vector) const { return head + vector * VecTraits<T>::kElems; }
+    __device__ __forceinline__ int64_t place_of_single(int32_t i) const { return i < head ? i : static_cast<int64_t>(vectors) * VecTraits<T>::kElems + i; }
+    __device__ __forceinline__ int64_t place(uint32_t vector) const { return head + static_cast<int64_t>(vector) * VecTraits<T>::kElems; }
 };
 
 // The kept keys' ranks among `n` in shared memory: those below k go to list[rank]. All threads call it.
@@ -127,20 +160,22 @@ __device__ __forceinline__ void take_largest(const Key* keys, int n, int k, Key*
 
 // CTAs of a cluster share a row (clusters of 1 to 8, along x): the first one joins them.
 template <typename T, bool TOP, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const __grid_constant__ LogprobParams<T> p) {
-    constexpr int E = VecTraits<T>::kElems, kWarps = THREADS / 32;
+__global__ void __launch_bounds__(THREADS, (TOP ? 1024 : 1536) / THREADS) logprobs_kernel(const __grid_constant__ LogprobParams<T> p) {
+    constexpr int E = VecTraits<T>::kElems;
     __shared__ float scratch[3][32];
     __shared__ float joined[4];  // maximum, S, T of this CTA
     __shared__ Key list[TOP ? kList : 1], group[TOP ? THREADS : 1], best[TOP ? MHLO_CUDA_TOP_LOGPROBS_MAX : 1], bound_shared;
     __shared__ int listed;
     grid_dependency_wait();
     cg::cluster_group cluster = cg::this_cluster();
-    const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
-    const int64_t row = blockIdx.x / parts;
+    const int parts = 1 << p.log2_parts;
+    const uint32_t part = blockIdx.x & (parts - 1);
+    const int64_t row = blockIdx.x >> p.log2_parts;
     const Row<T> r(p.x + row * p.row_stride, p.vocab);
-    const int64_t v0 = r.vectors * part / parts, v1 = r.vectors * (part + 1) / parts;
+    const uint32_t v0 = static_cast<uint32_t>(static_cast<uint64_t>(r.vectors) * part >> p.log2_parts);
+    const uint32_t v1 = static_cast<uint32_t>(static_cast<uint64_t>(r.vectors) * (part + 1) >> p.log2_parts);
     const uint4* const vectors = reinterpret_cast<const uint4*>(r.x + r.head);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x;
     const float c = p.scale * 1.4426950408889634f;
 
     float m = -INFINITY, s = 0.f, t = 0.f;
@@ -148,55 +183,69 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logprobs_kernel(const
     int kept = 0;  // keys on the list before this batch
     if (TOP && tid == 0) listed = 0;
     bool first = true;
-    for (int64_t base = v0; first || base < v1; base += THREADS * kBatch) {
+    for (uint32_t base = v0; first || base < v1; base += THREADS * kBatch) {
         uint4 raw[kBatch];
         float single = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int64_t v = base + tid + i * THREADS;
+            const uint32_t v = base + tid + i * THREADS;
             raw[i] = v < v1 ? ld_stream16(vectors + v) : all_lowest<T>();
         }
         const bool has_single = first && part == 0 && tid < r.singles();
         if (has_single) single = VecTraits<T>::to_float(r.x[r.place_of_single(tid)]);
         float most = single;
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) most = max_nan(most, largest_of<T>(raw[i]));
+        for (int i = 0; i < kBatch; ++i) {
+            if (base + i * THREADS >= v1) break;
+            most = max_nan(most, largest_of<T>(raw[i]));
+        }
         if (most > m) {
             const float delta = fmaxf((m - most) * c, kLowest), f = ex2(delta);
             t = f * fmaf(s, delta, t);
             s *= f;
             m = most;
         }
-        const float from = m == -INFINITY ? 0.f : m;
-        const float2 minus = make_float2(-from, -from), by = make_float2(c, c);
-        float2 s2 = make_float2(0.f, 0.f), t2 = make_float2(0.f, 0.f);
+        if (m == -INFINITY) {  // nothing but -infinities so far, or a NaN
+            if (most != most) s = most;
+        } else {
+            // Elements so far below the maximum that their exponential is 0 are kept above -infinity, so that 0 * -infinity never
+            // comes up: 16-bit types two at a time before they are widened.
+            const Floor<T> floor(m, -kLowest / c);
+            const bool by_two = floor.below() * c >= 100.f;  // 2^-100 of 2^31 elements are still nothing beside the maximum's 1
+            const float2 minus = make_float2(-m, -m), by = make_float2(c, c);
+            float2 s2 = make_float2(0.f, 0.f), t2 = make_float2(0.f, 0.f);
+            auto add_vectors = [&](auto two) {
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            float2 f[E / 2];
-            VecTraits<T>::unpack2(raw[i], f);
+                for (int i = 0; i < kBatch; ++i) {
+                    if (base + i * THREADS >= v1) break;
+                    float2 f[E / 2];
+                    VecTraits<T>::unpack2(decltype(two)::value ? floor.raise(raw[i]) : raw[i], f);
 #pragma unroll
-            for (int e = 0; e < E / 2; ++e) {
-                float2 d = __fmul2_rn(__fadd2_rn(f[e], minus), by);
-                d.x = max_nan(d.x, kLowest);
-                d.y = max_nan(d.y, kLowest);
-                const float2 w = make_float2(ex2(d.x), ex2(d.y));
-                s2 = __fadd2_rn(s2, w);
-                t2 = __ffma2_rn(w, d, t2);
+                    for (int e = 0; e < E / 2; ++e) {
+                        float2 d = __fmul2_rn(__fadd2_rn(f[e], minus), by);
+                        if (!decltype(two)::value) d = make_float2(max_nan(d.x, kLowest), max_nan(d.y, kLowest));
+                        const float2 w = make_float2(ex2(d.x), ex2(d.y));
+                        s2 = __fadd2_rn(s2, w);
+                        t2 = __ffma2_rn(w, d, t2);
+                    }
+                }
+            };
+            if (by_two) add_vectors(std::true_type{});
+            else add_vectors(std::false_type{});
+            if (has_single) {
+                const float d = max_nan((single - m) * c, kLowest), w = ex2(d);
+                s2.x += w;
+                t2.x = fmaf(w, d, t2.x);
             }
+            s += s2.x + s2.y;
+            t += t2.x + t2.y;
         }
-        if (has_single) {
-            const float d = max_nan((single - from) * c, kLowest), w = ex2(d);
-            s2.x += w;
-            t2.x = fmaf(w, d, t2.x);
-        }
-        s += s2.x + s2.y;
-        t += t2.x + t2.y;
 
         if constexpr (TOP) {
             auto each_key = [&](auto&& use) {  // this thread's keys of the batch
 #pragma unroll
                 for (int i = 0; i < kBatch; ++i) {
-                    const int64_t v = base + tid + i * THREADS;
+                    const uint32_t v = base + tid + i * THREADS;
                     if (v >= v1) continue;
                     float f[E];
                     VecTraits<T>::unpack(raw[i], f);
@@ -376,16 +425,16 @@ __global__ void __launch_bounds__(THREADS) logprobs_grad_kernel(const __grid_con
     const float picked = g * p.scale;
     const bool together = ((reinterpret_cast<uintptr_t>(r.x) ^ reinterpret_cast<uintptr_t>(dx)) & 15) == 0;  // both rows' vectors on the grid
     const uint4* const vectors = reinterpret_cast<const uint4*>(r.x + r.head);
-    for (int64_t base = 0; base < r.vectors; base += THREADS * kBatch) {
+    for (uint32_t base = 0; base < r.vectors; base += THREADS * kBatch) {
         uint4 raw[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int64_t v = base + tid + i * THREADS;
+            const uint32_t v = base + tid + i * THREADS;
             if (v < r.vectors) raw[i] = __ldcs(vectors + v);
         }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int64_t v = base + tid + i * THREADS;
+            const uint32_t v = base + tid + i * THREADS;
             if (v >= r.vectors) break;
             float f[E];
             VecTraits<T>::unpack(raw[i], f);
@@ -435,10 +484,14 @@ int check_rows(const char* what, int32_t dtype, const void* x, int64_t row_strid
 inline bool short_rows(int64_t vocab, int64_t size) { return vocab * size <= 16 * 512; }
 
 template <typename T, bool TOP>
-int launch(const LogprobParams<T>& p, int64_t rows, cudaStream_t stream) {
+int launch(LogprobParams<T> p, int64_t rows, cudaStream_t stream) {
     // Few long rows are shared by clusters of CTAs, as long as a thread gets two vectors of its own.
     int parts = 1;
-    while (parts < 8 && rows * parts * 2 <= kNumSMs && p.vocab * static_cast<int64_t>(sizeof(T)) >= int64_t{16} * 512 * 2 * parts * 2) parts *= 2;
+    p.log2_parts = 0;
+    while (parts < 8 && rows * parts * 2 <= kNumSMs && p.vocab * static_cast<int64_t>(sizeof(T)) >= int64_t{16} * 512 * 2 * parts * 2) {
+        parts *= 2;
+        ++p.log2_parts;
+    }
     if (rows * parts > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "token_logprobs: too many rows");
     const dim3 grid(static_cast<unsigned>(rows * parts));
     const cudaError_t e = short_rows(p.vocab, sizeof(T)) ? launch_dependent(logprobs_kernel<T, TOP, 128>, grid, dim3(128), 0, stream, 1, rows < kNumSMs, p)
@@ -473,7 +526,7 @@ int mhlo_cuda_token_logprobs(int32_t dtype, const void* x_dev, int64_t row_strid
     if (top_k > 0 && (!top_logprobs_dev || !top_ids_dev)) return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: null result for the alternatives", what);
     auto run = [&](auto zero) {
         using T = decltype(zero);
-        LogprobParams<T> p{static_cast<const T*>(x_dev), row_stride, vocab, scale, targets_dev, target_dtype == MHLO_DT_I64, logprobs_dev, entropy_dev, lse_dev, top_k, top_logprobs_dev, top_ids_dev};
+        LogprobParams<T> p{static_cast<const T*>(x_dev), row_stride, vocab, scale, targets_dev, target_dtype == MHLO_DT_I64, logprobs_dev, entropy_dev, lse_dev, top_k, top_logprobs_dev, top_ids_dev, 0};
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         return top_k > 0 ? launch<T, true>(p, rows, st) : launch<T, false>(p, rows, st);
     };

@@ -109,6 +109,44 @@ def test_masked_and_broken_rows(dtype, vocab):
     assert bool((r.top_logprobs[4, 1:] == -inf).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("vocab", [100, 20001])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -12, 3.0])
+def test_rows_far_from_zero(dtype, vocab, scale):
+    """Maxima whose type has steps wider than any exponent that counts, next to the lowest number, and all equal there; every other
+    entry is a step or much more below the maximum, or -infinity."""
+    cuda = cuda_mod()
+    big = {torch.float16: 60000.0, torch.bfloat16: 1e5, torch.float32: 1e12}[dtype]
+    least = torch.finfo(dtype).min
+    x = torch.full((8, vocab), -float("inf"), dtype=torch.float32)
+    x[0], x[0, 3] = -big, big
+    x[1], x[1, 3] = big * (1 - torch.finfo(dtype).eps), big  # next number but one below, or the one below
+    x[2], x[2, 3], x[2, 4] = 0.0, -big, 1.0
+    x[3] = least
+    x[4, :50] = least
+    x[5], x[5, 7] = least, least * (1 - torch.finfo(dtype).eps)
+    x[6, 5], x[6, 9] = -big, -big
+    x[7] = big
+    x = x.to(dtype)
+    t = torch.full((8,), 3)
+    r = cuda.token_logprobs(x.cuda(), t.cuda(), scale=scale)
+    z = x.double() * scale
+    m = z.amax(1, keepdim=True)
+    d = z - m
+    log_s = torch.exp(d).sum(1).log()
+    p = torch.exp(d - log_s[:, None])
+    entropy = log_s - torch.where(p > 0, p * d, torch.zeros_like(p)).sum(1)
+    # Relative to the maximum everything is as exact as anywhere: (x - max) scale is one rounding of the difference and one of the
+    # product, and differences of equal or neighbouring numbers are exact.
+    order = (vocab / 128 + 32) * U
+    want = d.gather(1, t[:, None])[:, 0] - log_s
+    got = r.logprobs.cpu().double()
+    assert bool((torch.isinf(want) == torch.isinf(got)).all())
+    off = torch.where(torch.isinf(want), torch.zeros_like(want), (got - want).abs())
+    assert bool((off <= order + 2.0 ** -20 + 4 * U * torch.where(torch.isinf(want), torch.zeros_like(want), want.abs())).all())
+    assert bool(((r.entropy.cpu() - entropy).abs() <= order * (1 + entropy.abs()) + 2.0 ** -18).all())
+
+
 def test_targets_that_name_no_token():
     cuda = cuda_mod()
     x, t = draw(5, 77, torch.float32, 4)
