@@ -11,9 +11,10 @@
 //
 // Alternatives come out of the same pass. Keys are 64 bits, the logit's order above the complement of its place, so no two are equal
 // and ties go to the lowest id. After the first batch the k-th largest of 64 groups' maxima bounds the k-th largest key from below;
-// from then on only elements above the bound, some dozens of a row, are put on a list. When a batch would overflow the list (rising
-// logits), the list is cut to its k largest and the bound raised by that batch's own maxima, at last by those of single threads: then
-// at most k threads have anything to add.
+// from then on only elements above the bound, some dozens of a row, are put on a list, and the threads never wait for one another.
+// Rows that overflow the list (rising logits) are gone over once more batch by batch: when a batch overflows it, the list is cut to
+// its k largest and the bound raised by that batch's own maxima, at last by those of single threads: then at most k threads have
+// anything to add.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -69,6 +70,9 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     if (x != x) return 0xffffffffu;
     const uint32_t u = __float_as_uint(x + 0.f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float number_of(uint32_t order) {  // back again; NaN for NaN's and for 0, which is no number's
+    return __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order);
 }
 __device__ __forceinline__ Key key_of(float x, uint32_t place) { return static_cast<Key>(order_of(x)) << 32 | (0xffffffffu - place); }
 
@@ -178,27 +182,82 @@ __global__ void __launch_bounds__(THREADS, (TOP ? 1024 : 1536) / THREADS) logpro
     const int tid = threadIdx.x;
     const float c = p.scale * 1.4426950408889634f;
 
-    float m = -INFINITY, s = 0.f, t = 0.f;
-    Key bound = 0;
-    int kept = 0;  // keys on the list before this batch
-    if (TOP && tid == 0) listed = 0;
-    bool first = true;
-    for (uint32_t base = v0; first || base < v1; base += THREADS * kBatch) {
-        uint4 raw[kBatch];
-        float single = -INFINITY;
+    // this thread's part of the batch of vectors that begins at `base`; returns the largest element
+    auto load = [&](uint4* raw, uint32_t base, bool has_single, float* single) {
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             const uint32_t v = base + tid + i * THREADS;
             raw[i] = v < v1 ? ld_stream16(vectors + v) : all_lowest<T>();
         }
-        const bool has_single = first && part == 0 && tid < r.singles();
-        if (has_single) single = VecTraits<T>::to_float(r.x[r.place_of_single(tid)]);
-        float most = single;
+        *single = has_single ? VecTraits<T>::to_float(r.x[r.place_of_single(tid)]) : -INFINITY;
+        float most = *single;
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             if (base + i * THREADS >= v1) break;
             most = max_nan(most, largest_of<T>(raw[i]));
         }
+        return most;
+    };
+    Key bound = 0;
+    if (TOP && tid == 0) listed = 0;
+    // The bound from the maxima of `groups` groups of neighbouring threads: the k-th largest of them.
+    auto raise_bound = [&](const uint4* raw, uint32_t base, bool has_single, float single, float most, int groups) {
+        uint32_t place = 0xffffffffu;  // the first place of this thread's largest element
+#pragma unroll
+        for (int i = kBatch - 1; i >= 0; --i) {
+            const uint32_t v = base + tid + i * THREADS;
+            if (v >= v1) continue;
+            float f[E];
+            VecTraits<T>::unpack(raw[i], f);
+#pragma unroll
+            for (int e = E - 1; e >= 0; --e)
+                if (f[e] == most || f[e] != f[e]) place = static_cast<uint32_t>(r.place(v) + e);
+        }
+        if (has_single && (single == most || single != single)) place = min(place, static_cast<uint32_t>(r.place_of_single(tid)));
+        Key mine = place == 0xffffffffu ? 0 : key_of(most, place);
+        const int width = THREADS / groups;
+        for (int o = 1; o < width; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+        if (tid % width == 0) group[tid / width] = mine;
+        if (tid == 0) bound_shared = 0;
+        __syncthreads();
+        for (int i = tid; i < groups; i += THREADS) {
+            const Key own = group[i];
+            int rank = 0;
+            for (int j = 0; j < groups; ++j) rank += group[j] > own || (group[j] == own && j < i);  // empty groups are equal
+            if (rank == p.top_k - 1) bound_shared = own;
+        }
+        __syncthreads();
+        bound = max(bound, bound_shared);
+    };
+    auto put = [&](Key key) {
+        if (key < bound) return;
+        const int at = atomicAdd(&listed, 1);
+        if (at < kList) list[at] = key;
+    };
+    // Elements not below the bound go on the list. Numbers are compared first: a key costs several instructions.
+    auto add = [&](const uint4* raw, uint32_t base, bool has_single, float single, float most) {
+        const float least = number_of(static_cast<uint32_t>(bound >> 32));
+        if (most < least) return;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const uint32_t v = base + tid + i * THREADS;
+            if (v >= v1) continue;
+            float f[E];
+            VecTraits<T>::unpack(raw[i], f);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (!(f[e] < least)) put(key_of(f[e], static_cast<uint32_t>(r.place(v) + e)));
+        }
+        if (has_single && !(single < least)) put(key_of(single, static_cast<uint32_t>(r.place_of_single(tid))));
+    };
+
+    float m = -INFINITY, s = 0.f, t = 0.f;
+    bool first = true;
+    for (uint32_t base = v0; first || base < v1; base += THREADS * kBatch) {
+        uint4 raw[kBatch];
+        float single;
+        const bool has_single = first && part == 0 && tid < r.singles();
+        const float most = load(raw, base, has_single, &single);
         if (most > m) {
             const float delta = fmaxf((m - most) * c, kLowest), f = ex2(delta);
             t = f * fmaf(s, delta, t);
@@ -242,66 +301,47 @@ __global__ void __launch_bounds__(THREADS, (TOP ? 1024 : 1536) / THREADS) logpro
         }
 
         if constexpr (TOP) {
-            auto each_key = [&](auto&& use) {  // this thread's keys of the batch
-#pragma unroll
-                for (int i = 0; i < kBatch; ++i) {
-                    const uint32_t v = base + tid + i * THREADS;
-                    if (v >= v1) continue;
-                    float f[E];
-                    VecTraits<T>::unpack(raw[i], f);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) use(key_of(f[e], static_cast<uint32_t>(r.place(v) + e)));
-                }
-                if (has_single) use(key_of(single, static_cast<uint32_t>(r.place_of_single(tid))));
-            };
-            // The bound from the maxima of `groups` groups of neighbouring threads: the k-th largest of them.
-            auto raise_bound = [&](int groups) {
-                Key mine = 0;
-                each_key([&](Key key) { mine = max(mine, key); });
-                const int width = THREADS / groups;
-                for (int o = 1; o < width; o <<= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-                if (tid % width == 0) group[tid / width] = mine;
-                if (tid == 0) bound_shared = 0;
-                __syncthreads();
-                for (int i = tid; i < groups; i += THREADS) {
-                    const Key own = group[i];
-                    int rank = 0;
-                    for (int j = 0; j < groups; ++j) rank += group[j] > own || (group[j] == own && j < i);  // empty groups are equal
-                    if (rank == p.top_k - 1) bound_shared = own;
-                }
-                __syncthreads();
-                bound = max(bound, bound_shared);
-            };
-            auto add = [&]() {
-                if (order_of(most) < static_cast<uint32_t>(bound >> 32)) return;
-                each_key([&](Key key) {
-                    if (key < bound) return;
-                    const int at = atomicAdd(&listed, 1);
-                    if (at < kList) list[at] = key;
-                });
-            };
-            if (first) raise_bound(kGroups);
-            add();
-            __syncthreads();
-            for (int groups = kGroups; listed > kList; groups = THREADS) {  // too many: at most twice
-                __syncthreads();
-                if (kept > p.top_k) {  // earlier batches' keys, cut to the k largest
-                    take_largest<THREADS>(list, kept, p.top_k, best);
-                    __syncthreads();
-                    if (tid < p.top_k) list[tid] = best[tid];
-                    kept = p.top_k;
-                }
-                if (tid == 0) listed = kept;
-                raise_bound(groups);
-                add();
-                __syncthreads();
-            }
-            kept = listed;
-            __syncthreads();  // everybody has read it
+            if (first) raise_bound(raw, base, has_single, single, most, kGroups);
+            add(raw, base, has_single, single, most);
         }
         first = false;
     }
 
+    int kept = 0;  // keys on the list
+    if constexpr (TOP) {
+        __syncthreads();
+        if (listed > kList) {
+            __syncthreads();
+            if (tid == 0) listed = 0;
+            __syncthreads();
+            first = true;
+            for (uint32_t base = v0; first || base < v1; base += THREADS * kBatch) {
+                uint4 raw[kBatch];
+                float single;
+                const bool has_single = first && part == 0 && tid < r.singles();
+                const float most = load(raw, base, has_single, &single);
+                add(raw, base, has_single, single, most);
+                __syncthreads();
+                for (int groups = kGroups; listed > kList; groups = THREADS) {  // at most twice
+                    __syncthreads();
+                    if (kept > p.top_k) {  // earlier batches' keys, cut to the k largest
+                        take_largest<THREADS>(list, kept, p.top_k, best);
+                        __syncthreads();
+                        if (tid < p.top_k) list[tid] = best[tid];
+                        kept = p.top_k;
+                    }
+                    if (tid == 0) listed = kept;
+                    raise_bound(raw, base, has_single, single, most, groups);
+                    add(raw, base, has_single, single, most);
+                    __syncthreads();
+                }
+                kept = listed;
+                __syncthreads();  // everybody has read it
+                first = false;
+            }
+        }
+        kept = listed;
+    }
     const float top = cta_reduce<MaxOp>(m, scratch[0]), from = top == -INFINITY ? 0.f : top;
     const float delta = fmaxf((m - from) * c, kLowest), f = ex2(delta);
     const float all_t = cta_reduce<SumOp>(f * fmaf(s, delta, t), scratch[1]);
@@ -483,6 +523,9 @@ int check_rows(const char* what, int32_t dtype, const void* x, int64_t row_strid
 // Short rows take CTAs of 128 threads: a row of 100 logits keeps 13 to 25 of them busy.
 inline bool short_rows(int64_t vocab, int64_t size) { return vocab * size <= 16 * 512; }
 
+// Threads of a row's CTA. What a warp spends on a row beside its elements (joining the threads, the ragged ends) is a few hundred
+// instructions, so with rows enough to fill the machine several times a CTA is small: [4096, 50257] bf16 95 us with 512 threads, 82
+// with 256, 79 with 128. The alternatives' first bound wants a large batch: 256.
 template <typename T, bool TOP>
 int launch(LogprobParams<T> p, int64_t rows, cudaStream_t stream) {
     // Few long rows are shared by clusters of CTAs, as long as a thread gets two vectors of its own.
@@ -493,9 +536,10 @@ int launch(LogprobParams<T> p, int64_t rows, cudaStream_t stream) {
         ++p.log2_parts;
     }
     if (rows * parts > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "token_logprobs: too many rows");
-    const dim3 grid(static_cast<unsigned>(rows * parts));
-    const cudaError_t e = short_rows(p.vocab, sizeof(T)) ? launch_dependent(logprobs_kernel<T, TOP, 128>, grid, dim3(128), 0, stream, 1, rows < kNumSMs, p)
-                                                         : launch_dependent(logprobs_kernel<T, TOP, 512>, grid, dim3(512), 0, stream, parts, rows * parts < kNumSMs, p);
+    const bool small = short_rows(p.vocab, sizeof(T)) || (!TOP && rows >= 8 * kNumSMs), large = rows < 2 * kNumSMs;
+    const int threads = small ? 128 : large ? 512 : 256;
+    const auto kernel = small ? logprobs_kernel<T, TOP, 128> : large ? logprobs_kernel<T, TOP, 512> : logprobs_kernel<T, TOP, 256>;
+    const cudaError_t e = launch_dependent(kernel, dim3(static_cast<unsigned>(rows * parts)), dim3(threads), 0, stream, parts, rows * parts < kNumSMs, p);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of token_logprobs failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("token_logprobs");
     return MHLO_CUDA_OK;
@@ -504,7 +548,7 @@ int launch(LogprobParams<T> p, int64_t rows, cudaStream_t stream) {
 template <typename T>
 int launch_grad(const GradParams<T>& p, int64_t rows, cudaStream_t stream) {
     if (short_rows(p.vocab, sizeof(T))) logprobs_grad_kernel<T, 128><<<static_cast<unsigned>(rows), 128, 0, stream>>>(p);
-    else logprobs_grad_kernel<T, 512><<<static_cast<unsigned>(rows), 512, 0, stream>>>(p);
+    else logprobs_grad_kernel<T, 256><<<static_cast<unsigned>(rows), 256, 0, stream>>>(p);
     MHLO_CUDA_CHECK_LAUNCH("token_logprobs_grad");
     return MHLO_CUDA_OK;
 }
