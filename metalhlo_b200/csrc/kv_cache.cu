@@ -29,7 +29,8 @@ struct AppendParams {
     int64_t rope_positions;
     int32_t rotary_dim, interleaved, q_heads;
     int32_t vec[4];      // k, v, q, q_out: rows on the 16-byte grid
-    FastDiv units;       // units of a row
+    FastDiv units, heads;  // units of a row of a head, query heads
+    int32_t rows;          // of queries to a CTA
     int64_t blocks;      // CTAs that append, a block of keys or values each; the CTAs behind them rotate queries
 };
 
@@ -98,33 +99,54 @@ __device__ __forceinline__ const float* rope_row(const AppendParams<T>& p, int32
 
 constexpr int kKeep = 4;  // units a thread keeps in registers between the maximum and the codes
 
+// Queries: a CTA takes p.rows rows, kKeep units a thread. Their elements are on the way before the rows' sequences are looked up: three
+// dependent reads of a few bytes each, which otherwise stood in front of every CTA's loads ([4400, 32, 128] bf16: 41 us).
+constexpr int kMostRows = 32;
+
 template <typename T>
-__device__ __forceinline__ void rotate_row(const AppendParams<T>& p, int32_t row) {
+__device__ __forceinline__ void rotate_rows(const AppendParams<T>& p, int32_t first_row) {
     const KvArgs& a = p.kv;
-    int32_t b = row;
-    if (a.starts != nullptr) b = kv_search(a.seqs, row, [&](int32_t i) { return static_cast<int64_t>(a.starts[i]); });
-    const KvSequence s = kv_sequence(a, b);
-    if (s.length == 0 || row < s.first || row >= s.first + s.count) return;
-    const float* const rope = rope_row(p, s.position(row));
-    const int32_t threads = blockDim.x, all = p.q_heads * static_cast<int32_t>(p.units.d);
-    float cs[8], sn[8];
-    int32_t have = -1;  // the unit whose cosines and sines are loaded: the same every time where the units of a row divide the threads
-    for (int32_t i = threadIdx.x; i < all; i += threads) {
-        const int32_t head = static_cast<int32_t>(p.units.div(i)), unit = i - head * static_cast<int32_t>(p.units.d);
-        const Unit u = unit_at(unit, p.rotary_dim, p.interleaved);
-        const T* const x = p.q + row * p.qs[0] + head * p.qs[1];
-        float f[16];
-        load8(x + u.low, p.vec[2], f);
-        load8(x + u.high, p.vec[2], f + 8);
-        if (u.rotated) {
-            if (have != unit) load_turn(rope, unit, p.rotary_dim, cs, sn);
-            have = unit;
-            if (p.interleaved) turn(f, cs, sn, 1);
-            else turn(f, cs, sn, 0);
+    __shared__ int32_t position[kMostRows];  // -1: the row is of no sequence
+    const int32_t rows = min(p.rows, a.tokens - first_row), threads = blockDim.x, d = static_cast<int32_t>(p.units.d), all = rows * p.q_heads * d;
+    for (int32_t start = 0; start < all; start += kKeep * threads) {
+        float f[kKeep][16];
+        int32_t row[kKeep], head[kKeep], unit[kKeep];
+#pragma unroll
+        for (int k = 0; k < kKeep; ++k) {
+            const int32_t i = start + threadIdx.x + k * threads, column = static_cast<int32_t>(p.units.div(i));
+            unit[k] = i - column * d;
+            row[k] = i < all ? static_cast<int32_t>(p.heads.div(column)) : -1;
+            head[k] = column - row[k] * p.q_heads;
+            if (row[k] < 0) continue;
+            const Unit u = unit_at(unit[k], p.rotary_dim, p.interleaved);
+            const T* const x = p.q + static_cast<int64_t>(first_row + row[k]) * p.qs[0] + head[k] * p.qs[1];
+            load8(x + u.low, p.vec[2], f[k]);
+            load8(x + u.high, p.vec[2], f[k] + 8);
         }
-        T* const y = p.q_out + row * p.os[0] + head * p.os[1];
-        store8(y + u.low, p.vec[3], f);
-        store8(y + u.high, p.vec[3], f + 8);
+        if (start == 0) {
+            for (int32_t i = threadIdx.x >> 5; i < rows; i += threads >> 5) {  // a warp per row
+                const int32_t r = first_row + i;
+                int32_t b = r;
+                if (a.starts != nullptr) b = kv_search(a.seqs, r, [&](int32_t j) { return static_cast<int64_t>(a.starts[j]); });
+                const KvSequence s = kv_sequence(a, b);
+                if ((threadIdx.x & 31) == 0) position[i] = s.length == 0 || r < s.first || r >= s.first + s.count ? -1 : s.position(r);
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int k = 0; k < kKeep; ++k) {
+            if (row[k] < 0 || position[row[k]] < 0) continue;
+            const Unit u = unit_at(unit[k], p.rotary_dim, p.interleaved);
+            if (u.rotated) {
+                float cs[8], sn[8];
+                load_turn(rope_row(p, position[row[k]]), unit[k], p.rotary_dim, cs, sn);
+                if (p.interleaved) turn(f[k], cs, sn, 1);
+                else turn(f[k], cs, sn, 0);
+            }
+            T* const y = p.q_out + static_cast<int64_t>(first_row + row[k]) * p.os[0] + head[k] * p.os[1];
+            store8(y + u.low, p.vec[3], f[k]);
+            store8(y + u.high, p.vec[3], f[k] + 8);
+        }
     }
 }
 
@@ -135,7 +157,7 @@ __device__ __forceinline__ uint32_t code_of(float x, float step) {
 template <typename T>
 __global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ AppendParams<T> p) {
     const KvArgs& a = p.kv;
-    if (blockIdx.x >= p.blocks) return rotate_row(p, static_cast<int32_t>(blockIdx.x - p.blocks));
+    if (blockIdx.x >= p.blocks) return rotate_rows(p, static_cast<int32_t>(blockIdx.x - p.blocks) * p.rows);
     // Block `slot` of the sequences' touched blocks. A sequence has n / P + 2 slots at least, as many as n tokens can touch:
     // slot of its first block = floor(first row / P) + 2 b.
     const int32_t which = static_cast<int32_t>(blockIdx.x & 1), head = static_cast<int32_t>((blockIdx.x >> 1) % a.heads);
@@ -153,16 +175,11 @@ __global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ App
     const int32_t page_index = ((s.length - s.count) >> a.page_shift) + nth, page_tokens = 1 << a.page_shift, dim = a.head_dim;
     const int32_t from = max(s.length - s.count, page_index << a.page_shift), to = min(s.length, (page_index + 1) << a.page_shift);
     if (from >= to) return;
-    const int32_t page = kv_page(a, b, page_index);
-    if (page < 0) return;
     const int32_t slot0 = from & (page_tokens - 1), row0 = from - (s.length - s.count) + s.first;
     const int32_t threads = blockDim.x, all = (to - from) * static_cast<int32_t>(p.units.d);
-    const int64_t block = static_cast<int64_t>(page) * a.heads + head, pitch = p.xs[which][0];
+    const int64_t pitch = p.xs[which][0];
     const T* const x = p.x[which] + row0 * pitch + head * p.xs[which][1];
-    int8_t* const codes = (which == 0 ? a.k_codes : a.v_codes) + block * page_tokens * dim;
-    float* const scales = (which == 0 ? a.k_scales : a.v_scales) + block;
     const int32_t rotary = which == 0 ? p.rotary_dim : 0;
-    const float before = slot0 == 0 ? 0.f : *scales;
 
     auto load_unit = [&](int32_t i, float* f) {
         const int32_t t = static_cast<int32_t>(p.units.div(i)), unit = i - t * static_cast<int32_t>(p.units.d);
@@ -195,6 +212,13 @@ __global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ App
         load_unit(i, f);
         largest_of(f);
     }
+    // only now the page: the elements are on the way meanwhile
+    const int32_t page = kv_page(a, b, page_index);
+    if (page < 0) return;
+    const int64_t block = static_cast<int64_t>(page) * a.heads + head;
+    int8_t* const codes = (which == 0 ? a.k_codes : a.v_codes) + block * page_tokens * dim;
+    float* const scales = (which == 0 ? a.k_scales : a.v_scales) + block;
+    const float before = slot0 == 0 ? 0.f : *scales;
     m = __reduce_max_sync(0xffffffffu, m);
     __shared__ uint32_t largest[16];
     if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = m;
@@ -320,11 +344,14 @@ int append(const KvArgs& kv, const void* k, const int64_t* ks, const void* v, co
     p.q_heads = static_cast<int32_t>(q_heads);
     p.units = FastDiv(static_cast<uint32_t>(kv.head_dim / 16));
     p.blocks = 2 * kv.heads * (kv.starts ? (static_cast<int64_t>(kv.tokens) >> kv.page_shift) + 2 * static_cast<int64_t>(kv.seqs) : kv.seqs);
-    const int64_t grid = p.blocks + (q ? kv.tokens : 0);
-    if (grid > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "kv_cache_append: too many blocks");
     // a whole block in the registers of a CTA, kKeep units a thread; single tokens need a warp or two
     const int units = (kv.starts ? 1 << kv.page_shift : 4) * (kv.head_dim / 16);
     const int threads = std::min(512, std::max(64, (units / kKeep + 31) / 32 * 32));
+    p.heads = FastDiv(static_cast<uint32_t>(std::max<int64_t>(1, q_heads)));
+    const int64_t row_units = std::max<int64_t>(1, q_heads * (kv.head_dim / 16));
+    p.rows = static_cast<int32_t>(std::min<int64_t>(kMostRows, std::max<int64_t>(1, kKeep * threads / row_units)));
+    const int64_t grid = p.blocks + (q ? (kv.tokens + p.rows - 1) / p.rows : 0);
+    if (grid > 0x7fffffff || q_heads * kMostRows * (kv.head_dim / 16) > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "kv_cache_append: too many blocks");
     append_kernel<T><<<static_cast<unsigned>(grid), threads, 0, stream>>>(p);
     MHLO_CUDA_CHECK_LAUNCH("kv_cache_append");
     return MHLO_CUDA_OK;

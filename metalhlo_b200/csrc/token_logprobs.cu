@@ -11,10 +11,12 @@
 //
 // Alternatives come out of the same pass. Keys are 64 bits, the logit's order above the complement of its place, so no two are equal
 // and ties go to the lowest id. After the first batch the k-th largest of 64 groups' maxima bounds the k-th largest key from below;
-// from then on only elements above the bound, some dozens of a row, are put on a list, and the threads never wait for one another.
-// Rows that overflow the list (rising logits) are gone over once more batch by batch: when a batch overflows it, the list is cut to
-// its k largest and the bound raised by that batch's own maxima, at last by those of single threads: then at most k threads have
-// anything to add.
+// from then on vectors whose maximum reaches the bound, some dozens to a few hundred of a row, are put on a list as they are, and the
+// threads never wait for one another (looking through a vector at once cost its warp more than the exponentials). At the end the
+// k-th largest maximum on the list is a bound again, and the keys of the vectors that reach it, hardly more than k, are ranked. Rows
+// that overflow the list (rising logits) are gone over once more batch by batch, with single keys on the list: when a batch
+// overflows it, it is cut to its k largest and the bound raised by that batch's own maxima, at last by those of single threads: then
+// at most k threads have anything to add.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -30,8 +32,14 @@ namespace {
 typedef unsigned long long Key;
 
 constexpr int kBatch = 4;     // vectors of a thread in flight
-constexpr int kGroups = 64;   // whose maxima give the first bound: twice the most alternatives
-constexpr int kList = 2048;   // keys
+// Groups of threads whose maxima give the first bound, and what the lists hold: keys (those of a batch at least, for as many threads
+// as there may be alternatives) and vectors. A warp by itself has short rows and needs little.
+template <int THREADS>
+struct Lists {
+    static constexpr int kGroups = THREADS < 64 ? THREADS : 64;
+    static constexpr int kKeys = THREADS < 64 ? 1152 : 2048;
+    static constexpr int kVectors = THREADS < 64 ? 128 : 512;
+};
 constexpr float kLowest = -150.f;  // 2^-150 is 0 in fp32: what exponents are kept above, so that 0 * -infinity never comes up
 
 template <typename T>
@@ -151,25 +159,36 @@ struct Row {
     __device__ __forceinline__ int64_t place(uint32_t vector) const { return head + static_cast<int64_t>(vector) * VecTraits<T>::kElems; }
 };
 
-// The kept keys' ranks among `n` in shared memory: those below k go to list[rank]. All threads call it.
+// How many of keys[0 .. n) are larger than `mine`: four neighbouring lanes share the count (all of a warp's lanes call it).
+__device__ __forceinline__ int larger_than(const Key* keys, int n, Key mine) {
+    int rank = 0;
+#pragma unroll 8
+    for (int j = threadIdx.x & 3; j < n; j += 4) rank += keys[j] > mine;
+    rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+    return rank + __shfl_xor_sync(0xffffffffu, rank, 2);
+}
+
+// The k largest of `n` keys in shared memory, in order. All threads call it.
 template <int THREADS>
 __device__ __forceinline__ void take_largest(const Key* keys, int n, int k, Key* list) {
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-        const Key mine = keys[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += keys[j] > mine;
-        if (rank < k) list[rank] = mine;
+    for (int base = 0; base < n; base += THREADS / 4) {
+        const int i = base + (threadIdx.x >> 2);
+        const Key mine = i < n ? keys[i] : 0;
+        const int rank = larger_than(keys, n, mine);
+        if (i < n && rank < k && mine != 0) list[rank] = mine;
     }
 }
 
 // CTAs of a cluster share a row (clusters of 1 to 8, along x): the first one joins them.
 template <typename T, bool TOP, int THREADS>
-__global__ void __launch_bounds__(THREADS, (TOP ? 1024 : 1536) / THREADS) logprobs_kernel(const __grid_constant__ LogprobParams<T> p) {
-    constexpr int E = VecTraits<T>::kElems;
+__global__ void __launch_bounds__(THREADS, (TOP || THREADS < 64 ? 1024 : 1536) / THREADS) logprobs_kernel(const __grid_constant__ LogprobParams<T> p) {
+    constexpr int E = VecTraits<T>::kElems, kGroups = Lists<THREADS>::kGroups, kList = Lists<THREADS>::kKeys, kVectors = Lists<THREADS>::kVectors;
     __shared__ float scratch[3][32];
     __shared__ float joined[4];  // maximum, S, T of this CTA
     __shared__ Key list[TOP ? kList : 1], group[TOP ? THREADS : 1], best[TOP ? MHLO_CUDA_TOP_LOGPROBS_MAX : 1], bound_shared;
-    __shared__ int listed;
+    __shared__ uint4 found[TOP ? kVectors : 1];
+    __shared__ uint32_t found_at[TOP ? kVectors : 1], found_order[TOP ? kVectors : 1], order_shared;
+    __shared__ int listed, keys_listed;
     grid_dependency_wait();
     cg::cluster_group cluster = cg::this_cluster();
     const int parts = 1 << p.log2_parts;
@@ -182,8 +201,8 @@ __global__ void __launch_bounds__(THREADS, (TOP ? 1024 : 1536) / THREADS) logpro
     const int tid = threadIdx.x;
     const float c = p.scale * 1.4426950408889634f;
 
-    // this thread's part of the batch of vectors that begins at `base`; returns the largest element
-    auto load = [&](uint4* raw, uint32_t base, bool has_single, float* single) {
+    // this thread's part of the batch of vectors that begins at `base`, with their maxima; returns the largest element
+    auto load = [&](uint4* raw, float* largest, uint32_t base, bool has_single, float* single) {
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             const uint32_t v = base + tid + i * THREADS;
@@ -193,8 +212,10 @@ __global__ void __launch_bounds__(THREADS, (TOP ? 1024 : 1536) / THREADS) logpro
         float most = *single;
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            if (base + i * THREADS >= v1) break;
-            most = max_nan(most, largest_of<T>(raw[i]));
+            largest[i] = -INFINITY;
+            if (base + i * THREADS >= v1) continue;
+            largest[i] = largest_of<T>(raw[i]);
+            most = max_nan(most, largest[i]);
         }
         return most;
     };
@@ -220,18 +241,33 @@ __global__ void __launch_bounds__(THREADS, (TOP ? 1024 : 1536) / THREADS) logpro
         if (tid % width == 0) group[tid / width] = mine;
         if (tid == 0) bound_shared = 0;
         __syncthreads();
-        for (int i = tid; i < groups; i += THREADS) {
-            const Key own = group[i];
-            int rank = 0;
-            for (int j = 0; j < groups; ++j) rank += group[j] > own || (group[j] == own && j < i);  // empty groups are equal
-            if (rank == p.top_k - 1) bound_shared = own;
+        for (int i = 0; i < groups; i += THREADS / 4) {
+            const Key own = i + (tid >> 2) < groups ? group[i + (tid >> 2)] : 0;
+            if (larger_than(group, groups, own) == p.top_k - 1 && own != 0) bound_shared = own;
         }
         __syncthreads();
         bound = max(bound, bound_shared);
     };
+    // The order of the k-th largest maximum on the list (0: there are fewer): another bound from below.
+    auto bound_of_list = [&](int n) {
+        if (tid == 0) order_shared = 0xffffffffu;
+        __syncthreads();
+        for (int from = 0; from < n; from += THREADS / 4) {
+            const int i = from + (tid >> 2);
+            const uint32_t own = i < n ? found_order[i] : 0;
+            int rank = 0;
+#pragma unroll 8
+            for (int j = tid & 3; j < n; j += 4) rank += found_order[j] > own;
+            rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+            rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+            if (i < n && rank < p.top_k) atomicMin(&order_shared, own);  // the least of those that fewer than k exceed
+        }
+        __syncthreads();
+        return n < p.top_k ? 0 : order_shared;
+    };
     auto put = [&](Key key) {
         if (key < bound) return;
-        const int at = atomicAdd(&listed, 1);
+        const int at = atomicAdd(&keys_listed, 1);
         if (at < kList) list[at] = key;
     };
     // Elements not below the bound go on the list. Numbers are compared first: a key costs several instructions.
@@ -253,11 +289,12 @@ __global__ void __launch_bounds__(THREADS, (TOP ? 1024 : 1536) / THREADS) logpro
 
     float m = -INFINITY, s = 0.f, t = 0.f;
     bool first = true;
+    int batches = 0;
     for (uint32_t base = v0; first || base < v1; base += THREADS * kBatch) {
         uint4 raw[kBatch];
-        float single;
+        float single, largest[kBatch];
         const bool has_single = first && part == 0 && tid < r.singles();
-        const float most = load(raw, base, has_single, &single);
+        const float most = load(raw, largest, base, has_single, &single);
         if (most > m) {
             const float delta = fmaxf((m - most) * c, kLowest), f = ex2(delta);
             t = f * fmaf(s, delta, t);
@@ -302,27 +339,70 @@ __global__ void __launch_bounds__(THREADS, (TOP ? 1024 : 1536) / THREADS) logpro
 
         if constexpr (TOP) {
             if (first) raise_bound(raw, base, has_single, single, most, kGroups);
-            add(raw, base, has_single, single, most);
+            const float least = number_of(static_cast<uint32_t>(bound >> 32));
+            if (!(most < least)) {
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const uint32_t v = base + tid + i * THREADS;
+                    // of a vector whose maximum equals the bound's number only places up to the bound's count
+                    if (largest[i] < least || v >= v1 || (largest[i] == least && static_cast<uint32_t>(r.place(v)) > ~static_cast<uint32_t>(bound))) continue;
+                    const int at = atomicAdd(&listed, 1);
+                    if (at < kVectors) {
+                        found[at] = raw[i];
+                        found_at[at] = static_cast<uint32_t>(r.place(v));
+                        found_order[at] = order_of(largest[i]);
+                    }
+                }
+            }
+        }
+        if constexpr (TOP) {  // each time the row has doubled the list bounds it anew: with it, k more vectors or so until it has doubled again
+            ++batches;
+            if ((batches & (batches - 1)) == 0 && batches > 1 && base + THREADS * kBatch < v1) {
+                __syncthreads();
+                const int n = min(listed, kVectors);
+                const uint32_t least = bound_of_list(n);
+                if (least > static_cast<uint32_t>(bound >> 32)) bound = static_cast<Key>(least) << 32;
+            }
         }
         first = false;
     }
 
     int kept = 0;  // keys on the list
     if constexpr (TOP) {
+        if (tid == 0) keys_listed = 0;
         __syncthreads();
-        if (listed > kList) {
+        const int n = listed;
+        if (n <= kVectors) {
+            const uint32_t least = bound_of_list(n);
+            for (int i = tid; i < n; i += THREADS) {
+                if (found_order[i] < least) continue;
+                float f[E];
+                VecTraits<T>::unpack(found[i], f);
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (order_of(f[e]) >= least) put(key_of(f[e], found_at[i] + e));
+            }
+            if (part == 0 && tid < r.singles()) {
+                const int64_t at = r.place_of_single(tid);
+                put(key_of(VecTraits<T>::to_float(r.x[at]), static_cast<uint32_t>(at)));
+            }
+        }
+        __syncthreads();
+        kept = keys_listed;
+        if (n > kVectors || kept > kList) {
             __syncthreads();
-            if (tid == 0) listed = 0;
+            kept = 0;
+            if (tid == 0) keys_listed = 0;
             __syncthreads();
             first = true;
             for (uint32_t base = v0; first || base < v1; base += THREADS * kBatch) {
                 uint4 raw[kBatch];
-                float single;
+                float single, largest[kBatch];
                 const bool has_single = first && part == 0 && tid < r.singles();
-                const float most = load(raw, base, has_single, &single);
+                const float most = load(raw, largest, base, has_single, &single);
                 add(raw, base, has_single, single, most);
                 __syncthreads();
-                for (int groups = kGroups; listed > kList; groups = THREADS) {  // at most twice
+                for (int groups = kGroups; keys_listed > kList; groups = THREADS) {  // at most twice
                     __syncthreads();
                     if (kept > p.top_k) {  // earlier batches' keys, cut to the k largest
                         take_largest<THREADS>(list, kept, p.top_k, best);
@@ -330,17 +410,16 @@ __global__ void __launch_bounds__(THREADS, (TOP ? 1024 : 1536) / THREADS) logpro
                         if (tid < p.top_k) list[tid] = best[tid];
                         kept = p.top_k;
                     }
-                    if (tid == 0) listed = kept;
+                    if (tid == 0) keys_listed = kept;
                     raise_bound(raw, base, has_single, single, most, groups);
                     add(raw, base, has_single, single, most);
                     __syncthreads();
                 }
-                kept = listed;
+                kept = keys_listed;
                 __syncthreads();  // everybody has read it
                 first = false;
             }
         }
-        kept = listed;
     }
     const float top = cta_reduce<MaxOp>(m, scratch[0]), from = top == -INFINITY ? 0.f : top;
     const float delta = fmaxf((m - from) * c, kLowest), f = ex2(delta);
@@ -520,12 +599,13 @@ int check_rows(const char* what, int32_t dtype, const void* x, int64_t row_strid
     return MHLO_CUDA_OK;
 }
 
-// Short rows take CTAs of 128 threads: a row of 100 logits keeps 13 to 25 of them busy.
+// Rows of up to 512 vectors: 4 batches of a warp.
 inline bool short_rows(int64_t vocab, int64_t size) { return vocab * size <= 16 * 512; }
 
 // Threads of a row's CTA. What a warp spends on a row beside its elements (joining the threads, the ragged ends) is a few hundred
 // instructions, so with rows enough to fill the machine several times a CTA is small: [4096, 50257] bf16 95 us with 512 threads, 82
-// with 256, 79 with 128. The alternatives' first bound wants a large batch: 256.
+// with 256, 79 with 128; short rows get a warp each ([32768, 1000] bf16 52 us with 128 threads, 20 with a warp). The
+// alternatives' first bound wants a large batch: 256.
 template <typename T, bool TOP>
 int launch(LogprobParams<T> p, int64_t rows, cudaStream_t stream) {
     // Few long rows are shared by clusters of CTAs, as long as a thread gets two vectors of its own.
@@ -536,9 +616,9 @@ int launch(LogprobParams<T> p, int64_t rows, cudaStream_t stream) {
         ++p.log2_parts;
     }
     if (rows * parts > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "token_logprobs: too many rows");
-    const bool small = short_rows(p.vocab, sizeof(T)) || (!TOP && rows >= 8 * kNumSMs), large = rows < 2 * kNumSMs;
-    const int threads = small ? 128 : large ? 512 : 256;
-    const auto kernel = small ? logprobs_kernel<T, TOP, 128> : large ? logprobs_kernel<T, TOP, 512> : logprobs_kernel<T, TOP, 256>;
+    const bool shortest = short_rows(p.vocab, sizeof(T)), small = !TOP && rows >= 8 * kNumSMs, large = rows < 2 * kNumSMs;
+    const int threads = shortest ? 32 : small ? 128 : large ? 512 : 256;
+    const auto kernel = shortest ? logprobs_kernel<T, TOP, 32> : small ? logprobs_kernel<T, TOP, TOP ? 256 : 128> : large ? logprobs_kernel<T, TOP, 512> : logprobs_kernel<T, TOP, 256>;
     const cudaError_t e = launch_dependent(kernel, dim3(static_cast<unsigned>(rows * parts)), dim3(threads), 0, stream, parts, rows * parts < kNumSMs, p);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of token_logprobs failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("token_logprobs");
@@ -547,7 +627,7 @@ int launch(LogprobParams<T> p, int64_t rows, cudaStream_t stream) {
 
 template <typename T>
 int launch_grad(const GradParams<T>& p, int64_t rows, cudaStream_t stream) {
-    if (short_rows(p.vocab, sizeof(T))) logprobs_grad_kernel<T, 128><<<static_cast<unsigned>(rows), 128, 0, stream>>>(p);
+    if (short_rows(p.vocab, sizeof(T))) logprobs_grad_kernel<T, 32><<<static_cast<unsigned>(rows), 32, 0, stream>>>(p);
     else logprobs_grad_kernel<T, 256><<<static_cast<unsigned>(rows), 256, 0, stream>>>(p);
     MHLO_CUDA_CHECK_LAUNCH("token_logprobs_grad");
     return MHLO_CUDA_OK;
