@@ -1,9 +1,5 @@
-// Attention of new tokens over the paged 8-bit key/value cache: o = softmax(scale q k^T) v with k = ks c, v = vs c.
-//
-// The work is cut into segments: (sequence, 8 or 16 rows, cache head). The rows of a segment are (token, query head) pairs that read the
-// same cache head: row r of a sequence is token r / group, query head head * group + r % group. A segment's keys are walked in tiles
-// of 32; CTAs share all tiles of the call evenly (Plan), so a CTA's piece may begin or end inside a segment. Whole segments are
-// written at once, pieces go to scratch as (maximum, sum, output) and a second kernel joins them in the order of the CTAs.
+// Attention of new tokens over the paged 8-bit key/value cache: o = softmax(scale q k^T) v with k = ks c, v = vs c. This is the kernel of
+// few rows; sequences with more go to cached_attention_tc.cu where that takes their type.
 //
 // Inside a CTA every warp takes tiles by itself and keeps a running maximum, sum and output of the rows; the warps are joined
 // through shared memory at the end of a segment. Nothing but the segment's end synchronises the warps.
@@ -14,14 +10,13 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "kv_cache.cuh"
+#include "cached_attention.cuh"
 
 namespace mhlo {
 namespace {
 
 constexpr int kTileKeys = 32;
 constexpr int kLeastTiles = 12;  // a CTA's share where there is little to do: a tile per warp
-constexpr int kGrid = kNumSMs;   // one CTA per SM: the rings of its warps take the shared memory
 
 template <int D>
 struct Layout {
@@ -37,60 +32,12 @@ struct Layout {
     static constexpr int kSteps = D / 16;
 };
 
-template <typename T>
-struct CachedParams {
-    KvArgs kv;
-    const T* q;
-    T* o;
-    float* lse;
-    int64_t qs[2], os[2];
-    int32_t q_heads, group;
-    float scale;
-    int32_t whole;      // no segment has more than kLeastTiles tiles: none is cut
-    int32_t o_vec;      // four results at a time
-    int32_t* pieces;    // [kGrid][8]: the cut segment that a CTA's share ends with (Piece), count 0 if none
-    float* partial;     // [kGrid][2][rows (D + 2)]
-};
-
-struct Piece {  // what joining a cut segment needs
-    int32_t count, first_row, rows, seq_first, head, pad[3];
-};
-
-// ---- how the work is shared ------------------------------------------------------------------------------------------------
-
-struct Share {  // of one sequence
-    KvSequence s;
-    int32_t row_tiles, tiles;  // of 8 or 16 rows; of 32 keys (1 where there are none: somebody has to write the zeros)
-};
-
-template <int kRows, typename T>
-__device__ __forceinline__ Share share_of(const CachedParams<T>& p, int32_t b) {
-    Share w;
-    w.s = kv_sequence(p.kv, b);
-    w.row_tiles = static_cast<int32_t>((static_cast<int64_t>(w.s.count) * p.group + kRows - 1) / kRows);
-    w.tiles = max(1, (w.s.length + kTileKeys - 1) / kTileKeys);
-    return w;
-}
-
-__device__ __forceinline__ int32_t padded(int32_t tiles) { return (tiles + kLeastTiles - 1) / kLeastTiles * kLeastTiles; }
-
-__device__ __forceinline__ int64_t warp_sum(int64_t v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
 // ---- the kernel's parts ----------------------------------------------------------------------------------------------------
 
 __device__ __forceinline__ float fmax3(float a, float b, float c) {  // one instruction on sm_100
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -194,103 +141,27 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
     __shared__ float sm[W][kRows], sl[W][kRows], sf[W][kRows], sv[W], top_m[kRows], top_l[kRows];
     __shared__ int32_t used[W];
     __shared__ float4 meta[W][L::kStages];  // scales of a tile's halves: keys 0, 1 (-infinity: not there), values 0, 1
-    __shared__ int64_t totals[2], found[2];
-    __shared__ int64_t scan[32];
+    __shared__ typename Work<kRows, kTileKeys, kLeastTiles, false>::Scratch scratch;
 
     const KvArgs& a = p.kv;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
 
-    // -- the share of this CTA
-    {
-        int64_t all = 0, all_padded = 0;
-        for (int32_t b = tid; b < a.seqs; b += L::kThreads) {
-            const Share w = share_of<kRows>(p, b);
-            const int64_t segments = static_cast<int64_t>(w.row_tiles) * a.heads;
-            all += segments * w.tiles;
-            all_padded += segments * padded(w.tiles);
-        }
-        all = warp_sum(all);
-        all_padded = warp_sum(all_padded);
-        if (lane == 0) scan[warp] = all, scan[16 + warp] = all_padded;
-        __syncthreads();
-        if (tid == 0) {
-            int64_t x = 0, y = 0;
-            for (int w = 0; w < W; ++w) x += scan[w], y += scan[16 + w];
-            totals[0] = x;
-            totals[1] = y;
-            found[0] = -1;
-        }
-        __syncthreads();
-    }
-    const bool pad = p.whole || totals[1] <= static_cast<int64_t>(kGrid) * kLeastTiles;
-    const int64_t total = totals[pad ? 1 : 0];
-    const int64_t per = pad ? (totals[1] / kLeastTiles + kGrid - 1) / kGrid * kLeastTiles : (total + kGrid - 1) / kGrid;
-    int64_t at = blockIdx.x * per;
-    const int64_t end = min(total, at + per);
-    if (tid == 0 && !p.whole) p.pieces[blockIdx.x * 8] = 0;
+    Work<kRows, kTileKeys, kLeastTiles, false> work;
+    const bool any = work.template start<L::kThreads>(p, scratch);
     grid_dependency_release();
-    if (at >= end) return;
-    // the sequence that holds tile `at`, and where in it
-    {
-        int64_t before = 0;
-        for (int32_t base = 0; base < a.seqs; base += L::kThreads) {
-            int64_t mine = 0;
-            if (base + tid < a.seqs) {
-                const Share w = share_of<kRows>(p, base + tid);
-                mine = static_cast<int64_t>(w.row_tiles) * a.heads * (pad ? padded(w.tiles) : w.tiles);
-            }
-            int64_t sum = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t other = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += other;
-            }
-            if (lane == 31) scan[warp] = sum;
-            __syncthreads();
-            int64_t chunk = 0, lower = 0;
-            for (int w = 0; w < W; ++w) {
-                lower += w < warp ? scan[w] : 0;
-                chunk += scan[w];
-            }
-            const int64_t first = before + lower + sum - mine;
-            if (mine > 0 && at >= first && at < first + mine) {
-                found[0] = base + tid;
-                found[1] = at - first;
-            }
-            before += chunk;
-            __syncthreads();
-            if (before > at) break;
-        }
-    }
-    int32_t b = static_cast<int32_t>(found[0]);
-    if (b < 0) return;  // cannot be: lengths that change under the kernel
-    Share w = share_of<kRows>(p, b);
-    int64_t inside = found[1];
-
-    while (at < end) {
-        const int32_t tiles = pad ? padded(w.tiles) : w.tiles;
-        const int64_t segments = static_cast<int64_t>(w.row_tiles) * a.heads;
-        if (inside >= segments * tiles) {  // on to the next sequence that has work
-            if (++b >= a.seqs) return;
-            w = share_of<kRows>(p, b);
-            inside = 0;
-            continue;
-        }
-        const int32_t segment = static_cast<int32_t>(inside / tiles), t0 = static_cast<int32_t>(inside % tiles);
-        const int32_t head = segment % a.heads, row_tile = segment / a.heads;
-        const int32_t t1 = static_cast<int32_t>(min(static_cast<int64_t>(tiles), t0 + (end - at)));
-        const int32_t all_rows = w.s.count * p.group, row0 = row_tile * kRows, rows = min(kRows, all_rows - row0);
-        // keys that row r sees
-        auto seen_by = [&](int r) { return w.s.length == 0 ? 0 : w.s.length - w.s.count + (row0 + r) / p.group + 1; };
+    if (!any) return;
+    Segment seg;
+    while (work.next(p, &seg)) {
+        const int32_t b = seg.b, head = seg.head, t0 = seg.t0, rows = seg.rows;
+        auto seen_by = [&](int r) { return seg.seen_by(r, p.group); };
         const int32_t limit = seen_by(rows - 1), least = seen_by(0);
-        const int32_t last = min(t1, (limit + kTileKeys - 1) / kTileKeys);  // tiles t0 .. last - 1 have keys to read
+        const int32_t last = min(seg.t1, (limit + kTileKeys - 1) / kTileKeys);  // tiles t0 .. last - 1 have keys to read
 
         // -- q as fragments in shared memory, rows brought to the same size by powers of two
         const float to_log2 = p.scale * 1.4426950408889634f;
         for (int r = warp; r < kRows; r += W) {
-            const int32_t row = row0 + r;
             float most = 0.f, x[D / 32];
-            const T* q = p.q + (w.s.first + row / p.group) * p.qs[0] + (head * p.group + row % p.group) * p.qs[1];
+            const T* q = p.q + seg.token(p, r) * p.qs[0] + seg.q_head(p, r) * p.qs[1];
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
                 x[i] = r < rows ? VecTraits<T>::to_float(q[lane + 32 * i]) : 0.f;
@@ -319,8 +190,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
             const int l = i & 31, j = (i >> 5) % NT, step = (i >> 5) / NT, r = 8 * j + (l >> 2);
             float x[4] = {0.f, 0.f, 0.f, 0.f};
             if (r < rows) {
-                const int32_t row = row0 + r;
-                const T* q = p.q + (w.s.first + row / p.group) * p.qs[0] + (head * p.group + row % p.group) * p.qs[1] + step_element<D>(step, l & 3);
+                const T* q = p.q + seg.token(p, r) * p.qs[0] + seg.q_head(p, r) * p.qs[1] + step_element<D>(step, l & 3);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[e] = VecTraits<T>::to_float(q[e]) * sf[0][r];
             }
@@ -657,8 +527,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
             top_l[tid] = sum;
         }
         __syncthreads();
-        const bool cut = t0 != 0 || t1 != tiles;
-        float* const out = p.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (t0 == 0 ? 1 : 0)) * (kRows * (D + 2));
+        float* const out = work.partial(p, seg, D);
         for (int i = tid; i < kRows * (D / 4); i += L::kThreads) {
             const int r = i / (D / 4), d4 = i % (D / 4);
             if (r >= rows) break;
@@ -673,13 +542,12 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
                 sum.z += x.z * f;
                 sum.w += x.w * f;
             }
-            if (cut) {
+            if (seg.cut) {
                 reinterpret_cast<float4*>(out + 2 * kRows)[i] = sum;
                 continue;
             }
             const float total_l = top_l[r], inv = total_l == 0.f ? 0.f : 1.f / total_l;
-            const int32_t row = row0 + r;
-            T* const y = p.o + (w.s.first + row / p.group) * p.os[0] + (head * p.group + row % p.group) * p.os[1] + d4 * 4;
+            T* const y = p.o + seg.token(p, r) * p.os[0] + seg.q_head(p, r) * p.os[1] + d4 * 4;
             const float4 x = total_l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
             if constexpr (sizeof(T) == 4) {
                 if (p.o_vec) *reinterpret_cast<float4*>(y) = x;
@@ -693,58 +561,26 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
             }
         }
         if (tid < rows) {
-            if (cut) {
+            if (seg.cut) {
                 out[tid] = top_m[tid];
                 out[kRows + tid] = top_l[tid];
             } else if (p.lse != nullptr) {
-                const int32_t row = row0 + tid;
-                p.lse[static_cast<int64_t>(w.s.first + row / p.group) * p.q_heads + head * p.group + row % p.group] =
-                    top_l[tid] == 0.f ? -INFINITY : (top_m[tid] + log2f(top_l[tid])) * 0.6931471805599453f;
+                p.lse[seg.token(p, tid) * p.q_heads + seg.q_head(p, tid)] = top_l[tid] == 0.f ? -INFINITY : (top_m[tid] + log2f(top_l[tid])) * 0.6931471805599453f;
             }
         }
-        if (cut && t0 == 0 && tid == 0) {
-            const int64_t last_cta = (at + tiles - 1) / per;
-            int32_t* const piece = p.pieces + blockIdx.x * 8;
-            piece[1] = row0;
-            piece[2] = rows;
-            piece[3] = w.s.first;
-            piece[4] = head;
-            piece[0] = static_cast<int32_t>(last_cta - blockIdx.x) + 1;
-        }
+        if (seg.cut && tid == 0) work.leave_piece(p, seg);
         __syncthreads();
-        at += t1 - t0;
-        inside += t1 - t0;
     }
 }
 
-// Joins the pieces of the segment that CTA blockIdx.x began and others went on with: sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
-template <typename T, int D, int kRows>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ CachedParams<T> p) {
-    grid_dependency_wait();
-    const int32_t* const piece = p.pieces + blockIdx.x * 8;
-    const int32_t count = piece[0];
-    if (count == 0) return;
-    const int32_t row0 = piece[1], rows = piece[2], seq_first = piece[3], head = piece[4];
-    auto part = [&](int32_t i) { return p.partial + ((static_cast<int64_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0)) * (kRows * (D + 2)); };
-    const int r = blockIdx.y;
-    if (r >= rows) return;
-    float most = -INFINITY;
-    for (int32_t i = 0; i < count; ++i) most = fmaxf(most, part(i)[r]);
-    const float shift = most == -INFINITY ? 0.f : most;
-    const int32_t row = row0 + r;
-    const int64_t token = seq_first + row / p.group, q_head = head * p.group + row % p.group;
-    float total = 0.f;
-    for (int32_t i = 0; i < count; ++i) total += part(i)[kRows + r] * ex2(part(i)[r] - shift);
-    for (int d = threadIdx.x; d < D; d += 128) {
-        float sum = 0.f;
-        for (int32_t i = 0; i < count; ++i) sum += part(i)[2 * kRows + r * D + d] * ex2(part(i)[r] - shift);
-        p.o[token * p.os[0] + q_head * p.os[1] + d] = VecTraits<T>::from_float(total == 0.f ? 0.f : sum / total);
-    }
-    if (p.lse != nullptr && threadIdx.x == 0) p.lse[token * p.q_heads + q_head] = total == 0.f ? -INFINITY : (most + log2f(total)) * 0.6931471805599453f;
-}
+int64_t few_rows_scratch(int64_t dim) { return kGrid * (8 * 4 + 2 * 16 * (dim + 2) * 4); }
 
-template <int D>
-constexpr int64_t scratch_bytes() { return kGrid * (8 * 4 + 2 * 16 * (D + 2) * 4); }
+// Sequences of up to this many rows are this kernel's, where the other takes the type: at 32 rows two passes of 16 over the keys cost
+// what one of 128 does there (6 us and 12.5 over 8 x 6000 keys of head dimension 128).
+constexpr int kFewRows = 32;
+bool long_takes(int64_t head_dim) { return head_dim == 64 || head_dim == 128; }
+// Whether a sequence of the call may have more rows: the host knows only how many there are in all.
+bool may_be_long(const int32_t* starts, int64_t tokens, int64_t group) { return starts != nullptr && tokens * group > kFewRows; }
 
 template <typename T, int D, int NT>
 int launch_rows(CachedParams<T> p, void* scratch, cudaStream_t stream) {
@@ -783,8 +619,17 @@ int launch(const KvArgs& kv, const void* q, const int64_t* qs, int64_t q_heads, 
     p.group = static_cast<int32_t>(q_heads / kv.heads);
     p.scale = scale;
     p.whole = scratch == nullptr;
-    const int64_t four = 4 * static_cast<int64_t>(sizeof(T));
-    p.o_vec = reinterpret_cast<uintptr_t>(o) % four == 0 && os[0] % 4 == 0 && os[1] % 4 == 0;
+    constexpr int64_t E = VecTraits<T>::kElems;
+    p.q_vec = aligned16(q) && qs[0] % E == 0 && qs[1] % E == 0;
+    p.o_vec = aligned16(o) && os[0] % E == 0 && os[1] % E == 0 ? 2 : reinterpret_cast<uintptr_t>(o) % (4 * sizeof(T)) == 0 && os[0] % 4 == 0 && os[1] % 4 == 0;
+    p.few_rows = 0x7fffffff;
+    if constexpr (sizeof(T) == 2) {
+        if (may_be_long(kv.starts, kv.tokens, p.group) && long_takes(kv.head_dim)) {
+            p.few_rows = kFewRows;
+            if (int st = cached_attention_long(p, scratch, stream)) return st;
+            if (scratch != nullptr) scratch = static_cast<uint8_t*>(scratch) + cached_attention_long_scratch(kv.head_dim);
+        }
+    }
     switch (kv.head_dim) {
         case 64: return launch_dim<T, 64>(p, scratch, stream);
         case 96: return launch_dim<T, 96>(p, scratch, stream);
@@ -795,7 +640,10 @@ int launch(const KvArgs& kv, const void* q, const int64_t* qs, int64_t q_heads, 
 
 }  // namespace
 
-int cached_attention_device_error() { return take_kv_error(); }
+int cached_attention_device_error() {
+    const int few = take_kv_error(), many = cached_attention_long_device_error();
+    return few < 0 || many < 0 ? -1 : few != 0 ? few : many;
+}
 
 }  // namespace mhlo
 
@@ -805,14 +653,12 @@ extern "C" {
 
 int64_t mhlo_cuda_cached_attention_scratch_bytes(const mhlo_cuda_kv_cache* cache, const mhlo_cuda_kv_batch* batch, int64_t q_heads) {
     if (!cache || !batch || q_heads < 1) return 0;
-    if (batch->pages_per_seq * cache->page_tokens <= kLeastTiles * kTileKeys) return 0;  // no segment is worth cutting
-    switch (cache->head_dim) {
-        case 64: return scratch_bytes<64>();
-        case 96: return scratch_bytes<96>();
-        case 128: return scratch_bytes<128>();
-        case 256: return scratch_bytes<256>();
-        default: return 0;
-    }
+    if (cache->head_dim < 1 || batch->pages_per_seq * cache->page_tokens <= kLeastTiles * kTileKeys) return 0;  // no segment is worth cutting
+    const int64_t group = q_heads / std::max<int64_t>(1, cache->heads);
+    int64_t bytes = few_rows_scratch(cache->head_dim);
+    if (may_be_long(batch->token_starts, batch->tokens, group) && long_takes(cache->head_dim))
+        bytes += cached_attention_long_scratch(static_cast<int>(cache->head_dim));
+    return bytes;
 }
 
 int mhlo_cuda_cached_attention(int32_t dtype, const void* q_dev, const int64_t q_strides[2], const mhlo_cuda_kv_cache* cache, const mhlo_cuda_kv_batch* batch,

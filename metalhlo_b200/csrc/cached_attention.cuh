@@ -1,0 +1,249 @@
+// What the two kernels of attention over the paged 8-bit cache share: how the work of a call is cut, and how cut pieces are joined.
+//
+// The work is cut into segments: (sequence, ROWS rows, cache head). The rows of a segment are (token, query head) pairs that read the
+// same cache head: row r of a sequence is token r / group, query head head * group + r % group. A segment's keys are walked in tiles
+// of KEYS; CTAs share all tiles of the call evenly, so a CTA's piece may begin or end inside a segment. Whole segments are written at
+// once, pieces go to scratch as (maximum, sum, output) and join_kernel joins them in the order of the CTAs: no atomics, and no order
+// of arrival in the result.
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace mhlo {
+
+constexpr int kGrid = kNumSMs;  // one CTA per SM: both kernels fill its shared memory
+
+template <typename T>
+struct CachedParams {
+    KvArgs kv;
+    const T* q;
+    T* o;
+    float* lse;
+    int64_t qs[2], os[2];
+    int32_t q_heads, group;
+    float scale;
+    int32_t q_vec;      // rows of q on the 16-byte grid
+    int32_t o_vec;      // 1: results four at a time, 2: rows of o on the 16-byte grid
+    int32_t whole;      // no segment has more than the least share of a CTA: none is cut
+    int32_t few_rows;   // sequences of up to this many rows belong to the kernel of few rows, longer ones to the other
+    int32_t* pieces;    // [kGrid][8]: the cut segment that a CTA's share ends with (Piece), count 0 if none
+    float* partial;     // [kGrid][2][ROWS (head_dim + 2)]: maxima (log2), sums, outputs
+};
+
+struct Piece {  // what joining a cut segment needs: CTAs it goes over, its rows
+    int32_t count, first_row, rows, seq_first, head, pad[3];
+};
+
+namespace {
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct Segment {
+    KvSequence s;
+    int32_t b, head, row0, rows;  // sequence, cache head, first row and rows
+    int32_t t0, t1, tiles;        // this piece's tiles, and all that the segment counts as
+    int64_t begin;                // its first tile among all tiles of the call
+    bool cut;
+    __device__ __forceinline__ int32_t seen_by(int32_t r, int32_t group) const {  // keys that row r of the segment sees
+        return s.length == 0 ? 0 : s.length - s.count + (row0 + r) / group + 1;
+    }
+    template <typename T>
+    __device__ __forceinline__ int64_t token(const CachedParams<T>& p, int32_t r) const { return s.first + (row0 + r) / p.group; }
+    template <typename T>
+    __device__ __forceinline__ int64_t q_head(const CachedParams<T>& p, int32_t r) const { return head * p.group + (row0 + r) % p.group; }
+};
+
+// ROWS, KEYS: of a segment and a tile. LEAST: a CTA's share, in tiles, where there is little to do. LONG: takes the sequences of many rows.
+template <int ROWS, int KEYS, int LEAST, bool LONG>
+struct Work {
+    struct Share {  // of one sequence
+        KvSequence s;
+        int32_t row_tiles, tiles;  // tiles: 1 where there are no keys: somebody has to write the zeros
+        __device__ __forceinline__ int32_t counted(bool pad) const { return pad ? (tiles + LEAST - 1) / LEAST * LEAST : tiles; }
+    };
+    struct Scratch {  // in shared memory
+        int64_t sums[64], totals[2], found[2];
+    };
+    int64_t at, end, per, inside;  // tiles of the call; inside: from the sequence's first
+    int32_t b;
+    bool pad;
+    Share w;
+
+    template <typename T>
+    __device__ __forceinline__ static Share share_of(const CachedParams<T>& p, int32_t b) {
+        Share w;
+        w.s = kv_sequence(p.kv, b);
+        const int64_t rows = static_cast<int64_t>(w.s.count) * p.group;
+        w.row_tiles = (rows > p.few_rows) != LONG ? 0 : static_cast<int32_t>((rows + ROWS - 1) / ROWS);
+        w.tiles = max(1, (w.s.length + KEYS - 1) / KEYS);
+        return w;
+    }
+    __device__ __forceinline__ static int64_t warp_sum(int64_t v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    }
+
+    // The share of this CTA; false: none. All THREADS threads of the CTA call it. Where there is little to do segments count in whole
+    // shares, so that no CTA gets the ends of two.
+    template <int THREADS, typename T>
+    __device__ __forceinline__ bool start(const CachedParams<T>& p, Scratch& scratch) {
+        constexpr int W = THREADS / 32;
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+        int64_t all = 0, all_padded = 0;
+        for (int32_t i = tid; i < p.kv.seqs; i += THREADS) {
+            const Share x = share_of(p, i);
+            const int64_t segments = static_cast<int64_t>(x.row_tiles) * p.kv.heads;
+            all += segments * x.tiles;
+            all_padded += segments * x.counted(true);
+        }
+        all = warp_sum(all);
+        all_padded = warp_sum(all_padded);
+        if (lane == 0) {
+            scratch.sums[warp] = all;
+            scratch.sums[32 + warp] = all_padded;
+        }
+        __syncthreads();
+        if (tid == 0) {
+            int64_t x = 0, y = 0;
+            for (int i = 0; i < W; ++i) {
+                x += scratch.sums[i];
+                y += scratch.sums[32 + i];
+            }
+            scratch.totals[0] = x;
+            scratch.totals[1] = y;
+            scratch.found[0] = -1;
+        }
+        __syncthreads();
+        pad = p.whole || scratch.totals[1] <= static_cast<int64_t>(kGrid) * LEAST;
+        const int64_t total = scratch.totals[pad ? 1 : 0];
+        per = pad ? (total / LEAST + kGrid - 1) / kGrid * LEAST : (total + kGrid - 1) / kGrid;
+        at = blockIdx.x * per;
+        end = min(total, at + per);
+        if (tid == 0 && !p.whole) p.pieces[blockIdx.x * 8] = 0;
+        if (at >= end) return false;
+        // the sequence that holds tile `at`, and where in it
+        int64_t before = 0;
+        for (int32_t base = 0; base < p.kv.seqs; base += THREADS) {
+            int64_t mine = 0;
+            if (base + tid < p.kv.seqs) {
+                const Share x = share_of(p, base + tid);
+                mine = static_cast<int64_t>(x.row_tiles) * p.kv.heads * x.counted(pad);
+            }
+            int64_t sum = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t other = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += other;
+            }
+            if (lane == 31) scratch.sums[warp] = sum;
+            __syncthreads();
+            int64_t chunk = 0, lower = 0;
+            for (int i = 0; i < W; ++i) {
+                lower += i < warp ? scratch.sums[i] : 0;
+                chunk += scratch.sums[i];
+            }
+            const int64_t first = before + lower + sum - mine;
+            if (mine > 0 && at >= first && at < first + mine) {
+                scratch.found[0] = base + tid;
+                scratch.found[1] = at - first;
+            }
+            before += chunk;
+            __syncthreads();
+            if (before > at) break;
+        }
+        b = static_cast<int32_t>(scratch.found[0]);
+        inside = scratch.found[1];
+        if (b < 0) return false;  // cannot be: lengths that change under the kernel
+        w = share_of(p, b);
+        return true;
+    }
+
+    // The next piece of this CTA's share.
+    template <typename T>
+    __device__ __forceinline__ bool next(const CachedParams<T>& p, Segment* s) {
+        while (at < end) {
+            const int32_t tiles = w.counted(pad);
+            if (inside >= static_cast<int64_t>(w.row_tiles) * p.kv.heads * tiles) {  // on to the next sequence
+                if (++b >= p.kv.seqs) return false;
+                w = share_of(p, b);
+                inside = 0;
+                continue;
+            }
+            const int32_t segment = static_cast<int32_t>(inside / tiles), row_tile = segment / p.kv.heads;
+            s->s = w.s;
+            s->b = b;
+            s->head = segment % p.kv.heads;
+            s->row0 = row_tile * ROWS;
+            s->rows = min(ROWS, w.s.count * p.group - s->row0);
+            s->t0 = static_cast<int32_t>(inside % tiles);
+            s->t1 = static_cast<int32_t>(min(static_cast<int64_t>(tiles), s->t0 + (end - at)));
+            s->tiles = tiles;
+            s->begin = at - s->t0;
+            s->cut = s->t0 != 0 || s->t1 != tiles;
+            at += s->t1 - s->t0;
+            inside += s->t1 - s->t0;
+            return true;
+        }
+        return false;
+    }
+
+    // Where a cut piece goes: a CTA may end one segment that others began, and begin one that others go on with.
+    template <typename T>
+    __device__ __forceinline__ float* partial(const CachedParams<T>& p, const Segment& s, int dim) const {
+        return p.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (s.t0 == 0 ? 1 : 0)) * (ROWS * (dim + 2));
+    }
+    // One thread, for a cut piece: the CTA that began a segment leaves what joining it needs.
+    template <typename T>
+    __device__ __forceinline__ void leave_piece(const CachedParams<T>& p, const Segment& s) const {
+        if (s.t0 != 0) return;
+        int32_t* const piece = p.pieces + blockIdx.x * 8;
+        piece[1] = s.row0;
+        piece[2] = s.rows;
+        piece[3] = s.s.first;
+        piece[4] = s.head;
+        piece[0] = static_cast<int32_t>((s.begin + s.tiles - 1) / per - blockIdx.x) + 1;
+    }
+};
+
+// Joins the pieces of the segment that CTA blockIdx.x began and others went on with: sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
+// blockIdx.y: rows in turn.
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ CachedParams<T> p) {
+    grid_dependency_wait();
+    const int32_t* const piece = p.pieces + blockIdx.x * 8;
+    const int32_t count = piece[0];
+    if (count == 0) return;
+    const int32_t row0 = piece[1], rows = piece[2], seq_first = piece[3], head = piece[4];
+    auto part = [&](int32_t i) { return p.partial + ((static_cast<int64_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0)) * (ROWS * (D + 2)); };
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+        float most = -INFINITY;
+        for (int32_t i = 0; i < count; ++i) most = fmaxf(most, part(i)[r]);
+        const float shift = most == -INFINITY ? 0.f : most;
+        const int32_t row = row0 + r;
+        const int64_t token = seq_first + row / p.group, q_head = head * p.group + row % p.group;
+        float total = 0.f;
+        for (int32_t i = 0; i < count; ++i) total += part(i)[ROWS + r] * ex2(part(i)[r] - shift);
+        for (int d = threadIdx.x; d < D; d += 128) {
+            float sum = 0.f;
+            for (int32_t i = 0; i < count; ++i) sum += part(i)[2 * ROWS + r * D + d] * ex2(part(i)[r] - shift);
+            p.o[token * p.os[0] + q_head * p.os[1] + d] = VecTraits<T>::from_float(total == 0.f ? 0.f : sum / total);
+        }
+        if (p.lse != nullptr && threadIdx.x == 0)
+            p.lse[token * p.q_heads + q_head] = total == 0.f ? -INFINITY : (most + log2f(total)) * 0.6931471805599453f;
+    }
+}
+
+}  // namespace
+
+// Sequences of many rows (16-bit types, head dimension 64 or 128): cached_attention_tc.cu.
+template <typename T>
+int cached_attention_long(CachedParams<T> p, void* scratch, cudaStream_t stream);
+int64_t cached_attention_long_scratch(int head_dim);
+int cached_attention_long_device_error();
+
+}  // namespace mhlo

@@ -165,7 +165,7 @@ int mhlo_cuda_device_error(int32_t* out_code) {
     if (*out_code > 200) {
         static const char* const what[] = {"", "a page outside the cache", "a length beyond the table or below the sequence's rows",
                                            "token_starts out of order", "a position behind the rotation table"};
-        return fail(MHLO_CUDA_EXECUTION_FAILED, "a key/value cache kernel met %s (code %d)", kv <= 4 ? what[kv] : "an error", *out_code);
+        return fail(MHLO_CUDA_EXECUTION_FAILED, "a key/value cache kernel met %s (code %d)", kv <= 4 ? what[kv] : "a bounded wait that ran out", *out_code);
     }
     if (*out_code != 0) return fail(MHLO_CUDA_EXECUTION_FAILED, "a tensor-core kernel gave up on a bounded wait (code %d)", *out_code);
     return MHLO_CUDA_OK;
