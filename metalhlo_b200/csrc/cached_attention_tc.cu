@@ -2,10 +2,11 @@
 // and fp16, head dimension 64 or 128.
 //
 // A CTA owns 256 rows of a segment as two halves of 128 and walks the keys in blocks of 128:
-//   warp 0          MMA issuer: S_h = Q_h K^T (both operands in shared memory), O_h += P_h V (P read from tensor memory)
-//   warps 1-3       producers: rows of q as fp16 into shared memory at a segment's start; then codes of keys and values from global
-//                   memory through registers (a block ahead) into the 128-byte-swizzled layout as fp16, exactly
-//   warps 4-7, 8-11 softmax of half 0 / 1, a thread per row, P written over the scores in tensor memory
+//   warp 0             MMA issuer: S_h = Q_h K^T (both operands in shared memory), O_h += P_h V (P read from tensor memory)
+//   warps 1-3, 12-15   producers: codes of keys and values from global memory through registers, half a block ahead, into the
+//                      128-byte-swizzled layout as fp16, exactly
+//   warps 4-7, 8-11    softmax of half 0 / 1, a thread per row: it puts its row of q into shared memory as fp16 at a piece's start and
+//                      writes P over the scores in tensor memory
 // The scales do not touch the codes: a key's scale multiplies its column of scores (16 keys at a time share one), a value's scale goes
 // into the exponent of the weights as its ratio to the largest of the piece, so the products run on integers up to 127.
 // Rows that are fp16 stay as they are; bf16 rows are brought to the same size by powers of two, which is exact.
@@ -23,13 +24,17 @@
 namespace mhlo {
 namespace {
 
-constexpr int kBlockM = 128, kHalves = 2, kRows = kHalves * kBlockM, kBlockN = 128, kStages = 2, kThreads = 384, kProducers = 3, kSlots = 4;
+constexpr int kBlockM = 128, kHalves = 2, kRows = kHalves * kBlockM, kBlockN = 128, kStages = 2, kThreads = 512, kProducers = 7, kSlots = 4;
 constexpr int kGroups = kBlockN / 16;  // keys with one scale
 constexpr int kLeast = 3;              // blocks of a CTA's share where there is little to do: 384 keys, as in the kernel of few rows
 constexpr float kUnitLog2 = 6.f;       // weights are held times 2^6, so that those far below the largest keep some bits of fp16
 constexpr float kUnit = 64.f;
 constexpr float kGrowth = 8.f;         // log2 of what scores may exceed the last maximum by before it moves
 constexpr float kSumLimit = 32768.f;   // weights of a row and block, in fp16
+// Registers: 512 threads are launched with 128 each, 512 for every four lanes of the four warpgroups. The softmax holds a row's 128
+// scores and weights; the others have little.
+constexpr int kSoftmaxRegs = 168, kOtherRegs = 88;
+static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * 128, "register shares above what the CTA is launched with wait forever");
 constexpr int kWaitError = 50;         // + where a bounded wait ran out
 
 struct Scales {  // of a block's groups
@@ -148,14 +153,13 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    __shared__ uint64_t bars[6 * kHalves + 4 * kStages];
+    __shared__ uint64_t bars[4 * kHalves + 4 * kStages];
     __shared__ uint32_t tmem_slot;
     __shared__ typename Works::Scratch scratch;
     __shared__ Scales scales[kSlots];
-    __shared__ float row_factor[2][kRows], v_most[2][kHalves];  // by the parity of the piece
+    __shared__ float v_most[kSlots];  // the largest value scale of the piece that a slot's block is of
     uint64_t* const q_full = bars;
-    uint64_t* const q_empty = q_full + kHalves;
-    uint64_t* const s_full = q_empty + kHalves;   // scores of the half's block are in tensor memory
+    uint64_t* const s_full = q_full + kHalves;    // scores of the half's block are in tensor memory
     uint64_t* const p_full = s_full + kHalves;    // its weights are, and O is rescaled if need be
     uint64_t* const pv_done = p_full + kHalves;   // every product with values so far has completed
     uint64_t* const k_full = pv_done + kHalves;
@@ -166,8 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int h = 0; h < kHalves; ++h) {
-            mbar_init(&q_full[h], kProducers);
-            mbar_init(&q_empty[h], 1);
+            mbar_init(&q_full[h], 4);
             mbar_init(&s_full[h], 1);
             mbar_init(&p_full[h], 4);
             mbar_init(&pv_done[h], 1);
@@ -201,6 +204,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
         }
     };
     Segment seg;
+    if (warp < 4 || warp >= 12) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
 
     if (warp == 0) {
         // ---- MMA issuer. Order on the pipe: for each half P.V of this block, then S of the next (of this piece, or the first of the
@@ -241,21 +246,21 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
         Blocks cur(Segment{}, 1), nxt(Segment{}, 1);
         bool has = next_blocks(&cur);
         int stage = 0;
-        uint32_t phase = 0, pieces = 0, it[kHalves] = {0, 0};
+        uint32_t phase = 0, it[kHalves] = {0, 0}, q_of[kHalves] = {0, 0};  // q_of: pieces the half has had blocks of
         // scores of half h in block j of a piece
-        auto scores = [&](const Blocks& of, int j, int h, int st, uint32_t ph, uint32_t piece) {
-            if (j == 0) wait(&q_full[h], piece & 1, 1);
+        auto scores = [&](const Blocks& of, int j, int h, int st, uint32_t ph) {
+            const bool takes_part = j < of.of_half[h];
+            if (takes_part && j == 0) wait(&q_full[h], q_of[h]++ & 1, 1);
             if (h == 0) wait(&k_full[st], ph, 2);
             if (!ok) return;
-            if (j < of.of_half[h]) {
+            if (takes_part) {
                 tc_fence_after();
                 issue_s(h, st);
             }
-            if (of.of_half[h] == 0 ? j == 0 : j + 1 == of.of_half[h]) commit_to(&q_empty[h]);
             if (h == kHalves - 1) commit_to(&k_empty[st]);
         };
         if (has)
-            for (int h = 0; h < kHalves; ++h) scores(cur, 0, h, 0, 0, 0);
+            for (int h = 0; h < kHalves; ++h) scores(cur, 0, h, 0, 0);
         while (has && ok) {
             const bool more_pieces = next_blocks(&nxt);
             for (int j = 0; j < cur.count && ok; ++j) {
@@ -272,98 +277,57 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                         ++it[h];
                     }
                     if (h == kHalves - 1) commit_to(&v_empty[stage]);
-                    if (!last) scores(cur, j + 1, h, next_stage, next_phase, pieces);
-                    else if (more_pieces) scores(nxt, 0, h, next_stage, next_phase, pieces + 1);
+                    if (!last) scores(cur, j + 1, h, next_stage, next_phase);
                 }
+                // the next piece's q comes only when the half is through with this one
+                for (int h = 0; h < kHalves && ok && last && more_pieces; ++h) scores(nxt, 0, h, next_stage, next_phase);
                 stage = next_stage;
                 phase = next_phase;
             }
             cur = nxt;
             has = more_pieces;
-            ++pieces;
         }
-    } else if (warp <= kProducers) {
+    } else if (warp < 4 || warp >= 12) {
         // ---- producers
         const KvArgs& a = p.kv;
-        const int wp = warp - 1;
-        const float to_log2 = p.scale * 1.4426950408889634f;
+        const int wp = warp < 4 ? warp - 1 : warp - 9;
         constexpr int kChunks = D / 16, kPassRows = 32 / kChunks, kPasses = kBlockN / kPassRows, kMine = (kPasses + kProducers - 1) / kProducers;
         // 16 codes a lane: four lanes of a quarter warp on one row and four on the next keep the stores free of bank conflicts
         const int chunk = D == 128 ? (lane & 3) | (lane >> 4) << 2 : lane & 3, row_in_pass = D == 128 ? (lane >> 2) & 3 : lane >> 2;
         int stage = 0;
-        uint32_t phase = 0, pieces = 0, block = 0;
+        uint32_t phase = 0, block = 0;
         while (ok && work.next(p, &seg)) {
             const Blocks bl(seg, p.group);
             if (bl.count == 0) continue;
-            const uint32_t parity = pieces & 1;
             // pages and scales of a block's groups, one per lane
-            int64_t base = -1, next_base = -1;
-            float ks = 0.f, vs = 0.f, next_ks = 0.f, next_vs = 0.f;
+            struct Groups {
+                int64_t base;
+                float ks, vs;
+            };
             auto look_up = [&](int j) {
-                next_base = -1;
-                next_ks = next_vs = 0.f;
+                Groups g{-1, 0.f, 0.f};
                 const int32_t key = (bl.kb0 + j) * kBlockN + lane * 16;
                 if (lane < kGroups && j < bl.count && key < bl.limit) {
                     const int32_t page = kv_page(a, seg.b, key >> a.page_shift);
                     if (page >= 0) {
                         const int64_t at = static_cast<int64_t>(page) * a.heads + seg.head;
-                        next_base = ((at << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * D;
-                        next_ks = a.k_scales[at];
-                        next_vs = a.v_scales[at];
+                        g.base = ((at << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * D;
+                        g.ks = a.k_scales[at];
+                        g.vs = a.v_scales[at];
                     }
                 }
+                return g;
             };
-            look_up(0);
+            Groups now = look_up(0), next = look_up(1);
             // the largest value scale of the piece
             float most = 0.f;
             const int32_t keys_end = min(bl.limit, (bl.kb0 + bl.count) * kBlockN);
+#pragma unroll 4
             for (int32_t i = (bl.kb0 * kBlockN >> a.page_shift) + lane; i <= (keys_end - 1) >> a.page_shift; i += 32) {
                 const int32_t page = kv_page(a, seg.b, i);
                 if (page >= 0) most = fmaxf(most, a.v_scales[static_cast<int64_t>(page) * a.heads + seg.head]);
             }
             most = warp_reduce<MaxOp>(most);
-            // rows of q: eight elements a lane
-            constexpr int kRowLanes = D / 8, kRowsAtOnce = 32 / kRowLanes;
-            for (int h = 0; h < kHalves; ++h) {
-                wait(&q_empty[h], (pieces & 1) ^ 1, 5);
-                if (!ok) break;
-                // The softmax of this half has read what these held two pieces ago: it did so before its first weights of that piece, and
-                // q_empty of the piece between is committed after all of them.
-                if (wp == 0 && lane == 0) v_most[parity][h] = most;
-#pragma unroll 4
-                for (int r = (wp * kRowsAtOnce) + lane / kRowLanes; r < kBlockM; r += kProducers * kRowsAtOnce) {
-                    const int row = h * kBlockM + r, part = lane % kRowLanes;
-                    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    if (row < seg.rows) {
-                        const T* const x = p.q + seg.token(p, row) * p.qs[0] + seg.q_head(p, row) * p.qs[1] + part * 8;
-                        if (p.q_vec) {
-                            VecTraits<T>::unpack(__ldcs(reinterpret_cast<const uint4*>(x)), f);  // not the read-only path: o may be q
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) f[e] = VecTraits<T>::to_float(x[e]);
-                        }
-                    }
-                    int shift = 0;
-                    if (kBf16) {
-                        float big = 0.f;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(f[e]));
-#pragma unroll
-                        for (int o = 1; o < kRowLanes; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-                        if (big > 0.f && big < INFINITY) shift = max(-120, ilogbf(big) - 13);
-                        const float unit = scalbnf(1.f, -shift);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] *= unit;
-                    }
-                    if (part == 0) row_factor[parity][row] = scalbnf(to_log2, shift);
-                    *reinterpret_cast<uint4*>(smem + L::kQ + h * L::kQHalf + (part >> 3) * kBlockM * 128 + r * 128 + (((part & 7) ^ (r & 7)) << 4)) =
-                        make_uint4(pack_f16(f[0], f[1]), pack_f16(f[2], f[3]), pack_f16(f[4], f[5]), pack_f16(f[6], f[7]));
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[h]);
-            }
-            if (!ok) break;
             uint4 raw_k[kMine], raw_v[kMine];
             auto load = [&](const int8_t* codes, int64_t from, uint4* raw) {
 #pragma unroll
@@ -390,60 +354,105 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                 fence_proxy_async();
                 __syncwarp();
             };
-            load(a.k_codes, next_base, raw_k);
+            load(a.k_codes, now.base, raw_k);
             for (int j = 0; j < bl.count && ok; ++j, ++block) {
-                base = next_base;
-                ks = next_ks;
-                vs = next_vs;
-                load(a.v_codes, base, raw_v);
-                look_up(j + 1);
-                const float ratio = most > 0.f ? vs / most : vs * 0.f;  // NaN stays
+                load(a.v_codes, now.base, raw_v);
+                const Groups after = look_up(j + 2);
+                const float ratio = most > 0.f ? now.vs / most : now.vs * 0.f;  // NaN stays
                 const bool nothing = ratio < 1e-18f;
-                const uint32_t missing = __ballot_sync(0xffffffffu, base < 0) & ((1u << kGroups) - 1), no_value = missing | __ballot_sync(0xffffffffu, nothing);
+                const uint32_t missing = __ballot_sync(0xffffffffu, now.base < 0) & ((1u << kGroups) - 1), no_value = missing | __ballot_sync(0xffffffffu, nothing);
                 wait(&k_empty[stage], phase ^ 1, 6);
                 if (!ok) break;
                 if (wp == 0 && lane < kGroups) {
-                    // Four slots: k_empty says that the scores of two blocks ago are done, and they were asked for only after the block
-                    // before those had its weights.
+                    // Four slots: k_empty says that the scores of two blocks ago are done, and they were asked for only after both halves
+                    // had the weights of the block before those.
                     Scales& s = scales[block % kSlots];
-                    s.key[lane] = base < 0 ? 0.f : ks;
+                    s.key[lane] = now.base < 0 ? 0.f : now.ks;
                     s.ratio_log2[lane] = nothing ? 0.f : __log2f(ratio);
                     s.out_again[lane] = nothing ? 1.f / kUnit : __fdividef(1.f / kUnit, ratio);
-                    if (lane == 0) s.missing = missing;
+                    if (lane == 0) {
+                        s.missing = missing;
+                        v_most[block % kSlots] = most;
+                    }
                 }
                 store(L::kK + stage * L::kTile, raw_k, missing);
                 if (lane == 0) mbar_arrive(&k_full[stage]);
-                load(a.k_codes, next_base, raw_k);
+                load(a.k_codes, next.base, raw_k);
                 wait(&v_empty[stage], phase ^ 1, 7);
                 if (!ok) break;
                 store(L::kV + stage * L::kTile, raw_v, no_value);
                 if (lane == 0) mbar_arrive(&v_full[stage]);
+                now = next;
+                next = after;
                 if (++stage == kStages) {
                     stage = 0;
                     phase ^= 1;
                 }
             }
-            ++pieces;
         }
     } else {
         // ---- softmax
         const int h = (warp - 4) >> 2, quarter = warp & 3, r = h * kBlockM + quarter * 32 + lane;
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t s_taddr = tmem + lane_base + kSCol + h * kBlockN, o_taddr = tmem + lane_base + kOCol + h * D;
-        uint32_t it = 0, block0 = 0, pieces = 0;
+        const float to_log2 = p.scale * 1.4426950408889634f;
+        uint32_t it = 0, block0 = 0;
         while (ok && work.next(p, &seg)) {
             const Blocks bl(seg, p.group);
             const int nb = bl.of_half[h];
             const int32_t seen = r < seg.rows ? seg.seen_by(r, p.group) : 0x7fffffff;  // rows that are none hide nothing
             float m_ref = -INFINITY, l = 0.f, factor = 0.f, largest = 0.f;
+            if (nb > 0) {
+                // This row of q. The half's last scores of the piece before are done (this thread has seen them): q may be replaced.
+                uint4 raw[D / 8];
+                const T* const x = r < seg.rows ? p.q + seg.token(p, r) * p.qs[0] + seg.q_head(p, r) * p.qs[1] : nullptr;
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    raw[c] = make_uint4(0, 0, 0, 0);
+                    if (x == nullptr) continue;
+                    if (p.q_vec) {
+                        raw[c] = __ldcs(reinterpret_cast<const uint4*>(x + c * 8));  // not the read-only path: o may be q
+                    } else {
+                        float f[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) f[e] = VecTraits<T>::to_float(x[c * 8 + e]);
+                        raw[c] = VecTraits<T>::pack(f);
+                    }
+                }
+                int shift = 0;
+                if (kBf16) {
+                    float big = 0.f;
+#pragma unroll
+                    for (int c = 0; c < D / 8; ++c) {
+                        float f[8];
+                        VecTraits<T>::unpack(raw[c], f);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(f[e]));
+                    }
+                    if (big > 0.f && big < INFINITY) shift = max(-120, ilogbf(big) - 13);
+                }
+                const float unit = scalbnf(1.f, -shift);
+                factor = scalbnf(to_log2, shift);
+                const int row = r - h * kBlockM;
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    uint4 w = raw[c];
+                    if (kBf16) {
+                        float f[8];
+                        VecTraits<T>::unpack(raw[c], f);
+                        w = make_uint4(pack_f16(f[0] * unit, f[1] * unit), pack_f16(f[2] * unit, f[3] * unit), pack_f16(f[4] * unit, f[5] * unit), pack_f16(f[6] * unit, f[7] * unit));
+                    }
+                    *reinterpret_cast<uint4*>(smem + L::kQ + h * L::kQHalf + (c >> 3) * kBlockM * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = w;
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[h]);
+            }
             for (int j = 0; j < nb && ok; ++j, ++it) {
                 wait(&s_full[h], it & 1, 8);
                 if (!ok) break;
                 tc_fence_after();
-                if (j == 0) {
-                    factor = row_factor[pieces & 1][r];
-                    largest = v_most[pieces & 1][h];
-                }
+                if (j == 0) largest = v_most[block0 % kSlots];
                 const Scales& sc = scales[(block0 + j) % kSlots];
                 const int32_t key0 = (bl.kb0 + j) * kBlockN;
                 const bool mask = __any_sync(0xffffffffu, key0 + kBlockN > seen) || sc.missing != 0;
@@ -549,10 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
             }
             if (seg.cut && r == 0) work.leave_piece(p, seg);
             __syncwarp();
-            if (bl.count > 0) {
-                block0 += bl.count;
-                ++pieces;
-            }
+            block0 += bl.count;
         }
     }
     tc_fence_before();
