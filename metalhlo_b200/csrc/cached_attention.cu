@@ -594,7 +594,7 @@ int launch_rows(CachedParams<T> p, void* scratch, cudaStream_t stream) {
     kernel<<<kGrid, L::kThreads, smem, stream>>>(p);
     MHLO_CUDA_CHECK_LAUNCH("cached_attention");
     if (p.whole) return MHLO_CUDA_OK;
-    const cudaError_t e = launch_dependent(join_kernel<T, D, 8 * NT>, dim3(kGrid, 8 * NT), dim3(128), 0, stream, 1, true, p);
+    const cudaError_t e = launch_dependent(join_kernel<T, D, 8 * NT>, dim3(kGrid, NT), dim3(32 * kJoinRows), 0, stream, 1, true, p);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of cached_attention failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("cached_attention (joining)");
     return MHLO_CUDA_OK;

@@ -211,31 +211,44 @@ struct Work {
 };
 
 // Joins the pieces of the segment that CTA blockIdx.x began and others went on with: sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
-// blockIdx.y: rows in turn.
+// A warp per row, kJoinRows rows to a CTA (blockIdx.y): the maxima and sums of up to 32 pieces are read at once, a lane each.
+constexpr int kJoinRows = 8;
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ CachedParams<T> p) {
+__global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ CachedParams<T> p) {
+    constexpr int kEach = D / 32;
     grid_dependency_wait();
     const int32_t* const piece = p.pieces + blockIdx.x * 8;
-    const int32_t count = piece[0];
-    if (count == 0) return;
-    const int32_t row0 = piece[1], rows = piece[2], seq_first = piece[3], head = piece[4];
+    const int32_t count = piece[0], row0 = piece[1], rows = piece[2], seq_first = piece[3], head = piece[4];
+    const int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (count == 0 || r >= rows) return;
     auto part = [&](int32_t i) { return p.partial + ((static_cast<int64_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0)) * (ROWS * (D + 2)); };
-    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-        float most = -INFINITY;
-        for (int32_t i = 0; i < count; ++i) most = fmaxf(most, part(i)[r]);
-        const float shift = most == -INFINITY ? 0.f : most;
-        const int32_t row = row0 + r;
-        const int64_t token = seq_first + row / p.group, q_head = head * p.group + row % p.group;
-        float total = 0.f;
-        for (int32_t i = 0; i < count; ++i) total += part(i)[ROWS + r] * ex2(part(i)[r] - shift);
-        for (int d = threadIdx.x; d < D; d += 128) {
-            float sum = 0.f;
-            for (int32_t i = 0; i < count; ++i) sum += part(i)[2 * ROWS + r * D + d] * ex2(part(i)[r] - shift);
-            p.o[token * p.os[0] + q_head * p.os[1] + d] = VecTraits<T>::from_float(total == 0.f ? 0.f : sum / total);
+    float most = -INFINITY, total = 0.f, sum[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) sum[e] = 0.f;
+    for (int32_t base = 0; base < count; base += 32) {
+        const bool mine = base + lane < count;
+        const float m = mine ? part(base + lane)[r] : -INFINITY, l = mine ? part(base + lane)[ROWS + r] : 0.f;
+        const float top = fmaxf(most, warp_reduce<MaxOp>(m)), shift = top == -INFINITY ? 0.f : top;
+        const float keep = ex2(most - shift), weight = ex2(m - shift);
+        most = top;
+        total = total * keep + warp_reduce<SumOp>(l * weight);
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) sum[e] *= keep;
+        const int32_t n = min(32, count - base);
+#pragma unroll 4
+        for (int32_t i = 0; i < n; ++i) {
+            const float w = __shfl_sync(0xffffffffu, weight, i);
+            const float* const o = part(base + i) + 2 * ROWS + r * D;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) sum[e] = fmaf(o[lane + 32 * e], w, sum[e]);
         }
-        if (p.lse != nullptr && threadIdx.x == 0)
-            p.lse[token * p.q_heads + q_head] = total == 0.f ? -INFINITY : (most + log2f(total)) * 0.6931471805599453f;
     }
+    const int32_t row = row0 + r;
+    const int64_t token = seq_first + row / p.group, q_head = head * p.group + row % p.group;
+    T* const y = p.o + token * p.os[0] + q_head * p.os[1];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) y[lane + 32 * e] = VecTraits<T>::from_float(total == 0.f ? 0.f : sum[e] / total);
+    if (p.lse != nullptr && lane == 0) p.lse[token * p.q_heads + q_head] = total == 0.f ? -INFINITY : (most + log2f(total)) * 0.6931471805599453f;
 }
 
 }  // namespace

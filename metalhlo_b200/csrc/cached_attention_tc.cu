@@ -30,7 +30,6 @@ constexpr int kLeast = 3;              // blocks of a CTA's share where there is
 constexpr float kUnitLog2 = 6.f;       // weights are held times 2^6, so that those far below the largest keep some bits of fp16
 constexpr float kUnit = 64.f;
 constexpr float kGrowth = 8.f;         // log2 of what scores may exceed the last maximum by before it moves
-constexpr float kSumLimit = 32768.f;   // weights of a row and block, in fp16
 // Registers: 512 threads are launched with 128 each, 512 for every four lanes of the four warpgroups. The softmax holds a row's 128
 // scores and weights; the others have little.
 constexpr int kSoftmaxRegs = 168, kOtherRegs = 88;
@@ -96,52 +95,52 @@ struct Blocks {
     }
 };
 
-// Exponentials of a row's 128 scores, packed over the score columns they came from. MASK: some columns are hidden. CHECK: m comes from
-// earlier blocks, and nothing is written unless all the warp's sums stay within fp16 (*stored). Returns the row's sum of weights.
-template <bool MASK, bool CHECK>
-__device__ __forceinline__ float exponentials(uint32_t taddr, const Scales& sc, float factor, float m, int32_t key0, int32_t seen, bool* stored) {
-    uint32_t packed[2][32];
-    float weights = 0.f, all = 0.f;
+// The weights of 64 of a row's scores, packed; *sum: what they add to the row's sum. MASK: some columns are hidden.
+template <bool MASK>
+__device__ __forceinline__ void weights_of(const uint32_t* sr, const Scales& sc, int g0, float factor, float m, int32_t key0, int32_t seen, uint32_t* packed, float* total) {
 #pragma unroll
-    for (int ci = 0; ci < 2; ++ci) {
-        uint32_t sr[64];
-        tmem_ld32(taddr + ci * 64, sr);
-        tmem_ld32(taddr + ci * 64 + 32, sr + 32);
-        tmem_ld_wait();
+    for (int gi = 0; gi < 4; ++gi) {
+        const int g = g0 + gi;
+        const float f = factor * sc.key[g], off = sc.ratio_log2[g] + (kUnitLog2 - m);
+        const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
+        const bool hidden = MASK && (sc.missing >> g & 1);
+        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int gi = 0; gi < 4; ++gi) {
-            const int g = ci * 4 + gi;
-            const float f = factor * sc.key[g], off = sc.ratio_log2[g] + (kUnitLog2 - m);
-            const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
-            const bool hidden = MASK && (sc.missing >> g & 1);
-            float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int c = 0; c < 16; c += 2) {
-                const int at = gi * 16 + c;
-                const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[at]), __uint_as_float(sr[at + 1])), f2, off2);
-                float2 e = make_float2(ex2(x.x), ex2(x.y));
-                if (MASK) {
-                    if (hidden || key0 + g * 16 + c >= seen) e.x = 0.f;
-                    if (hidden || key0 + g * 16 + c + 1 >= seen) e.y = 0.f;
-                }
-                sum = __fadd2_rn(sum, e);
-                packed[ci][at / 2] = pack_f16(e.x, e.y);
+        for (int c = 0; c < 16; c += 2) {
+            const int at = gi * 16 + c;
+            const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[at]), __uint_as_float(sr[at + 1])), f2, off2);
+            float2 e = make_float2(ex2(x.x), ex2(x.y));
+            if (MASK) {
+                if (hidden || key0 + at >= seen) e.x = 0.f;
+                if (hidden || key0 + at + 1 >= seen) e.y = 0.f;
             }
-            const float s = sum.x + sum.y;
-            all += s;
-            weights = MASK && s == 0.f ? weights : fmaf(s, sc.out_again[g], weights);
+            sum = __fadd2_rn(sum, e);
+            packed[at / 2] = pack_f16(e.x, e.y);
         }
-        if (!CHECK) tmem_st32(taddr + ci * 32, packed[ci]);  // those columns have been read
+        const float s = sum.x + sum.y;
+        *total = MASK && s == 0.f ? *total : fmaf(s, sc.out_again[g], *total);
     }
-    if (CHECK) {
-        const bool safe = !__any_sync(0xffffffffu, !(all < kSumLimit));
-        if (safe) {
+}
+
+// The largest of 64 scores in units of log2(e); hidden ones are not looked at.
+template <bool MASK>
+__device__ __forceinline__ float largest_of(const uint32_t* sr, const Scales& sc, int g0, float factor, int32_t key0, int32_t seen) {
+    float mx = -INFINITY;
 #pragma unroll
-            for (int ci = 0; ci < 2; ++ci) tmem_st32(taddr + ci * 32, packed[ci]);
+    for (int gi = 0; gi < 4; ++gi) {
+        float gm = -INFINITY;
+        if (MASK) {
+            const bool hidden = sc.missing >> (g0 + gi) & 1;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) gm = hidden || key0 + gi * 16 + c >= seen ? gm : fmaxf(gm, __uint_as_float(sr[gi * 16 + c]));
+            mx = gm == -INFINITY ? mx : fmaxf(mx, gm * (factor * sc.key[g0 + gi]));
+        } else {
+#pragma unroll
+            for (int c = 0; c < 16; c += 2) gm = fmax3(gm, __uint_as_float(sr[gi * 16 + c]), __uint_as_float(sr[gi * 16 + c + 1]));
+            mx = fmaxf(mx, gm * (factor * sc.key[g0 + gi]));
         }
-        *stored = safe;
     }
-    return weights;
+    return mx;
 }
 
 template <typename T, int D>
@@ -456,54 +455,52 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                 const Scales& sc = scales[(block0 + j) % kSlots];
                 const int32_t key0 = (bl.kb0 + j) * kBlockN;
                 const bool mask = __any_sync(0xffffffffu, key0 + kBlockN > seen) || sc.missing != 0;
-                bool done = false;
-                if (j > 0) {
-                    const float m = m_ref == -INFINITY ? 0.f : m_ref;
-                    const float w = mask ? exponentials<true, true>(s_taddr, sc, factor, m, key0, seen, &done) : exponentials<false, true>(s_taddr, sc, factor, m, key0, seen, &done);
-                    if (done) l += w;
-                }
-                if (!done) {
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int ci = 0; ci < 2; ++ci) {
-                        uint32_t sr[64];
-                        tmem_ld32(s_taddr + ci * 64, sr);
-                        tmem_ld32(s_taddr + ci * 64 + 32, sr + 32);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int gi = 0; gi < 4; ++gi) {
-                            const int g = ci * 4 + gi;
-                            const bool hidden = sc.missing >> g & 1;
-                            float gm = -INFINITY;
-#pragma unroll
-                            for (int c = 0; c < 16; ++c) {
-                                const float x = __uint_as_float(sr[gi * 16 + c]);
-                                gm = mask && (hidden || key0 + g * 16 + c >= seen) ? gm : fmaxf(gm, x);
-                            }
-                            mx = gm == -INFINITY ? mx : fmaxf(mx, gm * (factor * sc.key[g]));
-                        }
-                    }
-                    const bool grow = mx > m_ref + kGrowth;
-                    float alpha = 1.f;
-                    if (grow) {
-                        alpha = m_ref == -INFINITY ? 0.f : ex2(m_ref - mx);
-                        m_ref = mx;
-                        l *= alpha;
-                    }
-                    // every product with values so far completed before these scores were signalled: O may be rescaled here
-                    if (j > 0 && __any_sync(0xffffffffu, grow)) {
+                // Two chunks of 64 keys, the loop not unrolled: instruction fetch was a third of the stalls with both and a variant that
+                // took the maximum of earlier blocks for granted. A chunk looks at its own maximum first; where it would push weights out of
+                // fp16 (a piece's first chunk, rarely later) everything so far is scaled anew. Every product with values so far completed
+                // before these scores were signalled.
 #pragma unroll 1
-                        for (int c0 = 0; c0 < D; c0 += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(o_taddr + c0, o);
+                for (int ci = 0; ci < 2; ++ci) {
+                    const int32_t first = key0 + ci * 64;
+                    uint32_t sr[64], packed[32];
+                    tmem_ld32(s_taddr + ci * 64, sr);
+                    tmem_ld32(s_taddr + ci * 64 + 32, sr + 32);
+                    tmem_ld_wait();
+                    const float mx = mask ? largest_of<true>(sr, sc, ci * 4, factor, first, seen) : largest_of<false>(sr, sc, ci * 4, factor, first, seen);
+                    const bool grow = mx > m_ref + kGrowth;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        float alpha = 1.f;
+                        if (grow) {
+                            alpha = m_ref == -INFINITY ? 0.f : ex2(m_ref - mx);
+                            m_ref = mx;
+                            l *= alpha;
+                        }
+                        // O of earlier blocks (j > 0), then this block's first weights (ci > 0)
+#pragma unroll 1
+                        for (int c0 = j > 0 ? 0 : D; c0 < D + (ci > 0 ? 32 : 0); c0 += 32) {
+                            const uint32_t at = c0 < D ? o_taddr + c0 : s_taddr;
+                            uint32_t w[32];
+                            if (c0 >= D) tmem_st_wait();  // this thread's own store of them
+                            tmem_ld32(at, w);
                             tmem_ld_wait();
+                            if (c0 < D) {
 #pragma unroll
-                            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
-                            tmem_st32(o_taddr + c0, o);
+                                for (int c = 0; c < 32; ++c) w[c] = __float_as_uint(__uint_as_float(w[c]) * alpha);
+                            } else {
+                                const __half2 by = __float2half2_rn(alpha);
+#pragma unroll
+                                for (int c = 0; c < 32; ++c) {
+                                    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&w[c]), by);
+                                    w[c] = *reinterpret_cast<const uint32_t*>(&x);
+                                }
+                            }
+                            tmem_st32(at, w);
                         }
                     }
                     const float m = m_ref == -INFINITY ? 0.f : m_ref;
-                    l += mask ? exponentials<true, false>(s_taddr, sc, factor, m, key0, seen, nullptr) : exponentials<false, false>(s_taddr, sc, factor, m, key0, seen, nullptr);
+                    if (mask) weights_of<true>(sr, sc, ci * 4, factor, m, first, seen, packed, &l);
+                    else weights_of<false>(sr, sc, ci * 4, factor, m, first, seen, packed, &l);
+                    tmem_st32(s_taddr + ci * 32, packed);  // over columns that have been read
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -579,7 +576,7 @@ int launch(CachedParams<T> p, void* scratch, cudaStream_t stream) {
     kernel<<<kGrid, kThreads, Smem<D>::kTotal, stream>>>(p);
     MHLO_CUDA_CHECK_LAUNCH("cached_attention (tcgen05)");
     if (p.whole) return MHLO_CUDA_OK;
-    const cudaError_t e = launch_dependent(join_kernel<T, D, kRows>, dim3(kGrid, 32), dim3(128), 0, stream, 1, true, p);
+    const cudaError_t e = launch_dependent(join_kernel<T, D, kRows>, dim3(kGrid, kRows / kJoinRows), dim3(32 * kJoinRows), 0, stream, 1, true, p);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of cached_attention failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("cached_attention (joining)");
     return MHLO_CUDA_OK;
