@@ -174,13 +174,16 @@ struct Work {
                 inside = 0;
                 continue;
             }
-            const int32_t segment = static_cast<int32_t>(inside / tiles), row_tile = segment / p.kv.heads;
+            // 64-bit divisions are routines of a hundred instructions, and every warp of the tensor-core kernel walks by itself
+            const bool small = inside < 0x80000000ll;
+            const int32_t segment = small ? static_cast<int32_t>(static_cast<uint32_t>(inside) / static_cast<uint32_t>(tiles)) : static_cast<int32_t>(inside / tiles);
+            const int32_t row_tile = segment / p.kv.heads;
             s->s = w.s;
             s->b = b;
-            s->head = segment % p.kv.heads;
+            s->head = segment - row_tile * p.kv.heads;
             s->row0 = row_tile * ROWS;
             s->rows = min(ROWS, w.s.count * p.group - s->row0);
-            s->t0 = static_cast<int32_t>(inside % tiles);
+            s->t0 = static_cast<int32_t>(inside - static_cast<int64_t>(segment) * tiles);
             s->t1 = static_cast<int32_t>(min(static_cast<int64_t>(tiles), s->t0 + (end - at)));
             s->tiles = tiles;
             s->begin = at - s->t0;

@@ -3,8 +3,8 @@
 //
 // A CTA owns 256 rows of a segment as two halves of 128 and walks the keys in blocks of 128:
 //   warp 0             MMA issuer: S_h = Q_h K^T (both operands in shared memory), O_h += P_h V (P read from tensor memory)
-//   warps 1-3, 12-15   producers: codes of keys and values from global memory through registers, half a block ahead, into the
-//                      128-byte-swizzled layout as fp16, exactly
+//   warps 1-3, 12-15   producers: codes of keys and values from global memory a block ahead (asynchronous copies into slots of their
+//                      own lanes), then into the 128-byte-swizzled layout as fp16, exactly
 //   warps 4-7, 8-11    softmax of half 0 / 1, a thread per row: it puts its row of q into shared memory as fp16 at a piece's start and
 //                      writes P over the scores in tensor memory
 // The scales do not touch the codes: a key's scale multiplies its column of scores (16 keys at a time share one), a value's scale goes
@@ -45,7 +45,8 @@ template <int D>
 struct Smem {
     static constexpr int kPanels = D / 64;
     static constexpr int kQHalf = kBlockM * D * 2, kTile = kBlockN * D * 2;
-    static constexpr int kQ = 0, kK = kQ + kHalves * kQHalf, kV = kK + kStages * kTile, kEnd = kV + kStages * kTile;
+    static constexpr int kQ = 0, kK = kQ + kHalves * kQHalf, kV = kK + kStages * kTile, kRaw = kV + kStages * kTile,
+                         kRawTile = kBlockN * D, kEnd = kRaw + 2 * kRawTile;
     static constexpr int kTotal = kEnd + 1024;  // the layout starts on 1024 bytes
 };
 
@@ -67,6 +68,10 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
         : "memory");
+}
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 
 // Four codes as four fp16 numbers: 0x64xx is 1024 + xx, xx = code + 128.
@@ -327,24 +332,27 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                 if (page >= 0) most = fmaxf(most, a.v_scales[static_cast<int64_t>(page) * a.heads + seg.head]);
             }
             most = warp_reduce<MaxOp>(most);
-            uint4 raw_k[kMine], raw_v[kMine];
-            auto load = [&](const int8_t* codes, int64_t from, uint4* raw) {
+            // Codes wait in shared memory, in slots that only the lane that copies them reads: in registers a block of both would not fit,
+            // and half a block ahead they were late (chunks of 512 tokens on 8192: 300 us that way, 215 with no copies at all).
+            auto load = [&](const int8_t* codes, int64_t from, int slots) {
 #pragma unroll
                 for (int i = 0; i < kMine; ++i) {
                     const int pass = wp + i * kProducers, row = pass * kPassRows + row_in_pass;
                     const int64_t b = __shfl_sync(0xffffffffu, from, (pass * kPassRows / 16) & 7);
-                    raw[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);  // marks nothing: replaced by zeros below
-                    if (pass < kPasses && b >= 0) raw[i] = ld_stream16(codes + b + (row & 15) * D + chunk * 16);
+                    if (pass < kPasses && b >= 0) copy16(smem_u32(smem + slots + (pass * 32 + lane) * 16), codes + b + (row & 15) * D + chunk * 16);
                 }
+                asm volatile("cp.async.commit_group;" ::: "memory");
             };
             // zeros: groups whose rows are stored as zeros (no page, or a value scale that is nothing)
-            auto store = [&](int offset, const uint4* raw, uint32_t zeros) {
+            auto store = [&](int offset, int slots, uint32_t zeros) {
+                asm volatile("cp.async.wait_group 1;" ::: "memory");  // all but the newest: keys and values take turns
 #pragma unroll
                 for (int i = 0; i < kMine; ++i) {
                     const int pass = wp + i * kProducers, row = pass * kPassRows + row_in_pass;
                     if (pass >= kPasses) break;
                     const bool zero = zeros >> (pass * kPassRows / 16) & 1;
-                    const uint2 c0 = codes_f16(raw[i].x), c1 = codes_f16(raw[i].y), c2 = codes_f16(raw[i].z), c3 = codes_f16(raw[i].w);
+                    const uint4 raw = *reinterpret_cast<const uint4*>(smem + slots + (pass * 32 + lane) * 16);
+                    const uint2 c0 = codes_f16(raw.x), c1 = codes_f16(raw.y), c2 = codes_f16(raw.z), c3 = codes_f16(raw.w);
                     uint8_t* const at = smem + offset + (chunk >> 2) * kBlockN * 128 + row * 128;
                     const int c = (chunk & 3) * 2;
                     *reinterpret_cast<uint4*>(at + ((c ^ (row & 7)) << 4)) = zero ? make_uint4(0, 0, 0, 0) : make_uint4(c0.x, c0.y, c1.x, c1.y);
@@ -353,9 +361,9 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                 fence_proxy_async();
                 __syncwarp();
             };
-            load(a.k_codes, now.base, raw_k);
+            load(a.k_codes, now.base, L::kRaw);
+            load(a.v_codes, now.base, L::kRaw + L::kRawTile);
             for (int j = 0; j < bl.count && ok; ++j, ++block) {
-                load(a.v_codes, now.base, raw_v);
                 const Groups after = look_up(j + 2);
                 const float ratio = most > 0.f ? now.vs / most : now.vs * 0.f;  // NaN stays
                 const bool nothing = ratio < 1e-18f;
@@ -374,13 +382,14 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                         v_most[block % kSlots] = most;
                     }
                 }
-                store(L::kK + stage * L::kTile, raw_k, missing);
+                store(L::kK + stage * L::kTile, L::kRaw, missing);
                 if (lane == 0) mbar_arrive(&k_full[stage]);
-                load(a.k_codes, next.base, raw_k);
+                load(a.k_codes, next.base, L::kRaw);
                 wait(&v_empty[stage], phase ^ 1, 7);
                 if (!ok) break;
-                store(L::kV + stage * L::kTile, raw_v, no_value);
+                store(L::kV + stage * L::kTile, L::kRaw + L::kRawTile, no_value);
                 if (lane == 0) mbar_arrive(&v_full[stage]);
+                load(a.v_codes, next.base, L::kRaw + L::kRawTile);
                 now = next;
                 next = after;
                 if (++stage == kStages) {
@@ -389,6 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                 }
             }
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
         // ---- softmax
         const int h = (warp - 4) >> 2, quarter = warp & 3, r = h * kBlockM + quarter * 32 + lane;
