@@ -149,9 +149,8 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
     Work<kRows, kTileKeys, kLeastTiles, false> work;
     const bool any = work.template start<L::kThreads>(p, scratch);
     grid_dependency_release();
-    if (!any) return;
     Segment seg;
-    while (work.next(p, &seg)) {
+    while (any && work.next(p, &seg)) {
         const int32_t b = seg.b, head = seg.head, t0 = seg.t0, rows = seg.rows;
         auto seen_by = [&](int r) { return seg.seen_by(r, p.group); };
         const int32_t limit = seen_by(rows - 1), least = seen_by(0);
@@ -571,9 +570,10 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
         if (seg.cut && tid == 0) work.leave_piece(p, seg);
         __syncthreads();
     }
+    // Where the kernel of many rows went before, this one began as that one's CTAs ended (their rows are not these); what joins the
+    // pieces of both waits for this kernel alone, so this kernel ends after that one.
+    grid_dependency_wait();
 }
-
-int64_t few_rows_scratch(int64_t dim) { return kGrid * (8 * 4 + 2 * 16 * (dim + 2) * 4); }
 
 // Sequences of up to this many rows are this kernel's, where the other takes the type: at 32 rows two passes of 16 over the keys cost
 // what one of 128 does there (6 us and 12.5 over 8 x 6000 keys of head dimension 128).
@@ -583,28 +583,45 @@ bool long_takes(int64_t head_dim) { return head_dim == 64 || head_dim == 128; }
 bool may_be_long(const int32_t* starts, int64_t tokens, int64_t group) { return starts != nullptr && tokens * group > kFewRows; }
 
 template <typename T, int D, int NT>
-int launch_rows(CachedParams<T> p, void* scratch, cudaStream_t stream) {
+int launch_rows(const CachedParams<T>& p, bool behind, cudaStream_t stream) {
     using L = Layout<D>;
-    p.pieces = static_cast<int32_t*>(scratch);
-    p.partial = reinterpret_cast<float*>(p.pieces + kGrid * 8);
     constexpr int smem = L::kRing + L::kSteps * NT * 32 * 8 * (sizeof(T) == 4 ? 2 : 1);
     auto kernel = cached_attention_kernel<T, D, NT>;
     static std::atomic<bool> smem_set[64];
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, smem_set)) return st;
-    kernel<<<kGrid, L::kThreads, smem, stream>>>(p);
-    MHLO_CUDA_CHECK_LAUNCH("cached_attention");
-    if (p.whole) return MHLO_CUDA_OK;
-    const cudaError_t e = launch_dependent(join_kernel<T, D, 8 * NT>, dim3(kGrid, NT), dim3(32 * kJoinRows), 0, stream, 1, true, p);
+    const cudaError_t e = launch_dependent(kernel, dim3(kGrid), dim3(L::kThreads), smem, stream, 1, behind, p);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of cached_attention failed: %s", cudaGetErrorString(e));
-    MHLO_CUDA_CHECK_LAUNCH("cached_attention (joining)");
+    MHLO_CUDA_CHECK_LAUNCH("cached_attention");
     return MHLO_CUDA_OK;
 }
 
 template <typename T, int D>
-int launch_dim(const CachedParams<T>& p, void* scratch, cudaStream_t stream) {
+int launch_dim(CachedParams<T> p, void* scratch, cudaStream_t stream) {
+    // Which kernels: sequences of many rows go to the one, where there may be any, the rest to the other. One sequence by itself that may
+    // have many rows goes to the one whatever it has.
+    const bool may_long = sizeof(T) == 2 && long_takes(D) && may_be_long(p.kv.starts, p.kv.tokens, p.group);
+    const bool few = !may_long || p.kv.seqs > 1;
+    CachedParams<T> many = p;
+    many.few_rows = p.few_rows = !may_long ? 0x7fffffff : few ? kFewRows : 0;
     // groups of 8 rows as long as the sequences have no more on average
-    if (static_cast<int64_t>(p.kv.tokens) * p.group <= 8 * static_cast<int64_t>(p.kv.seqs)) return launch_rows<T, D, 1>(p, scratch, stream);
-    return launch_rows<T, D, 2>(p, scratch, stream);
+    const int groups = static_cast<int64_t>(p.kv.tokens) * p.group <= 8 * static_cast<int64_t>(p.kv.seqs) ? 1 : 2;
+    cached_scratch(&p, scratch);
+    if constexpr (sizeof(T) == 2 && (D == 64 || D == 128)) {
+        if (may_long) {
+            cached_scratch(&many, scratch != nullptr ? static_cast<uint8_t*>(scratch) + cached_scratch(16, D) : nullptr);
+            if (int st = cached_attention_long(many, stream)) return st;
+        }
+    }
+    if (few) {
+        if (int st = groups == 1 ? launch_rows<T, D, 1>(p, may_long, stream) : launch_rows<T, D, 2>(p, may_long, stream)) return st;
+    }
+    if (p.whole) return MHLO_CUDA_OK;
+    const int first = may_long ? kLongRows : 8 * groups, second = may_long && few ? 8 * groups : 0;
+    const cudaError_t e = launch_dependent(join_kernel<T, D>, dim3(kGrid, (first + second) / kJoinRows), dim3(32 * kJoinRows), 0, stream, 1, true,
+                                           may_long ? many : p, first, static_cast<const int32_t*>(p.pieces), static_cast<const float*>(p.partial), second);
+    if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of cached_attention failed: %s", cudaGetErrorString(e));
+    MHLO_CUDA_CHECK_LAUNCH("cached_attention (joining)");
+    return MHLO_CUDA_OK;
 }
 
 template <typename T>
@@ -622,14 +639,6 @@ int launch(const KvArgs& kv, const void* q, const int64_t* qs, int64_t q_heads, 
     constexpr int64_t E = VecTraits<T>::kElems;
     p.q_vec = aligned16(q) && qs[0] % E == 0 && qs[1] % E == 0;
     p.o_vec = aligned16(o) && os[0] % E == 0 && os[1] % E == 0 ? 2 : reinterpret_cast<uintptr_t>(o) % (4 * sizeof(T)) == 0 && os[0] % 4 == 0 && os[1] % 4 == 0;
-    p.few_rows = 0x7fffffff;
-    if constexpr (sizeof(T) == 2) {
-        if (may_be_long(kv.starts, kv.tokens, p.group) && long_takes(kv.head_dim)) {
-            p.few_rows = kFewRows;
-            if (int st = cached_attention_long(p, scratch, stream)) return st;
-            if (scratch != nullptr) scratch = static_cast<uint8_t*>(scratch) + cached_attention_long_scratch(kv.head_dim);
-        }
-    }
     switch (kv.head_dim) {
         case 64: return launch_dim<T, 64>(p, scratch, stream);
         case 96: return launch_dim<T, 96>(p, scratch, stream);
@@ -655,9 +664,9 @@ int64_t mhlo_cuda_cached_attention_scratch_bytes(const mhlo_cuda_kv_cache* cache
     if (!cache || !batch || q_heads < 1) return 0;
     if (cache->head_dim < 1 || batch->pages_per_seq * cache->page_tokens <= kLeastTiles * kTileKeys) return 0;  // no segment is worth cutting
     const int64_t group = q_heads / std::max<int64_t>(1, cache->heads);
-    int64_t bytes = few_rows_scratch(cache->head_dim);
+    int64_t bytes = cached_scratch(16, cache->head_dim);
     if (may_be_long(batch->token_starts, batch->tokens, group) && long_takes(cache->head_dim))
-        bytes += cached_attention_long_scratch(static_cast<int>(cache->head_dim));
+        bytes += cached_scratch(kLongRows, cache->head_dim);
     return bytes;
 }
 

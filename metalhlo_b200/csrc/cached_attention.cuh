@@ -30,6 +30,15 @@ struct CachedParams {
     float* partial;     // [kGrid][2][ROWS (head_dim + 2)]: maxima (log2), sums, outputs
 };
 
+// Scratch of one of the kernels, its rows of a segment given: pieces, then partial results.
+constexpr int64_t cached_scratch(int64_t rows, int64_t dim) { return kGrid * (8 * 4 + 2 * rows * (dim + 2) * 4); }
+template <typename T>
+void cached_scratch(CachedParams<T>* p, void* scratch) {
+    p->pieces = static_cast<int32_t*>(scratch);
+    p->partial = reinterpret_cast<float*>(p->pieces + kGrid * 8);
+}
+constexpr int kLongRows = 256;
+
 struct Piece {  // what joining a cut segment needs: CTAs it goes over, its rows
     int32_t count, first_row, rows, seq_first, head, pad[3];
 };
@@ -215,16 +224,21 @@ struct Work {
 
 // Joins the pieces of the segment that CTA blockIdx.x began and others went on with: sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
 // A warp per row, kJoinRows rows to a CTA (blockIdx.y): the maxima and sums of up to 32 pieces are read at once, a lane each.
+// The first ROWS / kJoinRows of y join p's pieces, those behind them other's (of other_rows): one launch after both kernels.
 constexpr int kJoinRows = 8;
-template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ CachedParams<T> p) {
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ CachedParams<T> p, int32_t of_segment, const int32_t* other_pieces,
+                                                              const float* other_partial, int32_t other_of_segment) {
     constexpr int kEach = D / 32;
     grid_dependency_wait();
-    const int32_t* const piece = p.pieces + blockIdx.x * 8;
+    const bool second = static_cast<int32_t>(blockIdx.y) * kJoinRows >= of_segment;
+    const int32_t ROWS = second ? other_of_segment : of_segment;
+    const float* const partial = second ? other_partial : p.partial;
+    const int32_t* const piece = (second ? other_pieces : p.pieces) + blockIdx.x * 8;
     const int32_t count = piece[0], row0 = piece[1], rows = piece[2], seq_first = piece[3], head = piece[4];
-    const int r = blockIdx.y * kJoinRows + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int r = blockIdx.y * kJoinRows - (second ? of_segment : 0) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (count == 0 || r >= rows) return;
-    auto part = [&](int32_t i) { return p.partial + ((static_cast<int64_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0)) * (ROWS * (D + 2)); };
+    auto part = [&](int32_t i) { return partial + ((static_cast<int64_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0)) * (ROWS * (D + 2)); };
     float most = -INFINITY, total = 0.f, sum[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) sum[e] = 0.f;
@@ -256,10 +270,9 @@ __global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_const
 
 }  // namespace
 
-// Sequences of many rows (16-bit types, head dimension 64 or 128): cached_attention_tc.cu.
+// The kernel of many rows (16-bit types, head dimension 64 or 128; cached_attention_tc.cu), with p's scratch set. Joining is the caller's.
 template <typename T>
-int cached_attention_long(CachedParams<T> p, void* scratch, cudaStream_t stream);
-int64_t cached_attention_long_scratch(int head_dim);
+int cached_attention_long(const CachedParams<T>& p, cudaStream_t stream);
 int cached_attention_long_device_error();
 
 }  // namespace mhlo

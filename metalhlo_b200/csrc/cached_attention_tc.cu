@@ -1,7 +1,7 @@
 // Attention over the paged 8-bit cache for sequences with many rows (chunks of a prompt, long drafts): the products on tcgen05, bf16
 // and fp16, head dimension 64 or 128.
 //
-// A CTA owns 256 rows of a segment as two halves of 128 and walks the keys in blocks of 128:
+// A CTA owns 256 rows of a segment as two halves of 128 and walks the keys in blocks of 128, two steps of 64 each:
 //   warp 0             MMA issuer: S_h = Q_h K^T (both operands in shared memory), O_h += P_h V (P read from tensor memory)
 //   warps 1-3, 12-15   producers: codes of keys and values from global memory a block ahead (asynchronous copies into slots of their
 //                      own lanes), then into the 128-byte-swizzled layout as fp16, exactly
@@ -10,6 +10,10 @@
 // The scales do not touch the codes: a key's scale multiplies its column of scores (16 keys at a time share one), a value's scale goes
 // into the exponent of the weights as its ratio to the largest of the piece, so the products run on integers up to 127.
 // Rows that are fp16 stay as they are; bf16 rows are brought to the same size by powers of two, which is exact.
+//
+// A half has two sets of scores (64 columns of tensor memory, O another head_dim): while the softmax works on step t the scores of
+// t + 1 are there already, and those of t + 2 go out behind P.V of t, whose weights lie in the same columns. With one set of 128
+// columns the softmax stood and waited for a third of the time; now it is what bounds a block, 1.1 us a step of either half.
 //
 // Per block and CTA the tensor pipe needs about 2050 clocks (4096 multiply-adds a clock), the exponentials as many (16 a clock), and
 // the producers some 2000 warp instructions beside the 6000 of the softmax, out of 4 a clock: three limits close together. Decoding
@@ -24,6 +28,7 @@
 namespace mhlo {
 namespace {
 
+constexpr int kStep = 64;  // keys whose scores are taken at once
 constexpr int kBlockM = 128, kHalves = 2, kRows = kHalves * kBlockM, kBlockN = 128, kStages = 2, kThreads = 512, kProducers = 7, kSlots = 4;
 constexpr int kGroups = kBlockN / 16;  // keys with one scale
 constexpr int kLeast = 3;              // blocks of a CTA's share where there is little to do: 384 keys, as in the kernel of few rows
@@ -83,20 +88,21 @@ __device__ __forceinline__ uint2 codes_f16(uint32_t w) {
     return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// What the roles need of a piece: blocks from kb0 on, how many each half takes part in (a half whose rows see nothing of the last ones
-// leaves them out; the second may have no rows at all).
+// What the roles need of a piece: blocks from kb0 on, and how many steps each half takes part in (a half whose rows see nothing of the
+// last ones leaves them out; the second may have no rows at all).
 struct Blocks {
-    int32_t kb0, count, of_half[kHalves], limit;
+    int32_t kb0, count, steps, of_half[kHalves], limit;
     __device__ __forceinline__ Blocks(const Segment& s, int32_t group) {
         kb0 = s.t0;
-        count = 0;
+        steps = 0;
         limit = s.seen_by(s.rows - 1, group);
         for (int h = 0; h < kHalves; ++h) {
             const int32_t rows = min(kBlockM, s.rows - h * kBlockM);
             const int32_t seen = rows > 0 ? s.seen_by(h * kBlockM + rows - 1, group) : 0;
-            of_half[h] = max(0, min(s.t1, (seen + kBlockN - 1) / kBlockN) - kb0);
-            count = max(count, of_half[h]);
+            of_half[h] = max(0, min(2 * s.t1, (seen + kStep - 1) / kStep) - 2 * kb0);
+            steps = max(steps, of_half[h]);
         }
+        count = (steps + 1) / 2;
     }
 };
 
@@ -153,20 +159,22 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
     using L = Smem<D>;
     using Works = Work<kRows, kBlockN, kLeast, true>;
     constexpr int kPanels = L::kPanels;
-    constexpr uint32_t kTmemCols = 512, kSCol = 0, kOCol = kHalves * kBlockN;
+    constexpr uint32_t kTmemCols = 512, kSCol = 0, kOCol = kHalves * 2 * kStep;  // scores: [half][set][64]
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    __shared__ uint64_t bars[4 * kHalves + 4 * kStages];
+    __shared__ uint64_t bars[7 * kHalves + 4 * kStages];
     __shared__ uint32_t tmem_slot;
     __shared__ typename Works::Scratch scratch;
     __shared__ Scales scales[kSlots];
     __shared__ float v_most[kSlots];  // the largest value scale of the piece that a slot's block is of
     uint64_t* const q_full = bars;
-    uint64_t* const s_full = q_full + kHalves;    // scores of the half's block are in tensor memory
-    uint64_t* const p_full = s_full + kHalves;    // its weights are, and O is rescaled if need be
-    uint64_t* const pv_done = p_full + kHalves;   // every product with values so far has completed
-    uint64_t* const k_full = pv_done + kHalves;
+    uint64_t* const s_full = q_full + kHalves;      // [half][set]: scores of a step are in tensor memory
+    uint64_t* const p_full = s_full + 2 * kHalves;  // [half][set]: its weights are, and O is rescaled if need be
+    // [half][set]: the step's product with values, and every one before it, has completed. A wait knows a phase only from its
+    // neighbours: with one barrier for both sets the last two products of a piece could complete before anybody looked.
+    uint64_t* const pv_done = p_full + 2 * kHalves;
+    uint64_t* const k_full = pv_done + 2 * kHalves;
     uint64_t* const k_empty = k_full + kStages;
     uint64_t* const v_full = k_empty + kStages;
     uint64_t* const v_empty = v_full + kStages;
@@ -175,9 +183,11 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
     if (tid == 0) {
         for (int h = 0; h < kHalves; ++h) {
             mbar_init(&q_full[h], 4);
-            mbar_init(&s_full[h], 1);
-            mbar_init(&p_full[h], 4);
-            mbar_init(&pv_done[h], 1);
+            for (int set = 0; set < 2; ++set) {
+                mbar_init(&pv_done[2 * h + set], 1);
+                mbar_init(&s_full[2 * h + set], 1);
+                mbar_init(&p_full[2 * h + set], 4);
+            }
         }
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&k_full[s], kProducers);
@@ -212,84 +222,73 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
 
     if (warp == 0) {
-        // ---- MMA issuer. Order on the pipe: for each half P.V of this block, then S of the next (of this piece, or the first of the
-        // next one): S overwrites the half's scores and weights only after its P.V has read them.
-        const uint32_t idesc_s = (1u << 4) | (static_cast<uint32_t>(kBlockN >> 3) << 17) | (static_cast<uint32_t>(kBlockM >> 4) << 24);
+        // ---- MMA issuer. Order on the pipe: for each half P.V of step t, then the scores of step t + 2, which overwrite the weights
+        // that this P.V has read.
+        const uint32_t idesc_s = (1u << 4) | (static_cast<uint32_t>(kStep >> 3) << 17) | (static_cast<uint32_t>(kBlockM >> 4) << 24);
         const uint32_t idesc_o = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(kBlockM >> 4) << 24);
         const uint32_t q_addr = smem_u32(smem + L::kQ), k_addr = smem_u32(smem + L::kK), v_addr = smem_u32(smem + L::kV);
         auto commit_to = [&](uint64_t* bar) {
             if (elect_one()) umma_commit(bar);
             __syncwarp();
         };
-        auto issue_s = [&](int h, int stage) {
-            const uint32_t qa = q_addr + h * L::kQHalf, ka = k_addr + stage * L::kTile;
+        auto issue_s = [&](int h, int t, int stage) {
+            const uint32_t qa = q_addr + h * L::kQHalf, ka = k_addr + stage * L::kTile + (t & 1) * kStep * 128;
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
                 const uint64_t da = make_smem_desc(qa + (kk / 4) * kBlockM * 128 + (kk % 4) * 32, 16, 1024);
                 const uint64_t db = make_smem_desc(ka + (kk / 4) * kBlockN * 128 + (kk % 4) * 32, 16, 1024);
-                if (elect_one()) umma_f16(tmem + kSCol + h * kBlockN, da, db, idesc_s, kk != 0 ? 1u : 0u);
+                if (elect_one()) umma_f16(tmem + kSCol + (2 * h + (t & 1)) * kStep, da, db, idesc_s, kk != 0 ? 1u : 0u);
             }
-            commit_to(&s_full[h]);
+            commit_to(&s_full[2 * h + (t & 1)]);
         };
-        auto issue_pv = [&](int h, int stage, bool accumulate) {
-            const uint32_t va = v_addr + stage * L::kTile;
+        auto issue_pv = [&](int h, int t, int stage) {
+            const uint32_t va = v_addr + stage * L::kTile + (t & 1) * kStep * 128;
 #pragma unroll
-            for (int kk = 0; kk < kBlockN / 16; ++kk) {
+            for (int kk = 0; kk < kStep / 16; ++kk) {
                 const uint64_t db = make_smem_desc(va + kk * 16 * 128, kBlockN * 128, 1024);
-                if (elect_one()) umma_ts(tmem + kOCol + h * D, tmem + kSCol + h * kBlockN + kk * 8, db, idesc_o, accumulate || kk != 0 ? 1u : 0u);
+                if (elect_one()) umma_ts(tmem + kOCol + h * D, tmem + kSCol + (2 * h + (t & 1)) * kStep + kk * 8, db, idesc_o, t > 0 || kk != 0 ? 1u : 0u);
             }
-            commit_to(&pv_done[h]);
+            commit_to(&pv_done[2 * h + (t & 1)]);
         };
-        auto next_blocks = [&](Blocks* out) {
-            while (work.next(p, &seg)) {
-                *out = Blocks(seg, p.group);
-                if (out->count > 0) return true;
-            }
-            return false;
-        };
-        Blocks cur(Segment{}, 1), nxt(Segment{}, 1);
-        bool has = next_blocks(&cur);
-        int stage = 0;
-        uint32_t phase = 0, it[kHalves] = {0, 0}, q_of[kHalves] = {0, 0};  // q_of: pieces the half has had blocks of
-        // scores of half h in block j of a piece
-        auto scores = [&](const Blocks& of, int j, int h, int st, uint32_t ph) {
-            const bool takes_part = j < of.of_half[h];
-            if (takes_part && j == 0) wait(&q_full[h], q_of[h]++ & 1, 1);
-            if (h == 0) wait(&k_full[st], ph, 2);
-            if (!ok) return;
-            if (takes_part) {
-                tc_fence_after();
-                issue_s(h, st);
-            }
-            if (h == kHalves - 1) commit_to(&k_empty[st]);
-        };
-        if (has)
-            for (int h = 0; h < kHalves; ++h) scores(cur, 0, h, 0, 0);
-        while (has && ok) {
-            const bool more_pieces = next_blocks(&nxt);
-            for (int j = 0; j < cur.count && ok; ++j) {
-                const bool last = j + 1 == cur.count;
-                const int next_stage = stage + 1 == kStages ? 0 : stage + 1;
-                const uint32_t next_phase = stage + 1 == kStages ? phase ^ 1 : phase;
-                wait(&v_full[stage], phase, 3);
+        uint32_t k_block = 0, v_block = 0;  // blocks so far: stage and parity
+        uint32_t weights[2 * kHalves] = {0, 0, 0, 0}, q_of[kHalves] = {0, 0};
+        while (ok && work.next(p, &seg)) {
+            const Blocks bl(seg, p.group);
+            if (bl.count == 0) continue;
+            // scores of step t, both halves or one (they come in order); the block's last scores free its keys
+            auto scores = [&](int t, int h) {
+                if (t >= bl.steps) return;
+                const uint32_t block = k_block + static_cast<uint32_t>(t >> 1);
+                if (h == 0 && (t & 1) == 0) wait(&k_full[block % kStages], block / kStages & 1, 2);
+                if (t == 0 && bl.of_half[h] > 0) wait(&q_full[h], q_of[h]++ & 1, 1);
+                if (!ok) return;
+                if (t < bl.of_half[h]) {
+                    tc_fence_after();
+                    issue_s(h, t, block % kStages);
+                }
+                if (h == kHalves - 1 && ((t & 1) == 1 || t + 1 == bl.steps)) commit_to(&k_empty[block % kStages]);
+            };
+            for (int t = 0; t < 2; ++t)
+                for (int h = 0; h < kHalves; ++h) scores(t, h);
+            for (int t = 0; t < bl.steps && ok; ++t) {
+                const int stage = v_block % kStages;
+                if ((t & 1) == 0) wait(&v_full[stage], v_block / kStages & 1, 3);
                 for (int h = 0; h < kHalves && ok; ++h) {
-                    if (j < cur.of_half[h]) {
-                        wait(&p_full[h], it[h] & 1, 4);
+                    if (t < bl.of_half[h]) {
+                        const int set = 2 * h + (t & 1);
+                        wait(&p_full[set], weights[set]++ & 1, 4);
                         if (!ok) break;
                         tc_fence_after();
-                        issue_pv(h, stage, j > 0);
-                        ++it[h];
+                        issue_pv(h, t, stage);
                     }
-                    if (h == kHalves - 1) commit_to(&v_empty[stage]);
-                    if (!last) scores(cur, j + 1, h, next_stage, next_phase);
+                    scores(t + 2, h);
                 }
-                // the next piece's q comes only when the half is through with this one
-                for (int h = 0; h < kHalves && ok && last && more_pieces; ++h) scores(nxt, 0, h, next_stage, next_phase);
-                stage = next_stage;
-                phase = next_phase;
+                if ((t & 1) == 1 || t + 1 == bl.steps) {
+                    commit_to(&v_empty[stage]);
+                    ++v_block;
+                }
             }
-            cur = nxt;
-            has = more_pieces;
+            k_block += bl.count;
         }
     } else if (warp < 4 || warp >= 12) {
         // ---- producers
@@ -401,166 +400,185 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
         // ---- softmax
-        const int h = (warp - 4) >> 2, quarter = warp & 3, r = h * kBlockM + quarter * 32 + lane;
+        const int h = (warp - 4) >> 2, quarter = warp & 3, row = quarter * 32 + lane, r = h * kBlockM + row;
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-        const uint32_t s_taddr = tmem + lane_base + kSCol + h * kBlockN, o_taddr = tmem + lane_base + kOCol + h * D;
+        const uint32_t s_taddr = tmem + lane_base + kSCol + h * 2 * kStep, o_taddr = tmem + lane_base + kOCol + h * D;
         const float to_log2 = p.scale * 1.4426950408889634f;
-        uint32_t it = 0, block0 = 0;
+        uint8_t* const q_smem = smem + L::kQ + h * L::kQHalf;  // this half's q; between pieces the way of its rows to and from memory
+        constexpr int kRowLanes = D / 8, kAtOnce = 32 / kRowLanes;  // lanes of 16 bytes a row of 16-bit elements takes
+        auto q_chunk = [&](int of_row, int c) { return q_smem + (c >> 3) * kBlockM * 128 + of_row * 128 + (((c & 7) ^ (of_row & 7)) << 4); };
+        uint32_t sets[2] = {0, 0}, block0 = 0;  // sets: steps so far that used the set
         while (ok && work.next(p, &seg)) {
             const Blocks bl(seg, p.group);
-            const int nb = bl.of_half[h];
+            const int steps = bl.of_half[h];
             const int32_t seen = r < seg.rows ? seg.seen_by(r, p.group) : 0x7fffffff;  // rows that are none hide nothing
+            const int64_t token = seg.token(p, min(r, seg.rows - 1)), q_head = seg.q_head(p, min(r, seg.rows - 1));
             float m_ref = -INFINITY, l = 0.f, factor = 0.f, largest = 0.f;
-            if (nb > 0) {
-                // This row of q. The half's last scores of the piece before are done (this thread has seen them): q may be replaced.
-                uint4 raw[D / 8];
-                const T* const x = r < seg.rows ? p.q + seg.token(p, r) * p.qs[0] + seg.q_head(p, r) * p.qs[1] : nullptr;
+            if (steps > 0) {
+                // This warp's 32 rows of q, whole rows at a time. The half's last scores of the piece before are done (its products with
+                // values are, and they came later): q may be replaced.
+                const int64_t from = token * p.qs[0] + q_head * p.qs[1];
+                float factors = 0.f;
+                uint4 raw[32 / kAtOnce];  // all on the way at once: four at a time took 8 us of a piece
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    raw[c] = make_uint4(0, 0, 0, 0);
-                    if (x == nullptr) continue;
-                    if (p.q_vec) {
-                        raw[c] = __ldcs(reinterpret_cast<const uint4*>(x + c * 8));  // not the read-only path: o may be q
-                    } else {
-                        float f[8];
+                for (int i = 0; i < 32; i += kAtOnce) {
+                    const int which = i + lane / kRowLanes;
+                    const int64_t at = __shfl_sync(0xffffffffu, from, which);
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (h * kBlockM + quarter * 32 + which < seg.rows) {
+                        const T* const x = p.q + at + lane % kRowLanes * 8;
+                        if (p.q_vec) {
+                            w = __ldcs(reinterpret_cast<const uint4*>(x));  // not the read-only path: o may be q
+                        } else {
+                            float f[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) f[e] = VecTraits<T>::to_float(x[c * 8 + e]);
-                        raw[c] = VecTraits<T>::pack(f);
+                            for (int e = 0; e < 8; ++e) f[e] = VecTraits<T>::to_float(x[e]);
+                            w = VecTraits<T>::pack(f);
+                        }
                     }
+                    raw[i / kAtOnce] = w;
                 }
-                int shift = 0;
-                if (kBf16) {
-                    float big = 0.f;
 #pragma unroll
-                    for (int c = 0; c < D / 8; ++c) {
-                        float f[8];
-                        VecTraits<T>::unpack(raw[c], f);
+                for (int i = 0; i < 32; i += kAtOnce) {
+                    const int which = i + lane / kRowLanes, c = lane % kRowLanes;
+                    float f[8];
+                    VecTraits<T>::unpack(raw[i / kAtOnce], f);
+                    float unit = 1.f, mine = to_log2;
+                    if (kBf16) {
+                        float big = 0.f;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(f[e]));
-                    }
-                    if (big > 0.f && big < INFINITY) shift = max(-120, ilogbf(big) - 13);
-                }
-                const float unit = scalbnf(1.f, -shift);
-                factor = scalbnf(to_log2, shift);
-                const int row = r - h * kBlockM;
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    uint4 w = raw[c];
-                    if (kBf16) {
-                        float f[8];
-                        VecTraits<T>::unpack(raw[c], f);
-                        w = make_uint4(pack_f16(f[0] * unit, f[1] * unit), pack_f16(f[2] * unit, f[3] * unit), pack_f16(f[4] * unit, f[5] * unit), pack_f16(f[6] * unit, f[7] * unit));
+                        for (int x = 1; x < kRowLanes; x <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+                        // 2^13 / (the power of two below the largest), and its inverse for the scores; ordinary exponents only
+                        const int e = min(max(static_cast<int>(__float_as_uint(big) >> 23), 24), 254) - 13;
+                        if (big > 0.f && big < INFINITY) {
+                            unit = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+                            mine = to_log2 * __uint_as_float(static_cast<uint32_t>(e) << 23);
+                        }
                     }
-                    *reinterpret_cast<uint4*>(smem + L::kQ + h * L::kQHalf + (c >> 3) * kBlockM * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = w;
+                    *reinterpret_cast<uint4*>(q_chunk(quarter * 32 + which, c)) =
+                        make_uint4(pack_f16(f[0] * unit, f[1] * unit), pack_f16(f[2] * unit, f[3] * unit), pack_f16(f[4] * unit, f[5] * unit), pack_f16(f[6] * unit, f[7] * unit));
+                    // to the lane whose row it is
+                    const float got = __shfl_sync(0xffffffffu, mine, (lane - i) * kRowLanes & 31);
+                    if (lane >= i && lane < i + kAtOnce) factors = got;
                 }
+                factor = factors;
                 fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full[h]);
             }
-            for (int j = 0; j < nb && ok; ++j, ++it) {
-                wait(&s_full[h], it & 1, 8);
+            for (int t = 0; t < steps && ok; ++t) {
+                const int set = t & 1;
+                wait(&s_full[2 * h + set], sets[set]++ & 1, 8);
                 if (!ok) break;
                 tc_fence_after();
-                if (j == 0) largest = v_most[block0 % kSlots];
-                const Scales& sc = scales[(block0 + j) % kSlots];
-                const int32_t key0 = (bl.kb0 + j) * kBlockN;
-                const bool mask = __any_sync(0xffffffffu, key0 + kBlockN > seen) || sc.missing != 0;
-                // Two chunks of 64 keys, the loop not unrolled: instruction fetch was a third of the stalls with both and a variant that
-                // took the maximum of earlier blocks for granted. A chunk looks at its own maximum first; where it would push weights out of
-                // fp16 (a piece's first chunk, rarely later) everything so far is scaled anew. Every product with values so far completed
-                // before these scores were signalled.
+                const Scales& sc = scales[(block0 + (t >> 1)) % kSlots];
+                if (t == 0) largest = v_most[block0 % kSlots];
+                const int32_t first = bl.kb0 * kBlockN + t * kStep;
+                const uint32_t taddr = s_taddr + set * kStep;
+                const bool mask = __any_sync(0xffffffffu, first + kStep > seen) || sc.missing != 0;
+                uint32_t sr[64], packed[32];
+                tmem_ld32(taddr, sr);
+                tmem_ld32(taddr + 32, sr + 32);
+                tmem_ld_wait();
+                // A step looks at its own maximum first; where it would push weights out of fp16 (a piece's first step, rarely later)
+                // the sum and O are scaled anew. The scores were asked for behind the product with values of two steps ago, so only the
+                // last one may be under way.
+                const float mx = mask ? largest_of<true>(sr, sc, set * 4, factor, first, seen) : largest_of<false>(sr, sc, set * 4, factor, first, seen);
+                const bool grow = mx > m_ref + kGrowth;
+                if (__any_sync(0xffffffffu, grow)) {
+                    float alpha = 1.f;
+                    if (grow) {
+                        alpha = m_ref == -INFINITY ? 0.f : ex2(m_ref - mx);
+                        m_ref = mx;
+                        l *= alpha;
+                    }
+                    if (t > 0) {
+                        wait(&pv_done[2 * h + (set ^ 1)], (sets[set ^ 1] - 1) & 1, 10);
+                        tc_fence_after();
 #pragma unroll 1
-                for (int ci = 0; ci < 2; ++ci) {
-                    const int32_t first = key0 + ci * 64;
-                    uint32_t sr[64], packed[32];
-                    tmem_ld32(s_taddr + ci * 64, sr);
-                    tmem_ld32(s_taddr + ci * 64 + 32, sr + 32);
-                    tmem_ld_wait();
-                    const float mx = mask ? largest_of<true>(sr, sc, ci * 4, factor, first, seen) : largest_of<false>(sr, sc, ci * 4, factor, first, seen);
-                    const bool grow = mx > m_ref + kGrowth;
-                    if (__any_sync(0xffffffffu, grow)) {
-                        float alpha = 1.f;
-                        if (grow) {
-                            alpha = m_ref == -INFINITY ? 0.f : ex2(m_ref - mx);
-                            m_ref = mx;
-                            l *= alpha;
-                        }
-                        // O of earlier blocks (j > 0), then this block's first weights (ci > 0)
-#pragma unroll 1
-                        for (int c0 = j > 0 ? 0 : D; c0 < D + (ci > 0 ? 32 : 0); c0 += 32) {
-                            const uint32_t at = c0 < D ? o_taddr + c0 : s_taddr;
-                            uint32_t w[32];
-                            if (c0 >= D) tmem_st_wait();  // this thread's own store of them
-                            tmem_ld32(at, w);
+                        for (int c0 = 0; c0 < D; c0 += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(o_taddr + c0, o);
                             tmem_ld_wait();
-                            if (c0 < D) {
 #pragma unroll
-                                for (int c = 0; c < 32; ++c) w[c] = __float_as_uint(__uint_as_float(w[c]) * alpha);
-                            } else {
-                                const __half2 by = __float2half2_rn(alpha);
-#pragma unroll
-                                for (int c = 0; c < 32; ++c) {
-                                    const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&w[c]), by);
-                                    w[c] = *reinterpret_cast<const uint32_t*>(&x);
-                                }
-                            }
-                            tmem_st32(at, w);
+                            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+                            tmem_st32(o_taddr + c0, o);
                         }
                     }
-                    const float m = m_ref == -INFINITY ? 0.f : m_ref;
-                    if (mask) weights_of<true>(sr, sc, ci * 4, factor, m, first, seen, packed, &l);
-                    else weights_of<false>(sr, sc, ci * 4, factor, m, first, seen, packed, &l);
-                    tmem_st32(s_taddr + ci * 32, packed);  // over columns that have been read
                 }
+                const float m = m_ref == -INFINITY ? 0.f : m_ref;
+                if (mask) weights_of<true>(sr, sc, set * 4, factor, m, first, seen, packed, &l);
+                else weights_of<false>(sr, sc, set * 4, factor, m, first, seen, packed, &l);
+                tmem_st32(taddr, packed);  // over scores that have been read
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[h]);
+                if (lane == 0) mbar_arrive(&p_full[2 * h + set]);
             }
             if (!ok) break;
             // The next piece's first product with values waits for this warp's weights, which come after these reads.
-            if (nb > 0) {
-                wait(&pv_done[h], (it - 1) & 1, 9);
-                if (!ok) break;
-                tc_fence_after();
-            }
+            const int last_set = (steps - 1) & 1;
+            if (steps > 0) wait(&pv_done[2 * h + last_set], (sets[last_set] - 1) & 1, 9);
+            if (!ok) break;
+            if (steps > 0) tc_fence_after();
             const bool nothing = l == 0.f;
             const float unit = largest * (1.f / kUnit), by = seg.cut ? unit : nothing ? 0.f : unit / l;
             float* const out = work.partial(p, seg, D);
-            T* const y = r < seg.rows ? p.o + seg.token(p, r) * p.os[0] + seg.q_head(p, r) * p.os[1] : nullptr;
+            // Results leave through the warp's part of q (its scores are done), so that whole rows are written at a time: 64 fp32 elements of
+            // a row, or all 16-bit ones, at once.
+            const int64_t to = token * p.os[0] + q_head * p.os[1];
+            constexpr int kPassElems = D == 128 ? 64 : 32;  // fp32 elements of a row that its bytes of q hold
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
-                uint32_t o[32];
-                if (nb > 0) {
-                    tmem_ld32(o_taddr + c0, o);
-                    tmem_ld_wait();
-                }
+            for (int c0 = 0; c0 < D; c0 += kPassElems) {
 #pragma unroll
-                for (int c = 0; c < 32; ++c) o[c] = nb == 0 || nothing ? 0u : __float_as_uint(__uint_as_float(o[c]) * by);
-                if (r < seg.rows && seg.cut) {
+                for (int part = 0; part < kPassElems; part += 32) {
+                    uint32_t o[32];
+                    if (steps > 0) {
+                        tmem_ld32(o_taddr + c0 + part, o);
+                        tmem_ld_wait();
+                    }
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) *reinterpret_cast<uint4*>(out + 2 * kRows + r * D + c0 + c) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
-                } else if (r < seg.rows) {
+                    for (int c = 0; c < 32; ++c) o[c] = steps == 0 || nothing ? 0u : __float_as_uint(__uint_as_float(o[c]) * by);
+                    if (seg.cut) {
 #pragma unroll
-                    for (int c = 0; c < 32; c += 8) {
-                        if (p.o_vec == 2) {
-                            *reinterpret_cast<uint4*>(y + c0 + c) =
+                        for (int c = 0; c < 32; c += 4) *reinterpret_cast<uint4*>(q_chunk(row, (part + c) / 4)) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 8)
+                            *reinterpret_cast<uint4*>(q_chunk(row, (c0 + part + c) / 8)) =
                                 make_uint4(pack_out<kBf16>(__uint_as_float(o[c]), __uint_as_float(o[c + 1])), pack_out<kBf16>(__uint_as_float(o[c + 2]), __uint_as_float(o[c + 3])),
                                            pack_out<kBf16>(__uint_as_float(o[c + 4]), __uint_as_float(o[c + 5])), pack_out<kBf16>(__uint_as_float(o[c + 6]), __uint_as_float(o[c + 7])));
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) y[c0 + c + e] = VecTraits<T>::from_float(__uint_as_float(o[c + e]));
-                        }
                     }
                 }
-                __syncwarp();  // loads from tensor memory are the whole warp's
+                __syncwarp();
+                if (seg.cut || c0 + kPassElems >= D) {
+#pragma unroll 4
+                    for (int i = 0; i < 32; i += kAtOnce) {
+                        const int which = i + lane / kRowLanes, c = lane % kRowLanes, of_row = quarter * 32 + which;
+                        const int64_t at = __shfl_sync(0xffffffffu, to, which);
+                        const uint4 w = *reinterpret_cast<const uint4*>(q_chunk(of_row, c));
+                        if (h * kBlockM + of_row >= seg.rows) continue;
+                        if (seg.cut) {
+                            *reinterpret_cast<uint4*>(out + 2 * kRows + (h * kBlockM + of_row) * D + c0 + c * 4) = w;
+                        } else if (p.o_vec == 2) {
+                            *reinterpret_cast<uint4*>(p.o + at + c * 8) = w;
+                        } else {
+                            const T* const x = reinterpret_cast<const T*>(&w);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) p.o[at + c * 8 + e] = x[e];
+                        }
+                    }
+                    __syncwarp();
+                }
             }
             if (r < seg.rows) {
                 if (seg.cut) {
                     out[r] = m_ref;
                     out[kRows + r] = l;
                 } else if (p.lse != nullptr) {
-                    p.lse[seg.token(p, r) * p.q_heads + seg.q_head(p, r)] = nothing ? -INFINITY : (m_ref + log2f(l)) * 0.6931471805599453f;
+                    p.lse[token * p.q_heads + q_head] = nothing ? -INFINITY : (m_ref + log2f(l)) * 0.6931471805599453f;
                 }
             }
             if (seg.cut && r == 0) work.leave_piece(p, seg);
@@ -577,31 +595,25 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
 }
 
 template <typename T, int D>
-int launch(CachedParams<T> p, void* scratch, cudaStream_t stream) {
-    p.pieces = static_cast<int32_t*>(scratch);
-    p.partial = reinterpret_cast<float*>(p.pieces + kGrid * 8);
+int launch(const CachedParams<T>& p, cudaStream_t stream) {
     auto kernel = cached_attention_tc_kernel<T, D>;
     static std::atomic<bool> smem_set[64];
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), Smem<D>::kTotal, smem_set)) return st;
     kernel<<<kGrid, kThreads, Smem<D>::kTotal, stream>>>(p);
     MHLO_CUDA_CHECK_LAUNCH("cached_attention (tcgen05)");
-    if (p.whole) return MHLO_CUDA_OK;
-    const cudaError_t e = launch_dependent(join_kernel<T, D, kRows>, dim3(kGrid, kRows / kJoinRows), dim3(32 * kJoinRows), 0, stream, 1, true, p);
-    if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of cached_attention failed: %s", cudaGetErrorString(e));
-    MHLO_CUDA_CHECK_LAUNCH("cached_attention (joining)");
     return MHLO_CUDA_OK;
 }
 
 }  // namespace
 
 template <typename T>
-int cached_attention_long(CachedParams<T> p, void* scratch, cudaStream_t stream) {
-    return p.kv.head_dim == 64 ? launch<T, 64>(p, scratch, stream) : launch<T, 128>(p, scratch, stream);
+int cached_attention_long(const CachedParams<T>& p, cudaStream_t stream) {
+    static_assert(kRows == kLongRows, "rows of a segment");
+    return p.kv.head_dim == 64 ? launch<T, 64>(p, stream) : launch<T, 128>(p, stream);
 }
-template int cached_attention_long<__half>(CachedParams<__half>, void*, cudaStream_t);
-template int cached_attention_long<__nv_bfloat16>(CachedParams<__nv_bfloat16>, void*, cudaStream_t);
+template int cached_attention_long<__half>(const CachedParams<__half>&, cudaStream_t);
+template int cached_attention_long<__nv_bfloat16>(const CachedParams<__nv_bfloat16>&, cudaStream_t);
 
-int64_t cached_attention_long_scratch(int head_dim) { return kGrid * (8 * 4 + 2 * kRows * (head_dim + 2) * int64_t{4}); }
 int cached_attention_long_device_error() { return take_kv_error(); }
 
 }  // namespace mhlo

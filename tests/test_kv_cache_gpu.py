@@ -297,6 +297,56 @@ def test_attention_reads_and_writes_strided_rows_and_in_place():
     assert torch.equal(q, out) and torch.equal(wide[:, :3], rest[:, :3]) and torch.equal(wide[:, 9:], rest[:, 9:])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (128, 128)])
+def test_chunks_off_the_grid_in_place_and_with_rows_behind(dtype, dim, page):
+    """Many rows: tensors whose rows are off the 16-byte grid, results in place of the queries, one sequence of few rows in a call that
+    could have held many, and rows behind the last sequence."""
+    cuda = cuda_mod()
+    heads, group = 2, 4
+    for new, lengths, behind in (([150, 1, 40], [150, 77, 700], 3), ([5], [333], 60), ([129], [1000], 0)):
+        starts = starts_of(new)
+        pages = sum(-(-n // page) for n in lengths) + 1
+        cache, want = make_cache(pages, heads, page, dim, 31)
+        table = make_table(lengths, page, pages, 32)
+        rows, width = int(starts[-1]) + behind, heads * group * dim + 6
+        flat = torch.randn(rows, width, generator=torch.Generator().manual_seed(33)).to(dtype).cuda()
+        q = flat[:, 3:3 + heads * group * dim].unflatten(1, (heads * group, dim))
+        args = (cache, on_gpu(table), on_gpu(lengths), 0.11)
+        lse = torch.full(q.shape[:2], 5.0, device="cuda")
+        out = torch.full(q.shape, 2.0, dtype=dtype, device="cuda")
+        cuda.cached_attention(q, *args, token_starts=on_gpu(starts), out=out, lse=lse)
+        assert cuda.device_error() == 0
+        check_attention(cache, want, q, table, lengths, starts, 0.11, out, lse, np.full(q.shape, 2.0))
+        assert bool((lse[int(starts[-1]):] == 5).all())
+        before = flat.clone()
+        cuda.cached_attention(q, *args, token_starts=on_gpu(starts), out=q)
+        assert torch.equal(q[:int(starts[-1])], out[:int(starts[-1])])
+        assert torch.equal(flat[int(starts[-1]):], before[int(starts[-1]):]) and torch.equal(flat[:, :3], before[:, :3]) and torch.equal(flat[:, -3:], before[:, -3:])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_chunks_of_unequal_blocks_and_growing_scores(dtype):
+    """Value scales that differ by 2^12 and blocks without values (scale 0), key norms that grow along the sequence: the maximum moves
+    many times, and what was summed up before is scaled anew."""
+    cuda = cuda_mod()
+    page, heads, group, dim, lengths, new = 32, 2, 8, 128, [900, 333], [40, 333]
+    starts = starts_of(new)
+    cache, want = make_cache(42, heads, page, dim, 34)
+    table = make_table(lengths, page, 42, 35)
+    for b, n in enumerate(lengths):
+        for i in range(-(-n // page)):
+            want.scales[0][table[b, i]] *= np.float32(0.05 * (i + 1))
+            want.scales[1][table[b, i]] *= np.float32(0.0 if i % 5 == 3 else 4.0 ** (i % 7 - 3))
+    cache.k_scale.copy_(torch.from_numpy(want.scales[0]))
+    cache.v_scale.copy_(torch.from_numpy(want.scales[1]))
+    q = (2 * torch.randn(int(starts[-1]), heads * group, dim, generator=torch.Generator().manual_seed(36))).to(dtype).cuda()
+    lse = torch.zeros(q.shape[:2], device="cuda")
+    got = cuda.cached_attention(q, cache, on_gpu(table), on_gpu(lengths), 0.2, token_starts=on_gpu(starts), lse=lse)
+    assert cuda.device_error() == 0
+    check_attention(cache, want, q, table, lengths, starts, 0.2, got, lse, np.zeros(q.shape))
+
+
 def test_a_poisoned_block_reaches_only_rows_that_see_it():
     cuda = cuda_mod()
     page, dim = 16, 64
