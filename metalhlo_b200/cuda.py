@@ -488,10 +488,17 @@ def _run_on(device, stream, call):
         return _run_on(device, stream, call)
 
 
+def _dense_like(t):
+    import torch
+
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _same_device(first, *others):
-    assert first.is_cuda
+    device = first.device
+    assert device.type == "cuda"
     for t in others:
-        assert t is None or t.device == first.device, f"{t.device} and {first.device} in one call"
+        assert t is None or t.device == device, f"{t.device} and {device} in one call"
 
 
 class KvCache:
@@ -574,7 +581,7 @@ def kv_cache_append(cache: KvCache, k, v, page_table, lengths, token_starts=None
     assert q_out is None or (q is not None and q_out.shape == q.shape and q_out.dtype == dtype)
 
     def call(s):
-        out = torch.empty(q.shape, dtype=dtype, device=q.device) if q is not None and q_out is None else q_out
+        out = _dense_like(q) if q is not None and q_out is None else q_out
         check(lib.mhlo_cuda_kv_cache_append(torch_dtype_code(dtype), cache.pointer, C.byref(batch), k.data_ptr(), _rows(k), v.data_ptr(), _rows(v),
                                             _ptr(q), q_strides, _ptr(out), None if q is None else _rows(out), q_heads, _ptr(rope), positions, rotary,
                                             1 if interleaved else 0, s))
@@ -620,9 +627,9 @@ def cached_attention(q, cache: KvCache, page_table, lengths, scale: float, token
     batch = _kv_batch(page_table, lengths, token_starts, tokens)
 
     def call(s):
-        o = torch.empty(shape, dtype=dtype, device=q.device) if out is None else out
+        o = _dense_like(q) if out is None else out
         need = lib.mhlo_cuda_cached_attention_scratch_bytes(cache.pointer, C.byref(batch), q_heads)
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need > 0 else None
+        scratch = lengths.new_empty(need >> 2) if need > 0 else None
         check(lib.mhlo_cuda_cached_attention(torch_dtype_code(dtype), q.data_ptr(), _rows(q), cache.pointer, C.byref(batch), q_heads, scale, o.data_ptr(),
                                              _rows(o), _ptr(lse), _ptr(scratch), need, s))
         return o
@@ -690,7 +697,7 @@ def token_logprobs_grad(logits, targets, lse, entropy=None, grad_logprobs=None, 
     assert out is None or (out.shape == logits.shape and out.dtype == logits.dtype)
 
     def call(s):
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device) if out is None else out
+        dx = _dense_like(logits) if out is None else out
         check(lib.mhlo_cuda_token_logprobs_grad(torch_dtype_code(logits.dtype), logits.data_ptr(), pitch, rows, logits.shape[-1], scale, _ptr(targets),
                                                 I64 if targets is None else torch_dtype_code(targets.dtype), lse.data_ptr(), _ptr(entropy), _ptr(grad_logprobs),
                                                 _ptr(grad_entropy), 0 if grad_top is None else grad_top.shape[-1], _ptr(top_ids), _ptr(grad_top),
