@@ -16,7 +16,11 @@ namespace mhlo {
 namespace {
 
 // Both kernels work in units of 16 elements of a row. A unit of a rotated row holds whole pairs: 8 neighbouring elements of the first
-// half and their partners, or 16 neighbours where pairs are interleaved.
+// half and their partners, or 16 neighbours where pairs are interleaved. A thread has the same unit of every row it takes, rows a
+// fixed number apart, and all of them in registers at once (kKeep): no division and no second read.
+//
+// What bounds it: 16-bit elements come in two bytes each and take about seven instructions, rotation and quantisation two elements at
+// a time; [4400, 32 + 8 + 8, 128] bf16 36 us
 template <typename T>
 struct AppendParams {
     KvArgs kv;
@@ -31,39 +35,48 @@ struct AppendParams {
     int32_t vec[4];      // k, v, q, q_out: rows on the 16-byte grid
     FastDiv units, heads;  // units of a row of a head, query heads
     int32_t rows;          // of queries to a CTA
+    float one;             // 1, which the compiler must not know
     int64_t blocks;      // CTAs that append, a block of keys or values each; the CTAs behind them rotate queries
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* x, bool vec, float* f) {
+__device__ __forceinline__ void load8(const T* x, bool vec, float2* f) {
     if (vec) {
         constexpr int E = VecTraits<T>::kElems;
 #pragma unroll
-        for (int i = 0; i < 8; i += E) VecTraits<T>::unpack(__ldcs(reinterpret_cast<const uint4*>(x + i)), f + i);  // not the read-only path: q may be rotated in place
+        for (int i = 0; i < 8; i += E) VecTraits<T>::unpack2(__ldcs(reinterpret_cast<const uint4*>(x + i)), f + i / 2);  // not the read-only path: q may be rotated in place
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = VecTraits<T>::to_float(x[i]);
+        for (int i = 0; i < 4; ++i) f[i] = make_float2(VecTraits<T>::to_float(x[2 * i]), VecTraits<T>::to_float(x[2 * i + 1]));
     }
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* y, bool vec, const float* f) {
+__device__ __forceinline__ void store8(T* y, bool vec, const float2* f) {
     if (vec) {
         constexpr int E = VecTraits<T>::kElems;
 #pragma unroll
-        for (int i = 0; i < 8; i += E) *reinterpret_cast<uint4*>(y + i) = VecTraits<T>::pack(f + i);
+        for (int i = 0; i < 8; i += E) *reinterpret_cast<uint4*>(y + i) = VecTraits<T>::pack2(f + i / 2);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = VecTraits<T>::from_float(f[i]);
+        for (int i = 0; i < 4; ++i) {
+            y[2 * i] = VecTraits<T>::from_float(f[i].x);
+            y[2 * i + 1] = VecTraits<T>::from_float(f[i].y);
+        }
     }
 }
 
+// Two products and two sums at once, each rounded by itself. Written as a product and a sum the assembler makes one rounding of them
+// (mul.rn.f32x2 and add.rn.f32x2 as well); a sum as x * 1 + y with a 1 that it does not know cannot be taken together with anything.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b, float one) { return __ffma2_rn(a, make_float2(one, one), b); }
+
 // Where a unit's two groups of eight elements lie.
 struct Unit {
-    int32_t low, high;
+    int32_t low, high, index;
     bool rotated;
 };
 __device__ __forceinline__ Unit unit_at(int32_t unit, int32_t rotary_dim, int32_t interleaved) {
-    Unit u{unit * 16, unit * 16 + 8, unit * 16 < rotary_dim};
+    Unit u{unit * 16, unit * 16 + 8, unit, unit * 16 < rotary_dim};
     if (u.rotated && !interleaved) {
         u.low = unit * 8;
         u.high = (rotary_dim >> 1) + unit * 8;
@@ -71,21 +84,26 @@ __device__ __forceinline__ Unit unit_at(int32_t unit, int32_t rotary_dim, int32_
     return u;
 }
 
-// The cosines and sines of a unit's eight pairs.
-__device__ __forceinline__ void load_turn(const float* row, int32_t unit, int32_t rotary_dim, float* cs, float* sn) {
+// Rotates a unit by the cosines and sines of its position: products and sums rounded one by one (-(b s) is b (-s) to the last bit).
+__device__ __forceinline__ void turn(float2* f, const float* row, int32_t unit, int32_t rotary_dim, int32_t interleaved, float one) {
+    float cs[8], sn[8];
 #pragma unroll
     for (int i = 0; i < 8; i += 4) {
         *reinterpret_cast<float4*>(cs + i) = __ldg(reinterpret_cast<const float4*>(row + unit * 8 + i));
         *reinterpret_cast<float4*>(sn + i) = __ldg(reinterpret_cast<const float4*>(row + (rotary_dim >> 1) + unit * 8 + i));
     }
-}
-__device__ __forceinline__ void turn(float* f, const float* cs, const float* sn, int32_t interleaved) {
+    if (interleaved) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int lo = interleaved ? 2 * i : i, hi = interleaved ? 2 * i + 1 : i + 8;
-        const float a = f[lo], b = f[hi];
-        f[lo] = __fsub_rn(__fmul_rn(a, cs[i]), __fmul_rn(b, sn[i]));
-        f[hi] = __fadd_rn(__fmul_rn(b, cs[i]), __fmul_rn(a, sn[i]));
+        for (int i = 0; i < 8; ++i)
+            f[i] = add2(mul2(f[i], make_float2(cs[i], cs[i])), mul2(make_float2(f[i].y, f[i].x), make_float2(-sn[i], sn[i])), one);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 c = make_float2(cs[2 * i], cs[2 * i + 1]), n = make_float2(sn[2 * i], sn[2 * i + 1]), m = make_float2(-n.x, -n.y);
+            const float2 a = f[i], b = f[4 + i];
+            f[i] = add2(mul2(a, c), mul2(b, m), one);
+            f[4 + i] = add2(mul2(b, c), mul2(a, n), one);
+        }
     }
 }
 template <typename T>
@@ -97,34 +115,56 @@ __device__ __forceinline__ const float* rope_row(const AppendParams<T>& p, int32
     return p.rope + static_cast<int64_t>(position) * p.rotary_dim;
 }
 
-constexpr int kKeep = 4;  // units a thread keeps in registers between the maximum and the codes
+constexpr int kKeep = 4;  // units of a thread
 
-// Queries: a CTA takes p.rows rows, kKeep units a thread. Their elements are on the way before the rows' sequences are looked up: three
-// dependent reads of a few bytes each, which otherwise stood in front of every CTA's loads ([4400, 32, 128] bf16: 41 us).
+// A unit as it lies in memory: half the registers of its numbers with 16-bit types.
+template <typename T>
+struct RawUnit {
+    static constexpr int kVectors = 16 / VecTraits<T>::kElems;
+    uint4 v[kVectors];
+    __device__ __forceinline__ void load(const T* x, const Unit& u, bool vec) {
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) {
+            const T* const at = x + (i < kVectors / 2 ? u.low + i * VecTraits<T>::kElems : u.high + (i - kVectors / 2) * VecTraits<T>::kElems);
+            if (vec) {
+                v[i] = __ldcs(reinterpret_cast<const uint4*>(at));  // not the read-only path: q may be rotated in place
+            } else {
+                float f[VecTraits<T>::kElems];
+#pragma unroll
+                for (int e = 0; e < VecTraits<T>::kElems; ++e) f[e] = VecTraits<T>::to_float(at[e]);
+                v[i] = VecTraits<T>::pack(f);
+            }
+        }
+    }
+    __device__ __forceinline__ void numbers(float2* f) const {
+#pragma unroll
+        for (int i = 0; i < kVectors; ++i) VecTraits<T>::unpack2(v[i], f + i * VecTraits<T>::kElems / 2);
+    }
+};
+
+// Queries: a CTA takes p.rows rows. Their elements are on the way before the rows' sequences are looked up: three dependent reads of
+// a few bytes each, which otherwise stood in front of every CTA's loads.
 constexpr int kMostRows = 32;
+template <typename T>
+constexpr int kUnitsOfRows = sizeof(T) == 2 ? 8 : 4;
 
 template <typename T>
 __device__ __forceinline__ void rotate_rows(const AppendParams<T>& p, int32_t first_row) {
     const KvArgs& a = p.kv;
     __shared__ int32_t position[kMostRows];  // -1: the row is of no sequence
-    const int32_t rows = min(p.rows, a.tokens - first_row), threads = blockDim.x, d = static_cast<int32_t>(p.units.d), all = rows * p.q_heads * d;
-    for (int32_t start = 0; start < all; start += kKeep * threads) {
-        float f[kKeep][16];
-        int32_t row[kKeep], head[kKeep], unit[kKeep];
+    const int32_t d = static_cast<int32_t>(p.units.d), rows = min(p.rows, a.tokens - first_row), all = rows * p.q_heads;
+    const int32_t mine = static_cast<int32_t>(p.units.div(threadIdx.x)), step = static_cast<int32_t>(p.units.div(blockDim.x));
+    const Unit u = unit_at(threadIdx.x - mine * d, p.rotary_dim, p.interleaved);
+    constexpr int kMine = kUnitsOfRows<T>;
+    for (int32_t start = 0; start < all; start += kMine * step) {
+        RawUnit<T> raw[kMine];
 #pragma unroll
-        for (int k = 0; k < kKeep; ++k) {
-            const int32_t i = start + threadIdx.x + k * threads, column = static_cast<int32_t>(p.units.div(i));
-            unit[k] = i - column * d;
-            row[k] = i < all ? static_cast<int32_t>(p.heads.div(column)) : -1;
-            head[k] = column - row[k] * p.q_heads;
-            if (row[k] < 0) continue;
-            const Unit u = unit_at(unit[k], p.rotary_dim, p.interleaved);
-            const T* const x = p.q + static_cast<int64_t>(first_row + row[k]) * p.qs[0] + head[k] * p.qs[1];
-            load8(x + u.low, p.vec[2], f[k]);
-            load8(x + u.high, p.vec[2], f[k] + 8);
+        for (int k = 0; k < kMine; ++k) {
+            const int32_t i = start + mine + k * step, row = static_cast<int32_t>(p.heads.div(i));
+            if (mine < step && i < all) raw[k].load(p.q + static_cast<int64_t>(first_row + row) * p.qs[0] + (i - row * p.q_heads) * p.qs[1], u, p.vec[2]);
         }
         if (start == 0) {
-            for (int32_t i = threadIdx.x >> 5; i < rows; i += threads >> 5) {  // a warp per row
+            for (int32_t i = threadIdx.x >> 5; i < rows; i += blockDim.x >> 5) {  // a warp per row
                 const int32_t r = first_row + i;
                 int32_t b = r;
                 if (a.starts != nullptr) b = kv_search(a.seqs, r, [&](int32_t j) { return static_cast<int64_t>(a.starts[j]); });
@@ -134,24 +174,31 @@ __device__ __forceinline__ void rotate_rows(const AppendParams<T>& p, int32_t fi
             __syncthreads();
         }
 #pragma unroll
-        for (int k = 0; k < kKeep; ++k) {
-            if (row[k] < 0 || position[row[k]] < 0) continue;
-            const Unit u = unit_at(unit[k], p.rotary_dim, p.interleaved);
-            if (u.rotated) {
-                float cs[8], sn[8];
-                load_turn(rope_row(p, position[row[k]]), unit[k], p.rotary_dim, cs, sn);
-                if (p.interleaved) turn(f[k], cs, sn, 1);
-                else turn(f[k], cs, sn, 0);
-            }
-            T* const y = p.q_out + static_cast<int64_t>(first_row + row[k]) * p.os[0] + head[k] * p.os[1];
-            store8(y + u.low, p.vec[3], f[k]);
-            store8(y + u.high, p.vec[3], f[k] + 8);
+        for (int k = 0; k < kMine; ++k) {
+            const int32_t i = start + mine + k * step, row = static_cast<int32_t>(p.heads.div(i));
+            if (mine >= step || i >= all || position[row] < 0) continue;
+            float2 f[8];
+            raw[k].numbers(f);
+            if (u.rotated) turn(f, rope_row(p, position[row]), u.index, p.rotary_dim, p.interleaved, p.one);
+            T* const y = p.q_out + static_cast<int64_t>(first_row + row) * p.os[0] + (i - row * p.q_heads) * p.os[1];
+            store8(y + u.low, p.vec[3], f);
+            store8(y + u.high, p.vec[3], f + 4);
         }
     }
 }
 
-__device__ __forceinline__ uint32_t code_of(float x, float step) {
-    return static_cast<uint32_t>(min(127, max(-127, __float2int_rn(__fmul_rn(x, step))))) & 255u;
+// round(x step) of four numbers as bytes: adding 1.5 * 2^23 leaves the integer, rounded to nearest even, in the low bits. |x step| is at
+// most 127 and a rounding, step being the inverse of the largest magnitude / 127.
+__device__ __forceinline__ uint32_t codes_of(float2 x, float2 y, float step, float one) {
+    const float2 by = make_float2(step, step), magic = make_float2(12582912.f, 12582912.f);
+    const float2 a = add2(mul2(x, by), magic, one), b = add2(mul2(y, by), magic, one);
+    const uint32_t lo = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), hi = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
 }
 
 template <typename T>
@@ -175,42 +222,20 @@ __global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ App
     const int32_t page_index = ((s.length - s.count) >> a.page_shift) + nth, page_tokens = 1 << a.page_shift, dim = a.head_dim;
     const int32_t from = max(s.length - s.count, page_index << a.page_shift), to = min(s.length, (page_index + 1) << a.page_shift);
     if (from >= to) return;
-    const int32_t slot0 = from & (page_tokens - 1), row0 = from - (s.length - s.count) + s.first;
-    const int32_t threads = blockDim.x, all = (to - from) * static_cast<int32_t>(p.units.d);
-    const int64_t pitch = p.xs[which][0];
-    const T* const x = p.x[which] + row0 * pitch + head * p.xs[which][1];
+    const int32_t slot0 = from & (page_tokens - 1), n = to - from, row0 = from - (s.length - s.count) + s.first;
+    const int32_t d = static_cast<int32_t>(p.units.d), mine = static_cast<int32_t>(p.units.div(threadIdx.x)), step_rows = static_cast<int32_t>(p.units.div(blockDim.x));
     const int32_t rotary = which == 0 ? p.rotary_dim : 0;
+    const Unit u = unit_at(threadIdx.x - mine * d, rotary, p.interleaved);
+    const T* const x = p.x[which] + row0 * p.xs[which][0] + head * p.xs[which][1];
+    auto token = [&](int k) { return mine < step_rows ? mine + k * step_rows : n; };  // of the block's new ones; n: none
 
-    auto load_unit = [&](int32_t i, float* f) {
-        const int32_t t = static_cast<int32_t>(p.units.div(i)), unit = i - t * static_cast<int32_t>(p.units.d);
-        const Unit u = unit_at(unit, rotary, p.interleaved);
-        load8(x + t * pitch + u.low, p.vec[which], f);
-        load8(x + t * pitch + u.high, p.vec[which], f + 8);
-        if (u.rotated) {
-            float cs[8], sn[8];
-            load_turn(rope_row(p, from + t), unit, rotary, cs, sn);
-            if (p.interleaved) turn(f, cs, sn, 1);
-            else turn(f, cs, sn, 0);
-        }
-    };
-    uint32_t m = 0;  // magnitudes as bits: ordered like the numbers, infinity and NaN above all
-    auto largest_of = [&](const float* f) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) m = max(m, __float_as_uint(f[e]) & 0x7fffffffu);
-    };
-    float kept[kKeep][16];
+    float2 f[kKeep][8];
 #pragma unroll
     for (int k = 0; k < kKeep; ++k) {
-        const int32_t i = threadIdx.x + k * threads;
-        if (i < all) {
-            load_unit(i, kept[k]);
-            largest_of(kept[k]);
-        }
-    }
-    for (int32_t i = threadIdx.x + kKeep * threads; i < all; i += threads) {  // blocks of more than 512 threads' units
-        float f[16];
-        load_unit(i, f);
-        largest_of(f);
+        const int32_t t = token(k);
+        if (t >= n) continue;
+        load8(x + t * p.xs[which][0] + u.low, p.vec[which], f[k]);
+        load8(x + t * p.xs[which][0] + u.high, p.vec[which], f[k] + 4);
     }
     // only now the page: the elements are on the way meanwhile
     const int32_t page = kv_page(a, b, page_index);
@@ -219,11 +244,21 @@ __global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ App
     int8_t* const codes = (which == 0 ? a.k_codes : a.v_codes) + block * page_tokens * dim;
     float* const scales = (which == 0 ? a.k_scales : a.v_scales) + block;
     const float before = slot0 == 0 ? 0.f : *scales;
-    m = __reduce_max_sync(0xffffffffu, m);
+    float most = 0.f;
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) {
+        const int32_t t = token(k);
+        if (t >= n) continue;
+        if (u.rotated) turn(f[k], rope_row(p, from + t), u.index, rotary, p.interleaved, p.one);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = max_nan(most, max_nan(fabsf(f[k][e].x), fabsf(f[k][e].y)));
+    }
+    // as bits, magnitudes are ordered like the numbers, infinity and NaN above all
+    uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
     __shared__ uint32_t largest[16];
     if ((threadIdx.x & 31) == 0) largest[threadIdx.x >> 5] = m;
     __syncthreads();
-    for (int w = 0; w < threads >> 5; ++w) m = max(m, largest[w]);
+    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) m = max(m, largest[w]);
     float scale = __fmul_rn(__uint_as_float(m), 1.f / 127.f);
     if (scale < 1.17549435e-38f) scale = 0.f;
     scale = before > scale || before != before ? before : scale;
@@ -231,42 +266,32 @@ __global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ App
     if (threadIdx.x == 0) *scales = scale;
     if (scale > before) {  // earlier tokens of the block
         const float ratio = __fdiv_rn(before, scale);
-        for (int32_t i = threadIdx.x * 16; i < slot0 * dim; i += threads * 16) {
+        for (int32_t i = threadIdx.x * 16; i < slot0 * dim; i += blockDim.x * 16) {
             uint4 v = *reinterpret_cast<const uint4*>(codes + i);
             uint32_t* const w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                uint32_t out = 0;
+                float c[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    out |= (static_cast<uint32_t>(__float2int_rn(__fmul_rn(static_cast<float>(static_cast<int8_t>(w[k] >> (8 * e))), ratio))) & 255u) << (8 * e);
-                w[k] = out;
+                for (int e = 0; e < 4; ++e) c[e] = static_cast<float>(static_cast<int8_t>(w[k] >> (8 * e)));
+                w[k] = codes_of(make_float2(c[0], c[1]), make_float2(c[2], c[3]), ratio, p.one);
             }
             *reinterpret_cast<uint4*>(codes + i) = v;
         }
     }
     const float step = scale > 0.f ? __fdiv_rn(1.f, scale) : 0.f;  // NaN scales: codes 0
-    auto store_unit = [&](int32_t i, const float* f) {
-        const int32_t t = static_cast<int32_t>(p.units.div(i)), unit = i - t * static_cast<int32_t>(p.units.d);
-        const Unit u = unit_at(unit, rotary, p.interleaved);
-        int8_t* const y = codes + (slot0 + t) * dim;
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) {
+        const int32_t t = token(k);
+        if (t >= n) continue;
         uint32_t w[4] = {0, 0, 0, 0};
         if (step > 0.f) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) w[e >> 2] |= code_of(f[e], step) << (8 * (e & 3));
+            for (int e = 0; e < 4; ++e) w[e] = codes_of(f[k][2 * e], f[k][2 * e + 1], step, p.one);
         }
+        int8_t* const y = codes + (slot0 + t) * dim;
         *reinterpret_cast<uint2*>(y + u.low) = make_uint2(w[0], w[1]);
         *reinterpret_cast<uint2*>(y + u.high) = make_uint2(w[2], w[3]);
-    };
-#pragma unroll
-    for (int k = 0; k < kKeep; ++k) {
-        const int32_t i = threadIdx.x + k * threads;
-        if (i < all) store_unit(i, kept[k]);
-    }
-    for (int32_t i = threadIdx.x + kKeep * threads; i < all; i += threads) {
-        float f[16];
-        load_unit(i, f);
-        store_unit(i, f);
     }
 }
 
@@ -295,19 +320,21 @@ __global__ void __launch_bounds__(128) read_kernel(const __grid_constant__ KvArg
 #pragma unroll 4
     for (int32_t i = threadIdx.x; i < tokens * static_cast<int32_t>(units.d); i += 128) {
         const int32_t t = static_cast<int32_t>(units.div(i)), unit = i - t * static_cast<int32_t>(units.d);
-        float f[16];
+        float2 f[8];
         if (t < there) {
             const uint4 v = ld_stream16(codes + i * 16);
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int e = 0; e < 16; ++e) f[e] = __fmul_rn(static_cast<float>(static_cast<int8_t>(w[e >> 2] >> (8 * (e & 3)))), scale);
+            for (int e = 0; e < 8; ++e)
+                f[e] = make_float2(__fmul_rn(static_cast<float>(static_cast<int8_t>(w[e >> 1] >> (16 * (e & 1)))), scale),
+                                   __fmul_rn(static_cast<float>(static_cast<int8_t>(w[e >> 1] >> (16 * (e & 1) + 8))), scale));
         } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) f[e] = 0.f;
+            for (int e = 0; e < 8; ++e) f[e] = make_float2(0.f, 0.f);
         }
         T* const y = out + t * s_token + unit * 16;
         store8(y, vec, f);
-        store8(y + 8, vec, f + 8);
+        store8(y + 8, vec, f + 4);
     }
 }
 
@@ -341,17 +368,22 @@ int append(const KvArgs& kv, const void* k, const int64_t* ks, const void* v, co
     p.rope_positions = rope_positions;
     p.rotary_dim = static_cast<int32_t>(rope ? rotary_dim : 0);
     p.interleaved = interleaved != 0;
+    p.one = 1.f;
     p.q_heads = static_cast<int32_t>(q_heads);
     p.units = FastDiv(static_cast<uint32_t>(kv.head_dim / 16));
     p.blocks = 2 * kv.heads * (kv.starts ? (static_cast<int64_t>(kv.tokens) >> kv.page_shift) + 2 * static_cast<int64_t>(kv.seqs) : kv.seqs);
-    // a whole block in the registers of a CTA, kKeep units a thread; single tokens need a warp or two
-    const int units = (kv.starts ? 1 << kv.page_shift : 4) * (kv.head_dim / 16);
-    const int threads = std::min(512, std::max(64, (units / kKeep + 31) / 32 * 32));
+    // A whole block in the registers of a CTA: kKeep of a thread's units, 512 threads at most (pages of 128 tokens of 256 elements).
+    // Single tokens need few threads for their keys and values, as many as there are query heads for those.
+    const int d = kv.head_dim / 16;
+    const int64_t wanted = kv.starts ? (int64_t{1} << kv.page_shift) / kKeep * d : q ? std::min<int64_t>(128, (q_heads + kKeep - 1) / kKeep * d) : 32;
+    const int threads = static_cast<int>((std::max<int64_t>(32, std::max<int64_t>(wanted, d)) + 31) / 32 * 32);
     p.heads = FastDiv(static_cast<uint32_t>(std::max<int64_t>(1, q_heads)));
-    const int64_t row_units = std::max<int64_t>(1, q_heads * (kv.head_dim / 16));
-    p.rows = static_cast<int32_t>(std::min<int64_t>(kMostRows, std::max<int64_t>(1, kKeep * threads / row_units)));
+    // Rows of queries to a CTA: as many as its threads hold, unless that would leave SMs idle (64 rows of 32 x 128: 6.2 us three at a
+    // time, 4.4 one by one).
+    const int64_t fit = kUnitsOfRows<T> * (threads / d) / std::max<int64_t>(1, q_heads), spread = (kv.tokens + 4 * kNumSMs - 1) / (4 * kNumSMs);
+    p.rows = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(kMostRows, std::min(fit, spread))));
     const int64_t grid = p.blocks + (q ? (kv.tokens + p.rows - 1) / p.rows : 0);
-    if (grid > 0x7fffffff || q_heads * kMostRows * (kv.head_dim / 16) > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "kv_cache_append: too many blocks");
+    if (grid > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "kv_cache_append: too many blocks");
     append_kernel<T><<<static_cast<unsigned>(grid), threads, 0, stream>>>(p);
     MHLO_CUDA_CHECK_LAUNCH("kv_cache_append");
     return MHLO_CUDA_OK;
