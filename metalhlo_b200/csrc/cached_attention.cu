@@ -16,11 +16,11 @@ namespace mhlo {
 namespace {
 
 constexpr int kTileKeys = 32;
-constexpr int kLeastTiles = 12;  // a CTA's share where there is little to do: a tile per warp
+constexpr int kLeastTiles = 12;  // a CTA's share where there is little to do: two tiles of a warp
 
 template <int D>
 struct Layout {
-    static constexpr int kWarps = D == 256 ? 6 : 12;
+    static constexpr int kWarps = D == 256 ? 3 : 6;  // two CTAs to an SM
     static constexpr int kThreads = 32 * kWarps;
     static constexpr int kStages = D == 64 ? 4 : 2;
     static constexpr int kTileBytes = kTileKeys * D;  // of keys, and of values
@@ -128,7 +128,7 @@ constexpr float kHeadroomOf = sizeof(T) == 4 ? 0.f : 8.f;
 
 // NT: groups of 8 rows.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kernel(const __grid_constant__ CachedParams<T> p) {
+__global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kernel(const __grid_constant__ CachedParams<T> p) {
     using L = Layout<D>;
     constexpr int kRows = 8 * NT;
     constexpr bool kTwoParts = sizeof(T) == 4;  // fp32: q and the weights as sums of two fp16 numbers
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 1) cached_attention_kerne
 // Sequences of up to this many rows are this kernel's, where the other takes the type: at 32 rows two passes of 16 over the keys cost
 // what one of 128 does there (6 us and 12.5 over 8 x 6000 keys of head dimension 128).
 constexpr int kFewRows = 32;
-bool long_takes(int64_t head_dim) { return head_dim == 64 || head_dim == 128; }
+constexpr bool long_takes(int64_t head_dim) { return head_dim == 64 || head_dim == 128; }
 // Whether a sequence of the call may have more rows: the host knows only how many there are in all.
 bool may_be_long(const int32_t* starts, int64_t tokens, int64_t group) { return starts != nullptr && tokens * group > kFewRows; }
 
@@ -589,7 +589,7 @@ int launch_rows(const CachedParams<T>& p, bool behind, cudaStream_t stream) {
     auto kernel = cached_attention_kernel<T, D, NT>;
     static std::atomic<bool> smem_set[64];
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, smem_set)) return st;
-    const cudaError_t e = launch_dependent(kernel, dim3(kGrid), dim3(L::kThreads), smem, stream, 1, behind, p);
+    const cudaError_t e = launch_dependent(kernel, dim3(kFewGrid), dim3(L::kThreads), smem, stream, 1, behind, p);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of cached_attention failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("cached_attention");
     return MHLO_CUDA_OK;
@@ -605,10 +605,10 @@ int launch_dim(CachedParams<T> p, void* scratch, cudaStream_t stream) {
     many.few_rows = p.few_rows = !may_long ? 0x7fffffff : few ? kFewRows : 0;
     // groups of 8 rows as long as the sequences have no more on average
     const int groups = static_cast<int64_t>(p.kv.tokens) * p.group <= 8 * static_cast<int64_t>(p.kv.seqs) ? 1 : 2;
-    cached_scratch(&p, scratch);
-    if constexpr (sizeof(T) == 2 && (D == 64 || D == 128)) {
+    cached_scratch(&p, kFewGrid, scratch);
+    cached_scratch(&many, kLongGrid, scratch != nullptr ? static_cast<uint8_t*>(scratch) + cached_scratch(kFewGrid, 16, D) : nullptr);
+    if constexpr (sizeof(T) == 2 && long_takes(D)) {
         if (may_long) {
-            cached_scratch(&many, scratch != nullptr ? static_cast<uint8_t*>(scratch) + cached_scratch(16, D) : nullptr);
             if (int st = cached_attention_long(many, stream)) return st;
         }
     }
@@ -616,9 +616,9 @@ int launch_dim(CachedParams<T> p, void* scratch, cudaStream_t stream) {
         if (int st = groups == 1 ? launch_rows<T, D, 1>(p, may_long, stream) : launch_rows<T, D, 2>(p, may_long, stream)) return st;
     }
     if (p.whole) return MHLO_CUDA_OK;
-    const int first = may_long ? kLongRows : 8 * groups, second = may_long && few ? 8 * groups : 0;
-    const cudaError_t e = launch_dependent(join_kernel<T, D>, dim3(kGrid, (first + second) / kJoinRows), dim3(32 * kJoinRows), 0, stream, 1, true,
-                                           may_long ? many : p, first, static_cast<const int32_t*>(p.pieces), static_cast<const float*>(p.partial), second);
+    const int few_rows = few ? 8 * groups : 0, long_rows = may_long ? kLongRows : 0;
+    const cudaError_t e = launch_dependent(join_kernel<T, D>, dim3(few ? kFewGrid : kLongGrid, (few_rows + long_rows) / kJoinRows), dim3(32 * kJoinRows), 0, stream,
+                                           1, true, p, few_rows, static_cast<const int32_t*>(many.pieces), static_cast<const float*>(many.partial), long_rows);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of cached_attention failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("cached_attention (joining)");
     return MHLO_CUDA_OK;
@@ -664,9 +664,9 @@ int64_t mhlo_cuda_cached_attention_scratch_bytes(const mhlo_cuda_kv_cache* cache
     if (!cache || !batch || q_heads < 1) return 0;
     if (cache->head_dim < 1 || batch->pages_per_seq * cache->page_tokens <= kLeastTiles * kTileKeys) return 0;  // no segment is worth cutting
     const int64_t group = q_heads / std::max<int64_t>(1, cache->heads);
-    int64_t bytes = cached_scratch(16, cache->head_dim);
+    int64_t bytes = cached_scratch(kFewGrid, 16, cache->head_dim);
     if (may_be_long(batch->token_starts, batch->tokens, group) && long_takes(cache->head_dim))
-        bytes += cached_scratch(kLongRows, cache->head_dim);
+        bytes += cached_scratch(kLongGrid, kLongRows, cache->head_dim);
     return bytes;
 }
 

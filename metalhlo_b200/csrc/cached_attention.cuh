@@ -11,7 +11,9 @@
 
 namespace mhlo {
 
-constexpr int kGrid = kNumSMs;  // one CTA per SM: both kernels fill its shared memory
+// CTAs of the two kernels, all of them resident: two to an SM for few rows (while one joins its warps or looks up its next segment, the
+// other reads: 32 ragged sequences of up to 4096 tokens 52 us with one of twice the warps, 48 with two), one for many.
+constexpr int kFewGrid = 2 * kNumSMs, kLongGrid = kNumSMs;
 
 template <typename T>
 struct CachedParams {
@@ -26,16 +28,16 @@ struct CachedParams {
     int32_t o_vec;      // 1: results four at a time, 2: rows of o on the 16-byte grid
     int32_t whole;      // no segment has more than the least share of a CTA: none is cut
     int32_t few_rows;   // sequences of up to this many rows belong to the kernel of few rows, longer ones to the other
-    int32_t* pieces;    // [kGrid][8]: the cut segment that a CTA's share ends with (Piece), count 0 if none
-    float* partial;     // [kGrid][2][ROWS (head_dim + 2)]: maxima (log2), sums, outputs
+    int32_t* pieces;    // [CTAs][8]: the cut segment that a CTA's share ends with (Piece), count 0 if none
+    float* partial;     // [CTAs][2][ROWS (head_dim + 2)]: maxima (log2), sums, outputs
 };
 
-// Scratch of one of the kernels, its rows of a segment given: pieces, then partial results.
-constexpr int64_t cached_scratch(int64_t rows, int64_t dim) { return kGrid * (8 * 4 + 2 * rows * (dim + 2) * 4); }
+// Scratch of one of the kernels: pieces, then partial results.
+constexpr int64_t cached_scratch(int64_t ctas, int64_t rows, int64_t dim) { return ctas * (8 * 4 + 2 * rows * (dim + 2) * 4); }
 template <typename T>
-void cached_scratch(CachedParams<T>* p, void* scratch) {
+void cached_scratch(CachedParams<T>* p, int64_t ctas, void* scratch) {
     p->pieces = static_cast<int32_t*>(scratch);
-    p->partial = reinterpret_cast<float*>(p->pieces + kGrid * 8);
+    p->partial = reinterpret_cast<float*>(p->pieces + ctas * 8);
 }
 constexpr int kLongRows = 256;
 
@@ -69,6 +71,7 @@ struct Segment {
 // ROWS, KEYS: of a segment and a tile. LEAST: a CTA's share, in tiles, where there is little to do. LONG: takes the sequences of many rows.
 template <int ROWS, int KEYS, int LEAST, bool LONG>
 struct Work {
+    static constexpr int kGrid = LONG ? kLongGrid : kFewGrid;
     struct Share {  // of one sequence
         KvSequence s;
         int32_t row_tiles, tiles;  // tiles: 1 where there are no keys: somebody has to write the zeros
@@ -224,27 +227,28 @@ struct Work {
 
 // Joins the pieces of the segment that CTA blockIdx.x began and others went on with: sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
 // A warp per row, kJoinRows rows to a CTA (blockIdx.y): the maxima and sums of up to 32 pieces are read at once, a lane each.
-// The first ROWS / kJoinRows of y join p's pieces, those behind them other's (of other_rows): one launch after both kernels.
+// One launch after both kernels: y below long_rows / kJoinRows joins the pieces of the kernel of many rows, y behind that the other's.
 constexpr int kJoinRows = 8;
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ CachedParams<T> p, int32_t of_segment, const int32_t* other_pieces,
-                                                              const float* other_partial, int32_t other_of_segment) {
+__global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ CachedParams<T> p, int32_t few_rows, const int32_t* long_pieces,
+                                                              const float* long_partial, int32_t long_rows) {
     constexpr int kEach = D / 32;
     grid_dependency_wait();
-    const bool second = static_cast<int32_t>(blockIdx.y) * kJoinRows >= of_segment;
-    const int32_t ROWS = second ? other_of_segment : of_segment;
-    const float* const partial = second ? other_partial : p.partial;
-    const int32_t* const piece = (second ? other_pieces : p.pieces) + blockIdx.x * 8;
+    const bool is_long = static_cast<int32_t>(blockIdx.y) * kJoinRows < long_rows;
+    if (is_long && blockIdx.x >= kLongGrid) return;
+    const int32_t of_segment = is_long ? long_rows : few_rows;
+    const float* const partial = is_long ? long_partial : p.partial;
+    const int32_t* const piece = (is_long ? long_pieces : p.pieces) + blockIdx.x * 8;
     const int32_t count = piece[0], row0 = piece[1], rows = piece[2], seq_first = piece[3], head = piece[4];
-    const int r = blockIdx.y * kJoinRows - (second ? of_segment : 0) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int r = blockIdx.y * kJoinRows - (is_long ? 0 : long_rows) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (count == 0 || r >= rows) return;
-    auto part = [&](int32_t i) { return partial + ((static_cast<int64_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0)) * (ROWS * (D + 2)); };
+    auto part = [&](int32_t i) { return partial + ((static_cast<int64_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0)) * (of_segment * (D + 2)); };
     float most = -INFINITY, total = 0.f, sum[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) sum[e] = 0.f;
     for (int32_t base = 0; base < count; base += 32) {
         const bool mine = base + lane < count;
-        const float m = mine ? part(base + lane)[r] : -INFINITY, l = mine ? part(base + lane)[ROWS + r] : 0.f;
+        const float m = mine ? part(base + lane)[r] : -INFINITY, l = mine ? part(base + lane)[of_segment + r] : 0.f;
         const float top = fmaxf(most, warp_reduce<MaxOp>(m)), shift = top == -INFINITY ? 0.f : top;
         const float keep = ex2(most - shift), weight = ex2(m - shift);
         most = top;
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_const
 #pragma unroll 4
         for (int32_t i = 0; i < n; ++i) {
             const float w = __shfl_sync(0xffffffffu, weight, i);
-            const float* const o = part(base + i) + 2 * ROWS + r * D;
+            const float* const o = part(base + i) + 2 * of_segment + r * D;
 #pragma unroll
             for (int e = 0; e < kEach; ++e) sum[e] = fmaf(o[lane + 32 * e], w, sum[e]);
         }

@@ -599,7 +599,7 @@ int launch(const CachedParams<T>& p, cudaStream_t stream) {
     auto kernel = cached_attention_tc_kernel<T, D>;
     static std::atomic<bool> smem_set[64];
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), Smem<D>::kTotal, smem_set)) return st;
-    kernel<<<kGrid, kThreads, Smem<D>::kTotal, stream>>>(p);
+    kernel<<<kLongGrid, kThreads, Smem<D>::kTotal, stream>>>(p);
     MHLO_CUDA_CHECK_LAUNCH("cached_attention (tcgen05)");
     return MHLO_CUDA_OK;
 }
