@@ -199,21 +199,28 @@ __global__ void __launch_bounds__(THREADS, (TOP || THREADS < 64 ? 1024 : 1536) /
     const uint32_t v1 = static_cast<uint32_t>(static_cast<uint64_t>(r.vectors) * (part + 1) >> p.log2_parts);
     const uint4* const vectors = reinterpret_cast<const uint4*>(r.x + r.head);
     const int tid = threadIdx.x;
-    const float c = p.scale * 1.4426950408889634f;
+    const float c = p.scale * 1.4426950408889634f, span = -kLowest / c;
 
     // this thread's part of the batch of vectors that begins at `base`, with their maxima; returns the largest element
     auto load = [&](uint4* raw, float* largest, uint32_t base, bool has_single, float* single) {
+        const bool whole = base + THREADS * kBatch <= v1;  // every batch of a row but its last
+        if (whole) {
+            const uint4* const at = vectors + base + tid;
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const uint32_t v = base + tid + i * THREADS;
-            raw[i] = v < v1 ? ld_stream16(vectors + v) : all_lowest<T>();
+            for (int i = 0; i < kBatch; ++i) raw[i] = ld_stream16(at + i * THREADS);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const uint32_t v = base + tid + i * THREADS;
+                raw[i] = v < v1 ? ld_stream16(vectors + v) : all_lowest<T>();
+            }
         }
         *single = has_single ? VecTraits<T>::to_float(r.x[r.place_of_single(tid)]) : -INFINITY;
         float most = *single;
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             largest[i] = -INFINITY;
-            if (base + i * THREADS >= v1) continue;
+            if (!whole && base + i * THREADS >= v1) continue;
             largest[i] = largest_of<T>(raw[i]);
             most = max_nan(most, largest[i]);
         }
@@ -287,6 +294,10 @@ __global__ void __launch_bounds__(THREADS, (TOP || THREADS < 64 ? 1024 : 1536) /
         if (has_single && !(single < least)) put(key_of(single, static_cast<uint32_t>(r.place_of_single(tid))));
     };
 
+    // Elements so far below the maximum that their exponential is 0 are kept above -infinity, so that 0 * -infinity never comes up:
+    // 16-bit types two at a time before they are widened, where the type has such a number.
+    Floor<T> floor(0.f, 0.f);
+    bool by_two = false;
     float m = -INFINITY, s = 0.f, t = 0.f;
     bool first = true;
     int batches = 0;
@@ -300,20 +311,19 @@ __global__ void __launch_bounds__(THREADS, (TOP || THREADS < 64 ? 1024 : 1536) /
             t = f * fmaf(s, delta, t);
             s *= f;
             m = most;
+            floor = Floor<T>(m, span);
+            by_two = floor.below() * c >= 100.f;  // 2^-100 of 2^31 elements are still nothing beside the maximum's 1
         }
         if (m == -INFINITY) {  // nothing but -infinities so far, or a NaN
             if (most != most) s = most;
         } else {
-            // Elements so far below the maximum that their exponential is 0 are kept above -infinity, so that 0 * -infinity never
-            // comes up: 16-bit types two at a time before they are widened.
-            const Floor<T> floor(m, -kLowest / c);
-            const bool by_two = floor.below() * c >= 100.f;  // 2^-100 of 2^31 elements are still nothing beside the maximum's 1
+            const bool whole = base + THREADS * kBatch <= v1;
             const float2 minus = make_float2(-m, -m), by = make_float2(c, c);
             float2 s2 = make_float2(0.f, 0.f), t2 = make_float2(0.f, 0.f);
             auto add_vectors = [&](auto two) {
 #pragma unroll
                 for (int i = 0; i < kBatch; ++i) {
-                    if (base + i * THREADS >= v1) break;
+                    if (!whole && base + i * THREADS >= v1) break;
                     float2 f[E / 2];
                     VecTraits<T>::unpack2(decltype(two)::value ? floor.raise(raw[i]) : raw[i], f);
 #pragma unroll
