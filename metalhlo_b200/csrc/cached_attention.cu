@@ -589,8 +589,14 @@ int launch_rows(const CachedParams<T>& p, bool behind, cudaStream_t stream) {
     auto kernel = cached_attention_kernel<T, D, NT>;
     static std::atomic<bool> smem_set[64];
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), smem, smem_set)) return st;
-    const cudaError_t e = launch_dependent(kernel, dim3(kFewGrid), dim3(L::kThreads), smem, stream, 1, behind, p);
-    if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of cached_attention failed: %s", cudaGetErrorString(e));
+    // Behind the kernel of many rows it may begin before that one ends. In front of it is then only what that one waited for; behind
+    // anything else it has to wait, whatever the environment says of overlap: it reads before grid_dependency_wait().
+    if (behind) {
+        const cudaError_t e = launch_dependent(kernel, dim3(kFewGrid), dim3(L::kThreads), smem, stream, 1, true, p);
+        if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of cached_attention failed: %s", cudaGetErrorString(e));
+    } else {
+        kernel<<<kFewGrid, L::kThreads, smem, stream>>>(p);
+    }
     MHLO_CUDA_CHECK_LAUNCH("cached_attention");
     return MHLO_CUDA_OK;
 }
