@@ -575,9 +575,11 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
     grid_dependency_wait();
 }
 
-// Sequences of up to this many rows are this kernel's, where the other takes the type: at 32 rows two passes of 16 over the keys cost
-// what one of 128 does there (6 us and 12.5 over 8 x 6000 keys of head dimension 128).
-constexpr int kFewRows = 32;
+// Sequences of up to this many rows are this kernel's, where the other takes the type. It walks the keys once for each 16 rows, the other
+// once for 256. Rows, this kernel and the other, 64 sequences of 1000 keys, 8 cache heads of 128: 32 rows 90 and 174 us, 64 rows 152 and
+// 176, 96 rows 224 and 176; 8 of 6000 keys: 64 rows 84 and 91, 96 rows 119 and 93; head dimension 64, 8 of 6000 keys: 64 rows 58 and 70,
+// 96 rows 83 and 71.
+constexpr int kFewRows = 64;
 constexpr bool long_takes(int64_t head_dim) { return head_dim == 64 || head_dim == 128; }
 // Whether a sequence of the call may have more rows: the host knows only how many there are in all.
 bool may_be_long(const int32_t* starts, int64_t tokens, int64_t group) { return starts != nullptr && tokens * group > kFewRows; }
