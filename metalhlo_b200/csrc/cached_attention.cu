@@ -611,7 +611,8 @@ int launch_dim(CachedParams<T> p, void* scratch, cudaStream_t stream) {
     const bool few = !may_long || p.kv.seqs > 1;
     CachedParams<T> many = p;
     many.few_rows = p.few_rows = !may_long ? 0x7fffffff : few ? kFewRows : 0;
-    // groups of 8 rows as long as the sequences have no more on average
+    // Groups of 8 rows as long as the sequences have no more on average: 16 sequences of 4000 keys, 8 cache heads of 128, 8 rows 37 us in
+    // groups of 8 and 43 in groups of 16; 12 rows 50 and 43.
     const int groups = static_cast<int64_t>(p.kv.tokens) * p.group <= 8 * static_cast<int64_t>(p.kv.seqs) ? 1 : 2;
     cached_scratch(&p, kFewGrid, scratch);
     cached_scratch(&many, kLongGrid, scratch != nullptr ? static_cast<uint8_t*>(scratch) + cached_scratch(kFewGrid, 16, D) : nullptr);

@@ -53,6 +53,19 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+template <int V>
+__device__ __forceinline__ void load_f32(const float* at, float* x) {
+    if constexpr (V == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(at);
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    } else if constexpr (V == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(at);
+        x[0] = v.x, x[1] = v.y;
+    } else {
+        x[0] = *at;
+    }
+}
+
 struct Segment {
     KvSequence s;
     int32_t b, head, row0, rows;  // sequence, cache head, first row and rows
@@ -225,30 +238,22 @@ struct Work {
     }
 };
 
-// Joins the pieces of the segment that CTA blockIdx.x began and others went on with: sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
-// A warp per row, kJoinRows rows to a CTA (blockIdx.y): the maxima and sums of up to 32 pieces are read at once, a lane each.
-// One launch after both kernels: y below long_rows / kJoinRows joins the pieces of the kernel of many rows, y behind that the other's.
-constexpr int kJoinRows = 8;
+// Joins row r of the segment that a CTA began and others went on with: sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m). A warp: the maxima
+// and sums of up to 32 pieces are read at once, a lane each.
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ CachedParams<T> p, int32_t few_rows, const int32_t* long_pieces,
-                                                              const float* long_partial, int32_t long_rows) {
-    constexpr int kEach = D / 32;
-    grid_dependency_wait();
-    const bool is_long = static_cast<int32_t>(blockIdx.y) * kJoinRows < long_rows;
-    if (is_long && blockIdx.x >= kLongGrid) return;
-    const int32_t of_segment = is_long ? long_rows : few_rows;
-    const float* const partial = is_long ? long_partial : p.partial;
-    const int32_t* const piece = (is_long ? long_pieces : p.pieces) + blockIdx.x * 8;
+__device__ __forceinline__ void join_row(const CachedParams<T>& p, const int32_t* pieces, const float* partial, int32_t of_segment, int32_t cta, int32_t r) {
+    constexpr int kEach = D / 32, V = D % 128 == 0 ? 4 : D == 64 ? 2 : 1;  // elements of a lane, and how many of them side by side
+    const int lane = threadIdx.x & 31;
+    const int32_t* const piece = pieces + cta * 8;
     const int32_t count = piece[0], row0 = piece[1], rows = piece[2], seq_first = piece[3], head = piece[4];
-    const int r = blockIdx.y * kJoinRows - (is_long ? 0 : long_rows) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (count == 0 || r >= rows) return;
-    auto part = [&](int32_t i) { return partial + ((static_cast<int64_t>(blockIdx.x) + i) * 2 + (i == 0 ? 1 : 0)) * (of_segment * (D + 2)); };
+    auto part = [&](int32_t i) { return partial + ((static_cast<int64_t>(cta) + i) * 2 + (i == 0 ? 1 : 0)) * (of_segment * (D + 2)); };
     float most = -INFINITY, total = 0.f, sum[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) sum[e] = 0.f;
     for (int32_t base = 0; base < count; base += 32) {
-        const bool mine = base + lane < count;
-        const float m = mine ? part(base + lane)[r] : -INFINITY, l = mine ? part(base + lane)[of_segment + r] : 0.f;
+        const bool there = base + lane < count;
+        const float m = there ? part(base + lane)[r] : -INFINITY, l = there ? part(base + lane)[of_segment + r] : 0.f;
         const float top = fmaxf(most, warp_reduce<MaxOp>(m)), shift = top == -INFINITY ? 0.f : top;
         const float keep = ex2(most - shift), weight = ex2(m - shift);
         most = top;
@@ -259,17 +264,34 @@ __global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_const
 #pragma unroll 4
         for (int32_t i = 0; i < n; ++i) {
             const float w = __shfl_sync(0xffffffffu, weight, i);
-            const float* const o = part(base + i) + 2 * of_segment + r * D;
+            const float* const o = part(base + i) + 2 * of_segment + r * D + lane * V;
+            float x[kEach];
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) sum[e] = fmaf(o[lane + 32 * e], w, sum[e]);
+            for (int e = 0; e < kEach; e += V) load_f32<V>(o + 32 * e, x + e);
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) sum[e] = fmaf(x[e], w, sum[e]);
         }
     }
     const int32_t row = row0 + r;
     const int64_t token = seq_first + row / p.group, q_head = head * p.group + row % p.group;
-    T* const y = p.o + token * p.os[0] + q_head * p.os[1];
+    T* const y = p.o + token * p.os[0] + q_head * p.os[1] + lane * V;
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) y[lane + 32 * e] = VecTraits<T>::from_float(total == 0.f ? 0.f : sum[e] / total);
+    for (int e = 0; e < kEach; ++e) y[32 * (e / V * V) + e % V] = VecTraits<T>::from_float(total == 0.f ? 0.f : sum[e] / total);
     if (p.lse != nullptr && lane == 0) p.lse[token * p.q_heads + q_head] = total == 0.f ? -INFINITY : (most + log2f(total)) * 0.6931471805599453f;
+}
+
+// One launch after both kernels, a CTA for kJoinRows rows of a CTA's note: y below long_rows / kJoinRows is of the kernel of many rows, y
+// behind that of the other. Most have nothing to do; CTAs that look through all notes and share the rows that there are take 395 us for
+// chunks of 512 tokens on four sequences of 8192, these 386.
+constexpr int kJoinRows = 8;
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ CachedParams<T> p, int32_t few_rows, const int32_t* long_pieces,
+                                                              const float* long_partial, int32_t long_rows) {
+    grid_dependency_wait();
+    const bool is_long = static_cast<int32_t>(blockIdx.y) * kJoinRows < long_rows;
+    if (is_long && blockIdx.x >= kLongGrid) return;
+    const int32_t r = blockIdx.y * kJoinRows - (is_long ? 0 : long_rows) + (threadIdx.x >> 5);
+    join_row<T, D>(p, is_long ? long_pieces : p.pieces, is_long ? long_partial : p.partial, is_long ? long_rows : few_rows, blockIdx.x, r);
 }
 
 }  // namespace
