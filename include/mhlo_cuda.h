@@ -753,7 +753,7 @@ enum {
  * nearest even. Rewriting adds at most half a step of the new scale to the error of an earlier value. A call that fills slot 0
  * starts the block afresh, whatever the page held. Values below 127 * 2^-126 become 0; a block that is given a NaN or an
  * infinity gets the scale NaN, so that it reads as NaN. Slots behind the last token keep their codes. One page must not be written
- * for two sequences in one call.
+ * twice in one call, for two sequences or for two places of one table.
  */
 int mhlo_cuda_kv_cache_append(int32_t dtype, const mhlo_cuda_kv_cache* cache, const mhlo_cuda_kv_batch* batch, const void* k_dev,
                               const int64_t k_strides[2], const void* v_dev, const int64_t v_strides[2], const void* q_dev,

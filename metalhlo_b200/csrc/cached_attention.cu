@@ -7,6 +7,10 @@
 // The products are transposed, S^T = C q^T and O^T = C^T P^T (16 x 8 x 16 steps): keys and elements of values take the long side of
 // the instruction, rows the short one. A decoding step has as many rows as query heads share a cache head, mostly 4 to 8, and would
 // fill 16 to a half or less: half the products, exponentials and output registers.
+//
+// What bounds it: the codes have to come from memory once, 64 sequences of 8192 keys with 8 heads of 128 (4 query heads each, bf16)
+// 176 us for 1.07 GB, 6.1 TB/s. With fewer or ragged sequences the ends of segments show: 32 of up to 4096 keys 48 us for 179 MB, of
+// which reading alone would take 28. ncu, 32 of 8192 keys: 47 % of issue slots, 21 % of the tensor pipe, 168 registers.
 #include <algorithm>
 #include <type_traits>
 

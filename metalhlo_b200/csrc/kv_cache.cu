@@ -20,7 +20,9 @@ namespace {
 // fixed number apart, and all of them in registers at once (kKeep): no division and no second read.
 //
 // What bounds it: 16-bit elements come in two bytes each and take about seven instructions, rotation and quantisation two elements at
-// a time; [4400, 32 + 8 + 8, 128] bf16 36 us
+// a time, and a CTA that owns a block waits for its rows once before the scale and once for the codes of before. Chunks of 4400 tokens in
+// all, 32 + 8 + 8 heads of 128, bf16: 36 us for 127 MB (79 MB come from memory, ncu counts 42 % of issue slots at 122 registers); one
+// token of 64 sequences 4.4 us, which is a launch and three dependent reads.
 template <typename T>
 struct AppendParams {
     KvArgs kv;
