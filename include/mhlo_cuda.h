@@ -773,7 +773,7 @@ int mhlo_cuda_kv_cache_read(int32_t dtype, const mhlo_cuda_kv_cache* cache, cons
  * Attention of the call's tokens over the cache, which already holds them: the token at position p of its sequence sees
  * positions 0 .. p. q, o: [tokens, q_heads, head_dim] of `dtype` (F16, BF16 or F32), *_strides = {token, head}, head_dim 64, 96,
  * 128 or 256 contiguous; q_heads a multiple of the cache's heads: query head i reads head i / (q_heads / heads).
- * o = softmax(scale * q . k) v with fp32 statistics; lse (NULL, or [tokens, q_heads] floats) receives the logarithm of the sum of
+ * o = softmax(scale * q . k) v with fp32 statistics, 0 < scale <= 1e38, tokens * q_heads < 2^31; lse (NULL, or [tokens, q_heads] floats) receives the logarithm of the sum of
  * exponentials. A token that sees nothing (its sequence is unused or was passed over) gets zeros and lse -infinity; where the
  * starts are out of order, rows may be left alone. o may be q itself.
  * scratch: cached_attention_scratch_bytes() bytes of device memory, 16-byte aligned, that nothing else uses until the call's
@@ -790,7 +790,7 @@ int mhlo_cuda_cached_attention(int32_t dtype, const void* q_dev, const int64_t q
 
 /*
  * Log probabilities of given tokens under z = scale * x, x [rows, vocab] of `dtype` (F16, BF16 or F32) with rows row_stride
- * elements apart, scale > 0 (1 / temperature): lse = log sum exp z, logprobs = z[target] - lse, entropy = lse - sum p z, and the
+ * elements apart, 0 < scale <= 1e38 (1 / temperature): lse = log sum exp z, logprobs = z[target] - lse, entropy = lse - sum p z, and the
  * top_k (0 .. 32) largest entries with their log probabilities in descending order, equal logits in ascending order of their
  * ids, NaN first. targets: [rows] of target_dtype (I32 or I64); a negative target names no token: log probability 0. A target
  * beyond the vocabulary gives NaN, and so does a row that has a NaN, a +infinity or nothing but -infinities. Statistics and

@@ -694,7 +694,9 @@ int mhlo_cuda_cached_attention(int32_t dtype, const void* q_dev, const int64_t q
         return fail(MHLO_CUDA_UNSUPPORTED, "%s: head dimension %d (64, 96, 128 or 256)", what, kv.head_dim);
     if (q_heads < 1 || q_heads > 65535 || q_heads % kv.heads != 0)
         return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: %lld query heads over %d heads", what, static_cast<long long>(q_heads), kv.heads);
-    if (!(scale > 0.f) || scale > 3.402823e38f) return fail(MHLO_CUDA_UNSUPPORTED, "%s: the scale has to be positive and finite", what);
+    if (!(scale > 0.f) || scale > 1e38f) return fail(MHLO_CUDA_UNSUPPORTED, "%s: the scale has to be positive and at most 1e38", what);
+    if (batch->tokens * q_heads > 0x7fffffff)
+        return fail(MHLO_CUDA_UNSUPPORTED, "%s: %lld tokens of %lld heads (2^31 - 1 rows at most)", what, static_cast<long long>(batch->tokens), static_cast<long long>(q_heads));
     if (batch->tokens == 0 || batch->seqs == 0) return MHLO_CUDA_OK;
     if (!batch->token_starts && batch->tokens != batch->seqs)
         return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: %lld tokens of %lld sequences need token_starts", what, static_cast<long long>(batch->tokens), static_cast<long long>(batch->seqs));

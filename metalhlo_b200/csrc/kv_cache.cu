@@ -220,7 +220,8 @@ __global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ App
         nth = static_cast<int32_t>(slot - first(b));
     }
     const KvSequence s = kv_sequence(a, b);
-    if (s.length == 0 || s.count == 0 || nth < 0) return;
+    // a sequence of n tokens touches n / P + 2 blocks at most; more slots come only from starts that are out of order
+    if (s.length == 0 || s.count == 0 || nth < 0 || nth > (s.count >> a.page_shift) + 1) return;
     const int32_t page_index = ((s.length - s.count) >> a.page_shift) + nth, page_tokens = 1 << a.page_shift, dim = a.head_dim;
     const int32_t from = max(s.length - s.count, page_index << a.page_shift), to = min(s.length, (page_index + 1) << a.page_shift);
     if (from >= to) return;

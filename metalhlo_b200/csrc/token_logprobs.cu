@@ -642,7 +642,7 @@ int check_rows(const char* what, int32_t dtype, const void* x, int64_t row_strid
     if (dtype != MHLO_DT_F16 && dtype != MHLO_DT_BF16 && dtype != MHLO_DT_F32) return fail(MHLO_CUDA_UNSUPPORTED, "%s: dtype %d", what, dtype);
     if (rows < 0 || rows > 0x7fffffff || vocab < 1 || vocab > 0x7fffffff || row_stride < vocab)
         return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: %lld rows of %lld logits, %lld apart", what, static_cast<long long>(rows), static_cast<long long>(vocab), static_cast<long long>(row_stride));
-    if (!(scale > 0.f) || scale > 3.402823e38f) return fail(MHLO_CUDA_UNSUPPORTED, "%s: the scale has to be positive and finite", what);
+    if (!(scale > 0.f) || scale > 1e38f) return fail(MHLO_CUDA_UNSUPPORTED, "%s: the scale has to be positive and at most 1e38", what);  // times log2(e) it is finite
     if (targets && target_dtype != MHLO_DT_I32 && target_dtype != MHLO_DT_I64) return fail(MHLO_CUDA_UNSUPPORTED, "%s: targets of dtype %d (I32 or I64)", what, target_dtype);
     if (top_k < 0 || top_k > MHLO_CUDA_TOP_LOGPROBS_MAX || top_k > vocab) return fail(MHLO_CUDA_UNSUPPORTED, "%s: %d alternatives of %lld", what, top_k, static_cast<long long>(vocab));
     if (rows > 0 && !x) return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: null logits", what);

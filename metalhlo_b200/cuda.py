@@ -644,13 +644,15 @@ TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprobs entropy lse to
 
 def _logit_rows(x):
     """[..., vocab] as rows of one stride: (rows, stride)."""
-    assert x.dim() >= 1 and (x.stride(-1) == 1 or x.shape[-1] == 1)
-    if x.dim() == 1:
-        return 1, x.shape[0]
-    for d in range(x.dim() - 2):
-        assert x.shape[d] == 1 or x.stride(d) == x.stride(d + 1) * x.shape[d + 1], "the rows of the logits need one stride"
-    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
-    return rows, max(x.stride(-2), x.shape[-1]) if rows > 1 else x.shape[-1]
+    vocab = x.shape[-1]
+    assert x.stride(-1) == 1 or vocab == 1
+    lead = [(n, step) for n, step in zip(x.shape[:-1], x.stride()[:-1]) if n != 1]
+    for (_, outer), (n, inner) in zip(lead, lead[1:]):
+        assert outer == n * inner, "the rows of the logits need one stride"
+    if not lead or not x.numel():
+        return x.numel() // vocab if vocab else 0, vocab
+    assert lead[-1][1] >= vocab, "the rows of the logits overlap"
+    return x.numel() // vocab, lead[-1][1]
 
 
 def token_logprobs(logits, targets=None, top_k: int = 0, scale: float = 1.0, entropy: bool = True, stream=None) -> TokenLogprobs:

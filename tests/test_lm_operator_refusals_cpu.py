@@ -127,3 +127,20 @@ def test_python_views_refuse_before_the_library():
     import math
 
     assert abs(float(table[1048575, 0]) - math.cos(1048575.0)) < 1e-7 and abs(float(table[1048575, 32 + 1]) - math.sin(1048575.0 * 10000.0 ** (-2 / 64))) < 1e-7
+
+
+def test_what_32_bits_cannot_hold_is_refused():
+    assert attention(scale=2e38) == UNSUPPORTED and logprobs(scale=2e38) == UNSUPPORTED and gradient(scale=2e38) == UNSUPPORTED
+    assert attention(b=batch(tokens=1 << 29, seqs=1 << 20, token_starts=P), q_heads=4) == UNSUPPORTED
+
+
+def test_rows_of_logits():
+    import torch
+
+    x = torch.zeros(4, 3, 50)
+    assert cuda._logit_rows(x) == (12, 50) and cuda._logit_rows(x[0, 0]) == (1, 50) and cuda._logit_rows(x[..., :7]) == (12, 50)
+    assert cuda._logit_rows(x[:, 1:2]) == (4, 150) and cuda._logit_rows(x[:, 1]) == (4, 150) and cuda._logit_rows(x[:0]) == (0, 50)
+    assert cuda._logit_rows(x[..., :1]) == (12, 50) and cuda._logit_rows(x[:1, :1, :9]) == (1, 9)
+    for bad in (x[0, 0].expand(4, 50), x[:, :2], x.transpose(1, 2), x.transpose(0, 1), x.as_strided((4, 50), (10, 1))):
+        with pytest.raises(AssertionError):
+            cuda._logit_rows(bad)

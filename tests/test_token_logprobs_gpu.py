@@ -88,6 +88,22 @@ def test_alternatives_among_many_equals(dtype, kind, vocab):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("vocab", [2049, 20011])
+def test_alternatives_of_many_rows_of_every_order(dtype, vocab):
+    """Rows in numbers that fill the machine, hard orders beside ordinary ones, most of them off the 16-byte grid; masks that leave fewer
+    numbers than there are alternatives; more NaN than alternatives."""
+    cuda = cuda_mod()
+    i = torch.arange(vocab)
+    hard = [torch.full((vocab,), 1.5), i / 50.0, -i / 50.0, (i * 7919 % 13).float(), torch.where(i >= vocab - 33, 3.0, -1.0), torch.where(i % 700 == 3, i / 50.0, -float("inf")),
+            torch.full((vocab,), -float("inf")), torch.where(i % 40 == 1, float("nan"), i / 50.0), torch.where(i % 2 == 0, i / 50.0, -i / 50.0)]
+    x, _ = draw(310, vocab, dtype, 41)
+    for r, h in enumerate(hard * 3):
+        x[11 * r] = h.roll(r).to(dtype)
+    for top in (1, 20, 32):
+        assert torch.equal(cuda.token_logprobs(x.cuda(), top_k=top).top_ids.cpu().long(), top_of(x, top))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("vocab", [100, 50257])
 def test_masked_and_broken_rows(dtype, vocab):
     """-infinity is probability 0 (log probability -infinity, no part in the entropy); a row with nothing else, an infinity or a NaN
