@@ -21,8 +21,7 @@ namespace {
 //
 // What bounds it: 16-bit elements come in two bytes each and take about seven instructions, rotation and quantisation two elements at
 // a time, and a CTA that owns a block waits for its rows once before the scale and once for the codes of before. Chunks of 4400 tokens in
-// all, 32 + 8 + 8 heads of 128, bf16: 36 us for 127 MB (79 MB come from memory, ncu counts 42 % of issue slots at 122 registers); one
-// token of 64 sequences 4.4 us, which is a launch and three dependent reads.
+// all, 32 + 8 + 8 heads of 128, bf16: 31 us for 127 MB; one token of 64 sequences 4.2 us, which is a launch and three dependent reads.
 template <typename T>
 struct AppendParams {
     KvArgs kv;
@@ -41,17 +40,6 @@ struct AppendParams {
     int64_t blocks;      // CTAs that append, a block of keys or values each; the CTAs behind them rotate queries
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* x, bool vec, float2* f) {
-    if (vec) {
-        constexpr int E = VecTraits<T>::kElems;
-#pragma unroll
-        for (int i = 0; i < 8; i += E) VecTraits<T>::unpack2(__ldcs(reinterpret_cast<const uint4*>(x + i)), f + i / 2);  // not the read-only path: q may be rotated in place
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = make_float2(VecTraits<T>::to_float(x[2 * i]), VecTraits<T>::to_float(x[2 * i + 1]));
-    }
-}
 template <typename T>
 __device__ __forceinline__ void store8(T* y, bool vec, const float2* f) {
     if (vec) {
@@ -148,7 +136,7 @@ struct RawUnit {
 // a few bytes each, which otherwise stood in front of every CTA's loads.
 constexpr int kMostRows = 32;
 template <typename T>
-constexpr int kUnitsOfRows = sizeof(T) == 2 ? 8 : 4;
+constexpr int kUnitsOfRows = sizeof(T) == 2 ? 4 : 2;
 
 template <typename T>
 __device__ __forceinline__ void rotate_rows(const AppendParams<T>& p, int32_t first_row) {
@@ -203,8 +191,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
     return y;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ AppendParams<T> p) {
+// A thread keeps the elements of its units as they are and rotates them twice, for the maximum and for the codes: that leaves registers
+// for three CTAs of 256 threads (80 each; chunks of 4400 tokens, 32 + 8 + 8 heads of 128: 37 us with the rotated numbers kept, 122
+// registers; 33 as they are with 122; 31 with 80). The largest pages of the widest heads have 512 threads to a CTA.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) append_kernel(const __grid_constant__ AppendParams<T> p) {
     const KvArgs& a = p.kv;
     if (blockIdx.x >= p.blocks) return rotate_rows(p, static_cast<int32_t>(blockIdx.x - p.blocks) * p.rows);
     // Block `slot` of the sequences' touched blocks. A sequence has n / P + 2 slots at least, as many as n tokens can touch:
@@ -232,14 +223,16 @@ __global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ App
     const T* const x = p.x[which] + row0 * p.xs[which][0] + head * p.xs[which][1];
     auto token = [&](int k) { return mine < step_rows ? mine + k * step_rows : n; };  // of the block's new ones; n: none
 
-    float2 f[kKeep][8];
+    RawUnit<T> raw[kKeep];
 #pragma unroll
     for (int k = 0; k < kKeep; ++k) {
         const int32_t t = token(k);
-        if (t >= n) continue;
-        load8(x + t * p.xs[which][0] + u.low, p.vec[which], f[k]);
-        load8(x + t * p.xs[which][0] + u.high, p.vec[which], f[k] + 4);
+        if (t < n) raw[k].load(x + t * p.xs[which][0], u, p.vec[which]);
     }
+    auto numbers = [&](int k, float2* f) {  // rotated
+        raw[k].numbers(f);
+        if (u.rotated) turn(f, rope_row(p, from + token(k)), u.index, rotary, p.interleaved, p.one);
+    };
     // only now the page: the elements are on the way meanwhile
     const int32_t page = kv_page(a, b, page_index);
     if (page < 0) return;
@@ -252,9 +245,10 @@ __global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ App
     for (int k = 0; k < kKeep; ++k) {
         const int32_t t = token(k);
         if (t >= n) continue;
-        if (u.rotated) turn(f[k], rope_row(p, from + t), u.index, rotary, p.interleaved, p.one);
+        float2 f[8];
+        numbers(k, f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) most = max_nan(most, max_nan(fabsf(f[k][e].x), fabsf(f[k][e].y)));
+        for (int e = 0; e < 8; ++e) most = max_nan(most, max_nan(fabsf(f[e].x), fabsf(f[e].y)));
     }
     // as bits, magnitudes are ordered like the numbers, infinity and NaN above all
     uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
@@ -289,8 +283,10 @@ __global__ void __launch_bounds__(512) append_kernel(const __grid_constant__ App
         if (t >= n) continue;
         uint32_t w[4] = {0, 0, 0, 0};
         if (step > 0.f) {
+            float2 f[8];
+            numbers(k, f);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = codes_of(f[k][2 * e], f[k][2 * e + 1], step, p.one);
+            for (int e = 0; e < 4; ++e) w[e] = codes_of(f[2 * e], f[2 * e + 1], step, p.one);
         }
         int8_t* const y = codes + (slot0 + t) * dim;
         *reinterpret_cast<uint2*>(y + u.low) = make_uint2(w[0], w[1]);
@@ -387,7 +383,8 @@ int append(const KvArgs& kv, const void* k, const int64_t* ks, const void* v, co
     p.rows = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>(kMostRows, std::min(fit, spread))));
     const int64_t grid = p.blocks + (q ? (kv.tokens + p.rows - 1) / p.rows : 0);
     if (grid > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "kv_cache_append: too many blocks");
-    append_kernel<T><<<static_cast<unsigned>(grid), threads, 0, stream>>>(p);
+    if (threads <= 256) append_kernel<T, 256><<<static_cast<unsigned>(grid), threads, 0, stream>>>(p);
+    else append_kernel<T, 512><<<static_cast<unsigned>(grid), threads, 0, stream>>>(p);
     MHLO_CUDA_CHECK_LAUNCH("kv_cache_append");
     return MHLO_CUDA_OK;
 }
