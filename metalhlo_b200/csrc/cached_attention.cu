@@ -56,7 +56,8 @@ __device__ __forceinline__ uint32_t turned(uint32_t x) {  // the transpose of an
 // Codes as fp16. A code with its sign bit turned round is code + 128 in 0 .. 255: as the low byte of an fp16 number with nothing else
 // that is the subnormal (code + 128) 2^-24, which the tensor cores take as it is. The 128 comes off again from the sums: those of q
 // are known beforehand, those of the weights are one more column of the product. With 16-bit inputs that saves the subtraction of
-// every code (a quarter of all instructions); in fp32 the sums would lose too much, so there a code is put behind 0x64 (1024 + x) and
+// every code (a quarter of all instructions) and costs an output some 2^-21 of the largest value that a code can stand for, whatever the
+// weights: a fraction of a percent of a code's step. In fp32 the sums would lose too much, so there a code is put behind 0x64 (1024 + x) and
 // 1152 is taken off, which is exact.
 constexpr uint32_t kSignBits = 0x80808080u;
 template <bool EXACT>
