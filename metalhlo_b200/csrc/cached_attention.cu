@@ -546,13 +546,13 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
                 sum.z += x.z * f;
                 sum.w += x.w * f;
             }
+            const float total_l = top_l[r], inv = total_l == 0.f ? 0.f : 1.f / total_l;
+            const float4 x = total_l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
             if (seg.cut) {
-                reinterpret_cast<float4*>(out + 2 * kRows)[i] = sum;
+                reinterpret_cast<float4*>(out + 2 * kRows)[i] = x;
                 continue;
             }
-            const float total_l = top_l[r], inv = total_l == 0.f ? 0.f : 1.f / total_l;
             T* const y = p.o + seg.token(p, r) * p.os[0] + seg.q_head(p, r) * p.os[1] + d4 * 4;
-            const float4 x = total_l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
             if constexpr (sizeof(T) == 4) {
                 if (p.o_vec) *reinterpret_cast<float4*>(y) = x;
                 else y[0] = x.x, y[1] = x.y, y[2] = x.z, y[3] = x.w;

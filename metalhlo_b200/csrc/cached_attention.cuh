@@ -3,8 +3,8 @@
 // The work is cut into segments: (sequence, ROWS rows, cache head). The rows of a segment are (token, query head) pairs that read the
 // same cache head: row r of a sequence is token r / group, query head head * group + r % group. A segment's keys are walked in tiles
 // of KEYS; CTAs share all tiles of the call evenly, so a CTA's piece may begin or end inside a segment. Whole segments are written at
-// once, pieces go to scratch as (maximum, sum, output) and join_kernel joins them in the order of the CTAs: no atomics, and no order
-// of arrival in the result.
+// once, pieces go to scratch as (maximum, sum, output), the output divided by the sum, and join_kernel joins them in the order of the
+// CTAs: no atomics, and no order of arrival in the result.
 #pragma once
 
 #include "kv_cache.cuh"
@@ -29,7 +29,7 @@ struct CachedParams {
     int32_t whole;      // no segment has more than the least share of a CTA: none is cut
     int32_t few_rows;   // sequences of up to this many rows belong to the kernel of few rows, longer ones to the other
     int32_t* pieces;    // [CTAs][8]: the cut segment that a CTA's share ends with (Piece), count 0 if none
-    float* partial;     // [CTAs][2][ROWS (head_dim + 2)]: maxima (log2), sums, outputs
+    float* partial;     // [CTAs][2][ROWS (head_dim + 2)]: maxima (log2), sums, outputs / sums
 };
 
 // Scratch of one of the kernels: pieces, then partial results.
@@ -238,7 +238,7 @@ struct Work {
     }
 };
 
-// Joins row r of the segment that a CTA began and others went on with: sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m). A warp: the maxima
+// Joins row r of the segment that a CTA began and others went on with: sum_i o_i l_i 2^(m_i - m) / sum_i l_i 2^(m_i - m). A warp: the maxima
 // and sums of up to 32 pieces are read at once, a lane each.
 template <typename T, int D>
 __device__ __forceinline__ void join_row(const CachedParams<T>& p, const int32_t* pieces, const float* partial, int32_t of_segment, int32_t cta, int32_t r) {
@@ -255,9 +255,9 @@ __device__ __forceinline__ void join_row(const CachedParams<T>& p, const int32_t
         const bool there = base + lane < count;
         const float m = there ? part(base + lane)[r] : -INFINITY, l = there ? part(base + lane)[of_segment + r] : 0.f;
         const float top = fmaxf(most, warp_reduce<MaxOp>(m)), shift = top == -INFINITY ? 0.f : top;
-        const float keep = ex2(most - shift), weight = ex2(m - shift);
+        const float keep = ex2(most - shift), weight = l * ex2(m - shift);
         most = top;
-        total = total * keep + warp_reduce<SumOp>(l * weight);
+        total = total * keep + warp_reduce<SumOp>(weight);
 #pragma unroll
         for (int e = 0; e < kEach; ++e) sum[e] *= keep;
         const int32_t n = min(32, count - base);

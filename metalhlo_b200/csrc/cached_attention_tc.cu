@@ -8,7 +8,8 @@
 //   warps 4-7, 8-11    softmax of half 0 / 1, a thread per row: it puts its row of q into shared memory as fp16 at a piece's start and
 //                      writes P over the scores in tensor memory
 // The scales do not touch the codes: a key's scale multiplies its column of scores (16 keys at a time share one), a value's scale goes
-// into the exponent of the weights as its ratio to the largest of the piece, so the products run on integers up to 127.
+// into the exponent of the weights, 2^(z + log2 vs - M), so the products run on integers up to 127. M is a row's own: the largest
+// z + log2 vs that it has seen (see weights_of()).
 // Rows that are fp16 stay as they are; bf16 rows are brought to the same size by powers of two, which is exact.
 //
 // A half has two sets of scores (64 columns of tensor memory, O another head_dim): while the softmax works on step t the scores of
@@ -18,7 +19,7 @@
 // Per block and CTA the tensor pipe needs about 2050 clocks (4096 multiply-adds a clock), the exponentials as many (16 a clock), and
 // the producers some 2000 warp instructions beside the 6000 of the softmax, out of 4 a clock: three limits close together. Decoding
 // steps would fill 128 rows to a few percent and pay the producers' instructions all the same; they have a kernel of their own.
-// Chunks of 512 tokens of four sequences behind 7680 others, 32 query heads of 128 on 8, bf16: 386 us, 690 TFLOP/s. A piece has 17 us
+// Chunks of 512 tokens of four sequences behind 7680 others, 32 query heads of 128 on 8, bf16: 367 us, 725 TFLOP/s. A piece has 17 us
 // besides its steps: 2.5 until it knows its work, 7 for the first page, its codes and q, 4.5 for its results; 3 for the first steps.
 #include <algorithm>
 #include <atomic>
@@ -43,10 +44,14 @@ constexpr int kSoftmaxRegs = 168, kOtherRegs = 88;
 static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * 128, "register shares above what the CTA is launched with wait forever");
 constexpr int kWaitError = 50;         // + where a bounded wait ran out
 
-struct Scales {  // of a block's groups
-    float key[kGroups], ratio_log2[kGroups], out_again[kGroups];
+struct __align__(16) Scales {  // of a block's groups
+    float key[kGroups], value_log2[kGroups], out_again[kGroups];  // out_again: 1 / (kUnit value scale)
+    float least[2];    // of each step, the least value_log2; -infinity where one is beyond 2^+-kReach or 2^kBelow of another, zero or no number
     uint32_t missing;  // groups without a page
 };
+// Where one exponential serves a weight and the row's sum: a weight is 2^(z - m) times 2^(log2 vs + m - M + 6), and as long as the second
+// factor is above 2^-50 nothing that counts in the sum (2^-76 of 2^m) is lost with the weight.
+constexpr float kReach = 100.f, kBelow = 56.f;
 
 template <int D>
 struct Smem {
@@ -81,6 +86,18 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+                 "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
 // Four codes as four fp16 numbers: 0x64xx is 1024 + xx, xx = code + 128.
 __device__ __forceinline__ uint2 codes_f16(uint32_t w) {
     w ^= 0x80808080u;
@@ -108,15 +125,29 @@ struct Blocks {
     }
 };
 
-// The weights of 64 of a row's scores, packed; *sum: what they add to the row's sum. MASK: some columns are hidden.
+__device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
+
+struct Step {  // the groups of a step as a row takes them
+    float f[4], value_log2[4];  // f: what turns a product into a score in units of log2(e)
+    __device__ __forceinline__ Step(const Scales& sc, int set, float factor) {
+        load_f32<4>(sc.key + set * 4, f);
+        load_f32<4>(sc.value_log2 + set * 4, value_log2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] *= factor;
+    }
+};
+
+// The weights of 64 of a row's scores, packed; *total: the row's sum, which they are added to. Two references, both of keys that the row
+// sees: weights are 2^(z + log2 vs - M) times kUnit, the sum is one of 2^(z - m) and gets the weights times conv / value scale, conv =
+// 2^(M - m). MASK: some columns are hidden.
 template <bool MASK>
-__device__ __forceinline__ void weights_of(const uint32_t* sr, const Scales& sc, int g0, float factor, float m, int32_t key0, int32_t seen, uint32_t* packed, float* total) {
+__device__ __forceinline__ void weights_of(const uint32_t* sr, const Step& st, const float* out_again, uint32_t missing, float big_m, float conv, int32_t key0, int32_t seen,
+                                           uint32_t* packed, float* total) {
 #pragma unroll
     for (int gi = 0; gi < 4; ++gi) {
-        const int g = g0 + gi;
-        const float f = factor * sc.key[g], off = sc.ratio_log2[g] + (kUnitLog2 - m);
+        const float f = st.f[gi], off = st.value_log2[gi] + (kUnitLog2 - big_m);
         const float2 f2 = make_float2(f, f), off2 = make_float2(off, off);
-        const bool hidden = MASK && (sc.missing >> g & 1);
+        const bool hidden = MASK && (missing >> gi & 1);
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < 16; c += 2) {
@@ -130,28 +161,27 @@ __device__ __forceinline__ void weights_of(const uint32_t* sr, const Scales& sc,
             sum = __fadd2_rn(sum, e);
             packed[at / 2] = pack_f16(e.x, e.y);
         }
-        const float s = sum.x + sum.y;
-        *total = MASK && s == 0.f ? *total : fmaf(s, sc.out_again[g], *total);
+        *total = fmaf(sum.x + sum.y, out_again[gi] * conv, *total);
     }
 }
 
-// The largest of 64 scores in units of log2(e); hidden ones are not looked at.
+// The largest z + log2 vs of 64 scores, in units of log2(e); hidden ones are not looked at, and neither are those that are no number.
 template <bool MASK>
-__device__ __forceinline__ float largest_of(const uint32_t* sr, const Scales& sc, int g0, float factor, int32_t key0, int32_t seen) {
+__device__ __forceinline__ float largest_of(const uint32_t* sr, const Step& st, uint32_t missing, int32_t key0, int32_t seen) {
     float mx = -INFINITY;
 #pragma unroll
     for (int gi = 0; gi < 4; ++gi) {
         float gm = -INFINITY;
         if (MASK) {
-            const bool hidden = sc.missing >> (g0 + gi) & 1;
+            const bool hidden = missing >> gi & 1;
 #pragma unroll
             for (int c = 0; c < 16; ++c) gm = hidden || key0 + gi * 16 + c >= seen ? gm : fmaxf(gm, __uint_as_float(sr[gi * 16 + c]));
-            mx = gm == -INFINITY ? mx : fmaxf(mx, gm * (factor * sc.key[g0 + gi]));
+            if (gm == -INFINITY) continue;
         } else {
 #pragma unroll
             for (int c = 0; c < 16; c += 2) gm = fmax3(gm, __uint_as_float(sr[gi * 16 + c]), __uint_as_float(sr[gi * 16 + c + 1]));
-            mx = fmaxf(mx, gm * (factor * sc.key[g0 + gi]));
         }
+        mx = fmaxf(mx, fmaf(gm, st.f[gi], st.value_log2[gi]));
     }
     return mx;
 }
@@ -169,7 +199,6 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
     __shared__ uint32_t tmem_slot;
     __shared__ typename Works::Scratch scratch;
     __shared__ Scales scales[kSlots];
-    __shared__ float v_most[kSlots];  // the largest value scale of the piece that a slot's block is of
     uint64_t* const q_full = bars;
     uint64_t* const s_full = q_full + kHalves;      // [half][set]: scores of a step are in tensor memory
     uint64_t* const p_full = s_full + 2 * kHalves;  // [half][set]: its weights are, and O is rescaled if need be
@@ -324,15 +353,6 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                 return g;
             };
             Groups now = look_up(0), next = look_up(1);
-            // the largest value scale of the piece
-            float most = 0.f;
-            const int32_t keys_end = min(bl.limit, (bl.kb0 + bl.count) * kBlockN);
-#pragma unroll 4
-            for (int32_t i = (bl.kb0 * kBlockN >> a.page_shift) + lane; i <= (keys_end - 1) >> a.page_shift; i += 32) {
-                const int32_t page = kv_page(a, seg.b, i);
-                if (page >= 0) most = fmaxf(most, a.v_scales[static_cast<int64_t>(page) * a.heads + seg.head]);
-            }
-            most = warp_reduce<MaxOp>(most);
             // Codes wait in shared memory, in slots that only the lane that copies them reads: in registers a block of both would not fit,
             // and half a block ahead they were late (chunks of 512 tokens on 8192: 300 us that way, 215 with no copies at all).
             auto load = [&](const int8_t* codes, int64_t from, int slots) {
@@ -344,20 +364,19 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
-            // zeros: groups whose rows are stored as zeros (no page, or a value scale that is nothing)
-            auto store = [&](int offset, int slots, uint32_t zeros) {
+            // Groups without a page have whatever the slots held: their scores are hidden, and all codes are numbers.
+            auto store = [&](int offset, int slots) {
                 asm volatile("cp.async.wait_group 1;" ::: "memory");  // all but the newest: keys and values take turns
 #pragma unroll
                 for (int i = 0; i < kMine; ++i) {
                     const int pass = wp + i * kProducers, row = pass * kPassRows + row_in_pass;
                     if (pass >= kPasses) break;
-                    const bool zero = zeros >> (pass * kPassRows / 16) & 1;
                     const uint4 raw = *reinterpret_cast<const uint4*>(smem + slots + (pass * 32 + lane) * 16);
                     const uint2 c0 = codes_f16(raw.x), c1 = codes_f16(raw.y), c2 = codes_f16(raw.z), c3 = codes_f16(raw.w);
                     uint8_t* const at = smem + offset + (chunk >> 2) * kBlockN * 128 + row * 128;
                     const int c = (chunk & 3) * 2;
-                    *reinterpret_cast<uint4*>(at + ((c ^ (row & 7)) << 4)) = zero ? make_uint4(0, 0, 0, 0) : make_uint4(c0.x, c0.y, c1.x, c1.y);
-                    *reinterpret_cast<uint4*>(at + (((c + 1) ^ (row & 7)) << 4)) = zero ? make_uint4(0, 0, 0, 0) : make_uint4(c2.x, c2.y, c3.x, c3.y);
+                    *reinterpret_cast<uint4*>(at + ((c ^ (row & 7)) << 4)) = make_uint4(c0.x, c0.y, c1.x, c1.y);
+                    *reinterpret_cast<uint4*>(at + (((c + 1) ^ (row & 7)) << 4)) = make_uint4(c2.x, c2.y, c3.x, c3.y);
                 }
                 fence_proxy_async();
                 __syncwarp();
@@ -366,29 +385,35 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
             load(a.v_codes, now.base, L::kRaw + L::kRawTile);
             for (int j = 0; j < bl.count && ok; ++j, ++block) {
                 const Groups after = look_up(j + 2);
-                const float ratio = most > 0.f ? now.vs / most : now.vs * 0.f;  // NaN stays
-                const bool nothing = ratio < 1e-18f;
-                const uint32_t missing = __ballot_sync(0xffffffffu, now.base < 0) & ((1u << kGroups) - 1), no_value = missing | __ballot_sync(0xffffffffu, nothing);
+                const uint32_t missing = __ballot_sync(0xffffffffu, now.base < 0) & ((1u << kGroups) - 1);
                 wait(&k_empty[stage], phase ^ 1, 6);
                 if (!ok) break;
-                if (wp == 0 && lane < kGroups) {
+                if (wp == 0) {
                     // Four slots: k_empty says that the scores of two blocks ago are done, and they were asked for only after both halves
                     // had the weights of the block before those.
                     Scales& s = scales[block % kSlots];
-                    s.key[lane] = now.base < 0 ? 0.f : now.ks;
-                    s.ratio_log2[lane] = nothing ? 0.f : __log2f(ratio);
-                    s.out_again[lane] = nothing ? 1.f / kUnit : __fdividef(1.f / kUnit, ratio);
-                    if (lane == 0) {
-                        s.missing = missing;
-                        v_most[block % kSlots] = most;
+                    const float value_log2 = now.base < 0 ? 0.f : log2f(now.vs);
+                    float least = now.base < 0 ? INFINITY : fabsf(value_log2) <= kReach ? value_log2 : -INFINITY, most = now.base < 0 ? -INFINITY : value_log2;
+#pragma unroll
+                    for (int i = 1; i < 4; i <<= 1) {
+                        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, i));
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, i));
+                    }
+                    if (most - least > kBelow) least = -INFINITY;
+                    if (lane < kGroups) {
+                        s.key[lane] = now.base < 0 ? 0.f : now.ks;
+                        s.value_log2[lane] = value_log2;
+                        s.out_again[lane] = now.base < 0 ? 0.f : __fdividef(1.f / kUnit, now.vs);
+                        if ((lane & 3) == 0) s.least[lane >> 2] = least;
+                        if (lane == 0) s.missing = missing;
                     }
                 }
-                store(L::kK + stage * L::kTile, L::kRaw, missing);
+                store(L::kK + stage * L::kTile, L::kRaw);
                 if (lane == 0) mbar_arrive(&k_full[stage]);
                 load(a.k_codes, next.base, L::kRaw);
                 wait(&v_empty[stage], phase ^ 1, 7);
                 if (!ok) break;
-                store(L::kV + stage * L::kTile, L::kRaw + L::kRawTile, no_value);
+                store(L::kV + stage * L::kTile, L::kRaw + L::kRawTile);
                 if (lane == 0) mbar_arrive(&v_full[stage]);
                 load(a.v_codes, next.base, L::kRaw + L::kRawTile);
                 now = next;
@@ -415,7 +440,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
             const int steps = bl.of_half[h];
             const int32_t seen = r < seg.rows ? seg.seen_by(r, p.group) : 0x7fffffff;  // rows that are none hide nothing
             const int64_t token = seg.token(p, min(r, seg.rows - 1)), q_head = seg.q_head(p, min(r, seg.rows - 1));
-            float m_ref = -INFINITY, l = 0.f, factor = 0.f, largest = 0.f;
+            // The row's sum is in units of 2^m_ref, O in units of 2^(big_m - kUnitLog2); near and conv follow from them.
+            float m_ref = -INFINITY, big_m = -INFINITY, l = 0.f, factor = 0.f, near = -kReach, conv = 0.f;
             if (steps > 0) {
                 // This warp's 32 rows of q, whole rows at a time. The half's last scores of the piece before are done (its products with
                 // values are, and they came later): q may be replaced.
@@ -470,54 +496,115 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full[h]);
             }
-            for (int t = 0; t < steps && ok; ++t) {
-                const int set = t & 1;
-                wait(&s_full[2 * h + set], sets[set]++ & 1, 8);
-                if (!ok) break;
-                tc_fence_after();
-                const Scales& sc = scales[(block0 + (t >> 1)) % kSlots];
-                if (t == 0) largest = v_most[block0 % kSlots];
-                const int32_t first = bl.kb0 * kBlockN + t * kStep;
-                const uint32_t taddr = s_taddr + set * kStep;
-                const bool mask = __any_sync(0xffffffffu, first + kStep > seen) || sc.missing != 0;
-                uint32_t sr[64], packed[32];
-                tmem_ld32(taddr, sr);
-                tmem_ld32(taddr + 32, sr + 32);
-                tmem_ld_wait();
-                // A step looks at its own maximum first; where it would push weights out of fp16 (a piece's first step, rarely later)
-                // the sum and O are scaled anew. The scores were asked for behind the product with values of two steps ago, so only the
-                // last one may be under way.
-                const float mx = mask ? largest_of<true>(sr, sc, set * 4, factor, first, seen) : largest_of<false>(sr, sc, set * 4, factor, first, seen);
-                const bool grow = mx > m_ref + kGrowth;
-                if (__any_sync(0xffffffffu, grow)) {
-                    float alpha = 1.f;
-                    if (grow) {
-                        alpha = m_ref == -INFINITY ? 0.f : ex2(m_ref - mx);
-                        m_ref = mx;
-                        l *= alpha;
-                    }
-                    if (t > 0) {
-                        wait(&pv_done[2 * h + (set ^ 1)], (sets[set ^ 1] - 1) & 1, 10);
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int c0 = 0; c0 < D; c0 += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(o_taddr + c0, o);
-                            tmem_ld_wait();
-#pragma unroll
-                            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
-                            tmem_st32(o_taddr + c0, o);
-                        }
-                    }
-                }
-                const float m = m_ref == -INFINITY ? 0.f : m_ref;
-                if (mask) weights_of<true>(sr, sc, set * 4, factor, m, first, seen, packed, &l);
-                else weights_of<false>(sr, sc, set * 4, factor, m, first, seen, packed, &l);
-                tmem_st32(taddr, packed);  // over scores that have been read
+            auto publish = [&](int set) {  // weights that are in tensor memory
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[2 * h + set]);
+            };
+            auto measure = [&]() {
+                const float d = big_m - m_ref;
+                const bool none = big_m == -INFINITY;  // nothing but hidden columns, if the step's scales are near
+                near = none ? -kReach : fabsf(d) <= kReach ? d - kBelow : INFINITY;
+                conv = none ? 0.f : ex2(d);
+            };
+            // Ordinary steps are the inner loop, one exponential a score; a step whose value scales lie too far from one another or from the
+            // references is taken by itself behind it.
+            for (int t = 0; t < steps && ok; ++t) {
+                int set;
+                uint32_t taddr, missing;
+                int32_t first;
+                for (; t < steps; ++t) {
+                    set = t & 1;
+                    wait(&s_full[2 * h + set], sets[set]++ & 1, 8);
+                    if (!ok) break;
+                    tc_fence_after();
+                    taddr = s_taddr + set * kStep;
+                    uint32_t sr[64], packed[32];
+                    tmem_ld32(taddr, sr);
+                    tmem_ld32(taddr + 32, sr + 32);
+                    const Scales& sc = scales[(block0 + (t >> 1)) % kSlots];
+                    first = bl.kb0 * kBlockN + t * kStep;
+                    missing = sc.missing >> (set * 4) & 15u;
+                    const Step st(sc, set, factor);
+                    const bool mask = __any_sync(0xffffffffu, first + kStep > seen) || missing != 0;
+                    const float least = sc.least[set];
+                    tmem_ld_wait();
+                    // A step looks at its own maximum first; where it would push weights out of fp16 (a piece's first step, rarely later)
+                    // O is scaled anew. The scores were asked for behind the product with values of two steps ago, so only the last one
+                    // may be under way. m_ref can stay: ordinary scores are within kBelow + kGrowth of it, and it need not be a maximum.
+                    const float mx = mask ? largest_of<true>(sr, st, missing, first, seen) : largest_of<false>(sr, st, missing, first, seen);
+                    const bool grow = mx > big_m + kGrowth;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        float alpha = 1.f;
+                        if (grow) {
+                            alpha = big_m == -INFINITY ? 0.f : ex2(big_m - mx);
+                            big_m = mx;
+                            if (m_ref == -INFINITY && fabsf(least) <= kReach) m_ref = big_m - least;
+                        }
+                        measure();
+                        if (t > 0) {
+                            wait(&pv_done[2 * h + (set ^ 1)], (sets[set ^ 1] - 1) & 1, 10);
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c0 = 0; c0 < D; c0 += 32) {
+                                uint32_t o[32];
+                                tmem_ld32(o_taddr + c0, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+                                tmem_st32(o_taddr + c0, o);
+                            }
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, !(least >= near))) break;
+                    float out_again[4];
+                    load_f32<4>(sc.out_again + set * 4, out_again);
+                    if (mask) weights_of<true>(sr, st, out_again, missing, reference(big_m), conv, first, seen, packed, &l);
+                    else weights_of<false>(sr, st, out_again, missing, big_m, conv, first, seen, packed, &l);
+                    tmem_st32(taddr, packed);  // over scores that have been read
+                    publish(set);
+                }
+                if (!ok || t >= steps) break;
+                // Step t by itself, a group at a time: the sum has exponentials of its own, and m_ref is their maximum.
+                const Scales& sc = scales[(block0 + (t >> 1)) % kSlots];
+                float top = -INFINITY, sum = 0.f, m = 0.f;
+#pragma unroll 1
+                for (int i = 0; i < 8; ++i) {  // the maximum, then weights and sum
+                    const int g = i & 3;
+                    const float f = factor * sc.key[set * 4 + g], off = sc.value_log2[set * 4 + g] + (kUnitLog2 - reference(big_m));
+                    const int32_t there = missing >> g & 1 ? 0 : seen - first - g * 16;  // columns of the group that the row sees
+                    uint32_t x[16], packed[8];
+                    tmem_ld16(taddr + g * 16, x);
+                    tmem_ld_wait();
+                    if (i == 4) {
+                        if (top > m_ref + kGrowth) {
+                            l *= m_ref == -INFINITY ? 0.f : ex2(m_ref - top);
+                            m_ref = top;
+                        }
+                        m = reference(m_ref);
+                    }
+                    if (i < 4) {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) top = c < there ? fmaxf(top, __uint_as_float(x[c]) * f) : top;
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 16; c += 2) {
+                            float e[2];
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const float z = __uint_as_float(x[c + j]);
+                                e[j] = c + j < there ? ex2(fmaf(z, f, off)) : 0.f;
+                                sum += c + j < there ? ex2(fmaf(z, f, -m)) : 0.f;
+                            }
+                            packed[c / 2] = pack_f16(e[0], e[1]);
+                        }
+                        tmem_st8(taddr + g * 8, packed);  // over scores that have been read
+                    }
+                }
+                l += sum;
+                measure();
+                publish(set);
             }
             if (!ok) break;
             // The next piece's first product with values waits for this warp's weights, which come after these reads.
@@ -526,7 +613,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
             if (!ok) break;
             if (steps > 0) tc_fence_after();
             const bool nothing = l == 0.f;
-            const float unit = largest * (1.f / kUnit), by = seg.cut ? unit : nothing ? 0.f : unit / l;
+            // 2^(big_m - m_ref) may be out of fp32 where the result is not: its root comes twice
+            const float half = ex2(0.5f * (big_m - m_ref - kUnitLog2)), by = half / l;
             float* const out = work.partial(p, seg, D);
             // Results leave through the warp's part of q (its scores are done), so that whole rows are written at a time: 64 fp32 elements of
             // a row, or all 16-bit ones, at once.
@@ -542,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                         tmem_ld_wait();
                     }
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) o[c] = steps == 0 || nothing ? 0u : __float_as_uint(__uint_as_float(o[c]) * by);
+                    for (int c = 0; c < 32; ++c) o[c] = steps == 0 || nothing ? 0u : __float_as_uint(__uint_as_float(o[c]) * half * by);
                     if (seg.cut) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 4) *reinterpret_cast<uint4*>(q_chunk(row, (part + c) / 4)) = make_uint4(o[c], o[c + 1], o[c + 2], o[c + 3]);

@@ -1,0 +1,136 @@
+"""Cached attention where the scales of blocks lie far apart. A row's result is a matter of the keys that it sees, and its error one of
+what they contribute: whatever blocks hold that a row does not see, or sees with a weight of nothing, is not noticed.
+
+Bounds as in test_kv_cache_gpu.py, with what a row sees of each block's value scale vs by its weights p in place of the largest scale: a
+weight times its value scale is lost below 2^-31 (fp32 inputs: 2^-39) of the largest, and a sum that carries 128 with every code is off by
+2^-23 of 128 sum p vs at most in each step of 16 keys."""
+import math
+
+import pytest
+import torch
+
+from test_kv_cache_gpu import HALF_STEP, HALF_SUBNORMAL, cuda_mod, make_cache, make_table, on_gpu, starts_of
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.bfloat16, torch.float16]
+# new tokens, lengths, query heads of a cache head: rows of the kernel of many
+CALLS = {"chunks": ([40, 130], [500, 290], 2), "long": ([200], [1500], 4)}
+
+
+def definition(cache, q, table, lengths, starts, scale):
+    """fp64 on the GPU: (o, lse, bound without the result's own rounding, keys each row sees)."""
+    o, bound = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    lse, seen_of = torch.zeros(q.shape[:2], dtype=torch.float64, device="cuda"), []
+    heads, page, dim = cache.k.shape[1:]
+    single = q.dtype == torch.float32
+    for b, length in enumerate(lengths):
+        first, n = int(starts[b]), int(starts[b + 1] - starts[b])
+        pages = torch.from_numpy(table[b, :-(-length // page)]).long().cuda()
+        (k, ks), (v, vs) = ((c[pages].double(), s[pages].double()[:, :, None].expand(-1, -1, page)) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+        k, v = ((c * s[..., None]).transpose(0, 1).flatten(1, 2)[:, :length] for c, s in ((k, ks), (v, vs)))  # [heads, keys, dim]
+        ks, vs = (s.transpose(0, 1).flatten(1, 2)[:, None, None, :length] for s in (ks, vs))
+        x = q[first:first + n].double().unflatten(1, (heads, -1)).permute(1, 2, 0, 3)  # [heads, group, new, dim]
+        position = torch.arange(length - n, length, device="cuda")
+        seen = torch.arange(length, device="cuda")[None] <= position[:, None]
+        z = (x @ k[:, None].transpose(2, 3) * scale).masked_fill(~seen, -math.inf)
+        p = torch.softmax(z, -1)
+        products = (x.abs() @ k.abs()[:, None].transpose(2, 3)) + (0 if single else 128) * ks * x.abs().sum(-1, keepdim=True)
+        products = torch.where(p > 2.0 ** -60, products, 0).amax(-1, keepdim=True)
+        weight = 2 * (dim / 16) * 2.0 ** -22 * scale * products + 2.0 ** -20 + (0 if single else 2.0 ** -11)
+        v = torch.nan_to_num(v)[:, None]
+        vs = torch.nan_to_num(vs)
+        lost = (2.0 ** -39 if single else 2.0 ** -31) * 127 * (position + 1)[:, None] * (p * vs).amax(-1, keepdim=True)
+        if not single:
+            lost = lost + 2.0 ** -27 * 128 * (position + 1)[:, None] * (p * vs).sum(-1, keepdim=True)
+
+        def rows(t):
+            return t.permute(2, 0, 1, 3).flatten(1, 2)
+
+        o[first:first + n], bound[first:first + n] = rows(p @ v), rows(weight * (p @ v.abs()) + lost)
+        lse[first:first + n] = rows(z.logsumexp(-1, keepdim=True))[..., 0]
+        seen_of += (position + 1).tolist()
+    return o, lse, bound, seen_of
+
+
+def run(cache, q, table, lengths, starts, scale):
+    lse = torch.zeros(q.shape[:2], device="cuda")
+    o = cuda_mod().cached_attention(q, cache, on_gpu(table), on_gpu(lengths), scale, token_starts=on_gpu(starts), lse=lse)
+    assert cuda_mod().device_error() == 0
+    return o, lse
+
+
+def check(o, want, bound, rows):
+    """The rows ``rows``; elements beyond their type may be anything."""
+    error = torch.nan_to_num((o.double() - want).abs(), nan=math.inf, posinf=math.inf) - HALF_STEP[o.dtype] * want.abs() - bound - HALF_SUBNORMAL[o.dtype]
+    error = torch.where(want.abs() > 0.99 * torch.finfo(o.dtype).max, -1.0, error)[rows]
+    assert bool((error <= 0).all()), f"{float(error.max())} above the bound"
+
+
+def setup(call, page, dim, dtype, seed):
+    new, lengths, group = CALLS[call]
+    pages = sum(-(-n // page) for n in lengths) + 1
+    cache, _ = make_cache(pages, 2, page, dim, seed)
+    starts = starts_of(new)
+    q = torch.randn(int(starts[-1]), 2 * group, dim, generator=torch.Generator().manual_seed(seed + 1)).to(dtype).cuda()
+    return cache, q, make_table(lengths, page, pages, seed + 2), lengths, starts
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("page,dim", [(16, 64), (32, 128), (64, 128), (128, 64)])
+@pytest.mark.parametrize("call", CALLS)
+def test_values_of_pages_that_a_row_does_not_see(dtype, page, dim, call):
+    """The newest page of each sequence stands for far larger values than all others: finite ones, and then NaN."""
+    cache, q, table, lengths, starts = setup(call, page, dim, dtype, 41)
+    last = torch.tensor([int(table[b, (n - 1) // page]) for b, n in enumerate(lengths)]).cuda()
+    ordinary = cache.v_scale[last].clone()
+    scale = 1.5 / math.sqrt(dim)
+    for factor in (2.0 ** 20, 1e19, 1e30):
+        cache.v_scale[last] = ordinary * factor
+        o, lse = run(cache, q, table, lengths, starts, scale)
+        want, want_lse, bound, seen_of = definition(cache, q, table, lengths, starts, scale)
+        check(o, want, bound, slice(None))
+        assert bool(((lse - want_lse).abs() <= 2.0 ** -14).all())
+    cache.v_scale[last] = float("nan")
+    o, lse = run(cache, q, table, lengths, starts, scale)
+    want, want_lse, bound, seen_of = definition(cache, q, table, lengths, starts, scale)
+    end_of = [lengths[b] for b in range(len(lengths)) for _ in range(int(starts[b + 1] - starts[b]))]
+    before = torch.tensor([seen <= (end - 1) // page * page for seen, end in zip(seen_of, end_of)]).cuda()
+    assert bool(before.any()) and bool((~before).any())
+    check(o, want, bound, before)
+    assert bool(o[~before].isnan().all())
+    assert bool(((lse - want_lse).abs() <= 2.0 ** -14).all())  # the sum of exponentials is one of keys alone
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("page,dim", [(16, 64), (64, 128)])
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("power", [-40, 40, 90])
+def test_values_far_from_the_others_that_nobody_attends_to(dtype, page, dim, call, power):
+    """The first page of each sequence holds values 2^power times the others' behind scores far below all others."""
+    cache, q, table, lengths, starts = setup(call, page, dim, dtype, 44)
+    first = torch.tensor([int(table[b, 0]) for b in range(len(lengths))]).cuda()
+    cache.k[first] = -120  # q is positive: these scores are negative, the others' of both signs
+    cache.k_scale[first] = 0.25
+    cache.v_scale[first] *= 2.0 ** power
+    q = (q.abs() + 0.4).to(dtype)
+    o, lse = run(cache, q, table, lengths, starts, 1 / math.sqrt(dim))
+    want, want_lse, bound, seen_of = definition(cache, q, table, lengths, starts, 1 / math.sqrt(dim))
+    rows = torch.tensor(seen_of).cuda() > page + 16  # they see others
+    assert bool(rows.any())
+    check(o, want, bound, rows)
+    assert bool(((lse - want_lse).abs() <= 2.0 ** -13)[rows].all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("scales", [(1e-36, 1e-36), (1e30, 1e30), (1e-30, 1e30), (0.0, 1.0), (0.0, 0.0), (1e-38, 1.0)], ids=str)
+def test_value_scales_at_the_ends_of_their_range(dtype, call, scales):
+    """Blocks whose value scales take turns between two numbers; values beyond fp16 are not looked at."""
+    cache, q, table, lengths, starts = setup(call, 32, 128, dtype, 47)
+    turn = torch.arange(cache.v_scale.shape[0], device="cuda")[:, None] % 2 == 0
+    cache.v_scale.copy_(torch.where(turn, scales[0], scales[1]).expand_as(cache.v_scale))
+    o, lse = run(cache, q, table, lengths, starts, 0.1)
+    want, want_lse, bound, _ = definition(cache, q, table, lengths, starts, 0.1)
+    check(o, want, bound, slice(None))
+    assert bool(((lse - want_lse).abs() <= 2.0 ** -14).all())
