@@ -8,6 +8,9 @@
 // the instruction, rows the short one. A decoding step has as many rows as query heads share a cache head, mostly 4 to 8, and would
 // fill 16 to a half or less: half the products, exponentials and output registers.
 //
+// A row's references for its sum and its output are of keys that it sees (m and d below): a block that it does not see, or whose keys have
+// nothing of its weight, costs it no digits, however large the block's values are.
+//
 // What bounds it: the codes have to come from memory once, 64 sequences of 8192 keys with 8 heads of 128 (4 query heads each, bf16)
 // 176 us for 1.07 GB, 6.1 TB/s. With fewer or ragged sequences the ends of segments show: 32 of up to 4096 keys 48 us for 179 MB, of
 // which reading alone would take 28. ncu, 32 of 8192 keys: 47 % of issue slots, 21 % of the tensor pipe, 168 registers.
@@ -123,13 +126,18 @@ __device__ __forceinline__ int step_element(int step, int c) {
     return 64 * (step >> 2) + 16 * c + 4 * (step & 3);
 }
 
-// fp16 weights are held times a power of two, so that those far below the largest keep some bits above the smallest step, 2^-24. In
-// fp32 the largest weight is 2^14; with 16-bit inputs 2^6, and scores may exceed the maximum that was seen last by 2^8 before
-// everything is scaled anew: with exact maxima some row of 16 found a new one in almost every tile, 10 % of all instructions.
+// Weights 2^(z - m + log2 vs - d), m + d a row's largest z + log2 vs so far, go into fp16 times a power of two, so that those far below the
+// largest keep some bits above the smallest step, 2^-24. In fp32 the unit is 2^14; with 16-bit inputs 2^6, and what a row sees may exceed
+// m + d by 2^8 before everything is scaled anew: with exact maxima some row of 16 found a new one in almost every tile, 10 % of all
+// instructions. m and d are whole numbers, so that what is scaled by their differences is not rounded.
 template <typename T>
-constexpr float kWeightUnitOf = sizeof(T) == 4 ? 16384.f : 64.f;
+constexpr float kUnitLog2Of = sizeof(T) == 4 ? 14.f : 6.f;
 template <typename T>
-constexpr float kHeadroomOf = sizeof(T) == 4 ? 0.f : 8.f;
+constexpr float kHeadroomOf = sizeof(T) == 4 ? 1.f : 8.f;
+constexpr float kNone = -3e38f;  // m + d of a row that has seen nothing: below every sum, but less -infinity it is not NaN
+__device__ __forceinline__ float pow2_of(float whole) {  // 2^whole; 0 and infinity out of fp32's ordinary exponents
+    return whole < -126.f ? 0.f : whole > 127.f ? INFINITY : __int_as_float((static_cast<int>(whole) + 127) << 23);
+}
 
 // NT: groups of 8 rows.
 template <typename T, int D, int NT>
@@ -137,15 +145,20 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
     using L = Layout<D>;
     constexpr int kRows = 8 * NT;
     constexpr bool kTwoParts = sizeof(T) == 4;  // fp32: q and the weights as sums of two fp16 numbers
-    constexpr float kWeightUnit = kWeightUnitOf<T>, kHeadroom = kHeadroomOf<T>;
+    constexpr float kUnitLog2 = kUnitLog2Of<T>, kHeadroom = kHeadroomOf<T>;
     constexpr int W = L::kWarps;
     extern __shared__ __align__(128) uint8_t smem[];
     uint2* const q_frag = reinterpret_cast<uint2*>(smem + L::kRing);  // [1 or 2 parts][steps][NT][32]
     __shared__ float row_factor[kRows];                               // scale log2(e) 2^exponent of the row's q
     __shared__ float row_bias[kRows];                                 // -128 2^-24 times the sum of the row's q as fp16
-    __shared__ float sm[W][kRows], sl[W][kRows], sf[W][kRows], sv[W], top_m[kRows], top_l[kRows];
+    __shared__ __align__(8) float sm[W][kRows], sd[W][kRows];  // references of a warp's rows
+    __shared__ float sl[W][kRows], sf[W][kRows], top_m[kRows], top_l[kRows];
     __shared__ int32_t used[W];
-    __shared__ float4 meta[W][L::kStages];  // scales of a tile's halves: keys 0, 1 (-infinity: not there), values 0, 1
+    __shared__ float2 top_unit[kRows];  // a power of two as two
+    // Of a tile's halves: scales of the keys (-infinity: not there) and log2 of those of the values (a half that is not there has the
+    // other's); those of the values, or with 16-bit inputs 1 / (weight unit * scale).
+    __shared__ float4 meta[W][L::kStages];
+    __shared__ float2 meta_v[W][L::kStages];
     __shared__ typename Work<kRows, kTileKeys, kLeastTiles, false>::Scratch scratch;
 
     const KvArgs& a = p.kv;
@@ -209,7 +222,11 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
 
         // -- this warp's tiles: t0 + warp, t0 + warp + W, ...
         // Lane (g, c) has rows 8 j + 2 c + i of keys g and g + 8 of a half, and of elements W / 8 g .. of each part of the values.
-        float o[D / 16][NT][4], m[NT][2], l[NT][2], v_most = 0.f, o_bias[NT][4], factor[NT][2], bias[NT][2];
+        // A row's references: m (z - m in the sum l) and d (z - m + log2 vs - d in weights and o). What follows from them: both (m + d), and
+        // near, the least log2 vs for which one exponential serves l and o. With 16-bit inputs l is in units of 2^(m + d), as far as
+        // kReach allows (sum_unit()), so it gets what o gets, and m and d lie in shared memory: ordinary tiles need only what follows from
+        // them, and registers are short. fp32: conv is 2^-d times the unit of the weights.
+        float o[D / 16][NT][4], m[NT][2], d[NT][2], both[NT][2], l[NT][2], conv[kTwoParts ? NT : 1][2], near = -kReach, conv_most = 0.f, o_bias[NT][4], factor[NT][2], bias[NT][2];
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -218,12 +235,51 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
                 for (int t = 0; t < D / 16; ++t) o[t][j][e] = 0.f;
                 o_bias[j][e] = 0.f;
                 if (e < 2) {
-                    m[j][e] = -INFINITY;
+                    m[j][e] = d[j][e] = -INFINITY;
+                    both[j][e] = kNone;
                     l[j][e] = 0.f;
+                    if (kTwoParts) conv[kTwoParts ? j : 0][e] = 0.f;
                     factor[j][e] = row_factor[8 * j + 2 * c + e];
                     bias[j][e] = row_bias[8 * j + 2 * c + e];
                 }
             }
+        auto sum_unit = [](float x) { return kTwoParts || x == -INFINITY ? 0.f : fminf(fmaxf(x, -kReach), kReach); };
+        auto measure = [&]() {
+            near = -kReach;
+            conv_most = 0.f;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float x = d[j][r];
+                    both[j][r] = x == -INFINITY ? kNone : m[j][r] + x;
+                    if (kTwoParts) {
+                        conv[kTwoParts ? j : 0][r] = x == -INFINITY ? 0.f : pow2_of(kUnitLog2 - x);
+                        conv_most = fmaxf(conv_most, conv[kTwoParts ? j : 0][r]);
+                    }
+                    if (x != -INFINITY) near = fabsf(x) <= kReach && fabsf(m[j][r]) <= kNearZero ? fmaxf(near, x - kBelow) : INFINITY;
+                }
+        };
+        auto load_references = [&]() {
+            if (kTwoParts) return;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const float2 x = *reinterpret_cast<const float2*>(&sm[warp][8 * j + 2 * c]), y = *reinterpret_cast<const float2*>(&sd[warp][8 * j + 2 * c]);
+                m[j][0] = x.x, m[j][1] = x.y, d[j][0] = y.x, d[j][1] = y.y;
+            }
+        };
+        auto store_references = [&]() {
+            __syncwarp();
+            if (g == 0) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    *reinterpret_cast<float2*>(&sm[warp][8 * j + 2 * c]) = make_float2(m[j][0], m[j][1]);
+                    *reinterpret_cast<float2*>(&sd[warp][8 * j + 2 * c]) = make_float2(d[j][0], d[j][1]);
+                }
+            }
+            __syncwarp();
+        };
+        if (!kTwoParts) store_references();
         constexpr bool kKeepQ = NT == 1 && !kTwoParts && D <= 128;  // in registers
         uint2 q_kept[kKeepQ ? L::kSteps : 1];
         if (kKeepQ) {
@@ -235,7 +291,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
         // Pages and scales of 16 tiles at a time, a half tile per lane.
         const int8_t *const k_lane = a.k_codes + lane * 16, *const v_lane = a.v_codes + lane * 16;
         int64_t base = -1;
-        float ks = 0.f, vs = 0.f;
+        float ks = 0.f, vs = 0.f, vs_log2 = 0.f;
         auto issue = [&](int32_t i) {
             if (i < mine) {
                 if ((i & 15) == 0) {
@@ -256,8 +312,15 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
                 if (base0 >= 0) load_half<D>(k_lane + base0, v_lane + base0, ring + stage * 2 * L::kTileBytes, 0);
                 if (base1 >= 0) load_half<D>(k_lane + base1, v_lane + base1, ring + stage * 2 * L::kTileBytes, 1);
                 asm volatile("cp.async.commit_group;" ::: "memory");
-                const float k1 = __shfl_down_sync(0xffffffffu, ks, 1), v1 = __shfl_down_sync(0xffffffffu, vs, 1);
-                if (lane == from) meta[warp][stage] = make_float4(base0 < 0 ? -INFINITY : ks, base1 < 0 ? -INFINITY : k1, vs, v1);
+                if ((i & 15) == 0) {  // only now: the copies do not wait for the scales
+                    vs_log2 = log2f(vs);
+                    if (!kTwoParts) vs = __fdividef(exp2f(-kUnitLog2), vs);
+                }
+                const float k1 = __shfl_down_sync(0xffffffffu, ks, 1), v1 = __shfl_down_sync(0xffffffffu, vs, 1), log1 = __shfl_down_sync(0xffffffffu, vs_log2, 1);
+                if (lane == from) {
+                    meta[warp][stage] = make_float4(base0 < 0 ? -INFINITY : ks, base1 < 0 ? -INFINITY : k1, base0 < 0 ? log1 : vs_log2, base1 < 0 ? vs_log2 : log1);
+                    meta_v[warp][stage] = make_float2(base0 < 0 ? 0.f : vs, base1 < 0 ? 0.f : v1);
+                }
             } else {
                 asm volatile("cp.async.commit_group;" ::: "memory");
             }
@@ -271,6 +334,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
             const uint8_t* const keys = smem + warp * L::kStages * 2 * L::kTileBytes + stage * 2 * L::kTileBytes;
             const uint8_t* const values = keys + L::kTileBytes;
             const float4 scales = meta[warp][stage];
+            const float out_again[2] = {meta_v[warp][stage].x, meta_v[warp][stage].y};
             const bool half_there[2] = {scales.x != -INFINITY, scales.y != -INFINITY};
 
             // S^T = C q^T, 16 keys a step
@@ -323,7 +387,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
             }
             // Scores in units of log2(e) are s f. Tiles that every row sees whole keep them so; others are brought to f = 1 and masked.
             const int32_t key0 = (t0 + warp + i * W) * kTileKeys;
-            const float v_scale[2] = {half_there[0] ? scales.z : 0.f, half_there[1] ? scales.w : 0.f};
+            const float values_log2[2] = {scales.z, scales.w};
             const bool edge = key0 + kTileKeys > least || !half_there[0] || !half_there[1];
             float f[2][NT][2];
 #pragma unroll
@@ -348,74 +412,164 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
                     }
                 }
             }
-            // The maxima that exponents are taken against, and the largest value scale so far, the unit of the output, move only when a
-            // score leaves the headroom of the weights: every lane looks at its own scores, and lanes talk only when they have to.
+            // plain: the scales of both halves are near enough to the references, so the value scale goes into the exponent, and the sum takes
+            // it out again once per half. Else the sum has exponentials of its own. References move only when what a row sees leaves
+            // the headroom of the weights: every lane looks at its own scores, and lanes talk once a tile and more only when they have to.
+            // A half that a row does not see is at -infinity, whatever its scales.
+            auto largest = [&](int j, int r, int half) { return fmaxf(s[half][j][r], s[half][j][2 + r]); };
             float top[NT][2];
-            const float v_top = fmax3(v_most, v_scale[0], v_scale[1]);
-            bool move = v_top > v_most;
+            bool plain = !kTwoParts, move = false;
+            if (plain) {
+                move = !(values_log2[0] >= near && values_log2[1] >= near && values_log2[0] <= kReach && values_log2[1] <= kReach);
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    top[j][r] = fmaxf(fmaxf(s[0][j][r], s[0][j][2 + r]) * f[0][j][r], fmaxf(s[1][j][r], s[1][j][2 + r]) * f[1][j][r]);
-                    move = move || top[j][r] > m[j][r] + kHeadroom;
-                }
-            if (__any_sync(0xffffffffu, move)) {
-                const float unit = v_top > v_most ? v_most / v_top : 1.f;
-                v_most = v_top;
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    float keep[2];
+                for (int j = 0; j < NT; ++j)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-#pragma unroll
-                        for (int x = 4; x < 32; x <<= 1) top[j][r] = fmaxf(top[j][r], __shfl_xor_sync(0xffffffffu, top[j][r], x));
-                        keep[r] = top[j][r] > m[j][r] ? ex2(m[j][r] - top[j][r]) : 1.f;
-                        l[j][r] *= keep[r];
-                        keep[r] *= unit;
-                        m[j][r] = fmaxf(m[j][r], top[j][r]);
+                        top[j][r] = fmaxf(fmaf(largest(j, r, 0), f[0][j][r], values_log2[0]), fmaf(largest(j, r, 1), f[1][j][r], values_log2[1]));
+                        move = move || top[j][r] > both[j][r] + kHeadroom;
                     }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-#pragma unroll
-                        for (int t = 0; t < D / 16; ++t) o[t][j][e] *= keep[e & 1];
-                        o_bias[j][e] *= keep[e & 1];
-                    }
-                }
+                move = __any_sync(0xffffffffu, move);
             }
-            const float ratio[2] = {v_scale[0] == 0.f ? 0.f : kWeightUnit * (v_scale[0] / v_most), v_scale[1] == 0.f ? 0.f : kWeightUnit * (v_scale[1] / v_most)};
-            // Weights times the ratio of the value scales. Where that is an ordinary number it goes into the exponent, and the sum takes it
-            // out again once per half.
-            const bool plain = !kTwoParts && !edge && ratio[0] > 1e-18f && ratio[1] > 1e-18f;
-            if (plain) {
+            if (!plain || move) {
+                load_references();
+                float keep[NT][2];
+                auto over_keys = [&](float x) {
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const float in_exponent = __log2f(ratio[half]), out_again = __fdividef(1.f, ratio[half]);
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        float sum[2] = {0.f, 0.f};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float& x = s[half][j][e];
-                            x = ex2(fmaf(x, f[half][j][e & 1], in_exponent - m[j][e & 1]));
-                            sum[e & 1] += x;
-                        }
-                        l[j][0] = fmaf(sum[0], out_again, l[j][0]);
-                        l[j][1] = fmaf(sum[1], out_again, l[j][1]);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
+                    for (int i = 4; i < 32; i <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, i));
+                    return x;
+                };
+                const float least = fminf(values_log2[0], values_log2[1]);
+                if (plain) {  // may one maximum do?
+                    bool odd = !(least >= near && fabsf(values_log2[0]) <= kReach && fabsf(values_log2[1]) <= kReach && fabsf(values_log2[0] - values_log2[1]) <= 30.f);
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float z = s[half][j][e], top_so_far = m[j][e & 1];
-                            const float weight = ex2(fmaf(z, f[half][j][e & 1], top_so_far == -INFINITY ? 0.f : -top_so_far));
-                            l[j][e & 1] += weight;
-                            s[half][j][e] = edge && z == -INFINITY ? 0.f : weight * ratio[half];  // 0 whatever the scale of a block that the row does not see
+                        for (int r = 0; r < 2; ++r) odd = odd || (fabsf(top[j][r]) > kNearZero && top[j][r] != -INFINITY);
+                    plain = !__any_sync(0xffffffffu, odd);
+                }
+                if (plain) {  // then m is as near to the largest z as the value scales are to one another
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float x = over_keys(top[j][r]);
+                            keep[j][r] = 1.f;
+                            if (x > both[j][r] + kHeadroom) {
+                                const float to = floorf(x), to_m = to - floorf(least);
+                                keep[j][r] = ex2(both[j][r] - to);
+                                l[j][r] *= m[j][r] == -INFINITY ? 0.f : ex2(m[j][r] + sum_unit(d[j][r]) - to);
+                                if (to_m > m[j][r]) m[j][r] = to_m;
+                                d[j][r] = to - m[j][r];
+                            }
                         }
+                } else {
+                    move = false;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float z0 = fmaf(largest(j, r, 0), f[0][j][r], -m[j][r]), z1 = fmaf(largest(j, r, 1), f[1][j][r], -m[j][r]);
+                            move = move || fmaxf(z0 + values_log2[0], z1 + values_log2[1]) > d[j][r] + kHeadroom || fmaxf(z0, z1) > kHeadroom;
+                        }
+                    move = __any_sync(0xffffffffu, move);
+                    if (move) {
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const float z = over_keys(fmaxf(largest(j, r, 0) * f[0][j][r], largest(j, r, 1) * f[1][j][r])), before = m[j][r], unit = sum_unit(d[j][r]);
+                                if (z > before + kHeadroom) {
+                                    m[j][r] = floorf(z);
+                                    d[j][r] += before == -INFINITY ? 0.f : before - m[j][r];
+                                }
+                                const float x = over_keys(fmaxf(fmaf(largest(j, r, 0), f[0][j][r], -m[j][r]) + values_log2[0], fmaf(largest(j, r, 1), f[1][j][r], -m[j][r]) + values_log2[1]));
+                                keep[j][r] = 1.f;
+                                if (x > d[j][r] + kHeadroom) {
+                                    const float to = floorf(x);
+                                    keep[j][r] = d[j][r] == -INFINITY ? 0.f : ex2(d[j][r] - to);
+                                    d[j][r] = to;
+                                }
+                                l[j][r] *= before == -INFINITY ? 0.f : ex2((before - m[j][r]) + (unit - sum_unit(d[j][r])));
+                            }
+                    }
+                }
+                if (move) {
+                    if (i > 0) {  // there is an output already
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                                for (int t = 0; t < D / 16; ++t) o[t][j][e] *= keep[j][e & 1];
+                                o_bias[j][e] *= keep[j][e & 1];
+                            }
+                    }
+                    measure();
+                    if (!kTwoParts) store_references();
+                }
+            }
+            if (plain) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const float in_exponent = values_log2[half] + kUnitLog2;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        float sum[2] = {0.f, 0.f}, off[2];
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) off[r] = in_exponent - both[j][r];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float& x = s[half][j][e];
+                            x = ex2(fmaf(x, f[half][j][e & 1], off[e & 1]));
+                            sum[e & 1] += x;
+                        }
+                        l[j][0] = fmaf(sum[0], out_again[half], l[j][0]);
+                        l[j][1] = fmaf(sum[1], out_again[half], l[j][1]);
+                    }
+                }
+            } else if (kTwoParts && !__any_sync(0xffffffffu, !(out_again[0] * conv_most <= 1e22f && out_again[1] * conv_most <= 1e22f))) {
+                // fp32: a weight is its exponential times conv and the value scale, which rounds once.
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const float ratio[2] = {out_again[half] * conv[kTwoParts ? j : 0][0], out_again[half] * conv[kTwoParts ? j : 0][1]};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float own = ex2(fmaf(s[half][j][e], f[half][j][e & 1], m[j][e & 1] == -INFINITY ? 0.f : -m[j][e & 1]));
+                            l[j][e & 1] += own;
+                            s[half][j][e] = own * ratio[e & 1];  // hidden: 0 times a number
+                        }
+                    }
+            } else {
+                // Two exponentials. In fp32 the value scale's whole power of two goes into that of the weights.
+                load_references();
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float rest = 1.f, whole = values_log2[half];
+                    if (kTwoParts) {
+                        const int exponent = ilogbf(out_again[half]);
+                        whole = out_again[half] == 0.f ? -INFINITY : static_cast<float>(exponent);
+                        rest = out_again[half] == 0.f ? 0.f : scalbnf(out_again[half], -exponent);
+                    }
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        float minus[2], unit[2], off[2];
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            minus[r] = m[j][r] == -INFINITY ? 0.f : -m[j][r];
+                            unit[r] = sum_unit(d[j][r]);
+                            off[r] = whole + (kUnitLog2 - (d[j][r] == -INFINITY ? 0.f : d[j][r]));
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool hidden = edge && s[half][j][e] == -INFINITY;
+                            const float z = fmaf(s[half][j][e], f[half][j][e & 1], minus[e & 1]);
+                            l[j][e & 1] += ex2(z - unit[e & 1]);
+                            s[half][j][e] = hidden ? 0.f : rest * ex2(z + off[e & 1]);  // whatever the scale of a block that the row does not see
+                        }
+                    }
+                }
             }
             // P^T as fragments: keys 2 c, 2 c + 1 and 8 + 2 c, 9 + 2 c of row g
             uint2 pa[2][NT], pb[2][NT];
@@ -487,14 +641,14 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) l[j][r] += __shfl_xor_sync(0xffffffffu, l[j][r], x);
                 if (g == 0) {
-                    sm[warp][8 * j + 2 * c + r] = m[j][r];
+                    if (kTwoParts) {
+                        sm[warp][8 * j + 2 * c + r] = m[j][r];
+                        sd[warp][8 * j + 2 * c + r] = d[j][r];
+                    }
                     sl[warp][8 * j + 2 * c + r] = l[j][r];
                 }
             }
-        if (lane == 0) {
-            sv[warp] = v_most;
-            used[warp] = mine > 0;
-        }
+        if (lane == 0) used[warp] = mine > 0;
         float4* const joined = reinterpret_cast<float4*>(smem);  // [warp][row][D / 4], chunks turned against bank conflicts
         auto joined_at = [](int w_, int row, int d4) {
             const int pair = (row >> 1) & 3;
@@ -519,14 +673,17 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
         }
         __syncthreads();
         if (tid < kRows) {
-            float most = -INFINITY, sum = 0.f;
+            float most = -INFINITY, unit = -INFINITY, sum = 0.f;  // unit: the largest m + d, less most
             for (int i = 0; i < W; ++i) most = fmaxf(most, sm[i][tid]);
-            const float shift = most == -INFINITY ? 0.f : most;
+            for (int i = 0; i < W; ++i)
+                if (sd[i][tid] != -INFINITY) unit = fmaxf(unit, sd[i][tid] + (sm[i][tid] - most));
             for (int i = 0; i < W; ++i) {
-                const float f = ex2(sm[i][tid] - shift);
-                sum += sl[i][tid] * f;
-                sf[i][tid] = f * sv[i] * ((kTwoParts ? 1.f : kCodeUnit) / kWeightUnit);
+                const float l = sl[i][tid] * ex2(sum_unit(sd[i][tid]));
+                sum += sm[i][tid] == -INFINITY ? l : l * ex2(sm[i][tid] - most);
+                sf[i][tid] = sd[i][tid] == -INFINITY ? 0.f : pow2_of(sd[i][tid] + (sm[i][tid] - most) - unit);
             }
+            const float whole = unit == -INFINITY ? 0.f : unit - kUnitLog2 + (kTwoParts ? 0.f : 24.f), first = floorf(0.5f * whole);
+            top_unit[tid] = make_float2(pow2_of(first), pow2_of(whole - first));
             top_m[tid] = most;
             top_l[tid] = sum;
         }
@@ -547,7 +704,9 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
                 sum.w += x.w * f;
             }
             const float total_l = top_l[r], inv = total_l == 0.f ? 0.f : 1.f / total_l;
-            const float4 x = total_l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+            const float2 unit = top_unit[r];
+            const float4 x = total_l == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                            : make_float4(sum.x * inv * unit.x * unit.y, sum.y * inv * unit.x * unit.y, sum.z * inv * unit.x * unit.y, sum.w * inv * unit.x * unit.y);
             if (seg.cut) {
                 reinterpret_cast<float4*>(out + 2 * kRows)[i] = x;
                 continue;

@@ -47,6 +47,11 @@ struct Piece {  // what joining a cut segment needs: CTAs it goes over, its rows
 
 namespace {
 
+// Where one exponential serves a weight and the row's sum. A row has two references: m, near its largest z, and d, so that m + d is near
+// its largest z + log2 vs. A weight is 2^(z - m) times 2^(log2 vs - d + unit): as long as the second factor is above 2^-40 nothing that
+// counts in the sum is lost with the weight. Beyond kNearZero, z - m comes first: log2 vs would be lost beside z.
+constexpr float kReach = 40.f, kBelow = 40.f, kNearZero = 4096.f;
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -8,8 +8,8 @@
 //   warps 4-7, 8-11    softmax of half 0 / 1, a thread per row: it puts its row of q into shared memory as fp16 at a piece's start and
 //                      writes P over the scores in tensor memory
 // The scales do not touch the codes: a key's scale multiplies its column of scores (16 keys at a time share one), a value's scale goes
-// into the exponent of the weights, 2^(z + log2 vs - M), so the products run on integers up to 127. M is a row's own: the largest
-// z + log2 vs that it has seen (see weights_of()).
+// into the exponent of the weights, 2^(z + log2 vs - M), so the products run on integers up to 127. M is a row's own, of the keys that it
+// has seen.
 // Rows that are fp16 stay as they are; bf16 rows are brought to the same size by powers of two, which is exact.
 //
 // A half has two sets of scores (64 columns of tensor memory, O another head_dim): while the softmax works on step t the scores of
@@ -46,12 +46,9 @@ constexpr int kWaitError = 50;         // + where a bounded wait ran out
 
 struct __align__(16) Scales {  // of a block's groups
     float key[kGroups], value_log2[kGroups], out_again[kGroups];  // out_again: 1 / (kUnit value scale)
-    float least[2];    // of each step, the least value_log2; -infinity where one is beyond 2^+-kReach or 2^kBelow of another, zero or no number
+    float least[2];    // of each step, the least value_log2; -infinity where one is beyond 2^+-kReach or 2^30 of another, zero or no number
     uint32_t missing;  // groups without a page
 };
-// Where one exponential serves a weight and the row's sum: a weight is 2^(z - m) times 2^(log2 vs + m - M + 6), and as long as the second
-// factor is above 2^-50 nothing that counts in the sum (2^-76 of 2^m) is lost with the weight.
-constexpr float kReach = 100.f, kBelow = 56.f;
 
 template <int D>
 struct Smem {
@@ -137,9 +134,8 @@ struct Step {  // the groups of a step as a row takes them
     }
 };
 
-// The weights of 64 of a row's scores, packed; *total: the row's sum, which they are added to. Two references, both of keys that the row
-// sees: weights are 2^(z + log2 vs - M) times kUnit, the sum is one of 2^(z - m) and gets the weights times conv / value scale, conv =
-// 2^(M - m). MASK: some columns are hidden.
+// The weights of 64 of a row's scores, packed; *total: the row's sum, which they are added to: it is one of 2^(z - m) and gets the weights
+// times conv / value scale, conv = 2^d, big_m = m + d. MASK: some columns are hidden.
 template <bool MASK>
 __device__ __forceinline__ void weights_of(const uint32_t* sr, const Step& st, const float* out_again, uint32_t missing, float big_m, float conv, int32_t key0, int32_t seen,
                                            uint32_t* packed, float* total) {
@@ -399,7 +395,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                         least = fminf(least, __shfl_xor_sync(0xffffffffu, least, i));
                         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, i));
                     }
-                    if (most - least > kBelow) least = -INFINITY;
+                    if (most - least > 30.f) least = -INFINITY;
                     if (lane < kGroups) {
                         s.key[lane] = now.base < 0 ? 0.f : now.ks;
                         s.value_log2[lane] = value_log2;
@@ -440,8 +436,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
             const int steps = bl.of_half[h];
             const int32_t seen = r < seg.rows ? seg.seen_by(r, p.group) : 0x7fffffff;  // rows that are none hide nothing
             const int64_t token = seg.token(p, min(r, seg.rows - 1)), q_head = seg.q_head(p, min(r, seg.rows - 1));
-            // The row's sum is in units of 2^m_ref, O in units of 2^(big_m - kUnitLog2); near and conv follow from them.
-            float m_ref = -INFINITY, big_m = -INFINITY, l = 0.f, factor = 0.f, near = -kReach, conv = 0.f;
+            // The row's sum is in units of 2^m_ref, O in units of 2^(m_ref + d - kUnitLog2), both whole numbers; the others follow from them.
+            float m_ref = -INFINITY, d = -INFINITY, big_m = -INFINITY, l = 0.f, factor = 0.f, near = -kReach, conv = 0.f;
             if (steps > 0) {
                 // This warp's 32 rows of q, whole rows at a time. The half's last scores of the piece before are done (its products with
                 // values are, and they came later): q may be replaced.
@@ -503,10 +499,25 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                 if (lane == 0) mbar_arrive(&p_full[2 * h + set]);
             };
             auto measure = [&]() {
-                const float d = big_m - m_ref;
-                const bool none = big_m == -INFINITY;  // nothing but hidden columns, if the step's scales are near
-                near = none ? -kReach : fabsf(d) <= kReach ? d - kBelow : INFINITY;
-                conv = none ? 0.f : ex2(d);
+                const bool none = d == -INFINITY;  // nothing but hidden columns, if the step's scales are near
+                big_m = none ? -INFINITY : m_ref + d;
+                near = none ? -kReach : fabsf(d) <= kReach && fabsf(m_ref) <= kNearZero ? d - kBelow : INFINITY;
+                conv = ex2(d);
+            };
+            // O times alpha. The scores of step t were asked for behind the product with values of t - 2, so only that of t - 1 may be under way.
+            auto scale_o = [&](int t, float alpha) {
+                const int other = (t & 1) ^ 1;
+                wait(&pv_done[2 * h + other], (sets[other] - 1) & 1, 10);
+                tc_fence_after();
+#pragma unroll 1
+                for (int c0 = 0; c0 < D; c0 += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(o_taddr + c0, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+                    tmem_st32(o_taddr + c0, o);
+                }
             };
             // Ordinary steps are the inner loop, one exponential a score; a step whose value scales lie too far from one another or from the
             // references is taken by itself behind it.
@@ -531,31 +542,18 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                     const float least = sc.least[set];
                     tmem_ld_wait();
                     // A step looks at its own maximum first; where it would push weights out of fp16 (a piece's first step, rarely later)
-                    // O is scaled anew. The scores were asked for behind the product with values of two steps ago, so only the last one
-                    // may be under way. m_ref can stay: ordinary scores are within kBelow + kGrowth of it, and it need not be a maximum.
+                    // O is scaled anew. m_ref can stay: ordinary scores are within kBelow + kGrowth of it, and it need not be a maximum.
                     const float mx = mask ? largest_of<true>(sr, st, missing, first, seen) : largest_of<false>(sr, st, missing, first, seen);
                     const bool grow = mx > big_m + kGrowth;
                     if (__any_sync(0xffffffffu, grow)) {
-                        float alpha = 1.f;
+                        if (__any_sync(0xffffffffu, grow && !(fabsf(mx) <= kNearZero && fabsf(least) <= kReach))) break;
+                        const float to = floorf(mx), alpha = grow ? ex2(big_m - to) : 1.f;
                         if (grow) {
-                            alpha = big_m == -INFINITY ? 0.f : ex2(big_m - mx);
-                            big_m = mx;
-                            if (m_ref == -INFINITY && fabsf(least) <= kReach) m_ref = big_m - least;
+                            if (m_ref == -INFINITY) m_ref = to - floorf(least);
+                            d = to - m_ref;
                         }
                         measure();
-                        if (t > 0) {
-                            wait(&pv_done[2 * h + (set ^ 1)], (sets[set ^ 1] - 1) & 1, 10);
-                            tc_fence_after();
-#pragma unroll 1
-                            for (int c0 = 0; c0 < D; c0 += 32) {
-                                uint32_t o[32];
-                                tmem_ld32(o_taddr + c0, o);
-                                tmem_ld_wait();
-#pragma unroll
-                                for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
-                                tmem_st32(o_taddr + c0, o);
-                            }
-                        }
+                        if (t > 0) scale_o(t, alpha);
                     }
                     if (__any_sync(0xffffffffu, !(least >= near))) break;
                     float out_again[4];
@@ -566,36 +564,49 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                     publish(set);
                 }
                 if (!ok || t >= steps) break;
-                // Step t by itself, a group at a time: the sum has exponentials of its own, and m_ref is their maximum.
+                // Step t by itself, a group at a time: the largest z, the largest z - m + log2 vs, and then weights and the sum, which has
+                // exponentials of its own.
                 const Scales& sc = scales[(block0 + (t >> 1)) % kSlots];
-                float top = -INFINITY, sum = 0.f, m = 0.f;
+                float top = -INFINITY, big_top = -INFINITY, sum = 0.f, m = 0.f;
 #pragma unroll 1
-                for (int i = 0; i < 8; ++i) {  // the maximum, then weights and sum
+                for (int i = 0; i < 12; ++i) {
                     const int g = i & 3;
-                    const float f = factor * sc.key[set * 4 + g], off = sc.value_log2[set * 4 + g] + (kUnitLog2 - reference(big_m));
+                    const float f = factor * sc.key[set * 4 + g], plus = sc.value_log2[set * 4 + g];
                     const int32_t there = missing >> g & 1 ? 0 : seen - first - g * 16;  // columns of the group that the row sees
-                    uint32_t x[16], packed[8];
-                    tmem_ld16(taddr + g * 16, x);
-                    tmem_ld_wait();
                     if (i == 4) {
                         if (top > m_ref + kGrowth) {
-                            l *= m_ref == -INFINITY ? 0.f : ex2(m_ref - top);
-                            m_ref = top;
+                            const float to = floorf(top);
+                            l *= m_ref == -INFINITY ? 0.f : ex2(m_ref - to);
+                            d += m_ref == -INFINITY ? 0.f : m_ref - to;
+                            m_ref = to;
                         }
                         m = reference(m_ref);
                     }
+                    if (i == 8) {
+                        const bool grow = big_top > d + kGrowth;
+                        const float to = floorf(big_top), alpha = !grow ? 1.f : ex2(d - to);
+                        if (grow) d = to;
+                        if (t > 0 && __any_sync(0xffffffffu, grow)) scale_o(t, alpha);
+                    }
+                    uint32_t x[16], packed[8];
+                    tmem_ld16(taddr + g * 16, x);
+                    tmem_ld_wait();
                     if (i < 4) {
 #pragma unroll
                         for (int c = 0; c < 16; ++c) top = c < there ? fmaxf(top, __uint_as_float(x[c]) * f) : top;
+                    } else if (i < 8) {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) big_top = c < there ? fmaxf(big_top, fmaf(__uint_as_float(x[c]), f, -m) + plus) : big_top;
                     } else {
+                        const float off = plus + (kUnitLog2 - reference(d));
 #pragma unroll
                         for (int c = 0; c < 16; c += 2) {
                             float e[2];
 #pragma unroll
                             for (int j = 0; j < 2; ++j) {
-                                const float z = __uint_as_float(x[c + j]);
-                                e[j] = c + j < there ? ex2(fmaf(z, f, off)) : 0.f;
-                                sum += c + j < there ? ex2(fmaf(z, f, -m)) : 0.f;
+                                const float z = fmaf(__uint_as_float(x[c + j]), f, -m);
+                                e[j] = c + j < there ? ex2(z + off) : 0.f;
+                                sum += c + j < there ? ex2(z) : 0.f;
                             }
                             packed[c / 2] = pack_f16(e[0], e[1]);
                         }
@@ -613,8 +624,8 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
             if (!ok) break;
             if (steps > 0) tc_fence_after();
             const bool nothing = l == 0.f;
-            // 2^(big_m - m_ref) may be out of fp32 where the result is not: its root comes twice
-            const float half = ex2(0.5f * (big_m - m_ref - kUnitLog2)), by = half / l;
+            // 2^d may be out of fp32 where the result is not: its root comes twice
+            const float half = ex2(0.5f * (d - kUnitLog2)), by = half / l;
             float* const out = work.partial(p, seg, D);
             // Results leave through the warp's part of q (its scores are done), so that whole rows are written at a time: 64 fp32 elements of
             // a row, or all 16-bit ones, at once.

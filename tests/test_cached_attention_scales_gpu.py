@@ -9,13 +9,12 @@ import math
 import pytest
 import torch
 
-from test_kv_cache_gpu import HALF_STEP, HALF_SUBNORMAL, cuda_mod, make_cache, make_table, on_gpu, starts_of
+from test_kv_cache_gpu import HALF_STEP, HALF_SUBNORMAL, TYPES, cuda_mod, make_cache, make_table, on_gpu, starts_of
 
 pytestmark = pytest.mark.gpu
 
-TYPES = [torch.bfloat16, torch.float16]
-# new tokens, lengths, query heads of a cache head: rows of the kernel of many
-CALLS = {"chunks": ([40, 130], [500, 290], 2), "long": ([200], [1500], 4)}
+# new tokens, lengths, query heads of a cache head: rows of the kernel of few rows (drafts, chunks) and of the one of many
+CALLS = {"drafts": ([20], [263], 1), "ragged": ([5, 1, 17], [66, 33, 387], 3), "chunks": ([40, 130], [500, 290], 2), "long": ([200], [1500], 4)}
 
 
 def definition(cache, q, table, lengths, starts, scale):
@@ -77,7 +76,7 @@ def setup(call, page, dim, dtype, seed):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("page,dim", [(16, 64), (32, 128), (64, 128), (128, 64)])
+@pytest.mark.parametrize("page,dim", [(16, 64), (32, 128), (64, 128), (128, 64), (16, 96), (32, 256)])
 @pytest.mark.parametrize("call", CALLS)
 def test_values_of_pages_that_a_row_does_not_see(dtype, page, dim, call):
     """The newest page of each sequence stands for far larger values than all others: finite ones, and then NaN."""
@@ -103,7 +102,7 @@ def test_values_of_pages_that_a_row_does_not_see(dtype, page, dim, call):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("page,dim", [(16, 64), (64, 128)])
+@pytest.mark.parametrize("page,dim", [(16, 64), (64, 128), (32, 256)])
 @pytest.mark.parametrize("call", CALLS)
 @pytest.mark.parametrize("power", [-40, 40, 90])
 def test_values_far_from_the_others_that_nobody_attends_to(dtype, page, dim, call, power):
@@ -134,3 +133,39 @@ def test_value_scales_at_the_ends_of_their_range(dtype, call, scales):
     want, want_lse, bound, _ = definition(cache, q, table, lengths, starts, 0.1)
     check(o, want, bound, slice(None))
     assert bool(((lse - want_lse).abs() <= 2.0 ** -14).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("values", [0.02, 1e-9, 3e5])
+@pytest.mark.parametrize("scale", [30.0, 3e4, 1e6])
+def test_scores_far_from_zero(dtype, call, values, scale):
+    """Scores of thousands to 10^8: one key has all of a row's weight but e^-30 unless the next one is within the scores' own rounding (rows
+    for which it is are not looked at). Then the result is its value: the weight's rounding, the result's, and e^-30 of the others,
+    whatever log2 of the value scale is beside the score."""
+    cache, q, table, lengths, starts = setup(call, 32, 128, dtype, 50)
+    cache.v_scale.fill_(values)
+    o, lse = run(cache, q, table, lengths, starts, scale)
+    heads, page, dim = cache.k.shape[1:]
+    looked_at = 0
+    for b, length in enumerate(lengths):
+        n = int(starts[b + 1] - starts[b])
+        pages = torch.from_numpy(table[b, :-(-length // page)]).long().cuda()
+        k, v = ((c[pages].double() * s[pages].double()[:, :, None, None]).transpose(0, 1).flatten(1, 2)[:, :length] for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+        for i in range(n):
+            row = int(starts[b]) + i
+            x = q[row].double().unflatten(0, (heads, -1))
+            seen = length - n + i + 1
+            z = torch.einsum("hgd,hkd->hgk", x, k[:, :seen]) * scale
+            error = (dim / 16) * 2.0 ** -22 * scale * (x.abs().sum(-1) * 255 * 0.025)
+            two, at = z.topk(2, dim=-1)
+            clear = (two[..., 0] - two[..., 1] > 2 * error + 30).flatten()
+            want = torch.stack([v[h, at[h, :, 0]] for h in range(heads)]).flatten(0, 1)
+            off = (o[row].double() - want).abs() - (HALF_STEP[dtype] + (2.0 ** -20 if dtype == torch.float32 else 2.0 ** -11 + 2.0 ** -20)) * want.abs() - HALF_SUBNORMAL[dtype]
+            others = seen * math.exp(-30) * 127 * values
+            lost = 0 if dtype == torch.float32 else 2.0 ** -27 * 128 * seen * values  # of sums with 128 beside every code
+            off = torch.where(want.abs() > 0.99 * torch.finfo(dtype).max, -1.0, off - lost - others)
+            assert bool((off[clear] <= 0).all()), float(off[clear].max())
+            assert bool(((lse[row].double() - two[..., 0].flatten()).abs() <= error.flatten() + 2.0 ** -22 * two[..., 0].abs().flatten() + 2.0 ** -19)[clear].all())
+            looked_at += int(clear.sum())
+    assert looked_at > 0
