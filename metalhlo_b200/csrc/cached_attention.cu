@@ -59,10 +59,13 @@ __device__ __forceinline__ uint32_t turned(uint32_t x) {  // the transpose of an
 // Codes as fp16. A code with its sign bit turned round is code + 128 in 0 .. 255: as the low byte of an fp16 number with nothing else
 // that is the subnormal (code + 128) 2^-24, which the tensor cores take as it is. The 128 comes off again from the sums: those of q
 // are known beforehand, those of the weights are one more column of the product. With 16-bit inputs that saves the subtraction of
-// every code (a quarter of all instructions) and costs an output some 2^-21 of the largest value that a code can stand for, whatever the
-// weights: a fraction of a percent of a code's step. In fp32 the sums would lose too much, so there a code is put behind 0x64 (1024 + x) and
-// 1152 is taken off, which is exact.
+// every code (a quarter of all instructions). A sum that carries 128 times the weights loses digits with every step of 16 keys (the
+// tensor cores cut off, all in one direction), so it comes off every kCorrect tiles: 2 steps each, 2^-22 of at most 255 weights a step, make
+// 2^-11 of a code's step at most, however many keys there are. Without, averages of 131072 keys were off by 0.015 of a code's step, 5 % of
+// what is left of them; now by 5e-6 (head dimension 128, 12 rows). In fp32 the sums would lose too much, so there a code is put behind 0x64
+// (1024 + x) and 1152 is taken off, which is exact.
 constexpr uint32_t kSignBits = 0x80808080u;
+constexpr int kCorrect = 4;
 template <bool EXACT>
 __device__ __forceinline__ uint32_t two_codes(uint32_t codes, uint32_t order) {
     if (!EXACT) return __byte_perm(codes, 0, order);
@@ -628,6 +631,16 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
                             }
                         }
                 }
+            if (!kTwoParts && (i & (kCorrect - 1)) == kCorrect - 1) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+                        for (int t = 0; t < D / 16; ++t) o[t][j][e] -= o_bias[j][e];
+                        o_bias[j][e] = 0.f;
+                    }
+            }
             __syncwarp();
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");

@@ -169,3 +169,31 @@ def test_scores_far_from_zero(dtype, call, values, scale):
             assert bool(((lse[row].double() - two[..., 0].flatten()).abs() <= error.flatten() + 2.0 ** -22 * two[..., 0].abs().flatten() + 2.0 ** -19)[clear].all())
             looked_at += int(clear.sum())
     assert looked_at > 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("dim,group", [(64, 1), (128, 12), (96, 4), (256, 2)])
+@pytest.mark.parametrize("length", [8192, 131072])
+def test_averages_over_many_keys(dtype, dim, group, length):
+    """q = 0: every key has the same probability, and value scales of 11 bits are exact as fp16 weights, so nothing is rounded but sums and the
+    result. What it costs to carry 128 with every code may not grow with the number of keys: between two corrections there are 8 steps of
+    16 keys, each off by 2^-22 of at most 255 times the weights since the last, together 2^-11 of the sum of the weights, which is below 2.
+    The codes' own sum: a step is off by 2^-22 of it; after k of a warp's n keys it is below six deviations, 6 * 73.6 * 1.5 sqrt(k), so over
+    n / 16 steps and divided by n it is 2^-22 * 6 * 110 * (2 / 3) sqrt(n) / 16, for a warp's 37900 keys at most (head dimension 256: three
+    warps) 2^-9.6."""
+    heads, seqs, page = 4, 64, 128
+    cuda = cuda_mod()
+    pages = length // page
+    cache = cuda.KvCache.empty(pages, heads, dim, page)
+    g = torch.Generator(device="cuda").manual_seed(47)
+    for codes in (cache.k, cache.v):
+        codes.copy_(torch.randint(-127, 128, codes.shape, generator=g, device="cuda", dtype=torch.int8))
+    cache.k_scale.fill_(1.0)
+    cache.v_scale.copy_(1 + torch.randint(0, 1024, cache.v_scale.shape, generator=g, device="cuda") / 1024)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(seqs, pages).contiguous()  # all sequences read the same pages
+    lengths = torch.full((seqs,), length, dtype=torch.int32, device="cuda")
+    q = torch.zeros(seqs, heads * group, dim, dtype=dtype, device="cuda")
+    o = cuda.cached_attention(q, cache, table, lengths, 1.0).double()
+    want = (cache.v.double() * cache.v_scale.double()[:, :, None, None]).mean(dim=(0, 2)).repeat_interleave(group, 0)
+    worst = ((o - want).abs() - HALF_STEP[dtype] * want.abs()).max()
+    assert float(worst) <= 2.0 ** -10 + 2.0 ** -9.6, float(worst)
