@@ -316,6 +316,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
                 if (base1 >= 0) load_half<D>(k_lane + base1, v_lane + base1, ring + stage * 2 * L::kTileBytes, 1);
                 asm volatile("cp.async.commit_group;" ::: "memory");
                 if ((i & 15) == 0) {  // only now: the copies do not wait for the scales
+                    ks = key_scale(ks, p.key_unit);
                     vs_log2 = log2f(vs);
                     if (!kTwoParts) vs = __fdividef(exp2f(-kUnitLog2), vs);
                 }
@@ -820,7 +821,7 @@ int launch(const KvArgs& kv, const void* q, const int64_t* qs, int64_t q_heads, 
     for (int i = 0; i < 2; ++i) p.qs[i] = qs[i], p.os[i] = os[i];
     p.q_heads = static_cast<int32_t>(q_heads);
     p.group = static_cast<int32_t>(q_heads / kv.heads);
-    p.scale = scale;
+    set_scale(&p, scale);
     p.whole = scratch == nullptr;
     constexpr int64_t E = VecTraits<T>::kElems;
     p.q_vec = aligned16(q) && qs[0] % E == 0 && qs[1] % E == 0;

@@ -7,6 +7,9 @@
 // CTAs: no atomics, and no order of arrival in the result.
 #pragma once
 
+#include <algorithm>
+#include <cmath>
+
 #include "kv_cache.cuh"
 
 namespace mhlo {
@@ -23,7 +26,7 @@ struct CachedParams {
     float* lse;
     int64_t qs[2], os[2];
     int32_t q_heads, group;
-    float scale;
+    float scale, key_unit;  // the scale of the scores is scale * key_unit: see set_scale()
     int32_t q_vec;      // rows of q on the 16-byte grid
     int32_t o_vec;      // 1: results four at a time, 2: rows of o on the 16-byte grid
     int32_t whole;      // no segment has more than the least share of a CTA: none is cut
@@ -41,6 +44,15 @@ void cached_scratch(CachedParams<T>* p, int64_t ctas, void* scratch) {
 }
 constexpr int kLongRows = 256;
 
+// A scale in [2^-12, 2^-11) goes with the queries, whose own powers of two (2^-120 .. 2^114, and 2^24 where codes are subnormals of fp16)
+// then leave it an ordinary number; the other power of two, as far as it is one itself, goes with the scales of the keys.
+template <typename T>
+void set_scale(CachedParams<T>* p, float scale) {
+    const int exponent = std::min(std::ilogb(scale) + 12, 120);
+    p->scale = std::scalbn(scale, -exponent);
+    p->key_unit = std::scalbn(1.f, exponent);
+}
+
 struct Piece {  // what joining a cut segment needs: CTAs it goes over, its rows
     int32_t count, first_row, rows, seq_first, head, pad[3];
 };
@@ -56,6 +68,12 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// A key scale in units of key_unit. It stays finite: products of zero are zero whatever the scale.
+__device__ __forceinline__ float key_scale(float ks, float unit) {
+    const float x = ks * unit;
+    return x > 3.4028235e38f ? 3.4028235e38f : x;
 }
 
 template <int V>

@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                     }
                     if (most - least > 30.f) least = -INFINITY;
                     if (lane < kGroups) {
-                        s.key[lane] = now.base < 0 ? 0.f : now.ks;
+                        s.key[lane] = now.base < 0 ? 0.f : key_scale(now.ks, p.key_unit);
                         s.value_log2[lane] = value_log2;
                         s.out_again[lane] = now.base < 0 ? 0.f : __fdividef(1.f / kUnit, now.vs);
                         if ((lane & 3) == 0) s.least[lane >> 2] = least;

@@ -171,6 +171,23 @@ def test_scores_far_from_zero(dtype, call, values, scale):
     assert looked_at > 0
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("scale,keys,queries", [(1e33, 1e-33, 1), (1e38, 1e-36, 1e-2), (1e-30, 1e30, 1), (1e-33, 1, 1e33), (1e-1, 1e-36, 1e37), (1e30, 1, 1e-30)])
+def test_scales_of_scores_keys_and_queries_that_make_up_for_one_another(dtype, call, scale, keys, queries):
+    """Ordinary scores from numbers that are not; a row of zeros has scores of zero whatever the scale."""
+    if dtype == torch.float16 and queries not in (1, 1e-2):
+        pytest.skip("queries beyond fp16")
+    cache, q, table, lengths, starts = setup(call, 32, 128, dtype, 53)
+    cache.k_scale.mul_(keys)
+    q = (q.double() * queries).to(dtype)
+    q[0] = 0
+    o, lse = run(cache, q, table, lengths, starts, scale * 0.1)
+    want, want_lse, bound, _ = definition(cache, q, table, lengths, starts, float(torch.tensor(scale * 0.1, dtype=torch.float32)))
+    check(o, want, bound, slice(None))
+    assert bool(((lse - want_lse).abs() <= 2.0 ** -14).all())
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
 @pytest.mark.parametrize("dim,group", [(64, 1), (128, 12), (96, 4), (256, 2)])
 @pytest.mark.parametrize("length", [8192, 131072])
