@@ -191,11 +191,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either i
     return y;
 }
 
-// A thread keeps the elements of its units as they are and rotates them twice, for the maximum and for the codes: that leaves registers
-// for three CTAs of 256 threads (80 each; chunks of 4400 tokens, 32 + 8 + 8 heads of 128: 37 us with the rotated numbers kept, 122
-// registers; 33 as they are with 122; 31 with 80). The largest pages of the widest heads have 512 threads to a CTA.
+// A thread keeps the elements of its units as they are and rotates them twice, for the maximum and for the codes: with 16-bit types that
+// leaves registers for three CTAs of 256 threads (80 each; chunks of 4400 tokens, 32 + 8 + 8 heads of 128: 37 us with the rotated numbers kept,
+// 122 registers; 33 as they are with 122; 31 with 80). fp32 elements are 64 registers by themselves: 80 in all spilled 1 KB a thread,
+// and two CTAs of 122 take 36.4 us for five chunks of 880 tokens instead of 42.6, 13.7 instead of 23.7 without queries. The largest pages
+// of the widest heads have 512 threads to a CTA.
 template <typename T, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 1) append_kernel(const __grid_constant__ AppendParams<T> p) {
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? (sizeof(T) == 2 ? 3 : 2) : 1) append_kernel(const __grid_constant__ AppendParams<T> p) {
     const KvArgs& a = p.kv;
     if (blockIdx.x >= p.blocks) return rotate_rows(p, static_cast<int32_t>(blockIdx.x - p.blocks) * p.rows);
     // Block `slot` of the sequences' touched blocks. A sequence has n / P + 2 slots at least, as many as n tokens can touch:
