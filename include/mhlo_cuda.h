@@ -647,9 +647,11 @@ int mhlo_cuda_peer_barrier(void* const* flag_devs, int32_t n_ranks, int32_t rank
 
 /*
  * Every wait inside the tensor-core kernels (mbarrier phases fed by TMA and tcgen05.commit) is bounded; a kernel
- * whose wait expires records a non-zero word and drains instead of spinning. This call synchronises the device,
- * reads and clears that word: *out_code = 0 when no kernel gave up since the last call. It also reports (200 and above) what
- * the key/value cache kernels found wrong with their page tables, lengths and starts.
+ * whose wait expires records a non-zero word and drains instead of spinning; the key/value cache kernels record what they
+ * found wrong with their page tables, lengths and starts. This call synchronises the device and reads the words in turn
+ * (GEMM, attention: 100 + code, cache and attention over it: 200 + code). *out_code = 0 and MHLO_CUDA_OK: none is set. Else the
+ * first one is cleared, *out_code has its code and MHLO_CUDA_EXECUTION_FAILED is returned with the text in
+ * mhlo_cuda_last_error(); words behind it are left for the next call.
  */
 int mhlo_cuda_device_error(int32_t* out_code);
 

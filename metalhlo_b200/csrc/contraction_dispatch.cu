@@ -158,17 +158,19 @@ extern "C" {
 
 int mhlo_cuda_device_error(int32_t* out_code) {
     if (!out_code) return fail(MHLO_CUDA_INVALID_ARGUMENT, "device_error: null output");
-    const int g = gemm_device_error(), a = attention_device_error(), c = kv_cache_device_error(), r = cached_attention_device_error();
-    if (g < 0 || a < 0 || c < 0 || r < 0) return fail(MHLO_CUDA_EXECUTION_FAILED, "device_error: %s", cudaGetErrorString(cudaGetLastError()));
-    const int kv = c != 0 ? c : r;
-    *out_code = g != 0 ? g : (a != 0 ? 100 + a : (kv != 0 ? 200 + kv : 0));
-    if (*out_code > 200) {
-        static const char* const what[] = {"", "a page outside the cache", "a length beyond the table or below the sequence's rows",
-                                           "token_starts out of order", "a position behind the rotation table"};
-        return fail(MHLO_CUDA_EXECUTION_FAILED, "a key/value cache kernel met %s (code %d)", kv <= 4 ? what[kv] : "a bounded wait that ran out", *out_code);
-    }
-    if (*out_code != 0) return fail(MHLO_CUDA_EXECUTION_FAILED, "a tensor-core kernel gave up on a bounded wait (code %d)", *out_code);
-    return MHLO_CUDA_OK;
+    // One word at a time: the others are left for the next calls.
+    *out_code = 0;
+    int v = gemm_device_error(), base = 0;
+    if (v == 0) v = attention_device_error(), base = 100;
+    if (v == 0) v = kv_cache_device_error(), base = 200;
+    if (v == 0) v = cached_attention_device_error();
+    if (v < 0) return fail(MHLO_CUDA_EXECUTION_FAILED, "device_error: %s", cudaGetErrorString(cudaGetLastError()));
+    if (v == 0) return MHLO_CUDA_OK;
+    *out_code = base + v;
+    static const char* const what[] = {"", "a page outside the cache", "a length beyond the table or below the sequence's rows", "token_starts out of order",
+                                       "a position behind the rotation table"};
+    if (base == 200 && v <= 4) return fail(MHLO_CUDA_EXECUTION_FAILED, "a key/value cache kernel met %s (code %d)", what[v], *out_code);
+    return fail(MHLO_CUDA_EXECUTION_FAILED, "a tensor-core kernel gave up on a bounded wait (code %d)", *out_code);
 }
 
 namespace {
