@@ -547,6 +547,15 @@ namespace {
 
 const char* dtype_key(int dtype) { return dtype == MHLO_DT_BF16 ? "bf16" : dtype == MHLO_DT_F16 ? "f16" : "f32"; }
 
+// The code that a GEMM or attention kernel left on the null stream when a wait of it expired, 0 if none; what the caller's key/value cache
+// kernels may have left stays for the caller.
+int32_t contraction_error() {
+    int32_t code = 0;
+    if (mhlo_cuda_device_error_fetch(nullptr) != 0 || mhlo_cuda_stream_sync(nullptr) != 0) return -1;
+    mhlo_cuda_device_error_take(&code);
+    return code;
+}
+
 // 5 warm-up + 20 timed launches of `launch`, median in seconds (AutoTuner.swift:242-245, 479-513); < 0 when a launch failed.
 double median_seconds(const std::function<int()>& launch, void* e0, void* e1) {
     constexpr int kWarmup = 5, kTimed = 20;
@@ -672,8 +681,7 @@ int tune_gemm(const GemmCase& c, int max_trials, TuningDatabase* db, TuningRecor
             best.measured_time_s = sec;
         }
     }
-    int32_t device_code = 0;
-    mhlo_cuda_device_error(&device_code);
+    const int32_t device_code = contraction_error();
     cleanup();
     if (tried == 0 || device_code != 0) {
         *why = tried == 0 ? "tune_gemm: no candidate could be launched" : "tune_gemm: a kernel gave up on a bounded wait";
@@ -751,8 +759,7 @@ int tune_attention(const AttentionCase& c, int max_trials, TuningDatabase* db, T
             best.measured_time_s = sec;
         }
     }
-    int32_t device_code = 0;
-    mhlo_cuda_device_error(&device_code);
+    const int32_t device_code = contraction_error();
     cleanup();
     if (tried == 0 || device_code != 0) {
         *why = tried == 0 ? "tune_attention: no candidate could be launched" : "tune_attention: a kernel gave up on a bounded wait";

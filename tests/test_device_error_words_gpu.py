@@ -35,3 +35,15 @@ def test_words_are_reported_one_after_the_other():
     bad_page(cuda, attend=False)
     assert take(cuda) == (failed, 201) and "a page outside the cache" in cuda.last_error()
     assert take(cuda) == (0, 0)
+
+
+def test_a_tuner_neither_takes_nor_minds_the_words_of_the_cache(tmp_path):
+    from metalhlo_b200 import capi, cuda
+
+    assert cuda.device_error() == 0
+    bad_page(cuda, attend=False)
+    capi.tuning.open(str(tmp_path / "gemm.json"))
+    client = capi.Client()
+    assert capi.tuning.tune_gemm(client, capi.F16, 1, 256, 256, 256, max_trials=2)["configsTried"] == 2
+    assert capi.tuning.tune_attention(client, capi.BF16, 1, 2, 256, 256, 64)["configsTried"] >= 1
+    assert cuda.device_error() == 201 and cuda.device_error() == 0
