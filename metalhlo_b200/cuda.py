@@ -593,18 +593,22 @@ def kv_cache_append(cache: KvCache, k, v, page_table, lengths, token_starts=None
 
 def kv_cache_read(cache: KvCache, page_table, lengths, max_tokens: int, dtype=None, k_out=None, v_out=None, stream=None):
     """(k, v), each [seqs, max_tokens, heads, head_dim] of ``dtype`` (float32): the values in the cache, zero behind a sequence's
-    length. See ``mhlo_cuda_kv_cache_read``."""
+    length. ``k_out`` and ``v_out`` have one set of strides; one that is not given gets the other's. See ``mhlo_cuda_kv_cache_read``."""
     import torch
 
     _same_device(cache.k, page_table, lengths, k_out, v_out)
     seqs = lengths.shape[0]
     batch = _kv_batch(page_table, lengths, None, seqs)
     shape = (seqs, max_tokens, *cache.head_shape)
-    dtype = k_out.dtype if k_out is not None else dtype or torch.float32
+    given = k_out if k_out is not None else v_out
+    dtype = given.dtype if given is not None else dtype or torch.float32
+
+    def fresh():
+        return torch.empty(shape, dtype=dtype, device=lengths.device) if given is None else torch.empty_strided(shape, given.stride(), dtype=dtype, device=lengths.device)
 
     def call(s):
-        k = torch.empty(shape, dtype=dtype, device=lengths.device) if k_out is None else k_out
-        v = torch.empty_like(k) if v_out is None else v_out
+        k = fresh() if k_out is None else k_out
+        v = fresh() if v_out is None else v_out
         seq, token, head, step = k.stride()
         assert k.shape == v.shape == shape and v.dtype == dtype and v.stride() == k.stride() and step == 1
         check(lib.mhlo_cuda_kv_cache_read(torch_dtype_code(dtype), cache.pointer, C.byref(batch), max_tokens, k.data_ptr(), v.data_ptr(),
