@@ -448,7 +448,10 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) odd = odd || (fabsf(top[j][r]) > kNearZero && top[j][r] != -INFINITY);
+                        for (int r = 0; r < 2; ++r) {
+                            const bool valueless = d[j][r] == -INFINITY && m[j][r] != -INFINITY;  // value scales of 0 so far: m may be anywhere
+                            odd = odd || valueless || (fabsf(top[j][r]) > kNearZero && top[j][r] != -INFINITY);
+                        }
                     plain = !__any_sync(0xffffffffu, odd);
                 }
                 if (plain) {  // then m is as near to the largest z as the value scales are to one another
@@ -655,11 +658,13 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) l[j][r] += __shfl_xor_sync(0xffffffffu, l[j][r], x);
                 if (g == 0) {
-                    if (kTwoParts) {
-                        sm[warp][8 * j + 2 * c + r] = m[j][r];
-                        sd[warp][8 * j + 2 * c + r] = d[j][r];
-                    }
-                    sl[warp][8 * j + 2 * c + r] = l[j][r];
+                    // the sum's power of two goes to its reference, which may have stayed behind: sums of other warps are weighed by that
+                    float &m_out = sm[warp][8 * j + 2 * c + r], &d_out = sd[warp][8 * j + 2 * c + r];
+                    if (kTwoParts) m_out = m[j][r], d_out = d[j][r];
+                    const float up = whole_log2(l[j][r]), unit = sum_unit(d_out);
+                    sl[warp][8 * j + 2 * c + r] = l[j][r] * ex2(-up);
+                    m_out += unit + up;
+                    d_out -= unit + up;
                 }
             }
         if (lane == 0) used[warp] = mine > 0;
@@ -692,8 +697,7 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
             for (int i = 0; i < W; ++i)
                 if (sd[i][tid] != -INFINITY) unit = fmaxf(unit, sd[i][tid] + (sm[i][tid] - most));
             for (int i = 0; i < W; ++i) {
-                const float l = sl[i][tid] * ex2(sum_unit(sd[i][tid]));
-                sum += sm[i][tid] == -INFINITY ? l : l * ex2(sm[i][tid] - most);
+                sum += sm[i][tid] == -INFINITY ? sl[i][tid] : sl[i][tid] * ex2(sm[i][tid] - most);
                 sf[i][tid] = sd[i][tid] == -INFINITY ? 0.f : pow2_of(sd[i][tid] + (sm[i][tid] - most) - unit);
             }
             const float whole = unit == -INFINITY ? 0.f : unit - kUnitLog2 + (kTwoParts ? 0.f : 24.f), first = floorf(0.5f * whole);

@@ -70,6 +70,11 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// The power of two of a sum; 0 for sums that have none.
+__device__ __forceinline__ float whole_log2(float l) {
+    return l > 1e-37f && l < INFINITY ? static_cast<float>(static_cast<int>(__float_as_uint(l) >> 23) - 127) : 0.f;
+}
+
 // A key scale in units of key_unit. It stays finite: products of zero are zero whatever the scale.
 __device__ __forceinline__ float key_scale(float ks, float unit) {
     const float x = ks * unit;

@@ -675,9 +675,10 @@ __global__ void __launch_bounds__(kThreads, 1) cached_attention_tc_kernel(const 
                 }
             }
             if (r < seg.rows) {
-                if (seg.cut) {
-                    out[r] = m_ref;
-                    out[kRows + r] = l;
+                if (seg.cut) {  // the sum's power of two goes to its reference, which may have stayed behind: other pieces are weighed by that
+                    const float up = whole_log2(l);
+                    out[r] = m_ref + up;
+                    out[kRows + r] = l * ex2(-up);
                 } else if (p.lse != nullptr) {
                     p.lse[token * p.q_heads + q_head] = nothing ? -INFINITY : (m_ref + log2f(l)) * 0.6931471805599453f;
                 }

@@ -135,6 +135,31 @@ def test_value_scales_at_the_ends_of_their_range(dtype, call, scales):
     assert bool(((lse - want_lse).abs() <= 2.0 ** -14).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("page,dim", [(16, 64), (64, 128), (32, 256)])
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("order", ["first", "last"])
+def test_pages_without_values_that_have_all_the_weight(dtype, page, dim, call, order):
+    """The first page, or the last that all rows see whole, has value scale 0 and scores some 2^95 above all others; those grow by 2^40 on
+    their way. What is left of a row is 2^-95 of its other pages' average, as exact as if it were all."""
+    cache, q, table, lengths, starts = setup(call, page, dim, dtype, 56)
+    q = (q.abs() * 0.05 + 1.0).to(dtype)
+    for b, length in enumerate(lengths):
+        known = (length - int(starts[b + 1] - starts[b])) // page  # pages that all of its rows see whole
+        pages = torch.from_numpy(table[b, :-(-length // page)].copy()).long().cuda()
+        for i, at in enumerate(pages.tolist()):  # scores of 2^-20 .. 2^20 around 0
+            cache.k[at] = 0
+            cache.k[at, :, :, 0] = -100 + 200 * i // max(1, len(pages) - 1)
+            cache.k_scale[at] = 0.2
+        if known > 1:
+            at = pages[0 if order == "first" else known - 1]
+            cache.k[at], cache.k_scale[at], cache.v_scale[at] = 100, 86 / 100 / dim, 0.0
+    o, lse = run(cache, q, table, lengths, starts, 1.0)
+    want, want_lse, bound, _ = definition(cache, q, table, lengths, starts, 1.0)
+    check(o, want, bound, slice(None))
+    assert bool(((lse - want_lse).abs() <= 2.0 ** -13).all())
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("call", CALLS)
 @pytest.mark.parametrize("values", [0.02, 1e-9, 3e5])
