@@ -41,11 +41,6 @@ struct Layout {
 
 // ---- the kernel's parts ----------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ float fmax3(float a, float b, float c) {  // one instruction on sm_100
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 __device__ __forceinline__ void mma_f16(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -136,11 +131,10 @@ __device__ __forceinline__ int step_element(int step, int c) {
 template <typename T>
 constexpr float kUnitLog2Of = sizeof(T) == 4 ? 14.f : 6.f;
 template <typename T>
-constexpr float kHeadroomOf = sizeof(T) == 4 ? 1.f : 8.f;
+constexpr float kHeadroomOf = sizeof(T) == 4 ? 1.9f : 8.f;
 constexpr float kNone = -3e38f;  // m + d of a row that has seen nothing: below every sum, but less -infinity it is not NaN
-__device__ __forceinline__ float pow2_of(float whole) {  // 2^whole; 0 and infinity out of fp32's ordinary exponents
-    return whole < -126.f ? 0.f : whole > 127.f ? INFINITY : __int_as_float((static_cast<int>(whole) + 127) << 23);
-}
+// 2^whole; 0 and infinity out of fp32's ordinary exponents. The sum leaves whole + 127 in the low bits.
+__device__ __forceinline__ float pow2_of(float whole) { return __int_as_float(__float_as_int(fminf(fmaxf(whole, -127.f), 128.f) + 12583039.f) << 23); }
 
 // NT: groups of 8 rows.
 template <typename T, int D, int NT>
@@ -437,10 +431,13 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
             if (!plain || move) {
                 load_references();
                 float keep[NT][2];
-                auto over_keys = [&](float x) {
+                auto over_keys = [&](float (&x)[NT][2]) {  // of all rows side by side
 #pragma unroll
-                    for (int i = 4; i < 32; i <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, i));
-                    return x;
+                    for (int lanes = 4; lanes < 32; lanes <<= 1)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) x[j][r] = fmaxf(x[j][r], __shfl_xor_sync(0xffffffffu, x[j][r], lanes));
                 };
                 const float least = fminf(values_log2[0], values_log2[1]);
                 if (plain) {  // may one maximum do?
@@ -455,19 +452,17 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
                     plain = !__any_sync(0xffffffffu, odd);
                 }
                 if (plain) {  // then m is as near to the largest z as the value scales are to one another
+                    over_keys(top);
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            const float x = over_keys(top[j][r]);
-                            keep[j][r] = 1.f;
-                            if (x > both[j][r] + kHeadroom) {
-                                const float to = floorf(x), to_m = to - floorf(least);
-                                keep[j][r] = ex2(both[j][r] - to);
-                                l[j][r] *= m[j][r] == -INFINITY ? 0.f : ex2(m[j][r] + sum_unit(d[j][r]) - to);
-                                if (to_m > m[j][r]) m[j][r] = to_m;
-                                d[j][r] = to - m[j][r];
-                            }
+                            const bool grow = top[j][r] > both[j][r] + kHeadroom;
+                            const float to = floorf(top[j][r]), was = m[j][r];
+                            keep[j][r] = grow ? ex2(both[j][r] - to) : 1.f;
+                            l[j][r] *= !grow ? 1.f : was == -INFINITY ? 0.f : ex2(was + sum_unit(d[j][r]) - to);
+                            m[j][r] = grow ? fmaxf(was, to - floorf(least)) : was;
+                            d[j][r] = grow ? to - m[j][r] : d[j][r];
                         }
                 } else {
                     move = false;
@@ -480,23 +475,46 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
                         }
                     move = __any_sync(0xffffffffu, move);
                     if (move) {
+                        // With value scales within a factor of 2 the largest z bounds the largest z - m + log2 vs closely enough.
+                        float mine[NT][2];
+                        bool odd = !(fabsf(values_log2[0] - values_log2[1]) <= 1.f);
 #pragma unroll
                         for (int j = 0; j < NT; ++j)
 #pragma unroll
                             for (int r = 0; r < 2; ++r) {
-                                const float z = over_keys(fmaxf(largest(j, r, 0) * f[0][j][r], largest(j, r, 1) * f[1][j][r])), before = m[j][r], unit = sum_unit(d[j][r]);
-                                if (z > before + kHeadroom) {
-                                    m[j][r] = floorf(z);
-                                    d[j][r] += before == -INFINITY ? 0.f : before - m[j][r];
-                                }
-                                const float x = over_keys(fmaxf(fmaf(largest(j, r, 0), f[0][j][r], -m[j][r]) + values_log2[0], fmaf(largest(j, r, 1), f[1][j][r], -m[j][r]) + values_log2[1]));
-                                keep[j][r] = 1.f;
-                                if (x > d[j][r] + kHeadroom) {
-                                    const float to = floorf(x);
-                                    keep[j][r] = d[j][r] == -INFINITY ? 0.f : ex2(d[j][r] - to);
-                                    d[j][r] = to;
-                                }
-                                l[j][r] *= before == -INFINITY ? 0.f : ex2((before - m[j][r]) + (unit - sum_unit(d[j][r])));
+                                mine[j][r] = fmaxf(largest(j, r, 0) * f[0][j][r], largest(j, r, 1) * f[1][j][r]);
+                                odd = odd || (fabsf(mine[j][r]) > kNearZero && mine[j][r] != -INFINITY);
+                            }
+                        odd = __any_sync(0xffffffffu, odd);
+                        over_keys(mine);
+                        float before[NT][2];
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const bool grow = mine[j][r] > m[j][r] + kHeadroom;
+                                before[j][r] = m[j][r];
+                                m[j][r] = grow ? floorf(mine[j][r]) : m[j][r];
+                                mine[j][r] = (mine[j][r] - m[j][r]) + fmaxf(values_log2[0], values_log2[1]);
+                            }
+                        if (odd) {
+#pragma unroll
+                            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                                for (int r = 0; r < 2; ++r)
+                                    mine[j][r] = fmaxf(fmaf(largest(j, r, 0), f[0][j][r], -m[j][r]) + values_log2[0], fmaf(largest(j, r, 1), f[1][j][r], -m[j][r]) + values_log2[1]);
+                            over_keys(mine);
+                        }
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const bool first = before[j][r] == -INFINITY;
+                                const float down = first ? 0.f : before[j][r] - m[j][r], unit = sum_unit(d[j][r]), now = d[j][r] + down, to = floorf(mine[j][r]);
+                                const bool grow = mine[j][r] > now + kHeadroom;
+                                keep[j][r] = !grow ? 1.f : now == -INFINITY ? 0.f : ex2(now - to);
+                                d[j][r] = grow ? to : now;
+                                l[j][r] *= first ? 0.f : ex2(down + (unit - sum_unit(d[j][r])));
                             }
                     }
                 }
@@ -692,14 +710,19 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
         }
         __syncthreads();
         if (tid < kRows) {
-            float most = -INFINITY, unit = -INFINITY, sum = 0.f;  // unit: the largest m + d, less most
-            for (int i = 0; i < W; ++i) most = fmaxf(most, sm[i][tid]);
-            for (int i = 0; i < W; ++i)
-                if (sd[i][tid] != -INFINITY) unit = fmaxf(unit, sd[i][tid] + (sm[i][tid] - most));
+            float ms[W], ds[W], ls[W], most = -INFINITY, unit = -INFINITY, sum = 0.f;  // unit: the largest m + d, less most
+#pragma unroll
+            for (int i = 0; i < W; ++i) ms[i] = sm[i][tid], ds[i] = sd[i][tid], ls[i] = sl[i][tid];
+#pragma unroll
+            for (int i = 0; i < W; ++i) most = fmaxf(most, ms[i]);
+#pragma unroll
             for (int i = 0; i < W; ++i) {
-                sum += sm[i][tid] == -INFINITY ? sl[i][tid] : sl[i][tid] * ex2(sm[i][tid] - most);
-                sf[i][tid] = sd[i][tid] == -INFINITY ? 0.f : pow2_of(sd[i][tid] + (sm[i][tid] - most) - unit);
+                sum += ms[i] == -INFINITY ? ls[i] : ls[i] * ex2(ms[i] - most);
+                ds[i] = ds[i] == -INFINITY ? -INFINITY : ds[i] + (ms[i] - most);
+                unit = fmaxf(unit, ds[i]);
             }
+#pragma unroll
+            for (int i = 0; i < W; ++i) sf[i][tid] = ds[i] == -INFINITY ? 0.f : pow2_of(ds[i] - unit);
             const float whole = unit == -INFINITY ? 0.f : unit - kUnitLog2 + (kTwoParts ? 0.f : 24.f), first = floorf(0.5f * whole);
             top_unit[tid] = make_float2(pow2_of(first), pow2_of(whole - first));
             top_m[tid] = most;
