@@ -31,7 +31,7 @@ struct CachedParams {
     int32_t o_vec;      // 1: results four at a time, 2: rows of o on the 16-byte grid
     int32_t whole;      // no segment has more than the least share of a CTA: none is cut
     int32_t few_rows;   // sequences of up to this many rows belong to the kernel of few rows, longer ones to the other
-    int32_t* pieces;    // [CTAs][8]: the cut segment that a CTA's share ends with (Piece), count 0 if none
+    int32_t* pieces;    // [CTAs][8]: the cut segment that a CTA's share ends with: CTAs it goes over (0: none), first row, rows, sequence's first row, head
     float* partial;     // [CTAs][2][ROWS (head_dim + 2)]: maxima (log2), sums, outputs / sums
 };
 
@@ -53,22 +53,12 @@ void set_scale(CachedParams<T>* p, float scale) {
     p->key_unit = std::scalbn(1.f, exponent);
 }
 
-struct Piece {  // what joining a cut segment needs: CTAs it goes over, its rows
-    int32_t count, first_row, rows, seq_first, head, pad[3];
-};
-
 namespace {
 
 // Where one exponential serves a weight and the row's sum. A row has two references: m, near its largest z, and d, so that m + d is near
 // its largest z + log2 vs. A weight is 2^(z - m) times 2^(log2 vs - d + unit): as long as the second factor is above 2^-40 nothing that
 // counts in the sum is lost with the weight. Beyond kNearZero, z - m comes first: log2 vs would be lost beside z.
 constexpr float kReach = 40.f, kBelow = 40.f, kNearZero = 4096.f;
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // The power of two of a sum; 0 for sums that have none.
 __device__ __forceinline__ float whole_log2(float l) {

@@ -132,6 +132,17 @@ inline int allow_dynamic_smem(const void* kernel, int bytes, std::atomic<bool> (
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
 // ---- 16-byte vectors of T <-> fp32 ------------------------------------------------------------------
 
 template <typename T>

@@ -185,11 +185,6 @@ __device__ __forceinline__ uint32_t codes_of(float2 x, float2 y, float step, flo
     const uint32_t lo = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), hi = __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040);
     return __byte_perm(lo, hi, 0x5410);
 }
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
-    float y;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-    return y;
-}
 
 // A thread keeps the elements of its units as they are and rotates them twice, for the maximum and for the codes: with 16-bit types that
 // leaves registers for three CTAs of 256 threads (80 each; chunks of 4400 tokens, 32 + 8 + 8 heads of 128: 37 us with the rotated numbers kept,

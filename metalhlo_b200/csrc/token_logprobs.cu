@@ -62,16 +62,6 @@ __device__ __forceinline__ int64_t target_of(const void* targets, int32_t wide, 
     return wide ? static_cast<const int64_t*>(targets)[row] : static_cast<const int32_t*>(targets)[row];
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
-    float y;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-    return y;
-}
 
 // Logits in the order of the alternatives: NaN above all, -0 = +0.
 __device__ __forceinline__ uint32_t order_of(float x) {
