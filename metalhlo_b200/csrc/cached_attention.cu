@@ -12,7 +12,7 @@
 // nothing of its weight, costs it no digits, however large the block's values are.
 //
 // What bounds it: the codes have to come from memory once, 64 sequences of 8192 keys with 8 heads of 128 (4 query heads each, bf16)
-// 176 us for 1.07 GB, 6.1 TB/s. With fewer or ragged sequences the ends of segments show: 32 of up to 4096 keys 48 us for 179 MB, of
+// 175 us for 1.07 GB, 6.1 TB/s. With fewer or ragged sequences the ends of segments show: 32 of up to 4096 keys 48 us for 179 MB, of
 // which reading alone would take 28. ncu, 32 of 8192 keys: 47 % of issue slots, 21 % of the tensor pipe, 168 registers.
 #include <algorithm>
 #include <type_traits>
@@ -780,14 +780,17 @@ __global__ void __launch_bounds__(Layout<D>::kThreads, 2) cached_attention_kerne
     grid_dependency_wait();
 }
 
-// Sequences of up to this many rows are this kernel's, where the other takes the type. It walks the keys once for each 16 rows, the other
-// once for 256. Rows, this kernel and the other, 64 sequences of 1000 keys, 8 cache heads of 128: 32 rows 90 and 174 us, 64 rows 152 and
-// 176, 96 rows 224 and 176; 8 of 6000 keys: 64 rows 84 and 91, 96 rows 119 and 93; head dimension 64, 8 of 6000 keys: 64 rows 58 and 70,
-// 96 rows 83 and 71.
-constexpr int kFewRows = 64;
 constexpr bool long_takes(int64_t head_dim) { return head_dim == 64 || head_dim == 128; }
+// Sequences of up to this many rows are this kernel's, where the other takes the type. It walks the keys once for each 16 rows, the other
+// once for 256. Calls through this kernel with the other's launch in front, which has nothing to do and takes 7 us, and through the other
+// alone, us, bf16: 64 sequences of 1000 keys, 8 cache heads of 128: 32 rows 105 and 148, 48 rows 143 and 149, 64 rows 165 (less the 7) and
+// 150; 8 of 6000 keys: 48 rows 80 and 84, 64 rows 90 (less the 7) and 85; 2 of 8000: 48 rows 46 and 40; head dimension 64, 64 of 1000: 48
+// rows 98 and 113, 64 rows 117 and 114; 8 of 6000: 48 rows 55 and 67, 64 rows 65 and 66; 2 of 8000: 48 rows 36 and 33.
+constexpr int kFewRows = 48;
 // Whether a sequence of the call may have more rows: the host knows only how many there are in all.
-bool may_be_long(const int32_t* starts, int64_t tokens, int64_t group) { return starts != nullptr && tokens * group > kFewRows; }
+bool may_be_long(const int32_t* starts, int64_t tokens, int64_t group, int64_t head_dim) {
+    return starts != nullptr && long_takes(head_dim) && tokens * group > kFewRows;
+}
 
 template <typename T, int D, int NT>
 int launch_rows(const CachedParams<T>& p, bool behind, cudaStream_t stream) {
@@ -812,12 +815,12 @@ template <typename T, int D>
 int launch_dim(CachedParams<T> p, void* scratch, cudaStream_t stream) {
     // Which kernels: sequences of many rows go to the one, where there may be any, the rest to the other. One sequence by itself that may
     // have many rows goes to the one whatever it has.
-    const bool may_long = sizeof(T) == 2 && long_takes(D) && may_be_long(p.kv.starts, p.kv.tokens, p.group);
+    const bool may_long = sizeof(T) == 2 && may_be_long(p.kv.starts, p.kv.tokens, p.group, D);
     const bool few = !may_long || p.kv.seqs > 1;
     CachedParams<T> many = p;
     many.few_rows = p.few_rows = !may_long ? 0x7fffffff : few ? kFewRows : 0;
-    // Groups of 8 rows as long as the sequences have no more on average: 16 sequences of 4000 keys, 8 cache heads of 128, 8 rows 37 us in
-    // groups of 8 and 43 in groups of 16; 12 rows 50 and 43.
+    // Groups of 8 rows as long as the sequences have no more on average: 16 sequences of 4000 keys, 8 cache heads of 128, 8 rows 38 us in
+    // groups of 8 and 47 in groups of 16; 12 rows 50 and 47.
     const int groups = static_cast<int64_t>(p.kv.tokens) * p.group <= 8 * static_cast<int64_t>(p.kv.seqs) ? 1 : 2;
     cached_scratch(&p, kFewGrid, scratch);
     cached_scratch(&many, kLongGrid, scratch != nullptr ? static_cast<uint8_t*>(scratch) + cached_scratch(kFewGrid, 16, D) : nullptr);
@@ -830,9 +833,9 @@ int launch_dim(CachedParams<T> p, void* scratch, cudaStream_t stream) {
         if (int st = groups == 1 ? launch_rows<T, D, 1>(p, may_long, stream) : launch_rows<T, D, 2>(p, may_long, stream)) return st;
     }
     if (p.whole) return MHLO_CUDA_OK;
-    const int few_rows = few ? 8 * groups : 0, long_rows = may_long ? kLongRows : 0;
-    const cudaError_t e = launch_dependent(join_kernel<T, D>, dim3(few ? kFewGrid : kLongGrid, (few_rows + long_rows) / kJoinRows), dim3(32 * kJoinRows), 0, stream,
-                                           1, true, p, few_rows, static_cast<const int32_t*>(many.pieces), static_cast<const float*>(many.partial), long_rows);
+    const int rows = few ? 8 * groups : 0, long_rows = may_long ? kLongRows : 0;
+    const cudaError_t e = launch_dependent(join_kernel<T, D>, dim3(few ? kFewGrid : kLongGrid, (rows + long_rows) / kJoinRows), dim3(32 * kJoinRows), 0, stream,
+                                           1, true, p, rows, static_cast<const int32_t*>(many.pieces), static_cast<const float*>(many.partial), long_rows);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of cached_attention failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("cached_attention (joining)");
     return MHLO_CUDA_OK;
@@ -879,7 +882,7 @@ int64_t mhlo_cuda_cached_attention_scratch_bytes(const mhlo_cuda_kv_cache* cache
     if (cache->head_dim < 1 || batch->pages_per_seq * cache->page_tokens <= kLeastTiles * kTileKeys) return 0;  // no segment is worth cutting
     const int64_t group = q_heads / std::max<int64_t>(1, cache->heads);
     int64_t bytes = cached_scratch(kFewGrid, 16, cache->head_dim);
-    if (may_be_long(batch->token_starts, batch->tokens, group) && long_takes(cache->head_dim))
+    if (may_be_long(batch->token_starts, batch->tokens, group, cache->head_dim))
         bytes += cached_scratch(kLongGrid, kLongRows, cache->head_dim);
     return bytes;
 }

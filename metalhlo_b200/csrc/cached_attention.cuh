@@ -299,8 +299,8 @@ __device__ __forceinline__ void join_row(const CachedParams<T>& p, const int32_t
 }
 
 // One launch after both kernels, a CTA for kJoinRows rows of a CTA's note: y below long_rows / kJoinRows is of the kernel of many rows, y
-// behind that of the other. Most have nothing to do; CTAs that look through all notes and share the rows that there are take 395 us for
-// chunks of 512 tokens on four sequences of 8192, these 386.
+// behind that of the other. Most have nothing to do; CTAs that look through all notes and share the rows that there are took 395 us for
+// chunks of 512 tokens on four sequences of 8192 when these took 386.
 constexpr int kJoinRows = 8;
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kJoinRows) join_kernel(const __grid_constant__ CachedParams<T> p, int32_t few_rows, const int32_t* long_pieces,
