@@ -748,7 +748,7 @@ enum {
  * multiple of 16 up to head_dim. Keys are rotated by their position before they are stored: pair i of the first rotary_dim
  * elements (i and i + rotary_dim / 2; interleaved: 2 i and 2 i + 1) becomes (a cos - b sin, b cos + a sin), products and sums
  * rounded to fp32 one by one. rope NULL: no rotation. q (may be NULL): [tokens, q_heads, head_dim], rotated by the same
- * positions into q_out (may be q itself with the same strides).
+ * positions into q_out (q itself with the same strides, or memory that overlaps with no input).
  *
  * The scale of a block is max |x| * (1 / 127) over the tokens that it holds (in fp32, 1 / 127 as well). When a call adds tokens to a block that has some and the
  * scale grows, the earlier codes are rewritten, c -> round(c * (old / new)); codes of new tokens are round(x * (1 / scale)), to
@@ -777,7 +777,13 @@ int mhlo_cuda_kv_cache_read(int32_t dtype, const mhlo_cuda_kv_cache* cache, cons
  * 128 or 256 contiguous; q_heads a multiple of the cache's heads: query head i reads head i / (q_heads / heads).
  * o = softmax(scale * q . k) v with fp32 statistics, 0 < scale <= 1e38, tokens * q_heads < 2^31; lse (NULL, or [tokens, q_heads] floats) receives the logarithm of the sum of
  * exponentials. A token that sees nothing (its sequence is unused or was passed over) gets zeros and lse -infinity; where the
- * starts are out of order, rows may be left alone. o may be q itself.
+ * starts are out of order, rows may be left alone. o may be q itself, or does not overlap with it.
+ * Rounded to fewer than 32 bits: with 16-bit types the weights, to 11 bits (fp16); with F32 queries and weights, to 22. A key is lost
+ * whose weight times value scale is below 2^-31 (F32: 2^-39) of the row's largest, or whose probability is below 2^-126. What a token
+ * does not see has no part in that. |scale * q . k| has to stay below 1e37.
+ * Without token_starts every sequence has one row and one kernel is launched. With them a call of F16 or BF16 at head_dim 64 or 128 and more
+ * than 48 rows (tokens times query heads of a cache head) launches a second one for sequences with that many, which costs 7 us where there
+ * are none.
  * scratch: cached_attention_scratch_bytes() bytes of device memory, 16-byte aligned, that nothing else uses until the call's
  * work is done; its contents do not matter.
  */
@@ -807,7 +813,8 @@ int mhlo_cuda_token_logprobs(int32_t dtype, const void* x_dev, int64_t row_strid
  * NULL = 0), ids as they were given and returned, and lse and entropy as computed (entropy may be NULL when e is),
  *   dx[i] = scale * ( g [i = target] + sum_k t_k [i = id_k] - p_i (g + sum_k t_k) - e p_i (log p_i + entropy) ).
  * Negative ids have no part in it, ids beyond the vocabulary make their row NaN. dx: like x, rows dx_row_stride elements apart; it
- * may be x itself (with the same stride).
+ * may be x itself (with the same stride), or does not overlap with it. p = exp(z - lse) with lse as it is given: of logits far from zero
+ * it is as exact as that fp32 number, |lse| 2^-24.
  */
 int mhlo_cuda_token_logprobs_grad(int32_t dtype, const void* x_dev, int64_t row_stride, int64_t rows, int64_t vocab, float scale,
                                   const void* targets_dev, int32_t target_dtype, const float* lse_dev, const float* entropy_dev,

@@ -12,8 +12,8 @@
 // nothing of its weight, costs it no digits, however large the block's values are.
 //
 // What bounds it: the codes have to come from memory once, 64 sequences of 8192 keys with 8 heads of 128 (4 query heads each, bf16)
-// 175 us for 1.07 GB, 6.1 TB/s. With fewer or ragged sequences the ends of segments show: 32 of up to 4096 keys 48 us for 179 MB, of
-// which reading alone would take 28. ncu, 32 of 8192 keys: 47 % of issue slots, 21 % of the tensor pipe, 168 registers.
+// 175 us in a graph for 1.07 GB, 6.1 TB/s. With fewer or ragged sequences the ends of segments show: 32 of up to 4096 keys 48 us for 179 MB,
+// of which reading alone would take 28. ncu, 32 of 8192 keys: 44 % of issue slots, 20 % of the tensor pipe, 168 registers.
 #include <algorithm>
 #include <type_traits>
 

@@ -14,7 +14,7 @@
 //
 // A half has two sets of scores (64 columns of tensor memory, O another head_dim): while the softmax works on step t the scores of
 // t + 1 are there already, and those of t + 2 go out behind P.V of t, whose weights lie in the same columns. With one set of 128
-// columns the softmax stood and waited for a third of the time; now it is what bounds a block, 1.1 us a step of either half.
+// columns the softmax stood and waited for a third of the time; now it is what bounds a block, about 1 us a step of either half.
 //
 // Per block and CTA the tensor pipe needs about 2050 clocks (4096 multiply-adds a clock), the exponentials as many (16 a clock), and
 // the producers some 2000 warp instructions beside the 6000 of the softmax, out of 4 a clock: three limits close together. Decoding

@@ -20,8 +20,9 @@ namespace {
 // fixed number apart, and all of them in registers at once (kKeep): no division and no second read.
 //
 // What bounds it: 16-bit elements come in two bytes each and take about seven instructions, rotation and quantisation two elements at
-// a time, and a CTA that owns a block waits for its rows once before the scale and once for the codes of before. Chunks of 4400 tokens in
-// all, 32 + 8 + 8 heads of 128, bf16: 31 us for 127 MB; one token of 64 sequences 4.2 us, which is a launch and three dependent reads.
+// a time, and a CTA that owns a block waits for its rows once before the scale and once for the codes of before. Five prompts of 6369
+// tokens in all, 32 + 8 + 8 heads of 128, bf16: 30.5 us in a graph for 143 MB; one token of 64 sequences 4.0 us, which is a launch and three
+// dependent reads.
 template <typename T>
 struct AppendParams {
     KvArgs kv;
@@ -187,7 +188,7 @@ __device__ __forceinline__ uint32_t codes_of(float2 x, float2 y, float step, flo
 }
 
 // A thread keeps the elements of its units as they are and rotates them twice, for the maximum and for the codes: with 16-bit types that
-// leaves registers for three CTAs of 256 threads (80 each; chunks of 4400 tokens, 32 + 8 + 8 heads of 128: 37 us with the rotated numbers kept,
+// leaves registers for three CTAs of 256 threads (80 each; prompts of 6369 tokens, 32 + 8 + 8 heads of 128: 37 us with the rotated numbers kept,
 // 122 registers; 33 as they are with 122; 31 with 80). fp32 elements are 64 registers by themselves: 80 in all spilled 1 KB a thread,
 // and two CTAs of 122 take 36.4 us for five chunks of 880 tokens instead of 42.6, 13.7 instead of 23.7 without queries. The largest pages
 // of the widest heads have 512 threads to a CTA.

@@ -7,8 +7,8 @@
 // One pass. A thread has 4 vectors of 16 bytes in flight and keeps a running maximum with its S and T; when a batch of its vectors
 // holds a larger logit, S and T move to it (T' = f (T + S delta), S' = f S with f = 2^delta). Everything is joined at the end of the
 // row. Per element that is about five instructions and one exponential (16 a clock and SM), against 11 16-bit elements a clock and
-// SM that the memory delivers. [4096, 50257] bf16: 77 us, 5.3 TB/s; ncu counts 70 % of issue slots and 67 % of the exponential unit.
-// Gradient (read, exponential, write): 132 us, 6.2 TB/s.
+// SM that the memory delivers. [4096, 50257] bf16: 77 us in a graph, 5.3 TB/s, 80 in calls one behind the other; ncu counts 70 % of issue
+// slots and 67 % of the exponential unit. Gradient (read, exponential, write): 132 us in a graph, 6.2 TB/s, 135 in calls.
 //
 // Alternatives come out of the same pass. Keys are 64 bits, the logit's order above the complement of its place, so no two are equal
 // and ties go to the lowest id. After the first batch a key that k threads' maxima reach bounds the k-th largest key from below; from
