@@ -867,8 +867,8 @@ int launch(const KvArgs& kv, const void* q, const int64_t* qs, int64_t q_heads, 
 }  // namespace
 
 int cached_attention_device_error() {
-    const int few = take_kv_error();
-    return few != 0 ? few : cached_attention_long_device_error();  // one word a call: the other is left for the next
+    const int few = take_kv_error(), many = cached_attention_long_device_error();  // one call's: reported, and cleared, as one
+    return few < 0 || many < 0 ? -1 : few != 0 ? few : many;
 }
 
 }  // namespace mhlo
