@@ -649,7 +649,7 @@ int mhlo_cuda_peer_barrier(void* const* flag_devs, int32_t n_ranks, int32_t rank
  * Every wait inside the tensor-core kernels (mbarrier phases fed by TMA and tcgen05.commit) is bounded; a kernel
  * whose wait expires records a non-zero word and drains instead of spinning; the key/value cache kernels record what they
  * found wrong with their page tables, lengths and starts. This call synchronises the device and reads the words in turn
- * (GEMM, attention: 100 + code, cache and attention over it: 200 + code). *out_code = 0 and MHLO_CUDA_OK: none is set. Else the
+ * (GEMM, attention: 100 + code, cache, attention over it and over packed sequences: 200 + code). *out_code = 0 and MHLO_CUDA_OK: none is set. Else the
  * first one is cleared, *out_code has its code and MHLO_CUDA_EXECUTION_FAILED is returned with the text in
  * mhlo_cuda_last_error(); words behind it are left for the next call.
  */
@@ -736,7 +736,8 @@ enum {
     MHLO_CUDA_KV_ERROR_PAGE = 1,     /* a page table entry outside [0, pages) */
     MHLO_CUDA_KV_ERROR_LENGTH = 2,   /* a length below 0, beyond the table, or below the sequence's rows in the call */
     MHLO_CUDA_KV_ERROR_STARTS = 3,   /* token_starts not ascending inside [0, tokens] */
-    MHLO_CUDA_KV_ERROR_POSITION = 4  /* a position behind the rotation table (its last row is taken) */
+    MHLO_CUDA_KV_ERROR_POSITION = 4, /* a position behind the rotation table (its last row is taken) */
+    MHLO_CUDA_KV_ERROR_PLAN = 5      /* a plan of packed sequences that is not of the batch (nothing is written) */
 };
 
 /*
@@ -791,6 +792,62 @@ int64_t mhlo_cuda_cached_attention_scratch_bytes(const mhlo_cuda_kv_cache* cache
 int mhlo_cuda_cached_attention(int32_t dtype, const void* q_dev, const int64_t q_strides[2], const mhlo_cuda_kv_cache* cache,
                                const mhlo_cuda_kv_batch* batch, int64_t q_heads, float scale, void* o_dev, const int64_t o_strides[2],
                                float* lse_dev, void* scratch_dev, int64_t scratch_bytes, mhlo_cuda_stream_t stream);
+
+/* ---- attention over packed sequences: whole prompts, forward and backward ---------------------------- */
+
+/*
+ * A batch of sequences that lie one behind the other in the rows of its tensors, in device memory:
+ *   starts    [seqs + 1] ascending: rows starts[b] .. starts[b + 1] - 1 are the tokens of sequence b (a sequence may have none)
+ *   plan      mhlo_cuda_packed_plan_bytes() bytes, 16-byte aligned: the sequences cut into tiles, longest first, as
+ *             mhlo_cuda_packed_plan leaves them. It depends on the starts and on what stands in this struct, and serves all layers
+ *             of a step, forward and backward, on any streams; starts is read by mhlo_cuda_packed_plan only
+ *   tokens    rows of the tensors; rows of no sequence are neither read into a result nor written
+ *   q_heads   a multiple of kv_heads: query head i reads head i / (q_heads / kv_heads)
+ *   causal    != 0: a token sees its sequence's tokens up to itself; 0: all of them
+ * tokens * q_heads < 2^31. Starts that are out of order (their sequence is passed over; where they go back on earlier ones rows may
+ * be left alone, or be written twice) and a plan that is not one of this batch (nothing is written) are reported by
+ * mhlo_cuda_device_error as 200 + one of MHLO_CUDA_KV_ERROR_*.
+ * No counterpart in the reference, whose attention is dense, of one length, and forward only
+ * (Sources/MetalHLOCore/Metal/Kernels/FlashAttentionKernel.swift:469-670).
+ */
+typedef struct {
+    const int32_t* starts;
+    void* plan;
+    int64_t seqs, tokens, q_heads, kv_heads;
+    int32_t causal;
+} mhlo_cuda_packed_batch;
+
+int64_t mhlo_cuda_packed_plan_bytes(const mhlo_cuda_packed_batch* batch);
+int mhlo_cuda_packed_plan(const mhlo_cuda_packed_batch* batch, mhlo_cuda_stream_t stream);
+
+/*
+ * o = softmax(scale * q . k) v over each token's own sequence. q, o: [tokens, q_heads, head_dim], k, v: [tokens, kv_heads, head_dim] of
+ * `dtype` (F16, BF16 or F32), *_strides = {token, head} in elements, head_dim (1 .. 128) contiguous; 0 < scale <= 1e38. lse (NULL, or
+ * [tokens, q_heads] floats) receives the logarithms of the sums of exponentials. o may be q itself with the same strides, or does not overlap with an input.
+ * Statistics and sums are fp32; 16-bit types round the weights to their own type. Tensors of 16 bits whose rows lie on the 16-byte grid, with
+ * head_dim a multiple of 8 and up to 128 query heads to a head of keys, run on the tensor cores, all others on the FMA units.
+ * |scale * q . k| has to stay below 1e37. An infinity or a NaN in a key or value may reach tokens of its own sequence that do not see it,
+ * but none of another.
+ */
+int mhlo_cuda_packed_attention(int32_t dtype, const mhlo_cuda_packed_batch* batch, int64_t head_dim, float scale, const void* q_dev,
+                               const int64_t q_strides[2], const void* k_dev, const int64_t k_strides[2], const void* v_dev,
+                               const int64_t v_strides[2], void* o_dev, const int64_t o_strides[2], float* lse_dev, mhlo_cuda_stream_t stream);
+
+/*
+ * Gradients of the above: grad = d/do, laid out like o; o and lse as the forward half left them;
+ *   p = exp(scale * q . k - lse), dv = p^T grad, ds = p (grad . v - grad . o), dq = scale * ds k, dk = scale * ds^T q,
+ * dk and dv summed over the query heads of a head of keys. dq, dk, dv are like q, k, v (any strides) and overlap with no input.
+ * Sums are fp32 in a fixed order: the same inputs give the same bits. 16-bit types round p and ds to their own type.
+ * scratch: packed_attention_grad_scratch_bytes() bytes of device memory, 16-byte aligned, that nothing else uses until the call's work is
+ * done; its contents do not matter.
+ */
+int64_t mhlo_cuda_packed_attention_grad_scratch_bytes(const mhlo_cuda_packed_batch* batch);
+int mhlo_cuda_packed_attention_grad(int32_t dtype, const mhlo_cuda_packed_batch* batch, int64_t head_dim, float scale, const void* q_dev,
+                                    const int64_t q_strides[2], const void* k_dev, const int64_t k_strides[2], const void* v_dev,
+                                    const int64_t v_strides[2], const void* o_dev, const int64_t o_strides[2], const float* lse_dev,
+                                    const void* grad_dev, const int64_t grad_strides[2], void* dq_dev, const int64_t dq_strides[2], void* dk_dev,
+                                    const int64_t dk_strides[2], void* dv_dev, const int64_t dv_strides[2], void* scratch_dev,
+                                    int64_t scratch_bytes, mhlo_cuda_stream_t stream);
 
 /* ---- log probabilities ------------------------------------------------------------------------------ */
 

@@ -1,0 +1,733 @@
+// Attention over packed sequences: entry points, the plan of a batch, and the kernels of what the tensor cores do not take (fp32, rows off the
+// 16-byte grid, head dimensions that are no multiple of 8), forward and backward, on the FMA units.
+#include <algorithm>
+#include <cmath>
+#include <initializer_list>
+
+#include "packed_attention.cuh"
+
+namespace mhlo {
+namespace {
+
+// ---- the plan ---------------------------------------------------------------------------------------------------------------------
+// One CTA: counts tiles by the 128-token blocks they meet, scans, and puts them in place, longest first. The order of tiles of one length
+// goes by arrival; no result depends on it. 32 sequences of 1024 tokens take 8 us, once for all layers of a step.
+constexpr int kBuckets = 2048, kPlanThreads = 1024;
+
+__device__ __forceinline__ int32_t bucket_of(int32_t tokens) { return kBuckets - 1 - min((tokens - 1) >> 7, kBuckets - 1); }
+
+__global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a) {
+    __shared__ int32_t counts[2][kBuckets];
+    __shared__ int32_t sums[2][32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i < 2 * kBuckets; i += kPlanThreads) counts[0][i] = 0;
+    __syncthreads();
+    const int32_t steps[2] = {2 * a.half_tokens, kKeyTile};
+    for (int place = 0; place < 2; ++place) {
+        for (int32_t b = warp; b < a.seqs; b += 32) {
+            const int32_t first = a.starts[b], end = a.starts[b + 1];
+            if (first < 0 || end > a.tokens || end < first) {
+                if (lane == 0) kv_report(MHLO_CUDA_KV_ERROR_STARTS);
+                continue;
+            }
+            const int32_t n = end - first;
+#pragma unroll
+            for (int list = 0; list < 2; ++list) {
+                for (int64_t z = static_cast<int64_t>(lane) * steps[list]; z < n; z += 32 * steps[list]) {
+                    const int32_t at = static_cast<int32_t>(z);
+                    const int32_t meets = !a.causal ? n : list == 0 ? static_cast<int32_t>(min(static_cast<int64_t>(n), z + steps[0])) : n - at;
+                    const int32_t slot = atomicAdd(&counts[list][bucket_of(meets)], 1);
+                    if (place == 0) continue;
+                    // starts that go back on earlier ones can make more tiles than there is room for
+                    if (slot < (list == 0 ? a.row_capacity : a.key_capacity)) const_cast<int4*>(list == 0 ? a.row_tiles() : a.key_tiles())[slot] = make_int4(first, n, at, 0);
+                }
+            }
+        }
+        __syncthreads();
+        if (place == 1) break;
+        // exclusive sums over the buckets
+        for (int list = 0; list < 2; ++list) {
+            const int32_t x = counts[list][2 * tid], y = counts[list][2 * tid + 1];
+            int32_t sum = x + y;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int32_t other = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += other;
+            }
+            if (lane == 31) sums[list][warp] = sum;
+            __syncthreads();
+            int32_t before = sum - x - y;
+            for (int w = 0; w < warp; ++w) before += sums[list][w];
+            counts[list][2 * tid] = before;
+            counts[list][2 * tid + 1] = before + x;
+            if (tid == kPlanThreads - 1) {
+                PlanHeader* const h = static_cast<PlanHeader*>(a.plan);
+                if (list == 0) h->row_tiles = min(before + x + y, a.row_capacity);
+                else h->key_tiles = min(before + x + y, a.key_capacity);
+            }
+        }
+        __syncthreads();
+    }
+    if (tid == 0) {
+        PlanHeader* const h = static_cast<PlanHeader*>(a.plan);
+        h->magic = kPlanMagic;
+        h->tokens = a.tokens;
+        h->q_heads = a.q_heads;
+        h->kv_heads = a.kv_heads;
+        h->causal = a.causal;
+        h->first = min(max(a.starts[0], 0), a.tokens);
+        h->end = min(max(a.starts[a.seqs], h->first), a.tokens);
+    }
+}
+
+// ---- the general kernels ------------------------------------------------------------------------------------------------------------
+// 128 threads on tiles of 64 x 64: thread (y, x) = (tid / 16, tid % 16) has 8 rows and, of every 64 columns, 4. All operands lie in shared memory in
+// fp32, rows of DP + 4 (64 + 4) floats: 16-byte loads of 16 neighbouring rows then meet all banks once. A step of four loads 12 vectors for
+// 128 multiply-adds a thread, 16 of the 32 clocks those take.
+constexpr int kGT = 128, kGRows = 64, kGKeys = 64;
+
+template <int DP>
+struct General {
+    static constexpr int kPitch = DP + 4, kTile = 64 * kPitch, kC = DP / 16;
+};
+constexpr int kWPitch = 64 + 4, kWTile = 64 * kWPitch;
+
+struct GeneralParams {
+    PackedArgs a;
+    PackedTensor q, k, v, o, grad, dq, dk, dv;
+    float* lse;
+    float2* stats;  // [kv_heads][tokens][group]: -lse log2(e), delta
+    uint32_t* norms;  // null, or where the largest squared norms of a row of grad and of a row of v go
+    float scale, scale_log2;
+    int32_t subs;   // tiles of this kernel to an entry of the plan
+};
+
+// acc[i][j] += sum over d of a[8 y + i][d] b[x + 16 j][d]
+template <int DP>
+__device__ __forceinline__ void dot_rows(const float* a, const float* b, int y, int x, float (&acc)[8][4]) {
+    constexpr int P = General<DP>::kPitch;
+    float2 s[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = make_float2(0.f, 0.f);
+#pragma unroll 2
+    for (int d = 0; d < DP; d += 4) {
+        float4 u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = *reinterpret_cast<const float4*>(b + (x + 16 * j) * P + d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 w = *reinterpret_cast<const float4*>(a + (8 * y + i) * P + d);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[i][j] = __ffma2_rn(make_float2(w.x, w.y), make_float2(u[j].x, u[j].y), s[i][j]);
+                s[i][j] = __ffma2_rn(make_float2(w.z, w.w), make_float2(u[j].z, u[j].w), s[i][j]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = s[i][j].x + s[i][j].y;
+}
+
+template <int DP>
+__device__ __forceinline__ void multiply_add(float (&acc)[8][DP / 16], const float (&w)[8], const float* row, int x) {
+#pragma unroll
+    for (int c = 0; c < DP / 16; c += 4) {
+        const float4 u = *reinterpret_cast<const float4*>(row + 4 * x + 16 * c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            acc[i][c] = fmaf(w[i], u.x, acc[i][c]);
+            acc[i][c + 1] = fmaf(w[i], u.y, acc[i][c + 1]);
+            acc[i][c + 2] = fmaf(w[i], u.z, acc[i][c + 2]);
+            acc[i][c + 3] = fmaf(w[i], u.w, acc[i][c + 3]);
+        }
+    }
+}
+
+// acc[i][.] += sum over k of w[8 y + i][k] b[k][.]
+template <int DP>
+__device__ __forceinline__ void add_rows(float (&acc)[8][DP / 16], const float* w, const float* b, int y, int x) {
+    constexpr int P = General<DP>::kPitch;
+#pragma unroll 1
+    for (int k = 0; k < 64; k += 4) {
+        float4 u[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = *reinterpret_cast<const float4*>(w + (8 * y + i) * kWPitch + k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float ww[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ww[i] = e == 0 ? u[i].x : e == 1 ? u[i].y : e == 2 ? u[i].z : u[i].w;
+            multiply_add<DP>(acc, ww, b + (k + e) * P, x);
+        }
+    }
+}
+
+// acc[i][.] += sum over k of w[k][8 y + i] b[k][.]
+template <int DP>
+__device__ __forceinline__ void add_columns(float (&acc)[8][DP / 16], const float* w, const float* b, int y, int x) {
+    constexpr int P = General<DP>::kPitch;
+#pragma unroll 2
+    for (int k = 0; k < 64; ++k) {
+        const float4 lo = *reinterpret_cast<const float4*>(w + k * kWPitch + 8 * y), hi = *reinterpret_cast<const float4*>(w + k * kWPitch + 8 * y + 4);
+        const float ww[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        multiply_add<DP>(acc, ww, b + k * P, x);
+    }
+}
+
+// 64 rows into shared memory; row(r): where row r starts, null: zeros (so are the elements behind head_dim).
+template <typename T, int DP, typename Row>
+__device__ __forceinline__ void stage(float* to, int32_t dim, bool vec, Row row) {
+    constexpr int P = General<DP>::kPitch, V = VecTraits<T>::kElems;
+    if (vec) {
+        for (int i = threadIdx.x; i < 64 * (DP / V); i += kGT) {
+            const int r = i / (DP / V), d = i % (DP / V) * V;
+            const T* const at = row(r);
+            float x[V];
+            if (at != nullptr && d < dim) {
+                VecTraits<T>::unpack(*reinterpret_cast<const uint4*>(at + d), x);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < V; e += 4) *reinterpret_cast<float4*>(to + r * P + d + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+        }
+        return;
+    }
+    for (int i = threadIdx.x; i < 64 * DP; i += kGT) {
+        const int r = i / DP, d = i % DP;
+        const T* const at = row(r);
+        to[r * P + d] = at != nullptr && d < dim ? VecTraits<T>::to_float(at[d]) : 0.f;
+    }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void store_row(T* to, int32_t dim, const float (&acc)[DP / 16], float factor, int x) {
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        const int d = 4 * x + 64 * (c / 4) + c % 4;
+        if (d < dim) to[d] = VecTraits<T>::from_float(acc[c] * factor);
+    }
+}
+
+// A run of 64 stacked rows: row r of it is token t0 + (r0 + r) / group.
+struct RowRun {
+    int32_t first, n, head, t0, r0, end;  // end: the entry's rows
+    __device__ __forceinline__ int32_t token(const PackedArgs& a, int32_t r) const { return t0 + (r0 + r) / a.group; }
+    __device__ __forceinline__ bool has(const PackedArgs& a, int32_t r) const { return r0 + r < end && token(a, r) < n; }
+    __device__ __forceinline__ int64_t q_head(const PackedArgs& a, int32_t r) const { return head * a.group + (r0 + r) % a.group; }
+    __device__ __forceinline__ int64_t stat(const PackedArgs& a, int32_t r) const {
+        return (static_cast<int64_t>(head) * a.tokens + first + token(a, r)) * a.group + (r0 + r) % a.group;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ T* row_at(const PackedTensor& t, int64_t token, int64_t head) {
+    return static_cast<T*>(t.base) + token * t.token + head * t.head;
+}
+
+// Item blockIdx.x of a list of `count` entries: (entry, sub, head), heads next to each other. False: none.
+__device__ __forceinline__ bool entry_of(const GeneralParams& p, const int4* list, int32_t count, int4* e, int32_t* sub, int32_t* head) {
+    const uint32_t i = blockIdx.x, at = i / static_cast<uint32_t>(p.a.kv_heads);
+    *head = i - at * p.a.kv_heads;
+    const uint32_t entry = at / static_cast<uint32_t>(p.subs);
+    *sub = at - entry * p.subs;
+    if (entry >= static_cast<uint32_t>(count)) return false;
+    *e = list[entry];
+    if (p.a.inside(*e)) return true;
+    if (threadIdx.x == 0) kv_report(MHLO_CUDA_KV_ERROR_PLAN);
+    return false;
+}
+
+__device__ __forceinline__ float reduce16(float x, bool most) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        const float y = __shfl_xor_sync(0xffffffffu, x, o);
+        x = most ? fmaxf(x, y) : x + y;
+    }
+    return x;
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kGT) packed_general_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
+    using G = General<DP>;
+    extern __shared__ __align__(16) float smem[];
+    float *const q = smem, *const k = q + G::kTile, *const v = k + G::kTile, *const w = v + G::kTile;
+    const PackedArgs& a = p.a;
+    const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
+    int4 e;
+    int32_t sub, head;
+    if (!a.matches(h) || !entry_of(p, a.row_tiles(), h.row_tiles, &e, &sub, &head)) return;
+    const RowRun run{e.x, e.y, head, e.z, sub * kGRows, 2 * a.half_tokens * a.group};
+    if (!run.has(a, 0)) return;
+    const int tid = threadIdx.x, y = tid >> 4, x = tid & 15;
+    stage<T, DP>(q, a.head_dim, vec, [&](int r) -> const T* { return run.has(a, r) ? row_at<const T>(p.q, run.first + run.token(a, r), run.q_head(a, r)) : nullptr; });
+    float acc[8][G::kC], most[8], total[8];
+    int32_t last[8], seen = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        most[i] = -INFINITY;
+        total[i] = 0.f;
+        last[i] = a.causal ? min(run.n - 1, run.token(a, 8 * y + i)) : run.n - 1;
+#pragma unroll
+        for (int c = 0; c < G::kC; ++c) acc[i][c] = 0.f;
+    }
+    seen = a.causal ? min(run.n, run.token(a, kGRows - 1) + 1) : run.n;
+    for (int32_t key0 = 0; key0 < seen; key0 += kGKeys) {
+        __syncthreads();
+        auto key_row = [&](const PackedTensor& t, int r) -> const T* { return key0 + r < run.n ? row_at<const T>(t, run.first + key0 + r, head) : nullptr; };
+        stage<T, DP>(k, a.head_dim, vec, [&](int r) { return key_row(p.k, r); });
+        stage<T, DP>(v, a.head_dim, vec, [&](int r) { return key_row(p.v, r); });
+        __syncthreads();
+        float s[8][4];
+        dot_rows<DP>(q, k, y, x, s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float m = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[i][j] = key0 + x + 16 * j <= last[i] ? s[i][j] * p.scale_log2 : -INFINITY;
+                m = fmaxf(m, s[i][j]);
+            }
+            m = fmaxf(most[i], reduce16(m, true));
+            const float shift = m == -INFINITY ? 0.f : m, keep = exp2f(most[i] - shift);
+            most[i] = m;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float weight = exp2f(s[i][j] - shift);
+                sum += weight;
+                w[(8 * y + i) * kWPitch + x + 16 * j] = weight;
+            }
+            total[i] = total[i] * keep + reduce16(sum, false);
+#pragma unroll
+            for (int c = 0; c < G::kC; ++c) acc[i][c] *= keep;
+        }
+        __syncwarp();  // rows 8 y .. 8 y + 7 are of this warp
+        add_rows<DP>(acc, w, v, y, x);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int32_t r = 8 * y + i;
+        if (!run.has(a, r)) continue;
+        const int64_t token = run.first + run.token(a, r), q_head = run.q_head(a, r);
+        store_row<T, DP>(row_at<T>(p.o, token, q_head), a.head_dim, acc[i], total[i] == 0.f ? 0.f : 1.f / total[i], x);
+        if (x == 0 && p.lse != nullptr) p.lse[token * a.q_heads + q_head] = total[i] == 0.f ? -INFINITY : (most[i] + log2f(total[i])) * 0.6931471805599453f;
+    }
+}
+
+// What the backward half needs of a row: -lse log2(e) and delta = grad . o, 16 lanes a row; bound by its bytes.
+constexpr int kStatsThreads = 256;
+template <typename T>
+__global__ void __launch_bounds__(kStatsThreads) packed_stats_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
+    const PackedArgs& a = p.a;
+    constexpr int V = VecTraits<T>::kElems;
+    const int lane = threadIdx.x & 15;
+    grid_dependency_wait();
+    grid_dependency_release();
+    const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
+    if (!a.matches(h) || h.end <= h.first) return;
+    const int64_t tokens = h.end - h.first, rows = tokens * a.q_heads;
+    const int64_t base = (static_cast<int64_t>(blockIdx.x) * kStatsThreads + threadIdx.x) >> 4;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (kStatsThreads / 16);
+    float largest = 0.f;  // squared norm; rows that are not finite have no say
+    auto norm = [&](float squares) {
+        squares = reduce16(squares, false);
+        if (squares <= 3.4028235e38f) largest = fmaxf(largest, squares);
+    };
+    auto squares_of = [&](const T* at) {
+        float squares = 0.f;
+        for (int d = lane; d < a.head_dim; d += 16) squares = fmaf(VecTraits<T>::to_float(at[d]), VecTraits<T>::to_float(at[d]), squares);
+        return squares;
+    };
+    auto leave = [&](uint32_t* to) {  // bits of numbers that are not negative have the numbers' order
+        const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
+        if ((threadIdx.x & 31) == 0 && most > 0) atomicMax(to, most);
+        largest = 0.f;
+    };
+    for (int64_t i = base; i - (base & 1) < rows; i += step) {  // both rows of a warp come along
+        const uint32_t row = static_cast<uint32_t>(min(i, rows - 1)) + static_cast<uint32_t>(h.first) * a.q_heads;
+        const uint32_t token = row / static_cast<uint32_t>(a.q_heads), head = row - token * a.q_heads;
+        const T *const o = row_at<const T>(p.o, token, head), *const g = row_at<const T>(p.grad, token, head);
+        float sum = 0.f;
+        if (vec) {
+            for (int d = lane * V; d < a.head_dim; d += 16 * V) {
+                float x[V], y[V];
+                VecTraits<T>::unpack(*reinterpret_cast<const uint4*>(o + d), x);
+                VecTraits<T>::unpack(*reinterpret_cast<const uint4*>(g + d), y);
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum = fmaf(x[e], y[e], sum);
+            }
+        } else {  // in the same order
+            for (int d = lane * V; d < a.head_dim; d += 16 * V)
+                for (int e = d; e < min(d + V, a.head_dim); ++e) sum = fmaf(VecTraits<T>::to_float(o[e]), VecTraits<T>::to_float(g[e]), sum);
+        }
+        sum = reduce16(sum, false);
+        if (p.norms != nullptr) norm(squares_of(g));
+        if (lane == 0 && i < rows) {
+            const uint32_t kv = head / static_cast<uint32_t>(a.group);
+            p.stats[(static_cast<int64_t>(kv) * a.tokens + token) * a.group + head - kv * a.group] = make_float2(-p.lse[row] * 1.4426950408889634f, sum);
+        }
+    }
+    if (p.norms == nullptr) return;
+    leave(p.norms);
+    const int64_t of_keys = tokens * a.kv_heads;
+    for (int64_t i = base; i - (base & 1) < of_keys; i += step) {
+        const uint32_t row = static_cast<uint32_t>(min(i, of_keys - 1)) + static_cast<uint32_t>(h.first) * a.kv_heads, token = row / static_cast<uint32_t>(a.kv_heads);
+        norm(squares_of(row_at<const T>(p.v, token, row - token * a.kv_heads)));
+    }
+    leave(p.norms + 1);
+}
+
+// P and scale dS of 64 rows x 64 keys, both rounded to nothing less than fp32. last(i): the last key that row 8 y + i sees, -1: none.
+template <int DP, typename Last, typename Stat>
+__device__ __forceinline__ void weights_and_grads(const float* q, const float* k, const float* g, const float* v, int y, int x, int32_t key0, const GeneralParams& p, Last last,
+                                                  Stat stat, float* w, float* dw) {
+    float s[8][4];
+    dot_rows<DP>(q, k, y, x, s);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float minus_lse = stat(i).x;
+        const int32_t end = last(i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = key0 + x + 16 * j <= end ? exp2f(fmaf(s[i][j], p.scale_log2, minus_lse)) : 0.f;
+    }
+    if (w != nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[(8 * y + i) * kWPitch + x + 16 * j] = s[i][j];
+    }
+    float t[8][4];
+    dot_rows<DP>(g, v, y, x, t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float delta = stat(i).y;
+        const int32_t end = last(i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dw[(8 * y + i) * kWPitch + x + 16 * j] = key0 + x + 16 * j <= end ? s[i][j] * (t[i][j] - delta) : 0.f;
+    }
+}
+
+// Gradients of keys and values: 64 keys, all rows that see them.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kGT) packed_general_key_grads_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
+    using G = General<DP>;
+    extern __shared__ __align__(16) float smem[];
+    __shared__ float2 stats[kGRows];
+    float *const k = smem, *const v = k + G::kTile, *const q = v + G::kTile, *const g = q + G::kTile, *const w = g + G::kTile, *const dw = w + kWTile;
+    const PackedArgs& a = p.a;
+    const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
+    int4 e;
+    int32_t sub, head;
+    if (!a.matches(h) || !entry_of(p, a.key_tiles(), h.key_tiles, &e, &sub, &head)) return;
+    const int32_t key0 = e.z + sub * kGKeys;
+    if (key0 >= e.y) return;
+    const int tid = threadIdx.x, y = tid >> 4, x = tid & 15;
+    auto key_row = [&](const PackedTensor& t, int r) -> const T* { return key0 + r < e.y ? row_at<const T>(t, e.x + key0 + r, head) : nullptr; };
+    stage<T, DP>(k, a.head_dim, vec, [&](int r) { return key_row(p.k, r); });
+    stage<T, DP>(v, a.head_dim, vec, [&](int r) { return key_row(p.v, r); });
+    float dk[8][G::kC], dv[8][G::kC];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < G::kC; ++c) dk[i][c] = dv[i][c] = 0.f;
+    const int32_t rows = e.y * a.group;
+    for (int32_t r0 = a.causal ? key0 * a.group : 0; r0 < rows; r0 += kGRows) {
+        const RowRun run{e.x, e.y, head, 0, r0, rows};
+        __syncthreads();
+        auto query_row = [&](const PackedTensor& t, int r) -> const T* { return run.has(a, r) ? row_at<const T>(t, run.first + run.token(a, r), run.q_head(a, r)) : nullptr; };
+        stage<T, DP>(q, a.head_dim, vec, [&](int r) { return query_row(p.q, r); });
+        stage<T, DP>(g, a.head_dim, vec, [&](int r) { return query_row(p.grad, r); });
+        if (tid < kGRows) stats[tid] = run.has(a, tid) ? p.stats[run.stat(a, tid)] : make_float2(0.f, 0.f);
+        __syncthreads();
+        weights_and_grads<DP>(q, k, g, v, y, x, key0, p,
+                              [&](int i) { return !run.has(a, 8 * y + i) ? -1 : a.causal ? min(run.token(a, 8 * y + i), e.y - 1) : e.y - 1; },
+                              [&](int i) { return stats[8 * y + i]; }, w, dw);
+        __syncthreads();
+        add_columns<DP>(dv, w, g, y, x);
+        add_columns<DP>(dk, dw, q, y, x);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int32_t key = key0 + 8 * y + i;
+        if (key >= e.y) continue;
+        store_row<T, DP>(row_at<T>(p.dk, e.x + key, head), a.head_dim, dk[i], p.scale, x);
+        store_row<T, DP>(row_at<T>(p.dv, e.x + key, head), a.head_dim, dv[i], 1.f, x);
+    }
+}
+
+// Gradients of queries: 64 rows, all keys that they see.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kGT) packed_general_query_grads_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
+    using G = General<DP>;
+    extern __shared__ __align__(16) float smem[];
+    __shared__ float2 stats[kGRows];
+    float *const q = smem, *const g = q + G::kTile, *const k = g + G::kTile, *const v = k + G::kTile, *const dw = v + G::kTile;
+    const PackedArgs& a = p.a;
+    const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
+    int4 e;
+    int32_t sub, head;
+    if (!a.matches(h) || !entry_of(p, a.row_tiles(), h.row_tiles, &e, &sub, &head)) return;
+    const RowRun run{e.x, e.y, head, e.z, sub * kGRows, 2 * a.half_tokens * a.group};
+    if (!run.has(a, 0)) return;
+    const int tid = threadIdx.x, y = tid >> 4, x = tid & 15;
+    auto query_row = [&](const PackedTensor& t, int r) -> const T* { return run.has(a, r) ? row_at<const T>(t, run.first + run.token(a, r), run.q_head(a, r)) : nullptr; };
+    stage<T, DP>(q, a.head_dim, vec, [&](int r) { return query_row(p.q, r); });
+    stage<T, DP>(g, a.head_dim, vec, [&](int r) { return query_row(p.grad, r); });
+    if (tid < kGRows) stats[tid] = run.has(a, tid) ? p.stats[run.stat(a, tid)] : make_float2(0.f, 0.f);
+    float dq[8][G::kC];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < G::kC; ++c) dq[i][c] = 0.f;
+    const int32_t seen = a.causal ? min(run.n, run.token(a, kGRows - 1) + 1) : run.n;
+    for (int32_t key0 = 0; key0 < seen; key0 += kGKeys) {
+        __syncthreads();
+        auto key_row = [&](const PackedTensor& t, int r) -> const T* { return key0 + r < run.n ? row_at<const T>(t, run.first + key0 + r, head) : nullptr; };
+        stage<T, DP>(k, a.head_dim, vec, [&](int r) { return key_row(p.k, r); });
+        stage<T, DP>(v, a.head_dim, vec, [&](int r) { return key_row(p.v, r); });
+        __syncthreads();
+        weights_and_grads<DP>(q, k, g, v, y, x, key0, p,
+                              [&](int i) { return !run.has(a, 8 * y + i) ? -1 : a.causal ? min(run.token(a, 8 * y + i), run.n - 1) : run.n - 1; },
+                              [&](int i) { return stats[8 * y + i]; }, static_cast<float*>(nullptr), dw);
+        __syncwarp();
+        add_rows<DP>(dq, dw, k, y, x);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int32_t r = 8 * y + i;
+        if (run.has(a, r)) store_row<T, DP>(row_at<T>(p.dq, run.first + run.token(a, r), run.q_head(a, r)), a.head_dim, dq[i], p.scale, x);
+    }
+}
+
+// ---- launches -------------------------------------------------------------------------------------------------------------------------
+
+template <typename T>
+bool vectors(const PackedTensor& t, int32_t dim) {
+    constexpr int V = VecTraits<T>::kElems;
+    return aligned16(t.base) && t.token % V == 0 && t.head % V == 0 && dim % V == 0;
+}
+
+GeneralParams general_params(const PackedCall& c) {
+    GeneralParams p;
+    p.a = c.a;
+    p.q = c.q, p.k = c.k, p.v = c.v, p.o = c.o, p.grad = c.grad, p.dq = c.dq, p.dk = c.dk, p.dv = c.dv;
+    p.lse = c.lse;
+    p.stats = c.scratch ? c.stats() : nullptr;
+    p.norms = nullptr;
+    p.scale = c.scale;
+    p.scale_log2 = c.scale * 1.4426950408889634f;
+    p.subs = 0;
+    return p;
+}
+
+template <typename K>
+int launch_general(const char* what, K kernel, GeneralParams p, int32_t subs, int64_t entries, int tiles, int weights, int dp, int32_t vec, std::atomic<bool> (&allowed)[64],
+                   cudaStream_t stream) {
+    const int bytes = (tiles * 64 * (dp + 4) + weights * kWTile) * 4;
+    if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), bytes, allowed)) return st;
+    p.subs = subs;
+    kernel<<<static_cast<unsigned>(entries * subs * p.a.kv_heads), kGT, bytes, stream>>>(p, vec);
+    MHLO_CUDA_CHECK_LAUNCH(what);
+    return MHLO_CUDA_OK;
+}
+
+int32_t row_subs(const PackedArgs& a) { return (2 * a.half_tokens * a.group + kGRows - 1) / kGRows; }
+
+template <typename T, int DP>
+int forward(const PackedCall& c, cudaStream_t stream) {
+    static std::atomic<bool> allowed[64];
+    const int32_t vec = vectors<T>(c.q, c.a.head_dim) && vectors<T>(c.k, c.a.head_dim) && vectors<T>(c.v, c.a.head_dim);
+    return launch_general("packed_attention", packed_general_kernel<T, DP>, general_params(c), row_subs(c.a), c.a.row_capacity, 3, 1, DP, vec, allowed, stream);
+}
+
+template <typename T, int DP>
+int backward(const PackedCall& c, cudaStream_t stream) {
+    static std::atomic<bool> allowed_keys[64], allowed_queries[64];
+    const int32_t vec = vectors<T>(c.q, c.a.head_dim) && vectors<T>(c.k, c.a.head_dim) && vectors<T>(c.v, c.a.head_dim) && vectors<T>(c.grad, c.a.head_dim);
+    if (int st = launch_general("packed_attention_grad", packed_general_key_grads_kernel<T, DP>, general_params(c), kKeyTile / kGKeys, c.a.key_capacity, 4, 2, DP, vec, allowed_keys, stream))
+        return st;
+    return launch_general("packed_attention_grad", packed_general_query_grads_kernel<T, DP>, general_params(c), row_subs(c.a), c.a.row_capacity, 4, 1, DP, vec, allowed_queries, stream);
+}
+
+template <typename T>
+int stats(const PackedCall& c, bool norms, cudaStream_t stream) {
+    const int32_t vec = vectors<T>(c.o, c.a.head_dim) && vectors<T>(c.grad, c.a.head_dim);
+    const int64_t rows = static_cast<int64_t>(c.a.tokens) * c.a.q_heads;
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((rows + 15) / 16, 8 * kNumSMs));
+    GeneralParams p = general_params(c);
+    if (norms) {
+        p.norms = c.norms();
+        MHLO_CUDA_TRY(cudaMemsetAsync(p.norms, 0, 2 * sizeof(uint32_t), stream), MHLO_CUDA_EXECUTION_FAILED);
+    }
+    const cudaError_t e = launch_dependent(packed_stats_kernel<T>, dim3(grid), dim3(kStatsThreads), 0, stream, 1, grid < kNumSMs, p, vec);
+    if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of packed_attention_grad failed: %s", cudaGetErrorString(e));
+    MHLO_CUDA_CHECK_LAUNCH("packed_attention_grad");
+    return MHLO_CUDA_OK;
+}
+
+template <typename F>
+int by_type(const PackedCall& c, F f) {
+    switch (c.dtype) {
+        case MHLO_DT_F32: return f(float{});
+        case MHLO_DT_F16: return f(__half{});
+        default: return f(__nv_bfloat16{});
+    }
+}
+
+// What the host can see of a batch.
+int packed_args(const char* what, const mhlo_cuda_packed_batch* b, PackedArgs* out) {
+    if (!b) return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: null batch", what);
+    if (b->seqs < 0 || b->seqs > (1 << 24) || b->tokens < 0 || b->tokens > (1 << 30))
+        return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: %lld sequences, %lld tokens", what, static_cast<long long>(b->seqs), static_cast<long long>(b->tokens));
+    if (b->kv_heads < 1 || b->kv_heads > 65535 || b->q_heads < 1 || b->q_heads > 65535 || b->q_heads % b->kv_heads != 0)
+        return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: %lld query heads on %lld heads of keys", what, static_cast<long long>(b->q_heads), static_cast<long long>(b->kv_heads));
+    if (b->tokens * b->q_heads >= (int64_t{1} << 31))
+        return fail(MHLO_CUDA_UNSUPPORTED, "%s: %lld tokens of %lld heads (fewer than 2^31 rows)", what, static_cast<long long>(b->tokens), static_cast<long long>(b->q_heads));
+    out->starts = b->starts;
+    out->plan = b->plan;
+    out->seqs = static_cast<int32_t>(b->seqs);
+    out->tokens = static_cast<int32_t>(b->tokens);
+    out->q_heads = static_cast<int32_t>(b->q_heads);
+    out->kv_heads = static_cast<int32_t>(b->kv_heads);
+    out->group = out->q_heads / out->kv_heads;
+    out->head_dim = 0;
+    out->causal = b->causal != 0;
+    out->half_tokens = std::max(1, kRows / out->group);
+    const int64_t most = std::min(b->seqs, b->tokens);  // sequences that have tokens
+    out->row_capacity = static_cast<int32_t>(b->tokens / (2 * out->half_tokens) + most);
+    out->key_capacity = static_cast<int32_t>(b->tokens / kKeyTile + most);
+    // items of the general kernels, the finest
+    const int64_t finest = std::max<int64_t>(static_cast<int64_t>(out->row_capacity) * std::max(2, row_subs(*out)), 2 * static_cast<int64_t>(out->key_capacity)) * out->kv_heads;
+    if (finest > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "%s: too many tiles", what);
+    return MHLO_CUDA_OK;
+}
+
+int64_t plan_bytes(const PackedArgs& a) { return static_cast<int64_t>(sizeof(PlanHeader)) + 16 * (static_cast<int64_t>(a.row_capacity) + a.key_capacity); }
+
+int tensor(const char* what, const char* name, const void* base, const int64_t* strides, PackedTensor* out) {
+    if (!base) return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: null %s", what, name);
+    if (int st = kv_row_strides(what, name, strides)) return st;
+    out->base = const_cast<void*>(base);
+    out->token = strides[0];
+    out->head = strides[1];
+    return MHLO_CUDA_OK;
+}
+// Results: no two rows in one place.
+int result(const char* what, const char* name, const void* base, const int64_t* strides, int64_t tokens, int64_t heads, int64_t dim, PackedTensor* out) {
+    if (int st = tensor(what, name, base, strides, out)) return st;
+    const bool apart = (tokens <= 1 || out->token >= dim) && (heads <= 1 || out->head >= dim) &&
+                       (tokens <= 1 || heads <= 1 || out->token >= (heads - 1) * out->head + dim || out->head >= (tokens - 1) * out->token + dim);
+    return apart ? MHLO_CUDA_OK : fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: rows of %s overlap", what, name);
+}
+
+int call_args(const char* what, int32_t dtype, const mhlo_cuda_packed_batch* batch, int64_t head_dim, float scale, PackedCall* c) {
+    if (dtype != MHLO_DT_F16 && dtype != MHLO_DT_BF16 && dtype != MHLO_DT_F32) return fail(MHLO_CUDA_UNSUPPORTED, "%s: dtype %d", what, dtype);
+    if (int st = packed_args(what, batch, &c->a)) return st;
+    if (head_dim < 1 || head_dim > 128) return fail(MHLO_CUDA_UNSUPPORTED, "%s: head dimension %lld (1 .. 128)", what, static_cast<long long>(head_dim));
+    if (!(scale > 0.f) || scale > 1e38f) return fail(MHLO_CUDA_UNSUPPORTED, "%s: scale %g", what, scale);
+    c->a.head_dim = static_cast<int32_t>(head_dim);
+    c->dtype = dtype;
+    c->scale = scale;
+    if (c->a.seqs > 0 && c->a.tokens > 0 && (!c->a.plan || !aligned16(c->a.plan))) return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: null or unaligned plan", what);
+    return MHLO_CUDA_OK;
+}
+
+bool on_tensor_cores(const PackedCall& c, std::initializer_list<const PackedTensor*> of_queries, std::initializer_list<const PackedTensor*> of_keys) {
+    if (c.dtype == MHLO_DT_F32 || c.a.head_dim % 8 != 0 || c.a.group > kRows) return false;
+    for (const PackedTensor* t : of_queries)
+        if (!packed_on_grid(*t, c.a.tokens, c.a.q_heads)) return false;
+    for (const PackedTensor* t : of_keys)
+        if (!packed_on_grid(*t, c.a.tokens, c.a.kv_heads)) return false;
+    return true;
+}
+
+}  // namespace
+
+int packed_attention_device_error() {
+    const int plan = take_kv_error(), forward = packed_attention_tc_device_error(), backward = packed_attention_grad_tc_device_error();
+    if (plan < 0 || forward < 0 || backward < 0) return -1;
+    return plan != 0 ? plan : forward != 0 ? forward : backward;
+}
+
+}  // namespace mhlo
+
+using namespace mhlo;
+
+extern "C" {
+
+int64_t mhlo_cuda_packed_plan_bytes(const mhlo_cuda_packed_batch* batch) {
+    PackedArgs a;
+    return packed_args("packed_plan", batch, &a) == MHLO_CUDA_OK ? plan_bytes(a) : 0;
+}
+
+int mhlo_cuda_packed_plan(const mhlo_cuda_packed_batch* batch, mhlo_cuda_stream_t stream) {
+    PackedArgs a;
+    if (int st = packed_args("packed_plan", batch, &a)) return st;
+    if (a.seqs == 0 || a.tokens == 0) return MHLO_CUDA_OK;
+    if (!a.starts || !a.plan || !aligned16(a.plan)) return fail(MHLO_CUDA_INVALID_ARGUMENT, "packed_plan: null starts, or null or unaligned plan");
+    packed_plan_kernel<<<1, kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    MHLO_CUDA_CHECK_LAUNCH("packed_plan");
+    return MHLO_CUDA_OK;
+}
+
+int mhlo_cuda_packed_attention(int32_t dtype, const mhlo_cuda_packed_batch* batch, int64_t head_dim, float scale, const void* q_dev, const int64_t q_strides[2],
+                               const void* k_dev, const int64_t k_strides[2], const void* v_dev, const int64_t v_strides[2], void* o_dev, const int64_t o_strides[2],
+                               float* lse_dev, mhlo_cuda_stream_t stream) {
+    static const char* const what = "packed_attention";
+    PackedCall c;
+    if (int st = call_args(what, dtype, batch, head_dim, scale, &c)) return st;
+    if (c.a.seqs == 0 || c.a.tokens == 0) return MHLO_CUDA_OK;
+    if (int st = tensor(what, "q", q_dev, q_strides, &c.q)) return st;
+    if (int st = tensor(what, "k", k_dev, k_strides, &c.k)) return st;
+    if (int st = tensor(what, "v", v_dev, v_strides, &c.v)) return st;
+    if (int st = result(what, "o", o_dev, o_strides, c.a.tokens, c.a.q_heads, head_dim, &c.o)) return st;
+    c.lse = lse_dev;
+    c.scratch = nullptr;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (on_tensor_cores(c, {&c.q, &c.o}, {&c.k, &c.v})) return packed_attention_tc(c, s);
+    return by_type(c, [&](auto t) { return c.a.head_dim <= 64 ? forward<decltype(t), 64>(c, s) : forward<decltype(t), 128>(c, s); });
+}
+
+int64_t mhlo_cuda_packed_attention_grad_scratch_bytes(const mhlo_cuda_packed_batch* batch) {
+    PackedArgs a;
+    if (packed_args("packed_attention_grad", batch, &a) != MHLO_CUDA_OK) return 0;
+    return static_cast<int64_t>(a.tokens) * a.q_heads * static_cast<int64_t>(sizeof(float2)) + 16;
+}
+
+int mhlo_cuda_packed_attention_grad(int32_t dtype, const mhlo_cuda_packed_batch* batch, int64_t head_dim, float scale, const void* q_dev, const int64_t q_strides[2],
+                                    const void* k_dev, const int64_t k_strides[2], const void* v_dev, const int64_t v_strides[2], const void* o_dev,
+                                    const int64_t o_strides[2], const float* lse_dev, const void* grad_dev, const int64_t grad_strides[2], void* dq_dev,
+                                    const int64_t dq_strides[2], void* dk_dev, const int64_t dk_strides[2], void* dv_dev, const int64_t dv_strides[2], void* scratch_dev,
+                                    int64_t scratch_bytes, mhlo_cuda_stream_t stream) {
+    static const char* const what = "packed_attention_grad";
+    PackedCall c;
+    if (int st = call_args(what, dtype, batch, head_dim, scale, &c)) return st;
+    if (c.a.seqs == 0 || c.a.tokens == 0) return MHLO_CUDA_OK;
+    if (int st = tensor(what, "q", q_dev, q_strides, &c.q)) return st;
+    if (int st = tensor(what, "k", k_dev, k_strides, &c.k)) return st;
+    if (int st = tensor(what, "v", v_dev, v_strides, &c.v)) return st;
+    if (int st = tensor(what, "o", o_dev, o_strides, &c.o)) return st;
+    if (int st = tensor(what, "grad", grad_dev, grad_strides, &c.grad)) return st;
+    if (int st = result(what, "dq", dq_dev, dq_strides, c.a.tokens, c.a.q_heads, head_dim, &c.dq)) return st;
+    if (int st = result(what, "dk", dk_dev, dk_strides, c.a.tokens, c.a.kv_heads, head_dim, &c.dk)) return st;
+    if (int st = result(what, "dv", dv_dev, dv_strides, c.a.tokens, c.a.kv_heads, head_dim, &c.dv)) return st;
+    if (!lse_dev) return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: null lse", what);
+    const int64_t need = mhlo_cuda_packed_attention_grad_scratch_bytes(batch);
+    if (!scratch_dev || !aligned16(scratch_dev) || scratch_bytes < need)
+        return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: %lld bytes of scratch, %lld needed, on 16 bytes", what, static_cast<long long>(scratch_bytes), static_cast<long long>(need));
+    c.lse = const_cast<float*>(lse_dev);
+    c.scratch = scratch_dev;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool tensor_cores = on_tensor_cores(c, {&c.q, &c.grad, &c.dq}, {&c.k, &c.v, &c.dk, &c.dv});
+    if (int st = by_type(c, [&](auto t) { return stats<decltype(t)>(c, tensor_cores && dtype == MHLO_DT_F16, s); })) return st;
+    if (tensor_cores) return packed_attention_grad_tc(c, s);
+    return by_type(c, [&](auto t) { return c.a.head_dim <= 64 ? backward<decltype(t), 64>(c, s) : backward<decltype(t), 128>(c, s); });
+}
+
+}  // extern "C"

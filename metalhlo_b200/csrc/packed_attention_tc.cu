@@ -1,0 +1,483 @@
+// Attention over packed sequences on tcgen05: o = softmax(scale q k^T) v for bf16 / f16, head dimensions up to 128, grouped heads,
+// causal or not, with the logarithms of the sums of exponentials. Scores do not leave the SM.
+//
+// A CTA takes items (tile of stacked query rows, head of keys) from the batch's plan, longest first. A tile is two halves of 128 rows:
+//   warp 0             producer: rows of q, then blocks of 128 keys and values through rings of two stages
+//   warp 1             MMA issuer: S_h = Q_h K^T (both in shared memory), O_h += P_h V (P in tensor memory); one half's products run
+//                      under the other's exponentials
+//   warps 2-5, 6-9     softmax of half 0 / 1, a thread per row
+// The maximum in the exponent moves only when scores exceed it by 2^8; O is rescaled in tensor memory only then.
+#include <algorithm>
+
+#include "packed_tc.cuh"
+
+namespace mhlo {
+namespace {
+
+constexpr int kStages = 2, kThreads = 32 * (2 + 4 * kHalves);
+constexpr float kGrowth = 8.f;
+constexpr float kCarry = 32768.f;  // a row's sum of a block below this bounds every weight below the largest f16
+constexpr int kWaitError = 60;     // + where a bounded wait ran out
+
+struct ForwardParams {
+    PackedArgs a;
+    void* o;
+    float* lse;
+    int64_t os_token, os_head;
+    float scale_log2;
+    int32_t k_steps;    // head_dim / 16, rounded up
+    int32_t one_half;   // items are half tiles: few rows, more CTAs
+};
+
+template <int D>
+struct ForwardSmem {
+    static constexpr int kTile = 128 * D * 2;
+    static constexpr int kQ = 0, kK = kQ + kHalves * kTile, kV = kK + kStages * kTile, kEnd = kV + kStages * kTile, kTotal = kEnd + 1024;
+};
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t scale16x2(uint32_t v, float a) {
+    if constexpr (BF16) {
+        const __nv_bfloat162 h = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), __float2bfloat162_rn(a));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&v), __float2half2_rn(a));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+// Weights of 64 scores, packed, and their sum: 2^(s * scale_log2 - m). MASK: scores of keys behind last become -infinity.
+template <bool BF16, bool MASK>
+__device__ __forceinline__ void weights(uint32_t* sr, float scale_log2, float m, int32_t key0, int32_t last, uint32_t* packed, float2* sums) {
+    const float2 c2 = make_float2(scale_log2, scale_log2), m2 = make_float2(-m, -m);
+    if (MASK) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+            if (key0 + c > last) sr[c] = 0xff800000u;
+    }
+#pragma unroll
+    for (int c = 0; c < 64; c += 2) {
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), c2, m2);
+        const float2 e = make_float2(ex2(x.x), ex2(x.y));
+        sums[(c >> 1) & 1] = __fadd2_rn(sums[(c >> 1) & 1], e);
+        packed[c / 2] = pack16<BF16>(e.x, e.y);
+    }
+}
+
+__device__ __forceinline__ float largest(const uint32_t* sr) {
+    float a = -INFINITY, b = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 64; c += 4) {
+        a = fmax3(a, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+        b = fmax3(b, __uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3]));
+    }
+    return fmaxf(a, b);
+}
+
+__device__ __forceinline__ void load64(uint32_t taddr, uint32_t* r) {
+    tmem_ld32(taddr, r);
+    tmem_ld32(taddr + 32, r + 32);
+    tmem_ld_wait();
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                                                                       const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ForwardParams p) {
+    using L = ForwardSmem<D>;
+    constexpr int kPanels = D / 64;
+    // Tensor memory: scores 2 x 128 columns, O 2 x D. At D = 64 there is room for the weights beside the scores, so the scores of a
+    // half's next block go out as soon as it has read those of this one; at 128 the weights lie over the scores.
+    constexpr bool kBeside = D == 64;
+    constexpr uint32_t kTmemCols = 512, kSCol = 0, kOCol = kHalves * 128, kPCol = kBeside ? kOCol + kHalves * D : kSCol, kPStride = kBeside ? 64 : 128;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    __shared__ uint64_t bars[7 * kHalves + 4 * kStages + 1];
+    __shared__ uint32_t tmem_slot;
+    uint64_t* const q_full = bars;                 // per half: the tile's rows of q are in shared memory
+    uint64_t* const q_empty = q_full + kHalves;    // per half: their last product is done
+    uint64_t* const s_full = q_empty + kHalves;    // per half: scores of a block are in tensor memory
+    uint64_t* const s_free = s_full + kHalves;     // per half (kBeside): they have been read
+    uint64_t* const p_full = s_free + kHalves;     // per half: the block's weights are, and O is rescaled if need be
+    uint64_t* const pv_done = p_full + kHalves;    // per half: the products with values so far have completed
+    uint64_t* const k_full = pv_done + kHalves;
+    uint64_t* const k_empty = k_full + kStages;
+    uint64_t* const v_full = k_empty + kStages;
+    uint64_t* const v_empty = v_full + kStages;
+    uint64_t* const own = v_empty + kStages;       // tiles that the producer waits for itself
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rows = p.a.half_tokens * p.a.group;  // of a half tile that hold a token
+    if (tid == 0) {
+        prefetch_tmap(&map_q);
+        prefetch_tmap(&map_k);
+        prefetch_tmap(&map_v);
+        for (int h = 0; h < kHalves; ++h) {
+            mbar_init(&q_full[h], 1);
+            mbar_init(&q_empty[h], 1);
+            mbar_init(&s_full[h], 1);
+            mbar_init(&s_free[h], 4);
+            mbar_init(&p_full[h], 4);
+            mbar_init(&pv_done[h], 1);
+        }
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&k_full[s], 1);
+            mbar_init(&k_empty[s], 1);
+            mbar_init(&v_full[s], 1);
+            mbar_init(&v_empty[s], 1);
+        }
+        mbar_init(own, 1);
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(&tmem_slot, kTmemCols);
+        tmem_relinquish();
+    }
+    // rows that no box brings hold numbers from the start
+    for (int i = rows * 8 + tid; i < 128 * 8; i += kThreads) {
+#pragma unroll
+        for (int pn = 0; pn < kHalves * kPanels; ++pn) *reinterpret_cast<uint4*>(smem + L::kQ + pn * kPanelBytes + i * 16) = make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    grid_dependency_wait();
+    grid_dependency_release();
+    RowWalk walk(p.a, p.one_half);
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+        if (ok && !mbar_wait(bar, parity)) {
+            kv_report(kWaitError + where);
+            ok = false;
+        }
+        return ok;
+    };
+
+    if (warp == 0) {
+        // ---- producer
+        RowTile t;
+        int stage = 0;
+        uint32_t phase = 0, own_phase = 0, q_of[kHalves] = {0, 0};
+        while (ok && walk.next(&t)) {
+            for (int h = 0; h < kHalves; ++h) {
+                if (t.nb[h] == 0) continue;
+                if (!wait(&q_empty[h], (q_of[h]++ & 1) ^ 1, 0)) break;
+                load_tile<kPanels>(smem + L::kQ + h * L::kTile, &map_q, &q_full[h], own, &own_phase, rows, rows, false, 0, t.head, t.first + t.t0 + h * p.a.half_tokens);
+            }
+            for (int j = 0; j < t.nblk && ok; ++j) {
+                if (!wait(&k_empty[stage], phase ^ 1, 1)) break;
+                load_tile<kPanels>(smem + L::kK + stage * L::kTile, &map_k, &k_full[stage], own, &own_phase, kKeyTile, kKeyTile, false, t.head, t.first + j * kKeyTile, 0);
+                if (!wait(&v_empty[stage], phase ^ 1, 2)) break;
+                if (!load_tile<kPanels>(smem + L::kV + stage * L::kTile, &map_v, &v_full[stage], own, &own_phase, kKeyTile, t.n - j * kKeyTile, true, t.head, t.first + j * kKeyTile, 0)) {
+                    kv_report(kWaitError + 3);
+                    ok = false;
+                }
+                if (++stage == kStages) stage = 0, phase ^= 1;
+            }
+        }
+    } else if (warp == 1) {
+        // ---- MMA issuer
+        const uint32_t idesc_s = instruction(BF16, false, kKeyTile), idesc_o = instruction(BF16, true, static_cast<uint32_t>(p.k_steps * 16));
+        const uint32_t q_addr = smem_u32(smem + L::kQ), k_addr = smem_u32(smem + L::kK), v_addr = smem_u32(smem + L::kV);
+        auto commit_to = [&](uint64_t* bar) {
+            if (elect_one()) umma_commit(bar);
+            __syncwarp();
+        };
+        auto issue_s = [&](int h, int stage) {
+            tc_fence_after();
+            const uint32_t qa = q_addr + h * L::kTile, ka = k_addr + stage * L::kTile;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                if (kk >= p.k_steps) break;
+                const uint64_t da = make_smem_desc(qa + (kk / 4) * kPanelBytes + (kk % 4) * 32, 16, 1024);
+                const uint64_t db = make_smem_desc(ka + (kk / 4) * kPanelBytes + (kk % 4) * 32, 16, 1024);
+                if (elect_one()) umma_f16(tmem + kSCol + h * 128, da, db, idesc_s, kk != 0 ? 1u : 0u);
+            }
+            commit_to(&s_full[h]);
+        };
+        auto issue_pv = [&](int h, int stage, bool more) {
+            tc_fence_after();
+            const uint32_t va = v_addr + stage * L::kTile;
+#pragma unroll
+            for (int kk = 0; kk < kKeyTile / 16; ++kk) {
+                const uint64_t db = make_smem_desc(va + kk * 16 * 128, kPanelBytes, 1024);
+                if (elect_one()) umma_ts(tmem + kOCol + h * D, tmem + kPCol + h * kPStride + kk * 8, db, idesc_o, more || kk != 0 ? 1u : 0u);
+            }
+            commit_to(&pv_done[h]);
+        };
+        RowTile cur, nxt;
+        bool has = walk.next(&cur);
+        uint32_t block = 0;                              // blocks of keys so far
+        uint32_t s_of[kHalves] = {0, 0}, p_of[kHalves] = {0, 0}, q_of[kHalves] = {0, 0};
+        // The scores of block j of tile t, half h (whose turn it is), with the waits for what they read.
+        auto scores = [&](const RowTile& t, int j, int h, uint32_t at) {
+            const int stage = at % kStages;
+            if (h == 0 && !wait(&k_full[stage], at / kStages & 1, 4)) return;
+            if (j < t.nb[h]) {
+                if (j == 0 && !wait(&q_full[h], q_of[h]++ & 1, 5)) return;
+                // one arrival on s_free for each block of scores: those before have been read
+                if (kBeside && s_of[h] > 0 && !wait(&s_free[h], (s_of[h] - 1) & 1, 6)) return;
+                ++s_of[h];
+                issue_s(h, stage);
+                if (j + 1 == t.nb[h]) commit_to(&q_empty[h]);
+            }
+            if (h == kHalves - 1) commit_to(&k_empty[stage]);
+        };
+        auto values = [&](const RowTile& t, int j, int h, uint32_t at) {
+            const int stage = at % kStages;
+            if (h == 0 && !wait(&v_full[stage], at / kStages & 1, 7)) return;
+            if (j < t.nb[h]) {
+                if (!wait(&p_full[h], p_of[h]++ & 1, 8)) return;
+                issue_pv(h, stage, j > 0);
+            }
+            if (h == kHalves - 1) commit_to(&v_empty[stage]);
+        };
+        if (has)
+            for (int h = 0; h < kHalves && ok; ++h) scores(cur, 0, h, block);
+        // Order on the pipe, which runs one thread's products in turn. Weights over the scores: PV_0(j), S_0(next), PV_1(j), S_1(next), so
+        // that scores replace weights that have been read. Beside them: S_0(next), S_1(next), PV_0(j), PV_1(j).
+        while (has && ok) {
+            const bool more_tiles = walk.next(&nxt);
+            for (int j = 0; j < cur.nblk && ok; ++j, ++block) {
+                const bool last = j + 1 == cur.nblk;
+                const RowTile& next = last ? nxt : cur;
+                const int nj = last ? 0 : j + 1;
+                const bool more = !last || more_tiles;
+                if (kBeside) {
+                    for (int h = 0; h < kHalves && ok && more; ++h) scores(next, nj, h, block + 1);
+                    for (int h = 0; h < kHalves && ok; ++h) values(cur, j, h, block);
+                } else {
+                    for (int h = 0; h < kHalves && ok; ++h) {
+                        values(cur, j, h, block);
+                        if (ok && more) scores(next, nj, h, block + 1);
+                    }
+                }
+            }
+            cur = nxt;
+            has = more_tiles;
+        }
+    } else {
+        // ---- softmax
+        const int h = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+        const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+        const uint32_t s_taddr = tmem + lane_base + kSCol + h * 128, o_taddr = tmem + lane_base + kOCol + h * D, p_taddr = tmem + lane_base + kPCol + h * kPStride;
+        const int32_t row_token = r / p.a.group, row_head = r - row_token * p.a.group;
+        RowTile t;
+        uint32_t it = 0;  // blocks of this half so far
+        while (ok && walk.next(&t)) {
+            const int32_t i = t.t0 + h * p.a.half_tokens + row_token;  // the row's token
+            const int32_t last = p.a.causal ? min(t.n - 1, i) : t.n - 1;
+            const int nb = t.nb[h];
+            float m_ref = -INFINITY, l = 0.f;
+            for (int j = 0; j < nb; ++j, ++it) {
+                if (!wait(&s_full[h], it & 1, 9)) break;
+                tc_fence_after();
+                const int32_t key0 = j * kKeyTile;
+                // one decision a warp: loads and stores of tensor memory are warp-wide
+                const bool mask = __any_sync(0xffffffffu, key0 + kKeyTile - 1 > last);
+                float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                if constexpr (kBeside) {
+                    bool pv_waited = it == 0;  // for the product of the block before this one, which reads its weights and adds to O
+#pragma unroll 1
+                    for (int ci = 0; ci < 2; ++ci) {
+                        uint32_t sr[64], packed[32];
+                        load64(s_taddr + ci * 64, sr);
+                        if (ci == 1) {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&s_free[h]);
+                        }
+                        if (mask) {
+#pragma unroll
+                            for (int c = 0; c < 64; ++c)
+                                if (key0 + ci * 64 + c > last) sr[c] = 0xff800000u;
+                        }
+                        const float mx = largest(sr) * p.scale_log2;
+                        const bool grow = mx > m_ref + kGrowth;
+                        if (__any_sync(0xffffffffu, grow)) {
+                            float alpha = 1.f;
+                            if (grow) {
+                                alpha = m_ref == -INFINITY ? 0.f : ex2(m_ref - mx);
+                                m_ref = mx;
+                                l *= alpha;
+                            }
+                            sums[0].x *= alpha, sums[0].y *= alpha, sums[1].x *= alpha, sums[1].y *= alpha;
+                            if (j > 0 || ci > 0) {
+                                if (!pv_waited) {
+                                    if (!wait(&pv_done[h], (it - 1) & 1, 10)) break;
+                                    tc_fence_after();
+                                    pv_waited = true;
+                                }
+                                // O of the blocks before, then the weights of this block's first half
+#pragma unroll 1
+                                for (int c0 = j > 0 ? 0 : D; c0 < D + (ci > 0 ? 32 : 0); c0 += 32) {
+                                    const uint32_t at = c0 < D ? o_taddr + c0 : p_taddr;
+                                    uint32_t x[32];
+                                    if (c0 >= D) tmem_st_wait();
+                                    tmem_ld32(at, x);
+                                    tmem_ld_wait();
+#pragma unroll
+                                    for (int c = 0; c < 32; ++c) x[c] = c0 < D ? __float_as_uint(__uint_as_float(x[c]) * alpha) : scale16x2<BF16>(x[c], alpha);
+                                    tmem_st32(at, x);
+                                }
+                            }
+                        }
+                        weights<BF16, false>(sr, p.scale_log2, m_ref == -INFINITY ? 0.f : m_ref, 0, 0, packed, sums);
+                        if (!pv_waited) {
+                            if (!wait(&pv_done[h], (it - 1) & 1, 11)) break;
+                            tc_fence_after();
+                            pv_waited = true;
+                        }
+                        tmem_st32(p_taddr + ci * 32, packed);
+                    }
+                    if (!ok) break;
+                    l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+                } else {
+                    // Against the maximum of earlier blocks first: nothing is written until the warp's sums have shown that no weight is
+                    // too large for 16 bits. Otherwise (first blocks, and where scores have grown) the block's own maximum is found.
+                    uint32_t packed[2][32];
+                    bool done = false;
+                    if (j > 0) {
+                        const float m = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll
+                        for (int ci = 0; ci < 2; ++ci) {
+                            uint32_t sr[64];
+                            load64(s_taddr + ci * 64, sr);
+                            if (mask) weights<BF16, true>(sr, p.scale_log2, m, key0 + ci * 64, last, packed[ci], sums);
+                            else weights<BF16, false>(sr, p.scale_log2, m, 0, 0, packed[ci], sums);
+                        }
+                        const float sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+                        done = !__any_sync(0xffffffffu, !(sum < kCarry));
+                        if (done) {
+                            l += sum;
+#pragma unroll
+                            for (int ci = 0; ci < 2; ++ci) tmem_st32(p_taddr + ci * 32, packed[ci]);
+                        }
+                    }
+                    if (!done) {
+                        float mx = -INFINITY;
+#pragma unroll 1
+                        for (int ci = 0; ci < 2; ++ci) {
+                            uint32_t sr[64];
+                            load64(s_taddr + ci * 64, sr);
+                            if (mask) {
+#pragma unroll
+                                for (int c = 0; c < 64; ++c)
+                                    if (key0 + ci * 64 + c > last) sr[c] = 0xff800000u;
+                            }
+                            mx = fmaxf(mx, largest(sr));
+                        }
+                        mx *= p.scale_log2;
+                        const bool grow = mx > m_ref + kGrowth;
+                        float alpha = 1.f;
+                        if (grow) {
+                            alpha = m_ref == -INFINITY ? 0.f : ex2(m_ref - mx);
+                            m_ref = mx;
+                            l *= alpha;
+                        }
+                        // the products so far completed before these scores did
+                        if (j > 0 && __any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
+                            for (int c0 = 0; c0 < D; c0 += 32) {
+                                uint32_t x[32];
+                                tmem_ld32(o_taddr + c0, x);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int c = 0; c < 32; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) * alpha);
+                                tmem_st32(o_taddr + c0, x);
+                            }
+                        }
+                        sums[0] = sums[1] = make_float2(0.f, 0.f);
+                        const float m = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll 1
+                        for (int ci = 0; ci < 2; ++ci) {  // the weights lie over scores that have been read
+                            uint32_t sr[64];
+                            load64(s_taddr + ci * 64, sr);
+                            weights<BF16, true>(sr, p.scale_log2, m, key0 + ci * 64, last, packed[0], sums);
+                            tmem_st32(p_taddr + ci * 32, packed[0]);
+                        }
+                        l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+                    }
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[h]);
+            }
+            if (!ok || nb == 0) continue;
+            // ---- results. The next tile's first product with values waits for weights that these warps write after this.
+            if (!wait(&pv_done[h], (it - 1) & 1, 12)) break;
+            tc_fence_after();
+            const bool mine = r < rows && i < t.n;
+            const int64_t token = t.first + i, head = t.head * p.a.group + row_head;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            uint8_t* const to = static_cast<uint8_t*>(p.o) + (token * p.os_token + head * p.os_head) * 2;
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 32) {
+                if (c0 >= p.a.head_dim) break;
+                uint32_t x[32];
+                tmem_ld32(o_taddr + c0, x);
+                tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 32; c += 8) {
+                    if (!mine || c0 + c >= p.a.head_dim) continue;
+                    uint4 w;
+                    w.x = pack16<BF16>(__uint_as_float(x[c]) * inv, __uint_as_float(x[c + 1]) * inv);
+                    w.y = pack16<BF16>(__uint_as_float(x[c + 2]) * inv, __uint_as_float(x[c + 3]) * inv);
+                    w.z = pack16<BF16>(__uint_as_float(x[c + 4]) * inv, __uint_as_float(x[c + 5]) * inv);
+                    w.w = pack16<BF16>(__uint_as_float(x[c + 6]) * inv, __uint_as_float(x[c + 7]) * inv);
+                    *reinterpret_cast<uint4*>(to + (c0 + c) * 2) = w;
+                }
+            }
+            if (mine && p.lse != nullptr) p.lse[token * p.a.q_heads + head] = l == 0.f ? -INFINITY : (m_ref + log2f(l)) * kLn2;
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+template <int D, bool BF16>
+int launch(const PackedCall& c, cudaStream_t stream) {
+    using L = ForwardSmem<D>;
+    const PackedArgs& a = c.a;
+    CUtensorMap mq, mk, mv;
+    if (int st = query_map(&mq, c.q, a)) return st;
+    if (int st = key_map(&mk, c.k, a)) return st;
+    if (int st = key_map(&mv, c.v, a)) return st;
+    ForwardParams p;
+    p.a = a;
+    p.o = c.o.base;
+    p.lse = c.lse;
+    p.os_token = c.o.token;
+    p.os_head = c.o.head;
+    p.scale_log2 = c.scale * kLog2e;
+    p.k_steps = (a.head_dim + 15) / 16;
+    const int64_t items = static_cast<int64_t>(a.row_capacity) * a.kv_heads;
+    p.one_half = 2 * items <= kNumSMs;
+    static std::atomic<bool> allowed[64];
+    auto kernel = packed_attention_kernel<D, BF16>;
+    if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kTotal, allowed)) return st;
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(kNumSMs, items * (p.one_half ? 2 : 1)));
+    const cudaError_t e = launch_dependent(kernel, dim3(grid), dim3(kThreads), L::kTotal, stream, 1, grid < kNumSMs, mq, mk, mv, p);
+    if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of packed_attention failed: %s", cudaGetErrorString(e));
+    MHLO_CUDA_CHECK_LAUNCH("packed_attention");
+    return MHLO_CUDA_OK;
+}
+
+}  // namespace
+
+int packed_attention_tc(const PackedCall& c, cudaStream_t stream) {
+    const bool bf16 = c.dtype == MHLO_DT_BF16;
+    if (c.a.head_dim <= 64) return bf16 ? launch<64, true>(c, stream) : launch<64, false>(c, stream);
+    return bf16 ? launch<128, true>(c, stream) : launch<128, false>(c, stream);
+}
+
+int packed_attention_tc_device_error() { return take_kv_error(); }
+
+}  // namespace mhlo

@@ -89,6 +89,11 @@ class KvBatchArgs(C.Structure):
                 ("pages_per_seq", C.c_int64), ("table_stride", C.c_int64), ("tokens", C.c_int64)]
 
 
+class PackedBatchArgs(C.Structure):
+    _fields_ = [("starts", C.c_void_p), ("plan", C.c_void_p), ("seqs", C.c_int64), ("tokens", C.c_int64), ("q_heads", C.c_int64),
+                ("kv_heads", C.c_int64), ("causal", C.c_int32)]
+
+
 if not os.path.exists(LIB_PATH):
     raise ImportError(
         f"{LIB_PATH} is missing: build it with `make -C metalhlo_b200/csrc` "
@@ -203,6 +208,12 @@ _PROTOTYPES = {
     "mhlo_cuda_cached_attention_scratch_bytes": (_i64, [C.POINTER(KvCacheArgs), C.POINTER(KvBatchArgs), _i64]),
     "mhlo_cuda_cached_attention": (C.c_int, [_i32, _vp, C.POINTER(_i64), C.POINTER(KvCacheArgs), C.POINTER(KvBatchArgs), _i64, _f32, _vp,
                                              C.POINTER(_i64), _vp, _vp, _i64, _vp]),
+    "mhlo_cuda_packed_plan_bytes": (_i64, [C.POINTER(PackedBatchArgs)]),
+    "mhlo_cuda_packed_plan": (C.c_int, [C.POINTER(PackedBatchArgs), _vp]),
+    "mhlo_cuda_packed_attention": (C.c_int, [_i32, C.POINTER(PackedBatchArgs), _i64, _f32] + [_vp, C.POINTER(_i64)] * 4 + [_vp, _vp]),
+    "mhlo_cuda_packed_attention_grad_scratch_bytes": (_i64, [C.POINTER(PackedBatchArgs)]),
+    "mhlo_cuda_packed_attention_grad": (C.c_int, [_i32, C.POINTER(PackedBatchArgs), _i64, _f32] + [_vp, C.POINTER(_i64)] * 4 + [_vp] +
+                                        [_vp, C.POINTER(_i64)] * 4 + [_vp, _i64, _vp]),
     "mhlo_cuda_token_logprobs": (C.c_int, [_i32, _vp, _i64, _i64, _i64, _f32, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
     "mhlo_cuda_token_logprobs_grad": (C.c_int, [_i32, _vp, _i64, _i64, _i64, _f32, _vp, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp]),
 }
@@ -314,7 +325,7 @@ def add_rms_norm(x, residual, gamma, eps: float = 1e-5, tuning=None, stream=None
 
 def device_error() -> int:
     """Synchronises, and returns and clears the first error word that a kernel left (0: none did): a bounded wait of a tensor-core kernel
-    expired, or (201 and above) a key/value cache kernel met a page, length, start or position that cannot be."""
+    expired, or (201 and above) a key/value cache or packed attention kernel met a page, length, start, position or plan that cannot be."""
     code = C.c_int32(0)
     lib.mhlo_cuda_device_error(C.byref(code))
     return code.value
@@ -638,6 +649,90 @@ def cached_attention(q, cache: KvCache, page_table, lengths, scale: float, token
         check(lib.mhlo_cuda_cached_attention(torch_dtype_code(dtype), q.data_ptr(), _rows(q), cache.pointer, C.byref(batch), q_heads, scale, o.data_ptr(),
                                              _rows(o), _ptr(lse), _ptr(scratch), need, s))
         return o
+
+    return _run_on(q.device, stream, call)
+
+
+# ---- attention over packed sequences -----------------------------------------------------------------------------------
+
+
+class PackedPlan:
+    """How a batch of packed sequences is cut into tiles: what :func:`packed_plan` returns. It holds for every layer of a step, forward and
+    backward, as long as ``starts`` holds; calls on other streams than its own have to be ordered behind it."""
+
+    def __init__(self, starts, tokens: int, q_heads: int, kv_heads: int, causal: bool):
+        import torch
+
+        _same_device(starts)
+        assert starts.dim() == 1 and starts.shape[0] >= 1 and starts.dtype == torch.int32 and starts.is_contiguous()
+        self.starts, self.tokens, self.q_heads, self.kv_heads, self.causal = starts, tokens, q_heads, kv_heads, bool(causal)
+        self._args = PackedBatchArgs(starts.data_ptr(), None, starts.shape[0] - 1, tokens, q_heads, kv_heads, 1 if causal else 0)
+        self.pointer = C.byref(self._args)
+        self.device = starts.device
+        self.tiles = None
+        self.scratch_bytes = lib.mhlo_cuda_packed_attention_grad_scratch_bytes(self.pointer)
+
+
+def packed_plan(starts, tokens: int, q_heads: int, kv_heads: int, causal: bool = True, stream=None) -> PackedPlan:
+    """The plan of sequences whose tokens are rows ``starts[b] .. starts[b + 1] - 1`` (int32) of tensors of ``tokens`` rows. See
+    ``mhlo_cuda_packed_plan``."""
+    plan = PackedPlan(starts, tokens, q_heads, kv_heads, causal)
+
+    def call(s):
+        plan.tiles = starts.new_empty(lib.mhlo_cuda_packed_plan_bytes(plan.pointer) >> 2)
+        plan._args.plan = plan.tiles.data_ptr()
+        check(lib.mhlo_cuda_packed_plan(plan.pointer, s))
+        return plan
+
+    return _run_on(plan.device, stream, call)
+
+
+def _packed_shapes(q, k, v, plan):
+    tokens, q_heads, dim = q.shape
+    assert (tokens, q_heads) == (plan.tokens, plan.q_heads), (tuple(q.shape), plan.tokens, plan.q_heads)
+    assert k.shape == v.shape == (tokens, plan.kv_heads, dim) and q.dtype == k.dtype == v.dtype
+    return dim
+
+
+def packed_attention(q, k, v, plan: PackedPlan, scale: float, out=None, lse=None, stream=None):
+    """Attention of q [tokens, q_heads, head_dim] over k, v [tokens, kv_heads, head_dim], each token over its own sequence. ``lse``
+    (float32 [tokens, q_heads]) receives the logarithms of the sums of exponentials, which the backward half needs. Rows of no sequence are
+    not written. See ``mhlo_cuda_packed_attention``."""
+    import torch
+
+    _same_device(q, k, v, plan.starts, out, lse)
+    dim = _packed_shapes(q, k, v, plan)
+    assert out is None or (out.shape == q.shape and out.dtype == q.dtype)
+    assert lse is None or (lse.shape == q.shape[:2] and lse.dtype == torch.float32 and lse.is_contiguous())
+
+    def call(s):
+        o = _dense_like(q) if out is None else out
+        check(lib.mhlo_cuda_packed_attention(torch_dtype_code(q.dtype), plan.pointer, dim, scale, q.data_ptr(), _rows(q), k.data_ptr(), _rows(k),
+                                             v.data_ptr(), _rows(v), o.data_ptr(), _rows(o), _ptr(lse), s))
+        return o
+
+    return _run_on(q.device, stream, call)
+
+
+def packed_attention_grad(q, k, v, out, lse, grad_out, plan: PackedPlan, scale: float, dq=None, dk=None, dv=None, stream=None):
+    """(dq, dk, dv) of :func:`packed_attention` from its results ``out`` and ``lse`` and the gradient of ``out``. See
+    ``mhlo_cuda_packed_attention_grad``."""
+    import torch
+
+    _same_device(q, k, v, plan.starts, out, lse, grad_out, dq, dk, dv)
+    dim = _packed_shapes(q, k, v, plan)
+    assert out.shape == grad_out.shape == q.shape and out.dtype == grad_out.dtype == q.dtype
+    assert lse.shape == q.shape[:2] and lse.dtype == torch.float32 and lse.is_contiguous()
+    for t, like in ((dq, q), (dk, k), (dv, v)):
+        assert t is None or (t.shape == like.shape and t.dtype == like.dtype)
+
+    def call(s):
+        grads = [_dense_like(like) if t is None else t for t, like in ((dq, q), (dk, k), (dv, v))]
+        scratch = lse.new_empty(plan.scratch_bytes >> 2) if plan.scratch_bytes else None
+        check(lib.mhlo_cuda_packed_attention_grad(torch_dtype_code(q.dtype), plan.pointer, dim, scale, q.data_ptr(), _rows(q), k.data_ptr(), _rows(k),
+                                                  v.data_ptr(), _rows(v), out.data_ptr(), _rows(out), lse.data_ptr(), grad_out.data_ptr(), _rows(grad_out),
+                                                  *(x for t in grads for x in (t.data_ptr(), _rows(t))), _ptr(scratch), plan.scratch_bytes, s))
+        return tuple(grads)
 
     return _run_on(q.device, stream, call)
 
