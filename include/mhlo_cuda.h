@@ -183,6 +183,25 @@ int mhlo_cuda_add_rms_norm_rows(int dtype, const void* x_dev, const void* residu
                                 const mhlo_cuda_row_tuning* tuning, mhlo_cuda_stream_t stream);
 
 /*
+ * Gradients of the two norms. x, gamma (may be NULL), dy, dx: like x, gamma, y of the forward half; with y^ = (x - mean) r, r = 1 / sqrt(var + eps)
+ * (RMS norm: mean 0) and t = dy * gamma,
+ *   dx = r (t - mean(t) - y^ mean(t y^)) + residual_grad (RMS norm: without mean(t)),
+ *   dgamma = sum over rows of dy y^, dbeta = sum over rows of dy: [hidden] floats, each may be NULL.
+ * residual_grad (may be NULL): [rows, hidden], the gradient of the sum that mhlo_cuda_add_layer_norm leaves beside y, whose inputs x and residual
+ * both have the gradient dx then. Statistics are taken from x again, everything is summed in fp32 and in a fixed order; dx may be x, dy or
+ * residual_grad itself. scratch: norm_grad_scratch_bytes() bytes of device memory, 16-byte aligned, that nothing else uses until the call's work
+ * is done; its contents do not matter. The reference has the forward half only
+ * (Sources/MetalHLOCore/Metal/Kernels/LayerNormKernel.swift:41-677).
+ */
+int64_t mhlo_cuda_norm_grad_scratch_bytes(int64_t rows, int64_t hidden);
+int mhlo_cuda_layer_norm_grad(int32_t dtype, const void* x_dev, const void* gamma_dev, const void* dy_dev, const void* residual_grad_dev,
+                              void* dx_dev, float* dgamma_dev, float* dbeta_dev, int64_t rows, int64_t hidden, float eps, void* scratch_dev,
+                              int64_t scratch_bytes, mhlo_cuda_stream_t stream);
+int mhlo_cuda_rms_norm_grad(int32_t dtype, const void* x_dev, const void* gamma_dev, const void* dy_dev, const void* residual_grad_dev,
+                            void* dx_dev, float* dgamma_dev, int64_t rows, int64_t hidden, float eps, void* scratch_dev,
+                            int64_t scratch_bytes, mhlo_cuda_stream_t stream);
+
+/*
  * Softmax along one axis of a tensor viewed as [outer, axis_len, inner] (inner = 1 for the last axis):
  * y = exp(x - max) / sum(exp(x - max)). Replaces kernel_softmax (CodeGenerator.swift:4690-4794) and
  * softmax_kernel(_half) (Sources/MetalHLOCore/Metal/Kernels/SoftmaxKernel.swift:23-167), semantics of
@@ -878,6 +897,42 @@ int mhlo_cuda_token_logprobs_grad(int32_t dtype, const void* x_dev, int64_t row_
                                   const float* grad_logprobs_dev, const float* grad_entropy_dev, int32_t top_k,
                                   const int32_t* top_ids_dev, const float* grad_top_dev, void* dx_dev, int64_t dx_row_stride,
                                   mhlo_cuda_stream_t stream);
+
+/*
+ * The clipped policy loss with a KL term on log probabilities of tokens, and its gradient: what stands between mhlo_cuda_token_logprobs and
+ * mhlo_cuda_token_logprobs_grad when a policy is trained on tokens that it sampled. All pointers are device memory, [tokens] each:
+ *   logprobs      of the policy that is trained
+ *   old_logprobs  of the policy that the tokens were sampled from
+ *   ref_logprobs  of a reference policy; NULL: no KL term
+ *   advantages
+ *   mask          bytes, 0: the token does not count, whatever its other values are; NULL: all tokens count
+ *   starts        [seqs + 1] ascending: tokens starts[b] .. starts[b + 1] - 1 are of sequence b, others count for nothing. NULL: one mean over
+ *                 all tokens
+ * With ratio = exp(logprob - old), x = ref - logprob and a token's weight w,
+ *   loss = sum of w (-min(ratio a, clip(ratio, 1 - clip_low, 1 + clip_high) a) + kl_weight (exp(x) - x - 1)),
+ *   grad = w ((clipped ? 0 : -ratio a) + kl_weight (1 - exp(x))); 0 for tokens that do not count.
+ * w: 1 / (counted tokens), or with starts 1 / (counted tokens of its sequence * sequences that have any). A token is clipped where its advantage
+ * is positive and its ratio above 1 + clip_high, or negative and below 1 - clip_low. results: 3 floats, the loss, the sum of w (exp(x) - x - 1)
+ * (0 without ref_logprobs) and the sum of w over clipped tokens; all 0 where nothing counts. Sums are fp64 in a fixed order.
+ * 0 <= clip_low < 1, 0 <= clip_high <= 1e30, |kl_weight| <= 1e30. grad may be one of the inputs. Starts that are out of order are reported by
+ * mhlo_cuda_device_error as 200 + MHLO_CUDA_KV_ERROR_STARTS; tokens between them may count or not.
+ * scratch: policy_loss_scratch_bytes() bytes of device memory (0: none), 16-byte aligned, that nothing else uses until the call's work is done;
+ * its contents do not matter. No counterpart in the reference.
+ */
+typedef struct {
+    const float* logprobs;
+    const float* old_logprobs;
+    const float* ref_logprobs;
+    const float* advantages;
+    const uint8_t* mask;
+    const int32_t* starts;
+    int64_t tokens, seqs;
+    double clip_low, clip_high, kl_weight;
+} mhlo_cuda_policy_batch;
+
+int64_t mhlo_cuda_policy_loss_scratch_bytes(int64_t tokens, int64_t seqs);
+int mhlo_cuda_policy_loss(const mhlo_cuda_policy_batch* batch, float* grad_dev, float* results_dev, void* scratch_dev, int64_t scratch_bytes,
+                          mhlo_cuda_stream_t stream);
 
 /*
  * stablehlo.rng: `count` values of `dtype` between the scalars *a_dev and *b_dev. distribution 0 = UNIFORM (floats in

@@ -99,6 +99,7 @@ int attention_device_error();  // same for the attention kernel
 int kv_cache_device_error();          // same for the kernels that write and read the key/value cache: MHLO_CUDA_KV_ERROR_*
 int cached_attention_device_error();  // same for the attention over it
 int packed_attention_device_error();  // same for the attention over packed sequences
+int policy_loss_device_error();       // same for the policy loss
 // Stream-ordered copies of the error words into pinned host memory, and host stores into them (clearing, or the test hook).
 bool gemm_error_fetch_async(int* pinned_dst, cudaStream_t stream);
 bool attention_error_fetch_async(int* pinned_dst, cudaStream_t stream);

@@ -165,6 +165,7 @@ int mhlo_cuda_device_error(int32_t* out_code) {
     if (v == 0) v = kv_cache_device_error(), base = 200;
     if (v == 0) v = cached_attention_device_error();
     if (v == 0) v = packed_attention_device_error();
+    if (v == 0) v = policy_loss_device_error();
     if (v < 0) return fail(MHLO_CUDA_EXECUTION_FAILED, "device_error: %s", cudaGetErrorString(cudaGetLastError()));
     if (v == 0) return MHLO_CUDA_OK;
     *out_code = base + v;

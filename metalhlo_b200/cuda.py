@@ -94,6 +94,12 @@ class PackedBatchArgs(C.Structure):
                 ("kv_heads", C.c_int64), ("causal", C.c_int32)]
 
 
+class PolicyBatchArgs(C.Structure):
+    _fields_ = [("logprobs", C.c_void_p), ("old_logprobs", C.c_void_p), ("ref_logprobs", C.c_void_p), ("advantages", C.c_void_p), ("mask", C.c_void_p),
+                ("starts", C.c_void_p), ("tokens", C.c_int64), ("seqs", C.c_int64), ("clip_low", C.c_double), ("clip_high", C.c_double),
+                ("kl_weight", C.c_double)]
+
+
 if not os.path.exists(LIB_PATH):
     raise ImportError(
         f"{LIB_PATH} is missing: build it with `make -C metalhlo_b200/csrc` "
@@ -208,6 +214,11 @@ _PROTOTYPES = {
     "mhlo_cuda_cached_attention_scratch_bytes": (_i64, [C.POINTER(KvCacheArgs), C.POINTER(KvBatchArgs), _i64]),
     "mhlo_cuda_cached_attention": (C.c_int, [_i32, _vp, C.POINTER(_i64), C.POINTER(KvCacheArgs), C.POINTER(KvBatchArgs), _i64, _f32, _vp,
                                              C.POINTER(_i64), _vp, _vp, _i64, _vp]),
+    "mhlo_cuda_policy_loss_scratch_bytes": (_i64, [_i64, _i64]),
+    "mhlo_cuda_policy_loss": (C.c_int, [C.POINTER(PolicyBatchArgs), _vp, _vp, _vp, _i64, _vp]),
+    "mhlo_cuda_norm_grad_scratch_bytes": (_i64, [_i64, _i64]),
+    "mhlo_cuda_layer_norm_grad": (C.c_int, [_i32] + [_vp] * 7 + [_i64, _i64, _f32, _vp, _i64, _vp]),
+    "mhlo_cuda_rms_norm_grad": (C.c_int, [_i32] + [_vp] * 6 + [_i64, _i64, _f32, _vp, _i64, _vp]),
     "mhlo_cuda_packed_plan_bytes": (_i64, [C.POINTER(PackedBatchArgs)]),
     "mhlo_cuda_packed_plan": (C.c_int, [C.POINTER(PackedBatchArgs), _vp]),
     "mhlo_cuda_packed_attention": (C.c_int, [_i32, C.POINTER(PackedBatchArgs), _i64, _f32] + [_vp, C.POINTER(_i64)] * 4 + [_vp, _vp]),
@@ -653,6 +664,42 @@ def cached_attention(q, cache: KvCache, page_table, lengths, scale: float, token
     return _run_on(q.device, stream, call)
 
 
+# ---- gradients of the norms ---------------------------------------------------------------------------------------------
+
+
+def _norm_grad(entry, beta, x, gamma, dy, eps, residual_grad, out, stream):
+    import torch
+
+    _same_device(x, gamma, dy, residual_grad, out)
+    hidden = x.shape[-1]
+    rows = x.numel() // hidden if hidden else 0
+    for t in (x, dy, residual_grad, out):
+        assert t is None or (t.shape == x.shape and t.dtype == x.dtype and t.is_contiguous())
+    assert gamma is None or (gamma.shape == (hidden,) and gamma.dtype == x.dtype and gamma.is_contiguous())
+
+    def call(s):
+        dx = torch.empty_like(x) if out is None else out
+        sums = torch.empty((2 if beta else 1, hidden), dtype=torch.float32, device=x.device).unbind(0)
+        need = lib.mhlo_cuda_norm_grad_scratch_bytes(rows, hidden)
+        scratch = x.new_empty((need + 3) >> 2, dtype=torch.float32) if need else None
+        check(entry(torch_dtype_code(x.dtype), x.data_ptr(), _ptr(gamma), dy.data_ptr(), _ptr(residual_grad), dx.data_ptr(), *(t.data_ptr() for t in sums),
+                    rows, hidden, eps, _ptr(scratch), need, s))
+        return (dx, *sums)
+
+    return _run_on(x.device, stream, call)
+
+
+def layer_norm_grad(x, gamma, dy, eps: float = 1e-5, residual_grad=None, out=None, stream=None):
+    """(dx, dgamma, dbeta) of :func:`layer_norm`, the last two in float32; ``residual_grad`` (of the sum that :func:`add_layer_norm` returns) is
+    added to dx. ``out`` may be an input. See ``mhlo_cuda_layer_norm_grad``."""
+    return _norm_grad(lib.mhlo_cuda_layer_norm_grad, True, x, gamma, dy, eps, residual_grad, out, stream)
+
+
+def rms_norm_grad(x, gamma, dy, eps: float = 1e-5, residual_grad=None, out=None, stream=None):
+    """(dx, dgamma) of :func:`rms_norm`, dgamma in float32. See ``mhlo_cuda_rms_norm_grad``."""
+    return _norm_grad(lib.mhlo_cuda_rms_norm_grad, False, x, gamma, dy, eps, residual_grad, out, stream)
+
+
 # ---- attention over packed sequences -----------------------------------------------------------------------------------
 
 
@@ -807,3 +854,34 @@ def token_logprobs_grad(logits, targets, lse, entropy=None, grad_logprobs=None, 
         return dx
 
     return _run_on(logits.device, stream, call)
+
+
+PolicyLoss = collections.namedtuple("PolicyLoss", "loss grad kl clip_fraction")
+
+
+def policy_loss(logprobs, old_logprobs, advantages, mask=None, ref_logprobs=None, starts=None, clip_low: float = 0.2, clip_high: float = 0.2,
+                kl_weight: float = 0.0, grad=None, stream=None) -> PolicyLoss:
+    """The clipped policy loss of tokens' log probabilities (float32, any shape; all tensors the same) with a KL term, and its gradient with respect
+    to ``logprobs``, for :func:`token_logprobs_grad`. A mean over the tokens that ``mask`` (bool) counts, or with ``starts`` (int32) a mean over
+    sequences of their means. ``kl`` is None without ``ref_logprobs``. See ``mhlo_cuda_policy_loss``."""
+    import torch
+
+    _same_device(logprobs, old_logprobs, advantages, mask, ref_logprobs, starts, grad)
+    for t in (logprobs, old_logprobs, advantages, ref_logprobs, grad):
+        assert t is None or (t.shape == logprobs.shape and t.dtype == torch.float32 and t.is_contiguous())
+    assert mask is None or (mask.shape == logprobs.shape and mask.dtype in (torch.bool, torch.uint8) and mask.is_contiguous())
+    assert starts is None or (starts.dim() == 1 and starts.shape[0] >= 1 and starts.dtype == torch.int32 and starts.is_contiguous())
+    tokens, seqs = logprobs.numel(), 0 if starts is None else starts.shape[0] - 1
+    batch = PolicyBatchArgs(logprobs.data_ptr(), old_logprobs.data_ptr(), _ptr(ref_logprobs), advantages.data_ptr(), _ptr(mask), _ptr(starts), tokens, seqs,
+                            clip_low, clip_high, kl_weight)
+
+    def call(s):
+        g = torch.empty_like(logprobs) if grad is None else grad
+        results = torch.empty(3, dtype=torch.float32, device=logprobs.device)
+        need = lib.mhlo_cuda_policy_loss_scratch_bytes(tokens, seqs)
+        scratch = results.new_empty(need >> 2) if need else None
+        check(lib.mhlo_cuda_policy_loss(C.byref(batch), g.data_ptr(), results.data_ptr(), _ptr(scratch), need, s))
+        loss, kl, clipped = results.unbind(0)
+        return PolicyLoss(loss, g, None if ref_logprobs is None else kl, clipped)
+
+    return _run_on(logprobs.device, stream, call)
