@@ -159,8 +159,8 @@ __global__ void __launch_bounds__(kWarpThreads, 2) norm_grad_warp_kernel(const _
     for (int i = tid; i < width; i += kWarpThreads) to[i] = columns[i];
 }
 
-// A row a CTA, 16 elements a thread. A stage of the ring holds a row of x and one of dy, each from the 16-byte boundary below its start on.
-constexpr int kEach = 16, kMostThreads = 1024;
+// A row a CTA, E elements a thread. A stage of the ring holds a row of x and one of dy, each from the 16-byte boundary below its start on.
+constexpr int kMostThreads = 1024;
 template <typename T>
 __host__ __device__ constexpr int ring_bytes(int hidden) { return (hidden * static_cast<int>(sizeof(T)) + 30) / 16 * 16; }
 
@@ -168,14 +168,117 @@ __device__ __forceinline__ void bulk_copy(void* to, const void* from, uint32_t b
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to)), "l"(from), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
-constexpr int kMostStages = 8;
-template <typename T, bool VEC, bool RMS, int THREADS>
-__global__ void __launch_bounds__(THREADS) norm_grad_kernel(const __grid_constant__ NormGradParams<T> p, int32_t stages) {
-    constexpr int W = VEC ? VecTraits<T>::kElems : 1, N = kEach / W;
+// Shuffles are what a row costs most of (one a clock and SM): sums of several values are taken together, the lanes that have `bit` going on with b, the
+// others with a.
+__device__ __forceinline__ float fold(float a, float b, int bit) {
+    const bool upper = (threadIdx.x & bit) != 0;
+    return (upper ? b : a) + __shfl_xor_sync(0xffffffffu, upper ? a : b, bit);
+}
+__device__ __forceinline__ float add_across(float v, int bit) { return v + __shfl_xor_sync(0xffffffffu, v, bit); }
+
+// Sums over the warp of one value a row, in all lanes.
+template <int R>
+__device__ __forceinline__ void sum_rows(float (&v)[R]) {
+    if constexpr (R == 1) {
+        v[0] = sum32(v[0]);
+    } else {
+        float x = fold(v[0], v[1], 16);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) x = add_across(x, o);
+        const float y = __shfl_xor_sync(0xffffffffu, x, 16);
+        const bool upper = (threadIdx.x & 16) != 0;
+        v[0] = upper ? y : x;
+        v[1] = upper ? x : y;
+    }
+}
+
+// Sums over the warp of three values a row, to where they are wanted: parts[row][warp] = {mean, a, b, c}.
+template <int R>
+__device__ __forceinline__ void leave_sums(float4 (*parts)[32], const float (&mean)[R], const float (&a)[R], const float (&b)[R], const float (&c)[R]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float x, y, z;
+    if constexpr (R == 2) x = fold(a[0], a[1], 16), y = fold(b[0], b[1], 16), z = fold(c[0], c[1], 16);
+    else x = add_across(a[0], 16), y = add_across(b[0], 16), z = add_across(c[0], 16);
+    x = fold(x, y, 8);
+    z = add_across(z, 8);
+    x = fold(x, z, 4);
+    x = add_across(add_across(x, 2), 1);
+    // lanes 0, 8, 4 of a row's half: a, b, c
+    const int row = R == 2 ? lane >> 4 : 0, which = lane & 15;
+    if ((R == 2 || lane < 16) && (which & 3) == 0) {
+        float* const to = reinterpret_cast<float*>(&parts[row][warp]);
+        to[which == 0 ? 1 : which == 8 ? 2 : which == 4 ? 3 : 0] = which == 12 ? (R == 2 && row == 1 ? mean[R - 1] : mean[0]) : x;
+    }
+}
+
+__device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+
+// A thread's elements of a row go in units of pairs, for two of which one instruction does: a 16-byte vector (VEC), or two elements by themselves,
+// threads apart.
+template <typename T, bool VEC>
+struct Unit {
+    static constexpr int kElems = VEC ? VecTraits<T>::kElems : 2, kPairs = kElems / 2;
+    using Held = typename std::conditional<VEC, uint4, T[2]>::type;  // as it is in memory
+    int at[VEC ? 1 : 2];
+    bool has[VEC ? 1 : 2];
+    __device__ __forceinline__ Unit(int u, int tid, int threads, int hidden) {
+#pragma unroll
+        for (int i = 0; i < (VEC ? 1 : 2); ++i) {
+            at[i] = VEC ? (u * threads + tid) * kElems : (2 * u + i) * threads + tid;
+            has[i] = at[i] < hidden;
+        }
+    }
+    __device__ __forceinline__ void hold(const T* row, Held& h) const {
+        if constexpr (VEC) {
+            if (has[0]) h = ld_stream16(row + at[0]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (has[i]) h[i] = row[at[i]];
+        }
+    }
+    __device__ __forceinline__ void unpack(const Held& h, float2* v) const {
+        if constexpr (VEC) VecTraits<T>::unpack2(h, v);
+        else *v = make_float2(VecTraits<T>::to_float(h[0]), VecTraits<T>::to_float(h[1]));
+    }
+    // Elements behind the row's end: not to be looked at (VEC), zero.
+    __device__ __forceinline__ void load(const T* row, float2* v) const {
+        if constexpr (VEC) VecTraits<T>::unpack2(*reinterpret_cast<const uint4*>(row + at[0]), v);
+        else *v = make_float2(has[0] ? VecTraits<T>::to_float(row[at[0]]) : 0.f, has[1] ? VecTraits<T>::to_float(row[at[1]]) : 0.f);
+    }
+    __device__ __forceinline__ bool any() const { return has[0]; }
+    __device__ __forceinline__ float2 only(float2 v) const {
+        if constexpr (!VEC) v = make_float2(has[0] ? v.x : 0.f, has[1] ? v.y : 0.f);
+        return v;
+    }
+    __device__ __forceinline__ void store(T* row, const float2* v) const {
+        if constexpr (VEC) {
+            st_stream16(row + at[0], VecTraits<T>::pack2(v));
+        } else {
+            if (has[0]) row[at[0]] = VecTraits<T>::from_float(v->x);
+            if (has[1]) row[at[1]] = VecTraits<T>::from_float(v->y);
+        }
+    }
+    __device__ __forceinline__ void store_sums(float* row, const float2* v) const {
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+            if (VEC || has[0]) row[at[0] + 2 * k] = v[k].x;
+            if (VEC) row[at[0] + 2 * k + 1] = v[k].y;
+            else if (has[VEC ? 0 : 1]) row[at[VEC ? 0 : 1]] = v[k].y;
+        }
+    }
+};
+
+constexpr int kMostStages = 12;
+// E: elements of a thread. R: rows at once, which share a barrier and the latency of the reductions.
+template <typename T, bool VEC, bool RMS, int E, int R, int THREADS, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS) norm_grad_kernel(const __grid_constant__ NormGradParams<T> p, int32_t stages) {
+    using U = Unit<T, VEC>;
+    constexpr int N = E / U::kElems, P = U::kPairs;
     extern __shared__ __align__(16) uint8_t ring[];
     __shared__ uint64_t full[kMostStages];
-    __shared__ float4 parts[2][32];  // of a row, by warp
-    __shared__ float counts[32];     // elements of a warp
+    __shared__ float4 parts[2][R][32];  // of a row, by warp: mean, squares, t, t times deviation
+    __shared__ float counts[32];        // elements of a warp
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
     const int row_bytes = ring_bytes<T>(p.hidden);
     const float over_hidden = 1.f / static_cast<float>(p.hidden);
@@ -185,7 +288,10 @@ __global__ void __launch_bounds__(THREADS) norm_grad_kernel(const __grid_constan
     }
     float mine = 0.f;
 #pragma unroll
-    for (int n = 0; n < N; ++n) mine += (n * threads + tid) * W < p.hidden ? W : 0;
+    for (int n = 0; n < N; ++n) {
+        const U u(n, tid, threads, p.hidden);
+        mine += VEC ? (u.has[0] ? U::kElems : 0) : u.has[0] + u.has[VEC ? 0 : 1];
+    }
     const float count = sum32(mine), over_count = count > 0.f ? 1.f / count : 0.f;
     if (lane == 0) counts[warp] = count;
     __syncthreads();
@@ -215,111 +321,158 @@ __global__ void __launch_bounds__(THREADS) norm_grad_kernel(const __grid_constan
             if (bytes[i] > 0) bulk_copy(ring + (stage * 2 + i) * row_bytes, reinterpret_cast<const void*>(start[i]), bytes[i], &full[stage]);
     };
     int64_t row = blockIdx.x;
+    const int64_t step = gridDim.x;
     if (tid == 0)
-        for (int s = 0; s < stages; ++s) send(row + static_cast<int64_t>(s) * gridDim.x, s);
-    float of_gamma[kEach], of_beta[kEach];
+        for (int s = 0; s < stages; ++s) send(row + s * step, s);
+    float2 gamma[E / 2], of_gamma[E / 2], of_beta[E / 2];
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) of_gamma[e] = of_beta[e] = 0.f;
+    for (int k = 0; k < E / 2; ++k) {
+        gamma[k] = twice(1.f);
+        of_gamma[k] = of_beta[k] = twice(0.f);
+    }
+    if (p.gamma != nullptr) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const U u(n, tid, threads, p.hidden);
+            if (u.any()) u.load(p.gamma, gamma + n * P);
+        }
+    }
     int stage = 0;
     uint32_t phase = 0;
-    for (int turn = 0; row < p.rows; row += gridDim.x, turn ^= 1) {
-        Raw<T, W> residual[N];
+    for (int turn = 0; row < p.rows; row += R * step, turn ^= 1) {
+        const T *x[R], *dy[R];
+        float mean[R], squares[R], sum_t[R], sum_td[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t r = row + i * step;
+            const int at = stage + i < stages ? stage + i : stage + i - stages;
+            x[i] = reinterpret_cast<const T*>(ring + at * 2 * row_bytes + (VEC ? 0 : reinterpret_cast<uintptr_t>(p.x + r * p.hidden) & 15));
+            dy[i] = reinterpret_cast<const T*>(ring + (at * 2 + 1) * row_bytes + (VEC ? 0 : reinterpret_cast<uintptr_t>(p.dy + r * p.hidden) & 15));
+            if (r < p.rows && !mbar_wait(&full[at], phase ^ (stage + i < stages ? 0u : 1u))) return;  // cannot be: nothing but the copies is waited for
+            mean[i] = 0.f;
+            if (!RMS && r < p.rows) {
+                float2 sum = twice(0.f);
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    const U u(n, tid, threads, p.hidden);
+                    if (!u.any()) continue;
+                    float2 v[P];
+                    u.load(x[i], v);
+#pragma unroll
+                    for (int k = 0; k < P; ++k) sum = __fadd2_rn(sum, v[k]);
+                }
+                mean[i] = sum.x + sum.y;
+            }
+        }
+        if (!RMS) {
+            sum_rows<R>(mean);
+#pragma unroll
+            for (int i = 0; i < R; ++i) mean[i] *= over_count;
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            float2 sq = twice(0.f), st = twice(0.f), std = twice(0.f);
+            const float2 minus_mean = twice(-mean[i]);
+            if (row + i * step < p.rows) {
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    const U u(n, tid, threads, p.hidden);
+                    if (!u.any()) continue;
+                    float2 v[P], t[P];
+                    u.load(x[i], v);
+                    u.load(dy[i], t);
+#pragma unroll
+                    for (int k = 0; k < P; ++k) {
+                        const float2 d = RMS ? v[k] : u.only(__fadd2_rn(v[k], minus_mean)), tg = __fmul2_rn(t[k], gamma[n * P + k]);
+                        sq = __ffma2_rn(d, d, sq);
+                        if (!RMS) st = __fadd2_rn(st, tg);
+                        std = __ffma2_rn(tg, d, std);
+                    }
+                }
+            }
+            squares[i] = sq.x + sq.y;
+            sum_t[i] = st.x + st.y;
+            sum_td[i] = std.x + std.y;
+        }
+        leave_sums<R>(parts[turn], mean, squares, sum_t, sum_td);
+        typename U::Held residual[R][N];
         if (p.residual != nullptr) {
 #pragma unroll
-            for (int n = 0; n < N; ++n)
-                if ((n * threads + tid) * W < p.hidden) residual[n].load(p.residual + row * p.hidden + (n * threads + tid) * W);
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                    if (row + i * step < p.rows) U(n, tid, threads, p.hidden).hold(p.residual + (row + i * step) * p.hidden, residual[i][n]);
         }
-        const T *const x = reinterpret_cast<const T*>(ring + stage * 2 * row_bytes + (VEC ? 0 : reinterpret_cast<uintptr_t>(p.x + row * p.hidden) & 15)),
-                *const dy = reinterpret_cast<const T*>(ring + (stage * 2 + 1) * row_bytes + (VEC ? 0 : reinterpret_cast<uintptr_t>(p.dy + row * p.hidden) & 15));
-        if (!mbar_wait(&full[stage], phase)) return;  // cannot be: nothing but the copies is waited for
-        float mean = 0.f;
-        float dev[kEach];
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int i = (n * threads + tid) * W;
-#pragma unroll
-            for (int e = 0; e < W; ++e) dev[n * W + e] = 0.f;
-            if (i < p.hidden) load<T, W>(x + i, dev + n * W);
-#pragma unroll
-            for (int e = 0; e < W; ++e) mean += dev[n * W + e];
-        }
-        mean = RMS ? 0.f : sum32(mean) * over_count;
-        float squares = 0.f, sum_t = 0.f, sum_td = 0.f;
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int i = (n * threads + tid) * W;
-            if (i < p.hidden) {
-                float t[W], g[W];
-                load<T, W>(dy + i, t);
-                if (p.gamma != nullptr) load<T, W>(p.gamma + i, g);
-#pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    if (p.gamma != nullptr) t[e] *= g[e];
-                    const float d = dev[n * W + e] - mean;
-                    squares = fmaf(d, d, squares);
-                    sum_t += t[e];
-                    sum_td = fmaf(t[e], d, sum_td);
-                }
-            }
-        }
-        squares = sum32(squares);
-        if (!RMS) sum_t = sum32(sum_t);
-        sum_td = sum32(sum_td);
-        if (lane == 0) parts[turn][warp] = make_float4(mean, squares, sum_t, sum_td);
         __syncthreads();
-        // all have done with the row before this one
-        if (tid == 0 && row >= gridDim.x) {
-            const int before = stage == 0 ? stages - 1 : stage - 1;
-            send(row + static_cast<int64_t>(stages - 1) * gridDim.x, before);
-        }
-        const bool there = lane < warps;
-        const float4 w = there ? parts[turn][lane] : make_float4(0.f, 0.f, 0.f, 0.f);
-        if (RMS) {
-            squares = sum32(w.y);
-            sum_td = sum32(w.w);
-        } else {
-            const float n = there ? counts[lane] : 0.f;
-            mean = sum32(n * w.x) * over_hidden;
-            const float d = w.x - mean;
-            squares = sum32(there ? fmaf(n * d, d, w.y) : 0.f);
-            sum_t = sum32(w.z);
-            sum_td = sum32(there ? fmaf(w.z, d, w.w) : 0.f);
-        }
-        const float r = rsqrtf(fmaf(squares, over_hidden, p.eps)), c1 = RMS ? 0.f : sum_t * over_hidden, c2 = sum_td * r * over_hidden;
+        // all have done with the rows before these
+        if (tid == 0 && row >= R * step) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int i = (n * threads + tid) * W;
-            if (i < p.hidden) {
-                float d[W], g[W], out[W], rest[W];
-                if (p.residual != nullptr) residual[n].unpack(rest);
-                load<T, W>(dy + i, d);
-                if (p.gamma != nullptr) load<T, W>(p.gamma + i, g);
+            for (int i = R; i > 0; --i) send(row + (stages - i) * step, stage >= i ? stage - i : stage - i + stages);
+        }
 #pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    const int k = n * W + e;
-                    const float y = (dev[k] - mean) * r, t = p.gamma != nullptr ? d[e] * g[e] : d[e];
-                    of_gamma[k] = fmaf(d[e], y, of_gamma[k]);
-                    if (!RMS) of_beta[k] += d[e];
-                    out[e] = r * fmaf(-y, c2, t - c1);
-                    if (p.residual != nullptr) out[e] += rest[e];
+        for (int i = 0; i < R; ++i) {
+            const int64_t r = row + i * step;
+            if (r >= p.rows) continue;
+            // The warps' sums around their own means, joined around the first one's: differences of means are small, or at most as large as the
+            // row's whole deviation.
+            const float base = parts[turn][i][0].x;
+            float sq = 0.f, td = 0.f, sum = 0.f, far = 0.f, far2 = 0.f;
+            for (int w = 0; w < warps; ++w) {
+                const float4 v = parts[turn][i][w];
+                sq += v.y;
+                td += v.w;
+                if (!RMS) {
+                    const float d = v.x - base, nd = counts[w] * d;
+                    far += nd;
+                    far2 = fmaf(nd, d, far2);
+                    sum += v.z;
+                    td = fmaf(v.z, d, td);
                 }
-                store<T, W>(p.dx + row * p.hidden + i, out);
+            }
+            const float shift = far * over_hidden, c1 = sum * over_hidden;
+            if (!RMS) {
+                sq += fmaf(-far, shift, far2);
+                td = fmaf(-shift, sum, td);
+            }
+            const float rs = rsqrtf(fmaf(fmaxf(sq, 0.f), over_hidden, p.eps)), c2 = td * rs * over_hidden;
+            const float2 rs2 = twice(rs), minus_mean = twice(-(base + shift)), minus_c1 = twice(-rs * c1), minus_c2 = twice(-rs * c2);
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const U u(n, tid, threads, p.hidden);
+                if (!u.any()) continue;
+                float2 v[P], d[P], out[P];
+                u.load(x[i], v);
+                u.load(dy[i], d);
+                if (p.residual != nullptr) {
+                    u.unpack(residual[i][n], out);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < P; ++k) out[k] = twice(0.f);
+                }
+#pragma unroll
+                for (int k = 0; k < P; ++k) {
+                    const float2 y = __fmul2_rn(RMS ? v[k] : __fadd2_rn(v[k], minus_mean), rs2), t = __fmul2_rn(d[k], gamma[n * P + k]);
+                    of_gamma[n * P + k] = __ffma2_rn(d[k], y, of_gamma[n * P + k]);
+                    if (!RMS) {
+                        of_beta[n * P + k] = __fadd2_rn(of_beta[n * P + k], d[k]);
+                        out[k] = __fadd2_rn(out[k], minus_c1);
+                    }
+                    out[k] = __ffma2_rn(t, rs2, __ffma2_rn(y, minus_c2, out[k]));
+                }
+                u.store(p.dx + r * p.hidden, out);
             }
         }
-        if (++stage == stages) stage = 0, phase ^= 1;
+        stage += R;
+        if (stage >= stages) stage -= stages, phase ^= 1;
     }
     if (p.partial == nullptr) return;
     float* const to = p.partial + static_cast<int64_t>(blockIdx.x) * (RMS ? 1 : 2) * p.hidden;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const int i = (n * threads + tid) * W;
-        if (i < p.hidden) {
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                to[i + e] = of_gamma[n * W + e];
-                if (!RMS) to[p.hidden + i + e] = of_beta[n * W + e];
-            }
-        }
+        const U u(n, tid, threads, p.hidden);
+        if (!u.any()) continue;
+        u.store_sums(to, of_gamma + n * P);
+        if (!RMS) u.store_sums(to + p.hidden, of_beta + n * P);
     }
 }
 
@@ -446,23 +599,26 @@ int warp_rows(const NormGradParams<T>& p, float* dgamma, float* dbeta, cudaStrea
 // Shared memory of an SM for the rings of all its CTAs.
 constexpr int kRingBytes = 220 * 1024;
 
-template <typename T, bool VEC, bool RMS, int THREADS>
-int cta_rows_of(const NormGradParams<T>& p, int threads, float* dgamma, float* dbeta, cudaStream_t stream) {
-    const int stage = 2 * ring_bytes<T>(p.hidden);
-    // as many CTAs as have 512 threads between them, and stages as there is room for
-    const int ctas = std::max(1, 512 / threads);
-    const int stages = std::max(2, std::min(kMostStages, kRingBytes / ctas / stage));
+template <typename T, bool VEC, bool RMS, int E, int R, int THREADS, int CTAS>
+int cta_rows_of(const NormGradParams<T>& p, float* dgamma, float* dbeta, cudaStream_t stream) {
+    auto kernel = norm_grad_kernel<T, VEC, RMS, E, R, THREADS, CTAS>;
+    const int threads = ((p.hidden + E - 1) / E + 31) / 32 * 32, stage = 2 * ring_bytes<T>(p.hidden);
+    // as many CTAs as the registers take, and stages as there is room for
+    const int ctas = std::max(1, THREADS * CTAS / threads);
+    const int stages = std::max(2 * R, std::min(kMostStages, kRingBytes / ctas / stage));  // the rows at hand, and the next ones
     static std::atomic<bool> allowed[64];
-    if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(norm_grad_kernel<T, VEC, RMS, THREADS>), kRingBytes, allowed)) return st;
-    return launch<RMS>(norm_grad_kernel<T, VEC, RMS, THREADS>, p, threads, 1, static_cast<size_t>(stages) * stage, dgamma, dbeta, stream, stages);
+    if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), kRingBytes, allowed)) return st;
+    return launch<RMS>(kernel, p, threads, 1, static_cast<size_t>(stages) * stage, dgamma, dbeta, stream, stages);
 }
-// A build for each number of registers that a thread can have: 128, 80, 64.
+// 512 threads an SM, of 128 registers, up to 8192 elements.
 template <typename T, bool VEC, bool RMS>
 int cta_rows(const NormGradParams<T>& p, float* dgamma, float* dbeta, cudaStream_t stream) {
-    const int threads = ((p.hidden + kEach - 1) / kEach + 31) / 32 * 32;
-    if (threads <= 512) return cta_rows_of<T, VEC, RMS, 512>(p, threads, dgamma, dbeta, stream);
-    if (threads <= 768) return cta_rows_of<T, VEC, RMS, 768>(p, threads, dgamma, dbeta, stream);
-    return cta_rows_of<T, VEC, RMS, kMostThreads>(p, threads, dgamma, dbeta, stream);
+    constexpr int R = VEC && sizeof(T) == 2 ? 2 : 1;  // four rows of x and dy in fp32 would not fit
+    if (p.hidden <= 16 * 128) return cta_rows_of<T, VEC, RMS, 16, R, 128, 4>(p, dgamma, dbeta, stream);
+    if (p.hidden <= 16 * 256) return cta_rows_of<T, VEC, RMS, 16, R, 256, 2>(p, dgamma, dbeta, stream);
+    if (p.hidden <= 16 * 512) return cta_rows_of<T, VEC, RMS, 16, R, 512, 1>(p, dgamma, dbeta, stream);
+    if (p.hidden <= 16 * 768) return cta_rows_of<T, VEC, RMS, 16, 1, 768, 1>(p, dgamma, dbeta, stream);
+    return cta_rows_of<T, VEC, RMS, 16, 1, 1024, 1>(p, dgamma, dbeta, stream);
 }
 
 template <typename T, bool RMS>
@@ -490,7 +646,7 @@ int norm_grad(const NormGradParams<T>& p, void* scratch, float* dgamma, float* d
     if (vec && p.hidden <= 32 * V) return warp_rows<T, V, 1, RMS>(p, dgamma, dbeta, stream);
     if (vec && p.hidden <= 64 * V) return warp_rows<T, V, 2, RMS>(p, dgamma, dbeta, stream);
     if (!vec && p.hidden <= 256) return warp_rows<T, 1, 8, RMS>(p, dgamma, dbeta, stream);
-    if (p.hidden <= kEach * kMostThreads && 4 * ring_bytes<T>(p.hidden) <= kRingBytes)  // two stages
+    if (p.hidden <= 16 * kMostThreads && 4 * ring_bytes<T>(p.hidden) <= kRingBytes)  // two stages
         return vec ? cta_rows<T, true, RMS>(p, dgamma, dbeta, stream) : cta_rows<T, false, RMS>(p, dgamma, dbeta, stream);
     return long_rows<T, RMS>(p, scratch, dgamma, dbeta, stream);
 }
