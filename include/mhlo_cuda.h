@@ -860,7 +860,7 @@ int mhlo_cuda_packed_attention(int32_t dtype, const mhlo_cuda_packed_batch* batc
  * scratch: packed_attention_grad_scratch_bytes() bytes of device memory, 16-byte aligned, that nothing else uses until the call's work is
  * done; its contents do not matter.
  */
-int64_t mhlo_cuda_packed_attention_grad_scratch_bytes(const mhlo_cuda_packed_batch* batch);
+int64_t mhlo_cuda_packed_attention_grad_scratch_bytes(int32_t dtype, const mhlo_cuda_packed_batch* batch, int64_t head_dim);
 int mhlo_cuda_packed_attention_grad(int32_t dtype, const mhlo_cuda_packed_batch* batch, int64_t head_dim, float scale, const void* q_dev,
                                     const int64_t q_strides[2], const void* k_dev, const int64_t k_strides[2], const void* v_dev,
                                     const int64_t v_strides[2], const void* o_dev, const int64_t o_strides[2], const float* lse_dev,

@@ -10,26 +10,50 @@ namespace mhlo {
 namespace {
 
 // ---- the plan ---------------------------------------------------------------------------------------------------------------------
-// One CTA: counts tiles by the 128-token blocks they meet, scans, and puts them in place, longest first. The order of tiles of one length
-// goes by arrival; no result depends on it. 32 sequences of 1024 tokens take 8 us, once for all layers of a step.
+// A CTA for each run of sequences, those whose first tokens lie in its run_tokens: it counts the tiles in front of its own, then its own by the
+// 128-token blocks they meet, scans, and puts them in place, longest first. The order of tiles of one length goes by arrival; no result depends
+// on it. 32 sequences of 1024 tokens take 5 us, once for all layers of a step.
 constexpr int kBuckets = 2048, kPlanThreads = 1024;
 
 __device__ __forceinline__ int32_t bucket_of(int32_t tokens) { return kBuckets - 1 - min((tokens - 1) >> 7, kBuckets - 1); }
 
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a) {
     __shared__ int32_t counts[2][kBuckets];
-    __shared__ int32_t sums[2][32];
+    __shared__ int32_t sums[2][32], before[2], all[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    for (int i = tid; i < 2 * kBuckets; i += kPlanThreads) counts[0][i] = 0;
-    __syncthreads();
     const int32_t steps[2] = {2 * a.half_tokens, kKeyTile};
+    for (int i = tid; i < 2 * kBuckets; i += kPlanThreads) counts[0][i] = 0;
+    if (tid < 2) before[tid] = all[tid] = 0;
+    __syncthreads();
+    // tiles of the runs in front of this one, and of all
+    int32_t mine[2] = {0, 0}, total[2] = {0, 0};
+    for (int32_t b = tid; b < a.seqs; b += kPlanThreads) {
+        const int32_t first = a.starts[b], end = a.starts[b + 1];
+        if (first < 0 || end > a.tokens || end < first) {
+            kv_report(MHLO_CUDA_KV_ERROR_STARTS);
+            continue;
+        }
+#pragma unroll
+        for (int list = 0; list < 2; ++list) {
+            const int32_t tiles = (end - first + steps[list] - 1) / steps[list];
+            total[list] += tiles;
+            if (first / a.run_tokens < static_cast<int32_t>(blockIdx.x)) mine[list] += tiles;
+        }
+    }
+#pragma unroll
+    for (int list = 0; list < 2; ++list) {
+        mine[list] = __reduce_add_sync(0xffffffffu, mine[list]);
+        total[list] = __reduce_add_sync(0xffffffffu, total[list]);
+        if (lane == 0 && total[list] > 0) {
+            atomicAdd(&before[list], mine[list]);
+            atomicAdd(&all[list], total[list]);
+        }
+    }
+    __syncthreads();
     for (int place = 0; place < 2; ++place) {
         for (int32_t b = warp; b < a.seqs; b += 32) {
             const int32_t first = a.starts[b], end = a.starts[b + 1];
-            if (first < 0 || end > a.tokens || end < first) {
-                if (lane == 0) kv_report(MHLO_CUDA_KV_ERROR_STARTS);
-                continue;
-            }
+            if (first < 0 || end > a.tokens || end < first || first / a.run_tokens != static_cast<int32_t>(blockIdx.x)) continue;
             const int32_t n = end - first;
 #pragma unroll
             for (int list = 0; list < 2; ++list) {
@@ -56,25 +80,22 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a)
             }
             if (lane == 31) sums[list][warp] = sum;
             __syncthreads();
-            int32_t before = sum - x - y;
-            for (int w = 0; w < warp; ++w) before += sums[list][w];
-            counts[list][2 * tid] = before;
-            counts[list][2 * tid + 1] = before + x;
-            if (tid == kPlanThreads - 1) {
-                PlanHeader* const h = static_cast<PlanHeader*>(a.plan);
-                if (list == 0) h->row_tiles = min(before + x + y, a.row_capacity);
-                else h->key_tiles = min(before + x + y, a.key_capacity);
-            }
+            int32_t at = before[list] + sum - x - y;
+            for (int w = 0; w < warp; ++w) at += sums[list][w];
+            counts[list][2 * tid] = at;
+            counts[list][2 * tid + 1] = at + x;
         }
         __syncthreads();
     }
-    if (tid == 0) {
+    if (tid == 0 && blockIdx.x == 0) {
         PlanHeader* const h = static_cast<PlanHeader*>(a.plan);
         h->magic = kPlanMagic;
         h->tokens = a.tokens;
         h->q_heads = a.q_heads;
         h->kv_heads = a.kv_heads;
         h->causal = a.causal;
+        h->row_tiles = min(all[0], a.row_capacity);
+        h->key_tiles = min(all[1], a.key_capacity);
         h->first = min(max(a.starts[0], 0), a.tokens);
         h->end = min(max(a.starts[a.seqs], h->first), a.tokens);
     }
@@ -100,6 +121,8 @@ struct GeneralParams {
     uint32_t* norms;  // null, or where the largest squared norms of a row of grad and of a row of v go
     float scale, scale_log2;
     int32_t subs;   // tiles of this kernel to an entry of the plan
+    int32_t splits; // shares of the rows that see a tile of keys
+    float* shares;
 };
 
 // acc[i][j] += sum over d of a[8 y + i][d] b[x + 16 j][d]
@@ -320,67 +343,130 @@ __global__ void __launch_bounds__(kGT) packed_general_kernel(const __grid_consta
     }
 }
 
-// What the backward half needs of a row: -lse log2(e) and delta = grad . o, 16 lanes a row; bound by its bytes.
-constexpr int kStatsThreads = 256;
-template <typename T>
-__global__ void __launch_bounds__(kStatsThreads) packed_stats_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
+// What the backward half needs of a row: -lse log2(e) and delta = grad . o; fp16: the largest norms of rows of grad and v. LANES of a warp to a row,
+// kStatsRows rows at once, as many bytes on their way as HBM wants (16 384 tokens of 32 heads of 128, bf16: 77 us with one row, 47 with four).
+constexpr int kStatsThreads = 256, kStatsRows = 4;
+template <typename T, int LANES, bool VEC>
+__global__ void __launch_bounds__(kStatsThreads) packed_stats_kernel(const __grid_constant__ GeneralParams p, FastDiv by_heads, FastDiv by_kv_heads, FastDiv by_group) {
     const PackedArgs& a = p.a;
     constexpr int V = VecTraits<T>::kElems;
-    const int lane = threadIdx.x & 15;
+    const int lane = threadIdx.x % LANES;
     grid_dependency_wait();
     grid_dependency_release();
     const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
     if (!a.matches(h) || h.end <= h.first) return;
-    const int64_t tokens = h.end - h.first, rows = tokens * a.q_heads;
-    const int64_t base = (static_cast<int64_t>(blockIdx.x) * kStatsThreads + threadIdx.x) >> 4;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * (kStatsThreads / 16);
+    const uint32_t first = (blockIdx.x * kStatsThreads + threadIdx.x) / LANES, step = gridDim.x * (kStatsThreads / LANES);
     float largest = 0.f;  // squared norm; rows that are not finite have no say
-    auto norm = [&](float squares) {
-        squares = reduce16(squares, false);
-        if (squares <= 3.4028235e38f) largest = fmaxf(largest, squares);
+    auto sum_lanes = [&](float v) {
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
     };
-    auto squares_of = [&](const T* at) {
-        float squares = 0.f;
-        for (int d = lane; d < a.head_dim; d += 16) squares = fmaf(VecTraits<T>::to_float(at[d]), VecTraits<T>::to_float(at[d]), squares);
-        return squares;
+    // this lane's elements of a row
+    auto get = [&](const T* row, float* x) {
+        if constexpr (VEC) {
+            uint4 raw = make_uint4(0, 0, 0, 0);
+            if (lane * V < a.head_dim) raw = ld_stream16(row + lane * V);
+            VecTraits<T>::unpack(raw, x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] = lane * V + e < a.head_dim ? VecTraits<T>::to_float(row[lane * V + e]) : 0.f;
+        }
     };
     auto leave = [&](uint32_t* to) {  // bits of numbers that are not negative have the numbers' order
         const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
         if ((threadIdx.x & 31) == 0 && most > 0) atomicMax(to, most);
         largest = 0.f;
     };
-    for (int64_t i = base; i - (base & 1) < rows; i += step) {  // both rows of a warp come along
-        const uint32_t row = static_cast<uint32_t>(min(i, rows - 1)) + static_cast<uint32_t>(h.first) * a.q_heads;
-        const uint32_t token = row / static_cast<uint32_t>(a.q_heads), head = row - token * a.q_heads;
-        const T *const o = row_at<const T>(p.o, token, head), *const g = row_at<const T>(p.grad, token, head);
-        float sum = 0.f;
-        if (vec) {
-            for (int d = lane * V; d < a.head_dim; d += 16 * V) {
-                float x[V], y[V];
-                VecTraits<T>::unpack(*reinterpret_cast<const uint4*>(o + d), x);
-                VecTraits<T>::unpack(*reinterpret_cast<const uint4*>(g + d), y);
+    const uint32_t from = static_cast<uint32_t>(h.first) * a.q_heads, end = static_cast<uint32_t>(h.end) * a.q_heads;
+    // rows of a warp's lanes go past the end together
+    for (uint32_t base = from + first - first % (32 / LANES); base < end; base += kStatsRows * step) {
+        float o[kStatsRows][V], g[kStatsRows][V], lse[kStatsRows];
+        uint32_t token[kStatsRows], head[kStatsRows];
 #pragma unroll
-                for (int e = 0; e < V; ++e) sum = fmaf(x[e], y[e], sum);
-            }
-        } else {  // in the same order
-            for (int d = lane * V; d < a.head_dim; d += 16 * V)
-                for (int e = d; e < min(d + V, a.head_dim); ++e) sum = fmaf(VecTraits<T>::to_float(o[e]), VecTraits<T>::to_float(g[e]), sum);
+        for (int r = 0; r < kStatsRows; ++r) {
+            const uint32_t row = min(base + r * step + first % (32 / LANES), end - 1);
+            by_heads.divmod(row, &token[r], &head[r]);
+            get(row_at<const T>(p.o, token[r], head[r]), o[r]);
+            get(row_at<const T>(p.grad, token[r], head[r]), g[r]);
+            lse[r] = p.lse[row];
         }
-        sum = reduce16(sum, false);
-        if (p.norms != nullptr) norm(squares_of(g));
-        if (lane == 0 && i < rows) {
-            const uint32_t kv = head / static_cast<uint32_t>(a.group);
-            p.stats[(static_cast<int64_t>(kv) * a.tokens + token) * a.group + head - kv * a.group] = make_float2(-p.lse[row] * 1.4426950408889634f, sum);
+#pragma unroll
+        for (int r = 0; r < kStatsRows; ++r) {
+            float sum = 0.f, squares = 0.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                sum = fmaf(o[r][e], g[r][e], sum);
+                squares = fmaf(g[r][e], g[r][e], squares);
+            }
+            sum = sum_lanes(sum);
+            if (p.norms != nullptr) {
+                squares = sum_lanes(squares);
+                if (squares <= 3.4028235e38f) largest = fmaxf(largest, squares);
+            }
+            if (lane == 0 && base + r * step + first % (32 / LANES) < end) {
+                const uint32_t kv = by_group.div(head[r]);
+                p.stats[(static_cast<int64_t>(kv) * a.tokens + token[r]) * a.group + head[r] - kv * a.group] = make_float2(-lse[r] * 1.4426950408889634f, sum);
+            }
         }
     }
     if (p.norms == nullptr) return;
     leave(p.norms);
-    const int64_t of_keys = tokens * a.kv_heads;
-    for (int64_t i = base; i - (base & 1) < of_keys; i += step) {
-        const uint32_t row = static_cast<uint32_t>(min(i, of_keys - 1)) + static_cast<uint32_t>(h.first) * a.kv_heads, token = row / static_cast<uint32_t>(a.kv_heads);
-        norm(squares_of(row_at<const T>(p.v, token, row - token * a.kv_heads)));
+    const uint32_t v_from = static_cast<uint32_t>(h.first) * a.kv_heads, v_end = static_cast<uint32_t>(h.end) * a.kv_heads;
+    for (uint32_t base = v_from + first - first % (32 / LANES); base < v_end; base += kStatsRows * step) {
+        float x[kStatsRows][V];
+#pragma unroll
+        for (int r = 0; r < kStatsRows; ++r) {
+            uint32_t token, head;
+            by_kv_heads.divmod(min(base + r * step + first % (32 / LANES), v_end - 1), &token, &head);
+            get(row_at<const T>(p.v, token, head), x[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < kStatsRows; ++r) {
+            float squares = 0.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) squares = fmaf(x[r][e], x[r][e], squares);
+            squares = sum_lanes(squares);
+            if (squares <= 3.4028235e38f) largest = fmaxf(largest, squares);
+        }
     }
     leave(p.norms + 1);
+}
+
+// Sums of the shares of dk and dv, in order; four elements a thread (ANY: one).
+template <typename T, bool ANY>
+__global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant__ GeneralParams p, FastDiv by_dim, FastDiv by_heads) {
+    constexpr int W = ANY ? 1 : 4;
+    const PackedArgs& a = p.a;
+    grid_dependency_wait();
+    const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
+    if (!a.matches(h)) return;
+    const int64_t all = static_cast<int64_t>(a.tokens) * a.kv_heads * a.head_dim;
+    const uint32_t from = static_cast<uint32_t>(h.first) * a.kv_heads * (a.head_dim / W), end = static_cast<uint32_t>(h.end) * a.kv_heads * (a.head_dim / W);
+    for (uint32_t i = from + blockIdx.x * 256 + threadIdx.x; i < end; i += gridDim.x * 256) {
+        uint32_t row, d, token, head;
+        by_dim.divmod(i, &row, &d);
+        by_heads.divmod(row, &token, &head);
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            const float* const at = p.shares + which * all + static_cast<int64_t>(i) * W;
+            float sum[W];
+#pragma unroll
+            for (int e = 0; e < W; ++e) sum[e] = 0.f;
+#pragma unroll 4
+            for (int32_t s = 0; s < p.splits; ++s) {
+                if constexpr (ANY) {
+                    sum[0] += at[2 * s * all];
+                } else {
+                    const float4 v = *reinterpret_cast<const float4*>(at + 2 * s * all);
+                    sum[0] += v.x, sum[1] += v.y, sum[2] += v.z, sum[3] += v.w;
+                }
+            }
+            T* const to = row_at<T>(which == 0 ? p.dk : p.dv, token, head) + d * W;
+#pragma unroll
+            for (int e = 0; e < W; ++e) to[e] = VecTraits<T>::from_float(sum[e]);
+        }
+    }
 }
 
 // P and scale dS of 64 rows x 64 keys, both rounded to nothing less than fp32. last(i): the last key that row 8 y + i sees, -1: none.
@@ -425,7 +511,7 @@ __global__ void __launch_bounds__(kGT) packed_general_key_grads_kernel(const __g
     int4 e;
     int32_t sub, head;
     if (!a.matches(h) || !entry_of(p, a.key_tiles(), h.key_tiles, &e, &sub, &head)) return;
-    const int32_t key0 = e.z + sub * kGKeys;
+    const int32_t split = sub >> 1, key0 = e.z + (sub & 1) * kGKeys;
     if (key0 >= e.y) return;
     const int tid = threadIdx.x, y = tid >> 4, x = tid & 15;
     auto key_row = [&](const PackedTensor& t, int r) -> const T* { return key0 + r < e.y ? row_at<const T>(t, e.x + key0 + r, head) : nullptr; };
@@ -436,8 +522,10 @@ __global__ void __launch_bounds__(kGT) packed_general_key_grads_kernel(const __g
     for (int i = 0; i < 8; ++i)
 #pragma unroll
         for (int c = 0; c < G::kC; ++c) dk[i][c] = dv[i][c] = 0.f;
-    const int32_t rows = e.y * a.group;
-    for (int32_t r0 = a.causal ? key0 * a.group : 0; r0 < rows; r0 += kGRows) {
+    const int32_t rows = e.y * a.group, row0 = a.causal ? key0 * a.group : 0;
+    const int64_t blocks = (rows - row0 + kGRows - 1) / kGRows;
+    const int32_t share0 = row0 + static_cast<int32_t>(blocks * split / p.splits) * kGRows, share1 = row0 + static_cast<int32_t>(blocks * (split + 1) / p.splits) * kGRows;
+    for (int32_t r0 = share0; r0 < min(rows, share1); r0 += kGRows) {
         const RowRun run{e.x, e.y, head, 0, r0, rows};
         __syncthreads();
         auto query_row = [&](const PackedTensor& t, int r) -> const T* { return run.has(a, r) ? row_at<const T>(t, run.first + run.token(a, r), run.q_head(a, r)) : nullptr; };
@@ -456,6 +544,12 @@ __global__ void __launch_bounds__(kGT) packed_general_key_grads_kernel(const __g
     for (int i = 0; i < 8; ++i) {
         const int32_t key = key0 + 8 * y + i;
         if (key >= e.y) continue;
+        if (p.splits > 1) {
+            float* const to = p.shares + ((static_cast<int64_t>(split) * 2 * a.tokens + e.x + key) * a.kv_heads + head) * a.head_dim;
+            store_row<float, DP>(to, a.head_dim, dk[i], p.scale, x);
+            store_row<float, DP>(to + static_cast<int64_t>(a.tokens) * a.kv_heads * a.head_dim, a.head_dim, dv[i], 1.f, x);
+            continue;
+        }
         store_row<T, DP>(row_at<T>(p.dk, e.x + key, head), a.head_dim, dk[i], p.scale, x);
         store_row<T, DP>(row_at<T>(p.dv, e.x + key, head), a.head_dim, dv[i], 1.f, x);
     }
@@ -520,6 +614,8 @@ GeneralParams general_params(const PackedCall& c) {
     p.lse = c.lse;
     p.stats = c.scratch ? c.stats() : nullptr;
     p.norms = nullptr;
+    p.splits = 1;
+    p.shares = c.scratch ? c.shares() : nullptr;
     p.scale = c.scale;
     p.scale_log2 = c.scale * 1.4426950408889634f;
     p.subs = 0;
@@ -537,6 +633,9 @@ int launch_general(const char* what, K kernel, GeneralParams p, int32_t subs, in
     return MHLO_CUDA_OK;
 }
 
+// Two CTAs to an SM.
+int32_t key_splits_general(const PackedArgs& a) { return key_splits(static_cast<int64_t>(a.key_capacity) * (kKeyTile / kGKeys) * a.kv_heads, 4 * kNumSMs); }
+
 int32_t row_subs(const PackedArgs& a) { return (2 * a.half_tokens * a.group + kGRows - 1) / kGRows; }
 
 template <typename T, int DP>
@@ -550,22 +649,49 @@ template <typename T, int DP>
 int backward(const PackedCall& c, cudaStream_t stream) {
     static std::atomic<bool> allowed_keys[64], allowed_queries[64];
     const int32_t vec = vectors<T>(c.q, c.a.head_dim) && vectors<T>(c.k, c.a.head_dim) && vectors<T>(c.v, c.a.head_dim) && vectors<T>(c.grad, c.a.head_dim);
-    if (int st = launch_general("packed_attention_grad", packed_general_key_grads_kernel<T, DP>, general_params(c), kKeyTile / kGKeys, c.a.key_capacity, 4, 2, DP, vec, allowed_keys, stream))
+    GeneralParams p = general_params(c);
+    p.splits = key_splits_general(c.a);
+    if (int st = launch_general("packed_attention_grad", packed_general_key_grads_kernel<T, DP>, p, kKeyTile / kGKeys * p.splits, c.a.key_capacity, 4, 2, DP, vec, allowed_keys, stream))
         return st;
+    if (p.splits > 1)
+        if (int st = packed_join_shares(c, p.splits, stream)) return st;
     return launch_general("packed_attention_grad", packed_general_query_grads_kernel<T, DP>, general_params(c), row_subs(c.a), c.a.row_capacity, 4, 1, DP, vec, allowed_queries, stream);
 }
 
-template <typename T>
-int stats(const PackedCall& c, bool norms, cudaStream_t stream) {
-    const int32_t vec = vectors<T>(c.o, c.a.head_dim) && vectors<T>(c.grad, c.a.head_dim);
-    const int64_t rows = static_cast<int64_t>(c.a.tokens) * c.a.q_heads;
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((rows + 15) / 16, 8 * kNumSMs));
+template <typename T, int LANES, bool VEC>
+int stats_of(const PackedCall& c, bool norms, cudaStream_t stream) {
+    const int64_t rows = static_cast<int64_t>(c.a.tokens) * c.a.q_heads, of_cta = kStatsRows * (kStatsThreads / LANES);
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((rows + of_cta - 1) / of_cta, 8 * kNumSMs));
     GeneralParams p = general_params(c);
     if (norms) {
         p.norms = c.norms();
         MHLO_CUDA_TRY(cudaMemsetAsync(p.norms, 0, 2 * sizeof(uint32_t), stream), MHLO_CUDA_EXECUTION_FAILED);
     }
-    const cudaError_t e = launch_dependent(packed_stats_kernel<T>, dim3(grid), dim3(kStatsThreads), 0, stream, 1, grid < kNumSMs, p, vec);
+    const auto by = [](int32_t n) { return FastDiv(static_cast<uint32_t>(n)); };
+    const cudaError_t e = launch_dependent(packed_stats_kernel<T, LANES, VEC>, dim3(grid), dim3(kStatsThreads), 0, stream, 1, grid < kNumSMs, p, by(c.a.q_heads), by(c.a.kv_heads),
+                                           by(c.a.group));
+    if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of packed_attention_grad failed: %s", cudaGetErrorString(e));
+    MHLO_CUDA_CHECK_LAUNCH("packed_attention_grad");
+    return MHLO_CUDA_OK;
+}
+template <typename T>
+int stats(const PackedCall& c, bool norms, cudaStream_t stream) {
+    constexpr int V = VecTraits<T>::kElems, kFew = 64 / V, kMany = 128 / V;
+    const bool vec = vectors<T>(c.o, c.a.head_dim) && vectors<T>(c.grad, c.a.head_dim) && vectors<T>(c.v, c.a.head_dim), few = c.a.head_dim <= 64;
+    if (vec) return few ? stats_of<T, kFew, true>(c, norms, stream) : stats_of<T, kMany, true>(c, norms, stream);
+    return few ? stats_of<T, kFew, false>(c, norms, stream) : stats_of<T, kMany, false>(c, norms, stream);
+}
+
+template <typename T>
+int join_shares(const PackedCall& c, int32_t splits, cudaStream_t stream) {
+    GeneralParams p = general_params(c);
+    p.splits = splits;
+    const bool any = c.a.head_dim % 4 != 0;
+    const int64_t threads = static_cast<int64_t>(c.a.tokens) * c.a.kv_heads * c.a.head_dim / (any ? 1 : 4);
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((threads + 255) / 256, 8 * kNumSMs)));
+    const FastDiv by_dim(static_cast<uint32_t>(c.a.head_dim / (any ? 1 : 4))), by_heads(static_cast<uint32_t>(c.a.kv_heads));
+    const cudaError_t e = any ? launch_dependent(packed_join_kernel<T, true>, grid, dim3(256), 0, stream, 1, true, p, by_dim, by_heads)
+                              : launch_dependent(packed_join_kernel<T, false>, grid, dim3(256), 0, stream, 1, true, p, by_dim, by_heads);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of packed_attention_grad failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("packed_attention_grad");
     return MHLO_CUDA_OK;
@@ -578,6 +704,13 @@ int by_type(const PackedCall& c, F f) {
         case MHLO_DT_F16: return f(__half{});
         default: return f(__nv_bfloat16{});
     }
+}
+
+// A call's layout may keep it from the tensor cores: the larger of both.
+int64_t grad_scratch_bytes(int32_t dtype, const PackedArgs& a, int64_t dim) {
+    const int64_t splits = std::max(key_splits_general(a), dtype == MHLO_DT_F32 ? 1 : key_splits_tc(a));
+    const int64_t shares = splits > 1 ? splits * 2 * a.tokens * a.kv_heads * dim * 4 : 0;
+    return (static_cast<int64_t>(a.tokens) * a.q_heads + 1) / 2 * 2 * static_cast<int64_t>(sizeof(float2)) + 16 + shares;
 }
 
 // What the host can see of a batch.
@@ -602,8 +735,10 @@ int packed_args(const char* what, const mhlo_cuda_packed_batch* b, PackedArgs* o
     const int64_t most = std::min(b->seqs, b->tokens);  // sequences that have tokens
     out->row_capacity = static_cast<int32_t>(b->tokens / (2 * out->half_tokens) + most);
     out->key_capacity = static_cast<int32_t>(b->tokens / kKeyTile + most);
+    // 16-bit keys and values of 128 elements a head: a quarter of L2
+    out->run_tokens = std::max<int32_t>(128, (32 << 20) / (512 * out->kv_heads));
     // items of the general kernels, the finest
-    const int64_t finest = std::max<int64_t>(static_cast<int64_t>(out->row_capacity) * std::max(2, row_subs(*out)), 2 * static_cast<int64_t>(out->key_capacity)) * out->kv_heads;
+    const int64_t finest = std::max<int64_t>(static_cast<int64_t>(out->row_capacity) * std::max(2, row_subs(*out)), 2 * static_cast<int64_t>(out->key_capacity) * key_splits_general(*out)) * out->kv_heads;
     if (finest > 0x7fffffff) return fail(MHLO_CUDA_UNSUPPORTED, "%s: too many tiles", what);
     return MHLO_CUDA_OK;
 }
@@ -649,6 +784,10 @@ bool on_tensor_cores(const PackedCall& c, std::initializer_list<const PackedTens
 
 }  // namespace
 
+int packed_join_shares(const PackedCall& c, int32_t splits, cudaStream_t stream) {
+    return by_type(c, [&](auto t) { return join_shares<decltype(t)>(c, splits, stream); });
+}
+
 int packed_attention_device_error() {
     const int plan = take_kv_error(), forward = packed_attention_tc_device_error(), backward = packed_attention_grad_tc_device_error();
     if (plan < 0 || forward < 0 || backward < 0) return -1;
@@ -671,7 +810,7 @@ int mhlo_cuda_packed_plan(const mhlo_cuda_packed_batch* batch, mhlo_cuda_stream_
     if (int st = packed_args("packed_plan", batch, &a)) return st;
     if (a.seqs == 0 || a.tokens == 0) return MHLO_CUDA_OK;
     if (!a.starts || !a.plan || !aligned16(a.plan)) return fail(MHLO_CUDA_INVALID_ARGUMENT, "packed_plan: null starts, or null or unaligned plan");
-    packed_plan_kernel<<<1, kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    packed_plan_kernel<<<static_cast<unsigned>((a.tokens + a.run_tokens - 1) / a.run_tokens), kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
     MHLO_CUDA_CHECK_LAUNCH("packed_plan");
     return MHLO_CUDA_OK;
 }
@@ -694,10 +833,10 @@ int mhlo_cuda_packed_attention(int32_t dtype, const mhlo_cuda_packed_batch* batc
     return by_type(c, [&](auto t) { return c.a.head_dim <= 64 ? forward<decltype(t), 64>(c, s) : forward<decltype(t), 128>(c, s); });
 }
 
-int64_t mhlo_cuda_packed_attention_grad_scratch_bytes(const mhlo_cuda_packed_batch* batch) {
+int64_t mhlo_cuda_packed_attention_grad_scratch_bytes(int32_t dtype, const mhlo_cuda_packed_batch* batch, int64_t head_dim) {
     PackedArgs a;
-    if (packed_args("packed_attention_grad", batch, &a) != MHLO_CUDA_OK) return 0;
-    return static_cast<int64_t>(a.tokens) * a.q_heads * static_cast<int64_t>(sizeof(float2)) + 16;
+    if (head_dim < 1 || head_dim > 128 || packed_args("packed_attention_grad", batch, &a) != MHLO_CUDA_OK) return 0;
+    return grad_scratch_bytes(dtype, a, head_dim);
 }
 
 int mhlo_cuda_packed_attention_grad(int32_t dtype, const mhlo_cuda_packed_batch* batch, int64_t head_dim, float scale, const void* q_dev, const int64_t q_strides[2],
@@ -718,7 +857,7 @@ int mhlo_cuda_packed_attention_grad(int32_t dtype, const mhlo_cuda_packed_batch*
     if (int st = result(what, "dk", dk_dev, dk_strides, c.a.tokens, c.a.kv_heads, head_dim, &c.dk)) return st;
     if (int st = result(what, "dv", dv_dev, dv_strides, c.a.tokens, c.a.kv_heads, head_dim, &c.dv)) return st;
     if (!lse_dev) return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: null lse", what);
-    const int64_t need = mhlo_cuda_packed_attention_grad_scratch_bytes(batch);
+    const int64_t need = grad_scratch_bytes(dtype, c.a, head_dim);
     if (!scratch_dev || !aligned16(scratch_dev) || scratch_bytes < need)
         return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: %lld bytes of scratch, %lld needed, on 16 bytes", what, static_cast<long long>(scratch_bytes), static_cast<long long>(need));
     c.lse = const_cast<float*>(lse_dev);

@@ -28,9 +28,12 @@ struct GradParams {
     const float2* stats;
     const uint32_t* norms;
     void *dq, *dk, *dv;
+    float* shares;   // where the rows of a tile of keys are cut into splits: their sums, [splits][dk, dv][tokens][kv_heads][head_dim]
+    int32_t splits;
     int64_t dq_token, dq_head, dk_token, dk_head, dv_token, dv_head;
     float scale, scale_log2;
     int32_t k_steps;  // head_dim / 16, rounded up
+    int32_t wide;     // results 32 bytes at a time
 };
 
 // The power of two of dS: 1 for bf16.
@@ -60,21 +63,6 @@ __device__ __forceinline__ void store_packed(uint32_t taddr, const float* w) {
 #pragma unroll
     for (int c = 0; c < 16; ++c) packed[c] = pack16<BF16>(w[2 * c], w[2 * c + 1]);
     tmem_st16(taddr, packed);
-}
-
-// 32 elements of a row's result, those below dim.
-template <bool BF16>
-__device__ __forceinline__ void store_result(uint8_t* to, const uint32_t* x, float factor, int c0, int dim) {
-#pragma unroll
-    for (int c = 0; c < 32; c += 8) {
-        if (c0 + c >= dim) continue;
-        uint4 w;
-        w.x = pack16<BF16>(__uint_as_float(x[c]) * factor, __uint_as_float(x[c + 1]) * factor);
-        w.y = pack16<BF16>(__uint_as_float(x[c + 2]) * factor, __uint_as_float(x[c + 3]) * factor);
-        w.z = pack16<BF16>(__uint_as_float(x[c + 4]) * factor, __uint_as_float(x[c + 5]) * factor);
-        w.w = pack16<BF16>(__uint_as_float(x[c + 6]) * factor, __uint_as_float(x[c + 7]) * factor);
-        *reinterpret_cast<uint4*>(to + (c0 + c) * 2) = w;
-    }
 }
 
 // One thread's products of a warp-uniform schedule.
@@ -129,6 +117,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
     __shared__ __align__(16) float minus_delta[kStages][128];
     __shared__ uint64_t bars[9 + 4 * kStages];
     __shared__ uint32_t tmem_slot;
+    __shared__ ItemRing ring;
     uint64_t* const kv_full = bars;
     uint64_t* const kv_empty = bars + 1;
     uint64_t* const s_full = bars + 2;    // scores of a block are in tensor memory
@@ -155,6 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
         mbar_init(sums_full, 1);
         mbar_init(sums_free, 8);
         mbar_init(own, 1);
+        ring.init(9);
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&q_full[s], 1);
             mbar_init(&g_full[s], 1);
@@ -179,9 +169,17 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
     const uint32_t tmem = tmem_slot;
     grid_dependency_wait();
     grid_dependency_release();
-    KeyWalk walk(p.a);
     KeyTile t;
     bool ok = true;
+    int4 entry;
+    int32_t part;
+    ItemSink sink(ring);
+    auto next = [&]() {
+        const bool more = sink.next(&entry, &part, &ok);
+        if (more) t = key_tile(p.a, p.splits, entry, part);
+        else if (!ok) kv_report(kWaitKeys + 13);
+        return more;
+    };
     auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
         if (ok && !mbar_wait(bar, parity)) {
             kv_report(kWaitKeys + where);
@@ -197,7 +195,12 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
             kv_report(kWaitKeys + 9);
             ok = false;
         };
-        while (ok && walk.next(&t)) {
+        ItemSource source(ring, p.a, true, p.a.kv_heads * p.splits);
+        auto take = [&]() { return source.next(&entry, &part, &ok, [](const int4&, int32_t) { return true; }); };
+        bool rest = take();
+        while (rest && ok) {
+            t = key_tile(p.a, p.splits, entry, part);
+            rest = take();
             for (int32_t b = t.b0; b < t.b1 && ok; ++b, ++block) {
                 const int stage = block % kStages;
                 const int32_t token0 = b * p.a.half_tokens, valid = min(rows, (t.n - token0) * p.a.group);
@@ -221,6 +224,10 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
                 if (lane == 0) mbar_arrive(&stats_full[stage]);
             }
         }
+        if (!ok) {
+            kv_report(kWaitKeys + 14);
+            source.drain();
+        }
     } else if (warp == 1) {
         // ---- MMA issuer
         const Issuer mma{p.k_steps};
@@ -237,7 +244,8 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
             mma.rows<D>(tmem + kP, v_addr, g_addr + at % kStages * L::kTile, idesc_rows);
             mma.commit(dp_full);
         };
-        while (ok && walk.next(&t)) {
+        while (ok && next()) {
+            if (t.b0 == t.b1) continue;
             if (!wait(kv_full, item & 1, 4)) break;
             scores(block);
             if (ok) grads(block);
@@ -268,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
         const float unit = unit_of<BF16>(p), from_dp = BF16 ? 1.f : unit / kUnit;
         const float2 from_dp2 = make_float2(from_dp, from_dp);
         uint32_t item = 0, block = 0;
-        while (ok && walk.next(&t)) {
+        while (ok && next()) {
             for (int32_t b = t.b0; b < t.b1; ++b, ++block) {
                 const int stage = block % kStages;
                 const int32_t token0 = b * p.a.half_tokens;
@@ -322,20 +330,41 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
                 if (lane == 0) mbar_arrive(ds_full);
             }
             // ---- results: the first warpgroup takes dV, the second dK
-            if (!wait(sums_full, item & 1, 12)) break;
+            const bool any = t.b0 < t.b1, mine = t.k0 + r < t.n;
+            if (!ok || (any && !wait(sums_full, item & 1, 12))) break;
             tc_fence_after();
-            const bool mine = t.k0 + r < t.n;
             const int64_t token = t.first + t.k0 + r;
-            uint8_t* const to = half == 0 ? static_cast<uint8_t*>(p.dv) + (token * p.dv_token + t.head * p.dv_head) * 2
-                                          : static_cast<uint8_t*>(p.dk) + (token * p.dk_token + t.head * p.dk_head) * 2;
             const float factor = half == 0 ? (BF16 ? 1.f : 1.f / kUnit) : p.scale / unit;
+            const uint32_t sums = tmem + lane_base + (half == 0 ? kDv : kDk);
+            if (p.splits > 1) {
+                float* const to = p.shares + (((static_cast<int64_t>(t.split) * 2 + 1 - half) * p.a.tokens + token) * p.a.kv_heads + t.head) * p.a.head_dim;
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 32) {
-                if (c0 >= p.a.head_dim) break;
-                uint32_t x[32];
-                tmem_ld32(tmem + lane_base + (half == 0 ? kDv : kDk) + c0, x);
-                tmem_ld_wait();
-                if (mine) store_result<BF16>(to, x, factor, c0, p.a.head_dim);
+                for (int c0 = 0; c0 < D; c0 += 32) {
+                    if (c0 >= p.a.head_dim) break;
+                    uint32_t x[32];
+                    if (any) {
+                        tmem_ld32(sums + c0, x);
+                        tmem_ld_wait();
+                    }
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4) {
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (any) v = make_float4(__uint_as_float(x[c]) * factor, __uint_as_float(x[c + 1]) * factor, __uint_as_float(x[c + 2]) * factor, __uint_as_float(x[c + 3]) * factor);
+                        if (mine && c0 + c < p.a.head_dim) *reinterpret_cast<float4*>(to + c0 + c) = v;
+                    }
+                }
+                if (!any) continue;
+            } else {
+                uint8_t* const to = half == 0 ? static_cast<uint8_t*>(p.dv) + (token * p.dv_token + t.head * p.dv_head) * 2
+                                              : static_cast<uint8_t*>(p.dk) + (token * p.dk_token + t.head * p.dk_head) * 2;
+#pragma unroll 1
+                for (int c0 = 0; c0 < D; c0 += 32) {
+                    if (c0 >= p.a.head_dim) break;
+                    uint32_t x[32];
+                    tmem_ld32(sums + c0, x);
+                    tmem_ld_wait();
+                    if (mine) store_result<BF16>(to, x, factor, c0, p.a.head_dim, p.wide != 0);
+                }
             }
             tc_fence_before();
             __syncwarp();
@@ -372,6 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     __shared__ uint64_t bars[14 + 2 * kKS + 2 * kVS];
     __shared__ uint32_t tmem_slot;
+    __shared__ ItemRing ring;
     uint64_t* const q_full = bars;
     uint64_t* const g_full = bars + 1;
     uint64_t* const qg_empty = bars + 2;
@@ -404,6 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
         mbar_init(sums_full, 1);
         mbar_init(sums_free, 8);
         mbar_init(own, 1);
+        ring.init(9);
         for (int s = 0; s < kKS; ++s) {
             mbar_init(&k_full[s], 1);
             mbar_init(&k_empty[s], 1);
@@ -424,9 +455,17 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
     const uint32_t tmem = tmem_slot;
     grid_dependency_wait();
     grid_dependency_release();
-    RowWalk walk(p.a, 1);
     RowTile t;
     bool ok = true;
+    int4 entry;
+    int32_t part;
+    ItemSink sink(ring);
+    auto next = [&]() {
+        const bool more = sink.next(&entry, &part, &ok);
+        if (more) t = row_tile(p.a, true, entry, part);
+        else if (!ok) kv_report(kWaitQueries + 14);
+        return more;
+    };
     auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
         if (ok && !mbar_wait(bar, parity)) {
             kv_report(kWaitQueries + where);
@@ -442,7 +481,12 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
             kv_report(kWaitQueries + 9);
             ok = false;
         };
-        while (ok && walk.next(&t)) {
+        ItemSource source(ring, p.a, false, p.a.kv_heads * 2);
+        auto take = [&]() { return source.next(&entry, &part, &ok, [&](const int4& e, int32_t i) { return row_tile(p.a, true, e, i).nblk > 0; }); };
+        bool rest = take();
+        while (rest && ok) {
+            t = row_tile(p.a, true, entry, part);
+            rest = take();
             for (int32_t b = 0; b < t.nblk && ok; ++b, ++block) {
                 const int32_t valid = t.n - b * kKeyTile, ks = block % kKS, vs = block % kVS;
                 if (!wait(&k_empty[ks], (block / kKS & 1) ^ 1, 0)) break;
@@ -456,6 +500,10 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
                 if (!wait(&v_empty[vs], (block / kVS & 1) ^ 1, 2)) break;
                 if (!load_tile<kPanels>(smem + L::kV + vs * L::kTile, &map_v, &v_full[vs], own, &own_phase, kKeyTile, valid, true, t.head, t.first + b * kKeyTile, 0)) failed();
             }
+        }
+        if (!ok) {
+            kv_report(kWaitQueries + 9);
+            source.drain();
         }
     } else if (warp == 1) {
         // ---- MMA issuer
@@ -475,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
             mma.commit(&dp_full[at & 1]);
             mma.commit(&v_empty[at % kVS]);
         };
-        while (ok && walk.next(&t)) {
+        while (ok && next()) {
             if (!wait(q_full, item & 1, 5)) break;
             scores(block);
             if (!wait(g_full, item & 1, 6)) break;
@@ -504,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
         const float unit = unit_of<BF16>(p);
         const int32_t row_token = r / p.a.group, row_head = r - row_token * p.a.group;
         uint32_t item = 0, block = 0;
-        while (ok && walk.next(&t)) {
+        while (ok && next()) {
             const int32_t i = t.t0 + row_token, last = p.a.causal ? min(t.n - 1, i) : t.n - 1;
             const bool mine = r < rows && i < t.n;
             const int64_t token = t.first + i;
@@ -567,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
                 uint32_t x[32];
                 tmem_ld32(tmem + lane_base + kDq + c0, x);
                 tmem_ld_wait();
-                if (mine) store_result<BF16>(to, x, factor, c0, p.a.head_dim);
+                if (mine) store_result<BF16>(to, x, factor, c0, p.a.head_dim, p.wide != 0);
             }
             tc_fence_before();
             __syncwarp();
@@ -603,18 +651,21 @@ int launch(const PackedCall& c, cudaStream_t stream) {
     p.scale = c.scale;
     p.scale_log2 = c.scale * kLog2e;
     p.k_steps = (a.head_dim + 15) / 16;
+    p.wide = on_wide_grid(c.dq, a.head_dim, a.tokens, a.q_heads) && on_wide_grid(c.dk, a.head_dim, a.tokens, a.kv_heads) && on_wide_grid(c.dv, a.head_dim, a.tokens, a.kv_heads);
+    p.splits = key_splits_tc(a);
+    p.shares = c.shares();
     static std::atomic<bool> keys_allowed[64], queries_allowed[64];
     auto keys = key_grads_kernel<D, BF16>;
     auto queries = query_grads_kernel<D, BF16>;
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(keys), KeySmem<D>::kTotal, keys_allowed)) return st;
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(queries), QuerySmem<D>::kTotal, queries_allowed)) return st;
-    const auto grid = [](int64_t items) { return dim3(static_cast<unsigned>(std::min<int64_t>(kNumSMs, items))); };
-    cudaError_t e = launch_dependent(keys, grid(static_cast<int64_t>(a.key_capacity) * a.kv_heads), dim3(kThreads), KeySmem<D>::kTotal, stream, 1, true, mq, mk, mv, mg, p);
+    const auto grid = [](int64_t items) { return dim3(static_cast<unsigned>(items)); };
+    cudaError_t e = launch_dependent(keys, grid(static_cast<int64_t>(a.key_capacity) * a.kv_heads * p.splits), dim3(kThreads), KeySmem<D>::kTotal, stream, 1, true, mq, mk, mv, mg, p);
     if (e == cudaSuccess)
         e = launch_dependent(queries, grid(2 * static_cast<int64_t>(a.row_capacity) * a.kv_heads), dim3(kThreads), QuerySmem<D>::kTotal, stream, 1, true, mq, mk, mv, mg, p);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of packed_attention_grad failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("packed_attention_grad");
-    return MHLO_CUDA_OK;
+    return p.splits > 1 ? packed_join_shares(c, p.splits, stream) : MHLO_CUDA_OK;
 }
 
 }  // namespace

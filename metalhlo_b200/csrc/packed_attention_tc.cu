@@ -1,7 +1,7 @@
 // Attention over packed sequences on tcgen05: o = softmax(scale q k^T) v for bf16 / f16, head dimensions up to 128, grouped heads,
 // causal or not, with the logarithms of the sums of exponentials. Scores do not leave the SM.
 //
-// A CTA takes items (tile of stacked query rows, head of keys) from the batch's plan, longest first. A tile is two halves of 128 rows:
+// A CTA takes items (tile of stacked query rows, head of keys) in the order of the batch's plan. A tile is two halves of 128 rows:
 //   warp 0             producer: rows of q, then blocks of 128 keys and values through rings of two stages
 //   warp 1             MMA issuer: S_h = Q_h K^T (both in shared memory), O_h += P_h V (P in tensor memory); one half's products run
 //                      under the other's exponentials
@@ -27,6 +27,8 @@ struct ForwardParams {
     float scale_log2;
     int32_t k_steps;    // head_dim / 16, rounded up
     int32_t one_half;   // items are half tiles: few rows, more CTAs
+    int32_t wide;       // results 32 bytes at a time
+    FastDiv by_group;
 };
 
 template <int D>
@@ -46,15 +48,21 @@ __device__ __forceinline__ uint32_t scale16x2(uint32_t v, float a) {
     }
 }
 
-// Weights of 64 scores, packed, and their sum: 2^(s * scale_log2 - m). MASK: scores of keys behind last become -infinity.
-template <bool BF16, bool MASK>
-__device__ __forceinline__ void weights(uint32_t* sr, float scale_log2, float m, int32_t key0, int32_t last, uint32_t* packed, float2* sums) {
-    const float2 c2 = make_float2(scale_log2, scale_log2), m2 = make_float2(-m, -m);
-    if (MASK) {
+// Scores of 64 keys behind number `last` become -infinity.
+__device__ __forceinline__ void hide(uint32_t* sr, int32_t last) {
+    const uint64_t seen = last < 0 ? 0 : last >= 63 ? ~0ull : (2ull << last) - 1;
+    const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
-            if (key0 + c > last) sr[c] = 0xff800000u;
+    for (int c = 0; c < 32; ++c) {
+        if (!(lo >> c & 1)) sr[c] = 0xff800000u;
+        if (!(hi >> c & 1)) sr[c + 32] = 0xff800000u;
     }
+}
+
+// Weights of 64 scores, packed, and their sum: 2^(s * scale_log2 - m).
+template <bool BF16>
+__device__ __forceinline__ void weights(const uint32_t* sr, float scale_log2, float m, uint32_t* packed, float2* sums) {
+    const float2 c2 = make_float2(scale_log2, scale_log2), m2 = make_float2(-m, -m);
 #pragma unroll
     for (int c = 0; c < 64; c += 2) {
         const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), c2, m2);
@@ -74,12 +82,6 @@ __device__ __forceinline__ float largest(const uint32_t* sr) {
     return fmaxf(a, b);
 }
 
-__device__ __forceinline__ void load64(uint32_t taddr, uint32_t* r) {
-    tmem_ld32(taddr, r);
-    tmem_ld32(taddr + 32, r + 32);
-    tmem_ld_wait();
-}
-
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                        const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ForwardParams p) {
@@ -93,6 +95,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     __shared__ uint64_t bars[7 * kHalves + 4 * kStages + 1];
     __shared__ uint32_t tmem_slot;
+    __shared__ ItemRing ring;
     uint64_t* const q_full = bars;                 // per half: the tile's rows of q are in shared memory
     uint64_t* const q_empty = q_full + kHalves;    // per half: their last product is done
     uint64_t* const s_full = q_empty + kHalves;    // per half: scores of a block are in tensor memory
@@ -126,6 +129,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
             mbar_init(&v_empty[s], 1);
         }
         mbar_init(own, 1);
+        ring.init(9);
         fence_barrier_init();
     }
     if (warp == 1) {
@@ -144,8 +148,16 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
     const uint32_t tmem = tmem_slot;
     grid_dependency_wait();
     grid_dependency_release();
-    RowWalk walk(p.a, p.one_half);
     bool ok = true;
+    int4 entry;
+    int32_t part;
+    ItemSink sink(ring);
+    auto next = [&](RowTile* t) {
+        const bool more = sink.next(&entry, &part, &ok);
+        if (more) *t = row_tile(p.a, p.one_half != 0, entry, part);
+        else if (!ok) kv_report(kWaitError + 13);
+        return more;
+    };
     auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
         if (ok && !mbar_wait(bar, parity)) {
             kv_report(kWaitError + where);
@@ -156,10 +168,14 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
 
     if (warp == 0) {
         // ---- producer
-        RowTile t;
         int stage = 0;
         uint32_t phase = 0, own_phase = 0, q_of[kHalves] = {0, 0};
-        while (ok && walk.next(&t)) {
+        ItemSource source(ring, p.a, false, p.a.kv_heads * (p.one_half ? 2 : 1));
+        auto take = [&]() { return source.next(&entry, &part, &ok, [&](const int4& e, int32_t i) { return row_tile(p.a, p.one_half != 0, e, i).nblk > 0; }); };
+        bool more = take();
+        while (more && ok) {
+            const RowTile t = row_tile(p.a, p.one_half != 0, entry, part);
+            more = take();
             for (int h = 0; h < kHalves; ++h) {
                 if (t.nb[h] == 0) continue;
                 if (!wait(&q_empty[h], (q_of[h]++ & 1) ^ 1, 0)) break;
@@ -175,6 +191,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                 }
                 if (++stage == kStages) stage = 0, phase ^= 1;
             }
+        }
+        if (!ok) {
+            kv_report(kWaitError + 14);
+            source.drain();
         }
     } else if (warp == 1) {
         // ---- MMA issuer
@@ -207,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
             commit_to(&pv_done[h]);
         };
         RowTile cur, nxt;
-        bool has = walk.next(&cur);
+        bool has = next(&cur);
         uint32_t block = 0;                              // blocks of keys so far
         uint32_t s_of[kHalves] = {0, 0}, p_of[kHalves] = {0, 0}, q_of[kHalves] = {0, 0};
         // The scores of block j of tile t, half h (whose turn it is), with the waits for what they read.
@@ -238,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
         // Order on the pipe, which runs one thread's products in turn. Weights over the scores: PV_0(j), S_0(next), PV_1(j), S_1(next), so
         // that scores replace weights that have been read. Beside them: S_0(next), S_1(next), PV_0(j), PV_1(j).
         while (has && ok) {
-            const bool more_tiles = walk.next(&nxt);
+            const bool more_tiles = next(&nxt);
             for (int j = 0; j < cur.nblk && ok; ++j, ++block) {
                 const bool last = j + 1 == cur.nblk;
                 const RowTile& next = last ? nxt : cur;
@@ -262,20 +282,22 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
         const int h = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t s_taddr = tmem + lane_base + kSCol + h * 128, o_taddr = tmem + lane_base + kOCol + h * D, p_taddr = tmem + lane_base + kPCol + h * kPStride;
-        const int32_t row_token = r / p.a.group, row_head = r - row_token * p.a.group;
+        uint32_t row_token, row_head;
+        p.by_group.divmod(r, &row_token, &row_head);
         RowTile t;
         uint32_t it = 0;  // blocks of this half so far
-        while (ok && walk.next(&t)) {
+        while (ok && next(&t)) {
             const int32_t i = t.t0 + h * p.a.half_tokens + row_token;  // the row's token
             const int32_t last = p.a.causal ? min(t.n - 1, i) : t.n - 1;
+            const bool mine = r < rows && i < t.n;
             const int nb = t.nb[h];
+            // what the warp's first and last row see: tokens ascend with the rows
+            const int32_t least = __shfl_sync(0xffffffffu, last, 0), most = __shfl_sync(0xffffffffu, last, 31);
             float m_ref = -INFINITY, l = 0.f;
             for (int j = 0; j < nb; ++j, ++it) {
                 if (!wait(&s_full[h], it & 1, 9)) break;
                 tc_fence_after();
                 const int32_t key0 = j * kKeyTile;
-                // one decision a warp: loads and stores of tensor memory are warp-wide
-                const bool mask = __any_sync(0xffffffffu, key0 + kKeyTile - 1 > last);
                 float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                 if constexpr (kBeside) {
                     bool pv_waited = it == 0;  // for the product of the block before this one, which reads its weights and adds to O
@@ -288,11 +310,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                             __syncwarp();
                             if (lane == 0) mbar_arrive(&s_free[h]);
                         }
-                        if (mask) {
-#pragma unroll
-                            for (int c = 0; c < 64; ++c)
-                                if (key0 + ci * 64 + c > last) sr[c] = 0xff800000u;
-                        }
+                        // one decision a warp: loads and stores of tensor memory are warp-wide
+                        if (key0 + ci * 64 + 63 > least) hide(sr, last - key0 - ci * 64);
                         const float mx = largest(sr) * p.scale_log2;
                         const bool grow = mx > m_ref + kGrowth;
                         if (__any_sync(0xffffffffu, grow)) {
@@ -323,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                                 }
                             }
                         }
-                        weights<BF16, false>(sr, p.scale_log2, m_ref == -INFINITY ? 0.f : m_ref, 0, 0, packed, sums);
+                        weights<BF16>(sr, p.scale_log2, m_ref == -INFINITY ? 0.f : m_ref, packed, sums);
                         if (!pv_waited) {
                             if (!wait(&pv_done[h], (it - 1) & 1, 11)) break;
                             tc_fence_after();
@@ -334,38 +353,40 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                     if (!ok) break;
                     l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
                 } else {
-                    // Against the maximum of earlier blocks first: nothing is written until the warp's sums have shown that no weight is
-                    // too large for 16 bits. Otherwise (first blocks, and where scores have grown) the block's own maximum is found.
+                    // Against the maximum of earlier blocks, in a tile's first block that of its first 64 keys: nothing is written until the
+                    // warp's sums have shown that no weight is too large for 16 bits. Otherwise the block's own maximum is found first.
                     uint32_t packed[2][32];
                     bool done = false;
-                    if (j > 0) {
-                        const float m = m_ref == -INFINITY ? 0.f : m_ref;
+                    float m_try = m_ref;
 #pragma unroll
-                        for (int ci = 0; ci < 2; ++ci) {
-                            uint32_t sr[64];
-                            load64(s_taddr + ci * 64, sr);
-                            if (mask) weights<BF16, true>(sr, p.scale_log2, m, key0 + ci * 64, last, packed[ci], sums);
-                            else weights<BF16, false>(sr, p.scale_log2, m, 0, 0, packed[ci], sums);
-                        }
-                        const float sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
-                        done = !__any_sync(0xffffffffu, !(sum < kCarry));
-                        if (done) {
-                            l += sum;
+                    for (int ci = 0; ci < 2; ++ci) {
+                        if (key0 + ci * 64 > most) {  // no row of the warp sees any of these
 #pragma unroll
-                            for (int ci = 0; ci < 2; ++ci) tmem_st32(p_taddr + ci * 32, packed[ci]);
+                            for (int c = 0; c < 32; ++c) packed[ci][c] = 0;
+                            continue;
                         }
+                        uint32_t sr[64];
+                        load64(s_taddr + ci * 64, sr);
+                        if (key0 + ci * 64 + 63 > least) hide(sr, last - key0 - ci * 64);
+                        if (ci == 0 && j == 0) m_try = largest(sr) * p.scale_log2;
+                        weights<BF16>(sr, p.scale_log2, m_try == -INFINITY ? 0.f : m_try, packed[ci], sums);
+                    }
+                    const float sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+                    done = !__any_sync(0xffffffffu, mine && !(sum < kCarry));  // rows that are another sequence's have no say
+                    if (done) {
+                        l += sum;
+                        m_ref = m_try;
+#pragma unroll
+                        for (int ci = 0; ci < 2; ++ci) tmem_st32(p_taddr + ci * 32, packed[ci]);
                     }
                     if (!done) {
                         float mx = -INFINITY;
 #pragma unroll 1
                         for (int ci = 0; ci < 2; ++ci) {
                             uint32_t sr[64];
+                            if (key0 + ci * 64 > most) break;
                             load64(s_taddr + ci * 64, sr);
-                            if (mask) {
-#pragma unroll
-                                for (int c = 0; c < 64; ++c)
-                                    if (key0 + ci * 64 + c > last) sr[c] = 0xff800000u;
-                            }
+                            if (key0 + ci * 64 + 63 > least) hide(sr, last - key0 - ci * 64);
                             mx = fmaxf(mx, largest(sr));
                         }
                         mx *= p.scale_log2;
@@ -394,7 +415,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                         for (int ci = 0; ci < 2; ++ci) {  // the weights lie over scores that have been read
                             uint32_t sr[64];
                             load64(s_taddr + ci * 64, sr);
-                            weights<BF16, true>(sr, p.scale_log2, m, key0 + ci * 64, last, packed[0], sums);
+                            if (key0 + ci * 64 + 63 > least) hide(sr, last - key0 - ci * 64);
+                            weights<BF16>(sr, p.scale_log2, m, packed[0], sums);
                             tmem_st32(p_taddr + ci * 32, packed[0]);
                         }
                         l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
@@ -409,7 +431,6 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
             // ---- results. The next tile's first product with values waits for weights that these warps write after this.
             if (!wait(&pv_done[h], (it - 1) & 1, 12)) break;
             tc_fence_after();
-            const bool mine = r < rows && i < t.n;
             const int64_t token = t.first + i, head = t.head * p.a.group + row_head;
             const float inv = l == 0.f ? 0.f : 1.f / l;
             uint8_t* const to = static_cast<uint8_t*>(p.o) + (token * p.os_token + head * p.os_head) * 2;
@@ -419,16 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                 uint32_t x[32];
                 tmem_ld32(o_taddr + c0, x);
                 tmem_ld_wait();
-#pragma unroll
-                for (int c = 0; c < 32; c += 8) {
-                    if (!mine || c0 + c >= p.a.head_dim) continue;
-                    uint4 w;
-                    w.x = pack16<BF16>(__uint_as_float(x[c]) * inv, __uint_as_float(x[c + 1]) * inv);
-                    w.y = pack16<BF16>(__uint_as_float(x[c + 2]) * inv, __uint_as_float(x[c + 3]) * inv);
-                    w.z = pack16<BF16>(__uint_as_float(x[c + 4]) * inv, __uint_as_float(x[c + 5]) * inv);
-                    w.w = pack16<BF16>(__uint_as_float(x[c + 6]) * inv, __uint_as_float(x[c + 7]) * inv);
-                    *reinterpret_cast<uint4*>(to + (c0 + c) * 2) = w;
-                }
+                if (mine) store_result<BF16>(to, x, inv, c0, p.a.head_dim, p.wide != 0);
             }
             if (mine && p.lse != nullptr) p.lse[token * p.a.q_heads + head] = l == 0.f ? -INFINITY : (m_ref + log2f(l)) * kLn2;
         }
@@ -460,10 +472,12 @@ int launch(const PackedCall& c, cudaStream_t stream) {
     p.k_steps = (a.head_dim + 15) / 16;
     const int64_t items = static_cast<int64_t>(a.row_capacity) * a.kv_heads;
     p.one_half = 2 * items <= kNumSMs;
+    p.wide = on_wide_grid(c.o, a.head_dim, a.tokens, a.q_heads);
+    p.by_group = FastDiv(static_cast<uint32_t>(a.group));
     static std::atomic<bool> allowed[64];
     auto kernel = packed_attention_kernel<D, BF16>;
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), L::kTotal, allowed)) return st;
-    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(kNumSMs, items * (p.one_half ? 2 : 1)));
+    const unsigned grid = static_cast<unsigned>(items * (p.one_half ? 2 : 1));
     const cudaError_t e = launch_dependent(kernel, dim3(grid), dim3(kThreads), L::kTotal, stream, 1, grid < kNumSMs, mq, mk, mv, p);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of packed_attention failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("packed_attention");

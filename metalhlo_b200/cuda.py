@@ -222,7 +222,7 @@ _PROTOTYPES = {
     "mhlo_cuda_packed_plan_bytes": (_i64, [C.POINTER(PackedBatchArgs)]),
     "mhlo_cuda_packed_plan": (C.c_int, [C.POINTER(PackedBatchArgs), _vp]),
     "mhlo_cuda_packed_attention": (C.c_int, [_i32, C.POINTER(PackedBatchArgs), _i64, _f32] + [_vp, C.POINTER(_i64)] * 4 + [_vp, _vp]),
-    "mhlo_cuda_packed_attention_grad_scratch_bytes": (_i64, [C.POINTER(PackedBatchArgs)]),
+    "mhlo_cuda_packed_attention_grad_scratch_bytes": (_i64, [_i32, C.POINTER(PackedBatchArgs), _i64]),
     "mhlo_cuda_packed_attention_grad": (C.c_int, [_i32, C.POINTER(PackedBatchArgs), _i64, _f32] + [_vp, C.POINTER(_i64)] * 4 + [_vp] +
                                         [_vp, C.POINTER(_i64)] * 4 + [_vp, _i64, _vp]),
     "mhlo_cuda_token_logprobs": (C.c_int, [_i32, _vp, _i64, _i64, _i64, _f32, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
@@ -717,7 +717,14 @@ class PackedPlan:
         self.pointer = C.byref(self._args)
         self.device = starts.device
         self.tiles = None
-        self.scratch_bytes = lib.mhlo_cuda_packed_attention_grad_scratch_bytes(self.pointer)
+        self._scratch = {}
+
+    def scratch_bytes(self, dtype: int, dim: int) -> int:
+        """Of the backward half for this type and head dimension."""
+        need = self._scratch.get((dtype, dim))
+        if need is None:
+            need = self._scratch[dtype, dim] = lib.mhlo_cuda_packed_attention_grad_scratch_bytes(dtype, self.pointer, dim)
+        return need
 
 
 def packed_plan(starts, tokens: int, q_heads: int, kv_heads: int, causal: bool = True, stream=None) -> PackedPlan:
@@ -775,10 +782,12 @@ def packed_attention_grad(q, k, v, out, lse, grad_out, plan: PackedPlan, scale: 
 
     def call(s):
         grads = [_dense_like(like) if t is None else t for t, like in ((dq, q), (dk, k), (dv, v))]
-        scratch = lse.new_empty(plan.scratch_bytes >> 2) if plan.scratch_bytes else None
-        check(lib.mhlo_cuda_packed_attention_grad(torch_dtype_code(q.dtype), plan.pointer, dim, scale, q.data_ptr(), _rows(q), k.data_ptr(), _rows(k),
+        code = torch_dtype_code(q.dtype)
+        need = plan.scratch_bytes(code, dim)
+        scratch = lse.new_empty((need + 3) >> 2) if need else None
+        check(lib.mhlo_cuda_packed_attention_grad(code, plan.pointer, dim, scale, q.data_ptr(), _rows(q), k.data_ptr(), _rows(k),
                                                   v.data_ptr(), _rows(v), out.data_ptr(), _rows(out), lse.data_ptr(), grad_out.data_ptr(), _rows(grad_out),
-                                                  *(x for t in grads for x in (t.data_ptr(), _rows(t))), _ptr(scratch), plan.scratch_bytes, s))
+                                                  *(x for t in grads for x in (t.data_ptr(), _rows(t))), _ptr(scratch), need, s))
         return tuple(grads)
 
     return _run_on(q.device, stream, call)

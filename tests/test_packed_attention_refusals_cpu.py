@@ -59,11 +59,11 @@ def test_results_that_overlap():
 def test_grad():
     for name in ("g", "dq", "dk", "dv", "lse"):
         assert grad(**{name: None}) == INVALID
-    need = cuda.lib.mhlo_cuda_packed_attention_grad_scratch_bytes(C.byref(batch()))
+    need = cuda.lib.mhlo_cuda_packed_attention_grad_scratch_bytes(cuda.BF16, C.byref(batch()), 64)
     assert need >= 100 * 4 * 8
     assert grad(size=need - 1) == INVALID and "scratch" in cuda.last_error()
     assert grad(scratch=None) == INVALID and grad(scratch=P + 4) == INVALID
-    assert cuda.lib.mhlo_cuda_packed_attention_grad_scratch_bytes(None) == 0
+    assert cuda.lib.mhlo_cuda_packed_attention_grad_scratch_bytes(cuda.BF16, None, 64) == 0 and cuda.lib.mhlo_cuda_packed_attention_grad_scratch_bytes(cuda.BF16, C.byref(batch()), 0) == 0
 
 
 def test_plan():
