@@ -10,34 +10,69 @@ namespace mhlo {
 namespace {
 
 // ---- the plan ---------------------------------------------------------------------------------------------------------------------
-// A CTA for each run of sequences, those whose first tokens lie in its run_tokens: it counts the tiles in front of its own, then its own by the
-// 128-token blocks they meet, scans, and puts them in place, longest first. The order of tiles of one length goes by arrival; no result depends
-// on it. 32 sequences of 1024 tokens take 5 us, once for all layers of a step.
-constexpr int kBuckets = 2048, kPlanThreads = 1024;
+// Tiles that meet more than a kLong-th of what a CTA of a full grid would meet altogether go first, longest first, wherever they are from: late in the
+// order they would keep one CTA busy when the others are done. The rest goes run by run. The first CTA places the long tiles, each other one
+// those of its run of sequences (first tokens inside run_tokens): it counts the tiles in front of its own, then its own by the 128-token
+// blocks they meet, scans, and puts them in place. The order of tiles of one length goes by arrival; no result depends on it. 32 sequences of
+// 1024 tokens take 6 us, once for all layers of a step.
+constexpr int kBuckets = 2048, kPlanThreads = 1024, kLong = 16;
 
 __device__ __forceinline__ int32_t bucket_of(int32_t tokens) { return kBuckets - 1 - min((tokens - 1) >> 7, kBuckets - 1); }
+
+// Tiles of a list, `step` tokens each, of a sequence of n tokens.
+struct TilesOf {
+    int32_t n, step;
+    bool ascending, causal;  // ascending: later tiles meet more
+    __device__ __forceinline__ int32_t all() const { return (n + step - 1) / step; }
+    __device__ __forceinline__ int32_t meets(int32_t at) const { return !causal ? n : ascending ? static_cast<int32_t>(min(static_cast<int64_t>(n), static_cast<int64_t>(at) + step)) : n - at; }
+    __device__ __forceinline__ unsigned long long sum() const {  // nearly, of what they meet
+        return static_cast<unsigned long long>(all()) * (causal ? (static_cast<unsigned long long>(n) + step + 1) / 2 : n);
+    }
+    __device__ __forceinline__ int32_t above(int32_t most) const {  // how many meet more
+        if (n <= most) return 0;
+        return !causal ? all() : ascending ? all() - min(all(), most / step) : (n - most + step - 1) / step;
+    }
+};
 
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a) {
     __shared__ int32_t counts[2][kBuckets];
     __shared__ int32_t sums[2][32], before[2], all[2];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ unsigned long long work[2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, run = static_cast<int>(blockIdx.x) - 1;
+    const bool causal = a.causal != 0;
     const int32_t steps[2] = {2 * a.half_tokens, kKeyTile};
     for (int i = tid; i < 2 * kBuckets; i += kPlanThreads) counts[0][i] = 0;
-    if (tid < 2) before[tid] = all[tid] = 0;
+    if (tid < 2) before[tid] = all[tid] = 0, work[tid] = 0;
     __syncthreads();
-    // tiles of the runs in front of this one, and of all
+    const auto sequence = [&](int32_t b, int32_t* first) {  // its tokens
+        const int32_t end = a.starts[b + 1];
+        *first = a.starts[b];
+        return *first < 0 || end > a.tokens || end < *first ? -1 : end - *first;
+    };
+    for (int32_t b = tid; b < a.seqs; b += kPlanThreads) {
+        int32_t first;
+        const int32_t n = sequence(b, &first);
+        if (n < 0) kv_report(MHLO_CUDA_KV_ERROR_STARTS);
+        if (n <= 0) continue;
+#pragma unroll
+        for (int list = 0; list < 2; ++list) atomicAdd(&work[list], TilesOf{n, steps[list], list == 0, causal}.sum());
+    }
+    __syncthreads();
+    int32_t most[2];  // that tiles of the runs meet
+#pragma unroll
+    for (int list = 0; list < 2; ++list) most[list] = static_cast<int32_t>(min(work[list] * a.kv_heads / (kLong * kNumSMs), static_cast<unsigned long long>(1) << 30));
+    // tiles in front of this CTA's, and of all
     int32_t mine[2] = {0, 0}, total[2] = {0, 0};
     for (int32_t b = tid; b < a.seqs; b += kPlanThreads) {
-        const int32_t first = a.starts[b], end = a.starts[b + 1];
-        if (first < 0 || end > a.tokens || end < first) {
-            kv_report(MHLO_CUDA_KV_ERROR_STARTS);
-            continue;
-        }
+        int32_t first;
+        const int32_t n = sequence(b, &first);
+        if (n <= 0) continue;
 #pragma unroll
         for (int list = 0; list < 2; ++list) {
-            const int32_t tiles = (end - first + steps[list] - 1) / steps[list];
+            const TilesOf t{n, steps[list], list == 0, causal};
+            const int32_t tiles = t.all(), above = t.above(most[list]);
             total[list] += tiles;
-            if (first / a.run_tokens < static_cast<int32_t>(blockIdx.x)) mine[list] += tiles;
+            if (run >= 0) mine[list] += above + (first / a.run_tokens < run ? tiles - above : 0);
         }
     }
 #pragma unroll
@@ -52,14 +87,15 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a)
     __syncthreads();
     for (int place = 0; place < 2; ++place) {
         for (int32_t b = warp; b < a.seqs; b += 32) {
-            const int32_t first = a.starts[b], end = a.starts[b + 1];
-            if (first < 0 || end > a.tokens || end < first || first / a.run_tokens != static_cast<int32_t>(blockIdx.x)) continue;
-            const int32_t n = end - first;
+            int32_t first;
+            const int32_t n = sequence(b, &first);
+            if (n <= 0 || (run >= 0 && first / a.run_tokens != run)) continue;
 #pragma unroll
             for (int list = 0; list < 2; ++list) {
+                const TilesOf t{n, steps[list], list == 0, causal};
                 for (int64_t z = static_cast<int64_t>(lane) * steps[list]; z < n; z += 32 * steps[list]) {
-                    const int32_t at = static_cast<int32_t>(z);
-                    const int32_t meets = !a.causal ? n : list == 0 ? static_cast<int32_t>(min(static_cast<int64_t>(n), z + steps[0])) : n - at;
+                    const int32_t at = static_cast<int32_t>(z), meets = t.meets(at);
+                    if ((meets > most[list]) != (run < 0)) continue;
                     const int32_t slot = atomicAdd(&counts[list][bucket_of(meets)], 1);
                     if (place == 0) continue;
                     // starts that go back on earlier ones can make more tiles than there is room for
@@ -810,7 +846,7 @@ int mhlo_cuda_packed_plan(const mhlo_cuda_packed_batch* batch, mhlo_cuda_stream_
     if (int st = packed_args("packed_plan", batch, &a)) return st;
     if (a.seqs == 0 || a.tokens == 0) return MHLO_CUDA_OK;
     if (!a.starts || !a.plan || !aligned16(a.plan)) return fail(MHLO_CUDA_INVALID_ARGUMENT, "packed_plan: null starts, or null or unaligned plan");
-    packed_plan_kernel<<<static_cast<unsigned>((a.tokens + a.run_tokens - 1) / a.run_tokens), kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    packed_plan_kernel<<<static_cast<unsigned>(1 + (a.tokens + a.run_tokens - 1) / a.run_tokens), kPlanThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
     MHLO_CUDA_CHECK_LAUNCH("packed_plan");
     return MHLO_CUDA_OK;
 }

@@ -16,8 +16,8 @@ constexpr int kKeyTile = 128;     // keys of a block, and of a tile of the gradi
 constexpr int kPlanMagic = 0x506c616e;
 
 // The plan in device memory: a header, then the tiles of query rows, then the tiles of keys, each {first token of the sequence, its tokens,
-// first token of the tile inside it, 0}. Sequences go by runs whose keys and values stay in L2 together (run_tokens), and inside a run tiles
-// go in descending order of the tokens that they meet. In one order for all, 64 sequences of 512 tokens read 603 MB where they have 403.
+// first token of the tile inside it, 0}: long tiles first, then runs of sequences whose keys and values stay in L2 together (run_tokens), inside
+// a run in descending order of the tokens that they meet. In one order for all, 64 sequences of 512 tokens read 603 MB where they have 403.
 struct PlanHeader {
     int32_t magic, tokens, q_heads, kv_heads, causal, row_tiles, key_tiles;
     int32_t first, end;  // rows of the sequences
