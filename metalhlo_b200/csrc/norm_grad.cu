@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(kJoin) norm_grad_join_kernel(const float* part
     const int64_t column = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     float sum = 0.f;
     if (column < width) {
-#pragma unroll 4
+#pragma unroll 8
         for (int32_t i = warp; i < parts; i += 32) sum += partial[static_cast<int64_t>(i) * width + column];
     }
     sums[warp][lane] = sum;
@@ -580,11 +580,10 @@ int join(const float* partial, int64_t parts, int64_t hidden, float* dgamma, flo
     return MHLO_CUDA_OK;
 }
 
+// per_sm: CTAs that an SM takes.
 template <bool RMS, typename K, typename T, typename... Args>
-int launch(K kernel, const NormGradParams<T>& p, int threads, int rows_of_cta, size_t smem, float* dgamma, float* dbeta, cudaStream_t stream, Args... args) {
-    int per_sm = 0;
-    MHLO_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem), MHLO_CUDA_EXECUTION_FAILED);
-    const int64_t grid = std::min<int64_t>((p.rows + rows_of_cta - 1) / rows_of_cta, std::min<int64_t>(kMostCtas, static_cast<int64_t>(std::max(per_sm, 1)) * kNumSMs));
+int launch(K kernel, const NormGradParams<T>& p, int threads, int rows_of_cta, size_t smem, int per_sm, float* dgamma, float* dbeta, cudaStream_t stream, Args... args) {
+    const int64_t grid = std::min<int64_t>((p.rows + rows_of_cta - 1) / rows_of_cta, std::min<int64_t>(kMostCtas, static_cast<int64_t>(per_sm) * kNumSMs));
     const cudaError_t e = launch_dependent(kernel, dim3(static_cast<unsigned>(grid)), dim3(static_cast<unsigned>(threads)), smem, stream, 1, grid < kNumSMs, p, args...);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of norm_grad failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("norm_grad");
@@ -593,7 +592,7 @@ int launch(K kernel, const NormGradParams<T>& p, int threads, int rows_of_cta, s
 
 template <typename T, int W, int N, bool RMS>
 int warp_rows(const NormGradParams<T>& p, float* dgamma, float* dbeta, cudaStream_t stream) {
-    return launch<RMS>(norm_grad_warp_kernel<T, W, N, RMS>, p, kWarpThreads, kWarpThreads / 32, 2 * static_cast<size_t>(p.hidden) * sizeof(float), dgamma, dbeta, stream);
+    return launch<RMS>(norm_grad_warp_kernel<T, W, N, RMS>, p, kWarpThreads, kWarpThreads / 32, 2 * static_cast<size_t>(p.hidden) * sizeof(float), 2, dgamma, dbeta, stream);
 }
 
 // Shared memory of an SM for the rings of all its CTAs.
@@ -608,7 +607,7 @@ int cta_rows_of(const NormGradParams<T>& p, float* dgamma, float* dbeta, cudaStr
     const int stages = std::max(2 * R, std::min(kMostStages, kRingBytes / ctas / stage));  // the rows at hand, and the next ones
     static std::atomic<bool> allowed[64];
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), kRingBytes, allowed)) return st;
-    return launch<RMS>(kernel, p, threads, 1, static_cast<size_t>(stages) * stage, dgamma, dbeta, stream, stages);
+    return launch<RMS>(kernel, p, threads, 1, static_cast<size_t>(stages) * stage, std::min(ctas, std::max(1, kRingBytes / (stages * stage))), dgamma, dbeta, stream, stages);
 }
 // 512 threads an SM, of 128 registers, up to 8192 elements.
 template <typename T, bool VEC, bool RMS>

@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
+#include <type_traits>
 
 #include "packed_attention.cuh"
 
@@ -138,10 +139,11 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a)
 }
 
 // ---- the general kernels ------------------------------------------------------------------------------------------------------------
-// 128 threads on tiles of 64 x 64: thread (y, x) = (tid / 16, tid % 16) has 8 rows and, of every 64 columns, 4. All operands lie in shared memory in
-// fp32, rows of DP + 4 (64 + 4) floats: 16-byte loads of 16 neighbouring rows then meet all banks once. A step of four loads 12 vectors for
-// 128 multiply-adds a thread, 16 of the 32 clocks those take.
-constexpr int kGT = 128, kGRows = 64, kGKeys = 64;
+// 256 threads on tiles of 64 x 64: thread (y, x) = (tid / 16, tid % 16) has 4 rows and, of every 64 columns, 4. All operands lie in shared memory in
+// fp32, rows of DP + 4 (64 + 4) floats: 16-byte loads of 16 neighbouring rows then meet all banks once. A step of four loads 8 vectors for
+// 64 multiply-adds a thread, three quarters of the clocks those take. 8 rows a thread loaded less, but left two warps to a scheduler: nine sequences
+// of up to 500 tokens, 12 heads of 64 in fp32, took 127 us.
+constexpr int kGT = 256, kGRows = 64, kGKeys = 64, kRT = kGRows / (kGT / 16);
 
 template <int DP>
 struct General {
@@ -156,18 +158,19 @@ struct GeneralParams {
     float2* stats;  // [kv_heads][tokens][group]: -lse log2(e), delta
     uint32_t* norms;  // null, or where the largest squared norms of a row of grad and of a row of v go
     float scale, scale_log2;
+    FastDiv by_group;
     int32_t subs;   // tiles of this kernel to an entry of the plan
     int32_t splits; // shares of the rows that see a tile of keys
     float* shares;
 };
 
-// acc[i][j] += sum over d of a[8 y + i][d] b[x + 16 j][d]
+// acc[i][j] += sum over d of a[4 y + i][d] b[x + 16 j][d]
 template <int DP>
-__device__ __forceinline__ void dot_rows(const float* a, const float* b, int y, int x, float (&acc)[8][4]) {
+__device__ __forceinline__ void dot_rows(const float* a, const float* b, int y, int x, float (&acc)[kRT][4]) {
     constexpr int P = General<DP>::kPitch;
-    float2 s[8][4];
+    float2 s[kRT][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < kRT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[i][j] = make_float2(0.f, 0.f);
 #pragma unroll 2
@@ -176,8 +179,8 @@ __device__ __forceinline__ void dot_rows(const float* a, const float* b, int y, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) u[j] = *reinterpret_cast<const float4*>(b + (x + 16 * j) * P + d);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float4 w = *reinterpret_cast<const float4*>(a + (8 * y + i) * P + d);
+        for (int i = 0; i < kRT; ++i) {
+            const float4 w = *reinterpret_cast<const float4*>(a + (kRT * y + i) * P + d);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 s[i][j] = __ffma2_rn(make_float2(w.x, w.y), make_float2(u[j].x, u[j].y), s[i][j]);
@@ -186,18 +189,18 @@ __device__ __forceinline__ void dot_rows(const float* a, const float* b, int y, 
         }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < kRT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = s[i][j].x + s[i][j].y;
 }
 
 template <int DP>
-__device__ __forceinline__ void multiply_add(float (&acc)[8][DP / 16], const float (&w)[8], const float* row, int x) {
+__device__ __forceinline__ void multiply_add(float (&acc)[kRT][DP / 16], const float (&w)[kRT], const float* row, int x) {
 #pragma unroll
     for (int c = 0; c < DP / 16; c += 4) {
         const float4 u = *reinterpret_cast<const float4*>(row + 4 * x + 16 * c);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kRT; ++i) {
             acc[i][c] = fmaf(w[i], u.x, acc[i][c]);
             acc[i][c + 1] = fmaf(w[i], u.y, acc[i][c + 1]);
             acc[i][c + 2] = fmaf(w[i], u.z, acc[i][c + 2]);
@@ -206,33 +209,33 @@ __device__ __forceinline__ void multiply_add(float (&acc)[8][DP / 16], const flo
     }
 }
 
-// acc[i][.] += sum over k of w[8 y + i][k] b[k][.]
+// acc[i][.] += sum over k of w[4 y + i][k] b[k][.]
 template <int DP>
-__device__ __forceinline__ void add_rows(float (&acc)[8][DP / 16], const float* w, const float* b, int y, int x) {
+__device__ __forceinline__ void add_rows(float (&acc)[kRT][DP / 16], const float* w, const float* b, int y, int x) {
     constexpr int P = General<DP>::kPitch;
 #pragma unroll 1
     for (int k = 0; k < 64; k += 4) {
-        float4 u[8];
+        float4 u[kRT];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = *reinterpret_cast<const float4*>(w + (8 * y + i) * kWPitch + k);
+        for (int i = 0; i < kRT; ++i) u[i] = *reinterpret_cast<const float4*>(w + (kRT * y + i) * kWPitch + k);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float ww[8];
+            float ww[kRT];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ww[i] = e == 0 ? u[i].x : e == 1 ? u[i].y : e == 2 ? u[i].z : u[i].w;
+            for (int i = 0; i < kRT; ++i) ww[i] = e == 0 ? u[i].x : e == 1 ? u[i].y : e == 2 ? u[i].z : u[i].w;
             multiply_add<DP>(acc, ww, b + (k + e) * P, x);
         }
     }
 }
 
-// acc[i][.] += sum over k of w[k][8 y + i] b[k][.]
+// acc[i][.] += sum over k of w[k][4 y + i] b[k][.]
 template <int DP>
-__device__ __forceinline__ void add_columns(float (&acc)[8][DP / 16], const float* w, const float* b, int y, int x) {
+__device__ __forceinline__ void add_columns(float (&acc)[kRT][DP / 16], const float* w, const float* b, int y, int x) {
     constexpr int P = General<DP>::kPitch;
 #pragma unroll 2
     for (int k = 0; k < 64; ++k) {
-        const float4 lo = *reinterpret_cast<const float4*>(w + k * kWPitch + 8 * y), hi = *reinterpret_cast<const float4*>(w + k * kWPitch + 8 * y + 4);
-        const float ww[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        const float4 u = *reinterpret_cast<const float4*>(w + k * kWPitch + kRT * y);
+        const float ww[kRT] = {u.x, u.y, u.z, u.w};
         multiply_add<DP>(acc, ww, b + k * P, x);
     }
 }
@@ -264,6 +267,19 @@ __device__ __forceinline__ void stage(float* to, int32_t dim, bool vec, Row row)
     }
 }
 
+// The same for fp32 by asynchronous copies; what is not there is zeros (any: an address that the copy of no bytes does not follow).
+template <int DP, typename Row>
+__device__ __forceinline__ void stage_ahead(float* to, const float* any, int32_t dim, Row row) {
+    constexpr int P = General<DP>::kPitch;
+    for (int i = threadIdx.x; i < 64 * (DP / 4); i += kGT) {
+        const int r = i / (DP / 4), d = i % (DP / 4) * 4;
+        const float* const at = row(r);
+        const uint32_t bytes = at != nullptr && d < dim ? 16 : 0;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to + r * P + d))), "l"(bytes ? at + d : any), "r"(bytes)
+                     : "memory");
+    }
+}
+
 template <typename T, int DP>
 __device__ __forceinline__ void store_row(T* to, int32_t dim, const float (&acc)[DP / 16], float factor, int x) {
 #pragma unroll
@@ -276,11 +292,13 @@ __device__ __forceinline__ void store_row(T* to, int32_t dim, const float (&acc)
 // A run of 64 stacked rows: row r of it is token t0 + (r0 + r) / group.
 struct RowRun {
     int32_t first, n, head, t0, r0, end;  // end: the entry's rows
-    __device__ __forceinline__ int32_t token(const PackedArgs& a, int32_t r) const { return t0 + (r0 + r) / a.group; }
+    FastDiv by_group;
+    __device__ __forceinline__ int32_t token(const PackedArgs&, int32_t r) const { return t0 + static_cast<int32_t>(by_group.div(r0 + r)); }
     __device__ __forceinline__ bool has(const PackedArgs& a, int32_t r) const { return r0 + r < end && token(a, r) < n; }
-    __device__ __forceinline__ int64_t q_head(const PackedArgs& a, int32_t r) const { return head * a.group + (r0 + r) % a.group; }
+    __device__ __forceinline__ int32_t of_group(const PackedArgs& a, int32_t r) const { return r0 + r - static_cast<int32_t>(by_group.div(r0 + r)) * a.group; }
+    __device__ __forceinline__ int64_t q_head(const PackedArgs& a, int32_t r) const { return head * a.group + of_group(a, r); }
     __device__ __forceinline__ int64_t stat(const PackedArgs& a, int32_t r) const {
-        return (static_cast<int64_t>(head) * a.tokens + first + token(a, r)) * a.group + (r0 + r) % a.group;
+        return (static_cast<int64_t>(head) * a.tokens + first + token(a, r)) * a.group + of_group(a, r);
     }
 };
 
@@ -312,40 +330,63 @@ __device__ __forceinline__ float reduce16(float x, bool most) {
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kGT) packed_general_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
+__global__ void __launch_bounds__(kGT, DP == 64 ? 2 : 1) packed_general_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
     using G = General<DP>;
     extern __shared__ __align__(16) float smem[];
-    float *const q = smem, *const k = q + G::kTile, *const v = k + G::kTile, *const w = v + G::kTile;
+    float *const q = smem, *const w = q + G::kTile, *const kv = w + kWTile;
     const PackedArgs& a = p.a;
     const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
     int4 e;
     int32_t sub, head;
     if (!a.matches(h) || !entry_of(p, a.row_tiles(), h.row_tiles, &e, &sub, &head)) return;
-    const RowRun run{e.x, e.y, head, e.z, sub * kGRows, 2 * a.half_tokens * a.group};
+    const RowRun run{e.x, e.y, head, e.z, sub * kGRows, 2 * a.half_tokens * a.group, p.by_group};
     if (!run.has(a, 0)) return;
     const int tid = threadIdx.x, y = tid >> 4, x = tid & 15;
+    // fp32 rows on the 16-byte grid come by asynchronous copies, a block ahead; others when it is their turn
+    constexpr bool kAhead = std::is_same<T, float>::value;
+    const bool ahead = kAhead && vec;
+    auto get = [&](int32_t key0, int turn) {
+        float *const k = kv + turn * 2 * G::kTile, *const v = k + G::kTile;
+        auto key_row = [&](const PackedTensor& t, int r) -> const T* { return key0 + r < run.n ? row_at<const T>(t, run.first + key0 + r, head) : nullptr; };
+        if (ahead) {
+            stage_ahead<DP>(k, static_cast<const float*>(p.k.base), a.head_dim, [&](int r) { return reinterpret_cast<const float*>(key_row(p.k, r)); });
+            stage_ahead<DP>(v, static_cast<const float*>(p.v.base), a.head_dim, [&](int r) { return reinterpret_cast<const float*>(key_row(p.v, r)); });
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        } else {
+            stage<T, DP>(k, a.head_dim, vec, [&](int r) { return key_row(p.k, r); });
+            stage<T, DP>(v, a.head_dim, vec, [&](int r) { return key_row(p.v, r); });
+        }
+    };
+    if (ahead) get(0, 0);
     stage<T, DP>(q, a.head_dim, vec, [&](int r) -> const T* { return run.has(a, r) ? row_at<const T>(p.q, run.first + run.token(a, r), run.q_head(a, r)) : nullptr; });
-    float acc[8][G::kC], most[8], total[8];
-    int32_t last[8], seen = 0;
+    float acc[kRT][G::kC], most[kRT], total[kRT];
+    int32_t last[kRT], seen = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kRT; ++i) {
         most[i] = -INFINITY;
         total[i] = 0.f;
-        last[i] = a.causal ? min(run.n - 1, run.token(a, 8 * y + i)) : run.n - 1;
+        last[i] = a.causal ? min(run.n - 1, run.token(a, kRT * y + i)) : run.n - 1;
 #pragma unroll
         for (int c = 0; c < G::kC; ++c) acc[i][c] = 0.f;
     }
     seen = a.causal ? min(run.n, run.token(a, kGRows - 1) + 1) : run.n;
+    int turn = 0;
     for (int32_t key0 = 0; key0 < seen; key0 += kGKeys) {
-        __syncthreads();
-        auto key_row = [&](const PackedTensor& t, int r) -> const T* { return key0 + r < run.n ? row_at<const T>(t, run.first + key0 + r, head) : nullptr; };
-        stage<T, DP>(k, a.head_dim, vec, [&](int r) { return key_row(p.k, r); });
-        stage<T, DP>(v, a.head_dim, vec, [&](int r) { return key_row(p.v, r); });
-        __syncthreads();
-        float s[8][4];
+        const float *const k = kv + turn * 2 * G::kTile, *const v = k + G::kTile;
+        if (ahead) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncthreads();  // this block has come, and the one before has been read
+            if (key0 + kGKeys < seen) get(key0 + kGKeys, turn ^ 1);
+            turn ^= 1;
+        } else {
+            __syncthreads();
+            get(key0, 0);
+            __syncthreads();
+        }
+        float s[kRT][4];
         dot_rows<DP>(q, k, y, x, s);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < kRT; ++i) {
             float m = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -360,18 +401,18 @@ __global__ void __launch_bounds__(kGT) packed_general_kernel(const __grid_consta
             for (int j = 0; j < 4; ++j) {
                 const float weight = exp2f(s[i][j] - shift);
                 sum += weight;
-                w[(8 * y + i) * kWPitch + x + 16 * j] = weight;
+                w[(kRT * y + i) * kWPitch + x + 16 * j] = weight;
             }
             total[i] = total[i] * keep + reduce16(sum, false);
 #pragma unroll
             for (int c = 0; c < G::kC; ++c) acc[i][c] *= keep;
         }
-        __syncwarp();  // rows 8 y .. 8 y + 7 are of this warp
+        __syncwarp();  // rows 4 y .. 4 y + 3 are of this warp
         add_rows<DP>(acc, w, v, y, x);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int32_t r = 8 * y + i;
+    for (int i = 0; i < kRT; ++i) {
+        const int32_t r = kRT * y + i;
         if (!run.has(a, r)) continue;
         const int64_t token = run.first + run.token(a, r), q_head = run.q_head(a, r);
         store_row<T, DP>(row_at<T>(p.o, token, q_head), a.head_dim, acc[i], total[i] == 0.f ? 0.f : 1.f / total[i], x);
@@ -505,14 +546,14 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant_
     }
 }
 
-// P and scale dS of 64 rows x 64 keys, both rounded to nothing less than fp32. last(i): the last key that row 8 y + i sees, -1: none.
+// P and scale dS of 64 rows x 64 keys, both rounded to nothing less than fp32. last(i): the last key that row 4 y + i sees, -1: none.
 template <int DP, typename Last, typename Stat>
 __device__ __forceinline__ void weights_and_grads(const float* q, const float* k, const float* g, const float* v, int y, int x, int32_t key0, const GeneralParams& p, Last last,
                                                   Stat stat, float* w, float* dw) {
-    float s[8][4];
+    float s[kRT][4];
     dot_rows<DP>(q, k, y, x, s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kRT; ++i) {
         const float minus_lse = stat(i).x;
         const int32_t end = last(i);
 #pragma unroll
@@ -520,24 +561,24 @@ __device__ __forceinline__ void weights_and_grads(const float* q, const float* k
     }
     if (w != nullptr) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < kRT; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[(8 * y + i) * kWPitch + x + 16 * j] = s[i][j];
+            for (int j = 0; j < 4; ++j) w[(kRT * y + i) * kWPitch + x + 16 * j] = s[i][j];
     }
-    float t[8][4];
+    float t[kRT][4];
     dot_rows<DP>(g, v, y, x, t);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < kRT; ++i) {
         const float delta = stat(i).y;
         const int32_t end = last(i);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) dw[(8 * y + i) * kWPitch + x + 16 * j] = key0 + x + 16 * j <= end ? s[i][j] * (t[i][j] - delta) : 0.f;
+        for (int j = 0; j < 4; ++j) dw[(kRT * y + i) * kWPitch + x + 16 * j] = key0 + x + 16 * j <= end ? s[i][j] * (t[i][j] - delta) : 0.f;
     }
 }
 
 // Gradients of keys and values: 64 keys, all rows that see them.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kGT) packed_general_key_grads_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
+__global__ void __launch_bounds__(kGT, DP == 64 ? 2 : 1) packed_general_key_grads_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
     using G = General<DP>;
     extern __shared__ __align__(16) float smem[];
     __shared__ float2 stats[kGRows];
@@ -553,16 +594,16 @@ __global__ void __launch_bounds__(kGT) packed_general_key_grads_kernel(const __g
     auto key_row = [&](const PackedTensor& t, int r) -> const T* { return key0 + r < e.y ? row_at<const T>(t, e.x + key0 + r, head) : nullptr; };
     stage<T, DP>(k, a.head_dim, vec, [&](int r) { return key_row(p.k, r); });
     stage<T, DP>(v, a.head_dim, vec, [&](int r) { return key_row(p.v, r); });
-    float dk[8][G::kC], dv[8][G::kC];
+    float dk[kRT][G::kC], dv[kRT][G::kC];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < kRT; ++i)
 #pragma unroll
         for (int c = 0; c < G::kC; ++c) dk[i][c] = dv[i][c] = 0.f;
     const int32_t rows = e.y * a.group, row0 = a.causal ? key0 * a.group : 0;
     const int64_t blocks = (rows - row0 + kGRows - 1) / kGRows;
     const int32_t share0 = row0 + static_cast<int32_t>(blocks * split / p.splits) * kGRows, share1 = row0 + static_cast<int32_t>(blocks * (split + 1) / p.splits) * kGRows;
     for (int32_t r0 = share0; r0 < min(rows, share1); r0 += kGRows) {
-        const RowRun run{e.x, e.y, head, 0, r0, rows};
+        const RowRun run{e.x, e.y, head, 0, r0, rows, p.by_group};
         __syncthreads();
         auto query_row = [&](const PackedTensor& t, int r) -> const T* { return run.has(a, r) ? row_at<const T>(t, run.first + run.token(a, r), run.q_head(a, r)) : nullptr; };
         stage<T, DP>(q, a.head_dim, vec, [&](int r) { return query_row(p.q, r); });
@@ -570,15 +611,15 @@ __global__ void __launch_bounds__(kGT) packed_general_key_grads_kernel(const __g
         if (tid < kGRows) stats[tid] = run.has(a, tid) ? p.stats[run.stat(a, tid)] : make_float2(0.f, 0.f);
         __syncthreads();
         weights_and_grads<DP>(q, k, g, v, y, x, key0, p,
-                              [&](int i) { return !run.has(a, 8 * y + i) ? -1 : a.causal ? min(run.token(a, 8 * y + i), e.y - 1) : e.y - 1; },
-                              [&](int i) { return stats[8 * y + i]; }, w, dw);
+                              [&](int i) { return !run.has(a, kRT * y + i) ? -1 : a.causal ? min(run.token(a, kRT * y + i), e.y - 1) : e.y - 1; },
+                              [&](int i) { return stats[kRT * y + i]; }, w, dw);
         __syncthreads();
         add_columns<DP>(dv, w, g, y, x);
         add_columns<DP>(dk, dw, q, y, x);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int32_t key = key0 + 8 * y + i;
+    for (int i = 0; i < kRT; ++i) {
+        const int32_t key = key0 + kRT * y + i;
         if (key >= e.y) continue;
         if (p.splits > 1) {
             float* const to = p.shares + ((static_cast<int64_t>(split) * 2 * a.tokens + e.x + key) * a.kv_heads + head) * a.head_dim;
@@ -593,7 +634,7 @@ __global__ void __launch_bounds__(kGT) packed_general_key_grads_kernel(const __g
 
 // Gradients of queries: 64 rows, all keys that they see.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kGT) packed_general_query_grads_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
+__global__ void __launch_bounds__(kGT, DP == 64 ? 2 : 1) packed_general_query_grads_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
     using G = General<DP>;
     extern __shared__ __align__(16) float smem[];
     __shared__ float2 stats[kGRows];
@@ -603,16 +644,16 @@ __global__ void __launch_bounds__(kGT) packed_general_query_grads_kernel(const _
     int4 e;
     int32_t sub, head;
     if (!a.matches(h) || !entry_of(p, a.row_tiles(), h.row_tiles, &e, &sub, &head)) return;
-    const RowRun run{e.x, e.y, head, e.z, sub * kGRows, 2 * a.half_tokens * a.group};
+    const RowRun run{e.x, e.y, head, e.z, sub * kGRows, 2 * a.half_tokens * a.group, p.by_group};
     if (!run.has(a, 0)) return;
     const int tid = threadIdx.x, y = tid >> 4, x = tid & 15;
     auto query_row = [&](const PackedTensor& t, int r) -> const T* { return run.has(a, r) ? row_at<const T>(t, run.first + run.token(a, r), run.q_head(a, r)) : nullptr; };
     stage<T, DP>(q, a.head_dim, vec, [&](int r) { return query_row(p.q, r); });
     stage<T, DP>(g, a.head_dim, vec, [&](int r) { return query_row(p.grad, r); });
     if (tid < kGRows) stats[tid] = run.has(a, tid) ? p.stats[run.stat(a, tid)] : make_float2(0.f, 0.f);
-    float dq[8][G::kC];
+    float dq[kRT][G::kC];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < kRT; ++i)
 #pragma unroll
         for (int c = 0; c < G::kC; ++c) dq[i][c] = 0.f;
     const int32_t seen = a.causal ? min(run.n, run.token(a, kGRows - 1) + 1) : run.n;
@@ -623,14 +664,14 @@ __global__ void __launch_bounds__(kGT) packed_general_query_grads_kernel(const _
         stage<T, DP>(v, a.head_dim, vec, [&](int r) { return key_row(p.v, r); });
         __syncthreads();
         weights_and_grads<DP>(q, k, g, v, y, x, key0, p,
-                              [&](int i) { return !run.has(a, 8 * y + i) ? -1 : a.causal ? min(run.token(a, 8 * y + i), run.n - 1) : run.n - 1; },
-                              [&](int i) { return stats[8 * y + i]; }, static_cast<float*>(nullptr), dw);
+                              [&](int i) { return !run.has(a, kRT * y + i) ? -1 : a.causal ? min(run.token(a, kRT * y + i), run.n - 1) : run.n - 1; },
+                              [&](int i) { return stats[kRT * y + i]; }, static_cast<float*>(nullptr), dw);
         __syncwarp();
         add_rows<DP>(dq, dw, k, y, x);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int32_t r = 8 * y + i;
+    for (int i = 0; i < kRT; ++i) {
+        const int32_t r = kRT * y + i;
         if (run.has(a, r)) store_row<T, DP>(row_at<T>(p.dq, run.first + run.token(a, r), run.q_head(a, r)), a.head_dim, dq[i], p.scale, x);
     }
 }
@@ -650,6 +691,7 @@ GeneralParams general_params(const PackedCall& c) {
     p.lse = c.lse;
     p.stats = c.scratch ? c.stats() : nullptr;
     p.norms = nullptr;
+    p.by_group = FastDiv(static_cast<uint32_t>(c.a.group));
     p.splits = 1;
     p.shares = c.scratch ? c.shares() : nullptr;
     p.scale = c.scale;
@@ -669,7 +711,7 @@ int launch_general(const char* what, K kernel, GeneralParams p, int32_t subs, in
     return MHLO_CUDA_OK;
 }
 
-// Two CTAs to an SM.
+// Two CTAs to an SM, twice over.
 int32_t key_splits_general(const PackedArgs& a) { return key_splits(static_cast<int64_t>(a.key_capacity) * (kKeyTile / kGKeys) * a.kv_heads, 4 * kNumSMs); }
 
 int32_t row_subs(const PackedArgs& a) { return (2 * a.half_tokens * a.group + kGRows - 1) / kGRows; }
@@ -678,7 +720,7 @@ template <typename T, int DP>
 int forward(const PackedCall& c, cudaStream_t stream) {
     static std::atomic<bool> allowed[64];
     const int32_t vec = vectors<T>(c.q, c.a.head_dim) && vectors<T>(c.k, c.a.head_dim) && vectors<T>(c.v, c.a.head_dim);
-    return launch_general("packed_attention", packed_general_kernel<T, DP>, general_params(c), row_subs(c.a), c.a.row_capacity, 3, 1, DP, vec, allowed, stream);
+    return launch_general("packed_attention", packed_general_kernel<T, DP>, general_params(c), row_subs(c.a), c.a.row_capacity, std::is_same<T, float>::value && vec ? 5 : 3, 1, DP, vec, allowed, stream);
 }
 
 template <typename T, int DP>

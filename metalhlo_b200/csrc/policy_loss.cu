@@ -26,7 +26,8 @@ struct PolicyParams {
     const int32_t* starts;  // null: one mean over all tokens
     float* grad;
     float* results;         // loss, KL, share of clipped tokens
-    int32_t* counts;        // [sequences], then sequences that count, tickets of the two launches; [1] and those without starts
+    int32_t* counts;        // [sequences], then sequences that count, tickets of the two launches; without starts a count of each CTA that counts
+    int32_t counters;       // those CTAs
     double* partial;        // [CTAs][3]
     int64_t tokens;
     int32_t seqs;
@@ -151,24 +152,21 @@ __device__ __forceinline__ void store(const PolicyParams& p, int64_t first, cons
         if (first + i < p.tokens) p.grad[first + i] = grad[i];
 }
 
-// Gradients and sums of the tokens first .. first + 3. weight(b): of a token of sequence b.
+// Gradients and sums of the tokens first .. first + 3. weight(b): of a token of sequence b; asked for once where all four are in one.
 template <typename Weight>
-__device__ __forceinline__ void step(const PolicyParams& p, const int32_t* starts, int64_t first, uint32_t bits, Place place, Sums* sums, Weight weight) {
-    Tokens t;
+__device__ __forceinline__ void step(const PolicyParams& p, const int32_t* starts, int64_t first, uint32_t bits, const Tokens& t, Place place, Sums* sums, Weight weight) {
     float grad[kEach];
-    if (bits != 0) t.load(p, first);
+    int32_t of = -1;
+    double w = 0.0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         grad[i] = 0.f;
         if (!(bits >> i & 1)) continue;
-        double w;
         if (starts != nullptr) {
             place.go(starts, p.seqs, first + i);
             if (!place.holds(starts, first + i)) continue;
-            w = weight(place.b);
-        } else {
-            w = weight(0);
         }
+        if (place.b != of) of = place.b, w = weight(of);
         grad[i] = token(p, t.logprob[i], t.old[i], t.ref[i], t.a[i], w, sums);
     }
     if (first < p.tokens) store(p, first, grad);
@@ -207,13 +205,16 @@ __device__ __forceinline__ Sums sum_over_cta(Sums s, Sums* scratch) {
     s.loss = sum_over_warp(s.loss);
     s.kl = sum_over_warp(s.kl);
     s.clipped = sum_over_warp(s.clipped);
+    if (warps == 1) return s;
     __syncthreads();
     if (lane == 0) scratch[warp] = s;
     __syncthreads();
-    Sums all;
-    if (threadIdx.x == 0)
-        for (int w = 0; w < warps; ++w) all.add(scratch[w]);
-    return all;
+    if (warp != 0) return s;
+    s = lane < warps ? scratch[lane] : Sums{};
+    s.loss = sum_over_warp(s.loss);
+    s.kl = sum_over_warp(s.kl);
+    s.clipped = sum_over_warp(s.clipped);
+    return s;
 }
 
 __device__ __forceinline__ double weight_of(int32_t n, int32_t sequences) { return n > 0 ? 1.0 / (static_cast<double>(n) * static_cast<double>(sequences)) : 0.0; }
@@ -233,11 +234,14 @@ __device__ __forceinline__ void check_starts(const PolicyParams& p, int32_t b) {
 __global__ void __launch_bounds__(kSmallThreads) policy_small_kernel(const __grid_constant__ PolicyParams p) {
     __shared__ int32_t counts[kSmallSeqs], starts[kSmallSeqs + 1], sequences;
     __shared__ Sums scratch[32];
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, threads = blockDim.x;
     const int32_t n = p.starts != nullptr ? p.seqs : 1;
     grid_dependency_wait();
     grid_dependency_release();
-    for (int32_t i = tid; i < n; i += kSmallThreads) {
+    Tokens ahead;  // the first ones of this thread
+    const uint32_t ahead_bits = counted(p, tid * kEach);
+    if (tid * kEach < p.tokens) ahead.load(p, tid * kEach);
+    for (int32_t i = tid; i < n; i += threads) {
         counts[i] = 0;
         if (p.starts != nullptr) {
             starts[i] = p.starts[i];
@@ -251,22 +255,27 @@ __global__ void __launch_bounds__(kSmallThreads) policy_small_kernel(const __gri
     __syncthreads();
     const int32_t* const from = p.starts != nullptr ? starts : nullptr;
     const int64_t all = (p.tokens + 32 * kEach - 1) / (32 * kEach) * (32 * kEach);  // warps stay whole
-    for (int64_t first = tid * kEach; first < all; first += kSmallThreads * kEach) {
+    for (int64_t first = tid * kEach; first < all; first += threads * kEach) {
         Place place{0, 0};
         if (from != nullptr) place.find(from, p.seqs, first - (tid & 31) * kEach, first);
-        count(p, from, first, counted(p, first), place, [&](int32_t b, int32_t k) { atomicAdd(&counts[b], k); });
+        count(p, from, first, first == tid * kEach ? ahead_bits : counted(p, first), place, [&](int32_t b, int32_t k) { atomicAdd(&counts[b], k); });
     }
     __syncthreads();
     int32_t some = 0;
-    for (int32_t i = tid; i < n; i += kSmallThreads) some += counts[i] > 0;
+    for (int32_t i = tid; i < n; i += threads) some += counts[i] > 0;
     some = __reduce_add_sync(0xffffffffu, some);
     if ((tid & 31) == 0 && some > 0) atomicAdd(&sequences, some);
     __syncthreads();
     Sums sums;
-    for (int64_t first = tid * kEach; first < all; first += kSmallThreads * kEach) {
+    for (int64_t first = tid * kEach; first < all; first += threads * kEach) {
         Place place{0, 0};
         if (from != nullptr) place.find(from, p.seqs, first - (tid & 31) * kEach, first);
-        step(p, from, first, counted(p, first), place, &sums, [&](int32_t b) { return weight_of(counts[b], sequences); });
+        uint32_t bits = ahead_bits;
+        if (first != tid * kEach) {
+            bits = counted(p, first);
+            if (bits != 0) ahead.load(p, first);
+        }
+        step(p, from, first, bits, ahead, place, &sums, [&](int32_t b) { return weight_of(counts[b], sequences); });
     }
     sums = sum_over_cta(sums, scratch);
     if (tid == 0) results(p, sums);
@@ -288,13 +297,13 @@ constexpr int64_t kOfCta = kThreads * kEach;
 __global__ void __launch_bounds__(kThreads) policy_count_kernel(const __grid_constant__ PolicyParams p) {
     __shared__ int32_t sequences;
     const int tid = threadIdx.x;
-    const int32_t n = p.starts != nullptr ? p.seqs : 1;
-    if (p.starts != nullptr)
-        for (int64_t b = static_cast<int64_t>(blockIdx.x) * kThreads + tid; b < p.seqs; b += static_cast<int64_t>(gridDim.x) * kThreads) check_starts(p, static_cast<int32_t>(b));
+    const int32_t n = p.seqs;
+    grid_dependency_release();
+    for (int64_t b = static_cast<int64_t>(blockIdx.x) * kThreads + tid; b < p.seqs; b += static_cast<int64_t>(gridDim.x) * kThreads) check_starts(p, static_cast<int32_t>(b));
     for (int64_t base = blockIdx.x * kOfCta; base < p.tokens; base += gridDim.x * kOfCta) {
         const int64_t first = base + tid * kEach;
-        Place place{0, 0};
-        if (p.starts != nullptr) place.find(p.starts, p.seqs, first - (tid & 31) * kEach, first);
+        Place place;
+        place.find(p.starts, p.seqs, first - (tid & 31) * kEach, first);
         count(p, p.starts, first, counted(p, first), place, [&](int32_t b, int32_t k) { atomicAdd(&p.counts[b], k); });
     }
     if (tid == 0) sequences = 0;
@@ -307,35 +316,84 @@ __global__ void __launch_bounds__(kThreads) policy_count_kernel(const __grid_con
     if (tid == 0) p.counts[n] = sequences;
 }
 
+// Without sequences: a count a CTA, which the next launch adds up. (An atomic addition a warp, all to one word, took 9 us for a million tokens.)
+__global__ void __launch_bounds__(kThreads) policy_count_all_kernel(const __grid_constant__ PolicyParams p, int32_t wide) {
+    __shared__ int32_t sums[kThreads / 32];
+    const int tid = threadIdx.x, step = gridDim.x * kThreads;
+    grid_dependency_release();
+    int32_t mine = 0;
+    if (p.mask == nullptr) {
+        mine = blockIdx.x == 0 && tid == 0 ? static_cast<int32_t>(p.tokens) : 0;
+    } else {
+        const int64_t vectors = wide ? p.tokens / 16 : 0;
+        const uint4* const v = reinterpret_cast<const uint4*>(p.mask);
+#pragma unroll 4
+        for (int64_t i = blockIdx.x * kThreads + tid; i < vectors; i += step) {
+            const uint4 m = v[i];
+            mine += __popc(__vcmpne4(m.x, 0)) + __popc(__vcmpne4(m.y, 0)) + __popc(__vcmpne4(m.z, 0)) + __popc(__vcmpne4(m.w, 0));
+        }
+        mine >>= 3;
+        for (int64_t i = vectors * 16 + blockIdx.x * kThreads + tid; i < p.tokens; i += step) mine += p.mask[i] != 0;
+    }
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    if ((tid & 31) == 0) sums[tid >> 5] = mine;
+    __syncthreads();
+    if (tid != 0) return;
+    for (int w = 1; w < kThreads / 32; ++w) mine += sums[w];
+    p.counts[blockIdx.x] = mine;
+    if (blockIdx.x == 0) p.counts[p.counters] = 0;  // the next launch's ticket
+}
+
+// The tokens' values do not wait for the counts: everything in front of the launch that counts is done when this one begins.
 __global__ void __launch_bounds__(kThreads) policy_loss_kernel(const __grid_constant__ PolicyParams p) {
     __shared__ Sums scratch[32];
+    __shared__ int32_t all;
     const int tid = threadIdx.x;
-    const int32_t n = p.starts != nullptr ? p.seqs : 1;
-    grid_dependency_wait();
-    grid_dependency_release();
-    const int32_t sequences = p.counts[n];
     Sums sums;
+    bool waited = false;
+    int32_t sequences = 1;
+    auto wait = [&]() {
+        grid_dependency_wait();
+        grid_dependency_release();
+        if (p.starts != nullptr) {
+            sequences = __ldcg(p.counts + p.seqs);
+        } else {
+            if (tid < 32) {
+                int32_t mine = 0;
+                for (int32_t i = tid; i < p.counters; i += 32) mine += __ldcg(p.counts + i);
+                mine = __reduce_add_sync(0xffffffffu, mine);
+                if (tid == 0) all = mine;
+            }
+            __syncthreads();
+        }
+        waited = true;
+    };
     for (int64_t base = blockIdx.x * kOfCta; base < p.tokens; base += gridDim.x * kOfCta) {
         const int64_t first = base + tid * kEach;
+        Tokens t;
+        const uint32_t bits = counted(p, first);
+        if (first < p.tokens) t.load(p, first);
         Place place{0, 0};
         if (p.starts != nullptr) place.find(p.starts, p.seqs, first - (tid & 31) * kEach, first);
-        step(p, p.starts, first, counted(p, first), place, &sums, [&](int32_t b) { return weight_of(p.counts[b], sequences); });
+        if (!waited) wait();
+        step(p, p.starts, first, bits, t, place, &sums, [&](int32_t b) { return p.starts != nullptr ? weight_of(__ldcg(p.counts + b), sequences) : weight_of(all, 1); });
     }
+    if (!waited) wait();
     sums = sum_over_cta(sums, scratch);
     if (tid == 0) {
         double* const to = p.partial + static_cast<int64_t>(blockIdx.x) * 3;
         to[0] = sums.loss, to[1] = sums.kl, to[2] = sums.clipped;
     }
-    if (!last_cta(p.counts + n + 2)) return;
+    if (!last_cta(p.counts + (p.starts != nullptr ? p.seqs + 2 : p.counters))) return;
     Sums mine;
     for (int32_t i = tid; i < static_cast<int32_t>(gridDim.x); i += kThreads) mine.add({__ldcg(p.partial + i * 3), __ldcg(p.partial + i * 3 + 1), __ldcg(p.partial + i * 3 + 2)});
     mine = sum_over_cta(mine, scratch);
     if (tid == 0) results(p, mine);
 }
 
-constexpr int64_t kMostCtas = 8 * kNumSMs;
+constexpr int64_t kMostCtas = 4 * kNumSMs;
 
-int64_t counts_bytes(int64_t seqs) { return ((std::max<int64_t>(seqs, 1) + 3) * 4 + 15) / 16 * 16; }
+int64_t counts_bytes(int64_t seqs) { return ((std::max<int64_t>(seqs, kNumSMs) + 3) * 4 + 15) / 16 * 16; }
 int64_t scratch_bytes(int64_t tokens, int64_t seqs) { return tokens <= kSmall && seqs <= kSmallSeqs ? 0 : counts_bytes(seqs) + kMostCtas * 24; }
 
 }  // namespace
@@ -390,17 +448,23 @@ int mhlo_cuda_policy_loss(const mhlo_cuda_policy_batch* batch, float* grad_dev, 
     cudaError_t e;
     if (need == 0) {
         p.counts = nullptr;
+        p.counters = 0;
         p.partial = nullptr;
-        e = launch_dependent(policy_small_kernel, dim3(1), dim3(kSmallThreads), 0, s, 1, true, p);
+        const int64_t threads = std::min<int64_t>(kSmallThreads, std::max<int64_t>(1, (b.tokens + 32 * kEach - 1) / (32 * kEach)) * 32);
+        e = launch_dependent(policy_small_kernel, dim3(1), dim3(static_cast<unsigned>(threads)), 0, s, 1, true, p);
     } else {
-        const int64_t n = p.starts ? b.seqs : 1;
         p.counts = static_cast<int32_t*>(scratch_dev);
-        p.partial = reinterpret_cast<double*>(static_cast<char*>(scratch_dev) + counts_bytes(n));
-        MHLO_CUDA_TRY(cudaMemsetAsync(p.counts, 0, (n + 3) * 4, s), MHLO_CUDA_EXECUTION_FAILED);
-        const unsigned grid = static_cast<unsigned>(std::min((b.tokens + kOfCta - 1) / kOfCta, kMostCtas));
-        policy_count_kernel<<<std::max(1u, grid), kThreads, 0, s>>>(p);
+        p.partial = reinterpret_cast<double*>(static_cast<char*>(scratch_dev) + counts_bytes(b.seqs));
+        const unsigned grid = static_cast<unsigned>(std::max<int64_t>(1, std::min((b.tokens + kOfCta - 1) / kOfCta, kMostCtas)));
+        p.counters = static_cast<int32_t>(std::min<unsigned>(grid, kNumSMs));
+        if (p.starts) {
+            MHLO_CUDA_TRY(cudaMemsetAsync(p.counts, 0, (b.seqs + 3) * 4, s), MHLO_CUDA_EXECUTION_FAILED);
+            policy_count_kernel<<<grid, kThreads, 0, s>>>(p);
+        } else {
+            policy_count_all_kernel<<<static_cast<unsigned>(p.counters), kThreads, 0, s>>>(p, aligned16(b.mask));
+        }
         MHLO_CUDA_CHECK_LAUNCH(what);
-        e = launch_dependent(policy_loss_kernel, dim3(std::max(1u, grid)), dim3(kThreads), 0, s, 1, true, p);
+        e = launch_dependent(policy_loss_kernel, dim3(grid), dim3(kThreads), 0, s, 1, true, p);
     }
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of %s failed: %s", what, cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH(what);

@@ -667,24 +667,35 @@ def cached_attention(q, cache: KvCache, page_table, lengths, scale: float, token
 # ---- gradients of the norms ---------------------------------------------------------------------------------------------
 
 
+@functools.lru_cache(maxsize=1024)
+def _norm_grad_scratch(rows, hidden):
+    return lib.mhlo_cuda_norm_grad_scratch_bytes(rows, hidden)
+
+
 def _norm_grad(entry, beta, x, gamma, dy, eps, residual_grad, out, stream):
     import torch
 
-    _same_device(x, gamma, dy, residual_grad, out)
-    hidden = x.shape[-1]
+    shape, dtype, device = x.shape, x.dtype, x.device
+    assert device.type == "cuda" and x.is_contiguous()
+    hidden = shape[-1]
     rows = x.numel() // hidden if hidden else 0
-    for t in (x, dy, residual_grad, out):
-        assert t is None or (t.shape == x.shape and t.dtype == x.dtype and t.is_contiguous())
-    assert gamma is None or (gamma.shape == (hidden,) and gamma.dtype == x.dtype and gamma.is_contiguous())
+    for t in (dy, residual_grad, out):
+        assert t is None or (t.shape == shape and t.dtype == dtype and t.device == device and t.is_contiguous())
+    assert gamma is None or (gamma.shape == (hidden,) and gamma.dtype == dtype and gamma.device == device and gamma.is_contiguous())
 
     def call(s):
         dx = torch.empty_like(x) if out is None else out
-        sums = torch.empty((2 if beta else 1, hidden), dtype=torch.float32, device=x.device).unbind(0)
-        need = lib.mhlo_cuda_norm_grad_scratch_bytes(rows, hidden)
-        scratch = x.new_empty((need + 3) >> 2, dtype=torch.float32) if need else None
-        check(entry(torch_dtype_code(x.dtype), x.data_ptr(), _ptr(gamma), dy.data_ptr(), _ptr(residual_grad), dx.data_ptr(), *(t.data_ptr() for t in sums),
-                    rows, hidden, eps, _ptr(scratch), need, s))
-        return (dx, *sums)
+        need = _norm_grad_scratch(rows, hidden)
+        scratch = torch.empty((need + 3) >> 2, dtype=torch.float32, device=device) if need else None
+        dgamma = torch.empty(hidden, dtype=torch.float32, device=device)
+        if not beta:
+            check(entry(torch_dtype_code(dtype), x.data_ptr(), _ptr(gamma), dy.data_ptr(), _ptr(residual_grad), dx.data_ptr(), dgamma.data_ptr(), rows, hidden, eps,
+                        _ptr(scratch), need, s))
+            return dx, dgamma
+        dbeta = dgamma.new_empty(hidden)
+        check(entry(torch_dtype_code(dtype), x.data_ptr(), _ptr(gamma), dy.data_ptr(), _ptr(residual_grad), dx.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), rows,
+                    hidden, eps, _ptr(scratch), need, s))
+        return dx, dgamma, dbeta
 
     return _run_on(x.device, stream, call)
 
@@ -742,9 +753,11 @@ def packed_plan(starts, tokens: int, q_heads: int, kv_heads: int, causal: bool =
 
 
 def _packed_shapes(q, k, v, plan):
+    """The head dimension of queries, keys and values that are of the plan's batch."""
     tokens, q_heads, dim = q.shape
-    assert (tokens, q_heads) == (plan.tokens, plan.q_heads), (tuple(q.shape), plan.tokens, plan.q_heads)
-    assert k.shape == v.shape == (tokens, plan.kv_heads, dim) and q.dtype == k.dtype == v.dtype
+    dtype, device = q.dtype, plan.device
+    assert tokens == plan.tokens and q_heads == plan.q_heads, (tuple(q.shape), plan.tokens, plan.q_heads)
+    assert k.shape == v.shape == (tokens, plan.kv_heads, dim) and k.dtype == dtype == v.dtype and q.device == device == k.device and v.device == device
     return dim
 
 
@@ -754,10 +767,9 @@ def packed_attention(q, k, v, plan: PackedPlan, scale: float, out=None, lse=None
     not written. See ``mhlo_cuda_packed_attention``."""
     import torch
 
-    _same_device(q, k, v, plan.starts, out, lse)
     dim = _packed_shapes(q, k, v, plan)
-    assert out is None or (out.shape == q.shape and out.dtype == q.dtype)
-    assert lse is None or (lse.shape == q.shape[:2] and lse.dtype == torch.float32 and lse.is_contiguous())
+    assert out is None or (out.shape == q.shape and out.dtype == q.dtype and out.device == plan.device)
+    assert lse is None or (lse.shape == q.shape[:2] and lse.dtype == torch.float32 and lse.device == plan.device and lse.is_contiguous())
 
     def call(s):
         o = _dense_like(q) if out is None else out
@@ -773,12 +785,13 @@ def packed_attention_grad(q, k, v, out, lse, grad_out, plan: PackedPlan, scale: 
     ``mhlo_cuda_packed_attention_grad``."""
     import torch
 
-    _same_device(q, k, v, plan.starts, out, lse, grad_out, dq, dk, dv)
     dim = _packed_shapes(q, k, v, plan)
-    assert out.shape == grad_out.shape == q.shape and out.dtype == grad_out.dtype == q.dtype
-    assert lse.shape == q.shape[:2] and lse.dtype == torch.float32 and lse.is_contiguous()
-    for t, like in ((dq, q), (dk, k), (dv, v)):
-        assert t is None or (t.shape == like.shape and t.dtype == like.dtype)
+    shape, dtype, device = q.shape, q.dtype, plan.device
+    for t in (out, grad_out):
+        assert t.shape == shape and t.dtype == dtype and t.device == device
+    assert lse.shape == shape[:2] and lse.dtype == torch.float32 and lse.device == device and lse.is_contiguous()
+    for t, like in ((dq, shape), (dk, k.shape), (dv, k.shape)):
+        assert t is None or (t.shape == like and t.dtype == dtype and t.device == device)
 
     def call(s):
         grads = [_dense_like(like) if t is None else t for t, like in ((dq, q), (dk, k), (dv, v))]
@@ -865,6 +878,11 @@ def token_logprobs_grad(logits, targets, lse, entropy=None, grad_logprobs=None, 
     return _run_on(logits.device, stream, call)
 
 
+@functools.lru_cache(maxsize=1024)
+def _policy_scratch(tokens, seqs):
+    return lib.mhlo_cuda_policy_loss_scratch_bytes(tokens, seqs)
+
+
 PolicyLoss = collections.namedtuple("PolicyLoss", "loss grad kl clip_fraction")
 
 
@@ -875,22 +893,26 @@ def policy_loss(logprobs, old_logprobs, advantages, mask=None, ref_logprobs=None
     sequences of their means. ``kl`` is None without ``ref_logprobs``. See ``mhlo_cuda_policy_loss``."""
     import torch
 
-    _same_device(logprobs, old_logprobs, advantages, mask, ref_logprobs, starts, grad)
-    for t in (logprobs, old_logprobs, advantages, ref_logprobs, grad):
-        assert t is None or (t.shape == logprobs.shape and t.dtype == torch.float32 and t.is_contiguous())
-    assert mask is None or (mask.shape == logprobs.shape and mask.dtype in (torch.bool, torch.uint8) and mask.is_contiguous())
-    assert starts is None or (starts.dim() == 1 and starts.shape[0] >= 1 and starts.dtype == torch.int32 and starts.is_contiguous())
-    tokens, seqs = logprobs.numel(), 0 if starts is None else starts.shape[0] - 1
+    shape, f32, device = logprobs.shape, torch.float32, logprobs.device
+    assert device.type == "cuda" and logprobs.dtype == f32 and logprobs.is_contiguous()
+    for t in (old_logprobs, advantages, ref_logprobs, grad):
+        assert t is None or (t.shape == shape and t.dtype == f32 and t.device == device and t.is_contiguous())
+    assert mask is None or (mask.shape == shape and mask.dtype in (torch.bool, torch.uint8) and mask.device == device and mask.is_contiguous())
+    tokens, seqs = logprobs.numel(), 0
+    if starts is not None:
+        assert starts.dim() == 1 and starts.dtype == torch.int32 and starts.device == device and starts.is_contiguous()
+        seqs = len(starts) - 1
+        assert seqs >= 0
     batch = PolicyBatchArgs(logprobs.data_ptr(), old_logprobs.data_ptr(), _ptr(ref_logprobs), advantages.data_ptr(), _ptr(mask), _ptr(starts), tokens, seqs,
                             clip_low, clip_high, kl_weight)
 
     def call(s):
         g = torch.empty_like(logprobs) if grad is None else grad
-        results = torch.empty(3, dtype=torch.float32, device=logprobs.device)
-        need = lib.mhlo_cuda_policy_loss_scratch_bytes(tokens, seqs)
+        results = logprobs.new_empty(3)
+        need = _policy_scratch(tokens, seqs)
         scratch = results.new_empty(need >> 2) if need else None
         check(lib.mhlo_cuda_policy_loss(C.byref(batch), g.data_ptr(), results.data_ptr(), _ptr(scratch), need, s))
-        loss, kl, clipped = results.unbind(0)
+        loss, kl, clipped = results.unbind()
         return PolicyLoss(loss, g, None if ref_logprobs is None else kl, clipped)
 
     return _run_on(logprobs.device, stream, call)
