@@ -72,26 +72,32 @@ struct Issuer {
         if (elect_one()) umma_commit(bar);
         __syncwarp();
     }
-    // d = a b^T over head_dim, both tiles [128][head_dim] in shared memory
+    // d = a b^T over head_dim, both tiles [128][head_dim] in shared memory; bar is arrived on when all products so far are done. One thread
+    // issues all of a product's instructions: with an election for each the issuer was what bounded D = 64.
     template <int D>
-    __device__ __forceinline__ void rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) const {
+    __device__ __forceinline__ void rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint64_t* bar) const {
         tc_fence_after();
+        if (elect_one()) {
+            const uint64_t da = make_smem_desc(a, 16, 1024), db = make_smem_desc(b, 16, 1024);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            if (kk >= k_steps) break;
-            const uint64_t da = make_smem_desc(a + (kk / 4) * kPanelBytes + (kk % 4) * 32, 16, 1024);
-            const uint64_t db = make_smem_desc(b + (kk / 4) * kPanelBytes + (kk % 4) * 32, 16, 1024);
-            if (elect_one()) umma_f16(d, da, db, idesc, kk != 0 ? 1u : 0u);
+            for (int kk = 0; kk < D / 16; ++kk) {
+                if (kk >= k_steps) break;
+                const uint32_t at = ((kk / 4) * kPanelBytes + (kk % 4) * 32) >> 4;
+                umma_f16(d, da + at, db + at, idesc, kk != 0 ? 1u : 0u);
+            }
+            umma_commit(bar);
         }
+        __syncwarp();
     }
     // d += a b over 128 columns of a: a in tensor memory, 64 packed columns from a on and 64 from a + 64 on; b [128][head_dim] in shared memory
     __device__ __forceinline__ void columns(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool more) const {
         tc_fence_after();
+        if (elect_one()) {
+            const uint64_t db = make_smem_desc(b, kPanelBytes, 1024);
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-            const uint64_t db = make_smem_desc(b + kk * 16 * 128, kPanelBytes, 1024);
-            if (elect_one()) umma_ts(d, a + (kk / 4) * 64 + (kk % 4) * 8, db, idesc, more || kk != 0 ? 1u : 0u);
+            for (int kk = 0; kk < 8; ++kk) umma_ts(d, a + (kk / 4) * 64 + (kk % 4) * 8, db + (kk * 16 * 128 >> 4), idesc, more || kk != 0 ? 1u : 0u);
         }
+        __syncwarp();
     }
 };
 
@@ -236,13 +242,11 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
         uint32_t item = 0, block = 0;
         auto scores = [&](uint32_t at) {
             if (!wait(&q_full[at % kStages], at / kStages & 1, 2)) return;
-            mma.rows<D>(tmem + kS, k_addr, q_addr + at % kStages * L::kTile, idesc_rows);
-            mma.commit(s_full);
+            mma.rows<D>(tmem + kS, k_addr, q_addr + at % kStages * L::kTile, idesc_rows, s_full);
         };
         auto grads = [&](uint32_t at) {
             if (!wait(&g_full[at % kStages], at / kStages & 1, 3)) return;
-            mma.rows<D>(tmem + kP, v_addr, g_addr + at % kStages * L::kTile, idesc_rows);
-            mma.commit(dp_full);
+            mma.rows<D>(tmem + kP, v_addr, g_addr + at % kStages * L::kTile, idesc_rows, dp_full);
         };
         while (ok && next()) {
             if (t.b0 == t.b1) continue;
@@ -514,13 +518,11 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
         auto region = [&](uint32_t i) { return tmem + kRegion + i % 3 * 128; };
         auto scores = [&](uint32_t at) {
             if (!wait(&k_full[at % kKS], at / kKS & 1, 3)) return;
-            mma.rows<D>(region(2 * at), q_addr, k_addr + at % kKS * L::kTile, idesc_rows);
-            mma.commit(&s_full[at & 1]);
+            mma.rows<D>(region(2 * at), q_addr, k_addr + at % kKS * L::kTile, idesc_rows, &s_full[at & 1]);
         };
         auto grads = [&](uint32_t at) {
             if (!wait(&v_full[at % kVS], at / kVS & 1, 4)) return;
-            mma.rows<D>(region(2 * at + 1), g_addr, v_addr + at % kVS * L::kTile, idesc_rows);
-            mma.commit(&dp_full[at & 1]);
+            mma.rows<D>(region(2 * at + 1), g_addr, v_addr + at % kVS * L::kTile, idesc_rows, &dp_full[at & 1]);
             mma.commit(&v_empty[at % kVS]);
         };
         while (ok && next()) {

@@ -206,25 +206,28 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
         };
         auto issue_s = [&](int h, int stage) {
             tc_fence_after();
-            const uint32_t qa = q_addr + h * L::kTile, ka = k_addr + stage * L::kTile;
+            if (elect_one()) {  // one thread issues all of a product's instructions: an election for each costs as much as the instruction
+                const uint64_t da = make_smem_desc(q_addr + h * L::kTile, 16, 1024), db = make_smem_desc(k_addr + stage * L::kTile, 16, 1024);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-                if (kk >= p.k_steps) break;
-                const uint64_t da = make_smem_desc(qa + (kk / 4) * kPanelBytes + (kk % 4) * 32, 16, 1024);
-                const uint64_t db = make_smem_desc(ka + (kk / 4) * kPanelBytes + (kk % 4) * 32, 16, 1024);
-                if (elect_one()) umma_f16(tmem + kSCol + h * 128, da, db, idesc_s, kk != 0 ? 1u : 0u);
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    if (kk >= p.k_steps) break;
+                    const uint32_t at = ((kk / 4) * kPanelBytes + (kk % 4) * 32) >> 4;
+                    umma_f16(tmem + kSCol + h * 128, da + at, db + at, idesc_s, kk != 0 ? 1u : 0u);
+                }
+                umma_commit(&s_full[h]);
             }
-            commit_to(&s_full[h]);
+            __syncwarp();
         };
         auto issue_pv = [&](int h, int stage, bool more) {
             tc_fence_after();
-            const uint32_t va = v_addr + stage * L::kTile;
+            if (elect_one()) {
+                const uint64_t db = make_smem_desc(v_addr + stage * L::kTile, kPanelBytes, 1024);
 #pragma unroll
-            for (int kk = 0; kk < kKeyTile / 16; ++kk) {
-                const uint64_t db = make_smem_desc(va + kk * 16 * 128, kPanelBytes, 1024);
-                if (elect_one()) umma_ts(tmem + kOCol + h * D, tmem + kPCol + h * kPStride + kk * 8, db, idesc_o, more || kk != 0 ? 1u : 0u);
+                for (int kk = 0; kk < kKeyTile / 16; ++kk)
+                    umma_ts(tmem + kOCol + h * D, tmem + kPCol + h * kPStride + kk * 8, db + (kk * 16 * 128 >> 4), idesc_o, more || kk != 0 ? 1u : 0u);
+                umma_commit(&pv_done[h]);
             }
-            commit_to(&pv_done[h]);
+            __syncwarp();
         };
         RowTile cur, nxt;
         bool has = next(&cur);
