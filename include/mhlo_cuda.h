@@ -819,12 +819,13 @@ int mhlo_cuda_cached_attention(int32_t dtype, const void* q_dev, const int64_t q
  *   starts    [seqs + 1] ascending: rows starts[b] .. starts[b + 1] - 1 are the tokens of sequence b (a sequence may have none)
  *   plan      mhlo_cuda_packed_plan_bytes() bytes, 16-byte aligned: the sequences cut into tiles, longest first, as
  *             mhlo_cuda_packed_plan leaves them. It depends on the starts and on what stands in this struct, and serves all layers
- *             of a step, forward and backward, on any streams; starts is read by mhlo_cuda_packed_plan only
+ *             of a step, forward and backward, at once and on any streams behind it; the starts themselves are read by
+ *             mhlo_cuda_packed_plan only, and where they change it has to be made again
  *   tokens    rows of the tensors; rows of no sequence are neither read into a result nor written
  *   q_heads   a multiple of kv_heads: query head i reads head i / (q_heads / kv_heads)
  *   causal    != 0: a token sees its sequence's tokens up to itself; 0: all of them
- * tokens * q_heads < 2^31. Starts that are out of order (their sequence is passed over; where they go back on earlier ones rows may
- * be left alone, or be written twice) and a plan that is not one of this batch (nothing is written) are reported by
+ * tokens * q_heads <= 2^30. Starts that are out of order (their sequence is passed over: what its rows of the results hold is not defined, and
+ * where starts go back on earlier ones no more is that of those) and a plan that is not one of this batch (nothing is written) are reported by
  * mhlo_cuda_device_error as 200 + one of MHLO_CUDA_KV_ERROR_*.
  * No counterpart in the reference, whose attention is dense, of one length, and forward only
  * (Sources/MetalHLOCore/Metal/Kernels/FlashAttentionKernel.swift:469-670).
@@ -855,7 +856,8 @@ int mhlo_cuda_packed_attention(int32_t dtype, const mhlo_cuda_packed_batch* batc
 /*
  * Gradients of the above: grad = d/do, laid out like o; o and lse as the forward half left them;
  *   p = exp(scale * q . k - lse), dv = p^T grad, ds = p (grad . v - grad . o), dq = scale * ds k, dk = scale * ds^T q,
- * dk and dv summed over the query heads of a head of keys. dq, dk, dv are like q, k, v (any strides) and overlap with no input.
+ * dk and dv summed over the query heads of a head of keys. dq, dk, dv are like q, k, v (any strides) and overlap neither
+ * with an input nor with one another.
  * Sums are fp32 in a fixed order: the same inputs give the same bits. 16-bit types round p and ds to their own type.
  * scratch: packed_attention_grad_scratch_bytes() bytes of device memory, 16-byte aligned, that nothing else uses until the call's work is
  * done; its contents do not matter.

@@ -798,8 +798,8 @@ int packed_args(const char* what, const mhlo_cuda_packed_batch* b, PackedArgs* o
         return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: %lld sequences, %lld tokens", what, static_cast<long long>(b->seqs), static_cast<long long>(b->tokens));
     if (b->kv_heads < 1 || b->kv_heads > 65535 || b->q_heads < 1 || b->q_heads > 65535 || b->q_heads % b->kv_heads != 0)
         return fail(MHLO_CUDA_INVALID_ARGUMENT, "%s: %lld query heads on %lld heads of keys", what, static_cast<long long>(b->q_heads), static_cast<long long>(b->kv_heads));
-    if (b->tokens * b->q_heads >= (int64_t{1} << 31))
-        return fail(MHLO_CUDA_UNSUPPORTED, "%s: %lld tokens of %lld heads (fewer than 2^31 rows)", what, static_cast<long long>(b->tokens), static_cast<long long>(b->q_heads));
+    if (b->tokens * b->q_heads > (int64_t{1} << 30))  // rows, and a tile behind the last one, are numbered in 32 bits
+        return fail(MHLO_CUDA_UNSUPPORTED, "%s: %lld tokens of %lld heads (up to 2^30 rows)", what, static_cast<long long>(b->tokens), static_cast<long long>(b->q_heads));
     out->starts = b->starts;
     out->plan = b->plan;
     out->seqs = static_cast<int32_t>(b->seqs);

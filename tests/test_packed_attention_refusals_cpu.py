@@ -28,7 +28,7 @@ def grad(b=None, dtype=cuda.BF16, dim=64, scale=0.1, q=P, qs=Q, k=P, ks=K, v=P, 
 @pytest.mark.parametrize("want,kw,text", [
     (INVALID, dict(seqs=-1), "sequences"), (INVALID, dict(tokens=-1), "tokens"), (INVALID, dict(seqs=1 << 25), "sequences"), (INVALID, dict(tokens=1 << 31), "tokens"),
     (INVALID, dict(q_heads=3), "3 query heads on 2"), (INVALID, dict(kv_heads=0), "heads"), (INVALID, dict(q_heads=0), "heads"), (INVALID, dict(q_heads=70000, kv_heads=70000), "heads"),
-    (UNSUPPORTED, dict(tokens=1 << 29), "fewer than 2^31 rows"), (INVALID, dict(plan=None), "plan"), (INVALID, dict(plan=P + 8), "plan")])
+    (UNSUPPORTED, dict(tokens=(1 << 28) + 1), "up to 2^30 rows"), (INVALID, dict(plan=None), "plan"), (INVALID, dict(plan=P + 8), "plan")])
 def test_batch(call, want, kw, text):
     assert call(batch(**kw)) == want
     assert text in cuda.last_error()
