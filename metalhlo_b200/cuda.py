@@ -894,15 +894,15 @@ def policy_loss(logprobs, old_logprobs, advantages, mask=None, ref_logprobs=None
     import torch
 
     shape, f32, device = logprobs.shape, torch.float32, logprobs.device
-    assert device.type == "cuda" and logprobs.dtype == f32 and logprobs.is_contiguous()
+    assert device.type == "cuda" and logprobs.dtype is f32 and logprobs.is_contiguous()
     for t in (old_logprobs, advantages, ref_logprobs, grad):
-        assert t is None or (t.shape == shape and t.dtype == f32 and t.device == device and t.is_contiguous())
+        assert t is None or (t.shape == shape and t.dtype is f32 and t.device == device and t.is_contiguous())
     assert mask is None or (mask.shape == shape and mask.dtype in (torch.bool, torch.uint8) and mask.device == device and mask.is_contiguous())
     tokens, seqs = logprobs.numel(), 0
     if starts is not None:
-        assert starts.dim() == 1 and starts.dtype == torch.int32 and starts.device == device and starts.is_contiguous()
-        seqs = len(starts) - 1
-        assert seqs >= 0
+        (seqs,) = starts.shape
+        seqs -= 1
+        assert seqs >= 0 and starts.dtype is torch.int32 and starts.device == device and starts.is_contiguous()
     batch = PolicyBatchArgs(logprobs.data_ptr(), old_logprobs.data_ptr(), _ptr(ref_logprobs), advantages.data_ptr(), _ptr(mask), _ptr(starts), tokens, seqs,
                             clip_low, clip_high, kl_weight)
 
@@ -912,7 +912,7 @@ def policy_loss(logprobs, old_logprobs, advantages, mask=None, ref_logprobs=None
         need = _policy_scratch(tokens, seqs)
         scratch = results.new_empty(need >> 2) if need else None
         check(lib.mhlo_cuda_policy_loss(C.byref(batch), g.data_ptr(), results.data_ptr(), _ptr(scratch), need, s))
-        loss, kl, clipped = results.unbind()
+        loss, kl, clipped = torch.unbind(results)
         return PolicyLoss(loss, g, None if ref_logprobs is None else kl, clipped)
 
     return _run_on(logprobs.device, stream, call)
