@@ -159,9 +159,11 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a)
 
 // ---- the general kernels ------------------------------------------------------------------------------------------------------------
 // 256 threads on tiles of 64 x 64: thread (y, x) = (tid / 16, tid % 16) has 4 rows and, of every 64 columns, 4. All operands lie in shared memory in
-// fp32, rows of DP + 4 (64 + 4) floats: 16-byte loads of 16 neighbouring rows then meet all banks once. A step of four loads 8 vectors for
-// 64 multiply-adds a thread, three quarters of the clocks those take. 8 rows a thread loaded less, but left two warps to a scheduler: nine sequences
-// of up to 500 tokens, 12 heads of 64 in fp32, took 127 us.
+// fp32, rows of DP + 4 (64 + 4) floats: 16-byte loads of 16 neighbouring rows then meet all banks once. What bounds it is what shared memory hands to
+// registers, 128 bytes a clock and SM: a step of four elements loads 8 vectors for 64 multiply-adds a thread, twice the clocks that those take. Nine
+// sequences of up to 500 tokens, 12 heads of 64 in fp32, take 93 us (4.1 GFLOP with what the diagonal tiles compute for nothing; 35 us at the rate of
+// the FMA units). 8 rows a thread, 128 threads, load less, but leave two warps to a scheduler: 127. A warp to 8 rows, lanes to columns, loads more:
+// 97. Values by columns, so that pairs of keys take one instruction, change nothing.
 constexpr int kGT = 256, kGRows = 64, kGKeys = 64, kRT = kGRows / (kGT / 16);
 
 template <int DP>

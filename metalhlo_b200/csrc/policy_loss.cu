@@ -4,7 +4,7 @@
 //   loss = sum of w (-min(ratio a, clip(ratio, 1 - low, 1 + high) a) + kl_weight (exp(x) - x - 1))
 //   dloss/dp = w ((clipped ? 0 : -ratio a) + kl_weight (1 - exp(x))).
 //
-// Bound by HBM for millions of tokens (21 bytes each), by launches below: up to kSmall tokens one CTA counts, weighs and sums; more take a
+// Bound by HBM for millions of tokens (21 bytes each; 0.9 million take 12 us, two launches of it), by launches below (4000: 7.6 us): up to kSmall tokens one CTA counts, weighs and sums; more take a
 // launch that counts and one that does the rest. Counts are integers, sums are fp64 in a fixed order. Whether a ratio is clipped goes by
 // p - o in fp64 against the logarithms of the borders: in fp32 one token in some million next to a border would get the other gradient.
 #include <algorithm>
