@@ -12,7 +12,7 @@
 //   warp 1             MMA issuer
 //   warps 2-5, 6-9     exponentials: columns 0-63 / 64-127
 //
-// Times: 3 causal sequences of 8192 tokens, 32 query heads of 128 on 8, bf16: 1.21 ms the keys, 0.86 the queries (1230 TFLOP/s of what they compute
+// Times: 3 causal sequences of up to 8192 tokens, 32 query heads of 128 on 8, bf16: 1.21 ms the keys, 0.86 the queries (1250 TFLOP/s of what they compute
 // where the mask leaves something; the tensor pipe is busy for 67 %). 32 of 1024, 12 heads of 64, f16: 0.20 and 0.147 ms, tensor pipe 30 %, exponential unit 31 and
 // 41 %, issue slots 32 %: the chain of a block - scores, exponentials, dP, dS, sums - is what both wait for. Built and measured at D = 64, and not kept:
 // products of the next tile issued ahead with results stored under them (keys 0, queries -5 %, at D = 128 +5 %), the two warpgroups' exponentials in turn (0

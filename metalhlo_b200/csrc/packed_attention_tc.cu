@@ -11,7 +11,7 @@
 // weights are those of the weights before that, in fp32.
 //
 // Bound by the exponential unit beside the tensor pipe: a block of 128 x 128 needs 1024 clocks of either at D = 128 (of the tensor pipe 512 at 64). Causal,
-// 32 query heads of 128 on 8, bf16: 24 sequences of 2048 tokens 404 us (990 TFLOP/s of what the mask leaves, the diagonal blocks' other half not
+// 32 query heads of 128 on 8, bf16: 24 sequences of up to 2048 tokens 404 us (990 TFLOP/s of what the mask leaves, the diagonal blocks' other half not
 // counted), one of 16 384 1.75 ms (1260); either unit is busy for half of the time (51 and 53 %). A chain of a half, scores to weights to the next scores,
 // is what both wait for; two run side by side, as many as tensor memory holds.
 #include <algorithm>
