@@ -442,10 +442,11 @@ __global__ void __launch_bounds__(kGT, DP == 64 ? 2 : 1) packed_general_kernel(c
 }
 
 // What the backward half needs of a row: -lse log2(e) and delta = grad . o; fp16: the largest norms of rows of grad and v. LANES of a warp to a row,
-// kStatsRows rows at once, as many bytes on their way as HBM wants (16 384 tokens of 32 heads of 128, bf16: 77 us with one row, 47 with four).
-constexpr int kStatsThreads = 256, kStatsRows = 4;
+// kStatsRows rows at once, and four CTAs to an SM, whose loads run under the others' sums (3 sequences of up to 8192 tokens, 32 heads of 128, bf16: 44 us, 5.6
+// TB/s; four rows and two CTAs, which the registers of four rows take, 77; one row 77; f16 with norms, 32 x 1024 tokens of 12 heads of 64: 36 us and 45).
+constexpr int kStatsThreads = 256, kStatsRows = 2;
 template <typename T, int LANES, bool VEC>
-__global__ void __launch_bounds__(kStatsThreads) packed_stats_kernel(const __grid_constant__ GeneralParams p, FastDiv by_heads, FastDiv by_kv_heads, FastDiv by_group) {
+__global__ void __launch_bounds__(kStatsThreads, 4) packed_stats_kernel(const __grid_constant__ GeneralParams p, FastDiv by_heads, FastDiv by_kv_heads, FastDiv by_group) {
     const PackedArgs& a = p.a;
     constexpr int V = VecTraits<T>::kElems;
     const int lane = threadIdx.x % LANES;
