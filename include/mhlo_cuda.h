@@ -844,8 +844,9 @@ int mhlo_cuda_packed_plan(const mhlo_cuda_packed_batch* batch, mhlo_cuda_stream_
  * o = softmax(scale * q . k) v over each token's own sequence. q, o: [tokens, q_heads, head_dim], k, v: [tokens, kv_heads, head_dim] of
  * `dtype` (F16, BF16 or F32), *_strides = {token, head} in elements, head_dim (1 .. 128) contiguous; 0 < scale <= 1e38. lse (NULL, or
  * [tokens, q_heads] floats) receives the logarithms of the sums of exponentials. o may be q itself with the same strides, or does not overlap with an input.
- * Statistics and sums are fp32; 16-bit types round the weights to their own type. Tensors of 16 bits whose rows lie on the 16-byte grid, with
- * head_dim a multiple of 8 and up to 128 query heads to a head of keys, run on the tensor cores, all others on the FMA units.
+ * Statistics and sums are fp32. Tensors of 16 bits whose rows lie on the 16-byte grid, with head_dim a multiple of 8 and up to 128 query heads to a
+ * head of keys, run on tcgen05 with weights rounded to their own type; all others take fp32 numbers (weights, p, ds, and those of fp32 tensors) as two
+ * of 11 bits each: products are off by 5 * 2^-22 of their size, and an infinity in an fp32 tensor counts as a NaN.
  * |scale * q . k| has to stay below 1e37. An infinity or a NaN in a key or value may reach tokens of its own sequence that do not see it,
  * but none of another.
  */
@@ -858,7 +859,7 @@ int mhlo_cuda_packed_attention(int32_t dtype, const mhlo_cuda_packed_batch* batc
  *   p = exp(scale * q . k - lse), dv = p^T grad, ds = p (grad . v - grad . o), dq = scale * ds k, dk = scale * ds^T q,
  * dk and dv summed over the query heads of a head of keys. dq, dk, dv are like q, k, v (any strides) and overlap neither
  * with an input nor with one another.
- * Sums are fp32 in a fixed order: the same inputs give the same bits. 16-bit types round p and ds to their own type.
+ * Sums are fp32 in a fixed order: the same inputs give the same bits. On tcgen05 p and ds are rounded to the tensors' type.
  * scratch: packed_attention_grad_scratch_bytes() bytes of device memory, 16-byte aligned, that nothing else uses until the call's work is
  * done; its contents do not matter.
  */

@@ -1,5 +1,5 @@
-// Attention over packed sequences: entry points, the plan of a batch, and the kernels of what the tensor cores do not take (fp32, rows off the
-// 16-byte grid, head dimensions that are no multiple of 8), forward and backward, on the FMA units.
+// Attention over packed sequences: entry points, the plan of a batch, and the kernels of what tcgen05 does not take (fp32, rows off the
+// 16-byte grid, head dimensions that are no multiple of 8), forward and backward.
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
@@ -158,19 +158,24 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a)
 }
 
 // ---- the general kernels ------------------------------------------------------------------------------------------------------------
-// 256 threads on tiles of 64 x 64: thread (y, x) = (tid / 16, tid % 16) has 4 rows and, of every 64 columns, 4. All operands lie in shared memory in
-// fp32, rows of DP + 4 (64 + 4) floats: 16-byte loads of 16 neighbouring rows then meet all banks once. What bounds it is what shared memory hands to
-// registers, 128 bytes a clock and SM: a step of four elements loads 8 vectors for 64 multiply-adds a thread, twice the clocks that those take. Nine
-// sequences of up to 500 tokens, 12 heads of 64 in fp32, take 93 us (4.1 GFLOP with what the diagonal tiles compute for nothing; 35 us at the rate of
-// the FMA units). 8 rows a thread, 128 threads, load less, but leave two warps to a scheduler: 127. A warp to 8 rows, lanes to columns, loads more:
-// 97. Values by columns, so that pairs of keys take one instruction, change nothing.
-constexpr int kGT = 256, kGRows = 64, kGKeys = 64, kRT = kGRows / (kGT / 16);
+// Tiles of 64 x 64, eight warps of 16 rows by 32 columns, on mma.sync with tf32 operands; what the two warps of a row have summed is joined at the end.
+// A number of fp32 goes in as two of 11 bits: x = hi + lo + at most 2^-21 |x|, and a product as hi hi + hi lo + lo hi in fp32, so a sum of products is off by
+// 5 * 2^-22 of the sum of their sizes at most, beside what fp32 sums round. (Below 2^-115 lo is less than the smallest normal number, and 11 bits are
+// what is left; infinities become NaN.) 16-bit numbers are their hi: one product instead of three, or two where the other side is weights.
+// A warp's result of one product (scores) is an operand of the next (times values) in the lanes that it lies in, if that takes keys in the order 0 2 4 6 1 3 5 7.
+// Operands lie in shared memory in fp32, rows of DP + 4 floats: the 32 numbers that a warp loads at once are in 32 banks by rows and by columns. The side
+// that four warps share is taken apart on its way there.
+// mma.sync cuts off what does not fit its fp32 result, so a sum goes through it for 16 terms and is added to the whole with a rounding: the error of all
+// is then that of fp32 arithmetic (2.7e-7 of the result, 6.7e-7 of the gradients; 1.0e-6 and 2.2e-6 if the products add up by themselves, for 4 and 9 us less).
+// Nine sequences of up to 500 tokens, 12 heads of 64 in fp32, take 72 us; 95 on the FMA units, whose 4 x 4 elements a thread wait for what shared memory
+// hands to registers (128 bytes a clock and SM, twice the clocks of the multiply-adds). Gradients of five of up to 333, 14 heads on 2: 97 us, and 127.
+// Four warps of 64 columns, both sides taken apart where they are used, took 82 and 137.
+constexpr int kGT = 256, kGRows = 64, kGKeys = 64, kWN = 4;  // kWN: columns of a warp, by 8
 
 template <int DP>
 struct General {
-    static constexpr int kPitch = DP + 4, kTile = 64 * kPitch, kC = DP / 16;
+    static constexpr int kPitch = DP + 4, kTile = 64 * kPitch, kSteps = DP / 8;
 };
-constexpr int kWPitch = 64 + 4, kWTile = 64 * kWPitch;
 
 struct GeneralParams {
     PackedArgs a;
@@ -185,87 +190,93 @@ struct GeneralParams {
     float* shares;
 };
 
-// acc[i][j] += sum over d of a[4 y + i][d] b[x + 16 j][d]
-template <int DP>
-__device__ __forceinline__ void dot_rows(const float* a, const float* b, int y, int x, float (&acc)[kRT][4]) {
-    constexpr int P = General<DP>::kPitch;
-    float2 s[kRT][4];
-#pragma unroll
-    for (int i = 0; i < kRT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = make_float2(0.f, 0.f);
-#pragma unroll 2
-    for (int d = 0; d < DP; d += 4) {
-        float4 u[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = *reinterpret_cast<const float4*>(b + (x + 16 * j) * P + d);
-#pragma unroll
-        for (int i = 0; i < kRT; ++i) {
-            const float4 w = *reinterpret_cast<const float4*>(a + (kRT * y + i) * P + d);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[i][j] = __ffma2_rn(make_float2(w.x, w.y), make_float2(u[j].x, u[j].y), s[i][j]);
-                s[i][j] = __ffma2_rn(make_float2(w.z, w.w), make_float2(u[j].z, u[j].w), s[i][j]);
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kRT; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = s[i][j].x + s[i][j].y;
+struct Parts {
+    uint32_t hi, lo;
+};
+// hi is the nearest of 11 bits, halves away from zero; lo the rest's first 11 bits. A NaN of all ones is lost in hi, but not in lo. (cvt.rna.tf32 for both, and
+// both sides taken apart where they are used, took twice the instructions.)
+template <bool EXACT>
+__device__ __forceinline__ Parts parts(float x) {
+    if constexpr (EXACT) return {__float_as_uint(x), 0};
+    const uint32_t hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    return {hi, __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u};
+}
+// Of a tile in shared memory whose lo parts, unless it is EXACT, are a tile behind it.
+template <int DP, bool EXACT>
+__device__ __forceinline__ Parts parts_at(const float* x) {
+    return {__float_as_uint(x[0]), EXACT ? 0 : __float_as_uint(x[General<DP>::kTile])};
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// c += a b over 8; A, B: whether the numbers are their hi.
+template <bool A, bool B>
+__device__ __forceinline__ void multiply(float (&c)[4], const Parts (&a)[4], const Parts (&b)[2]) {
+    if constexpr (!A) mma_tf32(c, a[0].lo, a[1].lo, a[2].lo, a[3].lo, b[0].hi, b[1].hi);
+    if constexpr (!B) mma_tf32(c, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[0].lo, b[1].lo);
+    mma_tf32(c, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[0].hi, b[1].hi);
 }
 
-template <int DP>
-__device__ __forceinline__ void multiply_add(float (&acc)[kRT][DP / 16], const float (&w)[kRT], const float* row, int x) {
-#pragma unroll
-    for (int c = 0; c < DP / 16; c += 4) {
-        const float4 u = *reinterpret_cast<const float4*>(row + 4 * x + 16 * c);
-#pragma unroll
-        for (int i = 0; i < kRT; ++i) {
-            acc[i][c] = fmaf(w[i], u.x, acc[i][c]);
-            acc[i][c + 1] = fmaf(w[i], u.y, acc[i][c + 1]);
-            acc[i][c + 2] = fmaf(w[i], u.z, acc[i][c + 2]);
-            acc[i][c + 3] = fmaf(w[i], u.w, acc[i][c + 3]);
-        }
-    }
-}
-
-// acc[i][.] += sum over k of w[4 y + i][k] b[k][.]
-template <int DP>
-__device__ __forceinline__ void add_rows(float (&acc)[kRT][DP / 16], const float* w, const float* b, int y, int x) {
+// What a thread has of a warp's 16 rows x 32 columns: element e of c[n] is row lane / 4 + 8 (e / 2), column 8 n + 2 (lane % 4) + e % 2.
+// c = a b^T: 16 rows of a tile by 32 rows of another, over their elements.
+template <int DP, bool EXACT>
+__device__ __forceinline__ void rows_by_rows(const float* a, const float* b, float (&c)[kWN][4]) {
     constexpr int P = General<DP>::kPitch;
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+    for (int n = 0; n < kWN; ++n) c[n][0] = c[n][1] = c[n][2] = c[n][3] = 0.f;
+    a += g * P + t;
+    b += g * P + t;
 #pragma unroll 1
-    for (int k = 0; k < 64; k += 4) {
-        float4 u[kRT];
+    for (int k = 0; k < DP; k += 16) {
+        const Parts x[2][4] = {{parts<EXACT>(a[k]), parts<EXACT>(a[8 * P + k]), parts<EXACT>(a[k + 4]), parts<EXACT>(a[8 * P + k + 4])},
+                               {parts<EXACT>(a[k + 8]), parts<EXACT>(a[8 * P + k + 8]), parts<EXACT>(a[k + 12]), parts<EXACT>(a[8 * P + k + 12])}};
 #pragma unroll
-        for (int i = 0; i < kRT; ++i) u[i] = *reinterpret_cast<const float4*>(w + (kRT * y + i) * kWPitch + k);
+        for (int n = 0; n < kWN; ++n) {
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float ww[kRT];
+            for (int h = 0; h < 2; ++h) {
+                const Parts y[2] = {parts_at<DP, EXACT>(b + 8 * n * P + k + 8 * h), parts_at<DP, EXACT>(b + 8 * n * P + k + 8 * h + 4)};
+                multiply<EXACT, EXACT>(d, x[h], y);
+            }
 #pragma unroll
-            for (int i = 0; i < kRT; ++i) ww[i] = e == 0 ? u[i].x : e == 1 ? u[i].y : e == 2 ? u[i].z : u[i].w;
-            multiply_add<DP>(acc, ww, b + (k + e) * P, x);
+            for (int e = 0; e < 4; ++e) c[n][e] += d[e];
+        }
+    }
+}
+// c += w b: a warp's weights, as rows_by_rows leaves them, by 32 rows of a tile.
+template <int DP, bool EXACT>
+__device__ __forceinline__ void weights_by_rows(const float (&w)[kWN][4], const float* b, float (&c)[DP / 8][4]) {
+    constexpr int P = General<DP>::kPitch;
+    const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+    b += 2 * t * P + g;
+#pragma unroll
+    for (int k = 0; k < kWN; k += 2) {
+        Parts x[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) x[h][0] = parts<false>(w[k + h][0]), x[h][1] = parts<false>(w[k + h][2]), x[h][2] = parts<false>(w[k + h][1]), x[h][3] = parts<false>(w[k + h][3]);
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n) {
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const Parts y[2] = {parts_at<DP, EXACT>(b + 8 * (k + h) * P + 8 * n), parts_at<DP, EXACT>(b + (8 * (k + h) + 1) * P + 8 * n)};
+                multiply<false, EXACT>(d, x[h], y);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[n][e] += d[e];
         }
     }
 }
 
-// acc[i][.] += sum over k of w[k][4 y + i] b[k][.]
-template <int DP>
-__device__ __forceinline__ void add_columns(float (&acc)[kRT][DP / 16], const float* w, const float* b, int y, int x) {
-    constexpr int P = General<DP>::kPitch;
-#pragma unroll 2
-    for (int k = 0; k < 64; ++k) {
-        const float4 u = *reinterpret_cast<const float4*>(w + k * kWPitch + kRT * y);
-        const float ww[kRT] = {u.x, u.y, u.z, u.w};
-        multiply_add<DP>(acc, ww, b + k * P, x);
-    }
-}
-
-// 64 rows into shared memory; row(r): where row r starts, null: zeros (so are the elements behind head_dim).
-template <typename T, int DP, typename Row>
+// 64 rows into shared memory, their lo parts (SPLIT) a tile behind them; row(r): where row r starts, null: zeros (so are the elements behind head_dim).
+template <typename T, int DP, bool SPLIT, typename Row>
 __device__ __forceinline__ void stage(float* to, int32_t dim, bool vec, Row row) {
     constexpr int P = General<DP>::kPitch, V = VecTraits<T>::kElems;
     if (vec) {
+#pragma unroll 4
         for (int i = threadIdx.x; i < 64 * (DP / V); i += kGT) {
             const int r = i / (DP / V), d = i % (DP / V) * V;
             const T* const at = row(r);
@@ -277,37 +288,50 @@ __device__ __forceinline__ void stage(float* to, int32_t dim, bool vec, Row row)
                 for (int e = 0; e < V; ++e) x[e] = 0.f;
             }
 #pragma unroll
-            for (int e = 0; e < V; e += 4) *reinterpret_cast<float4*>(to + r * P + d + e) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+            for (int e = 0; e < V; e += 4) {
+                float4 v = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                if constexpr (SPLIT) {
+                    const Parts a = parts<false>(v.x), b = parts<false>(v.y), c = parts<false>(v.z), f = parts<false>(v.w);
+                    v = make_float4(__uint_as_float(a.hi), __uint_as_float(b.hi), __uint_as_float(c.hi), __uint_as_float(f.hi));
+                    *reinterpret_cast<uint4*>(to + General<DP>::kTile + r * P + d + e) = make_uint4(a.lo, b.lo, c.lo, f.lo);
+                }
+                *reinterpret_cast<float4*>(to + r * P + d + e) = v;
+            }
         }
         return;
     }
     for (int i = threadIdx.x; i < 64 * DP; i += kGT) {
         const int r = i / DP, d = i % DP;
         const T* const at = row(r);
-        to[r * P + d] = at != nullptr && d < dim ? VecTraits<T>::to_float(at[d]) : 0.f;
+        const float x = at != nullptr && d < dim ? VecTraits<T>::to_float(at[d]) : 0.f;
+        const Parts part = parts<!SPLIT>(x);
+        to[r * P + d] = __uint_as_float(part.hi);
+        if (SPLIT) to[General<DP>::kTile + r * P + d] = __uint_as_float(part.lo);
     }
 }
 
-// The same for fp32 by asynchronous copies; what is not there is zeros (any: an address that the copy of no bytes does not follow).
-template <int DP, typename Row>
-__device__ __forceinline__ void stage_ahead(float* to, const float* any, int32_t dim, Row row) {
-    constexpr int P = General<DP>::kPitch;
-    for (int i = threadIdx.x; i < 64 * (DP / 4); i += kGT) {
-        const int r = i / (DP / 4), d = i % (DP / 4) * 4;
-        const float* const at = row(r);
-        const uint32_t bytes = at != nullptr && d < dim ? 16 : 0;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to + r * P + d))), "l"(bytes ? at + d : any), "r"(bytes)
-                     : "memory");
-    }
-}
-
-template <typename T, int DP>
-__device__ __forceinline__ void store_row(T* to, int32_t dim, const float (&acc)[DP / 16], float factor, int x) {
+// What the second warp of a row has goes to shared memory (add: comes from there, to the first).
+template <int N>
+__device__ __forceinline__ void leave_sums(float* to, const float (&c)[N][4]) {
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-        const int d = 4 * x + 64 * (c / 4) + c % 4;
-        if (d < dim) to[d] = VecTraits<T>::from_float(acc[c] * factor);
-    }
+    for (int i = 0; i < N * 4; ++i) to[i * (kGT / 2) + threadIdx.x % (kGT / 2)] = c[i / 4][i % 4];
+}
+template <int N>
+__device__ __forceinline__ void add_sums(const float* from, float (&c)[N][4]) {
+#pragma unroll
+    for (int i = 0; i < N * 4; ++i) c[i / 4][i % 4] += from[i * (kGT / 2) + threadIdx.x % (kGT / 2)];
+}
+
+// Row i of the two that a thread has a part of.
+template <typename T, int DP>
+__device__ __forceinline__ void store_row(T* to, int32_t dim, const float (&c)[DP / 8][4], int i, float factor) {
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int d = 8 * n + 2 * (threadIdx.x & 3) + e;
+            if (d < dim) to[d] = VecTraits<T>::from_float(c[n][2 * i + e] * factor);
+        }
 }
 
 // A run of 64 stacked rows: row r of it is token t0 + (r0 + r) / group.
@@ -341,20 +365,22 @@ __device__ __forceinline__ bool entry_of(const GeneralParams& p, const int4* lis
     return false;
 }
 
-__device__ __forceinline__ float reduce16(float x, bool most) {
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-        const float y = __shfl_xor_sync(0xffffffffu, x, o);
-        x = most ? fmaxf(x, y) : x + y;
-    }
-    return x;
+// Over the four lanes that share rows.
+__device__ __forceinline__ float most_of_row(float x) {
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+    return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+}
+__device__ __forceinline__ float sum_of_row(float x) {
+    x += __shfl_xor_sync(0xffffffffu, x, 1);
+    return x + __shfl_xor_sync(0xffffffffu, x, 2);
 }
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kGT, DP == 64 ? 2 : 1) packed_general_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
     using G = General<DP>;
     extern __shared__ __align__(16) float smem[];
-    float *const q = smem, *const w = q + G::kTile, *const kv = w + kWTile;
+    constexpr bool kExact = !std::is_same<T, float>::value;
+    float *const q = smem, *const k = q + G::kTile, *const v = k + (kExact ? 1 : 2) * G::kTile;
     const PackedArgs& a = p.a;
     const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
     int4 e;
@@ -362,82 +388,76 @@ __global__ void __launch_bounds__(kGT, DP == 64 ? 2 : 1) packed_general_kernel(c
     if (!a.matches(h) || !entry_of(p, a.row_tiles(), h.row_tiles, &e, &sub, &head)) return;
     const RowRun run{e.x, e.y, head, e.z, sub * kGRows, 2 * a.half_tokens * a.group, p.by_group};
     if (!run.has(a, 0)) return;
-    const int tid = threadIdx.x, y = tid >> 4, x = tid & 15;
-    // fp32 rows on the 16-byte grid come by asynchronous copies, a block ahead; others when it is their turn
-    constexpr bool kAhead = std::is_same<T, float>::value;
-    const bool ahead = kAhead && vec;
-    auto get = [&](int32_t key0, int turn) {
-        float *const k = kv + turn * 2 * G::kTile, *const v = k + G::kTile;
-        auto key_row = [&](const PackedTensor& t, int r) -> const T* { return key0 + r < run.n ? row_at<const T>(t, run.first + key0 + r, head) : nullptr; };
-        if (ahead) {
-            stage_ahead<DP>(k, static_cast<const float*>(p.k.base), a.head_dim, [&](int r) { return reinterpret_cast<const float*>(key_row(p.k, r)); });
-            stage_ahead<DP>(v, static_cast<const float*>(p.v.base), a.head_dim, [&](int r) { return reinterpret_cast<const float*>(key_row(p.v, r)); });
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        } else {
-            stage<T, DP>(k, a.head_dim, vec, [&](int r) { return key_row(p.k, r); });
-            stage<T, DP>(v, a.head_dim, vec, [&](int r) { return key_row(p.v, r); });
-        }
-    };
-    if (ahead) get(0, 0);
-    stage<T, DP>(q, a.head_dim, vec, [&](int r) -> const T* { return run.has(a, r) ? row_at<const T>(p.q, run.first + run.token(a, r), run.q_head(a, r)) : nullptr; });
-    float acc[kRT][G::kC], most[kRT], total[kRT];
-    int32_t last[kRT], seen = 0;
+    const int row0 = threadIdx.x / 32 % 4 * 16, column0 = threadIdx.x / 128 * 32, g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+    stage<T, DP, false>(q, a.head_dim, vec, [&](int r) -> const T* { return run.has(a, r) ? row_at<const T>(p.q, run.first + run.token(a, r), run.q_head(a, r)) : nullptr; });
+    float acc[G::kSteps][4], most[2], total[2];
+    int32_t last[2];
 #pragma unroll
-    for (int i = 0; i < kRT; ++i) {
+    for (int i = 0; i < 2; ++i) {
         most[i] = -INFINITY;
         total[i] = 0.f;
-        last[i] = a.causal ? min(run.n - 1, run.token(a, kRT * y + i)) : run.n - 1;
-#pragma unroll
-        for (int c = 0; c < G::kC; ++c) acc[i][c] = 0.f;
+        last[i] = a.causal ? min(run.n - 1, run.token(a, row0 + g + 8 * i)) : run.n - 1;
     }
-    seen = a.causal ? min(run.n, run.token(a, kGRows - 1) + 1) : run.n;
-    int turn = 0;
-    for (int32_t key0 = 0; key0 < seen; key0 += kGKeys) {
-        const float *const k = kv + turn * 2 * G::kTile, *const v = k + G::kTile;
-        if (ahead) {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            __syncthreads();  // this block has come, and the one before has been read
-            if (key0 + kGKeys < seen) get(key0 + kGKeys, turn ^ 1);
-            turn ^= 1;
-        } else {
-            __syncthreads();
-            get(key0, 0);
-            __syncthreads();
-        }
-        float s[kRT][4];
-        dot_rows<DP>(q, k, y, x, s);
 #pragma unroll
-        for (int i = 0; i < kRT; ++i) {
+    for (int n = 0; n < G::kSteps; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+    const int32_t seen = a.causal ? min(run.n, run.token(a, kGRows - 1) + 1) : run.n;
+    for (int32_t key0 = 0; key0 < seen; key0 += kGKeys) {
+        auto key_row = [&](const PackedTensor& x, int r) -> const T* { return key0 + r < run.n ? row_at<const T>(x, run.first + key0 + r, head) : nullptr; };
+        __syncthreads();
+        stage<T, DP, !kExact>(k, a.head_dim, vec, [&](int r) { return key_row(p.k, r); });
+        stage<T, DP, !kExact>(v, a.head_dim, vec, [&](int r) { return key_row(p.v, r); });
+        __syncthreads();
+        float s[kWN][4];
+        rows_by_rows<DP, kExact>(q + row0 * G::kPitch, k + column0 * G::kPitch, s);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
             float m = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[i][j] = key0 + x + 16 * j <= last[i] ? s[i][j] * p.scale_log2 : -INFINITY;
-                m = fmaxf(m, s[i][j]);
-            }
-            m = fmaxf(most[i], reduce16(m, true));
+            for (int n = 0; n < kWN; ++n)
+#pragma unroll
+                for (int e = 2 * i; e < 2 * i + 2; ++e) {
+                    s[n][e] = key0 + column0 + 8 * n + 2 * t + (e & 1) <= last[i] ? s[n][e] * p.scale_log2 : -INFINITY;
+                    m = fmaxf(m, s[n][e]);
+                }
+            m = fmaxf(most[i], most_of_row(m));
             const float shift = m == -INFINITY ? 0.f : m, keep = exp2f(most[i] - shift);
             most[i] = m;
             float sum = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float weight = exp2f(s[i][j] - shift);
-                sum += weight;
-                w[(kRT * y + i) * kWPitch + x + 16 * j] = weight;
-            }
-            total[i] = total[i] * keep + reduce16(sum, false);
+            for (int n = 0; n < kWN; ++n)
 #pragma unroll
-            for (int c = 0; c < G::kC; ++c) acc[i][c] *= keep;
+                for (int e = 2 * i; e < 2 * i + 2; ++e) sum += s[n][e] = exp2f(s[n][e] - shift);
+            total[i] = total[i] * keep + sum;  // of this thread's columns
+#pragma unroll
+            for (int n = 0; n < G::kSteps; ++n) acc[n][2 * i] *= keep, acc[n][2 * i + 1] *= keep;
         }
-        __syncwarp();  // rows 4 y .. 4 y + 3 are of this warp
-        add_rows<DP>(acc, w, v, y, x);
+        weights_by_rows<DP, kExact>(s, v + column0 * G::kPitch, acc);
     }
+    float4* const of_rows = reinterpret_cast<float4*>(smem + G::kTile);
+    __syncthreads();
+    if (column0 > 0) {
+        leave_sums(smem, acc);
+        of_rows[threadIdx.x % (kGT / 2)] = make_float4(most[0], total[0], most[1], total[1]);
+    }
+    __syncthreads();
+    if (column0 > 0) return;
+    const float4 other = of_rows[threadIdx.x];
 #pragma unroll
-    for (int i = 0; i < kRT; ++i) {
-        const int32_t r = kRT * y + i;
+    for (int i = 0; i < 2; ++i) {
+        const float m1 = i == 0 ? other.x : other.z, t1 = i == 0 ? other.y : other.w, m = fmaxf(most[i], m1), shift = m == -INFINITY ? 0.f : m;
+        const float keep = exp2f(most[i] - shift), take = exp2f(m1 - shift);
+#pragma unroll
+        for (int c = 0; c < G::kSteps * 2; ++c) {
+            const int n = c / 2, at = 2 * i + c % 2;
+            acc[n][at] = acc[n][at] * keep + smem[(n * 4 + at) * (kGT / 2) + threadIdx.x] * take;
+        }
+        most[i] = m;
+        total[i] = sum_of_row(total[i] * keep + t1 * take);
+        const int32_t r = row0 + g + 8 * i;
         if (!run.has(a, r)) continue;
         const int64_t token = run.first + run.token(a, r), q_head = run.q_head(a, r);
-        store_row<T, DP>(row_at<T>(p.o, token, q_head), a.head_dim, acc[i], total[i] == 0.f ? 0.f : 1.f / total[i], x);
-        if (x == 0 && p.lse != nullptr) p.lse[token * a.q_heads + q_head] = total[i] == 0.f ? -INFINITY : (most[i] + log2f(total[i])) * 0.6931471805599453f;
+        store_row<T, DP>(row_at<T>(p.o, token, q_head), a.head_dim, acc, i, total[i] == 0.f ? 0.f : 1.f / total[i]);
+        if (t == 0 && p.lse != nullptr) p.lse[token * a.q_heads + q_head] = total[i] == 0.f ? -INFINITY : (most[i] + log2f(total[i])) * 0.6931471805599453f;
     }
 }
 
@@ -568,43 +588,15 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant_
     }
 }
 
-// P and scale dS of 64 rows x 64 keys, both rounded to nothing less than fp32. last(i): the last key that row 4 y + i sees, -1: none.
-template <int DP, typename Last, typename Stat>
-__device__ __forceinline__ void weights_and_grads(const float* q, const float* k, const float* g, const float* v, int y, int x, int32_t key0, const GeneralParams& p, Last last,
-                                                  Stat stat, float* w, float* dw) {
-    float s[kRT][4];
-    dot_rows<DP>(q, k, y, x, s);
-#pragma unroll
-    for (int i = 0; i < kRT; ++i) {
-        const float minus_lse = stat(i).x;
-        const int32_t end = last(i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] = key0 + x + 16 * j <= end ? exp2f(fmaf(s[i][j], p.scale_log2, minus_lse)) : 0.f;
-    }
-    if (w != nullptr) {
-#pragma unroll
-        for (int i = 0; i < kRT; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[(kRT * y + i) * kWPitch + x + 16 * j] = s[i][j];
-    }
-    float t[kRT][4];
-    dot_rows<DP>(g, v, y, x, t);
-#pragma unroll
-    for (int i = 0; i < kRT; ++i) {
-        const float delta = stat(i).y;
-        const int32_t end = last(i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) dw[(kRT * y + i) * kWPitch + x + 16 * j] = key0 + x + 16 * j <= end ? s[i][j] * (t[i][j] - delta) : 0.f;
-    }
-}
-
 // Gradients of keys and values: 64 keys, all rows that see them.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kGT, DP == 64 ? 2 : 1) packed_general_key_grads_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
     using G = General<DP>;
+    constexpr bool kExact = !std::is_same<T, float>::value;
     extern __shared__ __align__(16) float smem[];
     __shared__ float2 stats[kGRows];
-    float *const k = smem, *const v = k + G::kTile, *const q = v + G::kTile, *const g = q + G::kTile, *const w = g + G::kTile, *const dw = w + kWTile;
+    __shared__ int32_t last[kGRows];  // the last key that a row sees, -1: none
+    float *const k = smem, *const v = k + G::kTile, *const q = v + G::kTile, *const grad = q + (kExact ? 1 : 2) * G::kTile;
     const PackedArgs& a = p.a;
     const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
     int4 e;
@@ -612,45 +604,71 @@ __global__ void __launch_bounds__(kGT, DP == 64 ? 2 : 1) packed_general_key_grad
     if (!a.matches(h) || !entry_of(p, a.key_tiles(), h.key_tiles, &e, &sub, &head)) return;
     const int32_t split = sub >> 1, key0 = e.z + (sub & 1) * kGKeys;
     if (key0 >= e.y) return;
-    const int tid = threadIdx.x, y = tid >> 4, x = tid & 15;
-    auto key_row = [&](const PackedTensor& t, int r) -> const T* { return key0 + r < e.y ? row_at<const T>(t, e.x + key0 + r, head) : nullptr; };
-    stage<T, DP>(k, a.head_dim, vec, [&](int r) { return key_row(p.k, r); });
-    stage<T, DP>(v, a.head_dim, vec, [&](int r) { return key_row(p.v, r); });
-    float dk[kRT][G::kC], dv[kRT][G::kC];
+    const int tid = threadIdx.x, row0 = tid / 32 % 4 * 16, column0 = tid / 128 * 32, g = (tid & 31) >> 2, t = tid & 3;
+    auto key_row = [&](const PackedTensor& x, int r) -> const T* { return key0 + r < e.y ? row_at<const T>(x, e.x + key0 + r, head) : nullptr; };
+    stage<T, DP, false>(k, a.head_dim, vec, [&](int r) { return key_row(p.k, r); });
+    stage<T, DP, false>(v, a.head_dim, vec, [&](int r) { return key_row(p.v, r); });
+    float dk[G::kSteps][4], dv[G::kSteps][4];
 #pragma unroll
-    for (int i = 0; i < kRT; ++i)
+    for (int n = 0; n < G::kSteps; ++n)
 #pragma unroll
-        for (int c = 0; c < G::kC; ++c) dk[i][c] = dv[i][c] = 0.f;
-    const int32_t rows = e.y * a.group, row0 = a.causal ? key0 * a.group : 0;
-    const int64_t blocks = (rows - row0 + kGRows - 1) / kGRows;
-    const int32_t share0 = row0 + static_cast<int32_t>(blocks * split / p.splits) * kGRows, share1 = row0 + static_cast<int32_t>(blocks * (split + 1) / p.splits) * kGRows;
+        for (int c = 0; c < 4; ++c) dk[n][c] = dv[n][c] = 0.f;
+    const int32_t rows = e.y * a.group, first_row = a.causal ? key0 * a.group : 0;
+    const int64_t blocks = (rows - first_row + kGRows - 1) / kGRows;
+    const int32_t share0 = first_row + static_cast<int32_t>(blocks * split / p.splits) * kGRows, share1 = first_row + static_cast<int32_t>(blocks * (split + 1) / p.splits) * kGRows;
     for (int32_t r0 = share0; r0 < min(rows, share1); r0 += kGRows) {
         const RowRun run{e.x, e.y, head, 0, r0, rows, p.by_group};
         __syncthreads();
-        auto query_row = [&](const PackedTensor& t, int r) -> const T* { return run.has(a, r) ? row_at<const T>(t, run.first + run.token(a, r), run.q_head(a, r)) : nullptr; };
-        stage<T, DP>(q, a.head_dim, vec, [&](int r) { return query_row(p.q, r); });
-        stage<T, DP>(g, a.head_dim, vec, [&](int r) { return query_row(p.grad, r); });
-        if (tid < kGRows) stats[tid] = run.has(a, tid) ? p.stats[run.stat(a, tid)] : make_float2(0.f, 0.f);
+        auto query_row = [&](const PackedTensor& x, int r) -> const T* { return run.has(a, r) ? row_at<const T>(x, run.first + run.token(a, r), run.q_head(a, r)) : nullptr; };
+        stage<T, DP, !kExact>(q, a.head_dim, vec, [&](int r) { return query_row(p.q, r); });
+        stage<T, DP, !kExact>(grad, a.head_dim, vec, [&](int r) { return query_row(p.grad, r); });
+        if (tid < kGRows) {
+            const bool has = run.has(a, tid);
+            stats[tid] = has ? p.stats[run.stat(a, tid)] : make_float2(0.f, 0.f);
+            last[tid] = !has ? -1 : a.causal ? min(run.token(a, tid), e.y - 1) : e.y - 1;
+        }
         __syncthreads();
-        weights_and_grads<DP>(q, k, g, v, y, x, key0, p,
-                              [&](int i) { return !run.has(a, kRT * y + i) ? -1 : a.causal ? min(run.token(a, kRT * y + i), e.y - 1) : e.y - 1; },
-                              [&](int i) { return stats[kRT * y + i]; }, w, dw);
-        __syncthreads();
-        add_columns<DP>(dv, w, g, y, x);
-        add_columns<DP>(dk, dw, q, y, x);
-    }
+        float s[kWN][4], ds[kWN][4];
+        rows_by_rows<DP, kExact>(k + row0 * G::kPitch, q + column0 * G::kPitch, s);
 #pragma unroll
-    for (int i = 0; i < kRT; ++i) {
-        const int32_t key = key0 + kRT * y + i;
+        for (int n = 0; n < kWN; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int column = column0 + 8 * n + 2 * t + (c & 1);
+                s[n][c] = key0 + row0 + g + 8 * (c >> 1) <= last[column] ? exp2f(fmaf(s[n][c], p.scale_log2, stats[column].x)) : 0.f;
+            }
+        weights_by_rows<DP, kExact>(s, grad + column0 * G::kPitch, dv);
+        rows_by_rows<DP, kExact>(v + row0 * G::kPitch, grad + column0 * G::kPitch, ds);
+#pragma unroll
+        for (int n = 0; n < kWN; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int column = column0 + 8 * n + 2 * t + (c & 1);
+                ds[n][c] = key0 + row0 + g + 8 * (c >> 1) <= last[column] ? s[n][c] * (ds[n][c] - stats[column].y) : 0.f;
+            }
+        weights_by_rows<DP, kExact>(ds, q + column0 * G::kPitch, dk);
+    }
+    __syncthreads();
+    if (column0 > 0) {
+        leave_sums(q, dk);
+        leave_sums(grad, dv);
+    }
+    __syncthreads();
+    if (column0 > 0) return;
+    add_sums(q, dk);
+    add_sums(grad, dv);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int32_t key = key0 + row0 + g + 8 * i;
         if (key >= e.y) continue;
         if (p.splits > 1) {
             float* const to = p.shares + ((static_cast<int64_t>(split) * 2 * a.tokens + e.x + key) * a.kv_heads + head) * a.head_dim;
-            store_row<float, DP>(to, a.head_dim, dk[i], p.scale, x);
-            store_row<float, DP>(to + static_cast<int64_t>(a.tokens) * a.kv_heads * a.head_dim, a.head_dim, dv[i], 1.f, x);
+            store_row<float, DP>(to, a.head_dim, dk, i, p.scale);
+            store_row<float, DP>(to + static_cast<int64_t>(a.tokens) * a.kv_heads * a.head_dim, a.head_dim, dv, i, 1.f);
             continue;
         }
-        store_row<T, DP>(row_at<T>(p.dk, e.x + key, head), a.head_dim, dk[i], p.scale, x);
-        store_row<T, DP>(row_at<T>(p.dv, e.x + key, head), a.head_dim, dv[i], 1.f, x);
+        store_row<T, DP>(row_at<T>(p.dk, e.x + key, head), a.head_dim, dk, i, p.scale);
+        store_row<T, DP>(row_at<T>(p.dv, e.x + key, head), a.head_dim, dv, i, 1.f);
     }
 }
 
@@ -658,9 +676,9 @@ __global__ void __launch_bounds__(kGT, DP == 64 ? 2 : 1) packed_general_key_grad
 template <typename T, int DP>
 __global__ void __launch_bounds__(kGT, DP == 64 ? 2 : 1) packed_general_query_grads_kernel(const __grid_constant__ GeneralParams p, int32_t vec) {
     using G = General<DP>;
+    constexpr bool kExact = !std::is_same<T, float>::value;
     extern __shared__ __align__(16) float smem[];
-    __shared__ float2 stats[kGRows];
-    float *const q = smem, *const g = q + G::kTile, *const k = g + G::kTile, *const v = k + G::kTile, *const dw = v + G::kTile;
+    float *const q = smem, *const grad = q + G::kTile, *const k = grad + G::kTile, *const v = k + (kExact ? 1 : 2) * G::kTile;
     const PackedArgs& a = p.a;
     const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
     int4 e;
@@ -668,33 +686,50 @@ __global__ void __launch_bounds__(kGT, DP == 64 ? 2 : 1) packed_general_query_gr
     if (!a.matches(h) || !entry_of(p, a.row_tiles(), h.row_tiles, &e, &sub, &head)) return;
     const RowRun run{e.x, e.y, head, e.z, sub * kGRows, 2 * a.half_tokens * a.group, p.by_group};
     if (!run.has(a, 0)) return;
-    const int tid = threadIdx.x, y = tid >> 4, x = tid & 15;
-    auto query_row = [&](const PackedTensor& t, int r) -> const T* { return run.has(a, r) ? row_at<const T>(t, run.first + run.token(a, r), run.q_head(a, r)) : nullptr; };
-    stage<T, DP>(q, a.head_dim, vec, [&](int r) { return query_row(p.q, r); });
-    stage<T, DP>(g, a.head_dim, vec, [&](int r) { return query_row(p.grad, r); });
-    if (tid < kGRows) stats[tid] = run.has(a, tid) ? p.stats[run.stat(a, tid)] : make_float2(0.f, 0.f);
-    float dq[kRT][G::kC];
+    const int tid = threadIdx.x, row0 = tid / 32 % 4 * 16, column0 = tid / 128 * 32, g = (tid & 31) >> 2, t = tid & 3;
+    auto query_row = [&](const PackedTensor& x, int r) -> const T* { return run.has(a, r) ? row_at<const T>(x, run.first + run.token(a, r), run.q_head(a, r)) : nullptr; };
+    stage<T, DP, false>(q, a.head_dim, vec, [&](int r) { return query_row(p.q, r); });
+    stage<T, DP, false>(grad, a.head_dim, vec, [&](int r) { return query_row(p.grad, r); });
+    float2 stats[2];
+    int32_t last[2];
 #pragma unroll
-    for (int i = 0; i < kRT; ++i)
+    for (int i = 0; i < 2; ++i) {
+        const int32_t r = row0 + g + 8 * i;
+        const bool has = run.has(a, r);
+        stats[i] = has ? p.stats[run.stat(a, r)] : make_float2(0.f, 0.f);
+        last[i] = !has ? -1 : a.causal ? min(run.token(a, r), run.n - 1) : run.n - 1;
+    }
+    float dq[G::kSteps][4];
 #pragma unroll
-        for (int c = 0; c < G::kC; ++c) dq[i][c] = 0.f;
+    for (int n = 0; n < G::kSteps; ++n) dq[n][0] = dq[n][1] = dq[n][2] = dq[n][3] = 0.f;
     const int32_t seen = a.causal ? min(run.n, run.token(a, kGRows - 1) + 1) : run.n;
     for (int32_t key0 = 0; key0 < seen; key0 += kGKeys) {
         __syncthreads();
-        auto key_row = [&](const PackedTensor& t, int r) -> const T* { return key0 + r < run.n ? row_at<const T>(t, run.first + key0 + r, head) : nullptr; };
-        stage<T, DP>(k, a.head_dim, vec, [&](int r) { return key_row(p.k, r); });
-        stage<T, DP>(v, a.head_dim, vec, [&](int r) { return key_row(p.v, r); });
+        auto key_row = [&](const PackedTensor& x, int r) -> const T* { return key0 + r < run.n ? row_at<const T>(x, run.first + key0 + r, head) : nullptr; };
+        stage<T, DP, !kExact>(k, a.head_dim, vec, [&](int r) { return key_row(p.k, r); });
+        stage<T, DP, !kExact>(v, a.head_dim, vec, [&](int r) { return key_row(p.v, r); });
         __syncthreads();
-        weights_and_grads<DP>(q, k, g, v, y, x, key0, p,
-                              [&](int i) { return !run.has(a, kRT * y + i) ? -1 : a.causal ? min(run.token(a, kRT * y + i), run.n - 1) : run.n - 1; },
-                              [&](int i) { return stats[kRT * y + i]; }, static_cast<float*>(nullptr), dw);
-        __syncwarp();
-        add_rows<DP>(dq, dw, k, y, x);
-    }
+        float s[kWN][4], ds[kWN][4];
+        rows_by_rows<DP, kExact>(q + row0 * G::kPitch, k + column0 * G::kPitch, s);
+        rows_by_rows<DP, kExact>(grad + row0 * G::kPitch, v + column0 * G::kPitch, ds);
 #pragma unroll
-    for (int i = 0; i < kRT; ++i) {
-        const int32_t r = kRT * y + i;
-        if (run.has(a, r)) store_row<T, DP>(row_at<T>(p.dq, run.first + run.token(a, r), run.q_head(a, r)), a.head_dim, dq[i], p.scale, x);
+        for (int n = 0; n < kWN; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float2 stat = stats[c >> 1];
+                ds[n][c] = key0 + column0 + 8 * n + 2 * t + (c & 1) <= last[c >> 1] ? exp2f(fmaf(s[n][c], p.scale_log2, stat.x)) * (ds[n][c] - stat.y) : 0.f;
+            }
+        weights_by_rows<DP, kExact>(ds, k + column0 * G::kPitch, dq);
+    }
+    __syncthreads();
+    if (column0 > 0) leave_sums(k, dq);
+    __syncthreads();
+    if (column0 > 0) return;
+    add_sums(k, dq);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int32_t r = row0 + g + 8 * i;
+        if (run.has(a, r)) store_row<T, DP>(row_at<T>(p.dq, run.first + run.token(a, r), run.q_head(a, r)), a.head_dim, dq, i, p.scale);
     }
 }
 
@@ -723,9 +758,9 @@ GeneralParams general_params(const PackedCall& c) {
 }
 
 template <typename K>
-int launch_general(const char* what, K kernel, GeneralParams p, int32_t subs, int64_t entries, int tiles, int weights, int dp, int32_t vec, std::atomic<bool> (&allowed)[64],
+int launch_general(const char* what, K kernel, GeneralParams p, int32_t subs, int64_t entries, int tiles, int dp, int32_t vec, std::atomic<bool> (&allowed)[64],
                    cudaStream_t stream) {
-    const int bytes = (tiles * 64 * (dp + 4) + weights * kWTile) * 4;
+    const int bytes = tiles * 64 * (dp + 4) * 4;
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(kernel), bytes, allowed)) return st;
     p.subs = subs;
     kernel<<<static_cast<unsigned>(entries * subs * p.a.kv_heads), kGT, bytes, stream>>>(p, vec);
@@ -742,7 +777,7 @@ template <typename T, int DP>
 int forward(const PackedCall& c, cudaStream_t stream) {
     static std::atomic<bool> allowed[64];
     const int32_t vec = vectors<T>(c.q, c.a.head_dim) && vectors<T>(c.k, c.a.head_dim) && vectors<T>(c.v, c.a.head_dim);
-    return launch_general("packed_attention", packed_general_kernel<T, DP>, general_params(c), row_subs(c.a), c.a.row_capacity, std::is_same<T, float>::value && vec ? 5 : 3, 1, DP, vec, allowed, stream);
+    return launch_general("packed_attention", packed_general_kernel<T, DP>, general_params(c), row_subs(c.a), c.a.row_capacity, std::is_same<T, float>::value ? 5 : 3, DP, vec, allowed, stream);
 }
 
 template <typename T, int DP>
@@ -751,11 +786,11 @@ int backward(const PackedCall& c, cudaStream_t stream) {
     const int32_t vec = vectors<T>(c.q, c.a.head_dim) && vectors<T>(c.k, c.a.head_dim) && vectors<T>(c.v, c.a.head_dim) && vectors<T>(c.grad, c.a.head_dim);
     GeneralParams p = general_params(c);
     p.splits = key_splits_general(c.a);
-    if (int st = launch_general("packed_attention_grad", packed_general_key_grads_kernel<T, DP>, p, kKeyTile / kGKeys * p.splits, c.a.key_capacity, 4, 2, DP, vec, allowed_keys, stream))
+    if (int st = launch_general("packed_attention_grad", packed_general_key_grads_kernel<T, DP>, p, kKeyTile / kGKeys * p.splits, c.a.key_capacity, std::is_same<T, float>::value ? 6 : 4, DP, vec, allowed_keys, stream))
         return st;
     if (p.splits > 1)
         if (int st = packed_join_shares(c, p.splits, stream)) return st;
-    return launch_general("packed_attention_grad", packed_general_query_grads_kernel<T, DP>, general_params(c), row_subs(c.a), c.a.row_capacity, 4, 1, DP, vec, allowed_queries, stream);
+    return launch_general("packed_attention_grad", packed_general_query_grads_kernel<T, DP>, general_params(c), row_subs(c.a), c.a.row_capacity, std::is_same<T, float>::value ? 6 : 4, DP, vec, allowed_queries, stream);
 }
 
 template <typename T, int LANES, bool VEC>

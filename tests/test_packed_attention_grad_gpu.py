@@ -148,3 +148,29 @@ def test_layouts(dtype):
     y = dict(x, k=x["k"][:, :1].expand(-1, 2, -1), v=x["v"][:, :1].expand(-1, 2, -1))
     ref, off = reference(y, 0.125, True)
     check(dict(zip(("dq", "dk", "dv"), run(y, 0.125, True, out=[torch.empty_like(t) for t in want]))), ref, off, ("dq", "dk", "dv"))
+
+
+@pytest.mark.parametrize("bits", [0x7fffffff, 0x7f800001, -1])
+@pytest.mark.parametrize("where", ["q", "k", "v", "grad"])
+def test_every_nan_counts(bits, where):
+    """fp32 goes through the products in two parts: neither may turn a NaN into a number, whatever its bits."""
+    from metalhlo_b200 import cuda
+
+    x = inputs([90, 40], 4, 2, 64, F32)
+    plan = cuda.packed_plan(x["starts_dev"], x["rows"], 4, 2, True)
+    bad = {n: x[n].clone() for n in ("q", "k", "v", "grad")}
+    bad[where].view(torch.int32)[20, 0, 7] = bits
+    lse = torch.empty(130, 4, device="cuda")
+    o = cuda.packed_attention(bad["q"], bad["k"], bad["v"], plan, 0.125, lse=lse)
+    dq, dk, dv = cuda.packed_attention_grad(bad["q"], bad["k"], bad["v"], o, lse, bad["grad"], plan, 0.125)
+    nan = {n: t.isnan() for n, t in dict(o=o, dq=dq, dk=dk, dv=dv).items()}
+    if where == "q":
+        assert nan["o"][20, 0].all() and nan["dq"][20, 0].all() and nan["dk"][:21, 0].all() and nan["dv"][:21, 0].all()
+    elif where == "k":
+        assert nan["o"][20:90, :2].all() and nan["dq"][20:90, :2].all() and nan["dk"][20, 0].all() and nan["dv"][20, 0].all()
+    elif where == "v":
+        assert nan["o"][20:90, :2, 7].all() and nan["dq"][20:90, :2].all() and nan["dk"][20, 0].all()
+    else:
+        assert nan["dq"][20, 0].all() and nan["dk"][:21, 0].all() and nan["dv"][:21, 0, 7].all()
+    for n in nan:
+        assert not nan[n][90:].any()
