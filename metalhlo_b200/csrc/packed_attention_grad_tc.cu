@@ -6,18 +6,19 @@
 // with P = 2^(scale log2(e) S - lse log2(e)) and dS = P (dP - delta). That is seven products where five would do; the two more cost less than
 // adding dQ up in memory, and nothing of them depends on an order of arrival.
 //
-// Threads hold a row of the tile in tensor memory, two warpgroups half of a block's columns each. P and dS go over the scores and dP
-// they came from and are the A operands of the products that follow, so they never pass through shared memory.
+// Threads hold a row of the tile in tensor memory. P and dS go over the scores and dP they came from and are the A operands of the products that
+// follow, so they never pass through shared memory.
 //   warp 0             producer (bulk tensor loads; rows behind a sequence's end become zeros, as they would be summed over)
 //   warp 1             MMA issuer
-//   warps 2-5, 6-9     exponentials: columns 0-63 / 64-127
+//   warps 2-5, 6-9     exponentials: columns 0-63 / 64-127 of a block
+// At D = 64 a block goes in two steps of 64 columns with warps 2-5 alone, in half of the tensor memory: two CTAs share an SM, and each works while the other
+// waits for its chain - scores, exponentials, dP, dS, sums.
 //
-// Times: 3 causal sequences of up to 8192 tokens, 32 query heads of 128 on 8, bf16: 1.21 ms the keys, 0.86 the queries (1250 TFLOP/s of what they compute
-// where the mask leaves something; the tensor pipe is busy for 67 %). 32 of 1024, 12 heads of 64, f16: 0.20 and 0.147 ms, tensor pipe 30 %, exponential unit 31 and
-// 41 %, issue slots 32 %: the chain of a block - scores, exponentials, dP, dS, sums - is what both wait for. Built and measured at D = 64, and not kept:
-// products of the next tile issued ahead with results stored under them (keys 0, queries -5 %, at D = 128 +5 %), the two warpgroups' exponentials in turn (0
-// alone, -10 % of the queries with that, +3 % at D = 128), loads of tensor memory a half ahead (0), a quarter of the exponentials by a polynomial (+2 %),
-// sixteen warps of exponentials (0), results through shared memory or by warps of their own (0).
+// Times: 3 causal sequences of up to 8192 tokens, 32 query heads of 128 on 8, bf16: 1.19 ms the keys, 0.855 the queries (1260 TFLOP/s of what they compute
+// where the mask leaves something; the tensor pipe is busy for 67 %). 32 of 1024, 12 heads of 64, f16: 0.181 and 0.128 ms; 0.200 and 0.147 with one CTA to an SM, which
+// none of these changed by more than a few percent: products of the next tile issued ahead with results stored under them (keys 0, queries -5 %, at D = 128
+// +5 %), the two warpgroups' exponentials in turn, loads of tensor memory a half ahead (0), a quarter of the exponentials by a polynomial (+2 %), sixteen warps
+// of exponentials (0), results through shared memory or by warps of their own (0).
 // P and dS are rounded to the type of q and of the gradient, as operands of one product are of one type: 2^-8 of each at most in bf16, 2^-11 in f16, beside which
 // the results' own rounding counts the same.
 // fp16 keeps numbers between 2^-14 and 2^16 whole. P goes to the product times 2^14, dS times a power of two that brings the largest possible
@@ -29,8 +30,15 @@
 namespace mhlo {
 namespace {
 
-constexpr int kThreads = 32 * 10, kWaitKeys = 70, kWaitQueries = 85;
+constexpr int kWaitKeys = 70, kWaitQueries = 85;
 constexpr float kUnit = 16384.f;  // of P in fp16
+
+// A block of 128 goes in kParts steps of kWide columns.
+template <int D>
+struct Shape {
+    static constexpr int kParts = D == 64 ? 2 : 1, kWide = 128 / kParts, kWarps = 8 / kParts, kThreads = 64 + 32 * kWarps, kCtas = kParts;
+    static constexpr uint32_t kTmem = 4 * kWide;  // columns
+};
 
 struct GradParams {
     PackedArgs a;
@@ -98,13 +106,14 @@ struct Issuer {
         }
         __syncwarp();
     }
-    // d += a b over 128 columns of a: a in tensor memory, 64 packed columns from a on and 64 from a + 64 on; b [128][head_dim] in shared memory
+    // d += a b over COLUMNS columns of a: a in tensor memory, 64 packed columns from a on and 64 from a + 64 on; b [COLUMNS][head_dim] in shared memory
+    template <int COLUMNS>
     __device__ __forceinline__ void columns(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool more) const {
         tc_fence_after();
         if (elect_one()) {
             const uint64_t db = make_smem_desc(b, kPanelBytes, 1024);
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk) umma_ts(d, a + (kk / 4) * 64 + (kk % 4) * 8, db + (kk * 16 * 128 >> 4), idesc, more || kk != 0 ? 1u : 0u);
+            for (int kk = 0; kk < COLUMNS / 16; ++kk) umma_ts(d, a + (kk / 4) * 64 + (kk % 4) * 8, db + (kk * 16 * 128 >> 4), idesc, more || kk != 0 ? 1u : 0u);
         }
         __syncwarp();
     }
@@ -112,20 +121,20 @@ struct Issuer {
 
 // ---- keys and values ------------------------------------------------------------------------------------------------------------------
 // The pipe runs dV(j), S(j + 1) while the threads turn dP(j) into dS(j), and dK(j), dP(j + 1) under the exponentials of j + 1: with two
-// regions of 128 columns beside the two sums (all 512 at D = 128) each product finds its region free, and neither side waits for long.
+// regions of a step's columns beside the two sums each product finds its region free.
 template <int D>
 struct KeySmem {
-    static constexpr int kTile = 128 * D * 2, kStages = D == 64 ? 3 : 2;
+    static constexpr int kTile = 128 * D * 2, kStages = 2;
     static constexpr int kK = 0, kV = kTile, kQ = 2 * kTile, kG = kQ + kStages * kTile, kEnd = kG + kStages * kTile, kTotal = kEnd + 1024;
 };
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) key_grads_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
                                                                 const __grid_constant__ GradParams p) {
     using L = KeySmem<D>;
-    constexpr int kPanels = D / 64, kStages = L::kStages;
-    constexpr uint32_t kS = 0, kP = 128, kDv = 256, kDk = 256 + D;
+    constexpr int kPanels = D / 64, kStages = L::kStages, kParts = Shape<D>::kParts, kWide = Shape<D>::kWide, kWarps = Shape<D>::kWarps, kThreads = Shape<D>::kThreads;
+    constexpr uint32_t kS = 0, kP = kWide, kDv = 2 * kWide, kDk = 2 * kWide + D, kPartBytes = kWide * 128;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     __shared__ __align__(16) float minus_lse[kStages][128];
@@ -153,13 +162,13 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
         mbar_init(kv_full, 2);
         mbar_init(kv_empty, 1);
         mbar_init(s_full, 1);
-        mbar_init(p_full, 8);
+        mbar_init(p_full, kWarps);
         mbar_init(dp_full, 1);
-        mbar_init(ds_full, 8);
+        mbar_init(ds_full, kWarps);
         mbar_init(sums_full, 1);
-        mbar_init(sums_free, 8);
+        mbar_init(sums_free, kWarps);
         mbar_init(own, 1);
-        ring.init(9);
+        ring.init(1 + kWarps);
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&q_full[s], 1);
             mbar_init(&g_full[s], 1);
@@ -169,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
         fence_barrier_init();
     }
     if (warp == 1) {
-        tmem_alloc(&tmem_slot, 512);
+        tmem_alloc(&tmem_slot, Shape<D>::kTmem);
         tmem_relinquish();
     }
     // rows that no box brings are summed over with weights of zero
@@ -246,36 +255,37 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
     } else if (warp == 1) {
         // ---- MMA issuer
         const Issuer mma{p.k_steps};
-        const uint32_t idesc_rows = instruction(BF16, false, 128), idesc_cols = instruction(BF16, true, static_cast<uint32_t>(p.k_steps * 16));
+        const uint32_t idesc_rows = instruction(BF16, false, kWide), idesc_cols = instruction(BF16, true, static_cast<uint32_t>(p.k_steps * 16));
         const uint32_t k_addr = smem_u32(smem + L::kK), v_addr = smem_u32(smem + L::kV), q_addr = smem_u32(smem + L::kQ), g_addr = smem_u32(smem + L::kG);
-        uint32_t item = 0, block = 0;
+        uint32_t item = 0, step = 0;
+        auto tile = [&](uint32_t base, uint32_t at) { return base + at / kParts % kStages * L::kTile + at % kParts * kPartBytes; };
         auto scores = [&](uint32_t at) {
-            if (!wait(&q_full[at % kStages], at / kStages & 1, 2)) return;
-            mma.rows<D>(tmem + kS, k_addr, q_addr + at % kStages * L::kTile, idesc_rows, s_full);
+            if (!wait(&q_full[at / kParts % kStages], at / kParts / kStages & 1, 2)) return;
+            mma.rows<D>(tmem + kS, k_addr, tile(q_addr, at), idesc_rows, s_full);
         };
         auto grads = [&](uint32_t at) {
-            if (!wait(&g_full[at % kStages], at / kStages & 1, 3)) return;
-            mma.rows<D>(tmem + kP, v_addr, g_addr + at % kStages * L::kTile, idesc_rows, dp_full);
+            if (!wait(&g_full[at / kParts % kStages], at / kParts / kStages & 1, 3)) return;
+            mma.rows<D>(tmem + kP, v_addr, tile(g_addr, at), idesc_rows, dp_full);
         };
         while (ok && next()) {
-            if (t.b0 == t.b1) continue;
+            const int32_t steps = (t.b1 - t.b0) * kParts;
+            if (steps == 0) continue;
             if (!wait(kv_full, item & 1, 4)) break;
-            scores(block);
-            if (ok) grads(block);
-            if (t.b0 + 1 == t.b1) mma.commit(kv_empty);
-            for (int32_t b = t.b0; b < t.b1 && ok; ++b, ++block) {
-                const bool more = b + 1 < t.b1;
-                const uint32_t stage = block % kStages;
-                if (!wait(p_full, block & 1, 5)) break;
-                if (b == t.b0 && item > 0 && !wait(sums_free, (item - 1) & 1, 6)) break;
-                mma.columns(tmem + kDv, tmem + kS, g_addr + stage * L::kTile, idesc_cols, b > t.b0);
-                if (more) scores(block + 1);
-                if (!wait(ds_full, block & 1, 7)) break;
-                mma.columns(tmem + kDk, tmem + kP, q_addr + stage * L::kTile, idesc_cols, b > t.b0);
-                mma.commit(&empty[stage]);
+            scores(step);
+            if (ok) grads(step);
+            if (steps == 1) mma.commit(kv_empty);
+            for (int32_t i = 0; i < steps && ok; ++i, ++step) {
+                const bool more = i + 1 < steps;
+                if (!wait(p_full, step & 1, 5)) break;
+                if (i == 0 && item > 0 && !wait(sums_free, (item - 1) & 1, 6)) break;
+                mma.columns<kWide>(tmem + kDv, tmem + kS, tile(g_addr, step), idesc_cols, i > 0);
+                if (more) scores(step + 1);
+                if (!wait(ds_full, step & 1, 7)) break;
+                mma.columns<kWide>(tmem + kDk, tmem + kP, tile(q_addr, step), idesc_cols, i > 0);
+                if (step % kParts == kParts - 1) mma.commit(&empty[step / kParts % kStages]);
                 if (more) {
-                    grads(block + 1);
-                    if (b + 2 == t.b1) mma.commit(kv_empty);
+                    grads(step + 1);
+                    if (i + 2 == steps) mma.commit(kv_empty);
                 }
             }
             if (ok) mma.commit(sums_full);
@@ -283,22 +293,23 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
         }
     } else {
         // ---- exponentials
-        const int half = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+        const int half = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane;  // half: 0 where there are four warps
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t s_taddr = tmem + lane_base + kS + half * 64, p_taddr = tmem + lane_base + kP + half * 64;
         const float unit = unit_of<BF16>(p), from_dp = BF16 ? 1.f : unit / kUnit;
         const float2 from_dp2 = make_float2(from_dp, from_dp);
-        uint32_t item = 0, block = 0;
+        uint32_t item = 0, step = 0;
         while (ok && next()) {
-            for (int32_t b = t.b0; b < t.b1; ++b, ++block) {
-                const int stage = block % kStages;
-                const int32_t token0 = b * p.a.half_tokens;
+            const int32_t steps = (t.b1 - t.b0) * kParts;
+            for (int32_t i = 0; i < steps; ++i, ++step) {
+                const uint32_t block = step / kParts, stage = block % kStages;
+                const int32_t token0 = (t.b0 + i / kParts) * p.a.half_tokens, part = kParts == 2 ? step % 2 : half;
                 // columns below hidden are rows of earlier tokens than this thread's key
-                const int32_t hidden = p.a.causal && t.k0 + kKeyTile - 1 > token0 ? (t.k0 + r - token0) * p.a.group - half * 64 : 0;
+                const int32_t hidden = p.a.causal && t.k0 + kKeyTile - 1 > token0 ? (t.k0 + r - token0) * p.a.group - part * 64 : 0;
                 const bool mask = __any_sync(0xffffffffu, hidden > 0);
-                if (!wait(&stats_full[stage], block / kStages & 1, 8) || !wait(s_full, block & 1, 10)) break;
+                if (!wait(&stats_full[stage], block / kStages & 1, 8) || !wait(s_full, step & 1, 10)) break;
                 tc_fence_after();
-                const float *const lse = minus_lse[stage] + half * 64, *const delta = minus_delta[stage] + half * 64;
+                const float *const lse = minus_lse[stage] + part * 64, *const delta = minus_delta[stage] + part * 64;
                 float w[64];
 #pragma unroll
                 for (int c0 = 0; c0 < 64; c0 += 32) {
@@ -319,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full);
-                if (!wait(dp_full, block & 1, 11)) break;
+                if (!wait(dp_full, step & 1, 11)) break;
                 tc_fence_after();
 #pragma unroll
                 for (int c0 = 0; c0 < 64; c0 += 32) {
@@ -342,43 +353,46 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
                 __syncwarp();
                 if (lane == 0) mbar_arrive(ds_full);
             }
-            // ---- results: the first warpgroup takes dV, the second dK
+            // ---- results: dV, dK; of two warpgroups each takes one
             const bool any = t.b0 < t.b1, mine = t.k0 + r < t.n;
             if (!ok || (any && !wait(sums_full, item & 1, 12))) break;
             tc_fence_after();
             const int64_t token = t.first + t.k0 + r;
-            const float factor = half == 0 ? (BF16 ? 1.f : 1.f / kUnit) : p.scale / unit;
-            const uint32_t sums = tmem + lane_base + (half == 0 ? kDv : kDk);
-            if (p.splits > 1) {
-                float* const to = p.shares + (((static_cast<int64_t>(t.split) * 2 + 1 - half) * p.a.tokens + token) * p.a.kv_heads + t.head) * p.a.head_dim;
 #pragma unroll 1
-                for (int c0 = 0; c0 < D; c0 += 32) {
-                    if (c0 >= p.a.head_dim) break;
-                    uint32_t x[32];
-                    if (any) {
+            for (int which = half; which < (kParts == 2 ? 2 : half + 1); ++which) {
+                const float factor = which == 0 ? (BF16 ? 1.f : 1.f / kUnit) : p.scale / unit;
+                const uint32_t sums = tmem + lane_base + (which == 0 ? kDv : kDk);
+                if (p.splits > 1) {
+                    float* const to = p.shares + (((static_cast<int64_t>(t.split) * 2 + 1 - which) * p.a.tokens + token) * p.a.kv_heads + t.head) * p.a.head_dim;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < D; c0 += 32) {
+                        if (c0 >= p.a.head_dim) break;
+                        uint32_t x[32];
+                        if (any) {
+                            tmem_ld32(sums + c0, x);
+                            tmem_ld_wait();
+                        }
+#pragma unroll
+                        for (int c = 0; c < 32; c += 4) {
+                            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                            if (any) v = make_float4(__uint_as_float(x[c]) * factor, __uint_as_float(x[c + 1]) * factor, __uint_as_float(x[c + 2]) * factor, __uint_as_float(x[c + 3]) * factor);
+                            if (mine && c0 + c < p.a.head_dim) *reinterpret_cast<float4*>(to + c0 + c) = v;
+                        }
+                    }
+                } else {
+                    uint8_t* const to = which == 0 ? static_cast<uint8_t*>(p.dv) + (token * p.dv_token + t.head * p.dv_head) * 2
+                                                   : static_cast<uint8_t*>(p.dk) + (token * p.dk_token + t.head * p.dk_head) * 2;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < D; c0 += 32) {
+                        if (c0 >= p.a.head_dim) break;
+                        uint32_t x[32];
                         tmem_ld32(sums + c0, x);
                         tmem_ld_wait();
+                        if (mine) store_result<BF16>(to, x, factor, c0, p.a.head_dim, p.wide != 0);
                     }
-#pragma unroll
-                    for (int c = 0; c < 32; c += 4) {
-                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (any) v = make_float4(__uint_as_float(x[c]) * factor, __uint_as_float(x[c + 1]) * factor, __uint_as_float(x[c + 2]) * factor, __uint_as_float(x[c + 3]) * factor);
-                        if (mine && c0 + c < p.a.head_dim) *reinterpret_cast<float4*>(to + c0 + c) = v;
-                    }
-                }
-                if (!any) continue;
-            } else {
-                uint8_t* const to = half == 0 ? static_cast<uint8_t*>(p.dv) + (token * p.dv_token + t.head * p.dv_head) * 2
-                                              : static_cast<uint8_t*>(p.dk) + (token * p.dk_token + t.head * p.dk_head) * 2;
-#pragma unroll 1
-                for (int c0 = 0; c0 < D; c0 += 32) {
-                    if (c0 >= p.a.head_dim) break;
-                    uint32_t x[32];
-                    tmem_ld32(sums + c0, x);
-                    tmem_ld_wait();
-                    if (mine) store_result<BF16>(to, x, factor, c0, p.a.head_dim, p.wide != 0);
                 }
             }
+            if (!any) continue;
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(sums_free);
@@ -390,26 +404,27 @@ __global__ void __launch_bounds__(kThreads, 1) key_grads_kernel(const __grid_con
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem, Shape<D>::kTmem);
     }
 }
 
 // ---- queries ----------------------------------------------------------------------------------------------------------------------------
-// Three regions of 128 columns beside dQ take turns: S(t) in region 2 t, dP(t) and dS(t) in 2 t + 1 (mod 3). Scores of the next block are
-// there before the threads get to it, and its dP goes where this block's scores were as soon as they have been read.
+// Three regions of a step's columns beside dQ take turns: S(t) in region 2 t, dP(t) and dS(t) in 2 t + 1 (mod 3). Scores of the next step are
+// there before the threads get to it, and its dP goes where this step's scores were as soon as they have been read.
 template <int D>
 struct QuerySmem {
-    static constexpr int kTile = 128 * D * 2, kKStages = 3, kVStages = 2;
+    static constexpr int kTile = 128 * D * 2, kKStages = D == 64 ? 2 : 3, kVStages = 2;
     static constexpr int kQ = 0, kG = kTile, kK = 2 * kTile, kV = kK + kKStages * kTile, kEnd = kV + kVStages * kTile, kTotal = kEnd + 1024;
 };
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) query_grads_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                                                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
                                                                   const __grid_constant__ GradParams p) {
     using L = QuerySmem<D>;
-    constexpr int kPanels = D / 64, kKS = L::kKStages, kVS = L::kVStages;
-    constexpr uint32_t kDq = 0, kRegion = 128;
+    constexpr int kPanels = D / 64, kKS = L::kKStages, kVS = L::kVStages, kParts = Shape<D>::kParts, kWide = Shape<D>::kWide, kWarps = Shape<D>::kWarps;
+    constexpr uint32_t kDq = 0, kRegion = D, kPartBytes = kWide * 128;
+    static_assert(kRegion + 3 * kWide <= Shape<D>::kTmem, "columns of tensor memory");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     __shared__ uint64_t bars[14 + 2 * kKS + 2 * kVS];
@@ -418,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
     uint64_t* const q_full = bars;
     uint64_t* const g_full = bars + 1;
     uint64_t* const qg_empty = bars + 2;
-    // Blocks take turns at two barriers each: products of the next block may complete before a warp has looked for this one's, and a
+    // Steps take turns at two barriers each: products of the next one may complete before a warp has looked for this one's, and a
     // wait knows a phase only from its neighbours.
     uint64_t* const s_full = bars + 3;
     uint64_t* const s_free = bars + 5;  // the scores of a block have been read
@@ -440,14 +455,14 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
         mbar_init(qg_empty, 1);
         for (int s = 0; s < 2; ++s) {
             mbar_init(&s_full[s], 1);
-            mbar_init(&s_free[s], 8);
+            mbar_init(&s_free[s], kWarps);
             mbar_init(&dp_full[s], 1);
-            mbar_init(&ds_full[s], 8);
+            mbar_init(&ds_full[s], kWarps);
         }
         mbar_init(sums_full, 1);
-        mbar_init(sums_free, 8);
+        mbar_init(sums_free, kWarps);
         mbar_init(own, 1);
-        ring.init(9);
+        ring.init(1 + kWarps);
         for (int s = 0; s < kKS; ++s) {
             mbar_init(&k_full[s], 1);
             mbar_init(&k_empty[s], 1);
@@ -459,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
         fence_barrier_init();
     }
     if (warp == 1) {
-        tmem_alloc(&tmem_slot, 512);
+        tmem_alloc(&tmem_slot, Shape<D>::kTmem);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -521,37 +536,40 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
     } else if (warp == 1) {
         // ---- MMA issuer
         const Issuer mma{p.k_steps};
-        const uint32_t idesc_rows = instruction(BF16, false, 128), idesc_cols = instruction(BF16, true, static_cast<uint32_t>(p.k_steps * 16));
+        const uint32_t idesc_rows = instruction(BF16, false, kWide), idesc_cols = instruction(BF16, true, static_cast<uint32_t>(p.k_steps * 16));
         const uint32_t k_addr = smem_u32(smem + L::kK), v_addr = smem_u32(smem + L::kV), q_addr = smem_u32(smem + L::kQ), g_addr = smem_u32(smem + L::kG);
-        uint32_t item = 0, block = 0;
-        auto region = [&](uint32_t i) { return tmem + kRegion + i % 3 * 128; };
+        uint32_t item = 0, step = 0;
+        auto region = [&](uint32_t i) { return tmem + kRegion + i % 3 * kWide; };
+        auto key_tile_at = [&](uint32_t at) { return k_addr + at / kParts % kKS * L::kTile + at % kParts * kPartBytes; };
         auto scores = [&](uint32_t at) {
-            if (!wait(&k_full[at % kKS], at / kKS & 1, 3)) return;
-            mma.rows<D>(region(2 * at), q_addr, k_addr + at % kKS * L::kTile, idesc_rows, &s_full[at & 1]);
+            if (!wait(&k_full[at / kParts % kKS], at / kParts / kKS & 1, 3)) return;
+            mma.rows<D>(region(2 * at), q_addr, key_tile_at(at), idesc_rows, &s_full[at & 1]);
         };
         auto grads = [&](uint32_t at) {
-            if (!wait(&v_full[at % kVS], at / kVS & 1, 4)) return;
-            mma.rows<D>(region(2 * at + 1), g_addr, v_addr + at % kVS * L::kTile, idesc_rows, &dp_full[at & 1]);
-            mma.commit(&v_empty[at % kVS]);
+            const uint32_t stage = at / kParts % kVS;
+            if (!wait(&v_full[stage], at / kParts / kVS & 1, 4)) return;
+            mma.rows<D>(region(2 * at + 1), g_addr, v_addr + stage * L::kTile + at % kParts * kPartBytes, idesc_rows, &dp_full[at & 1]);
+            if (at % kParts == kParts - 1) mma.commit(&v_empty[stage]);
         };
         while (ok && next()) {
+            const int32_t steps = t.nblk * kParts;
             if (!wait(q_full, item & 1, 5)) break;
-            scores(block);
+            scores(step);
             if (!wait(g_full, item & 1, 6)) break;
             // the region of this dP held the last item's last scores, which were read before its last dS
-            if (ok) grads(block);
-            if (t.nblk == 1) mma.commit(qg_empty);
-            for (int32_t b = 0; b < t.nblk && ok; ++b, ++block) {
-                if (b + 1 < t.nblk) {
-                    scores(block + 1);
-                    if (!wait(&s_free[block & 1], block >> 1 & 1, 7)) break;
-                    grads(block + 1);
-                    if (b + 2 == t.nblk) mma.commit(qg_empty);
+            if (ok) grads(step);
+            if (steps == 1) mma.commit(qg_empty);
+            for (int32_t i = 0; i < steps && ok; ++i, ++step) {
+                if (i + 1 < steps) {
+                    scores(step + 1);
+                    if (!wait(&s_free[step & 1], step >> 1 & 1, 7)) break;
+                    grads(step + 1);
+                    if (i + 2 == steps) mma.commit(qg_empty);
                 }
-                if (!wait(&ds_full[block & 1], block >> 1 & 1, 8)) break;
-                if (b == 0 && item > 0 && !wait(sums_free, (item - 1) & 1, 10)) break;
-                mma.columns(tmem + kDq, region(2 * block + 1), k_addr + block % kKS * L::kTile, idesc_cols, b > 0);
-                mma.commit(&k_empty[block % kKS]);
+                if (!wait(&ds_full[step & 1], step >> 1 & 1, 8)) break;
+                if (i == 0 && item > 0 && !wait(sums_free, (item - 1) & 1, 10)) break;
+                mma.columns<kWide>(tmem + kDq, region(2 * step + 1), key_tile_at(step), idesc_cols, i > 0);
+                if (step % kParts == kParts - 1) mma.commit(&k_empty[step / kParts % kKS]);
             }
             if (ok) mma.commit(sums_full);
             ++item;
@@ -562,18 +580,18 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
         const float unit = unit_of<BF16>(p);
         const int32_t row_token = r / p.a.group, row_head = r - row_token * p.a.group;
-        uint32_t item = 0, block = 0;
+        uint32_t item = 0, step = 0;
         while (ok && next()) {
-            const int32_t i = t.t0 + row_token, last = p.a.causal ? min(t.n - 1, i) : t.n - 1;
+            const int32_t i = t.t0 + row_token, steps = t.nblk * kParts, last = p.a.causal ? min(t.n - 1, i) : t.n - 1;
             const bool mine = r < rows && i < t.n;
             const int64_t token = t.first + i;
             const float2 stat = mine ? p.stats[(static_cast<int64_t>(t.head) * p.a.tokens + token) * p.a.group + row_head] : make_float2(-INFINITY, 0.f);
             const float2 lse2 = make_float2(stat.x, stat.x), unit2 = make_float2(unit, unit), delta2 = make_float2(-stat.y * unit, -stat.y * unit);
-            for (int32_t b = 0; b < t.nblk; ++b, ++block) {
-                const uint32_t s_taddr = tmem + lane_base + kRegion + 2 * block % 3 * 128 + half * 64, p_taddr = tmem + lane_base + kRegion + (2 * block + 1) % 3 * 128 + half * 64;
-                const int32_t seen = last + 1 - b * kKeyTile - half * 64;  // columns that this thread's row sees
+            for (int32_t at = 0; at < steps; ++at, ++step) {
+                const uint32_t s_taddr = tmem + lane_base + kRegion + 2 * step % 3 * kWide + half * 64, p_taddr = tmem + lane_base + kRegion + (2 * step + 1) % 3 * kWide + half * 64;
+                const int32_t seen = last + 1 - at * kWide - half * 64;  // columns that this thread's row sees
                 const bool mask = __any_sync(0xffffffffu, seen < 64);
-                if (!wait(&s_full[block & 1], block >> 1 & 1, 11)) break;
+                if (!wait(&s_full[step & 1], step >> 1 & 1, 11)) break;
                 tc_fence_after();
                 float w[64];
 #pragma unroll
@@ -589,11 +607,11 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
                     if (c0 == 32) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&s_free[block & 1]);
+                        if (lane == 0) mbar_arrive(&s_free[step & 1]);
                     }
                     weights(s, p.scale_log2, w + c0, [&](int) { return lse2; });
                 }
-                if (!wait(&dp_full[block & 1], block >> 1 & 1, 12)) break;
+                if (!wait(&dp_full[step & 1], step >> 1 & 1, 12)) break;
                 tc_fence_after();
 #pragma unroll
                 for (int c0 = 0; c0 < 64; c0 += 32) {
@@ -612,16 +630,16 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&ds_full[block & 1]);
+                if (lane == 0) mbar_arrive(&ds_full[step & 1]);
             }
-            // ---- results: a warpgroup takes half of the elements
+            // ---- results: of two warpgroups each takes half of the elements
             if (!wait(sums_full, item & 1, 13)) break;
             tc_fence_after();
             const int64_t head = t.head * p.a.group + row_head;
             uint8_t* const to = static_cast<uint8_t*>(p.dq) + (token * p.dq_token + head * p.dq_head) * 2;
             const float factor = p.scale / unit;
 #pragma unroll 1
-            for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 32) {
+            for (int c0 = half * (D / 2); c0 < (kParts == 2 ? D : (half + 1) * (D / 2)); c0 += 32) {
                 if (c0 >= p.a.head_dim) break;
                 uint32_t x[32];
                 tmem_ld32(tmem + lane_base + kDq + c0, x);
@@ -639,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1) query_grads_kernel(const __grid_c
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem, Shape<D>::kTmem);
     }
 }
 
@@ -671,9 +689,9 @@ int launch(const PackedCall& c, cudaStream_t stream) {
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(keys), KeySmem<D>::kTotal, keys_allowed)) return st;
     if (int st = allow_dynamic_smem(reinterpret_cast<const void*>(queries), QuerySmem<D>::kTotal, queries_allowed)) return st;
     const auto grid = [](int64_t items) { return dim3(static_cast<unsigned>(items)); };
-    cudaError_t e = launch_dependent(keys, grid(static_cast<int64_t>(a.key_capacity) * a.kv_heads * p.splits), dim3(kThreads), KeySmem<D>::kTotal, stream, 1, true, mq, mk, mv, mg, p);
+    cudaError_t e = launch_dependent(keys, grid(static_cast<int64_t>(a.key_capacity) * a.kv_heads * p.splits), dim3(Shape<D>::kThreads), KeySmem<D>::kTotal, stream, 1, true, mq, mk, mv, mg, p);
     if (e == cudaSuccess)
-        e = launch_dependent(queries, grid(2 * static_cast<int64_t>(a.row_capacity) * a.kv_heads), dim3(kThreads), QuerySmem<D>::kTotal, stream, 1, true, mq, mk, mv, mg, p);
+        e = launch_dependent(queries, grid(2 * static_cast<int64_t>(a.row_capacity) * a.kv_heads), dim3(Shape<D>::kThreads), QuerySmem<D>::kTotal, stream, 1, true, mq, mk, mv, mg, p);
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of packed_attention_grad failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("packed_attention_grad");
     return p.splits > 1 ? packed_join_shares(c, p.splits, stream) : MHLO_CUDA_OK;
