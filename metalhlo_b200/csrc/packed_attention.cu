@@ -146,6 +146,7 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a)
     if (tid == 0 && blockIdx.x == 0) {
         PlanHeader* const h = static_cast<PlanHeader*>(a.plan);
         h->magic = kPlanMagic;
+        h->seqs = a.seqs;
         h->tokens = a.tokens;
         h->q_heads = a.q_heads;
         h->kv_heads = a.kv_heads;

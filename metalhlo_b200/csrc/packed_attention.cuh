@@ -21,7 +21,8 @@ constexpr int kPlanMagic = 0x506c616e;
 struct PlanHeader {
     int32_t magic, tokens, q_heads, kv_heads, causal, row_tiles, key_tiles;
     int32_t first, end;  // rows of the sequences
-    int32_t reserved[3];
+    int32_t seqs;        // how far the second list lies behind the first goes by them
+    int32_t reserved[2];
 };
 
 struct PackedArgs {
@@ -35,7 +36,7 @@ struct PackedArgs {
     __host__ __device__ __forceinline__ const int4* key_tiles() const { return row_tiles() + row_capacity; }
     // Whether the plan is one of such a batch; one thread reports.
     __device__ __forceinline__ bool matches(const PlanHeader& h) const {
-        const bool ok = h.magic == kPlanMagic && h.tokens == tokens && h.q_heads == q_heads && h.kv_heads == kv_heads && h.causal == causal &&
+        const bool ok = h.magic == kPlanMagic && h.seqs == seqs && h.tokens == tokens && h.q_heads == q_heads && h.kv_heads == kv_heads && h.causal == causal &&
                         h.row_tiles >= 0 && h.row_tiles <= row_capacity && h.key_tiles >= 0 && h.key_tiles <= key_capacity;
         if (!ok && threadIdx.x == 0) kv_report(MHLO_CUDA_KV_ERROR_PLAN);
         return ok;
