@@ -825,7 +825,8 @@ int mhlo_cuda_cached_attention(int32_t dtype, const void* q_dev, const int64_t q
  *   q_heads   a multiple of kv_heads: query head i reads head i / (q_heads / kv_heads)
  *   causal    != 0: a token sees its sequence's tokens up to itself; 0: all of them
  * tokens * q_heads <= 2^30. Starts that are out of order (their sequence is passed over: what its rows of the results hold is not defined, and
- * where starts go back on earlier ones no more is that of those) and a plan that is not one of this batch (nothing is written) are reported by
+ * where starts go back on earlier ones no more is that of those; where sequences that lie over one another have more than `tokens` tokens together, none is
+ * computed) and a plan that is not one of this batch (nothing is written) are reported by
  * mhlo_cuda_device_error as 200 + one of MHLO_CUDA_KV_ERROR_*.
  * No counterpart in the reference, whose attention is dense, of one length, and forward only
  * (Sources/MetalHLOCore/Metal/Kernels/FlashAttentionKernel.swift:469-670).

@@ -39,27 +39,32 @@ struct TilesOf {
 __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a) {
     __shared__ int32_t counts[2][kBuckets];
     __shared__ int32_t sums[2][32], before[2], all[2];
-    __shared__ unsigned long long work[2];
+    __shared__ unsigned long long work[2], held;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, run = static_cast<int>(blockIdx.x) - 1;
     const bool causal = a.causal != 0;
     const int32_t steps[2] = {2 * a.half_tokens, kKeyTile};
     for (int i = tid; i < 2 * kBuckets; i += kPlanThreads) counts[0][i] = 0;
     if (tid < 2) before[tid] = all[tid] = 0, work[tid] = 0;
+    if (tid == 0) held = 0;
     __syncthreads();
     const auto sequence = [&](int32_t b, int32_t* first) {  // its tokens
         const int32_t end = a.starts[b + 1];
         *first = a.starts[b];
         return *first < 0 || end > a.tokens || end < *first ? -1 : end - *first;
     };
-    unsigned long long met[2] = {0, 0};
+    unsigned long long met[2] = {0, 0}, tokens_of = 0;
     for (int32_t b = tid; b < a.seqs; b += kPlanThreads) {
         int32_t first;
         const int32_t n = sequence(b, &first);
         if (n < 0) kv_report(MHLO_CUDA_KV_ERROR_STARTS);
         if (n <= 0) continue;
+        tokens_of += static_cast<unsigned long long>(n);
 #pragma unroll
         for (int list = 0; list < 2; ++list) met[list] += TilesOf{n, steps[list], list == 0, causal}.sum();
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) tokens_of += __shfl_xor_sync(0xffffffffu, tokens_of, o);
+    if (lane == 0 && tokens_of > 0) atomicAdd(&held, tokens_of);
 #pragma unroll
     for (int list = 0; list < 2; ++list) {
 #pragma unroll
@@ -67,6 +72,16 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a)
         if (lane == 0 && met[list] > 0) atomicAdd(&work[list], met[list]);
     }
     __syncthreads();
+    PlanHeader* const header = static_cast<PlanHeader*>(a.plan);
+    if (held > static_cast<unsigned long long>(a.tokens)) {
+        // Starts go back, and sequences that lie over one another have more tokens than there are: their tiles could be more than the lists, and 32 bits, hold.
+        // A plan without any. Those of fewer tokens altogether fit: a sequence of n tokens has no more than n / step + 1 tiles of a list.
+        if (blockIdx.x == 0 && tid == 0) {
+            kv_report(MHLO_CUDA_KV_ERROR_STARTS);
+            *header = PlanHeader{kPlanMagic, a.tokens, a.q_heads, a.kv_heads, a.causal, 0, 0, 0, 0, a.seqs, {0, 0}};
+        }
+        return;
+    }
     int32_t most[2];  // that tiles of the runs meet
 #pragma unroll
     for (int list = 0; list < 2; ++list) most[list] = static_cast<int32_t>(min(work[list] * a.kv_heads / (kLong * kNumSMs), static_cast<unsigned long long>(1) << 30));
@@ -112,8 +127,8 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a)
                         if ((meets > most[list]) != (run < 0)) continue;
                         const int32_t slot = atomicAdd(&counts[list][bucket_of(meets)], 1);
                         if (place == 0) continue;
-                        // starts that go back on earlier ones can make more tiles than there is room for
-                        if (slot < (list == 0 ? a.row_capacity : a.key_capacity)) const_cast<int4*>(list == 0 ? a.row_tiles() : a.key_tiles())[slot] = make_int4(first, n, at, 0);
+                        // starts that another stream changes meanwhile may make more tiles than were counted
+                        if (static_cast<uint32_t>(slot) < static_cast<uint32_t>(list == 0 ? a.row_capacity : a.key_capacity)) const_cast<int4*>(list == 0 ? a.row_tiles() : a.key_tiles())[slot] = make_int4(first, n, at, 0);
                     }
                 }
             };
@@ -144,17 +159,9 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a)
         __syncthreads();
     }
     if (tid == 0 && blockIdx.x == 0) {
-        PlanHeader* const h = static_cast<PlanHeader*>(a.plan);
-        h->magic = kPlanMagic;
-        h->seqs = a.seqs;
-        h->tokens = a.tokens;
-        h->q_heads = a.q_heads;
-        h->kv_heads = a.kv_heads;
-        h->causal = a.causal;
-        h->row_tiles = min(all[0], a.row_capacity);
-        h->key_tiles = min(all[1], a.key_capacity);
-        h->first = min(max(a.starts[0], 0), a.tokens);
-        h->end = min(max(a.starts[a.seqs], h->first), a.tokens);
+        const int32_t first = min(max(a.starts[0], 0), a.tokens);
+        *header = PlanHeader{kPlanMagic, a.tokens, a.q_heads, a.kv_heads, a.causal, min(all[0], a.row_capacity), min(all[1], a.key_capacity),
+                             first, min(max(a.starts[a.seqs], first), a.tokens), a.seqs, {0, 0}};
     }
 }
 
