@@ -435,9 +435,10 @@ __global__ void __launch_bounds__(THREADS, CTAS) norm_grad_kernel(const __grid_c
             const float shift = far * over_hidden, c1 = sum * over_hidden;
             if (!RMS) {
                 sq += fmaf(-far, shift, far2);
+                sq = sq < 0.f ? 0.f : sq;  // not fmaxf, which makes a number of a NaN
                 td = fmaf(-shift, sum, td);
             }
-            const float rs = rsqrtf(fmaf(fmaxf(sq, 0.f), over_hidden, p.eps)), c2 = td * rs * over_hidden;
+            const float rs = rsqrtf(fmaf(sq, over_hidden, p.eps)), c2 = td * rs * over_hidden;
             const float2 rs2 = twice(rs), minus_mean = twice(-(base + shift)), minus_c1 = twice(-rs * c1), minus_c2 = twice(-rs * c2);
 #pragma unroll
             for (int n = 0; n < N; ++n) {
