@@ -44,16 +44,17 @@ struct ForwardSmem {
     static constexpr int kQ = 0, kK = kQ + kHalves * kTile, kV = kK + kStages * kTile, kEnd = kV + kStages * kTile, kTotal = kEnd + 1024;
 };
 
+// Two packed weights by alpha: through fp32, as alpha may be less than the smallest f16 number where their product is not.
 template <bool BF16>
-__device__ __forceinline__ uint32_t scale16x2(uint32_t v, float a) {
-    if constexpr (BF16) {
-        const __nv_bfloat162 h = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v), __float2bfloat162_rn(a));
-        return *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-        const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&v), __float2half2_rn(a));
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
+__device__ __forceinline__ uint32_t scale16x2(uint32_t v, float alpha) {
+    float2 f;
+    if constexpr (BF16) f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+    else f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+    return pack16<BF16>(f.x * alpha, f.y * alpha);
 }
+
+// 2^d of a whole number d <= 0 (-infinity: 0).
+__device__ __forceinline__ float power_of_two(float d) { return d < -126.f ? 0.f : __uint_as_float(static_cast<uint32_t>(static_cast<int>(d) + 127) << 23); }
 
 // Scores of 64 keys behind number `last` become -infinity.
 __device__ __forceinline__ void hide(uint32_t* sr, int32_t last) {
@@ -327,8 +328,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                         if (__any_sync(0xffffffffu, grow)) {
                             float alpha = 1.f;
                             if (grow) {
-                                alpha = m_ref == -INFINITY ? 0.f : ex2(m_ref - mx);
-                                m_ref = mx;
+                                // by whole steps: weights that are rounded already follow by a power of two, which rounds them no further
+                                const float rise = ceilf(mx - m_ref);
+                                alpha = power_of_two(-rise);
+                                m_ref = m_ref == -INFINITY ? mx : m_ref + rise;
                                 l *= alpha;
                             }
                             sums[0].x *= alpha, sums[0].y *= alpha, sums[1].x *= alpha, sums[1].y *= alpha;
