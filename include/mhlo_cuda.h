@@ -846,7 +846,7 @@ int mhlo_cuda_packed_plan(const mhlo_cuda_packed_batch* batch, mhlo_cuda_stream_
  * `dtype` (F16, BF16 or F32), *_strides = {token, head} in elements, head_dim (1 .. 128) contiguous; 0 < scale <= 1e38. lse (NULL, or
  * [tokens, q_heads] floats) receives the logarithms of the sums of exponentials. o may be q itself with the same strides, or does not overlap with an input.
  * Statistics and sums are fp32. Tensors of 16 bits whose rows lie on the 16-byte grid, with head_dim a multiple of 8 and up to 128 query heads to a
- * head of keys, run on tcgen05 with weights rounded to their own type; all others take fp32 numbers (weights, p, ds, and those of fp32 tensors) as two
+ * head of keys, run on tcgen05 with weights rounded to their own type (half a step of each; f16 weights below 2^-20 of a row's largest by up to 2^-31 of that); all others take fp32 numbers (weights, p, ds, and those of fp32 tensors) as two
  * of 11 bits each: products are off by 5 * 2^-22 of their size, and an infinity in an fp32 tensor counts as a NaN.
  * |scale * q . k| has to stay below 1e37. An infinity or a NaN in a key or value may reach tokens of its own sequence that do not see it,
  * but none of another.

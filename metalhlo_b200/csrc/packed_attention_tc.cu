@@ -23,6 +23,10 @@ namespace {
 
 constexpr int kStages = 2, kThreads = 32 * (2 + 4 * kHalves);
 constexpr float kGrowth = 8.f;
+// f16 weights go to their product times 2^7: growth to 2^8 of the reference leaves room for that below 2^16. Weights down to 2^-21 of the reference keep all their bits
+// then, smaller ones are off by 2^-32 of it (unscaled, 16 000 keys 16 nats below another lost 6 % of what they add up to, scaled 0.1 %).
+template <bool BF16>
+constexpr float kUnit = BF16 ? 0.f : 7.f;
 constexpr float kCarry = 32768.f;  // a row's sum of a block below this bounds every weight below the largest f16
 constexpr int kWaitError = 60;     // + where a bounded wait ran out
 
@@ -67,7 +71,7 @@ __device__ __forceinline__ void hide(uint32_t* sr, int32_t last) {
     }
 }
 
-// Weights of 64 scores, packed, and their sum: 2^(s * scale_log2 - m).
+// Weights of 64 scores, packed, and their sum: 2^(s * scale_log2 - m), m: the reference less the unit.
 template <bool BF16>
 __device__ __forceinline__ void weights(const uint32_t* sr, float scale_log2, float m, uint32_t* packed, float2* sums) {
     const float2 c2 = make_float2(scale_log2, scale_log2), m2 = make_float2(-m, -m);
@@ -304,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
             const int nb = t.nb[h];
             // what the warp's first and last row see: tokens ascend with the rows
             const int32_t least = __shfl_sync(0xffffffffu, last, 0), most = __shfl_sync(0xffffffffu, last, 31);
-            float m_ref = -INFINITY, l = 0.f;
+            float m_ref = -INFINITY, l = 0.f;  // m_ref: with the unit taken off
             for (int j = 0; j < nb; ++j, ++it) {
                 if (!wait(&s_full[h], it & 1, 9)) break;
                 tc_fence_after();
@@ -324,14 +328,14 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                         // one decision a warp: loads and stores of tensor memory are warp-wide
                         if (key0 + ci * 64 + 63 > least) hide(sr, last - key0 - ci * 64);
                         const float mx = largest(sr) * p.scale_log2;
-                        const bool grow = mx > m_ref + kGrowth;
+                        const bool grow = mx - m_ref > kGrowth + kUnit<BF16>;
                         if (__any_sync(0xffffffffu, grow)) {
                             float alpha = 1.f;
                             if (grow) {
                                 // by whole steps: weights that are rounded already follow by a power of two, which rounds them no further
-                                const float rise = ceilf(mx - m_ref);
+                                const float rise = ceilf(mx - kUnit<BF16> - m_ref);
                                 alpha = power_of_two(-rise);
-                                m_ref = m_ref == -INFINITY ? mx : m_ref + rise;
+                                m_ref = m_ref == -INFINITY ? mx - kUnit<BF16> : m_ref + rise;
                                 l *= alpha;
                             }
                             sums[0].x *= alpha, sums[0].y *= alpha, sums[1].x *= alpha, sums[1].y *= alpha;
@@ -381,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                         uint32_t sr[64];
                         load64(s_taddr + ci * 64, sr);
                         if (key0 + ci * 64 + 63 > least) hide(sr, last - key0 - ci * 64);
-                        if (ci == 0 && j == 0) m_try = largest(sr) * p.scale_log2;
+                        if (ci == 0 && j == 0) m_try = largest(sr) * p.scale_log2 - kUnit<BF16>;
                         weights<BF16>(sr, p.scale_log2, m_try == -INFINITY ? 0.f : m_try, packed[ci], sums);
                     }
                     const float sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
@@ -403,11 +407,12 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                             mx = fmaxf(mx, largest(sr));
                         }
                         mx *= p.scale_log2;
-                        const bool grow = mx > m_ref + kGrowth;
+                        const bool grow = mx - m_ref > kGrowth + kUnit<BF16>;
                         float alpha = 1.f;
                         if (grow) {
-                            alpha = m_ref == -INFINITY ? 0.f : ex2(m_ref - mx);
-                            m_ref = mx;
+                            const float next = mx - kUnit<BF16>;
+                            alpha = m_ref == -INFINITY ? 0.f : ex2(m_ref - next);
+                            m_ref = next;
                             l *= alpha;
                         }
                         // the products so far completed before these scores did
