@@ -71,6 +71,12 @@ __device__ __forceinline__ void hide(uint32_t* sr, int32_t last) {
     }
 }
 
+// A reference is a rounded product, and one instruction takes it off the unrounded one: beyond 2^22 the difference, common to all of a row's weights, would take them
+// out of their type's range (beyond 2^27 f16 overflowed and all weights of a row could vanish). There the products are rounded like the reference first: row by row, as
+// a row's bits do not depend on other sequences'. The code for it costs other calls 1 % and 0.4 us of the smallest.
+constexpr float kFar = 4194304.f;
+__device__ __forceinline__ bool is_far(float m_ref) { return __any_sync(0xffffffffu, fabsf(m_ref) > kFar); }
+
 // Weights of 64 scores, packed, and their sum: 2^(s * scale_log2 - m), m: the reference less the unit.
 template <bool BF16>
 __device__ __forceinline__ void weights(const uint32_t* sr, float scale_log2, float m, uint32_t* packed, float2* sums) {
@@ -82,6 +88,14 @@ __device__ __forceinline__ void weights(const uint32_t* sr, float scale_log2, fl
         sums[(c >> 1) & 1] = __fadd2_rn(sums[(c >> 1) & 1], e);
         packed[c / 2] = pack16<BF16>(e.x, e.y);
     }
+}
+// Scores of a far row become exponents, and what weights() then takes is 1 and 0.
+__device__ __forceinline__ void from_far(uint32_t* sr, float* scale_log2, float* m) {
+    if (!(fabsf(*m) > kFar)) return;
+#pragma unroll
+    for (int c = 0; c < 64; ++c) sr[c] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(sr[c]), *scale_log2), *m));
+    *scale_log2 = 1.f;
+    *m = 0.f;
 }
 
 __device__ __forceinline__ float largest(const uint32_t* sr) {
@@ -309,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
             // what the warp's first and last row see: tokens ascend with the rows
             const int32_t least = __shfl_sync(0xffffffffu, last, 0), most = __shfl_sync(0xffffffffu, last, 31);
             float m_ref = -INFINITY, l = 0.f;  // m_ref: with the unit taken off
+            bool far = false;
             for (int j = 0; j < nb; ++j, ++it) {
                 if (!wait(&s_full[h], it & 1, 9)) break;
                 tc_fence_after();
@@ -327,17 +342,19 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                         }
                         // one decision a warp: loads and stores of tensor memory are warp-wide
                         if (key0 + ci * 64 + 63 > least) hide(sr, last - key0 - ci * 64);
-                        const float mx = largest(sr) * p.scale_log2;
+                        const float mx = __fmul_rn(largest(sr), p.scale_log2);  // rounded for itself, as the weights of far rows are
                         const bool grow = mx - m_ref > kGrowth + kUnit<BF16>;
                         if (__any_sync(0xffffffffu, grow)) {
                             float alpha = 1.f;
                             if (grow) {
                                 // by whole steps: weights that are rounded already follow by a power of two, which rounds them no further
-                                const float rise = ceilf(mx - kUnit<BF16> - m_ref);
-                                alpha = power_of_two(-rise);
-                                m_ref = m_ref == -INFINITY ? mx - kUnit<BF16> : m_ref + rise;
+                                const float top = mx - kUnit<BF16>, rise = ceilf(top - m_ref);
+                                const bool whole = fabsf(top) <= kFar && rise <= kFar;  // else m_ref + rise may round to less than top; the first reference is top
+                                alpha = whole ? power_of_two(-rise) : ex2(m_ref - top);
+                                m_ref = whole ? m_ref + rise : top;
                                 l *= alpha;
                             }
+                            far = is_far(m_ref);
                             sums[0].x *= alpha, sums[0].y *= alpha, sums[1].x *= alpha, sums[1].y *= alpha;
                             if (j > 0 || ci > 0) {
                                 if (!pv_waited) {
@@ -359,7 +376,9 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                                 }
                             }
                         }
-                        weights<BF16>(sr, p.scale_log2, m_ref == -INFINITY ? 0.f : m_ref, packed, sums);
+                        float by = p.scale_log2, m = m_ref == -INFINITY ? 0.f : m_ref;
+                        if (far) from_far(sr, &by, &m);
+                        weights<BF16>(sr, by, m, packed, sums);
                         if (!pv_waited) {
                             if (!wait(&pv_done[h], (it - 1) & 1, 11)) break;
                             tc_fence_after();
@@ -385,11 +404,11 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                         uint32_t sr[64];
                         load64(s_taddr + ci * 64, sr);
                         if (key0 + ci * 64 + 63 > least) hide(sr, last - key0 - ci * 64);
-                        if (ci == 0 && j == 0) m_try = largest(sr) * p.scale_log2 - kUnit<BF16>;
+                        if (ci == 0 && j == 0) m_try = __fmul_rn(largest(sr), p.scale_log2) - kUnit<BF16>;
                         weights<BF16>(sr, p.scale_log2, m_try == -INFINITY ? 0.f : m_try, packed[ci], sums);
                     }
                     const float sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
-                    done = !__any_sync(0xffffffffu, mine && !(sum < kCarry));  // rows that are another sequence's have no say
+                    done = !__any_sync(0xffffffffu, mine && !(sum < kCarry && fabsf(m_try) <= kFar));  // rows that are another sequence's have no say
                     if (done) {
                         l += sum;
                         m_ref = m_try;
@@ -406,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                             if (key0 + ci * 64 + 63 > least) hide(sr, last - key0 - ci * 64);
                             mx = fmaxf(mx, largest(sr));
                         }
-                        mx *= p.scale_log2;
+                        mx = __fmul_rn(mx, p.scale_log2);
                         const bool grow = mx - m_ref > kGrowth + kUnit<BF16>;
                         float alpha = 1.f;
                         if (grow) {
@@ -428,13 +447,14 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                             }
                         }
                         sums[0] = sums[1] = make_float2(0.f, 0.f);
-                        const float m = m_ref == -INFINITY ? 0.f : m_ref;
 #pragma unroll 1
                         for (int ci = 0; ci < 2; ++ci) {  // the weights lie over scores that have been read
                             uint32_t sr[64];
                             load64(s_taddr + ci * 64, sr);
                             if (key0 + ci * 64 + 63 > least) hide(sr, last - key0 - ci * 64);
-                            weights<BF16>(sr, p.scale_log2, m, packed[0], sums);
+                            float by = p.scale_log2, m = m_ref == -INFINITY ? 0.f : m_ref;
+                            from_far(sr, &by, &m);
+                            weights<BF16>(sr, by, m, packed[0], sums);
                             tmem_st32(p_taddr + ci * 32, packed[0]);
                         }
                         l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
