@@ -190,7 +190,8 @@ struct GeneralParams {
     PackedTensor q, k, v, o, grad, dq, dk, dv;
     float* lse;
     float2* stats;  // [kv_heads][tokens][group]: -lse log2(e), delta
-    uint32_t* norms;  // null, or where the largest squared norms of a row of grad and of a row of v go
+    float2* largest;  // of each tile, see PackedCall
+    float *grad_norms, *value_norms;  // null, or where the norms of grad's rows (like stats) and of v's ([kv_heads][tokens]) go
     float scale, scale_log2;
     FastDiv by_group;
     int32_t subs;   // tiles of this kernel to an entry of the plan
@@ -469,7 +470,7 @@ __global__ void __launch_bounds__(kGT, DP == 64 ? 2 : 1) packed_general_kernel(c
     }
 }
 
-// What the backward half needs of a row: -lse log2(e) and delta = grad . o; fp16: the largest norms of rows of grad and v. LANES of a warp to a row,
+// What the backward half needs of a row: -lse log2(e) and delta = grad . o; f16 on tcgen05: the norms of grad's rows and of v's, 0 for those that are not finite. LANES of a warp to a row,
 // kStatsRows rows at once, and four CTAs to an SM, whose loads run under the others' sums (3 sequences of up to 8192 tokens, 32 heads of 128, bf16: 44 us, 5.6
 // TB/s; four rows and two CTAs, which the registers of four rows take, 77; one row 77; f16 with norms, 32 x 1024 tokens of 12 heads of 64: 36 us and 45).
 constexpr int kStatsThreads = 256, kStatsRows = 2;
@@ -483,7 +484,7 @@ __global__ void __launch_bounds__(kStatsThreads, 4) packed_stats_kernel(const __
     const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
     if (!a.matches(h) || h.end <= h.first) return;
     const uint32_t first = (blockIdx.x * kStatsThreads + threadIdx.x) / LANES, step = gridDim.x * (kStatsThreads / LANES);
-    float largest = 0.f;  // squared norm; rows that are not finite have no say
+    auto norm_of = [](float squares) { return squares <= 3.4028235e38f ? sqrtf(squares) : 0.f; };
     auto sum_lanes = [&](float v) {
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -499,11 +500,6 @@ __global__ void __launch_bounds__(kStatsThreads, 4) packed_stats_kernel(const __
 #pragma unroll
             for (int e = 0; e < V; ++e) x[e] = lane * V + e < a.head_dim ? VecTraits<T>::to_float(row[lane * V + e]) : 0.f;
         }
-    };
-    auto leave = [&](uint32_t* to) {  // bits of numbers that are not negative have the numbers' order
-        const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(largest));
-        if ((threadIdx.x & 31) == 0 && most > 0) atomicMax(to, most);
-        largest = 0.f;
     };
     const uint32_t from = static_cast<uint32_t>(h.first) * a.q_heads, end = static_cast<uint32_t>(h.end) * a.q_heads;
     // rows of a warp's lanes go past the end together
@@ -527,26 +523,24 @@ __global__ void __launch_bounds__(kStatsThreads, 4) packed_stats_kernel(const __
                 squares = fmaf(g[r][e], g[r][e], squares);
             }
             sum = sum_lanes(sum);
-            if (p.norms != nullptr) {
-                squares = sum_lanes(squares);
-                if (squares <= 3.4028235e38f) largest = fmaxf(largest, squares);
-            }
+            if (p.grad_norms != nullptr) squares = sum_lanes(squares);
             if (lane == 0 && base + r * step + first % (32 / LANES) < end) {
                 const uint32_t kv = by_group.div(head[r]);
-                p.stats[(static_cast<int64_t>(kv) * a.tokens + token[r]) * a.group + head[r] - kv * a.group] = make_float2(-lse[r] * 1.4426950408889634f, sum);
+                const int64_t at = (static_cast<int64_t>(kv) * a.tokens + token[r]) * a.group + head[r] - kv * a.group;
+                p.stats[at] = make_float2(-lse[r] * 1.4426950408889634f, sum);
+                if (p.grad_norms != nullptr) p.grad_norms[at] = norm_of(squares);
             }
         }
     }
-    if (p.norms == nullptr) return;
-    leave(p.norms);
+    if (p.grad_norms == nullptr) return;
     const uint32_t v_from = static_cast<uint32_t>(h.first) * a.kv_heads, v_end = static_cast<uint32_t>(h.end) * a.kv_heads;
     for (uint32_t base = v_from + first - first % (32 / LANES); base < v_end; base += kStatsRows * step) {
         float x[kStatsRows][V];
+        uint32_t token[kStatsRows], head[kStatsRows];
 #pragma unroll
         for (int r = 0; r < kStatsRows; ++r) {
-            uint32_t token, head;
-            by_kv_heads.divmod(min(base + r * step + first % (32 / LANES), v_end - 1), &token, &head);
-            get(row_at<const T>(p.v, token, head), x[r]);
+            by_kv_heads.divmod(min(base + r * step + first % (32 / LANES), v_end - 1), &token[r], &head[r]);
+            get(row_at<const T>(p.v, token[r], head[r]), x[r]);
         }
 #pragma unroll
         for (int r = 0; r < kStatsRows; ++r) {
@@ -554,10 +548,36 @@ __global__ void __launch_bounds__(kStatsThreads, 4) packed_stats_kernel(const __
 #pragma unroll
             for (int e = 0; e < V; ++e) squares = fmaf(x[r][e], x[r][e], squares);
             squares = sum_lanes(squares);
-            if (squares <= 3.4028235e38f) largest = fmaxf(largest, squares);
+            if (lane == 0 && base + r * step + first % (32 / LANES) < v_end) p.value_norms[static_cast<int64_t>(head[r]) * a.tokens + token[r]] = norm_of(squares);
         }
     }
-    leave(p.norms + 1);
+}
+
+// The largest of those norms in each tile of query rows and head of keys, a warp to each: what a sequence's largest are is then a few loads. (The backward kernels
+// themselves over all rows of the sequence, per item: 18 of 167 and 15 of 142 us for 32 x 1024 tokens, 12 heads of 64.)
+__global__ void __launch_bounds__(256) packed_largest_kernel(const __grid_constant__ GeneralParams p) {
+    const PackedArgs& a = p.a;
+    const int lane = threadIdx.x & 31;
+    grid_dependency_wait();
+    grid_dependency_release();
+    const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
+    if (!a.matches(h)) return;
+    const int64_t items = static_cast<int64_t>(h.row_tiles) * a.kv_heads;
+    for (int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); item < items; item += static_cast<int64_t>(gridDim.x) * 8) {
+        const int64_t entry = item / a.kv_heads, head = item - entry * a.kv_heads;
+        const int4 e = a.row_tiles()[entry];
+        if (!a.inside(e)) continue;
+        const int32_t tokens = min(e.y - e.z, 2 * a.half_tokens);
+        const int64_t at = head * a.tokens + e.x + e.z;
+        float g = 0.f, v = 0.f;
+#pragma unroll 8
+        for (int32_t i = lane; i < tokens * a.group; i += 32) g = fmaxf(g, p.grad_norms[at * a.group + i]);
+#pragma unroll 4
+        for (int32_t i = lane; i < tokens; i += 32) v = fmaxf(v, p.value_norms[at + i]);
+        g = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(g)));  // bits of numbers that are not negative have the numbers' order
+        v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+        if (lane == 0) p.largest[at] = make_float2(g, v);
+    }
 }
 
 // Sums of the shares of dk and dv, in order; four elements a thread (ANY: one).
@@ -755,7 +775,8 @@ GeneralParams general_params(const PackedCall& c) {
     p.q = c.q, p.k = c.k, p.v = c.v, p.o = c.o, p.grad = c.grad, p.dq = c.dq, p.dk = c.dk, p.dv = c.dv;
     p.lse = c.lse;
     p.stats = c.scratch ? c.stats() : nullptr;
-    p.norms = nullptr;
+    p.largest = nullptr;
+    p.grad_norms = p.value_norms = nullptr;
     p.by_group = FastDiv(static_cast<uint32_t>(c.a.group));
     p.splits = 1;
     p.shares = c.scratch ? c.shares() : nullptr;
@@ -806,13 +827,14 @@ int stats_of(const PackedCall& c, bool norms, cudaStream_t stream) {
     const int64_t rows = static_cast<int64_t>(c.a.tokens) * c.a.q_heads, of_cta = kStatsRows * (kStatsThreads / LANES);
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>((rows + of_cta - 1) / of_cta, 8 * kNumSMs));
     GeneralParams p = general_params(c);
-    if (norms) {
-        p.norms = c.norms();
-        MHLO_CUDA_TRY(cudaMemsetAsync(p.norms, 0, 2 * sizeof(uint32_t), stream), MHLO_CUDA_EXECUTION_FAILED);
-    }
+    if (norms) p.largest = c.largest(), p.grad_norms = c.grad_norms(), p.value_norms = c.value_norms();
     const auto by = [](int32_t n) { return FastDiv(static_cast<uint32_t>(n)); };
-    const cudaError_t e = launch_dependent(packed_stats_kernel<T, LANES, VEC>, dim3(grid), dim3(kStatsThreads), 0, stream, 1, grid < kNumSMs, p, by(c.a.q_heads), by(c.a.kv_heads),
+    cudaError_t e = launch_dependent(packed_stats_kernel<T, LANES, VEC>, dim3(grid), dim3(kStatsThreads), 0, stream, 1, grid < kNumSMs, p, by(c.a.q_heads), by(c.a.kv_heads),
                                            by(c.a.group));
+    if (e == cudaSuccess && norms) {
+        const int64_t items = static_cast<int64_t>(c.a.row_capacity) * c.a.kv_heads;
+        e = launch_dependent(packed_largest_kernel, dim3(static_cast<unsigned>(std::min<int64_t>((items + 7) / 8, 8 * kNumSMs))), dim3(256), 0, stream, 1, true, p);
+    }
     if (e != cudaSuccess) return fail(MHLO_CUDA_EXECUTION_FAILED, "launch of packed_attention_grad failed: %s", cudaGetErrorString(e));
     MHLO_CUDA_CHECK_LAUNCH("packed_attention_grad");
     return MHLO_CUDA_OK;
@@ -853,7 +875,7 @@ int by_type(const PackedCall& c, F f) {
 int64_t grad_scratch_bytes(int32_t dtype, const PackedArgs& a, int64_t dim) {
     const int64_t splits = std::max(key_splits_general(a), dtype == MHLO_DT_F32 ? 1 : key_splits_tc(a));
     const int64_t shares = splits > 1 ? splits * 2 * a.tokens * a.kv_heads * dim * 4 : 0;
-    return (static_cast<int64_t>(a.tokens) * a.q_heads + 1) / 2 * 2 * static_cast<int64_t>(sizeof(float2)) + 16 + shares;
+    return (static_cast<int64_t>(a.tokens) * a.q_heads + 1) / 2 * 2 * static_cast<int64_t>(sizeof(float2)) + packed_norms(dtype, a) * 4 + shares;
 }
 
 // What the host can see of a batch.

@@ -52,6 +52,11 @@ struct PackedTensor {
     int64_t token = 0, head = 0;
 };
 
+// Floats of the norms that the backward half takes of f16 tensors.
+inline int64_t packed_norms(int32_t dtype, const PackedArgs& a) {
+    return dtype == MHLO_DT_F16 ? (static_cast<int64_t>(a.tokens) * (a.q_heads + 3 * a.kv_heads) + 3) / 4 * 4 : 0;
+}
+
 // A call of the forward or backward half.
 struct PackedCall {
     PackedArgs a;
@@ -62,10 +67,13 @@ struct PackedCall {
     void* scratch;
     // of scratch: what the backward half needs of a row, [kv_heads][tokens][group]: -lse log2(e), and grad . o
     float2* stats() const { return static_cast<float2*>(scratch); }
-    // fp16: the largest squared norms of a row of grad and of a row of v, as bits
-    uint32_t* norms() const { return reinterpret_cast<uint32_t*>(stats() + (static_cast<int64_t>(a.tokens) * a.q_heads + 1) / 2 * 2); }
+    // f16: the largest norms of a row of grad and of a row of v in a tile of query rows, [kv_heads][tokens] by the tile's first token; norms of grad's rows, laid out
+    // like stats, and of v's, [kv_heads][tokens]
+    float2* largest() const { return stats() + (static_cast<int64_t>(a.tokens) * a.q_heads + 1) / 2 * 2; }
+    float* grad_norms() const { return reinterpret_cast<float*>(largest() + static_cast<int64_t>(a.tokens) * a.kv_heads); }
+    float* value_norms() const { return grad_norms() + static_cast<int64_t>(a.tokens) * a.q_heads; }
     // Gradients of keys and values that several CTAs share, [splits][dk, dv][tokens][kv_heads][head_dim]
-    float* shares() const { return reinterpret_cast<float*>(norms() + 4); }
+    float* shares() const { return reinterpret_cast<float*>(largest()) + packed_norms(dtype, a); }
 };
 
 // Into how many shares the rows that see a tile of keys are cut where `items` tiles would leave most of `ctas` without work.

@@ -21,8 +21,10 @@
 // of exponentials (0), results through shared memory or by warps of their own (0).
 // P and dS are rounded to the type of q and of the gradient, as operands of one product are of one type: 2^-8 of each at most in bf16, 2^-11 in f16, beside which
 // the results' own rounding counts the same.
-// fp16 keeps numbers between 2^-14 and 2^16 whole. P goes to the product times 2^14, dS times a power of two that brings the largest possible
-// one, 2 max|grad row| max|v row|, below 2^15; both are undone in the results.
+// f16 keeps numbers between 2^-14 and 2^16 whole. P goes to the product times 2^14, dS times a power of two that brings the largest possible one below 2^15; both are
+// undone in the results. The power is a result row's own, as the sum over a row of dS or of dS^T has to have one: for a query 2 |grad| max|v|, for a key
+// max|grad| (|v| + max|v|), each maximum over its sequence (delta is grad times weighted values). Taken over all of the call, sequences whose gradients are 2^20 smaller
+// than another's were left with no bits.
 #include <algorithm>
 
 #include "packed_tc.cuh"
@@ -30,7 +32,7 @@
 namespace mhlo {
 namespace {
 
-constexpr int kWaitKeys = 70, kWaitQueries = 85;
+constexpr int kWaitKeys = 70, kWaitQueries = 90;
 constexpr float kUnit = 16384.f;  // of P in fp16
 
 // A block of 128 goes in kParts steps of kWide columns.
@@ -43,7 +45,8 @@ struct Shape {
 struct GradParams {
     PackedArgs a;
     const float2* stats;
-    const uint32_t* norms;
+    const float2* largest;  // f16: see PackedCall
+    const float *grad_norms, *value_norms;
     void *dq, *dk, *dv;
     float* shares;   // where the rows of a tile of keys are cut into splits: their sums, [splits][dk, dv][tokens][kv_heads][head_dim]
     int32_t splits;
@@ -53,15 +56,34 @@ struct GradParams {
     int32_t wide;     // results 32 bytes at a time
 };
 
-// The power of two of dS: 1 for bf16.
-template <bool BF16>
-__device__ __forceinline__ float unit_of(const GradParams& p) {
-    if constexpr (BF16) return 1.f;
-    const float most = 2.f * sqrtf(__uint_as_float(p.norms[0])) * sqrtf(__uint_as_float(p.norms[1]));
+// The power of two that brings numbers of up to `most` below 2^15.
+__device__ __forceinline__ float unit_of(float most) {
     if (!(most > 0.f) || most > 1e38f) return 1.f;
     const int exponent = static_cast<int>(__float_as_uint(most) >> 23) - 127;  // most < 2^(exponent + 1)
     return ldexpf(1.f, min(14 - exponent, 100));
 }
+
+// The largest norms of a row of grad and of v in a sequence, of one head of keys: a lane has those of every 32nd tile of query rows. The first are on their way from
+// the constructor on.
+struct Largest {
+    const float2* from;
+    int32_t tiles, step;
+    float2 mine;
+    __device__ __forceinline__ Largest(const float2* largest, const PackedArgs& a, int32_t first, int32_t n, int32_t head)
+        : from(largest + static_cast<int64_t>(head) * a.tokens + first), tiles((n + 2 * a.half_tokens - 1) / (2 * a.half_tokens)), step(2 * a.half_tokens) {
+        const int32_t lane = threadIdx.x & 31;
+        mine = lane < tiles ? from[static_cast<int64_t>(lane) * step] : make_float2(0.f, 0.f);
+    }
+    __device__ __forceinline__ float2 get() const {
+        float2 most = mine;
+#pragma unroll 4
+        for (int32_t i = 32 + (threadIdx.x & 31); i < tiles; i += 32) {
+            const float2 x = from[static_cast<int64_t>(i) * step];
+            most = make_float2(fmaxf(most.x, x.x), fmaxf(most.y, x.y));
+        }
+        return make_float2(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most.x))), __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most.y))));
+    }
+};
 
 // Weights of 32 scores: 2^(s scale_log2 + offset), offset(c) of column pair c.
 template <typename Offset>
@@ -296,11 +318,13 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) key_grads
         const int half = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane;  // half: 0 where there are four warps
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t s_taddr = tmem + lane_base + kS + half * 64, p_taddr = tmem + lane_base + kP + half * 64;
-        const float unit = unit_of<BF16>(p), from_dp = BF16 ? 1.f : unit / kUnit;
-        const float2 from_dp2 = make_float2(from_dp, from_dp);
         uint32_t item = 0, step = 0;
         while (ok && next()) {
             const int32_t steps = (t.b1 - t.b0) * kParts;
+            // this thread's key: the norm of its value, and the power of two of its sum
+            const Largest largest(p.largest, p.a, t.first, BF16 ? 0 : t.n, t.head);
+            float v = 0.f, unit = 1.f, from_dp = 1.f;
+            if (!BF16 && t.k0 + r < t.n) v = p.value_norms[static_cast<int64_t>(t.head) * p.a.tokens + t.first + t.k0 + r];
             for (int32_t i = 0; i < steps; ++i, ++step) {
                 const uint32_t block = step / kParts, stage = block % kStages;
                 const int32_t token0 = (t.b0 + i / kParts) * p.a.half_tokens, part = kParts == 2 ? step % 2 : half;
@@ -309,6 +333,11 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) key_grads
                 const bool mask = __any_sync(0xffffffffu, hidden > 0);
                 if (!wait(&stats_full[stage], block / kStages & 1, 8) || !wait(s_full, step & 1, 10)) break;
                 tc_fence_after();
+                if (!BF16 && i == 0) {
+                    const float2 most = largest.get();
+                    unit = unit_of(most.x * (v + most.y));
+                    from_dp = unit / kUnit;
+                }
                 const float *const lse = minus_lse[stage] + part * 64, *const delta = minus_delta[stage] + part * 64;
                 float w[64];
 #pragma unroll
@@ -341,7 +370,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) key_grads
                     for (int c = 0; c < 32; c += 2) {
                         float2 x = *reinterpret_cast<const float2*>(delta + c0 + c);
                         x = __fadd2_rn(make_float2(__uint_as_float(g[c]), __uint_as_float(g[c + 1])), x);
-                        if (!BF16) x = __fmul2_rn(x, from_dp2);
+                        if (!BF16) x = __fmul2_rn(x, make_float2(from_dp, from_dp));
                         x = __fmul2_rn(x, make_float2(w[c0 + c], w[c0 + c + 1]));
                         w[c0 + c] = x.x;
                         w[c0 + c + 1] = x.y;
@@ -578,7 +607,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) query_gra
         // ---- exponentials
         const int half = (warp - 2) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
         const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-        const float unit = unit_of<BF16>(p);
         const int32_t row_token = r / p.a.group, row_head = r - row_token * p.a.group;
         uint32_t item = 0, step = 0;
         while (ok && next()) {
@@ -586,13 +614,18 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) query_gra
             const bool mine = r < rows && i < t.n;
             const int64_t token = t.first + i;
             const float2 stat = mine ? p.stats[(static_cast<int64_t>(t.head) * p.a.tokens + token) * p.a.group + row_head] : make_float2(-INFINITY, 0.f);
-            const float2 lse2 = make_float2(stat.x, stat.x), unit2 = make_float2(unit, unit), delta2 = make_float2(-stat.y * unit, -stat.y * unit);
+            // this thread's row: the norm of its gradient, and the power of two of its sum
+            const Largest largest(p.largest, p.a, t.first, BF16 ? 0 : t.n, t.head);
+            float g = 0.f, unit = 1.f;
+            if (!BF16 && mine) g = p.grad_norms[(static_cast<int64_t>(t.head) * p.a.tokens + token) * p.a.group + row_head];
+            const float2 lse2 = make_float2(stat.x, stat.x);
             for (int32_t at = 0; at < steps; ++at, ++step) {
                 const uint32_t s_taddr = tmem + lane_base + kRegion + 2 * step % 3 * kWide + half * 64, p_taddr = tmem + lane_base + kRegion + (2 * step + 1) % 3 * kWide + half * 64;
                 const int32_t seen = last + 1 - at * kWide - half * 64;  // columns that this thread's row sees
                 const bool mask = __any_sync(0xffffffffu, seen < 64);
                 if (!wait(&s_full[step & 1], step >> 1 & 1, 11)) break;
                 tc_fence_after();
+                if (!BF16 && at == 0) unit = unit_of(2.f * g * largest.get().y);
                 float w[64];
 #pragma unroll
                 for (int c0 = 0; c0 < 64; c0 += 32) {
@@ -613,14 +646,15 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) query_gra
                 }
                 if (!wait(&dp_full[step & 1], step >> 1 & 1, 12)) break;
                 tc_fence_after();
+                const float minus_delta = -stat.y * unit;
 #pragma unroll
                 for (int c0 = 0; c0 < 64; c0 += 32) {
-                    uint32_t g[32];
-                    tmem_ld32(p_taddr + c0, g);
+                    uint32_t dp[32];
+                    tmem_ld32(p_taddr + c0, dp);
                     tmem_ld_wait();
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
-                        float2 x = __ffma2_rn(make_float2(__uint_as_float(g[c]), __uint_as_float(g[c + 1])), unit2, delta2);
+                        float2 x = __ffma2_rn(make_float2(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), make_float2(unit, unit), make_float2(minus_delta, minus_delta));
                         x = __fmul2_rn(x, make_float2(w[c0 + c], w[c0 + c + 1]));
                         w[c0 + c] = x.x;
                         w[c0 + c + 1] = x.y;
@@ -672,7 +706,9 @@ int launch(const PackedCall& c, cudaStream_t stream) {
     GradParams p;
     p.a = a;
     p.stats = c.stats();
-    p.norms = c.norms();
+    p.largest = c.largest();
+    p.grad_norms = c.grad_norms();
+    p.value_norms = c.value_norms();
     p.dq = c.dq.base, p.dk = c.dk.base, p.dv = c.dv.base;
     p.dq_token = c.dq.token, p.dq_head = c.dq.head;
     p.dk_token = c.dk.token, p.dk_head = c.dk.head;
