@@ -41,6 +41,12 @@ struct Sums {
     __device__ __forceinline__ void add(const Sums& o) { loss += o.loss, kl += o.kl, clipped += o.clipped; }
 };
 
+// Through fp32 and what it leaves of x. Where the result is 0 or infinite anyway that rest may be whole units, or no number.
+__device__ __forceinline__ float exp_of(double x) {
+    const float near = static_cast<float>(x), e = expf(near);
+    return fabsf(near) <= 128.f ? e * (1.f + static_cast<float>(x - near)) : e;
+}
+
 // exp(x) - x - 1 and exp(x) - 1; up to 1 by the series, whose terms do not cancel.
 __device__ __forceinline__ void kl_terms(double x64, float* k3, float* em1) {
     const float x = static_cast<float>(x64);
@@ -59,11 +65,9 @@ __device__ __forceinline__ void kl_terms(double x64, float* k3, float* em1) {
         *k3 = s * x * x;
         *em1 = x + *k3;
     } else {
-        const float e = expf(x) * (1.f + static_cast<float>(x64 - x));
+        const float e = exp_of(x64);
         *em1 = e - 1.f;
-        *k3 = *em1 - x;
-        if (x == -INFINITY) *em1 = -1.f, *k3 = INFINITY;  // x64 - x is no number there
-        if (x == INFINITY) *em1 = *k3 = INFINITY;
+        *k3 = e == INFINITY ? INFINITY : *em1 - x;
     }
 }
 
@@ -77,9 +81,7 @@ __device__ __forceinline__ float token(const PolicyParams& p, float logprob, flo
         grad = 0.f;
         sums->clipped += w;
     } else {
-        const float hi = static_cast<float>(d), rest = static_cast<float>(d - hi);
-        const float ratio = fabsf(hi) <= 3.4028235e38f ? expf(hi) * (1.f + rest) : expf(hi);
-        grad = loss = -ratio * a;
+        grad = loss = -exp_of(d) * a;
     }
     if (p.ref != nullptr) {
         float k3, em1;
