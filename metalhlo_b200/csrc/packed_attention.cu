@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(kStatsThreads, 4) packed_stats_kernel(const __
     grid_dependency_wait();
     grid_dependency_release();
     const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
-    if (!a.matches(h) || h.end <= h.first) return;
+    if (!a.matches(h, false) || h.end <= h.first) return;
     const uint32_t first = (blockIdx.x * kStatsThreads + threadIdx.x) / LANES, step = gridDim.x * (kStatsThreads / LANES);
     auto norm_of = [](float squares) { return squares <= 3.4028235e38f ? sqrtf(squares) : 0.f; };
     auto sum_lanes = [&](float v) {
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(256) packed_largest_kernel(const __grid_consta
     grid_dependency_wait();
     grid_dependency_release();
     const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
-    if (!a.matches(h)) return;
+    if (!a.matches(h, false)) return;
     const int64_t items = static_cast<int64_t>(h.row_tiles) * a.kv_heads;
     for (int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); item < items; item += static_cast<int64_t>(gridDim.x) * 8) {
         const int64_t entry = item / a.kv_heads, head = item - entry * a.kv_heads;
@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(256) packed_join_kernel(const __grid_constant_
     const PackedArgs& a = p.a;
     grid_dependency_wait();
     const PlanHeader h = *static_cast<const PlanHeader*>(a.plan);
-    if (!a.matches(h)) return;
+    if (!a.matches(h, false)) return;
     const int64_t all = static_cast<int64_t>(a.tokens) * a.kv_heads * a.head_dim;
     const uint32_t from = static_cast<uint32_t>(h.first) * a.kv_heads * (a.head_dim / W), end = static_cast<uint32_t>(h.end) * a.kv_heads * (a.head_dim / W);
     for (uint32_t i = from + blockIdx.x * 256 + threadIdx.x; i < end; i += gridDim.x * 256) {
@@ -954,9 +954,10 @@ int packed_join_shares(const PackedCall& c, int32_t splits, cudaStream_t stream)
 }
 
 int packed_attention_device_error() {
-    const int plan = take_kv_error(), forward = packed_attention_tc_device_error(), backward = packed_attention_grad_tc_device_error();
-    if (plan < 0 || forward < 0 || backward < 0) return -1;
-    return plan != 0 ? plan : forward != 0 ? forward : backward;
+    // One word at a time: each is of calls of its own, the others are left for the next one.
+    int v = take_kv_error();
+    if (v == 0) v = packed_attention_tc_device_error();
+    return v == 0 ? packed_attention_grad_tc_device_error() : v;
 }
 
 }  // namespace mhlo

@@ -34,11 +34,11 @@ struct PackedArgs {
     int32_t run_tokens;
     __host__ __device__ __forceinline__ const int4* row_tiles() const { return reinterpret_cast<const int4*>(static_cast<const char*>(plan) + sizeof(PlanHeader)); }
     __host__ __device__ __forceinline__ const int4* key_tiles() const { return row_tiles() + row_capacity; }
-    // Whether the plan is one of such a batch; one thread reports.
-    __device__ __forceinline__ bool matches(const PlanHeader& h) const {
+    // Whether the plan is one of such a batch; one thread reports (not in launches beside the tensor-core kernels of the same call, whose word is another: report).
+    __device__ __forceinline__ bool matches(const PlanHeader& h, bool report = true) const {
         const bool ok = h.magic == kPlanMagic && h.seqs == seqs && h.tokens == tokens && h.q_heads == q_heads && h.kv_heads == kv_heads && h.causal == causal &&
                         h.row_tiles >= 0 && h.row_tiles <= row_capacity && h.key_tiles >= 0 && h.key_tiles <= key_capacity;
-        if (!ok && threadIdx.x == 0) kv_report(MHLO_CUDA_KV_ERROR_PLAN);
+        if (!ok && report && threadIdx.x == 0) kv_report(MHLO_CUDA_KV_ERROR_PLAN);
         return ok;
     }
     __device__ __forceinline__ bool inside(const int4& e) const {
