@@ -665,10 +665,10 @@ int mhlo_cuda_peer_barrier(void* const* flag_devs, int32_t n_ranks, int32_t rank
                            mhlo_cuda_stream_t stream);
 
 /*
- * Every wait inside the tensor-core kernels (mbarrier phases fed by TMA and tcgen05.commit) is bounded; a kernel
+ * Every wait inside the tensor-core kernels and the gradients of the norms (mbarrier phases fed by TMA, bulk copies and tcgen05.commit) is bounded; a kernel
  * whose wait expires records a non-zero word and drains instead of spinning; the key/value cache kernels record what they
  * found wrong with their page tables, lengths and starts. This call synchronises the device and reads the words in turn
- * (GEMM, attention: 100 + code, cache, attention over it and over packed sequences: 200 + code). *out_code = 0 and MHLO_CUDA_OK: none is set. Else the
+ * (GEMM, attention: 100 + code, cache, attention over it and over packed sequences, policy loss, gradients of the norms: 200 + code). *out_code = 0 and MHLO_CUDA_OK: none is set. Else the
  * first one is cleared, *out_code has its code and MHLO_CUDA_EXECUTION_FAILED is returned with the text in
  * mhlo_cuda_last_error(); words behind it are left for the next call.
  */
@@ -686,7 +686,7 @@ int mhlo_cuda_device_error_take(int32_t* out_code);
 
 /*
  * Test hooks for that path; neither faults, traps or hangs the device. _store_device_error writes `code` into the
- * error word of the GEMM kernel (which = 0) or the attention kernel (which = 1) from the host. _wait_expiry_probe
+ * error word of the GEMM kernel (which = 0), the attention kernel (which = 1) or the norms' gradients (which = 2) from the host. _wait_expiry_probe
  * launches one CTA that waits on an mbarrier nobody arrives at for at most limit_ns (<= 1 s) and then records code 90
  * exactly as the contraction kernels record an expired wait.
  */

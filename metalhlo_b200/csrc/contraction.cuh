@@ -100,11 +100,13 @@ int kv_cache_device_error();          // same for the kernels that write and rea
 int cached_attention_device_error();  // same for the attention over it
 int packed_attention_device_error();  // same for the attention over packed sequences
 int policy_loss_device_error();       // same for the policy loss
+int norm_grad_device_error();         // same for the gradients of the norms
 // Stream-ordered copies of the error words into pinned host memory, and host stores into them (clearing, or the test hook).
 bool gemm_error_fetch_async(int* pinned_dst, cudaStream_t stream);
 bool attention_error_fetch_async(int* pinned_dst, cudaStream_t stream);
 bool gemm_error_store(int code);
 bool attention_error_store(int code);
+bool norm_grad_error_store(int code);
 bool gemm_wait_expiry_probe(uint64_t limit_ns, cudaStream_t stream);
 // One CTA: stores `epoch` into word `rank` of every other rank's flag array, then waits (at most limit_ns) until every word
 // of this rank's own array has reached `epoch`; an expired wait records code 95 in the GEMM error word.

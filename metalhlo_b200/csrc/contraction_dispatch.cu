@@ -166,6 +166,7 @@ int mhlo_cuda_device_error(int32_t* out_code) {
     if (v == 0) v = cached_attention_device_error();
     if (v == 0) v = packed_attention_device_error();
     if (v == 0) v = policy_loss_device_error();
+    if (v == 0) v = norm_grad_device_error();
     if (v < 0) return fail(MHLO_CUDA_EXECUTION_FAILED, "device_error: %s", cudaGetErrorString(cudaGetLastError()));
     if (v == 0) return MHLO_CUDA_OK;
     *out_code = base + v;
@@ -217,7 +218,7 @@ int mhlo_cuda_device_error_take(int32_t* out_code) {
 }
 
 int mhlo_cuda_debug_store_device_error(int32_t which, int32_t code) {
-    const bool ok = which == 0 ? gemm_error_store(code) : attention_error_store(code);
+    const bool ok = which == 0 ? gemm_error_store(code) : which == 2 ? norm_grad_error_store(code) : attention_error_store(code);
     return ok ? MHLO_CUDA_OK : fail(MHLO_CUDA_EXECUTION_FAILED, "debug_store_device_error: %s", cudaGetErrorString(cudaGetLastError()));
 }
 

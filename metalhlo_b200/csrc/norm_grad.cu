@@ -14,7 +14,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "common.cuh"
+#include "kv_cache.cuh"
 #include "tc_ptx.cuh"
 
 namespace mhlo {
@@ -273,6 +273,16 @@ struct Unit {
 };
 
 constexpr int kMostStages = 12;
+constexpr int kWaitError = 40;  // a copy did not come: what the call leaves is not its result
+// A copy did not come. Those still under way end, if they do, before the CTA does. slot, parity: of the row that did not come; rows: that are left from it on.
+__device__ __noinline__ void give_up(uint64_t* full, int stages, int slot, uint32_t parity, int64_t rows, int64_t step) {
+    kv_report(kWaitError);
+    for (int k = 1; k < stages && k * step < rows; ++k) {
+        if (++slot == stages) slot = 0, parity ^= 1;
+        if (!mbar_wait(&full[slot], parity)) return;
+    }
+}
+
 // E: elements of a thread. R: rows at once, which share a barrier and the latency of the reductions.
 template <typename T, bool VEC, bool RMS, int E, int R, int THREADS, int CTAS>
 __global__ void __launch_bounds__(THREADS, CTAS) norm_grad_kernel(const __grid_constant__ NormGradParams<T> p, int32_t stages) {
@@ -351,7 +361,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) norm_grad_kernel(const __grid_c
             const int at = stage + i < stages ? stage + i : stage + i - stages;
             x[i] = reinterpret_cast<const T*>(ring + at * 2 * row_bytes + (VEC ? 0 : reinterpret_cast<uintptr_t>(p.x + r * p.hidden) & 15));
             dy[i] = reinterpret_cast<const T*>(ring + (at * 2 + 1) * row_bytes + (VEC ? 0 : reinterpret_cast<uintptr_t>(p.dy + r * p.hidden) & 15));
-            if (r < p.rows && !mbar_wait(&full[at], phase ^ (stage + i < stages ? 0u : 1u))) return;  // cannot be: nothing but the copies is waited for
+            if (r < p.rows && !mbar_wait(&full[at], phase ^ (stage + i < stages ? 0u : 1u))) return give_up(full, stages, at, phase ^ (stage + i < stages ? 0u : 1u), p.rows - r, step);
             mean[i] = 0.f;
             if (!RMS && r < p.rows) {
                 float2 sum = twice(0.f);
@@ -697,6 +707,10 @@ int entry(const char* what, bool rms, int32_t dtype, const void* x, const void* 
 }
 
 }  // namespace
+
+int norm_grad_device_error() { return take_kv_error(); }
+bool norm_grad_error_store(int code) { return cudaMemcpyToSymbol(g_kv_error, &code, sizeof code) == cudaSuccess; }
+
 }  // namespace mhlo
 
 using namespace mhlo;

@@ -31,3 +31,17 @@ def test_words_of_several_calls_are_reported_one_after_the_other():
         for call in calls:
             call()
         assert [cuda.device_error() for _ in range(len(codes) + 1)] == codes + [0]
+
+
+def test_the_word_of_the_norms_gradients():
+    """A copy that does not come is reported (the word is written from the host here), behind what others met."""
+    from metalhlo_b200 import cuda
+
+    assert cuda.device_error() == 0
+    assert cuda.lib.mhlo_cuda_debug_store_device_error(2, 40) == 0
+    cuda.packed_plan(torch.tensor([0, 100, 50, 128], dtype=torch.int32, device="cuda"), 128, 2, 2)
+    assert [cuda.device_error() for _ in range(2)] == [203, 240] and "bounded wait (code 240)" in cuda.last_error()
+    assert cuda.device_error() == 0
+    x = torch.randn(4, 1024, device="cuda")
+    cuda.layer_norm_grad(x, None, x)
+    assert cuda.device_error() == 0
