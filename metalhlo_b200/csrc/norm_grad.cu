@@ -32,6 +32,13 @@ struct NormGradParams {
 
 __device__ __forceinline__ float sum32(float v) { return warp_reduce<SumOp>(v); }
 
+// Read once, and not through the path for constants (ld.global.nc): the call may write its result over the tensor.
+__device__ __forceinline__ uint4 ld_once16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 // W elements side by side; where they are not on the 16-byte grid, one.
 template <typename T, int W>
 __device__ __forceinline__ void load(const T* p, float* f) {
@@ -44,7 +51,7 @@ struct Raw {
     typename std::conditional<W == 1, T, uint4>::type raw;
     __device__ __forceinline__ void load(const T* p) {
         if constexpr (W == 1) raw = *p;
-        else raw = ld_stream16(p);
+        else raw = ld_once16(p);
     }
     __device__ __forceinline__ void unpack(float* f) const {
         if constexpr (W == 1) *f = VecTraits<T>::to_float(raw);
@@ -233,7 +240,7 @@ struct Unit {
     }
     __device__ __forceinline__ void hold(const T* row, Held& h) const {
         if constexpr (VEC) {
-            if (has[0]) h = ld_stream16(row + at[0]);
+            if (has[0]) h = ld_once16(row + at[0]);
         } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
