@@ -672,7 +672,8 @@ int norm_grad(const NormGradParams<T>& p, void* scratch, float* dgamma, float* d
 }
 
 int64_t scratch_bytes(int64_t rows, int64_t hidden) {
-    const int64_t joined = std::min<int64_t>(rows, kMostCtas) * 2 * hidden * 4;
+    const int64_t parts = hidden > 16 * kMostThreads ? kSplits : kMostCtas;  // such rows are not a CTA's
+    const int64_t joined = std::min(rows, parts) * 2 * hidden * 4;
     return rows * static_cast<int64_t>(sizeof(RowSums)) + joined;
 }
 
