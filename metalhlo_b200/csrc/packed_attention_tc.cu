@@ -71,31 +71,24 @@ __device__ __forceinline__ void hide(uint32_t* sr, int32_t last) {
     }
 }
 
-// A reference is a rounded product, and one instruction takes it off the unrounded one: beyond 2^22 the difference, common to all of a row's weights, would take them
-// out of their type's range (beyond 2^27 f16 overflowed and all weights of a row could vanish). There the products are rounded like the reference first: row by row, as
-// a row's bits do not depend on other sequences'. The code for it costs other calls 1 % and 0.4 us of the smallest.
+// A reference is a rounded product. Taken off the unrounded one, in one instruction, it leaves a difference that is common to all of a row's weights: nothing up to 2^22, beyond 2^27 more
+// than f16 has room for, and all weights of a row could vanish. So the products are rounded like the reference first, where that costs nothing (head dimensions up to 64: 32 x 1024
+// tokens, 12 heads, f16 108 and 109 us, 24 x 2048, 32 heads on 8, bf16 385 and 364; a branch for far rows 116 and 421) or where a reference is far (at 128, the slow way of a block:
+// 414 and 417 us).
 constexpr float kFar = 4194304.f;
-__device__ __forceinline__ bool is_far(float m_ref) { return __any_sync(0xffffffffu, fabsf(m_ref) > kFar); }
 
-// Weights of 64 scores, packed, and their sum: 2^(s * scale_log2 - m), m: the reference less the unit.
-template <bool BF16>
+// Weights of 64 scores, packed, and their sum: 2^(s * scale_log2 - m), m: the reference less the unit. ROUNDED: the products are rounded like the reference.
+template <bool BF16, bool ROUNDED>
 __device__ __forceinline__ void weights(const uint32_t* sr, float scale_log2, float m, uint32_t* packed, float2* sums) {
     const float2 c2 = make_float2(scale_log2, scale_log2), m2 = make_float2(-m, -m);
 #pragma unroll
     for (int c = 0; c < 64; c += 2) {
-        const float2 x = __ffma2_rn(make_float2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), c2, m2);
+        const float2 s = make_float2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+        const float2 x = ROUNDED ? __fadd2_rn(make_float2(__fmul_rn(s.x, scale_log2), __fmul_rn(s.y, scale_log2)), m2) : __ffma2_rn(s, c2, m2);
         const float2 e = make_float2(ex2(x.x), ex2(x.y));
         sums[(c >> 1) & 1] = __fadd2_rn(sums[(c >> 1) & 1], e);
         packed[c / 2] = pack16<BF16>(e.x, e.y);
     }
-}
-// Scores of a far row become exponents, and what weights() then takes is 1 and 0.
-__device__ __forceinline__ void from_far(uint32_t* sr, float* scale_log2, float* m) {
-    if (!(fabsf(*m) > kFar)) return;
-#pragma unroll
-    for (int c = 0; c < 64; ++c) sr[c] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(sr[c]), *scale_log2), *m));
-    *scale_log2 = 1.f;
-    *m = 0.f;
 }
 
 __device__ __forceinline__ float largest(const uint32_t* sr) {
@@ -323,7 +316,6 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
             // what the warp's first and last row see: tokens ascend with the rows
             const int32_t least = __shfl_sync(0xffffffffu, last, 0), most = __shfl_sync(0xffffffffu, last, 31);
             float m_ref = -INFINITY, l = 0.f;  // m_ref: with the unit taken off
-            bool far = false;
             for (int j = 0; j < nb; ++j, ++it) {
                 if (!wait(&s_full[h], it & 1, 9)) break;
                 tc_fence_after();
@@ -354,7 +346,6 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                                 m_ref = whole ? m_ref + rise : top;
                                 l *= alpha;
                             }
-                            far = is_far(m_ref);
                             sums[0].x *= alpha, sums[0].y *= alpha, sums[1].x *= alpha, sums[1].y *= alpha;
                             if (j > 0 || ci > 0) {
                                 if (!pv_waited) {
@@ -376,9 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                                 }
                             }
                         }
-                        float by = p.scale_log2, m = m_ref == -INFINITY ? 0.f : m_ref;
-                        if (far) from_far(sr, &by, &m);
-                        weights<BF16>(sr, by, m, packed, sums);
+                        weights<BF16, true>(sr, p.scale_log2, m_ref == -INFINITY ? 0.f : m_ref, packed, sums);
                         if (!pv_waited) {
                             if (!wait(&pv_done[h], (it - 1) & 1, 11)) break;
                             tc_fence_after();
@@ -405,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                         load64(s_taddr + ci * 64, sr);
                         if (key0 + ci * 64 + 63 > least) hide(sr, last - key0 - ci * 64);
                         if (ci == 0 && j == 0) m_try = __fmul_rn(largest(sr), p.scale_log2) - kUnit<BF16>;
-                        weights<BF16>(sr, p.scale_log2, m_try == -INFINITY ? 0.f : m_try, packed[ci], sums);
+                        weights<BF16, false>(sr, p.scale_log2, m_try == -INFINITY ? 0.f : m_try, packed[ci], sums);
                     }
                     const float sum = (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
                     done = !__any_sync(0xffffffffu, mine && !(sum < kCarry && fabsf(m_try) <= kFar));  // rows that are another sequence's have no say
@@ -452,9 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_attention_kernel(const __g
                             uint32_t sr[64];
                             load64(s_taddr + ci * 64, sr);
                             if (key0 + ci * 64 + 63 > least) hide(sr, last - key0 - ci * 64);
-                            float by = p.scale_log2, m = m_ref == -INFINITY ? 0.f : m_ref;
-                            from_far(sr, &by, &m);
-                            weights<BF16>(sr, by, m, packed[0], sums);
+                            weights<BF16, true>(sr, p.scale_log2, m_ref == -INFINITY ? 0.f : m_ref, packed[0], sums);
                             tmem_st32(p_taddr + ci * 32, packed[0]);
                         }
                         l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
