@@ -190,7 +190,7 @@ struct GeneralParams {
     PackedTensor q, k, v, o, grad, dq, dk, dv;
     float* lse;
     float2* stats;  // [kv_heads][tokens][group]: -lse log2(e), delta
-    float2* largest;  // of each tile, see PackedCall
+    float2* largest;  // of each sequence, see PackedCall
     float *grad_norms, *value_norms;  // null, or where the norms of grad's rows (like stats) and of v's ([kv_heads][tokens]) go
     float scale, scale_log2;
     FastDiv by_group;
@@ -548,13 +548,17 @@ __global__ void __launch_bounds__(kStatsThreads, 4) packed_stats_kernel(const __
 #pragma unroll
             for (int e = 0; e < V; ++e) squares = fmaf(x[r][e], x[r][e], squares);
             squares = sum_lanes(squares);
-            if (lane == 0 && base + r * step + first % (32 / LANES) < v_end) p.value_norms[static_cast<int64_t>(head[r]) * a.tokens + token[r]] = norm_of(squares);
+            if (lane == 0 && base + r * step + first % (32 / LANES) < v_end) {
+                const int64_t at = static_cast<int64_t>(head[r]) * a.tokens + token[r];
+                p.value_norms[at] = norm_of(squares);
+                p.largest[at] = make_float2(0.f, 0.f);
+            }
         }
     }
 }
 
-// The largest of those norms in each tile of query rows and head of keys, a warp to each: what a sequence's largest are is then a few loads. (The backward kernels
-// themselves over all rows of the sequence, per item: 18 of 167 and 15 of 142 us for 32 x 1024 tokens, 12 heads of 64.)
+// The largest of those norms in each sequence, by head of keys: a warp to each tile of query rows. (The backward kernels themselves over all rows of the sequence, per item: 18 of
+// 167 and 15 of 142 us for 32 x 1024 tokens, 12 heads of 64.)
 __global__ void __launch_bounds__(256) packed_largest_kernel(const __grid_constant__ GeneralParams p) {
     const PackedArgs& a = p.a;
     const int lane = threadIdx.x & 31;
@@ -574,9 +578,13 @@ __global__ void __launch_bounds__(256) packed_largest_kernel(const __grid_consta
         for (int32_t i = lane; i < tokens * a.group; i += 32) g = fmaxf(g, p.grad_norms[at * a.group + i]);
 #pragma unroll 4
         for (int32_t i = lane; i < tokens; i += 32) v = fmaxf(v, p.value_norms[at + i]);
-        g = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(g)));  // bits of numbers that are not negative have the numbers' order
-        v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
-        if (lane == 0) p.largest[at] = make_float2(g, v);
+        // bits of numbers that are not negative have the numbers' order
+        const uint32_t most_g = __reduce_max_sync(0xffffffffu, __float_as_uint(g)), most_v = __reduce_max_sync(0xffffffffu, __float_as_uint(v));
+        if (lane == 0) {
+            uint32_t* const to = reinterpret_cast<uint32_t*>(p.largest + head * a.tokens + e.x);
+            atomicMax(to, most_g);
+            atomicMax(to + 1, most_v);
+        }
     }
 }
 

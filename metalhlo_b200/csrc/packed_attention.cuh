@@ -67,8 +67,8 @@ struct PackedCall {
     void* scratch;
     // of scratch: what the backward half needs of a row, [kv_heads][tokens][group]: -lse log2(e), and grad . o
     float2* stats() const { return static_cast<float2*>(scratch); }
-    // f16: the largest norms of a row of grad and of a row of v in a tile of query rows, [kv_heads][tokens] by the tile's first token; norms of grad's rows, laid out
-    // like stats, and of v's, [kv_heads][tokens]
+    // f16: the largest norms of a row of grad and of a row of v in a sequence, at its first token of [kv_heads][tokens]; norms of grad's rows, laid out like stats, and of
+    // v's, [kv_heads][tokens]
     float2* largest() const { return stats() + (static_cast<int64_t>(a.tokens) * a.q_heads + 1) / 2 * 2; }
     float* grad_norms() const { return reinterpret_cast<float*>(largest() + static_cast<int64_t>(a.tokens) * a.kv_heads); }
     float* value_norms() const { return grad_norms() + static_cast<int64_t>(a.tokens) * a.q_heads; }

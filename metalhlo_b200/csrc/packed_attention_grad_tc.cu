@@ -63,28 +63,6 @@ __device__ __forceinline__ float unit_of(float most) {
     return ldexpf(1.f, min(14 - exponent, 100));
 }
 
-// The largest norms of a row of grad and of v in a sequence, of one head of keys: a lane has those of every 32nd tile of query rows. The first are on their way from
-// the constructor on.
-struct Largest {
-    const float2* from;
-    int32_t tiles, step;
-    float2 mine;
-    __device__ __forceinline__ Largest(const float2* largest, const PackedArgs& a, int32_t first, int32_t n, int32_t head)
-        : from(largest + static_cast<int64_t>(head) * a.tokens + first), tiles((n + 2 * a.half_tokens - 1) / (2 * a.half_tokens)), step(2 * a.half_tokens) {
-        const int32_t lane = threadIdx.x & 31;
-        mine = lane < tiles ? from[static_cast<int64_t>(lane) * step] : make_float2(0.f, 0.f);
-    }
-    __device__ __forceinline__ float2 get() const {
-        float2 most = mine;
-#pragma unroll 4
-        for (int32_t i = 32 + (threadIdx.x & 31); i < tiles; i += 32) {
-            const float2 x = from[static_cast<int64_t>(i) * step];
-            most = make_float2(fmaxf(most.x, x.x), fmaxf(most.y, x.y));
-        }
-        return make_float2(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most.x))), __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most.y))));
-    }
-};
-
 // Weights of 32 scores: 2^(s scale_log2 + offset), offset(c) of column pair c.
 template <typename Offset>
 __device__ __forceinline__ void weights(const uint32_t* s, float scale_log2, float* w, Offset offset) {
@@ -322,9 +300,10 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) key_grads
         while (ok && next()) {
             const int32_t steps = (t.b1 - t.b0) * kParts;
             // this thread's key: the norm of its value, and the power of two of its sum
-            const Largest largest(p.largest, p.a, t.first, BF16 ? 0 : t.n, t.head);
-            float v = 0.f, unit = 1.f, from_dp = 1.f;
-            if (!BF16 && t.k0 + r < t.n) v = p.value_norms[static_cast<int64_t>(t.head) * p.a.tokens + t.first + t.k0 + r];
+            const int64_t of_head = static_cast<int64_t>(t.head) * p.a.tokens + t.first;
+            const float2 most = BF16 ? make_float2(0.f, 0.f) : p.largest[of_head];
+            const float v = !BF16 && t.k0 + r < t.n ? p.value_norms[of_head + t.k0 + r] : 0.f;
+            float unit = 1.f, from_dp = 1.f;
             for (int32_t i = 0; i < steps; ++i, ++step) {
                 const uint32_t block = step / kParts, stage = block % kStages;
                 const int32_t token0 = (t.b0 + i / kParts) * p.a.half_tokens, part = kParts == 2 ? step % 2 : half;
@@ -334,7 +313,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) key_grads
                 if (!wait(&stats_full[stage], block / kStages & 1, 8) || !wait(s_full, step & 1, 10)) break;
                 tc_fence_after();
                 if (!BF16 && i == 0) {
-                    const float2 most = largest.get();
                     unit = unit_of(most.x * (v + most.y));
                     from_dp = unit / kUnit;
                 }
@@ -615,9 +593,9 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) query_gra
             const int64_t token = t.first + i;
             const float2 stat = mine ? p.stats[(static_cast<int64_t>(t.head) * p.a.tokens + token) * p.a.group + row_head] : make_float2(-INFINITY, 0.f);
             // this thread's row: the norm of its gradient, and the power of two of its sum
-            const Largest largest(p.largest, p.a, t.first, BF16 ? 0 : t.n, t.head);
-            float g = 0.f, unit = 1.f;
-            if (!BF16 && mine) g = p.grad_norms[(static_cast<int64_t>(t.head) * p.a.tokens + token) * p.a.group + row_head];
+            const int64_t of_head = static_cast<int64_t>(t.head) * p.a.tokens;
+            const float most_v = BF16 ? 0.f : p.largest[of_head + t.first].y, g = !BF16 && mine ? p.grad_norms[(of_head + token) * p.a.group + row_head] : 0.f;
+            float unit = 1.f;
             const float2 lse2 = make_float2(stat.x, stat.x);
             for (int32_t at = 0; at < steps; ++at, ++step) {
                 const uint32_t s_taddr = tmem + lane_base + kRegion + 2 * step % 3 * kWide + half * 64, p_taddr = tmem + lane_base + kRegion + (2 * step + 1) % 3 * kWide + half * 64;
@@ -625,7 +603,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtas) query_gra
                 const bool mask = __any_sync(0xffffffffu, seen < 64);
                 if (!wait(&s_full[step & 1], step >> 1 & 1, 11)) break;
                 tc_fence_after();
-                if (!BF16 && at == 0) unit = unit_of(2.f * g * largest.get().y);
+                if (!BF16 && at == 0) unit = unit_of(2.f * g * most_v);
                 float w[64];
 #pragma unroll
                 for (int c0 = 0; c0 < 64; c0 += 32) {
