@@ -824,10 +824,10 @@ int mhlo_cuda_cached_attention(int32_t dtype, const void* q_dev, const int64_t q
  *   tokens    rows of the tensors; rows of no sequence are neither read into a result nor written
  *   q_heads   a multiple of kv_heads: query head i reads head i / (q_heads / kv_heads)
  *   causal    != 0: a token sees its sequence's tokens up to itself; 0: all of them
- * tokens * q_heads <= 2^30. Starts that are out of order (their sequence is passed over: what its rows of the results hold is not defined, and
- * where starts go back on earlier ones no more is that of those; where sequences that lie over one another have more than `tokens` tokens together, none is
- * computed) and a plan that is not one of this batch (nothing is written) are reported by
- * mhlo_cuda_device_error as 200 + one of MHLO_CUDA_KV_ERROR_*.
+ * tokens * q_heads <= 2^30. Starts that are out of order are reported by mhlo_cuda_device_error as 200 + MHLO_CUDA_KV_ERROR_STARTS: a sequence whose end lies in front of
+ * its start, or outside the tensors, is passed over, and what results hold is then not defined in its rows, in rows that two sequences have, and between the first and the last
+ * row of any sequence in rows of none; where sequences have more than `tokens` tokens together, none is computed. A plan that is not one of this batch is reported as
+ * MHLO_CUDA_KV_ERROR_PLAN, and nothing is written.
  * No counterpart in the reference, whose attention is dense, of one length, and forward only
  * (Sources/MetalHLOCore/Metal/Kernels/FlashAttentionKernel.swift:469-670).
  */

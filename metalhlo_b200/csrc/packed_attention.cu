@@ -40,12 +40,13 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a)
     __shared__ int32_t counts[2][kBuckets];
     __shared__ int32_t sums[2][32], before[2], all[2];
     __shared__ unsigned long long work[2], held;
+    __shared__ int32_t lowest, highest;  // rows of the sequences, in whatever order they come
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, run = static_cast<int>(blockIdx.x) - 1;
     const bool causal = a.causal != 0;
     const int32_t steps[2] = {2 * a.half_tokens, kKeyTile};
     for (int i = tid; i < 2 * kBuckets; i += kPlanThreads) counts[0][i] = 0;
     if (tid < 2) before[tid] = all[tid] = 0, work[tid] = 0;
-    if (tid == 0) held = 0;
+    if (tid == 0) held = 0, lowest = a.tokens, highest = 0;
     __syncthreads();
     const auto sequence = [&](int32_t b, int32_t* first) {  // its tokens
         const int32_t end = a.starts[b + 1];
@@ -53,18 +54,27 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a)
         return *first < 0 || end > a.tokens || end < *first ? -1 : end - *first;
     };
     unsigned long long met[2] = {0, 0}, tokens_of = 0;
+    int32_t low = a.tokens, high = 0;
     for (int32_t b = tid; b < a.seqs; b += kPlanThreads) {
         int32_t first;
         const int32_t n = sequence(b, &first);
         if (n < 0) kv_report(MHLO_CUDA_KV_ERROR_STARTS);
         if (n <= 0) continue;
         tokens_of += static_cast<unsigned long long>(n);
+        low = min(low, first);
+        high = max(high, first + n);
 #pragma unroll
         for (int list = 0; list < 2; ++list) met[list] += TilesOf{n, steps[list], list == 0, causal}.sum();
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) tokens_of += __shfl_xor_sync(0xffffffffu, tokens_of, o);
-    if (lane == 0 && tokens_of > 0) atomicAdd(&held, tokens_of);
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    if (lane == 0 && tokens_of > 0) {
+        atomicAdd(&held, tokens_of);
+        atomicMin(&lowest, low);
+        atomicMax(&highest, high);
+    }
 #pragma unroll
     for (int list = 0; list < 2; ++list) {
 #pragma unroll
@@ -158,11 +168,8 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a)
         }
         __syncthreads();
     }
-    if (tid == 0 && blockIdx.x == 0) {
-        const int32_t first = min(max(a.starts[0], 0), a.tokens);
-        *header = PlanHeader{kPlanMagic, a.tokens, a.q_heads, a.kv_heads, a.causal, min(all[0], a.row_capacity), min(all[1], a.key_capacity),
-                             first, min(max(a.starts[a.seqs], first), a.tokens), a.seqs, {0, 0}};
-    }
+    if (tid == 0 && blockIdx.x == 0)
+        *header = PlanHeader{kPlanMagic, a.tokens, a.q_heads, a.kv_heads, a.causal, min(all[0], a.row_capacity), min(all[1], a.key_capacity), min(lowest, highest), highest, a.seqs, {0, 0}};
 }
 
 // ---- the general kernels ------------------------------------------------------------------------------------------------------------

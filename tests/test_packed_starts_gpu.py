@@ -60,3 +60,32 @@ def test_starts_whose_tiles_no_32_bits_count(pairs):
     plan = plan_of([0, tokens], tokens, 1, 1)
     assert cuda.device_error() == 0
     assert plan.tiles[ROW_TILES] == tokens // 256 and plan.tiles[KEY_TILES] == tokens // 128
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("starts", [[100, 150, 50, 60], [60, 90, 30, 50, 50, 10, 20], [120, 192, 0, 120]], ids=str)
+def test_sequences_in_front_of_earlier_ones(dtype, starts):
+    """A start that goes back without another sequence's rows being met: those around it have the results and gradients that they have alone."""
+    from metalhlo_b200 import cuda
+
+    x = inputs([192], 2, 2, 64, dtype)
+
+    def run(starts):
+        plan = plan_of(starts, 192)
+        lse = torch.zeros(192, 2, device="cuda")
+        o = cuda.packed_attention(x["q"], x["k"], x["v"], plan, 0.1, lse=lse)
+        scratch = torch.full((1 << 18,), float("nan"), device="cuda")  # what lay in memory before is no result
+        del scratch
+        return (o, lse, *cuda.packed_attention_grad(x["q"], x["k"], x["v"], o, lse, x["grad"], plan, 0.1))
+
+    got = run(starts)
+    assert cuda.device_error() == 203
+    for a, b in zip(starts, starts[1:]):
+        if b <= a:
+            continue
+        alone = run([a, b])
+        assert cuda.device_error() == 0
+        for g, w in zip(got, alone):
+            assert torch.isfinite(w[a:b]).all()
+            # few tiles of keys are cut into shares by the number of sequences, and added in another order
+            assert (g[a:b].double() - w[a:b].double()).abs().max() <= 4 * torch.finfo(dtype).eps * w[a:b].double().abs().max()
