@@ -860,7 +860,9 @@ int mhlo_cuda_packed_attention(int32_t dtype, const mhlo_cuda_packed_batch* batc
  *   p = exp(scale * q . k - lse), dv = p^T grad, ds = p (grad . v - grad . o), dq = scale * ds k, dk = scale * ds^T q,
  * dk and dv summed over the query heads of a head of keys. dq, dk, dv are like q, k, v (any strides) and overlap neither
  * with an input nor with one another.
- * Sums are fp32 in a fixed order: the same inputs give the same bits. On tcgen05 p and ds are rounded to the tensors' type.
+ * Sums are fp32 in a fixed order: the same inputs give the same bits. On tcgen05 p and ds are rounded to the tensors' type (f16: and p is off by up to 2^-39, ds by up to 2^-38 of
+ * the row's |grad| times the largest |v| of its sequence, or for dk of the largest of its sequence's |grad|). p goes by lse, a rounded number: it is off by |lse| 2^-22 of itself, so scores
+ * beyond 2^14 or so leave gradients few bits. An infinity or a NaN in a row of q, k, v or grad may reach gradients of tokens of its own sequence that do not see it or that it does not see, but of no other.
  * scratch: packed_attention_grad_scratch_bytes() bytes of device memory, 16-byte aligned, that nothing else uses until the call's work is
  * done; its contents do not matter.
  */

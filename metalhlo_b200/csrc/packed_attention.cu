@@ -180,11 +180,13 @@ __global__ void __launch_bounds__(kPlanThreads) packed_plan_kernel(PackedArgs a)
 // A warp's result of one product (scores) is an operand of the next (times values) in the lanes that it lies in, if that takes keys in the order 0 2 4 6 1 3 5 7.
 // Operands lie in shared memory in fp32, rows of DP + 4 floats: the 32 numbers that a warp loads at once are in 32 banks by rows and by columns. The side
 // that four warps share is taken apart on its way there.
-// mma.sync cuts off what does not fit its fp32 result, so a sum goes through it for 16 terms and is added to the whole with a rounding: the error of all
-// is then that of fp32 arithmetic (2.7e-7 of the result, 6.7e-7 of the gradients; 1.0e-6 and 2.2e-6 if the products add up by themselves, for 4 and 9 us less).
+// mma.sync cuts off what does not fit its fp32 result, so a sum goes through it for 16 terms and is added to the whole with a rounding: 2.7e-7 of the result and 6.7e-7 of
+// the gradients are errors like those of fp32 arithmetic (3.8e-7; dq 3.9e-7, dk and dv 7.6e-7). 1.0e-6 and 2.2e-6 if the products add up by themselves, for 4 and 9 us less; 2.2e-7 and
+// 5.0e-7 if every 8 terms are added, for 3 and 5 us more.
 // Nine sequences of up to 500 tokens, 12 heads of 64 in fp32, take 72 us; 95 on the FMA units, whose 4 x 4 elements a thread wait for what shared memory
 // hands to registers (128 bytes a clock and SM, twice the clocks of the multiply-adds). Gradients of five of up to 333, 14 heads on 2: 97 us, and 127.
 // Four warps of 64 columns, both sides taken apart where they are used, took 82 and 137.
+// The keys' kernel in fp32 holds two sums of 32 numbers beside a step's products and spills 204 bytes at 128 registers (364 at 255 for heads of up to 128).
 constexpr int kGT = 256, kGRows = 64, kGKeys = 64, kWN = 4;  // kWN: columns of a warp, by 8
 
 template <int DP>

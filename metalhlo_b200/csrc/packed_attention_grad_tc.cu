@@ -14,8 +14,9 @@
 // At D = 64 a block goes in two steps of 64 columns with warps 2-5 alone, in half of the tensor memory: two CTAs share an SM, and each works while the other
 // waits for its chain - scores, exponentials, dP, dS, sums.
 //
-// Times: 3 causal sequences of up to 8192 tokens, 32 query heads of 128 on 8, bf16: 1.19 ms the keys, 0.855 the queries (1260 TFLOP/s of what they compute
-// where the mask leaves something; the tensor pipe is busy for 67 %). 32 of 1024, 12 heads of 64, f16: 0.181 and 0.128 ms; 0.200 and 0.147 with one CTA to an SM, which
+// Times: 3 causal sequences of up to 8192 tokens, 32 query heads of 128 on 8, bf16: 1.18 ms the keys, 0.86 to 0.92 the queries (1260 TFLOP/s of what they compute
+// where the mask leaves something; the tensor pipe is busy for 67 %). 32 of 1024, 12 heads of 64, f16: 0.192 and 0.137 ms (0.181 and 0.128 with one power of two for all of the call, see below); 0.200 and
+// 0.147 with one CTA to an SM, which
 // none of these changed by more than a few percent: products of the next tile issued ahead with results stored under them (keys 0, queries -5 %, at D = 128
 // +5 %), the two warpgroups' exponentials in turn, loads of tensor memory a half ahead (0), a quarter of the exponentials by a polynomial (+2 %), sixteen warps
 // of exponentials (0), results through shared memory or by warps of their own (0).

@@ -7,13 +7,13 @@
 //                      under the other's exponentials
 //   warps 2-5, 6-9     softmax of half 0 / 1, a thread per row
 // The maximum in the exponent moves only when scores exceed it by 2^8; O is rescaled in tensor memory only then.
-// Weights are rounded to the type of the values, as their product has operands of one type (half a step: 2^-8 of a weight at most in bf16, 2^-11 in f16); sums of
-// weights are those of the weights before that, in fp32.
+// Weights are rounded once, to the type of the values, as their product has operands of one type (half a step: 2^-8 of a weight at most in bf16, 2^-11 in f16); sums of
+// weights are those of the weights before that, in fp32. Sums of the rounded ones would leave the same error: it is that of each weight, not of their sum.
 //
 // Bound by the exponential unit beside the tensor pipe: a block of 128 x 128 needs 1024 clocks of either at D = 128 (of the tensor pipe 512 at 64). Causal,
-// 32 query heads of 128 on 8, bf16: 24 sequences of up to 2048 tokens 404 us (990 TFLOP/s of what the mask leaves, the diagonal blocks' other half not
-// counted), one of 16 384 1.75 ms (1260); either unit is busy for half of the time (51 and 53 %). A chain of a half, scores to weights to the next scores,
-// is what both wait for; two run side by side, as many as tensor memory holds.
+// 32 query heads of 128 on 8, bf16: 24 sequences of up to 2048 tokens 417 us (958 TFLOP/s of what the mask leaves, the diagonal blocks' other half not
+// counted), one of 16 384 1.73 ms (1270), at 1965 MHz (called on end, at 1.56 GHz and 1000 W, 499 us and 1.99 ms); either unit is busy for half of the time (50 and 52 %). A chain of a
+// half, scores to weights to the next scores, is what both wait for; two run side by side, as many as tensor memory holds.
 #include <algorithm>
 
 #include "packed_tc.cuh"
