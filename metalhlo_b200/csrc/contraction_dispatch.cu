@@ -170,10 +170,10 @@ int mhlo_cuda_device_error(int32_t* out_code) {
     if (v < 0) return fail(MHLO_CUDA_EXECUTION_FAILED, "device_error: %s", cudaGetErrorString(cudaGetLastError()));
     if (v == 0) return MHLO_CUDA_OK;
     *out_code = base + v;
-    static const char* const what[] = {"", "a page outside the cache", "a length beyond the table or below the sequence's rows", "token_starts out of order",
+    static const char* const what[] = {"", "a page outside the cache", "a length beyond the table or below the sequence's rows", "starts out of order",
                                        "a position behind the rotation table", "a plan that is not of its batch"};
-    if (base == 200 && v <= 5) return fail(MHLO_CUDA_EXECUTION_FAILED, "a key/value cache kernel met %s (code %d)", what[v], *out_code);
-    return fail(MHLO_CUDA_EXECUTION_FAILED, "a tensor-core kernel gave up on a bounded wait (code %d)", *out_code);
+    if (base == 200 && v <= 5) return fail(MHLO_CUDA_EXECUTION_FAILED, "a kernel over cached or packed sequences met %s (code %d)", what[v], *out_code);
+    return fail(MHLO_CUDA_EXECUTION_FAILED, "a kernel gave up on a bounded wait (code %d)", *out_code);
 }
 
 namespace {

@@ -335,8 +335,8 @@ def add_rms_norm(x, residual, gamma, eps: float = 1e-5, tuning=None, stream=None
 
 
 def device_error() -> int:
-    """Synchronises, and returns and clears the first error word that a kernel left (0: none did): a bounded wait of a tensor-core kernel
-    expired, or (201 and above) a key/value cache or packed attention kernel met a page, length, start, position or plan that cannot be."""
+    """Synchronises, and returns and clears the first error word that a kernel left (0: none did): a bounded wait of a kernel
+    expired, or (201 to 205) one over cached or packed sequences met a page, length, start, position or plan that cannot be."""
     code = C.c_int32(0)
     lib.mhlo_cuda_device_error(C.byref(code))
     return code.value

@@ -45,3 +45,12 @@ def test_the_word_of_the_norms_gradients():
     x = torch.randn(4, 1024, device="cuda")
     cuda.layer_norm_grad(x, None, x)
     assert cuda.device_error() == 0
+
+
+def test_texts_name_no_other_operator():
+    from metalhlo_b200 import cuda
+
+    cuda.packed_plan(torch.tensor([0, 100, 50, 128], dtype=torch.int32, device="cuda"), 128, 2, 2)
+    assert cuda.device_error() == 203 and "cached or packed sequences met starts out of order (code 203)" in cuda.last_error()
+    assert cuda.lib.mhlo_cuda_debug_store_device_error(2, 40) == 0
+    assert cuda.device_error() == 240 and "tensor-core" not in cuda.last_error()
